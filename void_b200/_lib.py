@@ -102,6 +102,10 @@ _PROTOTYPES = {
     "void_copy_rows": (ctypes.c_int, [c_vp, c_i64, c_vp, c_i64, c_i32, c_i64, c_i32, c_vp]),
     "void_column_sum": (ctypes.c_int, [c_vp, c_i32, c_i64, c_i32, c_i32, c_vp, c_vp]),
     "void_spmm_i8_static_scratch": (ctypes.c_int, [ctypes.POINTER(SpmmArgs), c_i32, c_vp]),
+    "void_layer_norm": (ctypes.c_int, [c_vp, c_i32, c_i64, c_i64, c_i32, c_vp, c_vp, c_i32, c_f32, c_vp, c_i64, c_vp, c_vp]),
+    "void_layer_norm_grad_ws_bytes": (c_sz, [c_i64, c_i32]),
+    "void_layer_norm_grad": (ctypes.c_int, [c_vp, c_i64, c_vp, c_i64, c_i32, c_i64, c_i32, c_vp, c_i32, c_vp, c_vp, c_i64, c_vp, c_vp,
+                                            c_vp, c_sz, c_vp]),
 }
 
 EXPORTED_SYMBOLS = tuple(_PROTOTYPES)

@@ -1321,6 +1321,129 @@ PyObject* tile_gradient(PyObject*, PyObject* const* a, Py_ssize_t n) {
   NATIVE_END
 }
 
+// ------------------------------------------------------------------------------------------ layer norm
+// The tokens of x [..., D] as rows with unit stride between features; copied where they do not lie so.
+at::Tensor token_rows(const at::Tensor& x) {
+  const at::Tensor rows = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
+  return rows.size(1) > 1 && (rows.stride(1) != 1 || (rows.size(0) > 1 && rows.stride(0) < rows.size(1))) ? rows.contiguous() : rows;
+}
+int64_t row_step(const at::Tensor& rows) { return rows.size(0) > 1 ? rows.stride(0) : rows.size(1); }
+// A recorded backward pass asks for gradients of gradients, which these nodes do not have.
+void no_second_derivative(const char* what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled(), what, " has no second derivative: its backward pass cannot be recorded (create_graph=True)");
+}
+struct NormBackward : torch::autograd::Node {
+  torch::autograd::SavedVariable x, weight;
+  at::Tensor stats;
+  at::ScalarType bias_type = at::kFloat;
+
+  std::string name() const override { return "VOIDLayerNormBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    x.reset_data();
+    weight.reset_data();
+    stats.reset();
+  }
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    torch::autograd::variable_list out(3);
+    if (!grads[0].defined()) return out;
+    no_second_derivative("the layer norm");
+    const at::Tensor xs = x.unpack(), given = weight.unpack();   // (raises where the graph has been freed)
+    c10::cuda::OptionalCUDAGuard guard(xs.device());
+    at::AutoDispatchBelowADInplaceOrView below;
+    const at::Tensor w = given.defined() ? given.contiguous() : given;
+    const at::Tensor rows = token_rows(xs), g = token_rows(as_type(grads[0], xs.scalar_type()));
+    const c10::Device dev = xs.device();
+    const int64_t n = rows.size(0), cols = rows.size(1);
+    const at::ScalarType params = w.defined() ? w.scalar_type() : bias_type;
+    at::Tensor dx, ws;
+    if (task_should_compute_output(0)) dx = new_cuda({n, cols}, xs.scalar_type(), dev);
+    for (int i = 1; i < 3; ++i)
+      if (task_should_compute_output((size_t)i)) out[i] = new_cuda({cols}, params, dev);
+    if (out[1].defined() || out[2].defined())
+      ws = new_cuda({(int64_t)void_layer_norm_grad_ws_bytes(n, (int32_t)cols)}, at::kByte, dev);
+    const int status = void_layer_norm_grad(
+        g.const_data_ptr(), row_step(g), rows.const_data_ptr(), row_step(rows), out_code(xs.scalar_type()), n, (int32_t)cols,
+        w.defined() ? w.const_data_ptr() : nullptr, out_code(params), stats.const_data_ptr<float>(), dx.defined() ? dx.data_ptr() : nullptr, cols,
+        out[1].defined() ? out[1].data_ptr() : nullptr, out[2].defined() ? out[2].data_ptr() : nullptr, ws.defined() ? ws.data_ptr() : nullptr,
+        ws.defined() ? (size_t)ws.numel() : 0, stream_of(dev.index()));
+    TORCH_CHECK(status == VOID_OK, "void_b200 void_layer_norm_grad failed: ", void_strerror(status), " (status ", status, ")");
+    if (dx.defined()) out[0] = dx.view(xs.sizes());
+    return out;
+  }
+};
+// layer_norm(x [..., D], weight [D] | None, bias [D] | None, eps, out | None) -> y; differentiable in the first three
+PyObject* layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NATIVE_BEGIN
+  if (n != 5) throw torch::TypeError("layer_norm takes 5 arguments");
+  const at::Tensor& x = cuda_tensor(a[0], "x");
+  const at::Tensor absent;
+  const at::Tensor& weight = none(a[1]) ? absent : cuda_tensor(a[1], "weight");
+  const at::Tensor& bias = none(a[2]) ? absent : cuda_tensor(a[2], "bias");
+  const double eps = real(a[3]);
+  const at::ScalarType type = x.scalar_type();
+  if (type != at::kFloat && type != at::kHalf && type != at::kBFloat16)
+    fail(std::string("the layer norm takes float32, float16 or bfloat16 tokens, got ") + c10::toString(type));
+  if (x.dim() < 1 || x.size(-1) == 0) fail("the layer norm needs tokens with at least one feature");
+  if (!(eps >= 0.0)) fail("eps must not be negative");
+  const int64_t cols = x.size(-1);
+  if (cols > (1 << 30)) fail("the layer norm takes at most 2^30 features");
+  at::ScalarType params = type;
+  for (const at::Tensor* t : {&weight, &bias}) {
+    if (!t->defined()) continue;
+    if (t->dim() != 1 || t->size(0) != cols) fail("weight and bias of the layer norm must be vectors of " + std::to_string(cols) + " elements");
+    if (t->device() != x.device()) fail("x and the parameters of the layer norm are on different devices");
+    if (t->scalar_type() != type && t->scalar_type() != at::kFloat)
+      fail(std::string("weight and bias of the layer norm must be float32 or of x's type, got ") + c10::toString(t->scalar_type()));
+    params = t->scalar_type();
+  }
+  if (weight.defined() && bias.defined() && weight.scalar_type() != bias.scalar_type())
+    fail("weight and bias of the layer norm must be of one type");
+  for (const at::Tensor* t : {&x, &weight, &bias})
+    TORCH_CHECK_NOT_IMPLEMENTED(!torch::autograd::isFwGradDefined(*t), "the layer norm has no forward-mode derivative: an operand carries a tangent");
+  const bool recorded = torch::autograd::compute_requires_grad(x, weight, bias);
+  const c10::Device dev = x.device();
+  c10::cuda::OptionalCUDAGuard guard;
+  if (c10::cuda::current_device() != dev.index()) guard.set_device(dev);
+  at::Tensor y, stats;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const at::Tensor rows = token_rows(x);
+    const int64_t count = rows.size(0);
+    if (none(a[4])) {
+      y = new_cuda(x.sizes(), type, dev);
+    } else {
+      y = cuda_tensor(a[4], "out");
+      if (recorded || (at::GradMode::is_enabled() && y.requires_grad())) fail("out= cannot be differentiated through");
+      if (y.sizes() != x.sizes() || y.scalar_type() != type || y.device() != dev || !y.is_contiguous())
+        fail("out must be a contiguous tensor of x's shape and type on its device");
+      if (!y.is_inference()) y.unsafeGetTensorImpl()->bump_version();
+    }
+    if (recorded) stats = new_cuda({2, count}, at::kFloat, dev);
+    const at::Tensor w = weight.defined() ? weight.contiguous() : weight, b = bias.defined() ? bias.contiguous() : bias;
+    check(void_layer_norm(rows.const_data_ptr(), out_code(type), row_step(rows), count, (int32_t)cols, w.defined() ? w.const_data_ptr() : nullptr,
+                          b.defined() ? b.const_data_ptr() : nullptr, out_code(params), (float)eps, y.data_ptr(), cols,
+                          stats.defined() ? stats.data_ptr<float>() : nullptr, stream_of(dev.index())),
+          "void_layer_norm");
+  }
+  if (!none(a[4])) {
+    Py_INCREF(a[4]);
+    return a[4];
+  }
+  if (recorded) {
+    auto node = std::shared_ptr<NormBackward>(new NormBackward(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(x, weight, bias));
+    node->x = torch::autograd::SavedVariable(x, false);
+    if (weight.defined()) node->weight = torch::autograd::SavedVariable(weight, false);
+    node->stats = std::move(stats);
+    node->bias_type = params;
+    torch::autograd::set_history(y, node);
+  }
+  return THPVariable_Wrap(y);
+  NATIVE_END
+}
+
 PyObject* set_error(PyObject*, PyObject* cls) {
   Py_INCREF(cls);
   g_error = cls;
@@ -1353,6 +1476,7 @@ PyMethodDef kMethods[] = {
     FAST(structure_captured),
     FAST(values_product),
     FAST(tile_gradient),
+    FAST(layer_norm),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
