@@ -421,6 +421,33 @@ VOID_API int void_group_build(const int32_t* row_ptr, const int32_t* row_order, 
                               int32_t* ws, void_stream_t stream);
 VOID_API int void_spmm_grouped(const void_spmm_args* args, const void_group_store* store, int32_t kind, void_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Linear layers with more in the epilogue (no counterpart in the reference, whose fused products end with the activation):
+ *     z = x A^T + bias        out = act(z) + residual
+ * args as for void_spmm_fp / void_spmm_i8 with transposed = 1 or 2 (kind VOID_KIND_I8, _F16, _BF16 or _TF32; no plan, no raw
+ * accumulators), or as for void_spmm_grouped with transposed = 2.
+ * ------------------------------------------------------------------------------------- */
+typedef struct void_epilogue {
+  const void* residual;    /* [N, M], ldr elements between rows, added behind the activation; or NULL.  May be `out`
+                              (the same place and pitch): every element is read by the thread that writes it         */
+  int64_t ldr;
+  int32_t residual_dtype;  /* VOID_OUT_F32, or args->out_dtype                                                       */
+  int32_t reserved;
+  void* pre;               /* [N, M] of type args->out_dtype, ldp elements between rows: z, for a backward pass; or NULL */
+  int64_t ldp;
+} void_epilogue;
+VOID_API int void_spmm_linear(const void_spmm_args* args, const void_epilogue* epilogue, int32_t kind, void_stream_t stream);
+VOID_API int void_spmm_grouped_linear(const void_spmm_args* args, const void_epilogue* epilogue, const void_group_store* store,
+                                      int32_t kind, void_stream_t stream);
+/* Backward pass of the activation of such a layer: dz = g act'(z), and column sums of dz (the bias's gradient) in the same
+ * pass.  g, z and dz [rows, cols] of type elem, rows of ldg / ldz / lddz elements; dbias [cols] of type bias_elem (elem, or
+ * VOID_ELEM_F32), or NULL.  Sums are fp32, in a fixed order; of dz as computed, ahead of its rounding.
+ * ws: void_activation_grad_ws_bytes(rows, cols) bytes, needed with dbias. */
+VOID_API size_t void_activation_grad_ws_bytes(int32_t rows, int32_t cols);
+VOID_API int void_activation_grad(const void* g, int64_t ldg, const void* z, int64_t ldz, int32_t elem, int32_t rows, int32_t cols,
+                                  int32_t act, void* dz, int64_t lddz, void* dbias, int32_t bias_elem, void* ws, size_t ws_bytes,
+                                  void_stream_t stream);
+
 VOID_API int void_spmm_i8(const void_spmm_args* args, void_stream_t stream);
 VOID_API int void_spmm_f8(const void_spmm_args* args, void_stream_t stream);
 

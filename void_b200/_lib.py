@@ -49,6 +49,11 @@ class SpmmArgs(ctypes.Structure):
     ]
 
 
+class Epilogue(ctypes.Structure):
+    """Mirror of ``struct void_epilogue``."""
+    _fields_ = [("residual", c_vp), ("ldr", c_i64), ("residual_dtype", c_i32), ("reserved", c_i32), ("pre", c_vp), ("ldp", c_i64)]
+
+
 class GroupStore(ctypes.Structure):
     """Mirror of ``struct void_group_store``."""
     _fields_ = [("blob", c_vp), ("records", c_vp), ("stage_ptr", c_vp), ("group_rows", c_vp), ("n_groups", c_i32),
@@ -102,6 +107,11 @@ _PROTOTYPES = {
     "void_copy_rows": (ctypes.c_int, [c_vp, c_i64, c_vp, c_i64, c_i32, c_i64, c_i32, c_vp]),
     "void_column_sum": (ctypes.c_int, [c_vp, c_i32, c_i64, c_i32, c_i32, c_vp, c_vp]),
     "void_spmm_i8_static_scratch": (ctypes.c_int, [ctypes.POINTER(SpmmArgs), c_i32, c_vp]),
+    "void_spmm_linear": (ctypes.c_int, [ctypes.POINTER(SpmmArgs), ctypes.POINTER(Epilogue), c_i32, c_vp]),
+    "void_spmm_grouped_linear": (ctypes.c_int, [ctypes.POINTER(SpmmArgs), ctypes.POINTER(Epilogue), ctypes.POINTER(GroupStore), c_i32, c_vp]),
+    "void_activation_grad_ws_bytes": (c_sz, [c_i32, c_i32]),
+    "void_activation_grad": (ctypes.c_int, [c_vp, c_i64, c_vp, c_i64, c_i32, c_i32, c_i32, c_i32, c_vp, c_i64, c_vp, c_i32, c_vp, c_sz,
+                                            c_vp]),
     "void_layer_norm": (ctypes.c_int, [c_vp, c_i32, c_i64, c_i64, c_i32, c_vp, c_vp, c_i32, c_f32, c_vp, c_i64, c_vp, c_vp]),
     "void_layer_norm_grad_ws_bytes": (c_sz, [c_i64, c_i32]),
     "void_layer_norm_grad": (ctypes.c_int, [c_vp, c_i64, c_vp, c_i64, c_i32, c_i64, c_i32, c_vp, c_i32, c_vp, c_vp, c_i64, c_vp, c_vp,

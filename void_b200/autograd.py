@@ -1,4 +1,4 @@
-"""Differentiable SpMM on B200: VOIDSpMMFunction, VOIDSpMM and SparseLinear.
+"""Differentiable SpMM on B200: VOIDSpMMFunction, VOIDSpMM and SparseLinear, and the feed-forward layers built of them.
 
 Mirrors void/autograd.py:99-347.  Forward is void_spmm (tensor cores, TF32 for fp32 operands).
 Backward, as in the reference (:160-221):
@@ -14,6 +14,8 @@ from torch.autograd import Function
 
 from . import _lib
 from .format import VOIDTensor, note_index
+from .fusion import layer_activation
+from .norm import VOIDLayerNorm
 
 
 # Index arrays per sparsity structure: tile index and column list of A and of A^T, work items of the tile gradient.  The
@@ -112,24 +114,28 @@ class VOIDSpMMFunction(Function):
         _require_operands(a_values, a_tile_size, b)
         assert b.dim() == 2 and a_shape[1] == b.shape[0], f"Dimension mismatch: A is {a_shape}, B is {tuple(b.shape)}"
         st = _structure(a_block_rows, a_block_cols, a_shape, a_n_blocks)[0]
-        return _lib.native().values_product(st, a_values, b, False, None)
+        return _lib.native().values_product(st, a_values, b, False, None, 0, None)
 
 
 class VOIDLinearFunction(Function):
-    """y = x @ A^T (+ bias) for x [batch, in]: the linear layer on activations as they lie in memory
-    (ops.void_linear), differentiable in A's stored tiles, x and the bias.
-        dL/dx        = dL/dy @ A          - void_linear with the transposed tensor
-        dL/dA_values = (dL/dy)^T @ x      - for the stored tiles only (void_linear_tile_grad reads both as they lie)
-        dL/dbias     = column sums of dL/dy
+    """y = act(z) (+ residual), z = x @ A^T (+ bias), for x [batch, in]: the linear layer on activations as they lie in memory
+    (ops.void_linear), differentiable in A's stored tiles, x, the bias and the residual.
+        dL/dz        = dL/dy act'(z)      - one pass, with the bias's gradient (void_activation_grad); dL/dy without an activation
+        dL/dx        = dL/dz @ A          - void_linear with the transposed tensor
+        dL/dA_values = (dL/dz)^T @ x      - for the stored tiles only (void_linear_tile_grad reads both as they lie)
+        dL/dbias     = column sums of dL/dz
+        dL/dresidual = dL/dy
+    With an activation z is kept for the backward pass, in y's type, and the layer can be differentiated once.
     The reference's SparseLinear computes (A @ x^T)^T through VOIDSpMMFunction and adds the bias as a
     separate op (void/autograd.py:320-344)."""
 
     @staticmethod
-    def apply(a_values, a_block_rows, a_block_cols, a_shape, a_tile_size, a_n_blocks: int, x, bias):
+    def apply(a_values, a_block_rows, a_block_cols, a_shape, a_tile_size, a_n_blocks: int, x, bias, activation: int = 0,
+              residual: Optional[torch.Tensor] = None):
         _require_operands(a_values, a_tile_size, x)
         assert x.dim() == 2 and x.shape[1] == a_shape[1], f"Dimension mismatch: A is {a_shape}, x is {tuple(x.shape)}"
         st = _structure(a_block_rows, a_block_cols, a_shape, a_n_blocks)[0]
-        return _lib.native().values_product(st, a_values, x, True, bias)
+        return _lib.native().values_product(st, a_values, x, True, bias, activation, residual)
 
 
 class VOIDSpMM(torch.nn.Module):
@@ -158,13 +164,15 @@ class VOIDSpMM(torch.nn.Module):
 
 
 class SparseLinear(torch.nn.Module):
-    """nn.Linear with a VOID weight: y = x W^T + b (void/autograd.py:294-347)."""
+    """nn.Linear with a VOID weight: y = x W^T + b (void/autograd.py:294-347).  Extensions: ``activation`` (none, relu, gelu, silu)
+    and a residual given to forward, both in the product's epilogue: y = act(x W^T + b) + residual."""
 
     def __init__(self, in_features: int, out_features: int, void_tensor: VOIDTensor, bias: bool = True,
-                 dtype: Optional[torch.dtype] = None):
+                 dtype: Optional[torch.dtype] = None, activation: str = "none"):
         super().__init__()
         assert void_tensor.shape == (out_features, in_features)
-        self.in_features, self.out_features = in_features, out_features
+        self.in_features, self.out_features, self.activation = in_features, out_features, activation
+        self._activation = layer_activation(activation)
         self.sparse_weight = VOIDSpMM(void_tensor, requires_grad=True)
         dtype = dtype or void_tensor.dtype
         if bias:
@@ -172,15 +180,42 @@ class SparseLinear(torch.nn.Module):
         else:
             self.register_parameter("bias", None)
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         w = self.sparse_weight
         flat = x.dim() == 2 and x.shape[1] == self.in_features      # no views (and none in the backward pass) needed
         y = VOIDLinearFunction.apply(w.values, w.block_rows, w.block_cols, w.shape, w.tile_size, w.n_blocks,
-                                     x if flat else x.reshape(-1, self.in_features), self.bias)
+                                     x if flat else x.reshape(-1, self.in_features), self.bias, self._activation,
+                                     residual if residual is None or flat else _residual_rows(residual, x, self.out_features))
         return y if flat else y.reshape(x.shape[:-1] + (self.out_features,))
 
     def extra_repr(self) -> str:
-        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
+        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}" + (
+            f", activation={self.activation}" if self._activation else "")
+
+
+class SparseFeedForward(torch.nn.Module):
+    """The feed-forward half of a transformer block with VOID weights, residual included:
+        y = x + W2 act(W1 norm(x) + b1) + b2          for x [*, features]
+    A layer norm and two linear layers, each with all it does in one kernel; everything is differentiable.  ``norm=False`` leaves
+    the norm out.  For inference with fixed weights fused_sparse_mlp does the same over packed weights."""
+
+    def __init__(self, w1: VOIDTensor, w2: VOIDTensor, activation: str = "gelu", bias: bool = True, norm: bool = True, eps: float = 1e-5,
+                 dtype: Optional[torch.dtype] = None):
+        super().__init__()
+        (hidden, features), shape2 = w1.shape, w2.shape
+        assert shape2 == (features, hidden), f"w2 must have shape {(features, hidden)} to go with w1 {tuple(w1.shape)}, got {tuple(shape2)}"
+        self.norm = VOIDLayerNorm(features, eps, dtype=dtype or w1.dtype, device=w1.values.device) if norm else None
+        self.up = SparseLinear(features, hidden, w1, bias, dtype, activation)
+        self.down = SparseLinear(hidden, features, w2, bias, dtype)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        h = x if self.norm is None else self.norm(x)
+        return self.down(self.up(h), residual=x)
+
+
+def _residual_rows(residual: torch.Tensor, x: torch.Tensor, features: int) -> torch.Tensor:
+    assert residual.shape == x.shape[:-1] + (features,), f"residual must have shape {tuple(x.shape[:-1]) + (features,)}, got {tuple(residual.shape)}"
+    return residual.reshape(-1, features)
 
 
 def void_spmm_autograd(a: VOIDTensor, b: torch.Tensor) -> torch.Tensor:
@@ -188,4 +223,4 @@ def void_spmm_autograd(a: VOIDTensor, b: torch.Tensor) -> torch.Tensor:
     return VOIDSpMMFunction.apply(a.values, a.block_rows, a.block_cols, a.shape, a.tile_size, a.n_blocks, b)
 
 
-__all__ = ["VOIDSpMMFunction", "VOIDLinearFunction", "VOIDSpMM", "SparseLinear", "spmm_tile_grad", "tile_grad_items", "void_spmm_autograd"]
+__all__ = ["VOIDSpMMFunction", "VOIDLinearFunction", "VOIDSpMM", "SparseLinear", "SparseFeedForward", "spmm_tile_grad", "tile_grad_items", "void_spmm_autograd"]

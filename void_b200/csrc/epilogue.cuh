@@ -225,21 +225,10 @@ __device__ __forceinline__ void finish_fragments(const OutDesc& o, int r0, const
   }
 }
 
-// Transposed output (C stored as [N, M], m contiguous): the thread owns output row n and sixteen consecutive
-// columns m0 .. m0 + 15 of it, so the values leave in 16-byte stores.  bias_n is the bias of this n, the
-// per-m bias (o.row_bias) is the same for every thread of the warp.
-template <int KIND, bool ACT = true>
-__device__ __forceinline__ void finish16_tr(const OutDesc& o, int row, int n, int m0, const uint32_t* r,
-                                            float row_scale, float cs, float bias_n) {
-  if (n >= o.N) return;
-  const int c0 = row * kTile + m0;   // first output column (a row index of A)
-  const int cols = o.M - c0;         // columns left
-  if (cols <= 0) return;
-  float v[16];
-  finished<KIND, 8, ACT>(o, c0, r, row_scale, cs, bias_n, v);
-  const size_t first = (size_t)n * o.ldc + c0;
-  if (o.dtype == VOID_OUT_F32) {
-    float* dst = reinterpret_cast<float*>(o.out) + first;
+// Sixteen consecutive elements of a row-major matrix from `first` on, `cols` of them inside, in 16-byte pieces where they lie so.
+__device__ __forceinline__ void store16_row(void* out, int dtype, size_t first, int cols, const float (&v)[16]) {
+  if (dtype == VOID_OUT_F32) {
+    float* dst = reinterpret_cast<float*>(out) + first;
     if (cols >= 16 && (reinterpret_cast<uintptr_t>(dst) & 15u) == 0) {
 #pragma unroll
       for (int k = 0; k < 16; k += 4) *reinterpret_cast<float4*>(dst + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
@@ -252,7 +241,7 @@ __device__ __forceinline__ void finish16_tr(const OutDesc& o, int row, int n, in
     uint32_t h[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      if (o.dtype == VOID_OUT_F16) {
+      if (dtype == VOID_OUT_F16) {
         const __half2 t = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
         h[k] = *reinterpret_cast<const uint32_t*>(&t);
       } else {
@@ -260,7 +249,7 @@ __device__ __forceinline__ void finish16_tr(const OutDesc& o, int row, int n, in
         h[k] = *reinterpret_cast<const uint32_t*>(&t);
       }
     }
-    uint16_t* dst = reinterpret_cast<uint16_t*>(o.out) + first;
+    uint16_t* dst = reinterpret_cast<uint16_t*>(out) + first;
     if (cols >= 16 && (reinterpret_cast<uintptr_t>(dst) & 15u) == 0) {
       *reinterpret_cast<uint4*>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
       *reinterpret_cast<uint4*>(dst + 8) = make_uint4(h[4], h[5], h[6], h[7]);
@@ -270,6 +259,91 @@ __device__ __forceinline__ void finish16_tr(const OutDesc& o, int row, int n, in
         if (k < cols) dst[k] = (uint16_t)(h[k >> 1] >> ((k & 1) * 16));
     }
   }
+}
+
+// Transposed output (C stored as [N, M], m contiguous): the thread owns output row n and sixteen consecutive
+// columns m0 .. m0 + 15 of it, so the values leave in 16-byte stores.  bias_n is the bias of this n, the
+// per-m bias (o.row_bias) is the same for every thread of the warp.
+template <int KIND, bool ACT = true>
+__device__ __forceinline__ void finish16_tr(const OutDesc& o, int row, int n, int m0, const uint32_t* r,
+                                            float row_scale, float cs, float bias_n) {
+  if (n >= o.N) return;
+  const int c0 = row * kTile + m0;   // first output column (a row index of A)
+  const int cols = o.M - c0;         // columns left
+  if (cols <= 0) return;
+  float v[16];
+  finished<KIND, 8, ACT>(o, c0, r, row_scale, cs, bias_n, v);
+  store16_row(o.out, o.dtype, (size_t)n * o.ldc + c0, cols, v);
+}
+
+// What a linear layer's epilogue may do besides: keep the value before the activation, add a residual behind it.
+struct Tail {
+  const void* residual;   // [N, M], or null
+  void* pre;              // [N, M] of the output's type, or null
+  long long ldr, ldp;
+  int residual_dtype;
+};
+__device__ __forceinline__ float f16_value(uint32_t bits, bool f16) {
+  return f16 ? __half2float(__ushort_as_half((unsigned short)bits)) : __uint_as_float(bits << 16);
+}
+// Sixteen elements of the residual, added in fp32.
+__device__ __forceinline__ void add_residual16(const Tail& t, size_t first, int cols, float (&v)[16]) {
+  if (t.residual_dtype == VOID_OUT_F32) {
+    const float* src = reinterpret_cast<const float*>(t.residual) + first;
+    if (cols >= 16 && (reinterpret_cast<uintptr_t>(src) & 15u) == 0) {
+#pragma unroll
+      for (int k = 0; k < 16; k += 4) {
+        const float4 r = *reinterpret_cast<const float4*>(src + k);
+        v[k] += r.x; v[k + 1] += r.y; v[k + 2] += r.z; v[k + 3] += r.w;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 16; ++k)
+        if (k < cols) v[k] += src[k];
+    }
+  } else {
+    const bool f16 = t.residual_dtype == VOID_OUT_F16;
+    const uint16_t* src = reinterpret_cast<const uint16_t*>(t.residual) + first;
+    if (cols >= 16 && (reinterpret_cast<uintptr_t>(src) & 15u) == 0) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint4 r = *reinterpret_cast<const uint4*>(src + 8 * h);
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          v[8 * h + 2 * k] += f16_value(w[k] & 0xffffu, f16);
+          v[8 * h + 2 * k + 1] += f16_value(w[k] >> 16, f16);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 16; ++k)
+        if (k < cols) v[k] += f16_value(src[k], f16);
+    }
+  }
+}
+// finish16_tr with the rest of a linear layer: z = dequantised accumulator + bias, kept where asked; act(z) + residual.
+template <int KIND>
+__device__ __forceinline__ void finish16_tail(const OutDesc& o, const Tail& t, int row, int n, int m0, const uint32_t* r, float row_scale,
+                                              float cs, float bias_n) {
+  if (n >= o.N) return;
+  const int c0 = row * kTile + m0, cols = o.M - c0;
+  if (cols <= 0) return;
+  OutDesc linear = o;
+  linear.act = VOID_ACT_NONE;
+  float v[16];
+  finished<KIND, 8, true>(linear, c0, r, row_scale, cs, bias_n, v);
+  if (t.pre != nullptr) store16_row(t.pre, o.dtype, (size_t)n * t.ldp + c0, cols, v);
+  if (o.act != VOID_ACT_NONE) {
+    f32x2 x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = pair(v[2 * k], v[2 * k + 1]);
+    activate<8>(x, o.act);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) unpair(x[k], v[2 * k], v[2 * k + 1]);
+  }
+  if (t.residual != nullptr) add_residual16(t, (size_t)n * t.ldr + c0, cols, v);
+  store16_row(o.out, o.dtype, (size_t)n * o.ldc + c0, cols, v);
 }
 
 }  // namespace vb

@@ -27,6 +27,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cudaTypedefs.h>
+#include <type_traits>
 
 #include "../../include/void_b200.h"
 #include "epilogue.cuh"
@@ -77,13 +78,17 @@ struct GroupParams {
   unsigned int idesc;
 };
 
+struct NoTail {};
+
 struct __align__(8) Bars {
   uint64_t full[kMaxRing], empty[kMaxRing];
   uint64_t acc_full[2][kClasses], acc_empty[2][kClasses];
 };
 
-template <int KIND>
+// TAIL: results [N, M] of a linear layer with a tail.
+template <int KIND, bool TAIL>
 __global__ void __launch_bounds__(kThreads, kCtas) group_kernel(const __grid_constant__ CUtensorMap tmap_b,
+                                                            const __grid_constant__ std::conditional_t<TAIL, Tail, NoTail> tail,
                                                             const __grid_constant__ GroupParams p) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ Bars bars;
@@ -287,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) group_kernel(const __grid_con
           const int has = __shfl_sync(0xffffffffu, my_has, r);
           const float rs = __shfl_sync(0xffffffffu, my_scale, r);
           const uint32_t acc = tmem_base + lane_sel + buf * (uint32_t)buf_cols + (uint32_t)(r * kTile);
-          if (p.staged) {
+          if (!TAIL && p.staged) {
             // 16-bit results: the warp's 32 x 32 part is put together in shared memory and leaves in 16-byte pieces, four
             // lanes per row.  (A tiled store by the copy engine waits there behind the panels' loads: 2.4 us per part.)
             uint32_t lo[16], hi[16];
@@ -319,7 +324,10 @@ __global__ void __launch_bounds__(kThreads, kCtas) group_kernel(const __grid_con
 #pragma unroll
               for (int k = 0; k < 32; ++k) v[k] = 0u;
             }
-            if (p.out_tr) {
+            if constexpr (TAIL) {
+              finish16_tail<KIND>(od, tail, row, n, 0, &v[0], rs, cs, bias);
+              finish16_tail<KIND>(od, tail, row, n, 16, &v[16], rs, cs, bias);
+            } else if (p.out_tr) {
               finish16_tr<KIND>(od, row, n, 0, &v[0], rs, cs, bias);
               finish16_tr<KIND>(od, row, n, 16, &v[16], rs, cs, bias);
             } else {
@@ -513,52 +521,18 @@ __global__ void __launch_bounds__(256) group_copy_kernel(const uint4* __restrict
 }
 
 template <int KIND>
-int launch_group(const GroupParams& p, const CUtensorMap& mb, int grid, int smem, cudaStream_t st) {
-  auto kernel = group_kernel<KIND>;
+int launch_group(const GroupParams& p, const Tail* tail, const CUtensorMap& mb, int grid, int smem, cudaStream_t st) {
+  if (tail != nullptr) {
+    auto kernel = group_kernel<KIND, true>;
+    if (ensure_smem((const void*)kernel, smem)) return VOID_ERR_CUDA;
+    return status_of(launch_pdl(kernel, grid, kThreads, smem, st, mb, *tail, p));
+  }
+  auto kernel = group_kernel<KIND, false>;
   if (ensure_smem((const void*)kernel, smem)) return VOID_ERR_CUDA;
-  return status_of(launch_pdl(kernel, grid, kThreads, smem, st, mb, p));
+  return status_of(launch_pdl(kernel, grid, kThreads, smem, st, mb, NoTail{}, p));
 }
 
-}  // namespace
-
-}  // namespace vb
-
-extern "C" {
-
-int void_group_build(const int32_t* row_ptr, const int32_t* row_order, const int32_t* tile_cols, const void* tiles, int32_t nbr,
-                     int64_t nnz, int32_t elem_bytes, int32_t n_groups, int32_t max_entries, int32_t max_tiles,
-                     int32_t* group_rows, int32_t* stage_ptr, int32_t* records, void* blob, int32_t* ws, void_stream_t stream) {
-  using namespace vb;
-  if (nbr <= 0 || nnz <= 0 || n_groups <= 0 || (long long)n_groups * kMaxGroupRows < nbr) return VOID_ERR_BAD_ARG;
-  if ((elem_bytes != 1 && elem_bytes != 2 && elem_bytes != 4)) return VOID_ERR_BAD_ARG;
-  const int tile_bytes = kTileBytes * elem_bytes;
-  if (max_entries < 1 || max_entries > kMaxEntries || max_tiles < 1 ||
-      max_tiles > kMaxStageTiles || (nbr + n_groups - 1) / n_groups > kMaxRows)
-    return VOID_ERR_BAD_ARG;
-  if (nnz > 0x7fffffffLL / 8) return VOID_ERR_TOO_LARGE;
-  if (row_ptr == nullptr || tile_cols == nullptr || tiles == nullptr || group_rows == nullptr || stage_ptr == nullptr ||
-      records == nullptr || blob == nullptr || ws == nullptr)
-    return VOID_ERR_BAD_ARG;
-  if ((reinterpret_cast<uintptr_t>(tiles) & 15u) != 0 || (reinterpret_cast<uintptr_t>(blob) & 127u) != 0) return VOID_ERR_ALIGN;
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  int32_t *counts = ws, *tile_base = ws + n_groups, *tile_at = ws + 2 * (size_t)n_groups;
-  uint8_t* heads = static_cast<uint8_t*>(blob) + (size_t)nnz * tile_bytes;
-  const int blocks = (n_groups + 3) / 4;
-  const int64_t pieces = nnz * (tile_bytes / 16);
-  Launches on(st);
-  on.run(group_rows_kernel, (unsigned)((n_groups * kMaxGroupRows + 255) / 256), 256, row_order, nbr, n_groups, group_rows);
-  on.run(group_walk_kernel<false>, (unsigned)blocks, 128, row_ptr, tile_cols, group_rows, n_groups, max_entries, max_tiles,
-         nullptr, nullptr, counts, nullptr, nullptr, nnz, nullptr);
-  on.run(group_scan_kernel, 1, 1024, counts, row_ptr, group_rows, n_groups, stage_ptr, tile_base);
-  on.run(group_walk_kernel<true>, (unsigned)blocks, 128, row_ptr, tile_cols, group_rows, n_groups, max_entries, max_tiles,
-         stage_ptr, tile_base, counts, records, heads, nnz, tile_at);
-  on.run(group_copy_kernel, (unsigned)((pieces + 255) / 256), 256, reinterpret_cast<const uint4*>(tiles), tile_at, nnz, tile_bytes / 16,
-         reinterpret_cast<uint4*>(blob));
-  return on.status();
-}
-
-int void_spmm_grouped(const void_spmm_args* a, const void_group_store* s, int32_t kind, void_stream_t stream) {
-  using namespace vb;
+static int spmm_grouped(const void_spmm_args* a, const void_group_store* s, int32_t kind, const Tail* tail, void_stream_t stream) {
   if (a == nullptr || s == nullptr || kind < VOID_KIND_I8 || kind > VOID_KIND_TF32 || kind == VOID_KIND_F8E4M3) return VOID_ERR_BAD_ARG;
   if (a->M <= 0 || a->N <= 0 || a->K <= 0 || a->nbr <= 0) return VOID_ERR_BAD_ARG;
   if (a->out == nullptr || a->b == nullptr || a->row_ptr == nullptr || s->blob == nullptr || s->records == nullptr ||
@@ -637,11 +611,58 @@ int void_spmm_grouped(const void_spmm_args* a, const void_group_store* s, int32_
   if (grid > p.n_items) grid = p.n_items;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   switch (kind) {
-    case VOID_KIND_I8: return launch_group<VOID_KIND_I8>(p, mb, grid, smem, st);
-    case VOID_KIND_TF32: return launch_group<VOID_KIND_TF32>(p, mb, grid, smem, st);
-    default: return launch_group<VOID_KIND_F16>(p, mb, grid, smem, st);
+    case VOID_KIND_I8: return launch_group<VOID_KIND_I8>(p, tail, mb, grid, smem, st);
+    case VOID_KIND_TF32: return launch_group<VOID_KIND_TF32>(p, tail, mb, grid, smem, st);
+    default: return launch_group<VOID_KIND_F16>(p, tail, mb, grid, smem, st);
   }
 }
 
-}  // extern "C"
+}  // namespace
 
+}  // namespace vb
+
+extern "C" {
+
+int void_group_build(const int32_t* row_ptr, const int32_t* row_order, const int32_t* tile_cols, const void* tiles, int32_t nbr,
+                     int64_t nnz, int32_t elem_bytes, int32_t n_groups, int32_t max_entries, int32_t max_tiles,
+                     int32_t* group_rows, int32_t* stage_ptr, int32_t* records, void* blob, int32_t* ws, void_stream_t stream) {
+  using namespace vb;
+  if (nbr <= 0 || nnz <= 0 || n_groups <= 0 || (long long)n_groups * kMaxGroupRows < nbr) return VOID_ERR_BAD_ARG;
+  if ((elem_bytes != 1 && elem_bytes != 2 && elem_bytes != 4)) return VOID_ERR_BAD_ARG;
+  const int tile_bytes = kTileBytes * elem_bytes;
+  if (max_entries < 1 || max_entries > kMaxEntries || max_tiles < 1 ||
+      max_tiles > kMaxStageTiles || (nbr + n_groups - 1) / n_groups > kMaxRows)
+    return VOID_ERR_BAD_ARG;
+  if (nnz > 0x7fffffffLL / 8) return VOID_ERR_TOO_LARGE;
+  if (row_ptr == nullptr || tile_cols == nullptr || tiles == nullptr || group_rows == nullptr || stage_ptr == nullptr ||
+      records == nullptr || blob == nullptr || ws == nullptr)
+    return VOID_ERR_BAD_ARG;
+  if ((reinterpret_cast<uintptr_t>(tiles) & 15u) != 0 || (reinterpret_cast<uintptr_t>(blob) & 127u) != 0) return VOID_ERR_ALIGN;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  int32_t *counts = ws, *tile_base = ws + n_groups, *tile_at = ws + 2 * (size_t)n_groups;
+  uint8_t* heads = static_cast<uint8_t*>(blob) + (size_t)nnz * tile_bytes;
+  const int blocks = (n_groups + 3) / 4;
+  const int64_t pieces = nnz * (tile_bytes / 16);
+  Launches on(st);
+  on.run(group_rows_kernel, (unsigned)((n_groups * kMaxGroupRows + 255) / 256), 256, row_order, nbr, n_groups, group_rows);
+  on.run(group_walk_kernel<false>, (unsigned)blocks, 128, row_ptr, tile_cols, group_rows, n_groups, max_entries, max_tiles,
+         nullptr, nullptr, counts, nullptr, nullptr, nnz, nullptr);
+  on.run(group_scan_kernel, 1, 1024, counts, row_ptr, group_rows, n_groups, stage_ptr, tile_base);
+  on.run(group_walk_kernel<true>, (unsigned)blocks, 128, row_ptr, tile_cols, group_rows, n_groups, max_entries, max_tiles,
+         stage_ptr, tile_base, counts, records, heads, nnz, tile_at);
+  on.run(group_copy_kernel, (unsigned)((pieces + 255) / 256), 256, reinterpret_cast<const uint4*>(tiles), tile_at, nnz, tile_bytes / 16,
+         reinterpret_cast<uint4*>(blob));
+  return on.status();
+}
+
+int void_spmm_grouped(const void_spmm_args* a, const void_group_store* s, int32_t kind, void_stream_t stream) {
+  return vb::spmm_grouped(a, s, kind, nullptr, stream);
+}
+int void_spmm_grouped_linear(const void_spmm_args* a, const void_epilogue* e, const void_group_store* s, int32_t kind, void_stream_t stream) {
+  vb::Tail tail;
+  const int st = vb::make_tail(a, e, &tail);
+  if (st != VOID_OK) return st;
+  return a->transposed != 2 ? VOID_ERR_BAD_ARG : vb::spmm_grouped(a, s, kind, &tail, stream);
+}
+
+}  // extern "C"

@@ -530,16 +530,45 @@ GroupStore* group_store(Packed* p, int64_t N, void_stream_t st) {
   }
   return hit_saves >= line ? hit : nullptr;
 }
+// What a linear layer's epilogue adds to a product (void_epilogue), with the tensors it points into.
+struct Tail {
+  void_epilogue e = {};
+  at::Tensor residual, pre;
+  const void_epilogue* get() const { return e.residual != nullptr || e.pre != nullptr ? &e : nullptr; }
+};
+// A residual [rows, cols] for a result `out`: of its type or fp32, rows with unit stride; other ones are copied, and so is one that
+// shares memory with `out` and is not the very same matrix.
+void set_residual(Tail& t, const at::Tensor& given, const at::Tensor& out) {
+  if (given.dim() != 2 || given.size(0) != out.size(0) || given.size(1) != out.size(1))
+    fail("residual must be a [" + std::to_string(out.size(0)) + ", " + std::to_string(out.size(1)) + "] tensor");
+  if (given.device() != out.device()) fail("residual and result are on different devices");
+  out_code(given.scalar_type());
+  const int64_t rows = given.size(0), cols = given.size(1);
+  at::Tensor r = given.scalar_type() == out.scalar_type() || given.scalar_type() == at::kFloat ? given : given.to(at::kFloat);
+  if ((cols > 1 && r.stride(1) != 1) || (rows > 1 && r.stride(0) < cols)) r = r.contiguous();
+  if (r.storage().unsafeGetStorageImpl() == out.storage().unsafeGetStorageImpl() &&
+      !(r.const_data_ptr() == out.const_data_ptr() && r.scalar_type() == out.scalar_type() && (rows <= 1 || r.stride(0) == out.stride(0))))
+    r = r.clone(at::MemoryFormat::Contiguous);
+  t.residual = r;
+  t.e.residual = rows > 0 && cols > 0 ? r.const_data_ptr() : nullptr;
+  t.e.ldr = rows > 1 ? r.stride(0) : cols;
+  t.e.residual_dtype = out_code(r.scalar_type());
+}
 // A plain product with everything filled in.
-void launch_product(Packed* p, const void_spmm_args& s, void_stream_t st) {
+void launch_product(Packed* p, const void_spmm_args& s, void_stream_t st, const void_epilogue* tail = nullptr) {
   if (s.transposed != 1 && s.scale_mode == VOID_SCALE_ROW_MEAN) {
     GroupStore* g = group_store(p, s.N, st);
     if (g != nullptr) {
       g->readers.add(c10::cuda::getCurrentCUDAStream(p->device), {&g->index, &g->blob});
       if (p->captured && capturing(st)) g->captured = true;
-      check(void_spmm_grouped(&s, &g->store, p->kind, st), "void_spmm_grouped");
+      if (tail != nullptr) check(void_spmm_grouped_linear(&s, tail, &g->store, p->kind, st), "void_spmm_grouped_linear");
+      else check(void_spmm_grouped(&s, &g->store, p->kind, st), "void_spmm_grouped");
       return;
     }
+  }
+  if (tail != nullptr) {
+    check(void_spmm_linear(&s, tail, p->kind, st), "void_spmm_linear");
+    return;
   }
   if (elem_bytes(p->kind) > 1) check(void_spmm_fp(&s, p->kind, st), "void_spmm_fp");
   else check(p->kind == VOID_KIND_I8 ? void_spmm_i8(&s, st) : void_spmm_f8(&s, st), "void_spmm");
@@ -555,12 +584,12 @@ void* raw_sums(PyObject* o, c10::Device dev, int64_t at_least, const char* what)
 }
 
 // spmm(handle, b, out | None, out_dtype | None, per_tile, col_scale | None, b_scale, bias | None, row_bias | None, act,
-//      transposed, options | None) -> out
+//      transposed, options | None[, residual | None]) -> out; residual: linear layers (transposed) without options
 // options: (plan | None, acc_out, worker_partials, panels, stages, grid, tiles_per_stage, cta_shape, trace, flags,
 //           test_hooks, sorted_rows | None, use_row_scale); plan: (segs, cta_seg_ptr, n_cta, partials | None, counters, panels)
 PyObject* spmm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   NATIVE_BEGIN
-  if (n != 12) throw torch::TypeError("spmm takes 12 arguments");
+  if (n != 12 && n != 13) throw torch::TypeError("spmm takes 12 or 13 arguments");
   Packed* pk = packed_of(a[0]);
   const at::Tensor& b_in = cuda_tensor(a[1], "B");
   const c10::Device dev = b_in.device();
@@ -617,6 +646,11 @@ PyObject* spmm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   s.ldc = out.stride(0);
   s.out_dtype = out_code(out.scalar_type());
   s.act = (int32_t)integer(a[9]);
+  Tail tail;
+  if (n == 13 && !none(a[12])) {
+    if (!tr || !none(a[11])) fail("a residual goes with linear layers only");
+    set_residual(tail, cuda_tensor(a[12], "residual"), out);
+  }
   s.transposed = copied ? 2 : (tr ? 1 : 0);
   // Tile rows taken by falling tile count: measured at the 4096^2 sweep and at 16384^2, INT8 gains 3 - 5 %
   // (6.80 -> 6.58 us at 90 %, 10.33 -> 10.02 at 70 %, 72.7 -> 68.7 at 16384^2); FP8 tiles stored as two terms gain at
@@ -661,7 +695,7 @@ PyObject* spmm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   // before it waits for the previous kernel; bit 30 (measurements) keeps it from doing so
   s.flags = (int32_t)(flags & 0xffff) | ((pk->stable && !(flags & (1ll << 30))) ? 4 : 0);
   const void_stream_t st = launch_stream(pk);
-  if (none(a[11])) launch_product(pk, s, st);
+  if (none(a[11])) launch_product(pk, s, st, tail.get());
   else if (es > 1) check(void_spmm_fp(&s, pk->kind, st), "void_spmm_fp");
   else check(pk->kind == VOID_KIND_I8 ? void_spmm_i8(&s, st) : void_spmm_f8(&s, st), "void_spmm");
   if (!none(a[2])) {
@@ -672,10 +706,10 @@ PyObject* spmm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   NATIVE_END
 }
 
-// act(x A1^T + b1) A2^T + b2 [N, M2] of x [N, K], in x's type
+// act(x A1^T + b1) A2^T + b2 (+ residual) [N, M2] of x [N, K], in x's type
 // The activations in between have the layout that suits the products: [N, M1] where the layers read them as they lie, or
 // [M1, N] where copying x pays, which then serves both layers.
-at::Tensor two_layers(Packed* first, Packed* second, const at::Tensor& x, PyObject* bias1, int32_t act, PyObject* bias2) {
+at::Tensor two_layers(Packed* first, Packed* second, const at::Tensor& x, PyObject* bias1, int32_t act, PyObject* bias2, PyObject* residual) {
   Packed* pk[2] = {first, second};
   PyObject* const given[2] = {bias1, bias2};
   const c10::Device dev = x.device();
@@ -712,25 +746,27 @@ at::Tensor two_layers(Packed* first, Packed* second, const at::Tensor& x, PyObje
     s.act = layer == 0 ? act : VOID_ACT_NONE;
     s.transposed = columns ? (layer == 0 ? 0 : 2) : 1;
     s.flags = p->stable ? 4 : 0;
-    launch_product(p, s, st);
+    Tail tail;
+    if (layer == 1 && !none(residual)) set_residual(tail, cuda_tensor(residual, "residual"), out);
+    launch_product(p, s, st, tail.get());
     in = out;
   }
   return out;
 }
-// mlp(handle1, handle2, x [N, K], bias1 | None, act, bias2 | None) -> y
+// mlp(handle1, handle2, x [N, K], bias1 | None, act, bias2 | None, residual | None) -> y
 PyObject* mlp(PyObject*, PyObject* const* a, Py_ssize_t n) {
   NATIVE_BEGIN
-  if (n != 6) throw torch::TypeError("mlp takes 6 arguments");
-  return THPVariable_Wrap(two_layers(packed_of(a[0]), packed_of(a[1]), cuda_tensor(a[2], "x"), a[3], (int32_t)integer(a[4]), a[5]));
+  if (n != 7) throw torch::TypeError("mlp takes 7 arguments");
+  return THPVariable_Wrap(two_layers(packed_of(a[0]), packed_of(a[1]), cuda_tensor(a[2], "x"), a[3], (int32_t)integer(a[4]), a[5], a[6]));
   NATIVE_END
 }
-// mlp_packed(handle1, values1, block_rows1, block_cols1, shape1, the same of the second layer, x, bias1 | None, act, bias2 | None)
-//   -> y, or None where a store is not current or an operand is not what two packed layers of one type take
+// mlp_packed(handle1, values1, block_rows1, block_cols1, shape1, the same of the second layer, x, bias1 | None, act, bias2 | None,
+//   residual | None) -> y, or None where a store is not current or an operand is not what two packed layers of one type take
 // One call with all checks: a decode step's kernels take less time than the interpreter would for them (8192 x 2048 and back,
 // eight tokens: kernels 8.8 us, the host 8.2, with a call for each check 10.2).
 PyObject* mlp_packed(PyObject*, PyObject* const* a, Py_ssize_t n) {
   NATIVE_BEGIN
-  if (n != 14) throw torch::TypeError("mlp_packed takes 14 arguments");
+  if (n != 15) throw torch::TypeError("mlp_packed takes 15 arguments");
   Packed* pk[2] = {packed_of(a[0]), packed_of(a[5])};
   const at::Tensor& x = tensor(a[10], "x");
   bool ok = x.is_cuda() && x.dim() == 2;
@@ -741,7 +777,7 @@ PyObject* mlp_packed(PyObject*, PyObject* const* a, Py_ssize_t n) {
          (none(b) || (tensor(b, "bias").dim() == 1 && tensor(b, "bias").size(0) == pk[layer]->M));
   }
   if (!ok || x.size(1) != pk[0]->K || pk[0]->M != pk[1]->K) Py_RETURN_NONE;
-  return THPVariable_Wrap(two_layers(pk[0], pk[1], x, a[11], (int32_t)integer(a[12]), a[13]));
+  return THPVariable_Wrap(two_layers(pk[0], pk[1], x, a[11], (int32_t)integer(a[12]), a[13], a[14]));
   NATIVE_END
 }
 
@@ -1161,9 +1197,11 @@ void check_tiles(const Structure& st, const at::Tensor& values) {
     fail("the sparse matrix stores " + std::to_string(st.nnz) + " tiles of 32x32, got values of another shape");
 }
 // Product with tiles that change from call to call: they are packed (their transposes for A^T) and multiplied at once.
-// linear: b is x [N, K] and the result x A^T [N, M]; otherwise b is [K, N] and the result A b [M, N].
+// linear: b is x [N, K] and the result act(x A^T + row_bias) + residual [N, M], pre (where not null) x A^T + row_bias; otherwise b is
+// [K, N] and the result A b [M, N].
 at::Tensor product_of_values(const Structure& st, bool a_transposed, const at::Tensor& values_in, const at::Tensor& b_in,
-                             bool linear, const at::Tensor* row_bias) {
+                             bool linear, const at::Tensor* row_bias, int32_t act = VOID_ACT_NONE, const at::Tensor* residual = nullptr,
+                             at::Tensor* pre = nullptr) {
   const c10::Device dev = b_in.device();
   const int kind = common_kind(values_in.scalar_type(), b_in.scalar_type());
   const int es = elem_bytes(kind);
@@ -1208,7 +1246,16 @@ at::Tensor product_of_values(const Structure& st, bool a_transposed, const at::T
   s.scale_mode = VOID_SCALE_ROW_MEAN;
   s.status = st.status.data_ptr<int32_t>();
   s.transposed = copied ? 2 : (linear ? 1 : 0);
-  check(void_spmm_fp(&s, kind, stream), "void_spmm_fp");
+  s.act = act;
+  Tail tail;
+  if (residual != nullptr) set_residual(tail, *residual, out);
+  if (pre != nullptr) {
+    *pre = tail.pre = pitched(N, M, out.scalar_type(), (int)out.element_size(), dev);
+    tail.e.pre = tail.pre.data_ptr();
+    tail.e.ldp = tail.pre.stride(0);
+  }
+  if (tail.get() != nullptr && N > 0 && M > 0) check(void_spmm_linear(&s, tail.get(), kind, stream), "void_spmm_linear");
+  else check(void_spmm_fp(&s, kind, stream), "void_spmm_fp");
   return out;
 }
 
@@ -1233,6 +1280,10 @@ at::Tensor gradient_of_values(const Structure& st, const at::Tensor& g_in, const
   return grad;
 }
 
+// A recorded backward pass asks for gradients of gradients, which these nodes do not have.
+void no_second_derivative(const char* what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled(), what, " has no second derivative: its backward pass cannot be recorded (create_graph=True)");
+}
 at::Tensor column_sums(const at::Tensor& m) {
   at::Tensor out = new_cuda({m.size(1)}, m.scalar_type(), m.device());
   check(void_column_sum(m.const_data_ptr(), out_code(m.scalar_type()), std::max<int64_t>(m.stride(0), m.size(1)), (int32_t)m.size(0),
@@ -1241,30 +1292,58 @@ at::Tensor column_sums(const at::Tensor& m) {
   return out;
 }
 
-// The gradients of A b (or of x A^T + bias): an autograd node of its own, so that a backward pass runs in the engine's
+// dz = g act'(z) [N, M] and its column sums, the gradient of the bias (of type bias_type; left out where `bias` is null).
+at::Tensor activation_gradient(const at::Tensor& g_in, const at::Tensor& z, int32_t act, at::Tensor* bias, at::ScalarType bias_type) {
+  const c10::Device dev = z.device();
+  const at::Tensor g = as_type(g_in, z.scalar_type()).contiguous();
+  const int64_t rows = z.size(0), cols = z.size(1);
+  const int elem = out_code(z.scalar_type());
+  const at::Tensor dz = pitched(rows, cols, z.scalar_type(), (int)z.element_size(), dev);
+  at::Tensor ws;
+  if (bias != nullptr) {
+    *bias = new_cuda({cols}, bias_type == at::kFloat ? at::kFloat : z.scalar_type(), dev);
+    ws = new_cuda({(int64_t)void_activation_grad_ws_bytes((int32_t)rows, (int32_t)cols)}, at::kByte, dev);
+  }
+  check(void_activation_grad(g.const_data_ptr(), cols, z.const_data_ptr(), z.stride(0), elem, (int32_t)rows, (int32_t)cols, act,
+                             dz.data_ptr(), dz.stride(0), bias != nullptr ? bias->data_ptr() : nullptr,
+                             bias != nullptr ? out_code(bias->scalar_type()) : elem, ws.defined() ? ws.data_ptr() : nullptr,
+                             ws.defined() ? (size_t)ws.numel() : 0, stream_of(dev.index())),
+        "void_activation_grad");
+  return dz;
+}
+
+// The gradients of A b (or of act(x A^T + bias) + residual): an autograd node of its own, so that a backward pass runs in the engine's
 // thread without taking the interpreter's lock.
 struct ProductBackward : torch::autograd::Node {
   torch::autograd::SavedVariable values, dense;
   std::shared_ptr<const Structure> st;
+  at::Tensor pre;   // x A^T + bias, where an activation follows
   bool linear = false;
+  int32_t act = VOID_ACT_NONE;
+  at::ScalarType bias_type = at::kFloat;
 
   std::string name() const override { return "VOIDProductBackward"; }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
     values.reset_data();
     dense.reset_data();
+    pre.reset();
   }
   torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
-    torch::autograd::variable_list out(3);
+    torch::autograd::variable_list out(4);
     if (!grads[0].defined()) return out;
+    if (act != VOID_ACT_NONE) no_second_derivative("a linear layer with an activation");
     // Unpacked with autograd on: a hook may run the user's code here, such as a checkpoint's second forward pass.
-    const at::Tensor v = values.unpack(), b = dense.unpack(), g = grads[0].contiguous();
+    const at::Tensor v = values.unpack(), b = dense.unpack();
+    at::Tensor g = grads[0].contiguous();
+    if (task_should_compute_output(3)) out[3] = grads[0];
     c10::cuda::OptionalCUDAGuard guard(b.device());
     // (a backward pass that is recorded itself gets the bias gradient from an operator that can be differentiated)
     if (task_should_compute_output(2) && at::GradMode::is_enabled()) out[2] = g.sum(0);
     at::AutoDispatchBelowADInplaceOrView below;
     try {
+      if (act != VOID_ACT_NONE) g = activation_gradient(g, pre, act, task_should_compute_output(2) ? &out[2] : nullptr, bias_type);
       if (task_should_compute_output(1))
         out[1] = st->nnz ? product_of_values(*st, true, v, as_type(g, b.scalar_type()), linear, nullptr) : at::zeros_like(b);
       if (task_should_compute_output(0)) out[0] = gradient_of_values(*st, g, b, v.scalar_type(), linear);
@@ -1276,10 +1355,11 @@ struct ProductBackward : torch::autograd::Node {
   }
 };
 
-// values_product(structure, values, b, linear, bias | None) -> A b, or x A^T + bias; differentiable in all three
+// values_product(structure, values, b, linear, bias | None, act, residual | None) -> A b, or act(x A^T + bias) + residual;
+// differentiable in all of them
 PyObject* values_product(PyObject*, PyObject* const* a, Py_ssize_t n) {
   NATIVE_BEGIN
-  if (n != 5) throw torch::TypeError("values_product takes 5 arguments");
+  if (n != 7) throw torch::TypeError("values_product takes 7 arguments");
   std::shared_ptr<const Structure> st = structure_of(a[0]);
   const at::Tensor& values = cuda_tensor(a[1], "values");
   const at::Tensor& b = cuda_tensor(a[2], "the dense operand");
@@ -1287,21 +1367,31 @@ PyObject* values_product(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const bool linear = PyObject_IsTrue(a[3]) == 1;
   const at::Tensor none_given;
   const at::Tensor& bias = none(a[4]) ? none_given : tensor(a[4], "bias");
-  for (const at::Tensor* t : {&values, &b, &bias})
+  const int32_t act = (int32_t)integer(a[5]);
+  const at::Tensor& residual = none(a[6]) ? none_given : cuda_tensor(a[6], "residual");
+  if (!linear && (act != VOID_ACT_NONE || residual.defined())) fail("activations and residuals go with linear layers only");
+  if (act < VOID_ACT_NONE || act > VOID_ACT_SILU) fail("unknown activation code " + std::to_string(act));
+  for (const at::Tensor* t : {&values, &b, &bias, &residual})
     TORCH_CHECK_NOT_IMPLEMENTED(!torch::autograd::isFwGradDefined(*t),
                                 "the sparse product has no forward-mode derivative: an operand carries a tangent");
-  at::Tensor out;
+  const bool recorded = torch::autograd::compute_requires_grad(values, b, bias, residual);
+  const bool kept = recorded && act != VOID_ACT_NONE;
+  at::Tensor out, pre;
   {
     at::AutoDispatchBelowADInplaceOrView below;
-    out = product_of_values(*st, false, values, b, linear, bias.defined() ? &bias : nullptr);
+    out = product_of_values(*st, false, values, b, linear, bias.defined() ? &bias : nullptr, act, residual.defined() ? &residual : nullptr,
+                            kept ? &pre : nullptr);
   }
-  if (torch::autograd::compute_requires_grad(values, b, bias)) {
+  if (recorded) {
     auto node = std::shared_ptr<ProductBackward>(new ProductBackward(), torch::autograd::deleteNode);
-    node->set_next_edges(torch::autograd::collect_next_edges(values, b, bias));
+    node->set_next_edges(torch::autograd::collect_next_edges(values, b, bias, residual));
     node->values = torch::autograd::SavedVariable(values, false);
     node->dense = torch::autograd::SavedVariable(b, false);
     node->st = std::move(st);
     node->linear = linear;
+    node->pre = std::move(pre);
+    node->act = act;
+    if (bias.defined()) node->bias_type = bias.scalar_type();
     torch::autograd::set_history(out, node);
   }
   return THPVariable_Wrap(out);
@@ -1328,10 +1418,6 @@ at::Tensor token_rows(const at::Tensor& x) {
   return rows.size(1) > 1 && (rows.stride(1) != 1 || (rows.size(0) > 1 && rows.stride(0) < rows.size(1))) ? rows.contiguous() : rows;
 }
 int64_t row_step(const at::Tensor& rows) { return rows.size(0) > 1 ? rows.stride(0) : rows.size(1); }
-// A recorded backward pass asks for gradients of gradients, which these nodes do not have.
-void no_second_derivative(const char* what) {
-  TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled(), what, " has no second derivative: its backward pass cannot be recorded (create_graph=True)");
-}
 struct NormBackward : torch::autograd::Node {
   torch::autograd::SavedVariable x, weight;
   at::Tensor stats;

@@ -111,6 +111,9 @@ class Launches {
   cudaError_t rc_ = cudaSuccess;
 };
 
+// What void_epilogue asks for, checked against the product it belongs to (spmm.cu).
+int make_tail(const void_spmm_args* a, const void_epilogue* e, Tail* t);
+
 // B as a tensor for the copy engine, 128-byte swizzle, zero fill outside [K, N].  Elements of es bytes: every box is 128
 // bytes (kPanelN / es columns) wide, a panel takes es of them.
 //   whole (asked for when N is a multiple of a box): 3-D, dim0 = the columns of a box, dim1 = k, dim2 = box; one copy

@@ -445,7 +445,8 @@ __device__ __forceinline__ void pipeline_teardown(const SpmmParams& p, int* ctl_
 //   kSplit   a work plan, raw sums for the caller
 //   kActive  activation, row bias
 //   kTraced  time stamps (slim INT8 only, with kActive)
-constexpr int kStaged = 1, kSplit = 2, kActive = 4, kTraced = 8;
+//   kTail    what a linear layer adds (Tail in epilogue.cuh; transposed results only, with kActive)
+constexpr int kStaged = 1, kSplit = 2, kActive = 4, kTraced = 8, kTail = 16;
 struct RowaccLaunch {
   int shape;   // 1 wide, 2 slim, 6 mid
   int transposed;
@@ -455,6 +456,7 @@ struct RowaccLaunch {
   const CUtensorMap& b;
   const CUtensorMap& c;
   const PeerParams& peers;
+  const Tail& tail;
   const SpmmParams& p;
 };
 template <int KIND>

@@ -22,11 +22,13 @@ __device__ __forceinline__ int32_t* row_sums(const SpmmParams& p, const X& x, in
   return base + ((size_t)word_of(seg_words, 7) * p.np + q) * (kTile * kPanelN);
 }
 
-// What a kernel is given besides B and the common parameters: C as a tensor, the peers of a sum over ranks, or nothing.  (A
+// What a kernel is given besides B and the common parameters: C as a tensor, the peers of a sum over ranks, a linear layer's tail, or
+// nothing.  (A
 // launch takes longer by about a nanosecond for every four bytes of parameters.)
 struct Nothing {};
 template <int EPI>
-using ExtraOf = std::conditional_t<(EPI & kStaged) != 0, CUtensorMap, std::conditional_t<(EPI & kSplit) != 0, PeerParams, Nothing>>;
+using ExtraOf = std::conditional_t<(EPI & kStaged) != 0, CUtensorMap,
+                                   std::conditional_t<(EPI & kSplit) != 0, PeerParams, std::conditional_t<(EPI & kTail) != 0, Tail, Nothing>>>;
 
 // TR: 1 = B and C transposed ([N, K] and [N, M]), 2 = C alone.  EPI: what the epilogue is asked for (kStaged ...).  What is not run
 // costs a little too, in spilled registers and in instructions fetched around it: INT8 4096^2, 90 %, N = 512, fp16 results 6.10 us,
@@ -36,7 +38,9 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) spmm_rowacc_kernel
                                                                                  const __grid_constant__ ExtraOf<EPI> x,
                                                                                  const __grid_constant__ SpmmParams p) {
   constexpr bool STAGED = (EPI & kStaged) != 0, SPLIT = (EPI & kSplit) != 0, ACT = (EPI & kActive) != 0, TRACE = (EPI & kTraced) != 0;
+  constexpr bool TAIL = (EPI & kTail) != 0;
   static_assert(!TR || (!STAGED && !SPLIT), "transposed results are stored directly, of whole rows");
+  static_assert(!TAIL || (TR && ACT), "linear layers only");
   static_assert(!STAGED || C::COLS == kTile, "an epilogue warp stages whole columns of a tile row");
   extern __shared__ uint8_t smem_raw[];
   __shared__ PipeBars bars;
@@ -388,7 +392,8 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) spmm_rowacc_kernel
           }
 #pragma unroll
           for (int c = 0; c < C::COLS; c += 16) {
-            if (TR) finish16_tr<KIND, ACT>(to, row, n, m_first + c, &r[c], rs, csq, biasq);
+            if constexpr (TAIL) finish16_tail<KIND>(to, x, row, n, m_first + c, &r[c], rs, csq, biasq);
+            else if (TR) finish16_tr<KIND, ACT>(to, row, n, m_first + c, &r[c], rs, csq, biasq);
             else finish16<KIND, ACT>(to, row, n, m_first + c, &r[c], rs, csq, biasq);
           }
         }
@@ -409,11 +414,14 @@ int launch_rowacc(const RowaccLaunch& l) {
   if (ensure_smem((const void*)kernel, l.smem_bytes)) return VOID_ERR_CUDA;
   if constexpr ((EPI & kStaged) != 0) return status_of(launch_pdl(kernel, l.grid, C::THREADS, l.smem_bytes, l.stream, l.b, l.c, l.p));
   else if constexpr ((EPI & kSplit) != 0) return status_of(launch_pdl(kernel, l.grid, C::THREADS, l.smem_bytes, l.stream, l.b, l.peers, l.p));
+  else if constexpr ((EPI & kTail) != 0) return status_of(launch_pdl(kernel, l.grid, C::THREADS, l.smem_bytes, l.stream, l.b, l.tail, l.p));
   else return status_of(launch_pdl(kernel, l.grid, C::THREADS, l.smem_bytes, l.stream, l.b, Nothing{}, l.p));
 }
 template <int KIND, class C>
 int launch_rowacc(const RowaccLaunch& l) {
   if constexpr (KIND != VOID_KIND_F8E4M3 && (KIND != VOID_KIND_I8 || C::COLS == kTile)) {
+    if (l.transposed && (l.epilogue & kTail))
+      return l.transposed == 1 ? launch_rowacc<KIND, C, 1, kActive | kTail>(l) : launch_rowacc<KIND, C, 2, kActive | kTail>(l);
     if (l.transposed)
       return l.transposed == 1
                  ? (l.epilogue & kActive ? launch_rowacc<KIND, C, 1, kActive>(l) : launch_rowacc<KIND, C, 1, 0>(l))

@@ -19,6 +19,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/void_b200.h"
 #include "epilogue.cuh"
 #include "kinds.cuh"
@@ -170,9 +172,19 @@ __device__ __forceinline__ void load_b(const uint8_t* b, long long ldb, int k0, 
   }
 }
 
-// ACT: whether there may be an activation or a row bias (the kernel without is 0.2 us faster).
-template <int KIND, bool TR, int NG, bool ACT>
-__global__ void __launch_bounds__(512) skinny_kernel(const __grid_constant__ SkinnyParams p) {
+__device__ __forceinline__ float load_value(const void* p, int dtype, long long at) {
+  if (dtype == VOID_OUT_F32) return reinterpret_cast<const float*>(p)[at];
+  return f16_value(reinterpret_cast<const uint16_t*>(p)[at], dtype == VOID_OUT_F16);
+}
+__device__ __forceinline__ void store_value(void* p, int dtype, long long at, float v) {
+  if (dtype == VOID_OUT_F16) reinterpret_cast<__half*>(p)[at] = __float2half_rn(v);
+  else if (dtype == VOID_OUT_BF16) reinterpret_cast<__nv_bfloat16*>(p)[at] = __float2bfloat16_rn(v);
+  else reinterpret_cast<float*>(p)[at] = v;
+}
+
+// ACT: whether there may be an activation or a row bias (the kernel without is 0.2 us faster).  TAIL: a linear layer's tail, too.
+template <int KIND, bool TR, int NG, bool ACT, bool TAIL>
+__global__ void __launch_bounds__(512) skinny_kernel(const __grid_constant__ std::conditional_t<TAIL, SkinnyTailParams, SkinnyParams> p) {
   constexpr int ES = Elem<KIND>::ES, NB = 8 * NG;
   using T = typename AccType<KIND>::T;
   extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -229,7 +241,7 @@ __global__ void __launch_bounds__(512) skinny_kernel(const __grid_constant__ Ski
                         bw[i][2 * q], bw[i][2 * q + 1]);
     }
   }
-  struct Output { int m, c, n, r; bool in; float cs, bias, row_bias; };
+  struct Output { int m, c, n, r; bool in; float cs, bias, row_bias, residual; };
   auto output = [&](int o) {
     Output x;
     x.m = TR ? (o & 31) : o / NB;
@@ -238,11 +250,13 @@ __global__ void __launch_bounds__(512) skinny_kernel(const __grid_constant__ Ski
     x.r = row * 32 + x.m;
     x.in = x.n < p.N && x.r < p.M;
     x.cs = p.b_scale;
-    x.bias = x.row_bias = 0.0f;
+    x.bias = x.row_bias = x.residual = 0.0f;
     if (x.in) {
       if (p.col_scale != nullptr) x.cs *= p.col_scale[x.n];
       if (p.bias != nullptr) x.bias = p.bias[x.n];
       if (ACT && p.row_bias != nullptr) x.row_bias = p.row_bias[x.r];
+      if constexpr (TAIL)
+        if (p.tail.residual != nullptr) x.residual = load_value(p.tail.residual, p.tail.residual_dtype, (long long)x.n * p.tail.ldr + x.r);
     }
     return x;
   };
@@ -272,45 +286,55 @@ __global__ void __launch_bounds__(512) skinny_kernel(const __grid_constant__ Ski
     for (int w = 0; w < warps; ++w) s += red[(w * 32 + x.m) * PITCH + x.c];
     float v = KIND == VOID_KIND_I8 ? __int2float_rn((int)s) : (float)s;
     v = (v * rs) * x.cs + x.bias;
-    if constexpr (ACT) v = activate(v + x.row_bias, p.act);
+    if constexpr (TAIL) {
+      v += x.row_bias;
+      if (p.tail.pre != nullptr) store_value(p.tail.pre, p.out_dtype, (long long)x.n * p.tail.ldp + x.r, v);
+      v = activate(v, p.act) + x.residual;
+    } else if constexpr (ACT) {
+      v = activate(v + x.row_bias, p.act);
+    }
     const long long at = TR ? (long long)x.n * p.ldc + x.r : (long long)x.r * p.ldc + x.n;
-    if (p.out_dtype == VOID_OUT_F16) reinterpret_cast<__half*>(p.out)[at] = __float2half_rn(v);
-    else if (p.out_dtype == VOID_OUT_BF16) reinterpret_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
-    else reinterpret_cast<float*>(p.out)[at] = v;
+    store_value(p.out, p.out_dtype, at, v);
   }
 }
 
-template <int KIND, bool TR, int NG, bool ACT>
-cudaError_t launch(const SkinnyParams& p, int nbr, int warps, cudaStream_t st) {
-  auto kernel = skinny_kernel<KIND, TR, NG, ACT>;
+template <int KIND, bool TR, int NG, bool ACT, bool TAIL>
+cudaError_t launch(const SkinnyTailParams& p, int nbr, int warps, cudaStream_t st) {
+  auto kernel = skinny_kernel<KIND, TR, NG, ACT, TAIL>;
   const int smem = warps * 32 * (8 * NG + 1) * 4;
   if (smem > 48 * 1024 && ensure_smem((const void*)kernel, smem)) return cudaErrorInvalidValue;
   return launch_pdl(kernel, dim3((unsigned)nbr, (unsigned)((p.N + 8 * NG - 1) / (8 * NG))), 32 * warps, smem, st, p);
 }
 template <int KIND, bool TR, int NG>
-cudaError_t launch(const SkinnyParams& p, int nbr, int warps, cudaStream_t st) {
-  return p.act != VOID_ACT_NONE || p.row_bias != nullptr ? launch<KIND, TR, NG, true>(p, nbr, warps, st) : launch<KIND, TR, NG, false>(p, nbr, warps, st);
+cudaError_t launch(const SkinnyTailParams& p, bool tail, int nbr, int warps, cudaStream_t st) {
+  if constexpr (TR)
+    if (tail) return launch<KIND, TR, NG, true, true>(p, nbr, warps, st);
+  return p.act != VOID_ACT_NONE || p.row_bias != nullptr ? launch<KIND, TR, NG, true, false>(p, nbr, warps, st)
+                                                         : launch<KIND, TR, NG, false, false>(p, nbr, warps, st);
 }
 template <int KIND, bool TR>
-cudaError_t launch_columns(const SkinnyParams& p, int nbr, int warps, cudaStream_t st) {
-  if (p.N <= 8) return launch<KIND, TR, 1>(p, nbr, warps, st);
-  if (p.N <= 16) return launch<KIND, TR, 2>(p, nbr, warps, st);
-  return launch<KIND, TR, 4>(p, nbr, warps, st);
+cudaError_t launch_columns(const SkinnyTailParams& p, bool tail, int nbr, int warps, cudaStream_t st) {
+  if (tail && !TR) return cudaErrorInvalidValue;
+  if (p.N <= 8) return launch<KIND, TR, 1>(p, tail, nbr, warps, st);
+  if (p.N <= 16) return launch<KIND, TR, 2>(p, tail, nbr, warps, st);
+  return launch<KIND, TR, 4>(p, tail, nbr, warps, st);
 }
 
 }  // namespace
 
-cudaError_t skinny_launch(const SkinnyParams& p, int kind, bool transposed, int nbr, long long nnz, cudaStream_t st) {
+cudaError_t skinny_launch(const SkinnyTailParams& p, int kind, bool transposed, bool tail, int nbr, long long nnz, cudaStream_t st) {
   // enough warps that a warp has a few tiles of its row, so that their loads are in flight together
   const long long avg = nbr > 0 ? nnz / nbr : 0;
   const int warps = avg >= 24 ? 16 : (avg >= 6 ? 8 : 4);
+#define VB_COLUMNS(KIND) (transposed ? launch_columns<KIND, true>(p, tail, nbr, warps, st) : launch_columns<KIND, false>(p, tail, nbr, warps, st))
   switch (kind) {
-    case VOID_KIND_I8: return transposed ? launch_columns<VOID_KIND_I8, true>(p, nbr, warps, st) : launch_columns<VOID_KIND_I8, false>(p, nbr, warps, st);
-    case VOID_KIND_F8E4M3: return transposed ? cudaErrorInvalidValue : launch_columns<VOID_KIND_F8E4M3, false>(p, nbr, warps, st);
-    case VOID_KIND_F16: return transposed ? launch_columns<VOID_KIND_F16, true>(p, nbr, warps, st) : launch_columns<VOID_KIND_F16, false>(p, nbr, warps, st);
-    case VOID_KIND_BF16: return transposed ? launch_columns<VOID_KIND_BF16, true>(p, nbr, warps, st) : launch_columns<VOID_KIND_BF16, false>(p, nbr, warps, st);
-    default: return transposed ? launch_columns<VOID_KIND_TF32, true>(p, nbr, warps, st) : launch_columns<VOID_KIND_TF32, false>(p, nbr, warps, st);
+    case VOID_KIND_I8: return VB_COLUMNS(VOID_KIND_I8);
+    case VOID_KIND_F8E4M3: return transposed ? cudaErrorInvalidValue : launch_columns<VOID_KIND_F8E4M3, false>(p, tail, nbr, warps, st);
+    case VOID_KIND_F16: return VB_COLUMNS(VOID_KIND_F16);
+    case VOID_KIND_BF16: return VB_COLUMNS(VOID_KIND_BF16);
+    default: return VB_COLUMNS(VOID_KIND_TF32);
   }
+#undef VB_COLUMNS
 }
 
 }  // namespace vb

@@ -3,6 +3,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "epilogue.cuh"
+
 namespace vb {
 
 struct SkinnyParams {
@@ -21,7 +23,10 @@ struct SkinnyParams {
   long long ldc;
   int out_dtype, act, terms, a_stable;
 };
+struct SkinnyTailParams : SkinnyParams {
+  Tail tail;                // read by the kernels with one
+};
 
-cudaError_t skinny_launch(const SkinnyParams& p, int kind, bool transposed, int nbr, long long nnz, cudaStream_t st);
+cudaError_t skinny_launch(const SkinnyTailParams& p, int kind, bool transposed, bool tail, int nbr, long long nnz, cudaStream_t st);
 
 }  // namespace vb

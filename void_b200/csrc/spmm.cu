@@ -232,7 +232,8 @@ static Passes make_passes(const DeviceInfo& dev, int rows, int n_chunks, long lo
   return p;
 }
 
-static int spmm_launch(const void_spmm_args* a, int kind, cudaStream_t stream) {
+// tail: what a linear layer's epilogue does besides, or null.
+static int spmm_launch(const void_spmm_args* a, int kind, cudaStream_t stream, const Tail* tail = nullptr) {
   if (a == nullptr) return VOID_ERR_BAD_ARG;
   if (a->M < 0 || a->N < 0 || a->K < 0 || a->nbr < 0 || a->nnz < 0) return VOID_ERR_BAD_ARG;
   if (a->M == 0 || a->N == 0) return VOID_OK;
@@ -267,7 +268,7 @@ static int spmm_launch(const void_spmm_args* a, int kind, cudaStream_t stream) {
 
   const bool drain = (a->scale_mode == VOID_SCALE_PER_TILE);
   if (few_columns(a, kind, es, drain)) {
-    SkinnyParams s;
+    SkinnyTailParams s;
     s.tiles = reinterpret_cast<const uint8_t*>(a->tiles);
     s.tile_cols = a->tile_cols;
     s.row_ptr = a->row_ptr;
@@ -283,10 +284,11 @@ static int spmm_launch(const void_spmm_args* a, int kind, cudaStream_t stream) {
     s.ldc = a->ldc;
     s.out_dtype = a->out_dtype;
     s.act = a->act;
+    s.tail = tail != nullptr ? *tail : Tail{};
     s.terms = a->tile_terms == 0 ? 1 : a->tile_terms;
     s.a_stable = (a->flags & 4) ? 1 : 0;
     if (s.terms < 1 || s.terms > 3 || (s.terms > 1 && kind != VOID_KIND_F8E4M3)) return VOID_ERR_BAD_ARG;
-    return status_of(skinny_launch(s, kind, tr, a->nbr, a->nnz, stream));
+    return status_of(skinny_launch(s, kind, tr, tail != nullptr, a->nbr, a->nnz, stream));
   }
   const int total_panels = (a->N + kPanelN - 1) / kPanelN;
   int np = a->panels_per_item;
@@ -561,9 +563,11 @@ static int spmm_launch(const void_spmm_args* a, int kind, cudaStream_t stream) {
   const bool traced = a->trace != nullptr;
   if (!drain) {
     const bool split = a->segs != nullptr || a->acc_out != nullptr || a->worker_partials != nullptr;
-    const bool active = split || traced || a->act != VOID_ACT_NONE || a->row_bias != nullptr;
-    const int epilogue = (staged ? kStaged : 0) | (split ? kSplit : 0) | (active ? kActive : 0) | (traced ? kTraced : 0);
-    const RowaccLaunch l = {shape, a->transposed, epilogue, grid, smem_bytes, stream, tmap, tmap_c, peers, p};
+    const bool active = split || traced || tail != nullptr || a->act != VOID_ACT_NONE || a->row_bias != nullptr;
+    const int epilogue = (staged ? kStaged : 0) | (split ? kSplit : 0) | (active ? kActive : 0) | (traced ? kTraced : 0) |
+                         (tail != nullptr ? kTail : 0);
+    const Tail none = {};
+    const RowaccLaunch l = {shape, a->transposed, epilogue, grid, smem_bytes, stream, tmap, tmap_c, peers, tail != nullptr ? *tail : none, p};
     return kind == VOID_KIND_I8       ? launch_rowacc<VOID_KIND_I8>(l)
            : kind == VOID_KIND_F8E4M3 ? launch_rowacc<VOID_KIND_F8E4M3>(l)
            : kind == VOID_KIND_TF32   ? launch_rowacc<VOID_KIND_TF32>(l)
@@ -617,6 +621,19 @@ static int static_scratch_ptr(unsigned char** out) {
     ptrs[dev] = static_cast<unsigned char*>(ptr);
   }
   *out = ptrs[dev];
+  return VOID_OK;
+}
+
+int make_tail(const void_spmm_args* a, const void_epilogue* e, Tail* t) {
+  if (a == nullptr || e == nullptr) return VOID_ERR_BAD_ARG;
+  if (a->transposed != 1 && a->transposed != 2) return VOID_ERR_BAD_ARG;
+  if (e->residual != nullptr && e->residual_dtype != VOID_OUT_F32 && e->residual_dtype != a->out_dtype) return VOID_ERR_BAD_ARG;
+  if ((e->residual != nullptr && e->ldr < a->M) || (e->pre != nullptr && e->ldp < a->M)) return VOID_ERR_SHAPE;
+  t->residual = e->residual;
+  t->pre = e->pre;
+  t->ldr = e->ldr;
+  t->ldp = e->ldp;
+  t->residual_dtype = e->residual_dtype;
   return VOID_OK;
 }
 
@@ -674,6 +691,12 @@ int void_spmm_f8(const void_spmm_args* args, void_stream_t stream) {
 int void_spmm_fp(const void_spmm_args* args, int32_t kind, void_stream_t stream) {
   if (kind != VOID_KIND_F16 && kind != VOID_KIND_BF16 && kind != VOID_KIND_TF32) return VOID_ERR_BAD_ARG;
   return vb::spmm_launch(args, kind, reinterpret_cast<cudaStream_t>(stream));
+}
+int void_spmm_linear(const void_spmm_args* args, const void_epilogue* epilogue, int32_t kind, void_stream_t stream) {
+  if (kind != VOID_KIND_I8 && kind != VOID_KIND_F16 && kind != VOID_KIND_BF16 && kind != VOID_KIND_TF32) return VOID_ERR_BAD_ARG;
+  vb::Tail tail;
+  const int st = vb::make_tail(args, epilogue, &tail);
+  return st != VOID_OK ? st : vb::spmm_launch(args, kind, reinterpret_cast<cudaStream_t>(stream), &tail);
 }
 int void_device_sm_count(void) {
   const vb::DeviceInfo d = vb::device_info();

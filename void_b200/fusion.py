@@ -12,7 +12,7 @@ FP8VOIDTensor selects the quantized kernels with the same epilogue.
 """
 from dataclasses import dataclass
 from enum import Enum
-from typing import List, Optional, Union
+from typing import List, Optional, Sequence, Union
 
 import torch
 
@@ -20,6 +20,7 @@ from . import _lib
 from .format import VOIDTensor
 from .fp8 import FP8VOIDTensor, void_spmm_fp8
 from .int_quant import Int8VOIDTensor, void_spmm_int8
+from .norm import void_layer_norm
 from .ops import _KIND_DTYPE, cached_fp, packed_fp, product_kind, void_linear, void_spmm
 
 
@@ -50,6 +51,17 @@ def get_activation_code(activation: Union[str, ActivationType]) -> int:
     if isinstance(activation, ActivationType):
         activation = activation.value
     return _ACTIVATION_CODES.get(activation.lower(), 0)
+
+
+def layer_activation(activation: Union[str, ActivationType]) -> int:
+    """Code of a layer's activation; names that no kernel fuses are refused."""
+    name = activation.value if isinstance(activation, ActivationType) else str(activation)
+    if name.lower() not in _ACTIVATION_CODES:
+        raise ValueError("unknown activation %r" % name)
+    code = _ACTIVATION_CODES[name.lower()]
+    if code > _lib.ACT_SILU:
+        raise NotImplementedError("activation %r is not fused on B200 (none, relu, gelu, silu are)" % name)
+    return code
 
 
 def _void_spmm_activation(a, b, bias, out, activation: str, **kw) -> torch.Tensor:
@@ -108,11 +120,23 @@ def _void_spmm_activation_row_bias(a, b: torch.Tensor, bias: Optional[torch.Tens
 
 
 def fused_sparse_mlp(x: torch.Tensor, w1: VOIDTensor, w2: VOIDTensor, activation: str = "gelu",
-                     bias1: Optional[torch.Tensor] = None, bias2: Optional[torch.Tensor] = None) -> torch.Tensor:
+                     bias1: Optional[torch.Tensor] = None, bias2: Optional[torch.Tensor] = None, *,
+                     residual: Optional[torch.Tensor] = None, norm: Optional[Sequence] = None) -> torch.Tensor:
     """y = W2 @ activation(W1 @ x + b1) + b2 for x of shape [*, in_features] (void/fusion.py:557-602): two
     launches, each with its bias and activation fused.  Activations stay [batch, features] (void_linear), or, where
     the layers are large enough to pay for one transposed copy of x, [features, batch] up to the result, which the
-    second product writes transposed: the reference makes three transposes."""
+    second product writes transposed: the reference makes three transposes.
+
+    Extensions: ``residual`` (shape of y, commonly x itself) is added in the second product's epilogue; ``norm`` = (weight | None,
+    bias | None[, eps]) puts a layer norm of x in front of W1.  With both, y = x + mlp(norm(x)), the feed-forward half of a
+    transformer block in three launches."""
+    if residual is not None:
+        assert residual.shape == x.shape[:-1] + (w2.shape[0],), f"residual must have shape {tuple(x.shape[:-1]) + (w2.shape[0],)}, got {tuple(residual.shape)}"
+        _lib.require_cuda(residual)
+        residual = residual if residual.dim() == 2 else residual.reshape(-1, residual.shape[-1])
+    if norm is not None:
+        with torch.no_grad():
+            x = void_layer_norm(x, *norm)
     code = get_activation_code(activation)
     if code > _lib.ACT_SILU:
         raise NotImplementedError("activation %r is not fused on B200 (none, relu, gelu, silu are)" % activation)
@@ -121,7 +145,7 @@ def fused_sparse_mlp(x: torch.Tensor, w1: VOIDTensor, w2: VOIDTensor, activation
         p1, p2 = cached_fp(w1, kind), cached_fp(w2, kind)
         if p1 is not None and p2 is not None:       # None: one of the checks that follow says why
             y = _lib.native().mlp_packed(p1.native, w1.values, w1.block_rows, w1.block_cols, w1.shape, p2.native, w2.values, w2.block_rows,
-                                         w2.block_cols, w2.shape, x, bias1, code, bias2)
+                                         w2.block_cols, w2.shape, x, bias1, code, bias2, residual)
             if y is not None:
                 return y
     if isinstance(w1, VOIDTensor) and isinstance(w2, VOIDTensor) and x.is_cuda and x.dtype in _lib.OUT_DTYPE_CODE:
@@ -129,11 +153,11 @@ def fused_sparse_mlp(x: torch.Tensor, w1: VOIDTensor, w2: VOIDTensor, activation
         if (_KIND_DTYPE[kind] is x.dtype and product_kind(w2, x) == kind and x.dim() >= 2 and x.shape[-1] == k1 and m1 == k2
                 and (bias1 is None or bias1.shape == (m1,)) and (bias2 is None or bias2.shape == (m2,))):
             y = _lib.native().mlp(packed_fp(w1, kind).native, packed_fp(w2, kind).native,
-                                  x if x.dim() == 2 else x.reshape(-1, k1), bias1, code, bias2)
+                                  x if x.dim() == 2 else x.reshape(-1, k1), bias1, code, bias2, residual)
             return y if x.dim() == 2 else y.reshape(x.shape[:-1] + (m2,))
     # mixed types, and the operands that an error has to be raised for
     hidden = void_linear(w1, x if x.dim() == 2 else x.reshape(-1, x.shape[-1]), bias1, code)
-    out = void_linear(w2, hidden, bias2, 0)
+    out = void_linear(w2, hidden, bias2, 0, residual=residual)
     return out if x.dim() == 2 else out.reshape(x.shape[:-1] + (out.shape[-1],))
 
 

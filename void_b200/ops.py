@@ -94,16 +94,20 @@ def void_spmm(a: VOIDTensor, b: torch.Tensor, out: Optional[torch.Tensor] = None
 
 
 def void_linear(a, x: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: int = 0,
-                out: Optional[torch.Tensor] = None, *, x_scale=None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-    """y = act(x @ A^T + bias) for activations x [batch, in] and a VOID weight A [out, in]: the linear layer
+                out: Optional[torch.Tensor] = None, *, x_scale=None, out_dtype: Optional[torch.dtype] = None,
+                residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """y = act(x @ A^T + bias) (+ residual) for activations x [batch, in] and a VOID weight A [out, in]: the linear layer
     without transposed copies.  The reference computes (A @ x^T)^T and so copies x^T and returns a strided
     view (void/fusion.py:586-598, :817-829; void/autograd.py:336); here the kernel reads x and writes y as
     they lie in memory.  ``a`` is a floating VOIDTensor (y in x's dtype) or an Int8VOIDTensor (x int8 with
     per-row scales ``x_scale`` [batch], or a float scalar; y fp32 unless ``out_dtype`` / ``out`` say otherwise).
-    ``bias`` has one value per output feature."""
+    ``bias`` has one value per output feature; ``residual`` [batch, out] (float32, float16 or bfloat16) is added in fp32 behind the
+    activation, in the same kernel.  It may be ``out`` itself: the residual stream is then updated in place."""
     assert x.dim() == 2 and x.shape[1] == a.shape[1], f"Dimension mismatch: A is {a.shape}, x is {tuple(x.shape)}"
-    _lib.require_cuda(a.values, x)
+    _lib.require_cuda(a.values, x, residual)
     M = a.shape[0]
+    if residual is not None:
+        assert residual.shape == (x.shape[0], M), f"residual must have shape {(x.shape[0], M)}, got {tuple(residual.shape)}"
     if bias is not None:
         assert bias.shape == (M,), f"bias must have shape ({M},), got {tuple(bias.shape)}"
     if isinstance(a, Int8VOIDTensor):
@@ -111,7 +115,7 @@ def void_linear(a, x: torch.Tensor, bias: Optional[torch.Tensor] = None, activat
             raise _lib.VoidB200Error("void_linear with an Int8VOIDTensor takes int8 activations, got %s" % x.dtype)
         scalar, col_scale = (1.0, x_scale) if isinstance(x_scale, torch.Tensor) else (1.0 if x_scale is None else float(x_scale), None)
         return _lib.native().spmm(a.packed().native, x, out, out_dtype or torch.float32, False, col_scale, scalar, None,
-                                  bias, activation, True, None)
+                                  bias, activation, True, None, residual)
     if x.dtype not in _lib.OUT_DTYPE_CODE:
         raise _lib.VoidB200Error("void_linear: x must be float32, float16 or bfloat16, got %s" % x.dtype)
     dtype = x.dtype
@@ -119,7 +123,7 @@ def void_linear(a, x: torch.Tensor, bias: Optional[torch.Tensor] = None, activat
     packed = packed_fp(a, kind)
     if dtype is not _KIND_DTYPE[kind]:
         x = x.to(_KIND_DTYPE[kind])
-    return _lib.native().spmm(packed.native, x, out, dtype, False, None, 1.0, None, bias, activation, True, None)
+    return _lib.native().spmm(packed.native, x, out, dtype, False, None, 1.0, None, bias, activation, True, None, residual)
 
 
 def void_spmv(a: VOIDTensor, x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
