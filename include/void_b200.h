@@ -448,6 +448,41 @@ VOID_API int void_activation_grad(const void* g, int64_t ldg, const void* z, int
                                   int32_t act, void* dz, int64_t lddz, void* dbias, int32_t bias_elem, void* ws, size_t ws_bytes,
                                   void_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Linear layers of experts (no counterpart in the reference): `rows` tokens sorted by expert, offsets[e] .. offsets[e + 1] those of
+ * expert e, each run multiplied with that expert's weight:  out_t = act(x_t A_e^T + bias_e).
+ * void_expert_plan cuts the runs into chunks of at most `chunk` tokens, on the device: offsets [n_experts + 1] of offset_bytes (4 or 8)
+ * bytes each; plan of void_expert_plan_words(n_experts, rows, chunk) int32, on 16 bytes.  Offsets are not trusted: each is brought into
+ * [0, rows] and not below the one before it, and the status word (where not NULL) reads 3 if one had to be.
+ * void_expert_linear: args as for void_spmm_linear with transposed = 1 and a kind of floating tiles, but with the weights of all
+ * experts in one packed store, expert behind expert: nbr tile rows, M outputs and K inputs are those of one expert, row_ptr
+ * [n_experts * nbr + 1], nnz all tiles, row_bias [n_experts * M] or NULL, N all tokens.  chunk 128, or 8, 16 or 32 (another kernel, for
+ * few tokens per expert).  Rows of out in no run are zeroed if zero_rest, else left alone.  epilogue: NULL, or `pre` alone.
+ * void_expert_tile_grad, void_expert_activation_grad: as void_linear_tile_grad and void_activation_grad, run by run: items name tile rows of
+ * all experts (e * ceil(M / 32) + r), dbias is [n_experts, cols]; z and dz may be NULL with VOID_ACT_NONE (then only the sums are
+ * taken).  Experts without tokens get zeros.  ws: void_expert_activation_grad_ws_bytes bytes, needed with dbias.
+ * ------------------------------------------------------------------------------------- */
+typedef struct void_experts {
+  const int32_t* plan;       /* of void_expert_plan */
+  int32_t n_experts, chunk;
+  const int32_t* row_order;  /* [n_experts * nbr]: tile row (within its expert) of the k-th row taken, or NULL for k; entries are
+                                clamped, see void_spmm_args.row_order */
+  int32_t zero_rest, reserved;
+} void_experts;
+VOID_API int64_t void_expert_plan_words(int32_t n_experts, int32_t rows, int32_t chunk);
+VOID_API int void_expert_plan(const void* offsets, int32_t offset_bytes, int32_t n_experts, int32_t rows, int32_t chunk, int32_t* plan,
+                              int32_t* status, void_stream_t stream);
+VOID_API int void_expert_linear(const void_spmm_args* args, const void_epilogue* epilogue, const void_experts* experts, int32_t kind,
+                                void_stream_t stream);
+VOID_API int void_expert_tile_grad(const void* grad_out, int64_t ldg, const void* x, int64_t ldx, int32_t M, int32_t K, int32_t N,
+                                   int32_t kind, const void_experts* experts, const int32_t* items, int32_t n_items,
+                                   const int32_t* tile_cols, const int32_t* block_indices, void* grad_tiles, int32_t out_dtype,
+                                   int32_t* status, void_stream_t stream);
+VOID_API size_t void_expert_activation_grad_ws_bytes(const void_experts* experts, int32_t rows, int32_t cols);
+VOID_API int void_expert_activation_grad(const void* g, int64_t ldg, const void* z, int64_t ldz, int32_t elem, const void_experts* experts,
+                                         int32_t rows, int32_t cols, int32_t act, void* dz, int64_t lddz, void* dbias, int32_t bias_elem,
+                                         void* ws, size_t ws_bytes, void_stream_t stream);
+
 VOID_API int void_spmm_i8(const void_spmm_args* args, void_stream_t stream);
 VOID_API int void_spmm_f8(const void_spmm_args* args, void_stream_t stream);
 

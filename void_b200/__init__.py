@@ -21,6 +21,7 @@ from .fusion import (ActivationType, FusedOpType, get_activation_code, void_spmm
 from .autograd import (VOIDSpMMFunction, VOIDLinearFunction, VOIDSpMM, SparseLinear, SparseFeedForward, spmm_tile_grad,
                        void_spmm_autograd)
 from .norm import void_layer_norm, VOIDLayerNorm
+from .experts import VOIDExperts, stack_experts, void_expert_linear, SparseExperts
 from .stream_k import (StreamKWorkload, compute_stream_k_workload, void_spmm_stream_k, analyze_workload_balance)
 from .scheduler import WorkloadProfile, analyze_workload
 from .distributed import (ShardingStrategy, DistributedVOIDTensor, shard_void_tensor, distributed_void_spmm,

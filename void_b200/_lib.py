@@ -54,6 +54,11 @@ class Epilogue(ctypes.Structure):
     _fields_ = [("residual", c_vp), ("ldr", c_i64), ("residual_dtype", c_i32), ("reserved", c_i32), ("pre", c_vp), ("ldp", c_i64)]
 
 
+class Experts(ctypes.Structure):
+    """Mirror of ``struct void_experts``."""
+    _fields_ = [("plan", c_vp), ("n_experts", c_i32), ("chunk", c_i32), ("row_order", c_vp), ("zero_rest", c_i32), ("reserved", c_i32)]
+
+
 class GroupStore(ctypes.Structure):
     """Mirror of ``struct void_group_store``."""
     _fields_ = [("blob", c_vp), ("records", c_vp), ("stage_ptr", c_vp), ("group_rows", c_vp), ("n_groups", c_i32),
@@ -112,6 +117,14 @@ _PROTOTYPES = {
     "void_activation_grad_ws_bytes": (c_sz, [c_i32, c_i32]),
     "void_activation_grad": (ctypes.c_int, [c_vp, c_i64, c_vp, c_i64, c_i32, c_i32, c_i32, c_i32, c_vp, c_i64, c_vp, c_i32, c_vp, c_sz,
                                             c_vp]),
+    "void_expert_plan_words": (c_i64, [c_i32, c_i32, c_i32]),
+    "void_expert_plan": (ctypes.c_int, [c_vp, c_i32, c_i32, c_i32, c_i32, c_vp, c_vp, c_vp]),
+    "void_expert_linear": (ctypes.c_int, [ctypes.POINTER(SpmmArgs), ctypes.POINTER(Epilogue), ctypes.POINTER(Experts), c_i32, c_vp]),
+    "void_expert_tile_grad": (ctypes.c_int, [c_vp, c_i64, c_vp, c_i64, c_i32, c_i32, c_i32, c_i32, ctypes.POINTER(Experts), c_vp, c_i32, c_vp,
+                                             c_vp, c_vp, c_i32, c_vp, c_vp]),
+    "void_expert_activation_grad_ws_bytes": (c_sz, [ctypes.POINTER(Experts), c_i32, c_i32]),
+    "void_expert_activation_grad": (ctypes.c_int, [c_vp, c_i64, c_vp, c_i64, c_i32, ctypes.POINTER(Experts), c_i32, c_i32, c_i32, c_vp, c_i64,
+                                                   c_vp, c_i32, c_vp, c_sz, c_vp]),
     "void_layer_norm": (ctypes.c_int, [c_vp, c_i32, c_i64, c_i64, c_i32, c_vp, c_vp, c_i32, c_f32, c_vp, c_i64, c_vp, c_vp]),
     "void_layer_norm_grad_ws_bytes": (c_sz, [c_i64, c_i32]),
     "void_layer_norm_grad": (ctypes.c_int, [c_vp, c_i64, c_vp, c_i64, c_i32, c_i64, c_i32, c_vp, c_i32, c_vp, c_vp, c_i64, c_vp, c_vp,
@@ -214,7 +227,8 @@ def status_word(device):
     return w
 
 
-STATUS_TEXT = {1: "a device-side wait gave up", 2: "a split row of the work plan does not fit the scratch it was given"}
+STATUS_TEXT = {1: "a device-side wait gave up", 2: "a split row of the work plan does not fit the scratch it was given",
+               3: "offsets of expert tokens that fall, or lie outside the batch"}
 
 
 def check_device_status(device=None):

@@ -8,8 +8,11 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/void_b200.h"
 #include "epilogue.cuh"
+#include "experts.cuh"
 #include "launch.cuh"
 #include "ptx.cuh"
 
@@ -19,7 +22,6 @@ namespace {
 
 // act'(z).  With s = sigmoid(w(z)): (z s)' = s + z s (1 - s) w'(z).
 __device__ __forceinline__ float slope(float z, int act) {
-  if (act == VOID_ACT_NONE) return 1.0f;
   if (act == VOID_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
   // (kGelu1, kGelu3 and kSilu carry -log2(e), for a sigmoid of powers of two)
   const bool gelu = act == VOID_ACT_GELU;
@@ -48,16 +50,30 @@ struct ActivationGradParams {
   long long ldg, ldz, lddz;
   int rows, cols, act;
 };
+struct RunsOfTokens {   // experts: a block takes a chunk of one expert's tokens (experts.cu)
+  const int32_t* head;
+  const int32_t* chunk_ptr;
+  const int4* chunks;
+};
+struct NoRuns {};
+template <bool RUNS>
+using RunsIf = std::conditional_t<RUNS, RunsOfTokens, NoRuns>;
 
 // VEC: elements of a 16-byte piece of rows that lie on such boundaries, else 1.
-template <typename T, int VEC>
-__global__ void __launch_bounds__(kGradThreads) activation_grad_kernel(const __grid_constant__ ActivationGradParams p) {
+template <typename T, int VEC, bool RUNS>
+__global__ void __launch_bounds__(kGradThreads) activation_grad_kernel(const __grid_constant__ ActivationGradParams p, const __grid_constant__ RunsIf<RUNS> runs) {
   constexpr int WARPS = kGradThreads / 32;
   __shared__ float part[WARPS][32 * VEC];
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c0 = (blockIdx.x * 32 + lane) * VEC;
-  const int r0 = blockIdx.y * kGradRows, r1 = r0 + kGradRows < p.rows ? r0 + kGradRows : p.rows;
+  int r0 = blockIdx.y * kGradRows, r1 = r0 + kGradRows < p.rows ? r0 + kGradRows : p.rows;
+  if constexpr (RUNS) {
+    if ((int)blockIdx.y >= runs.head[0]) return;
+    const int4 c = runs.chunks[blockIdx.y];
+    r0 = c.y;
+    r1 = c.z;
+  }
   float s[VEC];
 #pragma unroll
   for (int e = 0; e < VEC; ++e) s[e] = 0.0f;
@@ -69,17 +85,18 @@ __global__ void __launch_bounds__(kGradThreads) activation_grad_kernel(const __g
       __align__(16) T gv[VEC], zv[VEC], o[VEC];
       if constexpr (VEC > 1) {
         *reinterpret_cast<uint4*>(gv) = *reinterpret_cast<const uint4*>(g);
-        *reinterpret_cast<uint4*>(zv) = *reinterpret_cast<const uint4*>(z);
+        if (p.act != VOID_ACT_NONE) *reinterpret_cast<uint4*>(zv) = *reinterpret_cast<const uint4*>(z);
       } else {
         gv[0] = *g;
-        zv[0] = *z;
+        if (p.act != VOID_ACT_NONE) zv[0] = *z;
       }
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const float d = value<T>(gv[e]) * slope(value<T>(zv[e]), p.act);
+        const float d = p.act != VOID_ACT_NONE ? value<T>(gv[e]) * slope(value<T>(zv[e]), p.act) : value<T>(gv[e]);
         s[e] += d;
         o[e] = rounded<T>(d);
       }
+      if (p.dz == nullptr) continue;
       if constexpr (VEC > 1) *reinterpret_cast<uint4*>(dz) = *reinterpret_cast<const uint4*>(o);
       else *dz = o[0];
     }
@@ -100,15 +117,22 @@ __global__ void __launch_bounds__(kGradThreads) activation_grad_kernel(const __g
 }
 
 // The row blocks' partial sums, in order: 32 columns and eight strands of blocks per block.
-template <typename P>
-__global__ void __launch_bounds__(256) partial_sums_kernel(const float* partials, int blocks, int cols, P* out) {
+// RUNS: the chunks of expert blockIdx.y.
+template <typename P, bool RUNS>
+__global__ void __launch_bounds__(256) partial_sums_kernel(const float* partials, int blocks, int cols, P* out, const __grid_constant__ RunsIf<RUNS> runs) {
   __shared__ float part[8][32];
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  int first = 0;
+  if constexpr (RUNS) {
+    first = runs.chunk_ptr[blockIdx.y];
+    blocks = runs.chunk_ptr[blockIdx.y + 1];
+    out += (size_t)blockIdx.y * (size_t)cols;
+  }
   float s = 0.0f;
   if (c < cols)
 #pragma unroll 4
-    for (int k = warp; k < blocks; k += 8) s += partials[(size_t)k * (size_t)cols + c];
+    for (int k = first + warp; k < blocks; k += 8) s += partials[(size_t)k * (size_t)cols + c];
   part[warp][lane] = s;
   __syncthreads();
   grid_launch_dependents();
@@ -122,20 +146,33 @@ __global__ void __launch_bounds__(256) partial_sums_kernel(const float* partials
 
 int row_blocks(int rows) { return (rows + kGradRows - 1) / kGradRows; }
 
-template <typename T, typename P>
-int activation_grad(const ActivationGradParams& p, P* dbias, cudaStream_t st) {
+// blocks: row blocks, or chunks there can be at most; experts: of runs
+template <typename T, typename P, bool RUNS>
+int activation_grad(const ActivationGradParams& p, const RunsIf<RUNS>& runs, int blocks, int experts, P* dbias, cudaStream_t st) {
   constexpr int V = 16 / (int)sizeof(T);
   auto on16 = [](const void* m, long long ld) { return (reinterpret_cast<uintptr_t>(m) & 15u) == 0 && ld % V == 0; };
   const bool wide = p.cols % V == 0 && on16(p.g, p.ldg) && on16(p.z, p.ldz) && on16(p.dz, p.lddz);
-  const int blocks = row_blocks(p.rows);
   cudaError_t rc = cudaSuccess;
   if (blocks > 0) {
-    if (wide) rc = launch_pdl(activation_grad_kernel<T, V>, dim3((unsigned)((p.cols + 32 * V - 1) / (32 * V)), (unsigned)blocks), kGradThreads, 0, st, p);
-    else rc = launch_pdl(activation_grad_kernel<T, 1>, dim3((unsigned)((p.cols + 31) / 32), (unsigned)blocks), kGradThreads, 0, st, p);
+    if (wide)
+      rc = launch_pdl(activation_grad_kernel<T, V, RUNS>, dim3((unsigned)((p.cols + 32 * V - 1) / (32 * V)), (unsigned)blocks), kGradThreads, 0, st, p, runs);
+    else rc = launch_pdl(activation_grad_kernel<T, 1, RUNS>, dim3((unsigned)((p.cols + 31) / 32), (unsigned)blocks), kGradThreads, 0, st, p, runs);
   }
   if (rc == cudaSuccess && dbias != nullptr)
-    rc = launch_pdl(partial_sums_kernel<P>, dim3((unsigned)((p.cols + 31) / 32)), 256, 0, st, p.partials, blocks, p.cols, dbias);
+    rc = launch_pdl(partial_sums_kernel<P, RUNS>, dim3((unsigned)((p.cols + 31) / 32), (unsigned)experts), 256, 0, st, p.partials, blocks, p.cols, dbias, runs);
   return status_of(rc);
+}
+template <bool RUNS>
+int activation_grad(const ActivationGradParams& p, const RunsIf<RUNS>& runs, int blocks, int experts, int elem, void* dbias, int bias_elem, cudaStream_t st) {
+  using H = __half;
+  using B = __nv_bfloat16;
+  float* f = reinterpret_cast<float*>(dbias);
+  if (elem == VOID_ELEM_F32) return activation_grad<float, float, RUNS>(p, runs, blocks, experts, f, st);
+  if (elem == VOID_ELEM_F16)
+    return bias_elem == VOID_ELEM_F32 ? activation_grad<H, float, RUNS>(p, runs, blocks, experts, f, st)
+                                      : activation_grad<H, H, RUNS>(p, runs, blocks, experts, reinterpret_cast<H*>(dbias), st);
+  return bias_elem == VOID_ELEM_F32 ? activation_grad<B, float, RUNS>(p, runs, blocks, experts, f, st)
+                                    : activation_grad<B, B, RUNS>(p, runs, blocks, experts, reinterpret_cast<B*>(dbias), st);
 }
 
 }  // namespace
@@ -162,13 +199,33 @@ int void_activation_grad(const void* g, int64_t ldg, const void* z, int64_t ldz,
   if (!dev.ok) return VOID_ERR_CUDA;
   if (dev.cc_major != 10) return VOID_ERR_ARCH;
   const ActivationGradParams p = {g, z, dz, dbias != nullptr ? reinterpret_cast<float*>(ws) : nullptr, ldg, ldz, lddz, rows, cols, act};
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const bool wide_bias = bias_elem == VOID_ELEM_F32;
-  if (elem == VOID_ELEM_F32) return activation_grad<float, float>(p, reinterpret_cast<float*>(dbias), st);
-  if (elem == VOID_ELEM_F16)
-    return wide_bias ? activation_grad<__half, float>(p, reinterpret_cast<float*>(dbias), st) : activation_grad<__half, __half>(p, reinterpret_cast<__half*>(dbias), st);
-  return wide_bias ? activation_grad<__nv_bfloat16, float>(p, reinterpret_cast<float*>(dbias), st)
-                   : activation_grad<__nv_bfloat16, __nv_bfloat16>(p, reinterpret_cast<__nv_bfloat16*>(dbias), st);
+  return activation_grad<false>(p, NoRuns{}, row_blocks(rows), 1, elem, dbias, bias_elem, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t void_expert_activation_grad_ws_bytes(const void_experts* x, int32_t rows, int32_t cols) {
+  if (x == nullptr || x->n_experts < 1 || x->chunk < 1 || rows <= 0 || cols <= 0) return 0;
+  return (size_t)vb::plan_capacity(x->n_experts, rows, x->chunk) * (size_t)cols * sizeof(float);
+}
+
+int void_expert_activation_grad(const void* g, int64_t ldg, const void* z, int64_t ldz, int32_t elem, const void_experts* x, int32_t rows,
+                                int32_t cols, int32_t act, void* dz, int64_t lddz, void* dbias, int32_t bias_elem, void* ws, size_t ws_bytes,
+                                void_stream_t stream) {
+  using namespace vb;
+  if (x == nullptr || x->plan == nullptr || x->n_experts < 1 || x->chunk < 1) return VOID_ERR_BAD_ARG;
+  if (elem < VOID_ELEM_F32 || elem > VOID_ELEM_BF16 || rows < 0 || cols < 0 || act < VOID_ACT_NONE || act > VOID_ACT_SILU) return VOID_ERR_BAD_ARG;
+  if (ldg < cols || (z != nullptr && ldz < cols) || (dz != nullptr && lddz < cols)) return VOID_ERR_BAD_ARG;
+  if (dbias != nullptr && bias_elem != elem && bias_elem != VOID_ELEM_F32) return VOID_ERR_BAD_ARG;
+  if (cols == 0 || (rows == 0 && dbias == nullptr)) return VOID_OK;
+  if (rows > 0 && (g == nullptr || (act != VOID_ACT_NONE && (z == nullptr || dz == nullptr)))) return VOID_ERR_BAD_ARG;
+  const PlanView v = plan_of(*x, rows);
+  if (v.capacity > 65535 || x->n_experts > 65535) return VOID_ERR_TOO_LARGE;
+  if (dbias != nullptr && rows > 0 && (ws == nullptr || ws_bytes < void_expert_activation_grad_ws_bytes(x, rows, cols))) return VOID_ERR_WORKSPACE;
+  const DeviceInfo dev = device_info();
+  if (!dev.ok) return VOID_ERR_CUDA;
+  if (dev.cc_major != 10) return VOID_ERR_ARCH;
+  const ActivationGradParams p = {g, z, dz, dbias != nullptr ? reinterpret_cast<float*>(ws) : nullptr, ldg, ldz, lddz, rows, cols, act};
+  const RunsOfTokens runs = {v.head, v.chunk_ptr, v.chunks};
+  return activation_grad<true>(p, runs, v.capacity, x->n_experts, elem, dbias, bias_elem, reinterpret_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -1132,7 +1132,8 @@ PyObject* finish_store(PyObject*, PyObject* const* a, Py_ssize_t n) {
 struct Structure {
   at::Tensor row_ptr[2], block_indices[2], tile_cols[2], row_order[2];   // of A, of A^T
   at::Tensor items, status;
-  int64_t M = 0, K = 0, nnz = 0;
+  int64_t M = 0, K = 0, nnz = 0;         // (of one expert's weight)
+  int64_t experts = 0;                   // weights of experts, tile row behind tile row; 0: one matrix
   mutable Readers readers;
   mutable std::atomic<bool> captured{false};   // a graph reads these arrays
 };
@@ -1143,10 +1144,10 @@ struct StructureObject {
 PyTypeObject* g_structure_type = nullptr;
 
 // structure(row_ptr, block_indices, tile_cols, row_ptr_t, block_indices_t, tile_cols_t, items, status, M, K, n_blocks,
-//           row_order | None, row_order_t | None)
+//           row_order | None, row_order_t | None[, experts]); experts: M and K are those of one expert, the tile rows those of all
 PyObject* structure(PyObject*, PyObject* const* a, Py_ssize_t n) {
   NATIVE_BEGIN
-  if (n != 13) throw torch::TypeError("structure takes 13 arguments");
+  if (n != 13 && n != 14) throw torch::TypeError("structure takes 13 or 14 arguments");
   auto st = std::make_shared<Structure>();
   for (int i = 0; i < 2; ++i) {
     st->row_ptr[i] = cuda_tensor(a[3 * i], "row_ptr");
@@ -1159,8 +1160,10 @@ PyObject* structure(PyObject*, PyObject* const* a, Py_ssize_t n) {
   st->M = integer(a[8]);
   st->K = integer(a[9]);
   st->nnz = integer(a[10]);
-  check_index(st->row_ptr[0], st->block_indices[0], (st->M + 31) / 32, st->nnz);
-  check_index(st->row_ptr[1], st->block_indices[1], (st->K + 31) / 32, st->nnz);
+  if (n == 14) st->experts = integer(a[13]);
+  const int64_t weights = st->experts > 0 ? st->experts : 1;
+  check_index(st->row_ptr[0], st->block_indices[0], (st->M + 31) / 32 * weights, st->nnz);
+  check_index(st->row_ptr[1], st->block_indices[1], (st->K + 31) / 32 * weights, st->nnz);
   PyObject* self = PyType_GenericAlloc(g_structure_type, 0);
   if (self == nullptr) return nullptr;
   new (&reinterpret_cast<StructureObject*>(self)->st) std::shared_ptr<const Structure>(std::move(st));
@@ -1398,6 +1401,257 @@ PyObject* values_product(PyObject*, PyObject* const* a, Py_ssize_t n) {
   NATIVE_END
 }
 
+// ------------------------------------------------------------------------------------------ experts
+// The runs of tokens of a batch, cut into chunks on the device.
+struct ExpertPlan {
+  at::Tensor words;
+  void_experts x = {};
+};
+// Tokens per chunk, which chooses the kernel: see experts.cu.
+int32_t expert_chunk(int64_t rows, int64_t experts) {
+  const int64_t each = (rows + experts - 1) / experts;
+  return each <= 8 ? 8 : (each <= 16 ? 16 : (each <= 48 ? 32 : 128));
+}
+ExpertPlan expert_plan(const at::Tensor& offsets_in, int64_t rows, int64_t experts, c10::Device dev, int32_t* status) {
+  if (offsets_in.dim() != 1 || offsets_in.size(0) != experts + 1)
+    fail("offsets must be a vector of " + std::to_string(experts + 1) + " integers, one more than there are experts");
+  if (offsets_in.device() != dev) fail("tokens and offsets are on different devices");
+  if (offsets_in.scalar_type() != at::kInt && offsets_in.scalar_type() != at::kLong)
+    fail(std::string("offsets must be int32 or int64, got ") + c10::toString(offsets_in.scalar_type()));
+  const at::Tensor offsets = offsets_in.contiguous();
+  ExpertPlan plan;
+  plan.x.n_experts = (int32_t)experts;
+  plan.x.chunk = expert_chunk(rows, experts);
+  plan.words = new_cuda({void_expert_plan_words(plan.x.n_experts, (int32_t)rows, plan.x.chunk)}, at::kInt, dev);
+  plan.x.plan = plan.words.const_data_ptr<int32_t>();
+  check(void_expert_plan(offsets.const_data_ptr(), (int32_t)offsets.element_size(), plan.x.n_experts, (int32_t)rows, plan.x.chunk,
+                         plan.words.data_ptr<int32_t>(), status, stream_of(dev.index())),
+        "void_expert_plan");
+  return plan;
+}
+void check_tokens(const at::Tensor& x, int64_t K, const char* what) {
+  if (x.dim() != 2 || x.size(1) != K)
+    fail(std::string(what) + " must be a matrix of tokens with " + std::to_string(K) + " features");
+  if (x.size(0) > 0x40000000) fail("a batch has at most 2^30 tokens");
+}
+// expert_linear(handle, experts, M, x [N, K], offsets, bias [experts, M] | None, act, out | None, row_order | None) -> out
+PyObject* expert_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NATIVE_BEGIN
+  if (n != 9) throw torch::TypeError("expert_linear takes 9 arguments");
+  Packed* pk = packed_of(a[0]);
+  const int64_t experts = integer(a[1]), M = integer(a[2]);
+  const at::Tensor& x_in = cuda_tensor(a[3], "x");
+  const at::Tensor& offsets = cuda_tensor(a[4], "offsets");
+  const c10::Device dev = x_in.device();
+  check_tokens(x_in, pk->K, "x");
+  if (dev.index() != pk->device) fail("A and x are on different devices");
+  const int64_t N = x_in.size(0);
+  const int es = elem_bytes(pk->kind);
+  c10::cuda::OptionalCUDAGuard guard;
+  if (c10::cuda::current_device() != dev.index()) guard.set_device(dev);
+  at::Tensor out;
+  if (none(a[7])) {
+    out = new_cuda({N, M}, x_in.scalar_type(), dev);
+  } else {
+    out = cuda_tensor(a[7], "out");
+    if (out.dim() != 2 || out.size(0) != N || out.size(1) != M || (M > 1 && out.stride(1) != 1) || (N > 1 && out.stride(0) < M))
+      fail("out must be a row-major [" + std::to_string(N) + ", " + std::to_string(M) + "] tensor");
+    if (out.device() != dev) fail("out and x are on different devices");
+  }
+  ExpertPlan plan = expert_plan(offsets, N, experts, dev, pk->args.status);
+  const at::Tensor x = kernel_operand(x_in, es);
+  void_spmm_args s = pk->args;
+  s.nbr = (int32_t)((M + 31) / 32);
+  s.M = (int32_t)M;
+  s.b = x.const_data_ptr();
+  s.ldb = row_pitch(x, es);
+  s.N = (int32_t)N;
+  s.b_scale = 1.0f;
+  s.scale_mode = VOID_SCALE_ROW_MEAN;
+  s.transposed = 1;
+  at::Tensor bias, order;
+  if (!none(a[5])) {
+    bias = fp32_vector(a[5], dev, "bias");
+    if (bias.numel() != experts * M) fail("bias must have " + std::to_string(experts) + " x " + std::to_string(M) + " elements");
+    s.row_bias = bias.const_data_ptr<float>();
+  }
+  s.act = (int32_t)integer(a[6]);
+  s.out = out.data_ptr();
+  s.ldc = N > 1 ? out.stride(0) : M;
+  s.out_dtype = out_code(out.scalar_type());
+  s.flags = pk->stable ? 4 : 0;
+  if (!none(a[8])) {
+    order = cuda_tensor(a[8], "row_order");
+    if (order.scalar_type() != at::kInt || !order.is_contiguous() || order.numel() != experts * s.nbr) fail("row_order does not belong to these experts");
+    c10::cuda::CUDACachingAllocator::recordStream(order.storage().data_ptr(), c10::cuda::getCurrentCUDAStream(dev.index()));
+    plan.x.row_order = order.const_data_ptr<int32_t>();
+  }
+  plan.x.zero_rest = none(a[7]) ? 1 : 0;
+  check(void_expert_linear(&s, nullptr, &plan.x, pk->kind, launch_stream(pk)), "void_expert_linear");
+  if (!none(a[7])) {
+    Py_INCREF(a[7]);
+    return a[7];
+  }
+  return THPVariable_Wrap(out);
+  NATIVE_END
+}
+
+// act(x A_e^T + bias_e) for the tokens of every run (A_e transposed: x A_e), zeros for the others.  pre: x A_e^T + bias_e, where not null.
+at::Tensor expert_product(const Structure& st, bool a_transposed, const at::Tensor& values_in, const at::Tensor& x_in, const ExpertPlan& plan,
+                          const at::Tensor* bias, int32_t act, at::Tensor* pre) {
+  const c10::Device dev = x_in.device();
+  const int kind = common_kind(values_in.scalar_type(), x_in.scalar_type()), es = elem_bytes(kind), way = a_transposed ? 1 : 0;
+  const at::Tensor values = as_type(values_in, kind_type(kind)).contiguous();
+  const int64_t M = a_transposed ? st.K : st.M, K = a_transposed ? st.M : st.K, N = x_in.size(0);
+  check_tokens(x_in, K, "the tokens");
+  check_tiles(st, values);
+  const at::Tensor x = kernel_operand(as_type(x_in, kind_type(kind)), es);
+  at::Tensor out = new_cuda({N, M}, x_in.scalar_type(), dev);
+  const at::Tensor store = new_cuda({std::max<int64_t>(st.nnz, 1) * 1024 * es + 1024}, at::kByte, dev);
+  uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(store.data_ptr()) + 1023) & ~uintptr_t(1023));
+  const void_stream_t stream = launch_stream(st, dev);
+  check(void_repack_tiles_fp(values.const_data_ptr(), es, st.block_indices[way].const_data_ptr<int32_t>(), st.nnz, way, tiles, stream),
+        "void_repack_tiles_fp");
+  void_spmm_args s = void_spmm_args();
+  s.tiles = tiles;
+  s.tile_cols = st.tile_cols[way].const_data_ptr<int32_t>();
+  s.row_ptr = st.row_ptr[way].const_data_ptr<int32_t>();
+  s.nbr = (int32_t)((M + 31) / 32);
+  s.nbc = (int32_t)((K + 31) / 32);
+  s.nnz = st.nnz;
+  s.b = x.const_data_ptr();
+  s.ldb = row_pitch(x, es);
+  s.K = (int32_t)K;
+  s.N = (int32_t)N;
+  s.M = (int32_t)M;
+  s.b_scale = 1.0f;
+  at::Tensor shift;
+  if (bias != nullptr) {
+    shift = bias->to(dev, at::kFloat).contiguous();
+    if (shift.numel() != st.experts * M) fail("bias must have " + std::to_string(st.experts) + " x " + std::to_string(M) + " elements");
+    s.row_bias = shift.const_data_ptr<float>();
+  }
+  s.act = act;
+  s.out = out.data_ptr();
+  s.ldc = M;
+  s.out_dtype = out_code(out.scalar_type());
+  s.scale_mode = VOID_SCALE_ROW_MEAN;
+  s.status = st.status.data_ptr<int32_t>();
+  s.transposed = 1;
+  void_experts e = plan.x;
+  e.zero_rest = 1;
+  if (st.row_order[way].defined()) e.row_order = st.row_order[way].const_data_ptr<int32_t>();
+  void_epilogue tail = {};
+  if (pre != nullptr) {
+    *pre = pitched(N, M, out.scalar_type(), (int)out.element_size(), dev);
+    tail.pre = pre->data_ptr();
+    tail.ldp = pre->stride(0);
+  }
+  check(void_expert_linear(&s, pre != nullptr ? &tail : nullptr, &e, kind, stream), "void_expert_linear");
+  return out;
+}
+struct ExpertBackward : torch::autograd::Node {
+  torch::autograd::SavedVariable values, dense;
+  std::shared_ptr<const Structure> st;
+  ExpertPlan plan;
+  at::Tensor pre;
+  int32_t act = VOID_ACT_NONE;
+  at::ScalarType bias_type = at::kFloat;
+
+  std::string name() const override { return "VOIDExpertBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    values.reset_data();
+    dense.reset_data();
+    pre.reset();
+    plan.words.reset();
+  }
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    torch::autograd::variable_list out(3);
+    if (!grads[0].defined()) return out;
+    no_second_derivative("a layer of experts");
+    const at::Tensor v = values.unpack(), x = dense.unpack();
+    c10::cuda::OptionalCUDAGuard guard(x.device());
+    at::AutoDispatchBelowADInplaceOrView below;
+    try {
+      const c10::Device dev = x.device();
+      const int64_t N = x.size(0), M = st->M, E = st->experts;
+      at::Tensor g = as_type(grads[0], x.scalar_type()).contiguous(), dz = g;
+      const int elem = out_code(g.scalar_type());
+      const bool sums = task_should_compute_output(2);
+      if (act != VOID_ACT_NONE || sums) {
+        at::Tensor ws;
+        if (act != VOID_ACT_NONE) dz = pitched(N, M, g.scalar_type(), (int)g.element_size(), dev);
+        if (sums) {
+          out[2] = new_cuda({E, M}, bias_type == at::kFloat ? at::kFloat : g.scalar_type(), dev);
+          ws = new_cuda({(int64_t)void_expert_activation_grad_ws_bytes(&plan.x, (int32_t)N, (int32_t)M)}, at::kByte, dev);
+        }
+        check(void_expert_activation_grad(g.const_data_ptr(), M, pre.defined() ? pre.const_data_ptr() : nullptr, pre.defined() ? pre.stride(0) : M, elem,
+                                          &plan.x, (int32_t)N, (int32_t)M, act, act != VOID_ACT_NONE ? dz.data_ptr() : nullptr, dz.stride(0),
+                                          sums ? out[2].data_ptr() : nullptr, sums ? out_code(out[2].scalar_type()) : elem,
+                                          ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? (size_t)ws.numel() : 0, stream_of(dev.index())),
+              "void_expert_activation_grad");
+      }
+      if (task_should_compute_output(1)) out[1] = expert_product(*st, true, v, dz, plan, nullptr, VOID_ACT_NONE, nullptr);
+      if (task_should_compute_output(0)) {
+        if (st->nnz == 0 || N == 0) {
+          out[0] = at::zeros({st->nnz, 32, 32}, x.options().dtype(v.scalar_type()));
+        } else {
+          const int kind = common_kind(dz.scalar_type(), x.scalar_type()), es = elem_bytes(kind);
+          const at::Tensor gk = kernel_operand(dz, es), xk = kernel_operand(x, es);
+          out[0] = new_cuda({st->nnz, 32, 32}, v.scalar_type(), dev);
+          check(void_expert_tile_grad(gk.const_data_ptr(), row_pitch(gk, es), xk.const_data_ptr(), row_pitch(xk, es), (int32_t)M, (int32_t)st->K,
+                                      (int32_t)N, kind, &plan.x, st->items.const_data_ptr<int32_t>(), (int32_t)st->items.size(0),
+                                      st->tile_cols[0].const_data_ptr<int32_t>(), st->block_indices[0].const_data_ptr<int32_t>(), out[0].data_ptr(),
+                                      out_code(v.scalar_type()), st->status.data_ptr<int32_t>(), launch_stream(*st, dev)),
+                "void_expert_tile_grad");
+        }
+      }
+    } catch (const Failure& f) {
+      TORCH_CHECK(false, f.text);
+    }
+    return out;
+  }
+};
+// expert_values_product(structure, values, x, offsets, bias | None, act) -> act(x A_e^T + bias_e); differentiable in values, x and bias
+PyObject* expert_values_product(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NATIVE_BEGIN
+  if (n != 6) throw torch::TypeError("expert_values_product takes 6 arguments");
+  std::shared_ptr<const Structure> st = structure_of(a[0]);
+  const at::Tensor &values = cuda_tensor(a[1], "values"), &x = cuda_tensor(a[2], "x"), &offsets = cuda_tensor(a[3], "offsets");
+  const at::Tensor none_given;
+  const at::Tensor& bias = none(a[4]) ? none_given : tensor(a[4], "bias");
+  const int32_t act = (int32_t)integer(a[5]);
+  out_code(x.scalar_type());
+  check_tokens(x, st->K, "x");
+  c10::cuda::OptionalCUDAGuard guard(x.device());
+  for (const at::Tensor* t : {&values, &x, &bias})
+    TORCH_CHECK_NOT_IMPLEMENTED(!torch::autograd::isFwGradDefined(*t), "a layer of experts has no forward-mode derivative: an operand carries a tangent");
+  const bool recorded = torch::autograd::compute_requires_grad(values, x, bias), kept = recorded && act != VOID_ACT_NONE;
+  at::Tensor out, pre;
+  ExpertPlan plan;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    plan = expert_plan(offsets, x.size(0), st->experts, x.device(), st->status.data_ptr<int32_t>());
+    out = expert_product(*st, false, values, x, plan, bias.defined() ? &bias : nullptr, act, kept ? &pre : nullptr);
+  }
+  if (recorded) {
+    auto node = std::shared_ptr<ExpertBackward>(new ExpertBackward(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(values, x, bias));
+    node->values = torch::autograd::SavedVariable(values, false);
+    node->dense = torch::autograd::SavedVariable(x, false);
+    node->st = std::move(st);
+    node->plan = std::move(plan);
+    node->pre = std::move(pre);
+    node->act = act;
+    if (bias.defined()) node->bias_type = bias.scalar_type();
+    torch::autograd::set_history(out, node);
+  }
+  return THPVariable_Wrap(out);
+  NATIVE_END
+}
+
 // tile_gradient(structure, grad, b, linear, dtype) -> dL/dA_values
 PyObject* tile_gradient(PyObject*, PyObject* const* a, Py_ssize_t n) {
   NATIVE_BEGIN
@@ -1563,6 +1817,8 @@ PyMethodDef kMethods[] = {
     FAST(values_product),
     FAST(tile_gradient),
     FAST(layer_norm),
+    FAST(expert_linear),
+    FAST(expert_values_product),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

@@ -49,6 +49,8 @@
 #include <cuda_fp16.h>
 #include <cudaTypedefs.h>
 
+#include <type_traits>
+
 #include "../../include/void_b200.h"
 #include "epilogue.cuh"
 #include "kinds.cuh"
@@ -182,15 +184,51 @@ __device__ __forceinline__ void stamp(const SpmmParams& p, int slot) {
   }
 }
 
+// A product whose weight is one of several experts', each multiplied with its own run of tokens (B and C transposed): work items are
+// (chunk of an expert's tokens, tile row), chunks as laid out by expert_plan_kernel (experts.cu).
+struct ExpertParams {
+  Tail tail;
+  const int32_t* head;        // number of chunks
+  const int32_t* bounds;      // [experts + 1]: where the experts' runs of tokens begin, and the end of the last
+  const int4* chunks;         // expert, first token, token behind the last
+  const int32_t* row_order;   // [experts][tile rows]: tile row of the k-th row taken, or null for k
+  int n_experts, zero_rest;   // zero_rest: tokens outside all runs get zeros
+};
+struct Nothing {};
+template <class X>
+constexpr bool kExpertsOf = std::is_same<X, ExpertParams>::value;
+
 struct Seg {
   int row, chunk, t0, t1, nseg, slot0, my_idx, ctr;
+  int n0, n1;   // experts: tokens of the chunk
 };
+// Item i of a product of experts, as words in the order row, chunk, first and last tile, tokens, expert.
+__device__ __forceinline__ void expert_item(const SpmmParams& p, const ExpertParams& x, int i, int& row, int& at, int4& c, int& chunk) {
+  chunk = i / p.nbr;
+  row = i - chunk * p.nbr;
+  c = x.chunks[chunk];
+  at = c.x * p.nbr;
+  if (x.row_order != nullptr) {
+    const int r = x.row_order[at + row];
+    row = r < 0 ? 0 : (r >= p.nbr ? p.nbr - 1 : r);
+  }
+  at += row;
+}
 
 // PLAN: the launch may come with a work plan.
-template <bool PLAN>
-__device__ __forceinline__ Seg load_seg(const SpmmParams& p, int i) {
+template <bool PLAN, class X = Nothing>
+__device__ __forceinline__ Seg load_seg(const SpmmParams& p, int i, const X& x = X{}) {
   Seg s;
-  if (PLAN && p.segs != nullptr) {
+  if constexpr (kExpertsOf<X>) {
+    int at;
+    int4 c;
+    expert_item(p, x, i, s.row, at, c, s.chunk);
+    s.t0 = p.row_ptr[at];
+    s.t1 = p.row_ptr[at + 1];
+    s.n0 = c.y;
+    s.n1 = c.z;
+    s.nseg = 1; s.slot0 = 0; s.my_idx = 0; s.ctr = 0;
+  } else if (PLAN && p.segs != nullptr) {
     const int4* q = reinterpret_cast<const int4*>(p.segs) + 2 * (size_t)i;
     const int4 a = q[0], b = q[1];
     s.row = a.x; s.chunk = a.y; s.t0 = a.z; s.t1 = a.w;
@@ -210,9 +248,17 @@ __device__ __forceinline__ Seg load_seg(const SpmmParams& p, int i) {
   return s;
 }
 
-// The same for a warp that waits with many values in registers: lane k holds word k (in the order of Seg's fields).
-template <bool PLAN>
-__device__ __forceinline__ int load_seg_word(const SpmmParams& p, int i, int lane) {
+// The same for a warp that waits with many values in registers: lane k holds word k (in the order of Seg's fields; experts: words 4, 5
+// and 6 are the chunk's tokens and the expert).
+template <bool PLAN, class X = Nothing>
+__device__ __forceinline__ int load_seg_word(const SpmmParams& p, int i, int lane, const X& x = X{}) {
+  if constexpr (kExpertsOf<X>) {
+    int r, at, c;
+    int4 t;
+    expert_item(p, x, i, r, at, t, c);
+    if (lane == 2 || lane == 3) return p.row_ptr[at + lane - 2];
+    return lane == 0 ? r : (lane == 1 ? c : (lane == 4 ? t.y : (lane == 5 ? t.z : t.x)));
+  }
   if (PLAN && p.segs != nullptr) return p.segs[8 * (size_t)i + (lane & 7)];   // (without a branch, whose register costs 0.1 us of 14.9)
   int k, chunk;
   p.passes.item(i, k, chunk);
@@ -227,9 +273,13 @@ __device__ __forceinline__ int load_seg_word(const SpmmParams& p, int i, int lan
 __device__ __forceinline__ int word_of(int words, int k) { return __shfl_sync(0xffffffffu, words, k); }
 
 // Range of segment indices of this CTA: [begin, end) with stride step.
-template <bool PLAN>
-__device__ __forceinline__ void seg_range(const SpmmParams& p, int& begin, int& end, int& step) {
-  if (PLAN && p.segs != nullptr) {
+template <bool PLAN, class X = Nothing>
+__device__ __forceinline__ void seg_range(const SpmmParams& p, int& begin, int& end, int& step, const X& x = X{}) {
+  if constexpr (kExpertsOf<X>) {
+    begin = blockIdx.x;
+    end = x.head[0] * p.nbr;
+    step = gridDim.x;
+  } else if (PLAN && p.segs != nullptr) {
     begin = p.cta_seg_ptr[blockIdx.x];
     end = p.cta_seg_ptr[blockIdx.x + 1];
     step = 1;
@@ -244,6 +294,11 @@ __device__ __forceinline__ int panels_in_chunk(const SpmmParams& p, int chunk) {
   const int total = (p.N + kPanelN - 1) / kPanelN;
   const int left = total - chunk * p.np;
   return left < p.np ? left : p.np;
+}
+
+template <class X>
+__device__ __forceinline__ int panels_of(const SpmmParams& p, const Seg& s) {
+  return kExpertsOf<X> ? (s.n1 - s.n0 + kPanelN - 1) / kPanelN : panels_in_chunk(p, s.chunk);
 }
 
 __device__ __forceinline__ OutDesc out_desc(const SpmmParams& p) {
@@ -285,26 +340,26 @@ __device__ __forceinline__ int stage_cap(const SpmmParams& p, int stage) {
 // claims its first ring stage and starts the bulk copy of that stage's tiles BEFORE the wait, while the
 // previous kernel is still draining; only the panels of B - typically that kernel's output - are
 // requested after it.
-template <class C, int ES, int TR, bool PLAN, bool TRACE>
+template <class C, int ES, int TR, bool PLAN, bool TRACE, class X = Nothing>
 __device__ __forceinline__ void producer_loop(const SpmmParams& p, const CUtensorMap* tmap, PipeBars* bars,
                                               uint32_t ring_base, uint32_t stage_bytes, volatile int* ctl,
-                                              int lane, int pw) {
+                                              int lane, int pw, const X& x = X{}) {
   bool waited = p.a_stable == 0;
   if (waited) grid_dependency_wait();
   if (TRACE && pw == 0 && lane == 0) stamp<TRACE>(p, 56);   // producer starts
   int begin, end, step;
-  seg_range<PLAN>(p, begin, end, step);
+  seg_range<PLAN>(p, begin, end, step, x);
   const int S = p.stages;
   // position of the next group in the ring: its stage, the parity of the stage's use, the warp it belongs to
   int stage = 0, owner = 0, gcount = 0;
   uint32_t phase = 0;
   Seg seg_next = {};  // the next segment's descriptor is fetched one item ahead
-  if (begin < end) seg_next = load_seg<PLAN>(p, begin);
+  if (begin < end) seg_next = load_seg<PLAN>(p, begin, x);
   for (int i = begin; i < end; i += step) {
     const Seg s = seg_next;
-    if (i + step < end) seg_next = load_seg<PLAN>(p, i + step);
-    const int npan = panels_in_chunk(p, s.chunk);
-    const int n0 = s.chunk * p.np * kPanelN;
+    if (i + step < end) seg_next = load_seg<PLAN>(p, i + step, x);
+    const int npan = panels_of<X>(p, s);
+    const int n0 = kExpertsOf<X> ? s.n0 : s.chunk * p.np * kPanelN;
     const uint32_t unit_bytes = (uint32_t)((kTileBytes * p.terms + ((p.use3d && TR != 1) ? p.np : npan) * kPanelBytes) * ES);
     if (TRACE && i == begin && pw == 0 && lane == 0) {
       asm volatile("" ::"r"(s.t1) : "memory");
@@ -446,7 +501,8 @@ __device__ __forceinline__ void pipeline_teardown(const SpmmParams& p, int* ctl_
 //   kActive  activation, row bias
 //   kTraced  time stamps (slim INT8 only, with kActive)
 //   kTail    what a linear layer adds (Tail in epilogue.cuh; transposed results only, with kActive)
-constexpr int kStaged = 1, kSplit = 2, kActive = 4, kTraced = 8, kTail = 16;
+//   kExperts the weight of one of several experts for each run of tokens (ExpertParams; B and C transposed, with kActive and kTail)
+constexpr int kStaged = 1, kSplit = 2, kActive = 4, kTraced = 8, kTail = 16, kExperts = 32;
 struct RowaccLaunch {
   int shape;   // 1 wide, 2 slim, 6 mid
   int transposed;
@@ -461,5 +517,15 @@ struct RowaccLaunch {
 };
 template <int KIND>
 int launch_rowacc(const RowaccLaunch& l);
+// The same for experts (mid shape).
+struct ExpertLaunch {
+  int grid, smem_bytes;
+  cudaStream_t stream;
+  const CUtensorMap& b;
+  const ExpertParams& x;
+  const SpmmParams& p;
+};
+template <int KIND>
+int launch_experts(const ExpertLaunch& l);
 
 }  // namespace vb

@@ -25,10 +25,28 @@ __device__ __forceinline__ int32_t* row_sums(const SpmmParams& p, const X& x, in
 // What a kernel is given besides B and the common parameters: C as a tensor, the peers of a sum over ranks, a linear layer's tail, or
 // nothing.  (A
 // launch takes longer by about a nanosecond for every four bytes of parameters.)
-struct Nothing {};
 template <int EPI>
-using ExtraOf = std::conditional_t<(EPI & kStaged) != 0, CUtensorMap,
-                                   std::conditional_t<(EPI & kSplit) != 0, PeerParams, std::conditional_t<(EPI & kTail) != 0, Tail, Nothing>>>;
+using ExtraOf = std::conditional_t<
+    (EPI & kStaged) != 0, CUtensorMap,
+    std::conditional_t<(EPI & kSplit) != 0, PeerParams,
+                       std::conditional_t<(EPI & kExperts) != 0, ExpertParams, std::conditional_t<(EPI & kTail) != 0, Tail, Nothing>>>>;
+
+template <bool EXPERTS, class X>
+__device__ __forceinline__ decltype(auto) runs_of(const X& x) {
+  if constexpr (EXPERTS) return (x);
+  else return Nothing{};
+}
+// Zeros for the tokens in no expert's run, dealt out over the CTAs.
+__device__ __forceinline__ void zero_rest_rows(const SpmmParams& p, const ExpertParams& x, int tid, int threads) {
+  const int before = x.bounds[0], behind = x.bounds[x.n_experts], rest = before + p.N - behind;
+  for (int i = blockIdx.x; i < rest; i += gridDim.x) {
+    const size_t first = (size_t)(i < before ? i : i - before + behind) * (size_t)p.ldc;
+    if (p.out_dtype == VOID_OUT_F32)
+      for (int c = tid; c < p.M; c += threads) reinterpret_cast<float*>(p.out)[first + c] = 0.0f;
+    else
+      for (int c = tid; c < p.M; c += threads) reinterpret_cast<uint16_t*>(p.out)[first + c] = 0;
+  }
+}
 
 // TR: 1 = B and C transposed ([N, K] and [N, M]), 2 = C alone.  EPI: what the epilogue is asked for (kStaged ...).  What is not run
 // costs a little too, in spilled registers and in instructions fetched around it: INT8 4096^2, 90 %, N = 512, fp16 results 6.10 us,
@@ -38,9 +56,12 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) spmm_rowacc_kernel
                                                                                  const __grid_constant__ ExtraOf<EPI> x,
                                                                                  const __grid_constant__ SpmmParams p) {
   constexpr bool STAGED = (EPI & kStaged) != 0, SPLIT = (EPI & kSplit) != 0, ACT = (EPI & kActive) != 0, TRACE = (EPI & kTraced) != 0;
-  constexpr bool TAIL = (EPI & kTail) != 0;
+  constexpr bool TAIL = (EPI & kTail) != 0, EXPERTS = (EPI & kExperts) != 0;
+  // (what the roles are told about experts; the others read nothing of it)
+  using Runs = std::conditional_t<EXPERTS, ExpertParams, Nothing>;
   static_assert(!TR || (!STAGED && !SPLIT), "transposed results are stored directly, of whole rows");
   static_assert(!TAIL || (TR && ACT), "linear layers only");
+  static_assert(!EXPERTS || (TR == 1 && TAIL), "tokens as they lie");
   static_assert(!STAGED || C::COLS == kTile, "an epilogue warp stages whole columns of a tile row");
   extern __shared__ uint8_t smem_raw[];
   __shared__ PipeBars bars;
@@ -59,13 +80,14 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) spmm_rowacc_kernel
   uint32_t tmem_cols = 32;
   while (tmem_cols < 2u * acc_cols) tmem_cols <<= 1;
   volatile int* ctl = ctl_s;
+  const Runs& runs = runs_of<EXPERTS>(x);
 
   if (threadIdx.x == 0) last_s = 0;
   pipeline_setup<C, ES, TRACE>(p, &tmap_b, bars, &tmem_base_s, ctl_s, 2, tmem_cols);
   const uint32_t tmem_base = tmem_base_s;
 
   if (warp < C::PW) {
-    producer_loop<C, ES, TR, SPLIT, TRACE>(p, &tmap_b, &bars, ring_base, stage_bytes, ctl, lane, warp);
+    producer_loop<C, ES, TR, SPLIT, TRACE, Runs>(p, &tmap_b, &bars, ring_base, stage_bytes, ctl, lane, warp, runs);
     if (warp == 0 && lane == 0) stamp<TRACE>(p, 2);
   } else if (warp == C::MMA) {
     {
@@ -86,18 +108,18 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) spmm_rowacc_kernel
       // (transposed B: the panel is K-major, 32 bytes of k lie inside one row of its swizzle atom)
       constexpr uint64_t kPanelKStep = TR == 1 ? 2 : ((kPanelBytes / ES) >> 4), kTileKStep = 256 >> 4;
       int begin, end, step;
-      seg_range<SPLIT>(p, begin, end, step);
+      seg_range<SPLIT>(p, begin, end, step, runs);
       int stage = 0;
       uint32_t phase = 0;
       uint32_t sbase = ring_base;
       uint32_t it = 0;
       bool ok = true;
       Seg seg_next = {};  // the next segment's descriptor is fetched one item ahead
-      if (begin < end) seg_next = load_seg<SPLIT>(p, begin);
+      if (begin < end) seg_next = load_seg<SPLIT>(p, begin, runs);
       for (int i = begin; i < end && ok; i += step, ++it) {
         const Seg s = seg_next;
-        if (i + step < end) seg_next = load_seg<SPLIT>(p, i + step);
-        const int npan = panels_in_chunk(p, s.chunk);
+        if (i + step < end) seg_next = load_seg<SPLIT>(p, i + step, runs);
+        const int npan = panels_of<Runs>(p, s);
         const uint32_t buf = it & 1u, aph = (it >> 1) & 1u;
         ok = mbar_wait_warp(smem_u32(&bars.acc_empty[buf]), aph ^ 1u, ctl);
         if (!ok) break;
@@ -163,25 +185,28 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) spmm_rowacc_kernel
     // of A may be read ahead of it when the caller vouches for A
     if (!p.a_stable) grid_dependency_wait();
     int begin, end, step;
-    seg_range<SPLIT>(p, begin, end, step);
+    seg_range<SPLIT>(p, begin, end, step, runs);
     uint32_t it = 0;
     int seg_next = 0;  // the next segment's descriptor is fetched one item ahead, a word per lane
-    if (begin < end) seg_next = load_seg_word<SPLIT>(p, begin, lane);
+    if (begin < end) seg_next = load_seg_word<SPLIT>(p, begin, lane, runs);
     if (p.a_stable) grid_dependency_wait();
+    if constexpr (EXPERTS)
+      if (x.zero_rest) zero_rest_rows(p, x, epi_tid, C::EPI_THREADS);
     if (epi_tid == 0) stamp<TRACE>(p, 0);
     for (int i = begin; i < end; i += step, ++it) {
       const int seg = seg_next;
-      if (i + step < end) seg_next = load_seg_word<SPLIT>(p, i + step, lane);
+      if (i + step < end) seg_next = load_seg_word<SPLIT>(p, i + step, lane, runs);
       const int row = word_of(seg, 0), chunk = word_of(seg, 1), nseg = SPLIT ? word_of(seg, 4) : 1;
-      const int npan = panels_in_chunk(p, chunk);
+      const int n_first = EXPERTS ? word_of(seg, 4) : chunk * p.np * kPanelN, n_end = EXPERTS ? word_of(seg, 5) : p.N;
+      const int npan = EXPERTS ? (n_end - n_first + kPanelN - 1) / kPanelN : panels_in_chunk(p, chunk);
       const uint32_t buf = it & 1u, aph = (it >> 1) & 1u;
       const bool has = word_of(seg, 3) > word_of(seg, 2);
       // an empty tile row is zeros (+ bias): nothing to scale, no scales to wait for
       const float rs = (p.row_scale != nullptr && (has || nseg > 1)) ? p.row_scale[row] : 1.0f;
-      const int n_base = chunk * p.np * kPanelN + quad * 32 + lane;
+      const int n_base = n_first + quad * 32 + lane;
       // per-column scale and bias of the first panel are fetched before the accumulator is ready
       float cs = p.b_scale, bias = 0.0f;
-      if (n_base < p.N) {
+      if (n_base < n_end) {
         if (p.col_scale != nullptr && (has || nseg > 1)) cs = p.col_scale[n_base] * p.b_scale;
         if (p.bias != nullptr) bias = p.bias[n_base];
       }
@@ -307,7 +332,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) spmm_rowacc_kernel
         float csq = cs, biasq = bias;   // the first panel's were read before the accumulator was ready
         if (q > 0) {
           csq = p.b_scale; biasq = 0.0f;
-          if (n < p.N) {
+          if (n < n_end) {
             if (p.col_scale != nullptr) csq = p.col_scale[n] * p.b_scale;
             if (p.bias != nullptr) biasq = p.bias[n];
           }
@@ -365,6 +390,10 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) spmm_rowacc_kernel
         } else {
           uint32_t r[C::COLS];
           OutDesc to = od;
+          if constexpr (EXPERTS) {
+            to.N = n_end;
+            if (to.row_bias != nullptr) to.row_bias += (size_t)word_of(seg, 6) * (size_t)p.M;
+          }
           if (!whole) {
             int32_t* sums = row_sums(p, x, seg, peers, q) + m_first * kPanelN + quad * 32;
 #pragma unroll
@@ -392,7 +421,8 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) spmm_rowacc_kernel
           }
 #pragma unroll
           for (int c = 0; c < C::COLS; c += 16) {
-            if constexpr (TAIL) finish16_tail<KIND>(to, x, row, n, m_first + c, &r[c], rs, csq, biasq);
+            if constexpr (EXPERTS) finish16_tail<KIND>(to, x.tail, row, n, m_first + c, &r[c], rs, csq, biasq);
+            else if constexpr (TAIL) finish16_tail<KIND>(to, x, row, n, m_first + c, &r[c], rs, csq, biasq);
             else if (TR) finish16_tr<KIND, ACT>(to, row, n, m_first + c, &r[c], rs, csq, biasq);
             else finish16<KIND, ACT>(to, row, n, m_first + c, &r[c], rs, csq, biasq);
           }
@@ -457,6 +487,13 @@ int launch_rowacc(const RowaccLaunch& l) {
   if constexpr (KIND == VOID_KIND_F16 || KIND == VOID_KIND_TF32)
     if (l.shape == 6) return launch_rowacc<KIND, Mid>(l);
   return l.shape == 2 ? launch_rowacc<KIND, Slim>(l) : launch_rowacc<KIND, Wide>(l);
+}
+
+template <int KIND>
+int launch_experts(const ExpertLaunch& l) {
+  auto kernel = spmm_rowacc_kernel<KIND, Mid, 1, kActive | kTail | kExperts>;
+  if (ensure_smem((const void*)kernel, l.smem_bytes)) return VOID_ERR_CUDA;
+  return status_of(launch_pdl(kernel, l.grid, Mid::THREADS, l.smem_bytes, l.stream, l.b, l.x, l.p));
 }
 
 }  // namespace vb

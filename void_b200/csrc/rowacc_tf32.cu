@@ -4,5 +4,6 @@
 namespace vb {
 
 template int launch_rowacc<VOID_KIND_TF32>(const RowaccLaunch&);
+template int launch_experts<VOID_KIND_TF32>(const ExpertLaunch&);
 
 }  // namespace vb

@@ -182,9 +182,14 @@ __device__ __forceinline__ void store_value(void* p, int dtype, long long at, fl
   else reinterpret_cast<float*>(p)[at] = v;
 }
 
-// ACT: whether there may be an activation or a row bias (the kernel without is 0.2 us faster).  TAIL: a linear layer's tail, too.
-template <int KIND, bool TR, int NG, bool ACT, bool TAIL>
-__global__ void __launch_bounds__(512) skinny_kernel(const __grid_constant__ std::conditional_t<TAIL, SkinnyTailParams, SkinnyParams> p) {
+// ACT: whether there may be an activation or a row bias (the kernel without is 0.2 us faster).
+// MODE: 1 a linear layer's tail, too; 2 that of experts.
+constexpr int kPlain = 0, kWithTail = 1, kOfExperts = 2;
+template <int MODE>
+using ParamsOf = std::conditional_t<MODE == kOfExperts, SkinnyExpertParams, std::conditional_t<MODE == kWithTail, SkinnyTailParams, SkinnyParams>>;
+template <int KIND, bool TR, int NG, bool ACT, int MODE>
+__global__ void __launch_bounds__(512) skinny_kernel(const __grid_constant__ ParamsOf<MODE> p) {
+  constexpr bool TAIL = MODE != kPlain, EXPERTS = MODE == kOfExperts;
   constexpr int ES = Elem<KIND>::ES, NB = 8 * NG;
   using T = typename AccType<KIND>::T;
   extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -192,9 +197,24 @@ __global__ void __launch_bounds__(512) skinny_kernel(const __grid_constant__ std
   constexpr int PITCH = NB + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int g = lane >> 2, t = lane & 3;
-  const int row = blockIdx.x, n0 = blockIdx.y * NB;
+  const int row = blockIdx.x;
   if (!p.a_stable) grid_dependency_wait();
-  const int t0 = p.row_ptr[row], t1 = p.row_ptr[row + 1];
+  int n0 = blockIdx.y * NB, n_end = p.N, packed_row = row;
+  const float* row_bias = p.row_bias;
+  if constexpr (EXPERTS) {
+    if (p.zero_rest) {   // zeros for the tokens in no expert's run: this tile row's columns, the tokens dealt out over the slots
+      const int before = p.bounds[0], behind = p.bounds[p.n_experts], rest = before + p.N - behind;
+      for (int i = (int)blockIdx.y + (int)gridDim.y * warp; i < rest; i += (int)gridDim.y * warps)
+        if (row * 32 + lane < p.M) store_value(p.out, p.out_dtype, (long long)(i < before ? i : i - before + behind) * p.ldc + row * 32 + lane, 0.0f);
+    }
+    if ((int)blockIdx.y >= p.head[0]) return;
+    const int4 c = p.chunks[blockIdx.y];
+    n0 = c.y;
+    n_end = c.z;
+    packed_row += c.x * (int)gridDim.x;
+    if (row_bias != nullptr) row_bias += (size_t)c.x * (size_t)p.M;
+  }
+  const int t0 = p.row_ptr[packed_row], t1 = p.row_ptr[packed_row + 1];
   T d[2][NG][4];
 #pragma unroll
   for (int h = 0; h < 2; ++h)
@@ -221,7 +241,7 @@ __global__ void __launch_bounds__(512) skinny_kernel(const __grid_constant__ std
 #pragma unroll
       for (int i = 0; i < NG; ++i) {
         const int n = n0 + 8 * i + g;
-        load_b_tr<ES>(b + (long long)n * p.ldb, k0, p.K, t, n < p.N, bw[i]);
+        load_b_tr<ES>(b + (long long)n * p.ldb, k0, p.K, t, n < n_end, bw[i]);
       }
     } else {
       load_b<ES, NG>(b, p.ldb, k0, p.K, n0 + NG * g, p.N, t, bw);
@@ -248,13 +268,13 @@ __global__ void __launch_bounds__(512) skinny_kernel(const __grid_constant__ std
     x.c = TR ? (o >> 5) : o % NB;
     x.n = n0 + x.c;
     x.r = row * 32 + x.m;
-    x.in = x.n < p.N && x.r < p.M;
+    x.in = x.n < n_end && x.r < p.M;
     x.cs = p.b_scale;
     x.bias = x.row_bias = x.residual = 0.0f;
     if (x.in) {
       if (p.col_scale != nullptr) x.cs *= p.col_scale[x.n];
       if (p.bias != nullptr) x.bias = p.bias[x.n];
-      if (ACT && p.row_bias != nullptr) x.row_bias = p.row_bias[x.r];
+      if (ACT && row_bias != nullptr) x.row_bias = row_bias[x.r];
       if constexpr (TAIL)
         if (p.tail.residual != nullptr) x.residual = load_value(p.tail.residual, p.tail.residual_dtype, (long long)x.n * p.tail.ldr + x.r);
     }
@@ -278,7 +298,7 @@ __global__ void __launch_bounds__(512) skinny_kernel(const __grid_constant__ std
         mine[m * PITCH + (TR ? 8 * i + j : NG * j + i)] = d[h][i][e];
       }
   __syncthreads();
-  const float rs = p.row_scale != nullptr && t1 > t0 ? p.row_scale[row] : 1.0f;
+  const float rs = p.row_scale != nullptr && t1 > t0 ? p.row_scale[packed_row] : 1.0f;
   for (int o = threadIdx.x; o < 32 * NB; o += blockDim.x) {
     if (!ACT || o >= (int)blockDim.x) x = output(o);
     if (!x.in) continue;
@@ -298,19 +318,20 @@ __global__ void __launch_bounds__(512) skinny_kernel(const __grid_constant__ std
   }
 }
 
-template <int KIND, bool TR, int NG, bool ACT, bool TAIL>
-cudaError_t launch(const SkinnyTailParams& p, int nbr, int warps, cudaStream_t st) {
-  auto kernel = skinny_kernel<KIND, TR, NG, ACT, TAIL>;
+template <int KIND, bool TR, int NG, bool ACT, int MODE>
+cudaError_t launch(const ParamsOf<MODE>& p, int nbr, int slots, int warps, cudaStream_t st) {
+  auto kernel = skinny_kernel<KIND, TR, NG, ACT, MODE>;
   const int smem = warps * 32 * (8 * NG + 1) * 4;
   if (smem > 48 * 1024 && ensure_smem((const void*)kernel, smem)) return cudaErrorInvalidValue;
-  return launch_pdl(kernel, dim3((unsigned)nbr, (unsigned)((p.N + 8 * NG - 1) / (8 * NG))), 32 * warps, smem, st, p);
+  return launch_pdl(kernel, dim3((unsigned)nbr, (unsigned)slots), 32 * warps, smem, st, p);
 }
 template <int KIND, bool TR, int NG>
 cudaError_t launch(const SkinnyTailParams& p, bool tail, int nbr, int warps, cudaStream_t st) {
+  const int slots = (p.N + 8 * NG - 1) / (8 * NG);
   if constexpr (TR)
-    if (tail) return launch<KIND, TR, NG, true, true>(p, nbr, warps, st);
-  return p.act != VOID_ACT_NONE || p.row_bias != nullptr ? launch<KIND, TR, NG, true, false>(p, nbr, warps, st)
-                                                         : launch<KIND, TR, NG, false, false>(p, nbr, warps, st);
+    if (tail) return launch<KIND, TR, NG, true, kWithTail>(p, nbr, slots, warps, st);
+  return p.act != VOID_ACT_NONE || p.row_bias != nullptr ? launch<KIND, TR, NG, true, kPlain>(p, nbr, slots, warps, st)
+                                                         : launch<KIND, TR, NG, false, kPlain>(p, nbr, slots, warps, st);
 }
 template <int KIND, bool TR>
 cudaError_t launch_columns(const SkinnyTailParams& p, bool tail, int nbr, int warps, cudaStream_t st) {
@@ -320,12 +341,31 @@ cudaError_t launch_columns(const SkinnyTailParams& p, bool tail, int nbr, int wa
   return launch<KIND, TR, 4>(p, tail, nbr, warps, st);
 }
 
+// Enough warps that a warp has a few tiles of its row, so that their loads are in flight together.
+int row_warps(long long tiles) { return tiles >= 24 ? 16 : (tiles >= 6 ? 8 : 4); }
+
+template <int KIND>
+cudaError_t launch_experts(const SkinnyExpertParams& p, int nbr, int slots, int chunk, int warps, cudaStream_t st) {
+  if (chunk == 8) return launch<KIND, true, 1, true, kOfExperts>(p, nbr, slots, warps, st);
+  if (chunk == 16) return launch<KIND, true, 2, true, kOfExperts>(p, nbr, slots, warps, st);
+  return chunk == 32 ? launch<KIND, true, 4, true, kOfExperts>(p, nbr, slots, warps, st) : cudaErrorInvalidValue;
+}
+
 }  // namespace
 
+// nnz_row: stored tiles of a tile row, on average; slots: chunks there can be at most.
+cudaError_t skinny_experts_launch(const SkinnyExpertParams& p, int kind, int nbr, long long nnz_row, int chunk, int slots, cudaStream_t st) {
+  const int warps = row_warps(nnz_row);
+  switch (kind) {
+    case VOID_KIND_F16: return launch_experts<VOID_KIND_F16>(p, nbr, slots, chunk, warps, st);
+    case VOID_KIND_BF16: return launch_experts<VOID_KIND_BF16>(p, nbr, slots, chunk, warps, st);
+    case VOID_KIND_TF32: return launch_experts<VOID_KIND_TF32>(p, nbr, slots, chunk, warps, st);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
 cudaError_t skinny_launch(const SkinnyTailParams& p, int kind, bool transposed, bool tail, int nbr, long long nnz, cudaStream_t st) {
-  // enough warps that a warp has a few tiles of its row, so that their loads are in flight together
-  const long long avg = nbr > 0 ? nnz / nbr : 0;
-  const int warps = avg >= 24 ? 16 : (avg >= 6 ? 8 : 4);
+  const int warps = row_warps(nbr > 0 ? nnz / nbr : 0);
 #define VB_COLUMNS(KIND) (transposed ? launch_columns<KIND, true>(p, tail, nbr, warps, st) : launch_columns<KIND, false>(p, tail, nbr, warps, st))
   switch (kind) {
     case VOID_KIND_I8: return VB_COLUMNS(VOID_KIND_I8);

@@ -23,13 +23,20 @@
 // tiles' blocks stand side by side along M, and an MMA takes 1024 bytes further along n each time.  It replaces two
 // transposed copies of 8 MB at 4096^2, N = 512 fp32 (20 us).
 //
+// Experts (RUNS): n are the tokens of the tile row's expert, [bounds[e], bounds[e + 1]) of the whole batch.  The last slice may reach
+// into the next expert's tokens: its rows behind the end are overwritten with zeros in shared memory, in both operands (what stands
+// there may be infinite), by the warp that issues the MMAs.
+//
 // Work items (tile row, first tile, tile count <= 4) come from the caller (they depend on A's
 // structure only).  Every wait is bounded like in the SpMM kernels.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cudaTypedefs.h>
 
+#include <type_traits>
+
 #include "../../include/void_b200.h"
+#include "experts.cuh"
 #include "kinds.cuh"
 #include "launch.cuh"
 #include "ptx.cuh"
@@ -57,6 +64,21 @@ struct GradParams {
   unsigned long long desc_hi;
   unsigned int idesc;
 };
+struct RunParams {
+  const int32_t* bounds;   // [experts + 1]
+  int rows;                // tile rows of an expert
+};
+struct NoRuns {};
+// Tokens of a tile row: first, number; and the tile row within its expert.
+template <bool RUNS, class R>
+__device__ __forceinline__ int3 run_of(const GradParams& p, const R& r, int row) {
+  if constexpr (RUNS) {
+    const int e = row / r.rows, lo = r.bounds[e];
+    return make_int3(lo, r.bounds[e + 1] - lo, row - e * r.rows);
+  } else {
+    return make_int3(0, p.n_slices * p.slice_elems, row);
+  }
+}
 
 struct __align__(8) Bars {
   uint64_t full[kMaxBars];
@@ -65,10 +87,12 @@ struct __align__(8) Bars {
   uint64_t acc_empty[2];
 };
 
-template <int KIND, bool MN>
+template <int KIND, bool MN, bool RUNS>
 __global__ void __launch_bounds__(kThreads, 2) tile_grad_kernel(const __grid_constant__ CUtensorMap tmap_b,
                                                                 const __grid_constant__ CUtensorMap tmap_g,
+                                                                const __grid_constant__ std::conditional_t<RUNS, RunParams, NoRuns> runs,
                                                                 const __grid_constant__ GradParams p) {
+  static_assert(!RUNS || MN, "runs of tokens are rows");
   extern __shared__ uint8_t smem_raw[];
   __shared__ Bars bars;
   __shared__ uint32_t tmem_base_s;
@@ -110,12 +134,14 @@ __global__ void __launch_bounds__(kThreads, 2) tile_grad_kernel(const __grid_con
     bool alive = true;
     for (int i = blockIdx.x; i < p.n_items && alive; i += gridDim.x) {
       const int4 it = __ldg(reinterpret_cast<const int4*>(p.items) + i);
-      const int row = it.x, t0 = it.y, cnt = it.z;
+      const int t0 = it.y, cnt = it.z;
+      const int3 run = run_of<RUNS>(p, runs, it.x);
+      const int n_slices = RUNS ? (run.y + p.slice_elems - 1) / p.slice_elems : p.n_slices;
       int y = 0;
       if (lane < cnt) y = __ldg(p.tile_cols + t0 + lane) * kTile;
-      if (lane == 4) y = row * kTile;
+      if (lane == 4) y = run.z * kTile;
       const bool mine = lane < cnt || lane == 4;
-      for (int s = 0; s < p.n_slices; ++s, ++g) {
+      for (int s = 0; s < n_slices; ++s, ++g) {
         const int stage = (int)(g % kStages);
         const uint32_t phase = (g / kStages) & 1u;
         const uint32_t full = smem_u32(&bars.full[stage]);
@@ -126,7 +152,7 @@ __global__ void __launch_bounds__(kThreads, 2) tile_grad_kernel(const __grid_con
         __syncwarp();
         if (mine)
           tma_load_2d(base + (uint32_t)lane * kBlockBytes, lane == 4 ? &tmap_g : &tmap_b, MN ? y : s * p.slice_elems,
-                      MN ? s * p.slice_elems : y, full);
+                      MN ? run.x + s * p.slice_elems : y, full);
       }
     }
   } else if (warp == 1) {
@@ -145,13 +171,32 @@ __global__ void __launch_bounds__(kThreads, 2) tile_grad_kernel(const __grid_con
         tc_fence_after();
         const uint32_t d = tmem_base + buf * 32u;
         uint32_t acc = 0u;
-        for (int s = 0; s < p.n_slices; ++s, ++g) {
+        int n_slices = p.n_slices, left = 0, blocks = 0;   // tokens and row blocks
+        if constexpr (RUNS) {
+          const int4 it = __ldg(reinterpret_cast<const int4*>(p.items) + i);
+          left = run_of<RUNS>(p, runs, it.x).y;
+          blocks = it.z;
+          n_slices = (left + p.slice_elems - 1) / p.slice_elems;
+        }
+        for (int s = 0; s < n_slices; ++s, ++g) {
           const int stage = (int)(g % kStages);
           const uint32_t phase = (g / kStages) & 1u;
           ok = mbar_wait_warp(smem_u32(&bars.full[stage]), phase, abort_flag);
           if (!ok) break;
           tc_fence_after();
           const uint32_t base = ring + (uint32_t)stage * kStageBytes;
+          if constexpr (RUNS) {
+            if (left < p.slice_elems) {
+              const int from = left * (kBlockBytes / p.slice_elems);   // a token's row of a block
+              for (int b = 0; b <= blocks; ++b) {
+                uint8_t* block = smem_raw + (base - smem_u32(smem_raw)) + (b < blocks ? b : 4) * kBlockBytes;
+                for (int o = from + lane * 16; o < kBlockBytes; o += 32 * 16) *reinterpret_cast<uint4*>(block + o) = make_uint4(0u, 0u, 0u, 0u);
+              }
+              fence_proxy_async_smem();
+              __syncwarp();
+            }
+            left -= p.slice_elems;
+          }
           const uint64_t ad = smem_desc(hi, base), bd = smem_desc(hi, base + 4u * kBlockBytes);
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) {  // 32 bytes of n per MMA (inside the swizzle atom), or 1024 bytes of its rows
@@ -163,7 +208,7 @@ __global__ void __launch_bounds__(kThreads, 2) tile_grad_kernel(const __grid_con
         }
         if (!ok) break;
         if (leader) {
-          if (p.n_slices > 0) tc_commit(smem_u32(&bars.acc_full[buf]));
+          if (n_slices > 0) tc_commit(smem_u32(&bars.acc_full[buf]));
           else mbar_arrive(smem_u32(&bars.acc_full[buf]));
         }
       }
@@ -180,10 +225,11 @@ __global__ void __launch_bounds__(kThreads, 2) tile_grad_kernel(const __grid_con
       const uint32_t buf = n & 1u, aph = (n >> 1) & 1u;
       long long orig = 0;
       if (j < cnt) orig = __ldg(p.block_indices + t0 + j);
+      const bool any = run_of<RUNS>(p, runs, it.x).y > 0;
       if (!mbar_wait_warp(smem_u32(&bars.acc_full[buf]), aph, abort_flag)) break;
       tc_fence_after();
       uint32_t r[32];
-      if (j < cnt && p.n_slices > 0) {
+      if (j < cnt && any) {
         tmem_ld_32x32(tmem_base + lane_sel + buf * 32u, r);
         tmem_ld_wait();
       } else {
@@ -241,19 +287,19 @@ static bool row_block_map(CUtensorMap* m, const void* base, int64_t ld_bytes, in
              CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int KIND, bool MN>
-static int launch(const GradParams& p, const CUtensorMap& map_b, const CUtensorMap& map_g, int sms, cudaStream_t st) {
-  auto kernel = tile_grad_kernel<KIND, MN>;
+template <int KIND, bool MN, bool RUNS, class R>
+static int launch(const GradParams& p, const R& runs, const CUtensorMap& map_b, const CUtensorMap& map_g, int sms, cudaStream_t st) {
+  auto kernel = tile_grad_kernel<KIND, MN, RUNS>;
   const int smem = kStages * kStageBytes + 1024;
   if (ensure_smem((const void*)kernel, smem)) return VOID_ERR_CUDA;
   int grid = 2 * sms;
   if (grid > p.n_items) grid = p.n_items;
-  return status_of(launch_kernel(false, kernel, grid, kThreads, smem, st, map_b, map_g, p));
+  return status_of(launch_kernel(false, kernel, grid, kThreads, smem, st, map_b, map_g, runs, p));
 }
 
 static int tile_grad(const void* grad_out, int64_t ldg, const void* b, int64_t ldb, int M, int K, int N, int kind,
                      const int32_t* items, int n_items, const int32_t* tile_cols, const int32_t* block_indices,
-                     void* grad_tiles, int out_dtype, int32_t* status, cudaStream_t st, bool mn) {
+                     void* grad_tiles, int out_dtype, int32_t* status, cudaStream_t st, bool mn, const RunParams* runs = nullptr) {
   if (M < 0 || K < 0 || N < 0 || n_items < 0) return VOID_ERR_BAD_ARG;
   if (kind != VOID_KIND_TF32 && kind != VOID_KIND_F16 && kind != VOID_KIND_BF16) return VOID_ERR_BAD_ARG;
   if (out_dtype < VOID_OUT_F32 || out_dtype > VOID_OUT_BF16) return VOID_ERR_BAD_ARG;
@@ -293,8 +339,13 @@ static int tile_grad(const void* grad_out, int64_t ldg, const void* b, int64_t l
     if (!row_block_map(&map_b, b, ldb, mn ? N : K, mn ? K : N, es, mn) || !row_block_map(&map_g, grad_out, ldg, mn ? N : M, mn ? M : N, es, mn))
       return VOID_ERR_TENSOR_MAP;
   }
-  if (kind == VOID_KIND_TF32) return mn ? launch<VOID_KIND_TF32, true>(p, map_b, map_g, dev.sms, st) : launch<VOID_KIND_TF32, false>(p, map_b, map_g, dev.sms, st);
-  return mn ? launch<VOID_KIND_F16, true>(p, map_b, map_g, dev.sms, st) : launch<VOID_KIND_F16, false>(p, map_b, map_g, dev.sms, st);
+  if (runs != nullptr)
+    return kind == VOID_KIND_TF32 ? launch<VOID_KIND_TF32, true, true>(p, *runs, map_b, map_g, dev.sms, st)
+                                  : launch<VOID_KIND_F16, true, true>(p, *runs, map_b, map_g, dev.sms, st);
+  const NoRuns all;
+  if (kind == VOID_KIND_TF32)
+    return mn ? launch<VOID_KIND_TF32, true, false>(p, all, map_b, map_g, dev.sms, st) : launch<VOID_KIND_TF32, false, false>(p, all, map_b, map_g, dev.sms, st);
+  return mn ? launch<VOID_KIND_F16, true, false>(p, all, map_b, map_g, dev.sms, st) : launch<VOID_KIND_F16, false, false>(p, all, map_b, map_g, dev.sms, st);
 }
 
 }  // namespace vbg
@@ -315,6 +366,15 @@ int void_linear_tile_grad(const void* grad_out, int64_t ldg, const void* x, int6
                           void_stream_t stream) {
   return vbg::tile_grad(grad_out, ldg, x, ldx, M, K, N, kind, items, n_items, tile_cols, block_indices, grad_tiles, out_dtype,
                         status, reinterpret_cast<cudaStream_t>(stream), true);
+}
+
+int void_expert_tile_grad(const void* grad_out, int64_t ldg, const void* x, int64_t ldx, int32_t M, int32_t K, int32_t N, int32_t kind,
+                          const void_experts* experts, const int32_t* items, int32_t n_items, const int32_t* tile_cols,
+                          const int32_t* block_indices, void* grad_tiles, int32_t out_dtype, int32_t* status, void_stream_t stream) {
+  if (experts == nullptr || experts->plan == nullptr || experts->n_experts < 1 || M < 1 || N < 1) return VOID_ERR_BAD_ARG;
+  const vbg::RunParams runs = {vb::plan_of(*experts, N).bounds, (M + 31) / 32};
+  return vbg::tile_grad(grad_out, ldg, x, ldx, M, K, N, kind, items, n_items, tile_cols, block_indices, grad_tiles, out_dtype, status,
+                        reinterpret_cast<cudaStream_t>(stream), true, &runs);
 }
 
 }  // extern "C"
