@@ -88,6 +88,19 @@ def test_forward_and_gradients(rows, cols, dtype, params):
     check(x, w, b, g, y, grads)
 
 
+@pytest.mark.parametrize("dtype, params", TYPES)
+@pytest.mark.parametrize("rows, cols", [(2700, 1032), (2700, 1031), (1800, 5000), (1801, 5001), (900, 9000), (900, 9002), (900, 9001)])
+def test_many_rows(rows, cols, dtype, params):
+    # (rows enough for blocks that walk them, on and off 16-byte pieces)
+    x, w, b, g = make(rows, cols, dtype, params)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    y = void.void_layer_norm(x, w, b)
+    check(x, w, b, g, y, torch.autograd.grad(y, leaves, g))
+    wide = torch.full((rows, cols + 3), float("nan"), device="cuda", dtype=dtype)    # what lies between the rows is not read as theirs
+    wide[:, :cols] = x.detach()
+    check(x, w, b, g, void.void_layer_norm(wide[:, :cols], w, b))
+
+
 @pytest.mark.parametrize("which", ["neither", "weight", "bias"])
 @pytest.mark.parametrize("cols", [100, 104, 20000])
 def test_parameters_may_be_left_out(which, cols):
