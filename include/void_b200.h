@@ -432,7 +432,7 @@ typedef struct void_epilogue {
                               (the same place and pitch): every element is read by the thread that writes it         */
   int64_t ldr;
   int32_t residual_dtype;  /* VOID_OUT_F32, or args->out_dtype                                                       */
-  int32_t reserved;
+  int32_t bias_dtype;      /* what args->row_bias points to: VOID_OUT_F32 (0), VOID_OUT_F16 or VOID_OUT_BF16         */
   void* pre;               /* [N, M] of type args->out_dtype, ldp elements between rows: z, for a backward pass; or NULL */
   int64_t ldp;
 } void_epilogue;

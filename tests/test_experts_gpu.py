@@ -146,6 +146,16 @@ def test_layouts():
     assert void.void_expert_linear(e, x[:0], torch.zeros(4, dtype=torch.int32, device="cuda")).shape == (0, 45)
 
 
+@pytest.mark.parametrize("counts", [[3, 4, 0], [70, 1, 200]])
+def test_biases_in_their_own_type(counts):
+    weights, e = experts_of(3, 45, 70, 0.5, torch.bfloat16)
+    x, offsets = rand(sum(counts), 70, dtype=torch.bfloat16), offsets_of(counts)
+    for t in (torch.float16, torch.bfloat16):
+        bias = rand(3, 45, seed=1, dtype=t)
+        check_forward(void.void_expert_linear(e, x, offsets, bias, 3), weights, x, counts, 0, bias, "silu")
+        check_forward(void.void_expert_linear(e, x, offsets, bias.t().contiguous().t(), 3), weights, x, counts, 0, bias, "silu")
+
+
 def test_weights_without_tiles():
     weights, e = experts_of(2, 64, 96, 0.0, torch.bfloat16)
     for counts in ([3, 4], [100, 80]):

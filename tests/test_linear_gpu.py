@@ -83,6 +83,21 @@ def test_a_weight_without_tiles(n):
     check_layer(void.void_linear(a, x, bias, 3, residual=r), a, x, bias, r, "silu")
 
 
+@pytest.mark.parametrize("n", [3, 100, 700])
+@pytest.mark.parametrize("bias_type", [torch.float16, torch.bfloat16])
+def test_biases_in_their_own_type(n, bias_type):
+    a, x, r = weight(333, 515, 0.3, torch.bfloat16), rand(n, 515, dtype=torch.bfloat16), rand(n, 333, dtype=torch.bfloat16, seed=2)
+    back = weight(515, 333, 0.3, torch.bfloat16, seed=5)
+    bias, bias2 = rand(333, seed=1, dtype=bias_type), rand(515, seed=1, dtype=bias_type)
+    check_layer(void.void_linear(a, x, bias, 2), a, x, bias, None, "gelu")
+    check_layer(void.void_linear(a, x, bias, 2, residual=r), a, x, bias, r, "gelu")
+    check_layer(void.void_linear(a, x, torch.stack([bias, bias], 1)[:, 0], 2), a, x, bias, None, "gelu")
+    odd = torch.empty(334, device="cuda", dtype=bias_type)[1:].copy_(bias)
+    check_layer(void.void_linear(a, x, odd, 2), a, x, bias, None, "gelu")
+    ref, e = feed_forward64(x, None, a, bias.double(), back, bias2.double(), "gelu", torch.bfloat16)
+    within(void.fused_sparse_mlp(x, a, back, "gelu", bias, bias2, residual=x), ref, e)
+
+
 def test_no_tokens():
     a = weight(64, 96, 0.5, torch.float16)
     x, r = torch.empty(0, 96, device="cuda", dtype=torch.float16), torch.empty(0, 64, device="cuda", dtype=torch.float16)

@@ -51,7 +51,7 @@ class SpmmArgs(ctypes.Structure):
 
 class Epilogue(ctypes.Structure):
     """Mirror of ``struct void_epilogue``."""
-    _fields_ = [("residual", c_vp), ("ldr", c_i64), ("residual_dtype", c_i32), ("reserved", c_i32), ("pre", c_vp), ("ldp", c_i64)]
+    _fields_ = [("residual", c_vp), ("ldr", c_i64), ("residual_dtype", c_i32), ("bias_dtype", c_i32), ("pre", c_vp), ("ldp", c_i64)]
 
 
 class Experts(ctypes.Structure):

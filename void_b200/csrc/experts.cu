@@ -108,7 +108,9 @@ int experts_launch(const void_spmm_args* a, const void_epilogue* e, const void_e
   if (a->transposed != 1 || a->scale_mode != VOID_SCALE_ROW_MEAN || a->row_scale != nullptr || a->col_scale != nullptr || a->bias != nullptr ||
       a->segs != nullptr || a->acc_out != nullptr || a->worker_partials != nullptr || a->trace != nullptr || a->n_peers != 0 || a->tile_terms > 1)
     return VOID_ERR_BAD_ARG;
-  if (e != nullptr && (e->residual != nullptr || (e->pre != nullptr && e->ldp < a->M))) return VOID_ERR_BAD_ARG;
+  if (e != nullptr && (e->residual != nullptr || (e->pre != nullptr && e->ldp < a->M) || e->bias_dtype < VOID_OUT_F32 ||
+                       e->bias_dtype > VOID_OUT_BF16))
+    return VOID_ERR_BAD_ARG;
   if ((long long)a->nbr * kTile < a->M || a->ldc < a->M) return VOID_ERR_SHAPE;
   const int es = kind == VOID_KIND_TF32 ? 4 : 2;
   if ((reinterpret_cast<uintptr_t>(a->tiles) & 1023u) != 0 || (reinterpret_cast<uintptr_t>(a->b) & 15u) != 0 || (a->ldb & 15) != 0 ||
@@ -123,6 +125,7 @@ int experts_launch(const void_spmm_args* a, const void_epilogue* e, const void_e
   if (e != nullptr) {
     tail.pre = e->pre;
     tail.ldp = e->ldp;
+    tail.bias_dtype = e->bias_dtype;
   }
   if (few_tokens(x->chunk)) {
     if (v.capacity > 65535) return VOID_ERR_TOO_LARGE;

@@ -534,8 +534,16 @@ GroupStore* group_store(Packed* p, int64_t N, void_stream_t st) {
 struct Tail {
   void_epilogue e = {};
   at::Tensor residual, pre;
-  const void_epilogue* get() const { return e.residual != nullptr || e.pre != nullptr ? &e : nullptr; }
+  const void_epilogue* get() const { return e.residual != nullptr || e.pre != nullptr || e.bias_dtype != VOID_OUT_F32 ? &e : nullptr; }
 };
+// A bias of `count` values as a kernel with a tail reads it, in its own type; kept in `keep`.
+const float* bias_as_it_is(const at::Tensor& bias, c10::Device dev, int64_t count, int32_t* dtype, at::Tensor& keep, const char* what) {
+  const at::ScalarType t = bias.scalar_type();
+  keep = bias.device() == dev && (t == at::kFloat || t == at::kHalf || t == at::kBFloat16) ? bias.contiguous() : bias.to(dev, at::kFloat).contiguous();
+  if (keep.numel() != count) fail(std::string(what) + " must have " + std::to_string(count) + " elements, got " + std::to_string(keep.numel()));
+  *dtype = out_code(keep.scalar_type());
+  return static_cast<const float*>(keep.const_data_ptr());
+}
 // A residual [rows, cols] for a result `out`: of its type or fp32, rows with unit stride; other ones are copied, and so is one that
 // shares memory with `out` and is not the very same matrix.
 void set_residual(Tail& t, const at::Tensor& given, const at::Tensor& out) {
@@ -636,17 +644,21 @@ PyObject* spmm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     bias = fp32_vector(a[7], dev, "bias", N);
     s.bias = bias.const_data_ptr<float>();
   }
+  Tail tail;
   if (!none(a[8])) {
-    row_bias = fp32_vector(a[8], dev, "row bias");
-    if (row_bias.numel() != pk->M)
-      fail("row bias must have " + std::to_string(pk->M) + " elements, got " + std::to_string(row_bias.numel()));
-    s.row_bias = row_bias.const_data_ptr<float>();
+    if (tr && none(a[11])) {   // a linear layer's, in its own type
+      s.row_bias = bias_as_it_is(tensor(a[8], "row bias"), dev, pk->M, &tail.e.bias_dtype, row_bias, "row bias");
+    } else {
+      row_bias = fp32_vector(a[8], dev, "row bias");
+      if (row_bias.numel() != pk->M)
+        fail("row bias must have " + std::to_string(pk->M) + " elements, got " + std::to_string(row_bias.numel()));
+      s.row_bias = row_bias.const_data_ptr<float>();
+    }
   }
   s.out = out.data_ptr();
   s.ldc = out.stride(0);
   s.out_dtype = out_code(out.scalar_type());
   s.act = (int32_t)integer(a[9]);
-  Tail tail;
   if (n == 13 && !none(a[12])) {
     if (!tr || !none(a[11])) fail("a residual goes with linear layers only");
     set_residual(tail, cuda_tensor(a[12], "residual"), out);
@@ -733,11 +745,8 @@ at::Tensor two_layers(Packed* first, Packed* second, const at::Tensor& x, PyObje
     s.ldb = row_pitch(in, es);
     s.N = (int32_t)N;
     s.b_scale = 1.0f;
-    if (!none(given[layer])) {
-      bias[layer] = fp32_vector(given[layer], dev, "bias");
-      if (bias[layer].numel() != p->M) fail("bias must have " + std::to_string(p->M) + " elements, got " + std::to_string(bias[layer].numel()));
-      s.row_bias = bias[layer].const_data_ptr<float>();
-    }
+    Tail tail;
+    if (!none(given[layer])) s.row_bias = bias_as_it_is(tensor(given[layer], "bias"), dev, p->M, &tail.e.bias_dtype, bias[layer], "bias");
     if (layer == 1) out = new_cuda({N, p->M}, x.scalar_type(), dev);
     else out = columns ? pitched(p->M, N, x.scalar_type(), es, dev) : pitched(N, p->M, x.scalar_type(), es, dev);
     s.out = out.data_ptr();
@@ -746,7 +755,6 @@ at::Tensor two_layers(Packed* first, Packed* second, const at::Tensor& x, PyObje
     s.act = layer == 0 ? act : VOID_ACT_NONE;
     s.transposed = columns ? (layer == 0 ? 0 : 2) : 1;
     s.flags = p->stable ? 4 : 0;
-    Tail tail;
     if (layer == 1 && !none(residual)) set_residual(tail, cuda_tensor(residual, "residual"), out);
     launch_product(p, s, st, tail.get());
     in = out;
@@ -1237,11 +1245,8 @@ at::Tensor product_of_values(const Structure& st, bool a_transposed, const at::T
   s.N = (int32_t)N;
   s.b_scale = 1.0f;
   at::Tensor bias;
-  if (row_bias != nullptr) {
-    bias = row_bias->to(dev, at::kFloat).contiguous();
-    if (bias.numel() != M) fail("row bias must have " + std::to_string(M) + " elements, got " + std::to_string(bias.numel()));
-    s.row_bias = bias.const_data_ptr<float>();
-  }
+  Tail tail;
+  if (row_bias != nullptr) s.row_bias = bias_as_it_is(linear ? *row_bias : row_bias->to(at::kFloat), dev, M, &tail.e.bias_dtype, bias, "row bias");
   s.out = out.data_ptr();
   s.ldc = out.stride(0);
   s.M = (int32_t)M;
@@ -1250,14 +1255,13 @@ at::Tensor product_of_values(const Structure& st, bool a_transposed, const at::T
   s.status = st.status.data_ptr<int32_t>();
   s.transposed = copied ? 2 : (linear ? 1 : 0);
   s.act = act;
-  Tail tail;
   if (residual != nullptr) set_residual(tail, *residual, out);
   if (pre != nullptr) {
     *pre = tail.pre = pitched(N, M, out.scalar_type(), (int)out.element_size(), dev);
     tail.e.pre = tail.pre.data_ptr();
     tail.e.ldp = tail.pre.stride(0);
   }
-  if (tail.get() != nullptr && N > 0 && M > 0) check(void_spmm_linear(&s, tail.get(), kind, stream), "void_spmm_linear");
+  if (tail.get() != nullptr && linear && N > 0 && M > 0) check(void_spmm_linear(&s, tail.get(), kind, stream), "void_spmm_linear");
   else check(void_spmm_fp(&s, kind, stream), "void_spmm_fp");
   return out;
 }
@@ -1470,11 +1474,8 @@ PyObject* expert_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   s.scale_mode = VOID_SCALE_ROW_MEAN;
   s.transposed = 1;
   at::Tensor bias, order;
-  if (!none(a[5])) {
-    bias = fp32_vector(a[5], dev, "bias");
-    if (bias.numel() != experts * M) fail("bias must have " + std::to_string(experts) + " x " + std::to_string(M) + " elements");
-    s.row_bias = bias.const_data_ptr<float>();
-  }
+  void_epilogue tail = {};
+  if (!none(a[5])) s.row_bias = bias_as_it_is(tensor(a[5], "bias"), dev, experts * M, &tail.bias_dtype, bias, "the experts' bias");
   s.act = (int32_t)integer(a[6]);
   s.out = out.data_ptr();
   s.ldc = N > 1 ? out.stride(0) : M;
@@ -1487,7 +1488,7 @@ PyObject* expert_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     plan.x.row_order = order.const_data_ptr<int32_t>();
   }
   plan.x.zero_rest = none(a[7]) ? 1 : 0;
-  check(void_expert_linear(&s, nullptr, &plan.x, pk->kind, launch_stream(pk)), "void_expert_linear");
+  check(void_expert_linear(&s, &tail, &plan.x, pk->kind, launch_stream(pk)), "void_expert_linear");
   if (!none(a[7])) {
     Py_INCREF(a[7]);
     return a[7];
@@ -1526,11 +1527,8 @@ at::Tensor expert_product(const Structure& st, bool a_transposed, const at::Tens
   s.M = (int32_t)M;
   s.b_scale = 1.0f;
   at::Tensor shift;
-  if (bias != nullptr) {
-    shift = bias->to(dev, at::kFloat).contiguous();
-    if (shift.numel() != st.experts * M) fail("bias must have " + std::to_string(st.experts) + " x " + std::to_string(M) + " elements");
-    s.row_bias = shift.const_data_ptr<float>();
-  }
+  void_epilogue tail = {};
+  if (bias != nullptr) s.row_bias = bias_as_it_is(*bias, dev, st.experts * M, &tail.bias_dtype, shift, "the experts' bias");
   s.act = act;
   s.out = out.data_ptr();
   s.ldc = M;
@@ -1541,13 +1539,12 @@ at::Tensor expert_product(const Structure& st, bool a_transposed, const at::Tens
   void_experts e = plan.x;
   e.zero_rest = 1;
   if (st.row_order[way].defined()) e.row_order = st.row_order[way].const_data_ptr<int32_t>();
-  void_epilogue tail = {};
   if (pre != nullptr) {
     *pre = pitched(N, M, out.scalar_type(), (int)out.element_size(), dev);
     tail.pre = pre->data_ptr();
     tail.ldp = pre->stride(0);
   }
-  check(void_expert_linear(&s, pre != nullptr ? &tail : nullptr, &e, kind, stream), "void_expert_linear");
+  check(void_expert_linear(&s, &tail, &e, kind, stream), "void_expert_linear");
   return out;
 }
 struct ExpertBackward : torch::autograd::Node {

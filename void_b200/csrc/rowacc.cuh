@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) spmm_rowacc_kernel
           OutDesc to = od;
           if constexpr (EXPERTS) {
             to.N = n_end;
-            if (to.row_bias != nullptr) to.row_bias += (size_t)word_of(seg, 6) * (size_t)p.M;
+            if (to.row_bias != nullptr) to.row_bias = bias_of_expert(to.row_bias, x.tail.bias_dtype, word_of(seg, 6), p.M);
           }
           if (!whole) {
             int32_t* sums = row_sums(p, x, seg, peers, q) + m_first * kPanelN + quad * 32;

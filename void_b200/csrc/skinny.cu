@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(512) skinny_kernel(const __grid_constant__ Par
     n0 = c.y;
     n_end = c.z;
     packed_row += c.x * (int)gridDim.x;
-    if (row_bias != nullptr) row_bias += (size_t)c.x * (size_t)p.M;
+    if (row_bias != nullptr) row_bias = bias_of_expert(row_bias, p.tail.bias_dtype, c.x, p.M);
   }
   const int t0 = p.row_ptr[packed_row], t1 = p.row_ptr[packed_row + 1];
   T d[2][NG][4];
@@ -274,7 +274,11 @@ __global__ void __launch_bounds__(512) skinny_kernel(const __grid_constant__ Par
     if (x.in) {
       if (p.col_scale != nullptr) x.cs *= p.col_scale[x.n];
       if (p.bias != nullptr) x.bias = p.bias[x.n];
-      if (ACT && row_bias != nullptr) x.row_bias = row_bias[x.r];
+      if constexpr (TAIL) {
+        if (row_bias != nullptr) x.row_bias = load_value(row_bias, p.tail.bias_dtype, x.r);
+      } else if (ACT && row_bias != nullptr) {
+        x.row_bias = row_bias[x.r];
+      }
       if constexpr (TAIL)
         if (p.tail.residual != nullptr) x.residual = load_value(p.tail.residual, p.tail.residual_dtype, (long long)x.n * p.tail.ldr + x.r);
     }

@@ -628,12 +628,14 @@ int make_tail(const void_spmm_args* a, const void_epilogue* e, Tail* t) {
   if (a == nullptr || e == nullptr) return VOID_ERR_BAD_ARG;
   if (a->transposed != 1 && a->transposed != 2) return VOID_ERR_BAD_ARG;
   if (e->residual != nullptr && e->residual_dtype != VOID_OUT_F32 && e->residual_dtype != a->out_dtype) return VOID_ERR_BAD_ARG;
+  if (e->bias_dtype < VOID_OUT_F32 || e->bias_dtype > VOID_OUT_BF16) return VOID_ERR_BAD_ARG;
   if ((e->residual != nullptr && e->ldr < a->M) || (e->pre != nullptr && e->ldp < a->M)) return VOID_ERR_SHAPE;
   t->residual = e->residual;
   t->pre = e->pre;
   t->ldr = e->ldr;
   t->ldp = e->ldp;
   t->residual_dtype = e->residual_dtype;
+  t->bias_dtype = e->bias_dtype;
   return VOID_OK;
 }
 
