@@ -405,7 +405,7 @@ typedef struct void_spmm_args {
  *   128-byte aligned), ws [2 * n_groups + nnz]; row_order as in void_spmm_args (rows are dealt to the groups in that order
  *   back and forth), or NULL; n_groups * 16 >= nbr and ceil(nbr / n_groups) <= 8; max_tiles <= 32; max_entries <= 6.
  * void_spmm_grouped multiplies it: args as for void_spmm_i8 / _fp (tiles, tile_cols and tile_scales are not read; no
- * plan, no raw accumulators); args->transposed 0 or 2.
+ * plan, no raw accumulators).
  * ------------------------------------------------------------------------------------- */
 #define VOID_GROUP_HEAD_BYTES 32
 typedef struct void_group_store {
@@ -425,7 +425,7 @@ VOID_API int void_spmm_grouped(const void_spmm_args* args, const void_group_stor
  * Linear layers with more in the epilogue (no counterpart in the reference, whose fused products end with the activation):
  *     z = x A^T + bias        out = act(z) + residual
  * args as for void_spmm_fp / void_spmm_i8 with transposed = 1 or 2 (kind VOID_KIND_I8, _F16, _BF16 or _TF32; no plan, no raw
- * accumulators), or as for void_spmm_grouped with transposed = 2.
+ * accumulators), or as for void_spmm_grouped with these.
  * ------------------------------------------------------------------------------------- */
 typedef struct void_epilogue {
   const void* residual;    /* [N, M], ldr elements between rows, added behind the activation; or NULL.  May be `out`

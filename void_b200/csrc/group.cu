@@ -85,8 +85,8 @@ struct __align__(8) Bars {
   uint64_t acc_full[2][kClasses], acc_empty[2][kClasses];
 };
 
-// TAIL: results [N, M] of a linear layer with a tail.
-template <int KIND, bool TAIL>
+// TRB: B stored transposed, [N, K], and C with it: tokens as they lie.  TAIL: results [N, M] of a linear layer with a tail.
+template <int KIND, bool TRB, bool TAIL>
 __global__ void __launch_bounds__(kThreads, kCtas) group_kernel(const __grid_constant__ CUtensorMap tmap_b,
                                                             const __grid_constant__ std::conditional_t<TAIL, Tail, NoTail> tail,
                                                             const __grid_constant__ GroupParams p) {
@@ -168,7 +168,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) group_kernel(const __grid_con
         }
         if (lane < entries) {
           const uint32_t dst = base + (uint32_t)lane * (kPanelBytes * ES);
-          if (p.use3d) tma_load_3d(dst, &tmap_b, 0, col * kTile, chunk * ES, full);
+          if (TRB) tma_load_2d(dst, &tmap_b, col * kTile, chunk * kPanelN, full);
+          else if (p.use3d) tma_load_3d(dst, &tmap_b, 0, col * kTile, chunk * ES, full);
           else
             for (int q = 0; q < ES; ++q)
               tma_load_2d(dst + (uint32_t)q * kPanelBytes, &tmap_b, chunk * kPanelN + q * (kPanelN / ES), col * kTile, full);
@@ -189,7 +190,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) group_kernel(const __grid_con
     const uint4* heads = reinterpret_cast<const uint4*>(p.blob + tiles * (size_t)(kTileBytes * ES)) + (size_t)cls * tiles;
     const uint32_t idesc = p.idesc;
     constexpr uint32_t kTileStep = (kTileBytes * ES) >> 4, kPanelStep = (kPanelBytes * ES) >> 4;
-    constexpr uint32_t kPanelKStep = (kPanelBytes / ES) >> 4, kTileKStep = 256 >> 4;
+    constexpr uint32_t kPanelKStep = TRB ? 2 : (kPanelBytes / ES) >> 4, kTileKStep = 256 >> 4;   // (as in rowacc.cuh)
     const uint32_t a_hi = (uint32_t)(p.desc_hi_a >> 32), b_hi = (uint32_t)(p.desc_hi_b >> 32);
     // the place in the ring: barriers, operand descriptors of the stage's first panel and first tile
     const uint32_t full0 = smem_u32(&bars.full[0]), empty_off = smem_u32(&bars.empty[0]) - full0, full_end = full0 + 8u * (uint32_t)p.stages;
@@ -292,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) group_kernel(const __grid_con
           const int has = __shfl_sync(0xffffffffu, my_has, r);
           const float rs = __shfl_sync(0xffffffffu, my_scale, r);
           const uint32_t acc = tmem_base + lane_sel + buf * (uint32_t)buf_cols + (uint32_t)(r * kTile);
-          if (!TAIL && p.staged) {
+          if (!TAIL && !TRB && p.staged) {
             // 16-bit results: the warp's 32 x 32 part is put together in shared memory and leaves in 16-byte pieces, four
             // lanes per row.  (A tiled store by the copy engine waits there behind the panels' loads: 2.4 us per part.)
             uint32_t lo[16], hi[16];
@@ -327,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) group_kernel(const __grid_con
             if constexpr (TAIL) {
               finish16_tail<KIND>(od, tail, row, n, 0, &v[0], rs, cs, bias);
               finish16_tail<KIND>(od, tail, row, n, 16, &v[16], rs, cs, bias);
-            } else if (p.out_tr) {
+            } else if (TRB || p.out_tr) {
               finish16_tr<KIND>(od, row, n, 0, &v[0], rs, cs, bias);
               finish16_tr<KIND>(od, row, n, 16, &v[16], rs, cs, bias);
             } else {
@@ -520,16 +521,20 @@ __global__ void __launch_bounds__(256) group_copy_kernel(const uint4* __restrict
   blob[(size_t)tile_at[t] * (size_t)pieces + (size_t)(i - t * pieces)] = tiles[i];
 }
 
-template <int KIND>
+template <int KIND, bool TRB>
 int launch_group(const GroupParams& p, const Tail* tail, const CUtensorMap& mb, int grid, int smem, cudaStream_t st) {
   if (tail != nullptr) {
-    auto kernel = group_kernel<KIND, true>;
+    auto kernel = group_kernel<KIND, TRB, true>;
     if (ensure_smem((const void*)kernel, smem)) return VOID_ERR_CUDA;
     return status_of(launch_pdl(kernel, grid, kThreads, smem, st, mb, *tail, p));
   }
-  auto kernel = group_kernel<KIND, false>;
+  auto kernel = group_kernel<KIND, TRB, false>;
   if (ensure_smem((const void*)kernel, smem)) return VOID_ERR_CUDA;
   return status_of(launch_pdl(kernel, grid, kThreads, smem, st, mb, NoTail{}, p));
+}
+template <int KIND>
+int launch_group(const GroupParams& p, bool tr_b, const Tail* tail, const CUtensorMap& mb, int grid, int smem, cudaStream_t st) {
+  return tr_b ? launch_group<KIND, true>(p, tail, mb, grid, smem, st) : launch_group<KIND, false>(p, tail, mb, grid, smem, st);
 }
 
 static int spmm_grouped(const void_spmm_args* a, const void_group_store* s, int32_t kind, const Tail* tail, void_stream_t stream) {
@@ -544,10 +549,10 @@ static int spmm_grouped(const void_spmm_args* a, const void_group_store* s, int3
     return VOID_ERR_BAD_ARG;
   const int es = (kind == VOID_KIND_TF32) ? 4 : ((kind == VOID_KIND_F16 || kind == VOID_KIND_BF16) ? 2 : 1);
   if (a->tile_terms > 1 || (es > 1 && a->row_scale != nullptr)) return VOID_ERR_BAD_ARG;
-  if (a->transposed != 0 && a->transposed != 2) return VOID_ERR_BAD_ARG;
-  const bool tr = a->transposed != 0;
+  if (a->transposed < 0 || a->transposed > 2) return VOID_ERR_BAD_ARG;
+  const bool tr = a->transposed != 0, tr_b = a->transposed == 1;
   if ((long long)a->nbr * kTile < a->M || a->ldc < (tr ? a->M : a->N)) return VOID_ERR_SHAPE;
-  if ((reinterpret_cast<uintptr_t>(a->b) & 15u) != 0 || (a->ldb & 15) != 0 || a->ldb < (long long)a->N * es) return VOID_ERR_ALIGN;
+  if ((reinterpret_cast<uintptr_t>(a->b) & 15u) != 0 || (a->ldb & 15) != 0 || a->ldb < (long long)(tr_b ? a->K : a->N) * es) return VOID_ERR_ALIGN;
   const int rows = (a->nbr + s->n_groups - 1) / (s->n_groups > 0 ? s->n_groups : 1);
   if (s->n_groups <= 0 || rows < 1 || rows > kMaxRows) return VOID_ERR_BAD_ARG;
   if (s->max_entries < 1 || s->max_entries > kMaxEntries || s->max_tiles < 1 || s->max_tiles > kMaxStageTiles) return VOID_ERR_BAD_ARG;
@@ -597,23 +602,26 @@ static int spmm_grouped(const void_spmm_args* a, const void_group_store* s, int3
   p.desc_hi_b = smem_desc_hi(128, 256 * es, kLayoutNone);
   p.desc_hi_a = es == 4 ? smem_desc_hi(4096, 512, kLayoutSw128Base32)
                         : (es == 2 ? smem_desc_hi(4096, 1024, kLayoutSw128) : smem_desc_hi(1024, 1024, kLayoutSw128));
-  if (kind == VOID_KIND_I8) p.idesc = instr_desc(/*c s32*/ 2, /*s8*/ 1, 1, /*a MN*/ 1, /*b K*/ 0, 128, 32);
-  else if (kind == VOID_KIND_F16) p.idesc = instr_desc(1, 0, 0, 1, 0, 128, 32);
-  else if (kind == VOID_KIND_BF16) p.idesc = instr_desc(1, 1, 1, 1, 0, 128, 32);
-  else p.idesc = instr_desc(1, 2, 2, 1, 0, 128, 32);
+  if (tr_b) p.desc_hi_a = smem_desc_hi(16, 256 * es, es == 4 ? kLayoutSw128 : (es == 2 ? kLayoutSw64 : kLayoutSw32));
+  const uint32_t mn = tr_b ? 0u : 1u;   // whether the panel is MN-major
+  if (kind == VOID_KIND_I8) p.idesc = instr_desc(/*c s32*/ 2, /*s8*/ 1, 1, mn, /*b K*/ 0, 128, 32);
+  else if (kind == VOID_KIND_F16) p.idesc = instr_desc(1, 0, 0, mn, 0, 128, 32);
+  else if (kind == VOID_KIND_BF16) p.idesc = instr_desc(1, 1, 1, mn, 0, 128, 32);
+  else p.idesc = instr_desc(1, 2, 2, mn, 0, 128, 32);
 
   CUtensorMap mb;
   memset(&mb, 0, sizeof(mb));
   bool whole = a->N % (kPanelN / es) == 0;
-  if (!panel_map(&mb, a->b, a->ldb, a->K, a->N, es, 1, &whole)) return VOID_ERR_TENSOR_MAP;
+  if (!(tr_b ? panel_map_transposed(&mb, a->b, a->ldb, a->K, a->N, es) : panel_map(&mb, a->b, a->ldb, a->K, a->N, es, 1, &whole)))
+    return VOID_ERR_TENSOR_MAP;
   p.use3d = whole ? 1 : 0;
   int grid = a->grid > 0 ? a->grid : dev.sms * kCtas;
   if (grid > p.n_items) grid = p.n_items;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   switch (kind) {
-    case VOID_KIND_I8: return launch_group<VOID_KIND_I8>(p, tail, mb, grid, smem, st);
-    case VOID_KIND_TF32: return launch_group<VOID_KIND_TF32>(p, tail, mb, grid, smem, st);
-    default: return launch_group<VOID_KIND_F16>(p, tail, mb, grid, smem, st);
+    case VOID_KIND_I8: return launch_group<VOID_KIND_I8>(p, tr_b, tail, mb, grid, smem, st);
+    case VOID_KIND_TF32: return launch_group<VOID_KIND_TF32>(p, tr_b, tail, mb, grid, smem, st);
+    default: return launch_group<VOID_KIND_F16>(p, tr_b, tail, mb, grid, smem, st);
   }
 }
 
@@ -662,7 +670,7 @@ int void_spmm_grouped_linear(const void_spmm_args* a, const void_epilogue* e, co
   vb::Tail tail;
   const int st = vb::make_tail(a, e, &tail);
   if (st != VOID_OK) return st;
-  return a->transposed != 2 ? VOID_ERR_BAD_ARG : vb::spmm_grouped(a, s, kind, &tail, stream);
+  return vb::spmm_grouped(a, s, kind, &tail, stream);
 }
 
 }  // extern "C"

@@ -460,6 +460,16 @@ double group_line(const Packed* p) {
     default: return 1.1;
   }
 }
+// Linear layers on tokens as they lie, without a transposed copy: the row kernel's loads are 64-byte pieces there (128 for fp32), so the
+// grouped kernel gains more.  bf16, us, rows, rows on a copy and groups: 4096^2, 2048 tokens 90 % 21.2 24.6 20.2, 80 % 35.2 35.9 26.4, 70 %
+// 48.6 46.3 34.2, 50 % 77 69 41; 4096 x 16384, 90 % 63 81 53; 8192 x 2048, 4096 tokens 80 % 72 65 59; 1024 x 4096, 2048 tokens 80 % 12.3 16.8 11.3;
+// 512 tokens 4096^2 80 % 12.4 14.7 11.3.  Predicted saving and gain: 0.90 (90 %) 1.03, 0.94 (80 %) 1.10, 0.97 - 0.99 (90 %) 0.99 - 1.04, 0.99 (70 %) 1.14,
+// 1.06 (90 %) 1.05, 1.12 (90 %) 1.05, 1.41 (80 %) 1.33; at 95 % 0.97 - 1.05 whatever is predicted.  fp32: 1.12 1.01, 1.24 0.99, 1.27 1.06, 1.36 1.28,
+// 1.41 1.13, 1.93 1.51.  INT8 (32-byte pieces) 8192^2, 60 %, 1024 tokens 109, on a copy 52 and in groups of the copy 40, groups 49: copied.
+bool groups_of_tokens(const Packed* p, double saves) {
+  if (p->kind == VOID_KIND_TF32) return saves >= 1.25;
+  return (p->kind == VOID_KIND_F16 || p->kind == VOID_KIND_BF16) && saves >= 0.93 && p->args.nnz * 12.5 >= (double)p->args.nbr * p->args.nbc;
+}
 // Whether the kernels that write the store are through.  Asked without waiting; not while the stream is captured, where the
 // store then is not used.  (Another thread may be capturing: relaxed mode keeps the question from ending its capture.)
 bool complete(GroupStore* g, void_stream_t st) {
@@ -507,13 +517,14 @@ std::unique_ptr<GroupStore> build_group_store(const Packed* p, int64_t G, void_s
 // The group store that serves this product, or null.  Its build is queued behind the third product it would have served - a
 // tensor that is multiplied once or twice does not pay for it - once for each of up to two widths.  Nothing waits for it:
 // products go to the other kernel until it is complete, and then read it on any stream and ahead of their stream's order.
-GroupStore* group_store(Packed* p, int64_t N, void_stream_t st) {
-  if (!p->grouped || N <= 64 || p->args.nnz < 4096 || p->kind == VOID_KIND_F8E4M3) return nullptr;   // (FP8 of two terms: within 5 % either way)
+// tokens: for a linear layer that reads them as they lie.
+GroupStore* group_store(Packed* p, int64_t N, void_stream_t st, bool tokens = false) {
+  if (!p->grouped || N <= 64 || p->args.nnz < (tokens ? 512 : 4096) || p->kind == VOID_KIND_F8E4M3) return nullptr;   // (FP8 of two terms: within 5 % either way)
   const int slots = 2 * void_device_sm_count();
-  if ((int64_t)p->args.nbr * ((N + 127) / 128) < 2ll * slots) return nullptr;
-  const double line = group_line(p);
+  if ((int64_t)p->args.nbr * ((N + 127) / 128) < (tokens ? 1ll : 2ll) * slots) return nullptr;
   const GroupShape shape = group_shape(p, N, slots);
-  if (shape.saves < line) return nullptr;
+  auto pays = [&](double saves) { return tokens ? groups_of_tokens(p, saves) : saves >= group_line(p); };
+  if (!pays(shape.saves)) return nullptr;
   GroupStore* hit = nullptr;
   double hit_saves = 0.0, best = 0.0;   // best: of those that are still being built, too
   int n = 0;
@@ -528,7 +539,7 @@ GroupStore* group_store(Packed* p, int64_t N, void_stream_t st) {
     p->groups[n] = build_group_store(p, shape.groups, st);
     if (p->groups[n] != nullptr) p->group_calls = 0;
   }
-  return hit_saves >= line ? hit : nullptr;
+  return pays(hit_saves) ? hit : nullptr;
 }
 // What a linear layer's epilogue adds to a product (void_epilogue), with the tensors it points into.
 struct Tail {
@@ -562,10 +573,10 @@ void set_residual(Tail& t, const at::Tensor& given, const at::Tensor& out) {
   t.e.ldr = rows > 1 ? r.stride(0) : cols;
   t.e.residual_dtype = out_code(r.scalar_type());
 }
-// A plain product with everything filled in.
-void launch_product(Packed* p, const void_spmm_args& s, void_stream_t st, const void_epilogue* tail = nullptr) {
-  if (s.transposed != 1 && s.scale_mode == VOID_SCALE_ROW_MEAN) {
-    GroupStore* g = group_store(p, s.N, st);
+// A plain product with everything filled in; tokens: the group store of a linear layer that reads them as they lie (transposed = 1).
+void launch_product(Packed* p, const void_spmm_args& s, void_stream_t st, const void_epilogue* tail = nullptr, GroupStore* tokens = nullptr) {
+  if (s.scale_mode == VOID_SCALE_ROW_MEAN) {
+    GroupStore* g = s.transposed == 1 ? tokens : group_store(p, s.N, st);
     if (g != nullptr) {
       g->readers.add(c10::cuda::getCurrentCUDAStream(p->device), {&g->index, &g->blob});
       if (p->captured && capturing(st)) g->captured = true;
@@ -624,7 +635,9 @@ PyObject* spmm(PyObject*, PyObject* const* a, Py_ssize_t n) {
       fail("out must be a row-major [" + std::to_string(rows) + ", " + std::to_string(cols) + "] tensor");
     if (out.device() != dev) fail("out and B are on different devices");
   }
-  const bool copied = tr && none(a[11]) && copy_pays(pk->kind, pk->args.nnz, N, pk->K);
+  const void_stream_t st = launch_stream(pk);
+  GroupStore* tokens = tr && none(a[11]) ? group_store(pk, N, st, true) : nullptr;
+  const bool copied = tr && none(a[11]) && tokens == nullptr && copy_pays(pk->kind, pk->args.nnz, N, pk->K);
   const at::Tensor b = copied ? transposed_copy(b_in, es) : kernel_operand(b_in, es, tr ? 0 : pk->args.nnz * ((N + 127) / 128));
 
   void_spmm_args s = pk->args;
@@ -706,8 +719,7 @@ PyObject* spmm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   // bit 2: the packed store (and the plan, whose builder synchronises) is complete, so the kernel may read it
   // before it waits for the previous kernel; bit 30 (measurements) keeps it from doing so
   s.flags = (int32_t)(flags & 0xffff) | ((pk->stable && !(flags & (1ll << 30))) ? 4 : 0);
-  const void_stream_t st = launch_stream(pk);
-  if (none(a[11])) launch_product(pk, s, st, tail.get());
+  if (none(a[11])) launch_product(pk, s, st, tail.get(), tokens);
   else if (es > 1) check(void_spmm_fp(&s, pk->kind, st), "void_spmm_fp");
   else check(pk->kind == VOID_KIND_I8 ? void_spmm_i8(&s, st) : void_spmm_f8(&s, st), "void_spmm");
   if (!none(a[2])) {
@@ -732,9 +744,11 @@ at::Tensor two_layers(Packed* first, Packed* second, const at::Tensor& x, PyObje
   if (c10::cuda::current_device() != dev.index()) guard.set_device(dev);
   const int kind = pk[0]->kind, es = elem_bytes(kind);
   const int64_t N = x.size(0);
-  const bool columns = N > 128 && copy_saves_ns(kind, pk[0]->args.nnz + pk[1]->args.nnz, N) > copy_costs_ns(N, pk[0]->K, es);
   const void_stream_t st = launch_stream(pk[0]);
   launch_stream(pk[1]);
+  GroupStore* tokens[2] = {group_store(pk[0], N, st, true), group_store(pk[1], N, st, true)};
+  const bool columns = (tokens[0] == nullptr || tokens[1] == nullptr) && N > 128 &&
+                       copy_saves_ns(kind, pk[0]->args.nnz + pk[1]->args.nnz, N) > copy_costs_ns(N, pk[0]->K, es);
   at::Tensor in = columns ? transposed_copy(x, es) : kernel_operand(x, es), bias[2], out;
   for (int layer = 0; layer < 2; ++layer) {
     Packed* p = pk[layer];
@@ -756,7 +770,7 @@ at::Tensor two_layers(Packed* first, Packed* second, const at::Tensor& x, PyObje
     s.transposed = columns ? (layer == 0 ? 0 : 2) : 1;
     s.flags = p->stable ? 4 : 0;
     if (layer == 1 && !none(residual)) set_residual(tail, cuda_tensor(residual, "residual"), out);
-    launch_product(p, s, st, tail.get());
+    launch_product(p, s, st, tail.get(), tokens[layer]);
     in = out;
   }
   return out;
