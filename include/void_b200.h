@@ -474,6 +474,14 @@ VOID_API int void_expert_plan(const void* offsets, int32_t offset_bytes, int32_t
                               int32_t* status, void_stream_t stream);
 VOID_API int void_expert_linear(const void_spmm_args* args, const void_epilogue* epilogue, const void_experts* experts, int32_t kind,
                                 void_stream_t stream);
+/* The same with the tiles of groups of tile rows (void_group_build) laid out expert by expert: n_groups of all experts together, a
+ * multiple of n_experts; row_order [n_experts * nbr] as in void_experts, nbr tile rows of one expert.  void_expert_grouped: chunk 128. */
+VOID_API int void_expert_group_build(const int32_t* row_ptr, const int32_t* row_order, const int32_t* tile_cols, const void* tiles,
+                                     int32_t nbr, int32_t n_experts, int64_t nnz, int32_t elem_bytes, int32_t n_groups,
+                                     int32_t max_entries, int32_t max_tiles, int32_t* group_rows, int32_t* stage_ptr, int32_t* records,
+                                     void* blob, int32_t* ws, void_stream_t stream);
+VOID_API int void_expert_grouped(const void_spmm_args* args, const void_epilogue* epilogue, const void_experts* experts,
+                                 const void_group_store* store, int32_t kind, void_stream_t stream);
 VOID_API int void_expert_tile_grad(const void* grad_out, int64_t ldg, const void* x, int64_t ldx, int32_t M, int32_t K, int32_t N,
                                    int32_t kind, const void_experts* experts, const int32_t* items, int32_t n_items,
                                    const int32_t* tile_cols, const int32_t* block_indices, void* grad_tiles, int32_t out_dtype,

@@ -77,6 +77,33 @@ def test_linear_refuses(kw, status):
     assert _linear(**kw) == status
 
 
+def test_grouped_form_refuses():
+    lib, a, x, g = _lib.load(), _lib.SpmmArgs(), _lib.Experts(plan=1024, n_experts=2, chunk=128), _lib.GroupStore()
+    a.row_ptr, a.out, a.b, a.nbr, a.nbc, a.M, a.K, a.N, a.ldb, a.ldc, a.transposed = 1024, 1024, 1024, 1, 1, 32, 32, 4, 64, 32, 1
+
+    def call(**kw):
+        keep = {}
+        for k, v in kw.items():
+            if k != "kind":
+                t = x if hasattr(_lib.Experts, k) else (g if hasattr(_lib.GroupStore, k) else a)
+                keep[k] = (t, getattr(t, k))
+                setattr(t, k, v)
+        st = lib.void_expert_grouped(ctypes.byref(a), None, ctypes.byref(x), ctypes.byref(g), kw.get("kind", _lib.KIND_F16), None)
+        for k, (t, v) in keep.items():
+            setattr(t, k, v)
+        return st
+    assert lib.void_expert_grouped(None, None, ctypes.byref(x), ctypes.byref(g), _lib.KIND_F16, None) == BAD_ARG
+    assert call() == BAD_ARG                                     # an empty store
+    for bad in (dict(kind=_lib.KIND_I8), dict(chunk=32), dict(n_experts=0), dict(plan=None), dict(transposed=2), dict(col_scale=1024), dict(row_scale=1024)):
+        assert call(**bad) == BAD_ARG, bad
+    g.blob = g.records = g.stage_ptr = g.group_rows = 1024
+    g.max_entries = g.max_tiles = 1
+    assert call(n_groups=3) == BAD_ARG                           # not the same number for every expert
+    p = ctypes.c_void_p(1024)
+    assert lib.void_expert_group_build(p, None, p, p, 4, 3, 10, 2, 4, 1, 1, p, p, p, p, p, None) == BAD_ARG
+    assert lib.void_expert_group_build(p, None, p, p, 100, 3, 10, 2, 3, 1, 1, p, p, p, p, p, None) == BAD_ARG     # more than eight rows in a group
+
+
 def test_no_tokens_is_no_work():
     assert _linear(args=dict(N=0, out=None)) == 0
     assert _lib.load().void_expert_linear(None, None, None, _lib.KIND_F16, None) == BAD_ARG

@@ -361,3 +361,34 @@ def test_refusals():
     torch.autograd.grad(y.sum(), x)
     with pytest.raises(RuntimeError, match="second time|freed"):
         torch.autograd.grad(y.sum(), x)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n, k, m, density, counts, before, behind", [
+    (4, 1024, 2000, 0.3, [700, 0, 1500, 331], 0, 0), (4, 1024, 2000, 0.3, [700, 0, 1500, 331], 5, 300), (3, 2048, 4096, 0.45, [900, 1, 400], 0, 77),
+    (8, 515, 1100, 0.5, [600, 601, 0, 0, 1, 700, 129, 1000], 3, 1),
+])
+def test_groups_of_tile_rows(n, k, m, density, counts, before, behind, dtype):
+    # (the first calls take the row kernel; from the fourth on a store for groups of each expert's tile rows is there)
+    weights, e = experts_of(n, m, k, density, dtype)
+    tokens = before + sum(counts) + behind
+    x, bias, offsets = rand(tokens, k, dtype=dtype), rand(n, m, seed=1), offsets_of(counts, before)
+    first = void.void_expert_linear(e, x, offsets, bias, 3)
+    check_forward(first, weights, x, counts, before, bias, "silu")
+    for _ in range(5):
+        y = void.void_expert_linear(e, x, offsets, bias, 3)
+        torch.cuda.synchronize()
+    check_forward(y, weights, x, counts, before, bias, "silu")
+    packed = next(iter(e.tensor._packed_fp_cache.values()))
+    allowed, stores, done = _lib.native().packed_grouped(packed.native, None)
+    assert allowed and (dtype == torch.float32 or (stores == 1 and done == 1))
+    other = list(reversed(counts))
+    y = void.void_expert_linear(e, x, offsets_of(other, before), bias.bfloat16(), 1)
+    check_forward(y, weights, x, other, before, bias.bfloat16(), "relu")
+    mine = rand(tokens, m, dtype=dtype, seed=8)
+    was = mine.clone()
+    void.void_expert_linear(e, x, offsets, None, 0, out=mine)
+    check_forward(mine, weights, x, counts, before, None, "none", untouched=was)
+    void.allow_group_stores(e.tensor, False)
+    assert torch.equal(void.void_expert_linear(e, x, offsets, bias, 3), first)
+    void.check_device_status()

@@ -120,6 +120,10 @@ _PROTOTYPES = {
     "void_expert_plan_words": (c_i64, [c_i32, c_i32, c_i32]),
     "void_expert_plan": (ctypes.c_int, [c_vp, c_i32, c_i32, c_i32, c_i32, c_vp, c_vp, c_vp]),
     "void_expert_linear": (ctypes.c_int, [ctypes.POINTER(SpmmArgs), ctypes.POINTER(Epilogue), ctypes.POINTER(Experts), c_i32, c_vp]),
+    "void_expert_group_build": (ctypes.c_int, [c_vp, c_vp, c_vp, c_vp, c_i32, c_i32, c_i64, c_i32, c_i32, c_i32, c_i32, c_vp, c_vp, c_vp, c_vp,
+                                               c_vp, c_vp]),
+    "void_expert_grouped": (ctypes.c_int, [ctypes.POINTER(SpmmArgs), ctypes.POINTER(Epilogue), ctypes.POINTER(Experts), ctypes.POINTER(GroupStore),
+                                           c_i32, c_vp]),
     "void_expert_tile_grad": (ctypes.c_int, [c_vp, c_i64, c_vp, c_i64, c_i32, c_i32, c_i32, c_i32, ctypes.POINTER(Experts), c_vp, c_i32, c_vp,
                                              c_vp, c_vp, c_i32, c_vp, c_vp]),
     "void_expert_activation_grad_ws_bytes": (c_sz, [ctypes.POINTER(Experts), c_i32, c_i32]),

@@ -5,6 +5,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/void_b200.h"
 #include "ptx.cuh"
 
@@ -298,6 +300,31 @@ struct Tail {
 };
 __device__ __forceinline__ float f16_value(uint32_t bits, bool f16) {
   return f16 ? __half2float(__ushort_as_half((unsigned short)bits)) : __uint_as_float(bits << 16);
+}
+// A product whose weight is one of several experts', each multiplied with its own run of tokens (B and C transposed): a work item is one
+// chunk of an expert's tokens and some of its tile rows, chunks as laid out by expert_plan_kernel (experts.cu).
+struct ExpertParams {
+  Tail tail;
+  const int32_t* head;        // number of chunks
+  const int32_t* bounds;      // [experts + 1]: where the experts' runs of tokens begin, and the end of the last
+  const int4* chunks;         // expert, first token, token behind the last
+  const int32_t* row_order;   // [experts][tile rows]: tile row of the k-th row taken, or null for k
+  int n_experts, zero_rest;   // zero_rest: tokens outside all runs get zeros
+};
+struct Nothing {};
+template <class X>
+constexpr bool kExpertsOf = std::is_same<X, ExpertParams>::value;
+
+// Zeros for the tokens in no expert's run, dealt out over the CTAs.
+__device__ __forceinline__ void zero_rest_rows(const OutDesc& o, const ExpertParams& x, int tid, int threads) {
+  const int before = x.bounds[0], behind = x.bounds[x.n_experts], rest = before + o.N - behind;
+  for (int i = blockIdx.x; i < rest; i += gridDim.x) {
+    const size_t first = (size_t)(i < before ? i : i - before + behind) * (size_t)o.ldc;
+    if (o.dtype == VOID_OUT_F32)
+      for (int c = tid; c < o.M; c += threads) reinterpret_cast<float*>(o.out)[first + c] = 0.0f;
+    else
+      for (int c = tid; c < o.M; c += threads) reinterpret_cast<uint16_t*>(o.out)[first + c] = 0;
+  }
 }
 // Expert e's biases of M each.
 __device__ __forceinline__ const float* bias_of_expert(const float* bias, int dtype, int e, int M) {

@@ -31,6 +31,7 @@
 
 #include "../../include/void_b200.h"
 #include "epilogue.cuh"
+#include "experts.cuh"
 #include "kinds.cuh"
 #include "launch.cuh"
 #include "ptx.cuh"
@@ -70,6 +71,7 @@ struct GroupParams {
   int32_t* status;
   int nbr, n_groups, n_chunks, n_items, rows;
   int classes;                 // MMA warps with rows
+  int expert_groups, expert_rows;   // groups and tile rows of one expert
   int panel_bytes;             // panels of a stage (their tiles follow)
   int stage_bytes, stages;
   int use3d, staged, out_tr, a_stable;
@@ -78,18 +80,39 @@ struct GroupParams {
   unsigned int idesc;
 };
 
-struct NoTail {};
-
 struct __align__(8) Bars {
   uint64_t full[kMaxRing], empty[kMaxRing];
   uint64_t acc_full[2][kClasses], acc_empty[2][kClasses];
 };
 
-// TRB: B stored transposed, [N, K], and C with it: tokens as they lie.  TAIL: results [N, M] of a linear layer with a tail.
-template <int KIND, bool TRB, bool TAIL>
+// A work item: a group and a chunk of columns (of tokens), those of one expert where there are several.
+struct Item {
+  int g, n0, n1, expert;
+};
+template <class X>
+__device__ __forceinline__ Item item_of(const GroupParams& p, const X& x, int i) {
+  if constexpr (kExpertsOf<X>) {   // the groups of a chunk one after the other
+    const int c = i / p.expert_groups;
+    const int4 t = x.chunks[c];
+    return {t.x * p.expert_groups + i - c * p.expert_groups, t.y, t.z, t.x};
+  } else {
+    const int g = i / p.n_chunks, chunk = i - g * p.n_chunks;
+    return {g, chunk * kPanelN, p.out.N, 0};
+  }
+}
+template <class X>
+__device__ __forceinline__ int items_of(const GroupParams& p, const X& x) {
+  if constexpr (kExpertsOf<X>) return x.head[0] * p.expert_groups;
+  else return p.n_items;
+}
+
+// TRB: B stored transposed, [N, K], and C with it: tokens as they lie.  X: Tail, results [N, M] of a linear layer with one; ExpertParams,
+// the same for every expert's tokens (with TRB); or Nothing.
+template <int KIND, bool TRB, class X>
 __global__ void __launch_bounds__(kThreads, kCtas) group_kernel(const __grid_constant__ CUtensorMap tmap_b,
-                                                            const __grid_constant__ std::conditional_t<TAIL, Tail, NoTail> tail,
-                                                            const __grid_constant__ GroupParams p) {
+                                                            const __grid_constant__ X x, const __grid_constant__ GroupParams p) {
+  constexpr bool EXPERTS = kExpertsOf<X>, TAIL = std::is_same<X, Tail>::value;
+  static_assert(!EXPERTS || TRB, "tokens as they lie");
   extern __shared__ uint8_t smem_raw[];
   __shared__ Bars bars;
   __shared__ uint32_t tmem_base_s;
@@ -135,9 +158,10 @@ __global__ void __launch_bounds__(kThreads, kCtas) group_kernel(const __grid_con
     uint32_t phase = 0;
     while (slot >= S) { slot -= S; phase ^= 1u; }
     bool ok = true;
-    for (int i = blockIdx.x; i < p.n_items && ok; i += gridDim.x) {
-      const int g = i / p.n_chunks, chunk = i - g * p.n_chunks;
-      const int s0 = p.stage_ptr[g], s1 = p.stage_ptr[g + 1];
+    const int n_items = items_of(p, x);
+    for (int i = blockIdx.x; i < n_items && ok; i += gridDim.x) {
+      const Item item = item_of(p, x, i);
+      const int s0 = p.stage_ptr[item.g], s1 = p.stage_ptr[item.g + 1];
       int s = s0 + ((warp - first) & (kProducers - 1));
       // records of this warp's next four stages, fetched four stages ahead
       const int mine = s + (lane >> 3) * kProducers;
@@ -168,11 +192,11 @@ __global__ void __launch_bounds__(kThreads, kCtas) group_kernel(const __grid_con
         }
         if (lane < entries) {
           const uint32_t dst = base + (uint32_t)lane * (kPanelBytes * ES);
-          if (TRB) tma_load_2d(dst, &tmap_b, col * kTile, chunk * kPanelN, full);
-          else if (p.use3d) tma_load_3d(dst, &tmap_b, 0, col * kTile, chunk * ES, full);
+          if (TRB) tma_load_2d(dst, &tmap_b, col * kTile, item.n0, full);
+          else if (p.use3d) tma_load_3d(dst, &tmap_b, 0, col * kTile, item.n0 / kPanelN * ES, full);
           else
             for (int q = 0; q < ES; ++q)
-              tma_load_2d(dst + (uint32_t)q * kPanelBytes, &tmap_b, chunk * kPanelN + q * (kPanelN / ES), col * kTile, full);
+              tma_load_2d(dst + (uint32_t)q * kPanelBytes, &tmap_b, item.n0 + q * (kPanelN / ES), col * kTile, full);
         }
         slot += kProducers;
         while (slot >= S) { slot -= S; phase ^= 1u; }
@@ -186,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) group_kernel(const __grid_con
     if (!p.a_stable) grid_dependency_wait();
     const bool leader = elect_one();
     const int cls = warp - kMmaWarp0;
-    const size_t tiles = (size_t)p.row_ptr[p.nbr];
+    const size_t tiles = (size_t)p.row_ptr[p.nbr];   // (of all experts)
     const uint4* heads = reinterpret_cast<const uint4*>(p.blob + tiles * (size_t)(kTileBytes * ES)) + (size_t)cls * tiles;
     const uint32_t idesc = p.idesc;
     constexpr uint32_t kTileStep = (kTileBytes * ES) >> 4, kPanelStep = (kPanelBytes * ES) >> 4;
@@ -200,18 +224,19 @@ __global__ void __launch_bounds__(kThreads, kCtas) group_kernel(const __grid_con
     bool ok = true;
     int s0 = 0, s1 = 0;
     uint4 h0 = {}, h1 = {}, h2 = {};   // heads of the next three stages
-    if ((int)blockIdx.x < p.n_items) {
-      const int g = blockIdx.x / p.n_chunks;
+    const int n_items = items_of(p, x);
+    if ((int)blockIdx.x < n_items) {
+      const int g = item_of(p, x, blockIdx.x).g;
       s0 = p.stage_ptr[g];
       s1 = p.stage_ptr[g + 1];
     }
-    for (int i = blockIdx.x; i < p.n_items && ok; i += gridDim.x, ++it) {
+    for (int i = blockIdx.x; i < n_items && ok; i += gridDim.x, ++it) {
       if (s0 < s1) h0 = heads[s0];
       if (s0 + 1 < s1) h1 = heads[s0 + 1];
       if (s0 + 2 < s1) h2 = heads[s0 + 2];
       int n0 = 0, n1 = 0;   // stages of the item after this one
-      if (i + (int)gridDim.x < p.n_items) {
-        const int g = (i + (int)gridDim.x) / p.n_chunks;
+      if (i + (int)gridDim.x < n_items) {
+        const int g = item_of(p, x, i + (int)gridDim.x).g;
         n0 = p.stage_ptr[g];
         n1 = p.stage_ptr[g + 1];
       }
@@ -262,22 +287,30 @@ __global__ void __launch_bounds__(kThreads, kCtas) group_kernel(const __grid_con
     const OutDesc od = p.out;
     const uint32_t part = ring + (uint32_t)p.stages * (uint32_t)p.stage_bytes + (uint32_t)(warp - kEpiWarp0) * kPartBytes;
     grid_dependency_wait();
+    if constexpr (EXPERTS)
+      if (x.zero_rest) zero_rest_rows(od, x, (int)threadIdx.x - 32 * kEpiWarp0, 32 * kEpiWarps);
     uint32_t it = 0;
     bool ok = true;
-    for (int i = blockIdx.x; i < p.n_items && ok; i += gridDim.x, ++it) {
-      const int g = i / p.n_chunks, chunk = i - g * p.n_chunks;
+    const int n_items = items_of(p, x);
+    for (int i = blockIdx.x; i < n_items && ok; i += gridDim.x, ++it) {
+      const Item item = item_of(p, x, i);
+      OutDesc to = od;
+      if constexpr (EXPERTS) {
+        to.N = item.n1;
+        if (to.row_bias != nullptr) to.row_bias = bias_of_expert(to.row_bias, x.tail.bias_dtype, item.expert, od.M);
+      }
       const uint32_t buf = n_buf == 2 ? (it & 1u) : 0u, use = n_buf == 2 ? (it >> 1) : it;
       // this lane's row of the group, with what its epilogue needs; scales and biases of the columns
-      const int my_row = lane < p.rows ? p.group_rows[g * kMaxGroupRows + lane] : -1;
+      const int my_row = lane < p.rows ? p.group_rows[item.g * kMaxGroupRows + lane] : -1;
       int my_has = 0;
       float my_scale = 1.0f;
       if (my_row >= 0) {
         my_has = p.row_ptr[my_row + 1] > p.row_ptr[my_row] ? 1 : 0;
         if (p.row_scale != nullptr && my_has) my_scale = p.row_scale[my_row];
       }
-      const int n = chunk * kPanelN + quad * 32 + lane;
+      const int n = item.n0 + quad * 32 + lane;
       float cs = p.b_scale, bias = 0.0f;
-      if (n < od.N) {
+      if (n < to.N) {
         if (p.col_scale != nullptr) cs *= p.col_scale[n];
         if (p.bias != nullptr) bias = p.bias[n];
       }
@@ -325,9 +358,13 @@ __global__ void __launch_bounds__(kThreads, kCtas) group_kernel(const __grid_con
 #pragma unroll
               for (int k = 0; k < 32; ++k) v[k] = 0u;
             }
-            if constexpr (TAIL) {
-              finish16_tail<KIND>(od, tail, row, n, 0, &v[0], rs, cs, bias);
-              finish16_tail<KIND>(od, tail, row, n, 16, &v[16], rs, cs, bias);
+            if constexpr (EXPERTS) {
+              const int own = row - item.expert * p.expert_rows;
+              finish16_tail<KIND>(to, x.tail, own, n, 0, &v[0], rs, cs, bias);
+              finish16_tail<KIND>(to, x.tail, own, n, 16, &v[16], rs, cs, bias);
+            } else if constexpr (TAIL) {
+              finish16_tail<KIND>(od, x, row, n, 0, &v[0], rs, cs, bias);
+              finish16_tail<KIND>(od, x, row, n, 16, &v[16], rs, cs, bias);
             } else if (TRB || p.out_tr) {
               finish16_tr<KIND>(od, row, n, 0, &v[0], rs, cs, bias);
               finish16_tr<KIND>(od, row, n, 16, &v[16], rs, cs, bias);
@@ -360,15 +397,16 @@ __global__ void __launch_bounds__(kThreads, kCtas) group_kernel(const __grid_con
 
 // ------------------------------------------------------------------------------------------ building a group store
 // Rows of falling length (row_order, or their own order) dealt to the groups back and forth.
-__global__ void group_rows_kernel(const int32_t* __restrict__ row_order, int nbr, int n_groups, int32_t* __restrict__ group_rows) {
+// (experts: nbr rows and n_groups groups of each, its rows in an order of its own)
+__global__ void group_rows_kernel(const int32_t* __restrict__ row_order, int nbr, int n_groups, int n_experts, int32_t* __restrict__ group_rows) {
   const int i = blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= n_groups * kMaxGroupRows) return;
-  const int g = i / kMaxGroupRows, slot = i - g * kMaxGroupRows;
+  if (i >= n_experts * n_groups * kMaxGroupRows) return;
+  const int all = i / kMaxGroupRows, slot = i - all * kMaxGroupRows, e = all / n_groups, g = all - e * n_groups;
   const long long k = (long long)slot * n_groups + ((slot & 1) ? n_groups - 1 - g : g);
   int row = -1;
   if (k < nbr) {
-    row = row_order != nullptr ? row_order[k] : (int)k;
-    if (row < 0 || row >= nbr) row = -1;
+    row = row_order != nullptr ? row_order[(size_t)e * nbr + k] : (int)k;
+    row = row < 0 || row >= nbr ? -1 : e * nbr + row;
   }
   group_rows[i] = row;
 }
@@ -521,23 +559,32 @@ __global__ void __launch_bounds__(256) group_copy_kernel(const uint4* __restrict
   blob[(size_t)tile_at[t] * (size_t)pieces + (size_t)(i - t * pieces)] = tiles[i];
 }
 
-template <int KIND, bool TRB>
-int launch_group(const GroupParams& p, const Tail* tail, const CUtensorMap& mb, int grid, int smem, cudaStream_t st) {
-  if (tail != nullptr) {
-    auto kernel = group_kernel<KIND, TRB, true>;
-    if (ensure_smem((const void*)kernel, smem)) return VOID_ERR_CUDA;
-    return status_of(launch_pdl(kernel, grid, kThreads, smem, st, mb, *tail, p));
-  }
-  auto kernel = group_kernel<KIND, TRB, false>;
-  if (ensure_smem((const void*)kernel, smem)) return VOID_ERR_CUDA;
-  return status_of(launch_pdl(kernel, grid, kThreads, smem, st, mb, NoTail{}, p));
+struct GroupLaunch {
+  const GroupParams& p;
+  bool tr_b;
+  const Tail* tail;              // or null
+  const ExpertParams* experts;   // or null
+  const CUtensorMap& b;
+  int grid, smem;
+  cudaStream_t stream;
+};
+template <int KIND, bool TRB, class X>
+int launch_group(const GroupLaunch& l, const X& x) {
+  auto kernel = group_kernel<KIND, TRB, X>;
+  if (ensure_smem((const void*)kernel, l.smem)) return VOID_ERR_CUDA;
+  return status_of(launch_pdl(kernel, l.grid, kThreads, l.smem, l.stream, l.b, x, l.p));
 }
 template <int KIND>
-int launch_group(const GroupParams& p, bool tr_b, const Tail* tail, const CUtensorMap& mb, int grid, int smem, cudaStream_t st) {
-  return tr_b ? launch_group<KIND, true>(p, tail, mb, grid, smem, st) : launch_group<KIND, false>(p, tail, mb, grid, smem, st);
+int launch_group(const GroupLaunch& l) {
+  if constexpr (KIND != VOID_KIND_I8)
+    if (l.experts != nullptr) return launch_group<KIND, true>(l, *l.experts);
+  if (l.tail != nullptr) return l.tr_b ? launch_group<KIND, true>(l, *l.tail) : launch_group<KIND, false>(l, *l.tail);
+  return l.tr_b ? launch_group<KIND, true>(l, Nothing{}) : launch_group<KIND, false>(l, Nothing{});
 }
 
-static int spmm_grouped(const void_spmm_args* a, const void_group_store* s, int32_t kind, const Tail* tail, void_stream_t stream) {
+// tail: what a linear layer's epilogue does besides, or null.  experts: nbr, M and K are one expert's, the store all experts' groups.
+static int spmm_grouped(const void_spmm_args* a, const void_group_store* s, int32_t kind, const Tail* tail, void_stream_t stream,
+                        const ExpertParams* experts = nullptr, int capacity = 0) {
   if (a == nullptr || s == nullptr || kind < VOID_KIND_I8 || kind > VOID_KIND_TF32 || kind == VOID_KIND_F8E4M3) return VOID_ERR_BAD_ARG;
   if (a->M <= 0 || a->N <= 0 || a->K <= 0 || a->nbr <= 0) return VOID_ERR_BAD_ARG;
   if (a->out == nullptr || a->b == nullptr || a->row_ptr == nullptr || s->blob == nullptr || s->records == nullptr ||
@@ -553,8 +600,10 @@ static int spmm_grouped(const void_spmm_args* a, const void_group_store* s, int3
   const bool tr = a->transposed != 0, tr_b = a->transposed == 1;
   if ((long long)a->nbr * kTile < a->M || a->ldc < (tr ? a->M : a->N)) return VOID_ERR_SHAPE;
   if ((reinterpret_cast<uintptr_t>(a->b) & 15u) != 0 || (a->ldb & 15) != 0 || a->ldb < (long long)(tr_b ? a->K : a->N) * es) return VOID_ERR_ALIGN;
-  const int rows = (a->nbr + s->n_groups - 1) / (s->n_groups > 0 ? s->n_groups : 1);
-  if (s->n_groups <= 0 || rows < 1 || rows > kMaxRows) return VOID_ERR_BAD_ARG;
+  const int n_experts = experts != nullptr ? experts->n_experts : 1;
+  if (s->n_groups <= 0 || s->n_groups % n_experts != 0) return VOID_ERR_BAD_ARG;
+  const int each = s->n_groups / n_experts, rows = (a->nbr + each - 1) / each;
+  if (rows < 1 || rows > kMaxRows) return VOID_ERR_BAD_ARG;
   if (s->max_entries < 1 || s->max_entries > kMaxEntries || s->max_tiles < 1 || s->max_tiles > kMaxStageTiles) return VOID_ERR_BAD_ARG;
   const DeviceInfo dev = device_info();
   if (!dev.ok) return VOID_ERR_CUDA;
@@ -579,16 +628,18 @@ static int spmm_grouped(const void_spmm_args* a, const void_group_store* s, int3
   p.out.dtype = a->out_dtype;
   p.out.act = a->act;
   p.status = a->status;
-  p.nbr = a->nbr;
+  p.nbr = a->nbr * n_experts;
   p.n_groups = s->n_groups;
-  p.n_chunks = (a->N + kPanelN - 1) / kPanelN;
+  p.expert_groups = each;
+  p.expert_rows = a->nbr;
+  p.n_chunks = experts != nullptr ? capacity : (a->N + kPanelN - 1) / kPanelN;
   p.classes = (rows + kClassRows - 1) / kClassRows;
-  if ((long long)p.n_groups * p.n_chunks > 0x7fffffffLL) return VOID_ERR_TOO_LARGE;
-  p.n_items = p.n_groups * p.n_chunks;
+  if ((long long)each * p.n_chunks > 0x7fffffffLL) return VOID_ERR_TOO_LARGE;
+  p.n_items = each * p.n_chunks;   // (experts: at most)
   p.rows = rows;
   p.out_tr = tr ? 1 : 0;
   p.staged = (!tr && a->out_dtype != VOID_OUT_F32 && a->N % 8 == 0 && a->ldc % 8 == 0 && (reinterpret_cast<uintptr_t>(a->out) & 15u) == 0) ? 1 : 0;
-  p.a_stable = (a->flags & 4) ? 1 : 0;
+  p.a_stable = (a->flags & 4) && experts == nullptr ? 1 : 0;   // (experts: the kernel before writes what every role reads first)
   p.wait_limit_ms = (a->test_hooks & 0xffff) ? (a->test_hooks & 0xffff) : kDefaultWaitLimitMs;
   p.panel_bytes = s->max_entries * kPanelBytes * es;
   p.stage_bytes = (p.panel_bytes + s->max_tiles * kTileBytes * es + 1023) / 1024 * 1024;
@@ -617,29 +668,23 @@ static int spmm_grouped(const void_spmm_args* a, const void_group_store* s, int3
   p.use3d = whole ? 1 : 0;
   int grid = a->grid > 0 ? a->grid : dev.sms * kCtas;
   if (grid > p.n_items) grid = p.n_items;
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const GroupLaunch l = {p, tr_b, tail, experts, mb, grid, smem, reinterpret_cast<cudaStream_t>(stream)};
   switch (kind) {
-    case VOID_KIND_I8: return launch_group<VOID_KIND_I8>(p, tr_b, tail, mb, grid, smem, st);
-    case VOID_KIND_TF32: return launch_group<VOID_KIND_TF32>(p, tr_b, tail, mb, grid, smem, st);
-    default: return launch_group<VOID_KIND_F16>(p, tr_b, tail, mb, grid, smem, st);
+    case VOID_KIND_I8: return launch_group<VOID_KIND_I8>(l);
+    case VOID_KIND_TF32: return launch_group<VOID_KIND_TF32>(l);
+    default: return launch_group<VOID_KIND_F16>(l);
   }
 }
-
-}  // namespace
-
-}  // namespace vb
-
-extern "C" {
-
-int void_group_build(const int32_t* row_ptr, const int32_t* row_order, const int32_t* tile_cols, const void* tiles, int32_t nbr,
-                     int64_t nnz, int32_t elem_bytes, int32_t n_groups, int32_t max_entries, int32_t max_tiles,
-                     int32_t* group_rows, int32_t* stage_ptr, int32_t* records, void* blob, int32_t* ws, void_stream_t stream) {
-  using namespace vb;
-  if (nbr <= 0 || nnz <= 0 || n_groups <= 0 || (long long)n_groups * kMaxGroupRows < nbr) return VOID_ERR_BAD_ARG;
+static int group_build(const int32_t* row_ptr, const int32_t* row_order, const int32_t* tile_cols, const void* tiles, int32_t nbr, int32_t n_experts,
+                       int64_t nnz, int32_t elem_bytes, int32_t n_groups, int32_t max_entries, int32_t max_tiles, int32_t* group_rows,
+                       int32_t* stage_ptr, int32_t* records, void* blob, int32_t* ws, void_stream_t stream) {
+  if (nbr <= 0 || n_experts <= 0 || nnz <= 0 || n_groups <= 0 || n_groups % n_experts != 0) return VOID_ERR_BAD_ARG;
+  const int each = n_groups / n_experts;
+  if ((long long)each * kMaxGroupRows < nbr) return VOID_ERR_BAD_ARG;
   if ((elem_bytes != 1 && elem_bytes != 2 && elem_bytes != 4)) return VOID_ERR_BAD_ARG;
   const int tile_bytes = kTileBytes * elem_bytes;
   if (max_entries < 1 || max_entries > kMaxEntries || max_tiles < 1 ||
-      max_tiles > kMaxStageTiles || (nbr + n_groups - 1) / n_groups > kMaxRows)
+      max_tiles > kMaxStageTiles || (nbr + each - 1) / each > kMaxRows)
     return VOID_ERR_BAD_ARG;
   if (nnz > 0x7fffffffLL / 8) return VOID_ERR_TOO_LARGE;
   if (row_ptr == nullptr || tile_cols == nullptr || tiles == nullptr || group_rows == nullptr || stage_ptr == nullptr ||
@@ -652,7 +697,7 @@ int void_group_build(const int32_t* row_ptr, const int32_t* row_order, const int
   const int blocks = (n_groups + 3) / 4;
   const int64_t pieces = nnz * (tile_bytes / 16);
   Launches on(st);
-  on.run(group_rows_kernel, (unsigned)((n_groups * kMaxGroupRows + 255) / 256), 256, row_order, nbr, n_groups, group_rows);
+  on.run(group_rows_kernel, (unsigned)((n_groups * kMaxGroupRows + 255) / 256), 256, row_order, nbr, each, n_experts, group_rows);
   on.run(group_walk_kernel<false>, (unsigned)blocks, 128, row_ptr, tile_cols, group_rows, n_groups, max_entries, max_tiles,
          nullptr, nullptr, counts, nullptr, nullptr, nnz, nullptr);
   on.run(group_scan_kernel, 1, 1024, counts, row_ptr, group_rows, n_groups, stage_ptr, tile_base);
@@ -663,8 +708,44 @@ int void_group_build(const int32_t* row_ptr, const int32_t* row_order, const int
   return on.status();
 }
 
+}  // namespace
+
+}  // namespace vb
+
+extern "C" {
+
+int void_group_build(const int32_t* row_ptr, const int32_t* row_order, const int32_t* tile_cols, const void* tiles, int32_t nbr,
+                     int64_t nnz, int32_t elem_bytes, int32_t n_groups, int32_t max_entries, int32_t max_tiles,
+                     int32_t* group_rows, int32_t* stage_ptr, int32_t* records, void* blob, int32_t* ws, void_stream_t stream) {
+  return vb::group_build(row_ptr, row_order, tile_cols, tiles, nbr, 1, nnz, elem_bytes, n_groups, max_entries, max_tiles, group_rows, stage_ptr,
+                         records, blob, ws, stream);
+}
+int void_expert_group_build(const int32_t* row_ptr, const int32_t* row_order, const int32_t* tile_cols, const void* tiles, int32_t nbr,
+                            int32_t n_experts, int64_t nnz, int32_t elem_bytes, int32_t n_groups, int32_t max_entries, int32_t max_tiles,
+                            int32_t* group_rows, int32_t* stage_ptr, int32_t* records, void* blob, int32_t* ws, void_stream_t stream) {
+  return vb::group_build(row_ptr, row_order, tile_cols, tiles, nbr, n_experts, nnz, elem_bytes, n_groups, max_entries, max_tiles, group_rows,
+                         stage_ptr, records, blob, ws, stream);
+}
+
 int void_spmm_grouped(const void_spmm_args* a, const void_group_store* s, int32_t kind, void_stream_t stream) {
   return vb::spmm_grouped(a, s, kind, nullptr, stream);
+}
+int void_expert_grouped(const void_spmm_args* a, const void_epilogue* e, const void_experts* x, const void_group_store* s, int32_t kind,
+                        void_stream_t stream) {
+  using namespace vb;
+  if (a == nullptr || x == nullptr || s == nullptr) return VOID_ERR_BAD_ARG;
+  if (x->plan == nullptr || x->n_experts < 1 || x->chunk != kPanelN || a->transposed != 1 || kind == VOID_KIND_I8) return VOID_ERR_BAD_ARG;
+  if (a->row_scale != nullptr || a->col_scale != nullptr || a->bias != nullptr) return VOID_ERR_BAD_ARG;
+  Tail tail = {};
+  if (e != nullptr) {
+    const int st = make_tail(a, e, &tail);
+    if (st != VOID_OK) return st;
+    if (e->residual != nullptr) return VOID_ERR_BAD_ARG;
+  }
+  if (a->M == 0 || a->N == 0) return VOID_OK;
+  const PlanView v = plan_of(*x, a->N);
+  const ExpertParams experts = {tail, v.head, v.bounds, v.chunks, nullptr, x->n_experts, x->zero_rest};
+  return spmm_grouped(a, s, kind, nullptr, stream, &experts, v.capacity);
 }
 int void_spmm_grouped_linear(const void_spmm_args* a, const void_epilogue* e, const void_group_store* s, int32_t kind, void_stream_t stream) {
   vb::Tail tail;

@@ -152,6 +152,7 @@ struct GroupStore {
   void_group_store store = {};
   cudaEvent_t built = nullptr;   // behind the kernels that write it; null once it is known to be complete
   bool captured = false;         // a graph reads it
+  int32_t experts = 0;           // weights of experts whose rows are not mixed; 0: one matrix
   Readers readers;
   GroupStore() = default;
   GroupStore(const GroupStore&) = delete;
@@ -399,9 +400,21 @@ struct GroupShape {
   int groups = 0;
   double saves = 0.0;
 };
-double group_saves(const Packed* p, int64_t N, int groups, int slots) {
-  const int es = elem_bytes(p->kind);
-  const double chunks = (double)((N + 127) / 128), nbr = p->args.nbr, nbc = p->args.nbc, nnz = (double)p->args.nnz;
+// What is multiplied: one weight (of experts: one of them) with chunks of 128 columns (of all experts).
+struct GroupLoad {
+  int es;
+  double nbr, nbc, nnz, chunks;
+  double density() const { return nnz / (nbr * nbc); }
+};
+GroupLoad group_load(const Packed* p, int64_t N, int32_t experts) {
+  const double n = experts > 0 ? experts : 1;
+  // (a run ends with half a chunk)
+  const double chunks = experts > 0 ? std::ceil((double)N / 128 + n / 2) : (double)((N + 127) / 128);
+  return {elem_bytes(p->kind), p->args.nbr / n, (double)p->args.nbc, (double)p->args.nnz / n, chunks};
+}
+double group_saves(const GroupLoad& w, int groups, int slots) {
+  const int es = w.es;
+  const double chunks = w.chunks, nbr = w.nbr, nbc = w.nbc, nnz = w.nnz;
   const double d = nnz / (nbr * nbc), panel = 4.0 * es, tile = es;
   const double rows = std::ceil(nbr / groups), turns = std::ceil(groups * chunks / slots);
   double cost = turns * nbc * ((1.0 - std::pow(1.0 - d, rows)) * panel + d * rows * tile);
@@ -431,16 +444,16 @@ void stage_shape(void_group_store& s, double tiles_per_column, int es) {
     }
   }
 }
-GroupShape group_shape(const Packed* p, int64_t N, int slots) {
+GroupShape group_shape(const GroupLoad& w, int slots) {
   GroupShape best;
-  const int64_t chunks = (N + 127) / 128, nbr = p->args.nbr;
+  const int64_t chunks = (int64_t)w.chunks, nbr = (int64_t)w.nbr;
   for (int64_t turns = 1; turns <= 256; ++turns) {
     const int64_t groups = turns * slots / chunks;
     if (groups < 1) continue;
     const int64_t rows = (nbr + groups - 1) / groups;
     if (rows > 8) continue;
     if (rows < 2) break;
-    const double saves = group_saves(p, N, (int)groups, slots);
+    const double saves = group_saves(w, (int)groups, slots);
     if (saves > best.saves) {
       best.saves = saves;
       best.groups = (int)groups;
@@ -466,9 +479,9 @@ double group_line(const Packed* p) {
 // 512 tokens 4096^2 80 % 12.4 14.7 11.3.  Predicted saving and gain: 0.90 (90 %) 1.03, 0.94 (80 %) 1.10, 0.97 - 0.99 (90 %) 0.99 - 1.04, 0.99 (70 %) 1.14,
 // 1.06 (90 %) 1.05, 1.12 (90 %) 1.05, 1.41 (80 %) 1.33; at 95 % 0.97 - 1.05 whatever is predicted.  fp32: 1.12 1.01, 1.24 0.99, 1.27 1.06, 1.36 1.28,
 // 1.41 1.13, 1.93 1.51.  INT8 (32-byte pieces) 8192^2, 60 %, 1024 tokens 109, on a copy 52 and in groups of the copy 40, groups 49: copied.
-bool groups_of_tokens(const Packed* p, double saves) {
-  if (p->kind == VOID_KIND_TF32) return saves >= 1.25;
-  return (p->kind == VOID_KIND_F16 || p->kind == VOID_KIND_BF16) && saves >= 0.93 && p->args.nnz * 12.5 >= (double)p->args.nbr * p->args.nbc;
+bool groups_of_tokens(int32_t kind, double density, double saves) {
+  if (kind == VOID_KIND_TF32) return saves >= 1.25;
+  return (kind == VOID_KIND_F16 || kind == VOID_KIND_BF16) && saves >= 0.93 && density >= 0.08;
 }
 // Whether the kernels that write the store are through.  Asked without waiting; not while the stream is captured, where the
 // store then is not used.  (Another thread may be capturing: relaxed mode keeps the question from ending its capture.)
@@ -485,9 +498,12 @@ bool complete(GroupStore* g, void_stream_t st) {
   return true;
 }
 int64_t group_blob_bytes(const Packed* p) { return p->args.nnz * (1024 * (int64_t)elem_bytes(p->kind) + VOID_GROUP_HEAD_BYTES); }
-// Queues the kernels that lay the tiles out for G groups; null where there is no memory for it.
-std::unique_ptr<GroupStore> build_group_store(const Packed* p, int64_t G, void_stream_t st) {
+// Queues the kernels that lay the tiles out for G groups; null where there is no memory for it.  experts: the groups of all of them, their
+// rows in the order `order` (else of the store).
+std::unique_ptr<GroupStore> build_group_store(const Packed* p, int64_t G, int32_t experts, const int32_t* order, void_stream_t st) {
   std::unique_ptr<GroupStore> g(new GroupStore);
+  g->experts = experts;
+  const int32_t n = experts > 0 ? experts : 1;
   const int64_t nnz = p->args.nnz, es = elem_bytes(p->kind);
   at::Tensor ws;
   try {
@@ -505,11 +521,12 @@ std::unique_ptr<GroupStore> build_group_store(const Packed* p, int64_t G, void_s
   g->store.stage_ptr = stages;
   g->store.group_rows = rows;
   g->store.n_groups = (int32_t)G;
-  const double d = (double)nnz / ((double)p->args.nbr * p->args.nbc), in_group = std::ceil((double)p->args.nbr / (double)G);
+  const double d = (double)nnz / ((double)p->args.nbr * p->args.nbc), in_group = std::ceil((double)(p->args.nbr / n) / (double)(G / n));
   stage_shape(g->store, in_group * d / (1.0 - std::pow(1.0 - d, in_group)), (int)es);
   if (cudaEventCreateWithFlags(&g->built, cudaEventDisableTiming) != cudaSuccess) return nullptr;
-  check(void_group_build(p->args.row_ptr, p->row_order, p->args.tile_cols, p->args.tiles, p->args.nbr, nnz, (int32_t)es, (int32_t)G,
-                         g->store.max_entries, g->store.max_tiles, rows, stages, records, blob, ws.data_ptr<int32_t>(), st),
+  check(void_expert_group_build(p->args.row_ptr, experts > 0 ? order : p->row_order, p->args.tile_cols, p->args.tiles, p->args.nbr / n, n, nnz,
+                                (int32_t)es, (int32_t)G, g->store.max_entries, g->store.max_tiles, rows, stages, records, blob,
+                                ws.data_ptr<int32_t>(), st),
         "void_group_build");
   if (cudaEventRecord(g->built, reinterpret_cast<cudaStream_t>(st)) != cudaSuccess) throw std::runtime_error("CUDA error: recording an event failed");
   return g;
@@ -517,26 +534,29 @@ std::unique_ptr<GroupStore> build_group_store(const Packed* p, int64_t G, void_s
 // The group store that serves this product, or null.  Its build is queued behind the third product it would have served - a
 // tensor that is multiplied once or twice does not pay for it - once for each of up to two widths.  Nothing waits for it:
 // products go to the other kernel until it is complete, and then read it on any stream and ahead of their stream's order.
-// tokens: for a linear layer that reads them as they lie.
-GroupStore* group_store(Packed* p, int64_t N, void_stream_t st, bool tokens = false) {
+// tokens: for a linear layer that reads them as they lie; experts: for that of so many experts, their rows in the order `order`.
+GroupStore* group_store(Packed* p, int64_t N, void_stream_t st, bool tokens = false, int32_t experts = 0, const int32_t* order = nullptr) {
   if (!p->grouped || N <= 64 || p->args.nnz < (tokens ? 512 : 4096) || p->kind == VOID_KIND_F8E4M3) return nullptr;   // (FP8 of two terms: within 5 % either way)
   const int slots = 2 * void_device_sm_count();
-  if ((int64_t)p->args.nbr * ((N + 127) / 128) < (tokens ? 1ll : 2ll) * slots) return nullptr;
-  const GroupShape shape = group_shape(p, N, slots);
-  auto pays = [&](double saves) { return tokens ? groups_of_tokens(p, saves) : saves >= group_line(p); };
+  const GroupLoad w = group_load(p, N, experts);
+  if (w.nbr * w.chunks < (tokens ? 1.0 : 2.0) * slots) return nullptr;
+  const GroupShape shape = group_shape(w, slots);
+  auto pays = [&](double saves) { return tokens ? groups_of_tokens(p->kind, w.density(), saves) : saves >= group_line(p); };
   if (!pays(shape.saves)) return nullptr;
+  const int32_t weights = experts > 0 ? experts : 1;
   GroupStore* hit = nullptr;
   double hit_saves = 0.0, best = 0.0;   // best: of those that are still being built, too
   int n = 0;
   for (; n < kMaxGroupStores && p->groups[n] != nullptr; ++n) {
-    const double saves = group_saves(p, N, p->groups[n]->store.n_groups, slots);
+    if (p->groups[n]->experts != experts) continue;
+    const double saves = group_saves(w, p->groups[n]->store.n_groups / weights, slots);
     best = std::max(best, saves);
     if (saves > hit_saves && complete(p->groups[n].get(), st)) { hit = p->groups[n].get(); hit_saves = saves; }
   }
   if (best < 0.93 * shape.saves && n < kMaxGroupStores && p->stable && group_blob_bytes(p) <= (4ll << 30) && p->group_calls >= 0 && !capturing(st) &&
       ++p->group_calls >= 3) {
     p->group_calls = -1;   // for good, if there is no room for it
-    p->groups[n] = build_group_store(p, shape.groups, st);
+    p->groups[n] = build_group_store(p, (int64_t)shape.groups * weights, experts, order, st);
     if (p->groups[n] != nullptr) p->group_calls = 0;
   }
   return pays(hit_saves) ? hit : nullptr;
@@ -1502,7 +1522,15 @@ PyObject* expert_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     plan.x.row_order = order.const_data_ptr<int32_t>();
   }
   plan.x.zero_rest = none(a[7]) ? 1 : 0;
-  check(void_expert_linear(&s, &tail, &plan.x, pk->kind, launch_stream(pk)), "void_expert_linear");
+  const void_stream_t st = launch_stream(pk);
+  GroupStore* g = plan.x.chunk == 128 ? group_store(pk, N, st, true, (int32_t)experts, plan.x.row_order) : nullptr;
+  if (g != nullptr) {
+    g->readers.add(c10::cuda::getCurrentCUDAStream(pk->device), {&g->index, &g->blob});
+    if (pk->captured && capturing(st)) g->captured = true;
+    check(void_expert_grouped(&s, &tail, &plan.x, &g->store, pk->kind, st), "void_expert_grouped");
+  } else {
+    check(void_expert_linear(&s, &tail, &plan.x, pk->kind, st), "void_expert_linear");
+  }
   if (!none(a[7])) {
     Py_INCREF(a[7]);
     return a[7];

@@ -184,20 +184,6 @@ __device__ __forceinline__ void stamp(const SpmmParams& p, int slot) {
   }
 }
 
-// A product whose weight is one of several experts', each multiplied with its own run of tokens (B and C transposed): work items are
-// (chunk of an expert's tokens, tile row), chunks as laid out by expert_plan_kernel (experts.cu).
-struct ExpertParams {
-  Tail tail;
-  const int32_t* head;        // number of chunks
-  const int32_t* bounds;      // [experts + 1]: where the experts' runs of tokens begin, and the end of the last
-  const int4* chunks;         // expert, first token, token behind the last
-  const int32_t* row_order;   // [experts][tile rows]: tile row of the k-th row taken, or null for k
-  int n_experts, zero_rest;   // zero_rest: tokens outside all runs get zeros
-};
-struct Nothing {};
-template <class X>
-constexpr bool kExpertsOf = std::is_same<X, ExpertParams>::value;
-
 struct Seg {
   int row, chunk, t0, t1, nseg, slot0, my_idx, ctr;
   int n0, n1;   // experts: tokens of the chunk

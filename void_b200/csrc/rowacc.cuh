@@ -36,18 +36,6 @@ __device__ __forceinline__ decltype(auto) runs_of(const X& x) {
   if constexpr (EXPERTS) return (x);
   else return Nothing{};
 }
-// Zeros for the tokens in no expert's run, dealt out over the CTAs.
-__device__ __forceinline__ void zero_rest_rows(const SpmmParams& p, const ExpertParams& x, int tid, int threads) {
-  const int before = x.bounds[0], behind = x.bounds[x.n_experts], rest = before + p.N - behind;
-  for (int i = blockIdx.x; i < rest; i += gridDim.x) {
-    const size_t first = (size_t)(i < before ? i : i - before + behind) * (size_t)p.ldc;
-    if (p.out_dtype == VOID_OUT_F32)
-      for (int c = tid; c < p.M; c += threads) reinterpret_cast<float*>(p.out)[first + c] = 0.0f;
-    else
-      for (int c = tid; c < p.M; c += threads) reinterpret_cast<uint16_t*>(p.out)[first + c] = 0;
-  }
-}
-
 // TR: 1 = B and C transposed ([N, K] and [N, M]), 2 = C alone.  EPI: what the epilogue is asked for (kStaged ...).  What is not run
 // costs a little too, in spilled registers and in instructions fetched around it: INT8 4096^2, 90 %, N = 512, fp16 results 6.10 us,
 // through the kernel that also splits rows and activates 6.20; with GELU 6.57, through that kernel 6.60.
@@ -191,7 +179,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) spmm_rowacc_kernel
     if (begin < end) seg_next = load_seg_word<SPLIT>(p, begin, lane, runs);
     if (p.a_stable) grid_dependency_wait();
     if constexpr (EXPERTS)
-      if (x.zero_rest) zero_rest_rows(p, x, epi_tid, C::EPI_THREADS);
+      if (x.zero_rest) zero_rest_rows(od, x, epi_tid, C::EPI_THREADS);
     if (epi_tid == 0) stamp<TRACE>(p, 0);
     for (int i = begin; i < end; i += step, ++it) {
       const int seg = seg_next;
