@@ -368,10 +368,24 @@ __device__ __forceinline__ void add16(const void* from, int dtype, size_t first,
     }
   }
 }
-// finish16_tr with the rest of a linear layer: z = dequantised accumulator + bias, kept where asked; act(z) + residual.
+// The residual of a tile row's 32 columns, asked for before the accumulators are there: 16-bit ones that lie in whole sectors.
+struct Ahead {
+  uint32_t w[16];
+  bool valid;
+  __device__ __forceinline__ void load(const OutDesc& o, const Tail& t, int row, int n) {
+    const uint16_t* src = reinterpret_cast<const uint16_t*>(t.residual) + (size_t)n * t.ldr + row * kTile;
+    valid = t.residual != nullptr && t.residual_dtype != VOID_OUT_F32 && n < o.N && row * kTile + kTile <= o.M && (reinterpret_cast<uintptr_t>(src) & 31u) == 0;
+    if (valid) {
+      ld_global_v8(src, *reinterpret_cast<uint32_t(*)[8]>(w));
+      ld_global_v8(src + 16, *reinterpret_cast<uint32_t(*)[8]>(w + 8));
+    }
+  }
+};
+// finish16_tr with the rest of a linear layer: z = dequantised accumulator + bias, kept where asked; act(z) + residual.  ahead: the
+// residual where it is there already.
 template <int KIND>
 __device__ __forceinline__ void finish16_tail(const OutDesc& o, const Tail& t, int row, int n, int m0, const uint32_t* r, float row_scale,
-                                              float cs, float bias_n) {
+                                              float cs, float bias_n, const uint32_t* ahead = nullptr) {
   if (n >= o.N) return;
   const int c0 = row * kTile + m0, cols = o.M - c0;
   if (cols <= 0) return;
@@ -387,7 +401,16 @@ __device__ __forceinline__ void finish16_tail(const OutDesc& o, const Tail& t, i
 #pragma unroll
     for (int k = 0; k < 8; ++k) unpair(x[k], v[2 * k], v[2 * k + 1]);
   }
-  if (t.residual != nullptr) add16(t.residual, t.residual_dtype, (size_t)n * t.ldr + c0, cols, v);
+  if (ahead != nullptr) {
+    const bool f16 = t.residual_dtype == VOID_OUT_F16;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      v[2 * k] += f16_value(ahead[k] & 0xffffu, f16);
+      v[2 * k + 1] += f16_value(ahead[k] >> 16, f16);
+    }
+  } else if (t.residual != nullptr) {
+    add16(t.residual, t.residual_dtype, (size_t)n * t.ldr + c0, cols, v);
+  }
   store16_row(o.out, o.dtype, (size_t)n * o.ldc + c0, cols, v);
 }
 

@@ -52,7 +52,10 @@ constexpr int kHeadBytes = 16;       // of a stage, per class: its first tile, i
 constexpr int kMaxRuns = kHeadBytes - 2;
 static_assert(kClasses * kHeadBytes == VOID_GROUP_HEAD_BYTES, "room for the heads of as many stages as there are tiles");
 constexpr int kMaxRing = 12;
-constexpr int kThreads = 32 * (kProducers + kClasses + kEpiWarps);
+// Warps that finish rows: one per lane quadrant of tensor memory, of tokens as they lie two, which take the rows of a group in turn (results
+// leave straight from registers there, so that another four warps take no shared memory).
+__host__ __device__ constexpr int epilogue_warps(bool trb) { return trb ? 2 * kEpiWarps : kEpiWarps; }
+__host__ __device__ constexpr int threads_of(bool trb) { return 32 * (kProducers + kClasses + epilogue_warps(trb)); }
 constexpr int kNone = 0x7fffffff;
 
 constexpr int kPartBytes = 32 * 32 * 2;   // staging of a 32 x 32 part of 16-bit results
@@ -109,8 +112,9 @@ __device__ __forceinline__ int items_of(const GroupParams& p, const X& x) {
 // TRB: B stored transposed, [N, K], and C with it: tokens as they lie.  X: Tail, results [N, M] of a linear layer with one; ExpertParams,
 // the same for every expert's tokens (with TRB); or Nothing.
 template <int KIND, bool TRB, class X>
-__global__ void __launch_bounds__(kThreads, kCtas) group_kernel(const __grid_constant__ CUtensorMap tmap_b,
+__global__ void __launch_bounds__(threads_of(TRB), kCtas) group_kernel(const __grid_constant__ CUtensorMap tmap_b,
                                                             const __grid_constant__ X x, const __grid_constant__ GroupParams p) {
+  constexpr int EW = epilogue_warps(TRB), TURNS = EW / 4;
   constexpr bool EXPERTS = kExpertsOf<X>, TAIL = std::is_same<X, Tail>::value;
   static_assert(!EXPERTS || TRB, "tokens as they lie");
   extern __shared__ uint8_t smem_raw[];
@@ -136,7 +140,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) group_kernel(const __grid_con
     for (int b = 0; b < 2; ++b)
       for (int c = 0; c < kClasses; ++c) {
         mbar_init(smem_u32(&bars.acc_full[b][c]), 1);
-        mbar_init(smem_u32(&bars.acc_empty[b][c]), 4);
+        mbar_init(smem_u32(&bars.acc_empty[b][c]), EW);
       }
     fence_mbar_init();
     prefetch_tmap(&tmap_b);
@@ -288,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) group_kernel(const __grid_con
     const uint32_t part = ring + (uint32_t)p.stages * (uint32_t)p.stage_bytes + (uint32_t)(warp - kEpiWarp0) * kPartBytes;
     grid_dependency_wait();
     if constexpr (EXPERTS)
-      if (x.zero_rest) zero_rest_rows(od, x, (int)threadIdx.x - 32 * kEpiWarp0, 32 * kEpiWarps);
+      if (x.zero_rest) zero_rest_rows(od, x, (int)threadIdx.x - 32 * kEpiWarp0, 32 * EW);
     uint32_t it = 0;
     bool ok = true;
     const int n_items = items_of(p, x);
@@ -314,15 +318,28 @@ __global__ void __launch_bounds__(kThreads, kCtas) group_kernel(const __grid_con
         if (p.col_scale != nullptr) cs *= p.col_scale[n];
         if (p.bias != nullptr) bias = p.bias[n];
       }
+      // the residual of this warp's next row, asked for while the products run or the row before is finished
+      Ahead ahead;
+      auto ask = [&](int r) {
+        ahead.valid = false;
+        if constexpr (TAIL) {
+          const int row = r < p.rows ? __shfl_sync(0xffffffffu, my_row, r & 31) : -1;
+          if (row >= 0) ahead.load(od, x, row, n);
+        }
+      };
+      ask((warp - kEpiWarp0) / 4);
 #pragma unroll 1
       for (int cls = 0; cls < p.classes; ++cls) {
         ok = mbar_wait_warp(smem_u32(&bars.acc_full[buf][cls]), use & 1u, ctl);
         if (!ok) break;
         tc_fence_after();
 #pragma unroll 1
-        for (int r = cls * kClassRows; r < (cls + 1) * kClassRows && r < p.rows; ++r) {
+        for (int r = cls * kClassRows + (warp - kEpiWarp0) / 4; r < (cls + 1) * kClassRows && r < p.rows; r += TURNS) {
           const int row = __shfl_sync(0xffffffffu, my_row, r);
-          if (row < 0) continue;
+          if (row < 0) {
+            ask(r + TURNS);
+            continue;
+          }
           const int has = __shfl_sync(0xffffffffu, my_has, r);
           const float rs = __shfl_sync(0xffffffffu, my_scale, r);
           const uint32_t acc = tmem_base + lane_sel + buf * (uint32_t)buf_cols + (uint32_t)(r * kTile);
@@ -363,8 +380,9 @@ __global__ void __launch_bounds__(kThreads, kCtas) group_kernel(const __grid_con
               finish16_tail<KIND>(to, x.tail, own, n, 0, &v[0], rs, cs, bias);
               finish16_tail<KIND>(to, x.tail, own, n, 16, &v[16], rs, cs, bias);
             } else if constexpr (TAIL) {
-              finish16_tail<KIND>(od, x, row, n, 0, &v[0], rs, cs, bias);
-              finish16_tail<KIND>(od, x, row, n, 16, &v[16], rs, cs, bias);
+              finish16_tail<KIND>(od, x, row, n, 0, &v[0], rs, cs, bias, ahead.valid ? ahead.w : nullptr);
+              finish16_tail<KIND>(od, x, row, n, 16, &v[16], rs, cs, bias, ahead.valid ? ahead.w + 8 : nullptr);
+              ask(r + TURNS);
             } else if (TRB || p.out_tr) {
               finish16_tr<KIND>(od, row, n, 0, &v[0], rs, cs, bias);
               finish16_tr<KIND>(od, row, n, 16, &v[16], rs, cs, bias);
@@ -572,7 +590,7 @@ template <int KIND, bool TRB, class X>
 int launch_group(const GroupLaunch& l, const X& x) {
   auto kernel = group_kernel<KIND, TRB, X>;
   if (ensure_smem((const void*)kernel, l.smem)) return VOID_ERR_CUDA;
-  return status_of(launch_pdl(kernel, l.grid, kThreads, l.smem, l.stream, l.b, x, l.p));
+  return status_of(launch_pdl(kernel, l.grid, threads_of(TRB), l.smem, l.stream, l.b, x, l.p));
 }
 template <int KIND>
 int launch_group(const GroupLaunch& l) {
