@@ -456,8 +456,8 @@ VOID_API int void_activation_grad(const void* g, int64_t ldg, const void* z, int
  * [0, rows] and not below the one before it, and the status word (where not NULL) reads 3 if one had to be.
  * void_expert_linear: args as for void_spmm_linear with transposed = 1 and a kind of floating tiles, but with the weights of all
  * experts in one packed store, expert behind expert: nbr tile rows, M outputs and K inputs are those of one expert, row_ptr
- * [n_experts * nbr + 1], nnz all tiles, row_bias [n_experts * M] or NULL, N all tokens.  chunk 128, or 8, 16 or 32 (another kernel, for
- * few tokens per expert).  Rows of out in no run are zeroed if zero_rest, else left alone.  epilogue: NULL, or `pre` alone.
+ * [n_experts * nbr + 1], nnz all tiles, row_bias [n_experts * M] or NULL, N all tokens.  chunk 8 (another kernel,
+ * for a handful of tokens per expert), 32, 64 or 128.  Rows of out in no run are zeroed if zero_rest, else left alone.  epilogue: NULL, or `pre` alone.
  * void_expert_tile_grad, void_expert_activation_grad: as void_linear_tile_grad and void_activation_grad, run by run: items name tile rows of
  * all experts (e * ceil(M / 32) + r), dbias is [n_experts, cols]; z and dz may be NULL with VOID_ACT_NONE (then only the sums are
  * taken).  Experts without tokens get zeros.  ws: void_expert_activation_grad_ws_bytes bytes, needed with dbias.

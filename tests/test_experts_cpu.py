@@ -68,7 +68,7 @@ def _linear(args=(), experts=(), tail=None, kind=_lib.KIND_F16):
     (dict(args=dict(segs=1024)), BAD_ARG), (dict(args=dict(acc_out=1024)), BAD_ARG), (dict(args=dict(tile_terms=2)), BAD_ARG),
     (dict(args=dict(n_peers=1)), BAD_ARG), (dict(args=dict(ldc=31)), SHAPE), (dict(args=dict(M=33, ldc=33)), SHAPE),
     (dict(args=dict(ldb=62)), ALIGN), (dict(args=dict(ldb=48)), ALIGN), (dict(args=dict(tiles=1040)), ALIGN), (dict(args=dict(b=1032)), ALIGN),
-    (dict(experts=dict(n_experts=0)), BAD_ARG), (dict(experts=dict(chunk=64)), BAD_ARG), (dict(experts=dict(chunk=0)), BAD_ARG),
+    (dict(experts=dict(n_experts=0)), BAD_ARG), (dict(experts=dict(chunk=48)), BAD_ARG), (dict(experts=dict(chunk=0)), BAD_ARG),
     (dict(experts=dict(plan=None)), BAD_ARG), (dict(experts=dict(plan=1032)), ALIGN),
     (dict(tail=dict(residual=1024, ldr=32)), BAD_ARG), (dict(tail=dict(pre=1024, ldp=31)), BAD_ARG),
     (dict(args=dict(N=2 ** 30, nbr=2 ** 20, M=2 ** 25, ldc=2 ** 25)), TOO_LARGE),

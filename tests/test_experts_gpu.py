@@ -36,14 +36,15 @@ def check_forward(y, weights, x, counts, first, bias, act, untouched=None):
     assert torch.equal(y[rest], expected[rest])
 
 
-# experts, features in and out, tokens per expert, tokens before the first and behind the last run.  The kernels: chunks of 8, 16, 32 and
-# 128 tokens (at most 8, 16, 48 tokens per expert on average, and more); experts that get none, one, all; more experts than a warp
+# experts, features in and out, tokens per expert, tokens before the first and behind the last run.  The kernels: chunks of 8, 32, 64 and
+# 128 tokens (at most 4, 8, 96 tokens per expert on average, and more); experts that get none, one, all; more experts than a warp
 # and than a block of the plan has threads.
 CASES = [
     (1, 64, 32, [1], 0, 0), (1, 96, 200, [300], 0, 0), (3, 70, 45, [0, 5, 2], 0, 0), (4, 256, 512, [9, 0, 0, 1], 0, 3), (4, 333, 100, [0, 60, 1, 0], 2, 1),
     (2, 515, 333, [31, 33], 0, 0), (8, 1024, 640, [0, 700, 1, 129, 128, 127, 0, 3], 0, 0), (5, 128, 64, [128, 256, 0, 1, 130], 7, 60),
     (3, 96, 64, [0, 0, 0], 0, 10), (40, 64, 64, [3, 0, 9, 1] * 10, 0, 0), (70, 64, 33, [100 * (e % 7 == 3) + e % 3 for e in range(70)], 1, 5),
     (1500, 32, 32, [e % 4 for e in range(1500)], 0, 2), (2, 2048, 1000, [1000, 1300], 0, 17),
+    (6, 130, 96, [40, 0, 1, 0, 3, 0], 0, 1), (2, 640, 300, [190, 1], 0, 0), (3, 1500, 90, [20, 2, 0], 1, 0), (2, 1500, 70, [4, 2], 0, 0),
 ]
 
 

@@ -310,6 +310,7 @@ struct ExpertParams {
   const int4* chunks;         // expert, first token, token behind the last
   const int32_t* row_order;   // [experts][tile rows]: tile row of the k-th row taken, or null for k
   int n_experts, zero_rest;   // zero_rest: tokens outside all runs get zeros
+  int panel_bytes;            // of a panel in shared memory (row kernel): as many tokens as a chunk has
 };
 struct Nothing {};
 template <class X>
@@ -368,30 +369,41 @@ __device__ __forceinline__ void add16(const void* from, int dtype, size_t first,
     }
   }
 }
-// The residual of a tile row's 32 columns, asked for before the accumulators are there: 16-bit ones that lie in whole sectors.
+// The residual of COLS columns of a tile row from m0 on, asked for before the accumulators are there: 16-bit ones that lie in whole
+// sectors.
+template <int COLS>
 struct Ahead {
-  uint32_t w[16];
+  uint32_t w[COLS / 2];
   bool valid;
-  __device__ __forceinline__ void load(const OutDesc& o, const Tail& t, int row, int n) {
-    const uint16_t* src = reinterpret_cast<const uint16_t*>(t.residual) + (size_t)n * t.ldr + row * kTile;
+  __device__ __forceinline__ void load(const OutDesc& o, const Tail& t, int row, int n, int m0 = 0) {
+    const uint16_t* src = reinterpret_cast<const uint16_t*>(t.residual) + (size_t)n * t.ldr + row * kTile + m0;
     valid = t.residual != nullptr && t.residual_dtype != VOID_OUT_F32 && n < o.N && row * kTile + kTile <= o.M && (reinterpret_cast<uintptr_t>(src) & 31u) == 0;
-    if (valid) {
-      ld_global_v8(src, *reinterpret_cast<uint32_t(*)[8]>(w));
-      ld_global_v8(src + 16, *reinterpret_cast<uint32_t(*)[8]>(w + 8));
-    }
+    if (valid)
+#pragma unroll
+      for (int k = 0; k < COLS / 2; k += 8) ld_global_v8(src + 2 * k, *reinterpret_cast<uint32_t(*)[8]>(w + k));
   }
 };
-// finish16_tr with the rest of a linear layer: z = dequantised accumulator + bias, kept where asked; act(z) + residual.  ahead: the
-// residual where it is there already.
+// The bias of the lane's row of a tile row, asked for before the accumulators are there: behind them, every row would wait for it, and
+// while weights are on their way that is a microsecond or two.  bias: the first of the layer's (or the expert's).
+__device__ __forceinline__ float bias_of_lane(const float* bias, int dtype, int row, int M) {
+  const int m = row * kTile + (int)(threadIdx.x & 31);
+  if (bias == nullptr || m >= M) return 0.0f;
+  if (dtype == VOID_OUT_F32) return bias[m];
+  return f16_value(reinterpret_cast<const uint16_t*>(bias)[m], dtype == VOID_OUT_F16);
+}
+// finish16_tr with the rest of a linear layer: z = dequantised accumulator + bias, kept where asked; act(z) + residual.  For whole
+// warps: of_lane is bias_of_lane.  ahead: the residual where it is there already.
 template <int KIND>
 __device__ __forceinline__ void finish16_tail(const OutDesc& o, const Tail& t, int row, int n, int m0, const uint32_t* r, float row_scale,
-                                              float cs, float bias_n, const uint32_t* ahead = nullptr) {
-  if (n >= o.N) return;
+                                              float cs, float bias_n, float of_lane, const uint32_t* ahead = nullptr) {
   const int c0 = row * kTile + m0, cols = o.M - c0;
   if (cols <= 0) return;
   float v[16];
   finished<KIND, 8, false>(o, c0, r, row_scale, cs, bias_n, v);
-  if (o.row_bias != nullptr) add16(o.row_bias, t.bias_dtype, c0, cols, v);
+  if (o.row_bias != nullptr)
+#pragma unroll
+    for (int k = 0; k < 16; ++k) v[k] += __shfl_sync(0xffffffffu, of_lane, m0 + k);
+  if (n >= o.N) return;
   if (t.pre != nullptr) store16_row(t.pre, o.dtype, (size_t)n * t.ldp + c0, cols, v);
   if (o.act != VOID_ACT_NONE) {
     f32x2 x[8];

@@ -3,12 +3,11 @@
 //     out_t = act(x_t A_e^T + bias_e)          offsets[e] <= t < offsets[e + 1]
 //
 // The weights are one packed store, expert behind expert; the runs are cut into chunks of tokens on the device (the host does not
-// know the offsets), and a work item is (chunk, tile row).  The products themselves are those of rowacc.cuh (chunks of 128 tokens, B and
-// C as they lie) and, for a handful of tokens per expert, of skinny.cu (chunks of 8, 16 or 32).  A chunk never spans two experts: what a
-// tile load brings beyond its end belongs to rows of the result that are not stored.
+// know the offsets), and a work item is (chunk, tile row).  The products themselves are those of rowacc.cuh (chunks of 32, 64 or 128
+// tokens, B and C as they lie) and, for a handful of tokens per expert, of skinny.cu (chunks of 8).  A chunk never spans two experts: what
+// a tile load brings beyond its end belongs to rows of the result that are not stored.
 #include "experts.cuh"
 #include "pipeline.cuh"
-#include "skinny.cuh"
 
 namespace vb {
 
@@ -94,13 +93,11 @@ __global__ void __launch_bounds__(kPlanThreads) expert_plan_kernel(const O* offs
   grid_launch_dependents();
 }
 
-bool few_tokens(int chunk) { return chunk == 8 || chunk == 16 || chunk == 32; }
-
 int experts_launch(const void_spmm_args* a, const void_epilogue* e, const void_experts* x, int kind, cudaStream_t st) {
   if (a == nullptr || x == nullptr) return VOID_ERR_BAD_ARG;
   if (kind != VOID_KIND_F16 && kind != VOID_KIND_BF16 && kind != VOID_KIND_TF32) return VOID_ERR_BAD_ARG;
   if (a->M < 0 || a->N < 0 || a->K < 0 || a->nbr < 0 || a->nnz < 0 || x->n_experts < 1) return VOID_ERR_BAD_ARG;
-  if (x->chunk != kPanelN && !few_tokens(x->chunk)) return VOID_ERR_BAD_ARG;
+  if (x->chunk != 8 && x->chunk != 32 && x->chunk != 64 && x->chunk != kPanelN) return VOID_ERR_BAD_ARG;
   if (a->M == 0 || a->N == 0) return VOID_OK;
   if (a->out == nullptr || a->row_ptr == nullptr || x->plan == nullptr) return VOID_ERR_BAD_ARG;
   if (a->nnz > 0 && (a->tiles == nullptr || a->tile_cols == nullptr || a->b == nullptr)) return VOID_ERR_BAD_ARG;
@@ -127,31 +124,6 @@ int experts_launch(const void_spmm_args* a, const void_epilogue* e, const void_e
     tail.ldp = e->ldp;
     tail.bias_dtype = e->bias_dtype;
   }
-  if (few_tokens(x->chunk)) {
-    if (v.capacity > 65535) return VOID_ERR_TOO_LARGE;
-    SkinnyExpertParams s = {};
-    s.tiles = reinterpret_cast<const uint8_t*>(a->tiles);
-    s.tile_cols = a->tile_cols;
-    s.row_ptr = a->row_ptr;
-    s.b = reinterpret_cast<const uint8_t*>(a->b);
-    s.ldb = a->ldb;
-    s.K = a->K; s.N = a->N; s.M = a->M;
-    s.b_scale = a->b_scale;
-    s.row_bias = a->row_bias;
-    s.out = a->out;
-    s.ldc = a->ldc;
-    s.out_dtype = a->out_dtype;
-    s.act = a->act;
-    s.terms = 1;
-    s.tail = tail;
-    s.head = v.head;
-    s.bounds = v.bounds;
-    s.chunks = v.chunks;
-    s.n_experts = x->n_experts;
-    s.zero_rest = x->zero_rest;
-    return status_of(skinny_experts_launch(s, kind, a->nbr, a->nnz / ((long long)a->nbr * x->n_experts), x->chunk, v.capacity, st));
-  }
-
   SpmmParams p = {};
   p.tiles = a->nnz > 0 ? reinterpret_cast<const uint8_t*>(a->tiles) : nullptr;
   p.tile_cols = a->tile_cols;
@@ -168,28 +140,36 @@ int experts_launch(const void_spmm_args* a, const void_epilogue* e, const void_e
   p.out_dtype = a->out_dtype;
   p.act = a->act;
   p.status = a->status;
+  p.wait_limit_ms = (a->test_hooks & 0xffff) ? (a->test_hooks & 0xffff) : kDefaultWaitLimitMs;
+  p.drop_group = (a->test_hooks >> 16) & 1;
+  const long long items = (long long)v.capacity * a->nbr;
+  if (items > 0x3fffffff) return VOID_ERR_TOO_LARGE;
+  const bool few = x->chunk == 8;   // another kernel: see skinny.cu
+  CUtensorMap tmap;
+  memset(&tmap, 0, sizeof(tmap));
+  if (a->nnz > 0 && !panel_map_transposed(&tmap, a->b, a->ldb, a->K, a->N, es, x->chunk, !few)) return VOID_ERR_TENSOR_MAP;
+  const int panel = x->chunk * kTile * es;
+  const ExpertParams experts = {tail, v.head, v.bounds, v.chunks, x->row_order, x->n_experts, x->zero_rest, panel};
+  if (few) return expert_stream_launch(p, experts, kind, tmap, items, dev, st);
   p.np = 1;
   p.terms = 1;
-  p.group = es == 2 ? 2 : 1;
-  const int unit = (kPanelBytes + kTileBytes) * es, room = dev.smem_per_sm / Mid::CTAS_PER_SM - 1024 - 640 - 1024;   // as in spmm.cu
+  // The ring takes the shared memory that three CTAs leave each other (as in spmm.cu), in stages of about 20 KB; panels of fewer tokens
+  // leave room for more tiles.  The tensor cores read 128 rows behind the start of every panel, the last one's end with the slack.
+  const int unit = panel + kTileBytes * es, slack = kPanelBytes * es - panel;
+  const int room = dev.smem_per_sm / Mid::CTAS_PER_SM - 1024 - 640 - 1024 - slack;
+  p.group = 2 * (kPanelBytes + kTileBytes) * 2 / unit;
+  if (p.group > 8) p.group = 8;
   p.stages = room / (unit * p.group);
   if (p.stages > 8) p.stages = 8;
   if (p.stages < Mid::PW) return VOID_ERR_SHAPE;
   p.last_group = p.group;
-  p.wait_limit_ms = (a->test_hooks & 0xffff) ? (a->test_hooks & 0xffff) : kDefaultWaitLimitMs;
-  p.drop_group = (a->test_hooks >> 16) & 1;
   p.desc_hi_b = smem_desc_hi(128, 256 * es, kLayoutNone);
   p.desc_hi_a = smem_desc_hi(16, 256 * es, es == 4 ? kLayoutSw128 : kLayoutSw64);
   const uint32_t format = kind == VOID_KIND_TF32 ? 2u : (kind == VOID_KIND_BF16 ? 1u : 0u);
   p.idesc = instr_desc(1, format, format, 0, 0, 128, 32);
-  const ExpertParams experts = {tail, v.head, v.bounds, v.chunks, x->row_order, x->n_experts, x->zero_rest};
-  CUtensorMap tmap;
-  memset(&tmap, 0, sizeof(tmap));
-  if (a->nnz > 0 && !panel_map_transposed(&tmap, a->b, a->ldb, a->K, a->N, es)) return VOID_ERR_TENSOR_MAP;
-  const long long items = (long long)v.capacity * a->nbr;
   int grid = dev.sms * Mid::CTAS_PER_SM;
   if (items < grid) grid = (int)items;
-  const ExpertLaunch l = {grid, p.stages * p.group * unit + 1024, st, tmap, experts, p};
+  const ExpertLaunch l = {grid, p.stages * p.group * unit + slack + 1024, st, tmap, experts, p};
   return kind == VOID_KIND_TF32 ? launch_experts<VOID_KIND_TF32>(l) : launch_experts<VOID_KIND_F16>(l);
 }
 

@@ -299,10 +299,7 @@ __global__ void __launch_bounds__(threads_of(TRB), kCtas) group_kernel(const __g
     for (int i = blockIdx.x; i < n_items && ok; i += gridDim.x, ++it) {
       const Item item = item_of(p, x, i);
       OutDesc to = od;
-      if constexpr (EXPERTS) {
-        to.N = item.n1;
-        if (to.row_bias != nullptr) to.row_bias = bias_of_expert(to.row_bias, x.tail.bias_dtype, item.expert, od.M);
-      }
+      if constexpr (EXPERTS) to.N = item.n1;
       const uint32_t buf = n_buf == 2 ? (it & 1u) : 0u, use = n_buf == 2 ? (it >> 1) : it;
       // this lane's row of the group, with what its epilogue needs; scales and biases of the columns
       const int my_row = lane < p.rows ? p.group_rows[item.g * kMaxGroupRows + lane] : -1;
@@ -318,13 +315,21 @@ __global__ void __launch_bounds__(threads_of(TRB), kCtas) group_kernel(const __g
         if (p.col_scale != nullptr) cs *= p.col_scale[n];
         if (p.bias != nullptr) bias = p.bias[n];
       }
-      // the residual of this warp's next row, asked for while the products run or the row before is finished
-      Ahead ahead;
+      // the residual and the bias of this warp's next row, asked for while the products run or the row before is finished
+      Ahead<kTile> ahead;
+      float of_lane = 0.0f;
       auto ask = [&](int r) {
         ahead.valid = false;
-        if constexpr (TAIL) {
+        if constexpr (TAIL || EXPERTS) {
           const int row = r < p.rows ? __shfl_sync(0xffffffffu, my_row, r & 31) : -1;
-          if (row >= 0) ahead.load(od, x, row, n);
+          if (row < 0) return;
+          if constexpr (EXPERTS) {
+            if (od.row_bias != nullptr)
+              of_lane = bias_of_lane(bias_of_expert(od.row_bias, x.tail.bias_dtype, item.expert, od.M), x.tail.bias_dtype, row - item.expert * p.expert_rows, od.M);
+          } else {
+            of_lane = bias_of_lane(od.row_bias, x.bias_dtype, row, od.M);
+            ahead.load(od, x, row, n);
+          }
         }
       };
       ask((warp - kEpiWarp0) / 4);
@@ -377,11 +382,12 @@ __global__ void __launch_bounds__(threads_of(TRB), kCtas) group_kernel(const __g
             }
             if constexpr (EXPERTS) {
               const int own = row - item.expert * p.expert_rows;
-              finish16_tail<KIND>(to, x.tail, own, n, 0, &v[0], rs, cs, bias);
-              finish16_tail<KIND>(to, x.tail, own, n, 16, &v[16], rs, cs, bias);
+              finish16_tail<KIND>(to, x.tail, own, n, 0, &v[0], rs, cs, bias, of_lane);
+              finish16_tail<KIND>(to, x.tail, own, n, 16, &v[16], rs, cs, bias, of_lane);
+              ask(r + TURNS);
             } else if constexpr (TAIL) {
-              finish16_tail<KIND>(od, x, row, n, 0, &v[0], rs, cs, bias, ahead.valid ? ahead.w : nullptr);
-              finish16_tail<KIND>(od, x, row, n, 16, &v[16], rs, cs, bias, ahead.valid ? ahead.w + 8 : nullptr);
+              finish16_tail<KIND>(od, x, row, n, 0, &v[0], rs, cs, bias, of_lane, ahead.valid ? ahead.w : nullptr);
+              finish16_tail<KIND>(od, x, row, n, 16, &v[16], rs, cs, bias, of_lane, ahead.valid ? ahead.w + 8 : nullptr);
               ask(r + TURNS);
             } else if (TRB || p.out_tr) {
               finish16_tr<KIND>(od, row, n, 0, &v[0], rs, cs, bias);
@@ -762,7 +768,7 @@ int void_expert_grouped(const void_spmm_args* a, const void_epilogue* e, const v
   }
   if (a->M == 0 || a->N == 0) return VOID_OK;
   const PlanView v = plan_of(*x, a->N);
-  const ExpertParams experts = {tail, v.head, v.bounds, v.chunks, nullptr, x->n_experts, x->zero_rest};
+  const ExpertParams experts = {tail, v.head, v.bounds, v.chunks, nullptr, x->n_experts, x->zero_rest, 0};
   return spmm_grouped(a, s, kind, nullptr, stream, &experts, v.capacity);
 }
 int void_spmm_grouped_linear(const void_spmm_args* a, const void_epilogue* e, const void_group_store* s, int32_t kind, void_stream_t stream) {

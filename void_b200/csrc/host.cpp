@@ -1445,10 +1445,18 @@ struct ExpertPlan {
   at::Tensor words;
   void_experts x = {};
 };
-// Tokens per chunk, which chooses the kernel: see experts.cu.
+// Tokens per chunk, which chooses the kernel, by the tokens that an expert has on average (the host does not know the runs; a popular
+// expert has several times as many).  A chunk too small reads its weights again for every further one, a chunk too large multiplies
+// rows of the result that are not there.  us, 8 experts of 2048 -> 8192, fp16, 80 %, popular ones up to three times the average
+// (128: without groups of tile rows, which need more tokens):
+//   tokens    8     32    64    128   256   512   1024
+//   8        15.9  20.4  23.2  32.8  61.5  111   209
+//   32       23.0  21.3  21.4  23.5  28.6  37.7  58.7
+//   64       31.6  22.6  22.7  22.8  26.4  29.1  39.1
+//   128      52.2  28.3  27.5  33.5  34.6  41.4  34.5
 int32_t expert_chunk(int64_t rows, int64_t experts) {
   const int64_t each = (rows + experts - 1) / experts;
-  return each <= 8 ? 8 : (each <= 16 ? 16 : (each <= 48 ? 32 : 128));
+  return each <= 4 ? 8 : (each <= 8 ? 32 : (each <= 96 ? 64 : 128));
 }
 ExpertPlan expert_plan(const at::Tensor& offsets_in, int64_t rows, int64_t experts, c10::Device dev, int32_t* status) {
   if (offsets_in.dim() != 1 || offsets_in.size(0) != experts + 1)

@@ -142,17 +142,18 @@ inline bool panel_map(CUtensorMap* m, const void* b, int64_t ldb, int K, int N, 
   return enc(m, dt, 2, const_cast<void*>(b), gdim, gstride, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
              CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-// B stored [N, K]: dim0 = k, dim1 = n; box 32 k x 128 n, swizzle span = the 32 * es bytes of a row
-inline bool panel_map_transposed(CUtensorMap* m, const void* b, int64_t ldb, int K, int N, int es) {
+// B stored [N, K]: dim0 = k, dim1 = n; box 32 k x 128 n (or fewer), swizzle span = the 32 * es bytes of a row (or none)
+inline bool panel_map_transposed(CUtensorMap* m, const void* b, int64_t ldb, int K, int N, int es, int rows = kPanelN, bool swizzled = true) {
   PFN_cuTensorMapEncodeTiled_v12000 enc = get_encode();
   if (enc == nullptr) return false;
   const CUtensorMapDataType dt = (es == 1) ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                  : (es == 2) ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT32;
   const cuuint64_t gdim[2] = {(cuuint64_t)K, (cuuint64_t)N};
   const cuuint64_t gstride[1] = {(cuuint64_t)ldb};
-  const cuuint32_t box[2] = {(cuuint32_t)kTile, (cuuint32_t)kPanelN};
+  const cuuint32_t box[2] = {(cuuint32_t)kTile, (cuuint32_t)rows};
   const cuuint32_t estride[2] = {1, 1};
-  const CUtensorMapSwizzle sw = (es == 4) ? CU_TENSOR_MAP_SWIZZLE_128B
+  const CUtensorMapSwizzle sw = !swizzled ? CU_TENSOR_MAP_SWIZZLE_NONE
+                                : (es == 4) ? CU_TENSOR_MAP_SWIZZLE_128B
                                 : (es == 2) ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
   return enc(m, dt, 2, const_cast<void*>(b), gdim, gstride, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
              CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;

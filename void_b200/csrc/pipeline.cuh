@@ -186,35 +186,71 @@ __device__ __forceinline__ void stamp(const SpmmParams& p, int slot) {
 
 struct Seg {
   int row, chunk, t0, t1, nseg, slot0, my_idx, ctr;
-  int n0, n1;   // experts: tokens of the chunk
+  int n0, n1, expert;   // experts: tokens of the chunk, and whose they are
 };
-// Item i of a product of experts, as words in the order row, chunk, first and last tile, tokens, expert.
-__device__ __forceinline__ void expert_item(const SpmmParams& p, const ExpertParams& x, int i, int& row, int& at, int4& c, int& chunk) {
-  chunk = i / p.nbr;
-  row = i - chunk * p.nbr;
-  c = x.chunks[chunk];
-  at = c.x * p.nbr;
-  if (x.row_order != nullptr) {
-    const int r = x.row_order[at + row];
-    row = r < 0 ? 0 : (r >= p.nbr ? p.nbr - 1 : r);
-  }
-  at += row;
+// What a product of experts reads in small pieces on its way - the index of the weights and the biases - comes into the second cache
+// while the kernel before it ends: asked for when the items reach it, each piece is a trip to memory behind the weights that are on
+// their way, two microseconds for every item of a CTA.  (A prefetch reads nothing, so it may come before the wait on that kernel.)
+__device__ __forceinline__ void warm_lines(const void* from, long long bytes) {
+  const long long step = (long long)gridDim.x * blockDim.x * 128;
+  for (long long at = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * 128; at < bytes; at += step)
+    prefetch_l2(reinterpret_cast<const uint8_t*>(from) + at);
 }
+__device__ __forceinline__ void warm_index(const SpmmParams& p, const ExpertParams& x) {
+  const long long rows = (long long)x.n_experts * p.nbr;
+  warm_lines(p.row_ptr, rows * 4 + 4);
+  if (x.row_order != nullptr) warm_lines(x.row_order, rows * 4);
+  if (p.tiles != nullptr) warm_lines(p.tile_cols, (long long)p.nnz * 4);
+  if (p.row_bias != nullptr) warm_lines(p.row_bias, (long long)x.n_experts * p.M * (x.tail.bias_dtype == VOID_OUT_F32 ? 4 : 2));
+}
+// Items of a product of experts, (chunk of tokens, tile row).  What is known of one comes through a chain of loads (the chunk, the row taken,
+// its tiles) as long as the item's own work where tokens are few, so a warp takes the next 32 items' together, one per lane.
+struct ExpertItems {
+  int row = 0, t0 = 0, t1 = 0, n0 = 0, n1 = 0, expert = 0;   // of the lane's item
+  int ready = 0;                                              // items still to be given out of those taken
+  // the item given next, i; step and end: of the CTA's items
+  __device__ __forceinline__ Seg next(const SpmmParams& p, const ExpertParams& x, int i, int step, int end) {
+    const int lane = threadIdx.x & 31;
+    if (ready == 0) {
+      ready = 32;
+      const long long mine = (long long)i + (long long)lane * step;
+      if (mine < end) {
+        const int c = (int)mine / p.nbr, k = (int)mine - c * p.nbr;
+        const int4 chunk = x.chunks[c];
+        expert = chunk.x;
+        n0 = chunk.y;
+        n1 = chunk.z;
+        row = k;
+        if (x.row_order != nullptr) {
+          const int r = x.row_order[(size_t)expert * p.nbr + k];
+          row = r < 0 ? 0 : (r >= p.nbr ? p.nbr - 1 : r);
+        }
+        const int32_t* at = p.row_ptr + (size_t)expert * p.nbr + row;
+        t0 = at[0];
+        t1 = at[1];
+      }
+    }
+    const int from = 32 - ready--;
+    Seg s = {};
+    s.row = __shfl_sync(0xffffffffu, row, from);
+    s.t0 = __shfl_sync(0xffffffffu, t0, from);
+    s.t1 = __shfl_sync(0xffffffffu, t1, from);
+    s.n0 = __shfl_sync(0xffffffffu, n0, from);
+    s.n1 = __shfl_sync(0xffffffffu, n1, from);
+    s.expert = __shfl_sync(0xffffffffu, expert, from);
+    s.nseg = 1;
+    return s;
+  }
+};
+struct NoItems {};
+template <class X>
+using ItemsOf = std::conditional_t<kExpertsOf<X>, ExpertItems, NoItems>;
 
 // PLAN: the launch may come with a work plan.
-template <bool PLAN, class X = Nothing>
-__device__ __forceinline__ Seg load_seg(const SpmmParams& p, int i, const X& x = X{}) {
+template <bool PLAN>
+__device__ __forceinline__ Seg load_seg(const SpmmParams& p, int i) {
   Seg s;
-  if constexpr (kExpertsOf<X>) {
-    int at;
-    int4 c;
-    expert_item(p, x, i, s.row, at, c, s.chunk);
-    s.t0 = p.row_ptr[at];
-    s.t1 = p.row_ptr[at + 1];
-    s.n0 = c.y;
-    s.n1 = c.z;
-    s.nseg = 1; s.slot0 = 0; s.my_idx = 0; s.ctr = 0;
-  } else if (PLAN && p.segs != nullptr) {
+  if (PLAN && p.segs != nullptr) {
     const int4* q = reinterpret_cast<const int4*>(p.segs) + 2 * (size_t)i;
     const int4 a = q[0], b = q[1];
     s.row = a.x; s.chunk = a.y; s.t0 = a.z; s.t1 = a.w;
@@ -234,17 +270,9 @@ __device__ __forceinline__ Seg load_seg(const SpmmParams& p, int i, const X& x =
   return s;
 }
 
-// The same for a warp that waits with many values in registers: lane k holds word k (in the order of Seg's fields; experts: words 4, 5
-// and 6 are the chunk's tokens and the expert).
-template <bool PLAN, class X = Nothing>
-__device__ __forceinline__ int load_seg_word(const SpmmParams& p, int i, int lane, const X& x = X{}) {
-  if constexpr (kExpertsOf<X>) {
-    int r, at, c;
-    int4 t;
-    expert_item(p, x, i, r, at, t, c);
-    if (lane == 2 || lane == 3) return p.row_ptr[at + lane - 2];
-    return lane == 0 ? r : (lane == 1 ? c : (lane == 4 ? t.y : (lane == 5 ? t.z : t.x)));
-  }
+// The same for a warp that waits with many values in registers: lane k holds word k (in the order of Seg's fields).
+template <bool PLAN>
+__device__ __forceinline__ int load_seg_word(const SpmmParams& p, int i, int lane) {
   if (PLAN && p.segs != nullptr) return p.segs[8 * (size_t)i + (lane & 7)];   // (without a branch, whose register costs 0.1 us of 14.9)
   int k, chunk;
   p.passes.item(i, k, chunk);
@@ -300,15 +328,22 @@ struct __align__(8) PipeBars {
   uint64_t acc_empty[kMaxSlots];
 };
 
+// Bytes of a panel in a ring stage: 128 columns, of experts the tokens a chunk can have.  (The tensor cores multiply 128 rows all the same:
+// behind a shorter panel they read what lies there, for rows of the result that are not stored.)
+template <int ES, class X = Nothing>
+__device__ __forceinline__ uint32_t panel_bytes(const X& x = X{}) {
+  if constexpr (kExpertsOf<X>) return (uint32_t)x.panel_bytes;
+  else return kPanelBytes * ES;
+}
 // shared-memory offsets inside one ring stage
-template <int ES>
-__device__ __forceinline__ uint32_t panel_off(const SpmmParams& p, int j, int q) {
-  return (uint32_t)(j * p.np + q) * (kPanelBytes * ES);
+template <int ES, class X = Nothing>
+__device__ __forceinline__ uint32_t panel_off(const SpmmParams& p, int j, int q, const X& x = X{}) {
+  return (uint32_t)(j * p.np + q) * panel_bytes<ES>(x);
 }
 // A stage holds the panels of its tiles first, then the tiles; `cap` is the stage's capacity in tiles
-template <int ES>
-__device__ __forceinline__ uint32_t tile_off(const SpmmParams& p, int cap, int j) {
-  return (uint32_t)(cap * p.np) * (kPanelBytes * ES) + (uint32_t)(j * p.terms) * (kTileBytes * ES);
+template <int ES, class X = Nothing>
+__device__ __forceinline__ uint32_t tile_off(const SpmmParams& p, int cap, int j, const X& x = X{}) {
+  return (uint32_t)(cap * p.np) * panel_bytes<ES>(x) + (uint32_t)(j * p.terms) * (kTileBytes * ES);
 }
 // Capacity of a ring stage: every stage takes p.group tiles except the last, which takes what is left of the
 // shared memory (p.last_group).  The groups of a tile row follow the stages they fall on: a group is
@@ -340,13 +375,33 @@ __device__ __forceinline__ void producer_loop(const SpmmParams& p, const CUtenso
   int stage = 0, owner = 0, gcount = 0;
   uint32_t phase = 0;
   Seg seg_next = {};  // the next segment's descriptor is fetched one item ahead
-  if (begin < end) seg_next = load_seg<PLAN>(p, begin, x);
+  ItemsOf<X> items;
+  int cols_next = 0;  // experts: and the block columns of its first 32 tiles, one per lane
+  auto fetch = [&](int i) {
+    if constexpr (kExpertsOf<X>) {
+      seg_next = items.next(p, x, i, step, end);
+      cols_next = seg_next.t0 + lane < seg_next.t1 ? p.tile_cols[seg_next.t0 + lane] : 0;
+    } else {
+      seg_next = load_seg<PLAN>(p, i);
+    }
+  };
+  if (begin < end) fetch(begin);
   for (int i = begin; i < end; i += step) {
     const Seg s = seg_next;
-    if (i + step < end) seg_next = load_seg<PLAN>(p, i + step, x);
+    const int cols = cols_next;
+    if (i + step < end) fetch(i + step);
+    // block column of tile t + lane, for the first `count` lanes
+    auto column = [&](int t, int count) {
+      const bool in = t + lane < s.t1 && lane < count;
+      if constexpr (kExpertsOf<X>) {
+        const int known = __shfl_sync(0xffffffffu, cols, (t - s.t0 + lane) & 31);
+        if (t - s.t0 + lane < 32) return in ? known : 0;
+      }
+      return in ? p.tile_cols[t + lane] : 0;
+    };
     const int npan = panels_of<X>(p, s);
     const int n0 = kExpertsOf<X> ? s.n0 : s.chunk * p.np * kPanelN;
-    const uint32_t unit_bytes = (uint32_t)((kTileBytes * p.terms + ((p.use3d && TR != 1) ? p.np : npan) * kPanelBytes) * ES);
+    const uint32_t unit_bytes = (uint32_t)(kTileBytes * p.terms * ES) + (uint32_t)((p.use3d && TR != 1) ? p.np : npan) * panel_bytes<ES>(x);
     if (TRACE && i == begin && pw == 0 && lane == 0) {
       asm volatile("" ::"r"(s.t1) : "memory");
       stamp<TRACE>(p, 57);   // the row's tile range has arrived
@@ -358,8 +413,7 @@ __device__ __forceinline__ void producer_loop(const SpmmParams& p, const CUtenso
       ct += stage_cap(p, cs);
       cs = (cs + 1 == S) ? 0 : cs + 1;
     }
-    int col = 0;
-    if (ct + lane < s.t1 && lane < stage_cap(p, cs)) col = p.tile_cols[ct + lane];
+    int col = column(ct, stage_cap(p, cs));
     if (TRACE && i == begin && pw == 0 && lane == 0) {
       asm volatile("" ::"r"(col) : "memory");
       stamp<TRACE>(p, 58);   // the first block columns have arrived
@@ -375,8 +429,7 @@ __device__ __forceinline__ void producer_loop(const SpmmParams& p, const CUtenso
           nt += stage_cap(p, ns);
           ns = (ns + 1 == S) ? 0 : ns + 1;
         }
-        int col_next = 0;
-        if (nt + lane < s.t1 && lane < stage_cap(p, ns)) col_next = p.tile_cols[nt + lane];
+        const int col_next = column(nt, stage_cap(p, ns));
         const uint32_t full = smem_u32(&bars->full[stage]);
         const uint32_t sbase = ring_base + (uint32_t)stage * stage_bytes;
         // test hook: the first group of the CTA is never delivered, so the consumer's bounded wait runs out
@@ -384,7 +437,7 @@ __device__ __forceinline__ void producer_loop(const SpmmParams& p, const CUtenso
         if (!mbar_wait_warp(smem_u32(&bars->empty[stage]), phase ^ 1u, ctl)) return;
         if (lane == 0 && !drop) {
           mbar_expect_tx(full, unit_bytes * (uint32_t)gcnt);
-          bulk_load(sbase + tile_off<ES>(p, cap, 0), p.tiles + (size_t)t * (size_t)(kTileBytes * ES * p.terms),
+          bulk_load(sbase + tile_off<ES>(p, cap, 0, x), p.tiles + (size_t)t * (size_t)(kTileBytes * ES * p.terms),
                     (uint32_t)(gcnt * p.terms) * (kTileBytes * ES), full);
         }
         __syncwarp();
@@ -398,13 +451,13 @@ __device__ __forceinline__ void producer_loop(const SpmmParams& p, const CUtenso
           if (TR == 1) {
             // B stored transposed ([N, K], k contiguous): one box of 128 rows of n x 32 k per panel
             for (int q = 0; q < npan; ++q)
-              tma_load_2d(sbase + panel_off<ES>(p, lane, q), tmap, col * kTile, n0 + q * kPanelN, full);
+              tma_load_2d(sbase + panel_off<ES>(p, lane, q, x), tmap, col * kTile, n0 + q * kPanelN, full);
           } else if (p.use3d) {
-            tma_load_3d(sbase + panel_off<ES>(p, lane, 0), tmap, 0, col * kTile, s.chunk * p.np * ES, full);
+            tma_load_3d(sbase + panel_off<ES>(p, lane, 0, x), tmap, 0, col * kTile, s.chunk * p.np * ES, full);
           } else {
             // one copy per 128-byte-wide block of columns: ES blocks of 128 / ES columns per panel
             for (int q = 0; q < npan * ES; ++q)
-              tma_load_2d(sbase + panel_off<ES>(p, lane, 0) + (uint32_t)q * kPanelBytes, tmap,
+              tma_load_2d(sbase + panel_off<ES>(p, lane, 0, x) + (uint32_t)q * kPanelBytes, tmap,
                           n0 + q * (kPanelN / ES), col * kTile, full);
           }
         }
@@ -513,5 +566,7 @@ struct ExpertLaunch {
 };
 template <int KIND>
 int launch_experts(const ExpertLaunch& l);
+// And for a few tokens per expert, chunks of 8 (skinny.cu); map: of panels without a swizzle; items: how many there can be at most.
+int expert_stream_launch(SpmmParams p, const ExpertParams& x, int kind, const CUtensorMap& map, long long items, const DeviceInfo& dev, cudaStream_t st);
 
 }  // namespace vb

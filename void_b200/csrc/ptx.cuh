@@ -124,6 +124,9 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, vo
 }
 
 // ---------------------------------------------------------------- TMA
+__device__ __forceinline__ void prefetch_l2(const void* at) {
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+}
 __device__ __forceinline__ void prefetch_tmap(const CUtensorMap* m) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
 }

@@ -62,15 +62,16 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) spmm_rowacc_kernel
   const int lane = threadIdx.x & 31;
   const uint32_t ring_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   constexpr int ES = Elem<KIND>::ES;
-  const uint32_t unit_smem = (uint32_t)((p.np * kPanelBytes + kTileBytes * p.terms) * ES);
+  const Runs& runs = runs_of<EXPERTS>(x);
+  const uint32_t unit_smem = (uint32_t)p.np * panel_bytes<ES>(runs) + (uint32_t)(kTileBytes * p.terms * ES);
   const uint32_t stage_bytes = (uint32_t)p.group * unit_smem;   // the last stage may be shorter (p.last_group tiles)
   const uint32_t acc_cols = (uint32_t)p.np * 32u;  // TMEM columns of one accumulator buffer
   uint32_t tmem_cols = 32;
   while (tmem_cols < 2u * acc_cols) tmem_cols <<= 1;
   volatile int* ctl = ctl_s;
-  const Runs& runs = runs_of<EXPERTS>(x);
 
   if (threadIdx.x == 0) last_s = 0;
+  if constexpr (EXPERTS) warm_index(p, x);
   pipeline_setup<C, ES, TRACE>(p, &tmap_b, bars, &tmem_base_s, ctl_s, 2, tmem_cols);
   const uint32_t tmem_base = tmem_base_s;
 
@@ -90,7 +91,8 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) spmm_rowacc_kernel
       const uint32_t idesc = p.idesc;
       const uint64_t hi_a = p.desc_hi_a, hi_b = p.desc_hi_b;
       const int S = p.stages, np = p.np, terms = p.terms;
-      constexpr uint64_t kPanelStep = (kPanelBytes * ES) >> 4, kTileStep = (kTileBytes * ES) >> 4;
+      const uint64_t kPanelStep = panel_bytes<ES>(runs) >> 4;
+      constexpr uint64_t kTileStep = (kTileBytes * ES) >> 4;
       // one MMA covers 32 bytes of k: 32 / ES k-rows of the panel (8-row groups 1024 bytes apart) and two
       // 16-byte k-chunks of the packed tile (128 bytes apart)
       // (transposed B: the panel is K-major, 32 bytes of k lie inside one row of its swizzle atom)
@@ -103,10 +105,15 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) spmm_rowacc_kernel
       uint32_t it = 0;
       bool ok = true;
       Seg seg_next = {};  // the next segment's descriptor is fetched one item ahead
-      if (begin < end) seg_next = load_seg<SPLIT>(p, begin, runs);
+      ItemsOf<Runs> items;
+      auto fetch = [&](int i) {
+        if constexpr (EXPERTS) seg_next = items.next(p, x, i, step, end);
+        else seg_next = load_seg<SPLIT>(p, i);
+      };
+      if (begin < end) fetch(begin);
       for (int i = begin; i < end && ok; i += step, ++it) {
         const Seg s = seg_next;
-        if (i + step < end) seg_next = load_seg<SPLIT>(p, i + step, runs);
+        if (i + step < end) fetch(i + step);
         const int npan = panels_of<Runs>(p, s);
         const uint32_t buf = it & 1u, aph = (it >> 1) & 1u;
         ok = mbar_wait_warp(smem_u32(&bars.acc_empty[buf]), aph ^ 1u, ctl);
@@ -125,7 +132,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) spmm_rowacc_kernel
           if (TRACE && leader && i == begin && gidx < 12) stamp<TRACE>(p, 16 + gidx);   // slots 28 .. 31: last arriver of a split row
           tc_fence_after();
           uint64_t ad = smem_desc(hi_a, sbase);
-          uint64_t bd = smem_desc(hi_b, sbase + tile_off<ES>(p, cap, 0));
+          uint64_t bd = smem_desc(hi_b, sbase + tile_off<ES>(p, cap, 0, runs));
           for (int j = 0; j < gcnt; ++j) {
             auto panel = [&](uint64_t a, uint32_t d) {
 #pragma unroll
@@ -176,19 +183,22 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) spmm_rowacc_kernel
     seg_range<SPLIT>(p, begin, end, step, runs);
     uint32_t it = 0;
     int seg_next = 0;  // the next segment's descriptor is fetched one item ahead, a word per lane
-    if (begin < end) seg_next = load_seg_word<SPLIT>(p, begin, lane, runs);
+    ItemsOf<Runs> items;
+    if (!EXPERTS && begin < end) seg_next = load_seg_word<SPLIT>(p, begin, lane);
     if (p.a_stable) grid_dependency_wait();
     if constexpr (EXPERTS)
       if (x.zero_rest) zero_rest_rows(od, x, epi_tid, C::EPI_THREADS);
     if (epi_tid == 0) stamp<TRACE>(p, 0);
     for (int i = begin; i < end; i += step, ++it) {
       const int seg = seg_next;
-      if (i + step < end) seg_next = load_seg_word<SPLIT>(p, i + step, lane, runs);
-      const int row = word_of(seg, 0), chunk = word_of(seg, 1), nseg = SPLIT ? word_of(seg, 4) : 1;
-      const int n_first = EXPERTS ? word_of(seg, 4) : chunk * p.np * kPanelN, n_end = EXPERTS ? word_of(seg, 5) : p.N;
+      if (!EXPERTS && i + step < end) seg_next = load_seg_word<SPLIT>(p, i + step, lane);
+      Seg item = {};
+      if constexpr (EXPERTS) item = items.next(p, x, i, step, end);
+      const int row = EXPERTS ? item.row : word_of(seg, 0), chunk = EXPERTS ? 0 : word_of(seg, 1), nseg = SPLIT ? word_of(seg, 4) : 1;
+      const int n_first = EXPERTS ? item.n0 : chunk * p.np * kPanelN, n_end = EXPERTS ? item.n1 : p.N;
       const int npan = EXPERTS ? (n_end - n_first + kPanelN - 1) / kPanelN : panels_in_chunk(p, chunk);
       const uint32_t buf = it & 1u, aph = (it >> 1) & 1u;
-      const bool has = word_of(seg, 3) > word_of(seg, 2);
+      const bool has = EXPERTS ? item.t1 > item.t0 : word_of(seg, 3) > word_of(seg, 2);
       // an empty tile row is zeros (+ bias): nothing to scale, no scales to wait for
       const float rs = (p.row_scale != nullptr && (has || nseg > 1)) ? p.row_scale[row] : 1.0f;
       const int n_base = n_first + quad * 32 + lane;
@@ -198,6 +208,16 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) spmm_rowacc_kernel
         if (p.col_scale != nullptr && (has || nseg > 1)) cs = p.col_scale[n_base] * p.b_scale;
         if (p.bias != nullptr) bias = p.bias[n_base];
       }
+      float of_lane = 0.0f;
+      if constexpr (EXPERTS) {
+        if (p.row_bias != nullptr) of_lane = bias_of_lane(bias_of_expert(p.row_bias, x.tail.bias_dtype, item.expert, p.M), x.tail.bias_dtype, row, p.M);
+      } else if constexpr (TAIL) {
+        of_lane = bias_of_lane(p.row_bias, x.bias_dtype, row, p.M);
+      }
+      // (of the first panel, where a warp has registers for it: a slim CTA's spill, 48 -> 58 us at bf16 4096^2, 90 %, 4096 tokens)
+      Ahead<C::COLS> ahead;
+      ahead.valid = false;
+      if constexpr (TAIL && !EXPERTS && C::COLS < kTile) ahead.load(od, x, row, n_base, m_first);
       // one warp waits, the named barrier hands its verdict to all epilogue warps, so that they
       // leave the loop together if the wait gave up (a warp that went on alone would wait at the next
       // named barrier for ever)
@@ -378,10 +398,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) spmm_rowacc_kernel
         } else {
           uint32_t r[C::COLS];
           OutDesc to = od;
-          if constexpr (EXPERTS) {
-            to.N = n_end;
-            if (to.row_bias != nullptr) to.row_bias = bias_of_expert(to.row_bias, x.tail.bias_dtype, word_of(seg, 6), p.M);
-          }
+          if constexpr (EXPERTS) to.N = n_end;
           if (!whole) {
             int32_t* sums = row_sums(p, x, seg, peers, q) + m_first * kPanelN + quad * 32;
 #pragma unroll
@@ -409,8 +426,9 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) spmm_rowacc_kernel
           }
 #pragma unroll
           for (int c = 0; c < C::COLS; c += 16) {
-            if constexpr (EXPERTS) finish16_tail<KIND>(to, x.tail, row, n, m_first + c, &r[c], rs, csq, biasq);
-            else if constexpr (TAIL) finish16_tail<KIND>(to, x, row, n, m_first + c, &r[c], rs, csq, biasq);
+            if constexpr (EXPERTS) finish16_tail<KIND>(to, x.tail, row, n, m_first + c, &r[c], rs, csq, biasq, of_lane);
+            else if constexpr (TAIL)
+              finish16_tail<KIND>(to, x, row, n, m_first + c, &r[c], rs, csq, biasq, of_lane, q == 0 && ahead.valid ? ahead.w + c / 2 : nullptr);
             else if (TR) finish16_tr<KIND, ACT>(to, row, n, m_first + c, &r[c], rs, csq, biasq);
             else finish16<KIND, ACT>(to, row, n, m_first + c, &r[c], rs, csq, biasq);
           }

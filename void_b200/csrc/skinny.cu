@@ -25,6 +25,7 @@
 #include "epilogue.cuh"
 #include "kinds.cuh"
 #include "launch.cuh"
+#include "pipeline.cuh"
 #include "ptx.cuh"
 #include "skinny.cuh"
 
@@ -183,13 +184,11 @@ __device__ __forceinline__ void store_value(void* p, int dtype, long long at, fl
 }
 
 // ACT: whether there may be an activation or a row bias (the kernel without is 0.2 us faster).
-// MODE: 1 a linear layer's tail, too; 2 that of experts.
-constexpr int kPlain = 0, kWithTail = 1, kOfExperts = 2;
-template <int MODE>
-using ParamsOf = std::conditional_t<MODE == kOfExperts, SkinnyExpertParams, std::conditional_t<MODE == kWithTail, SkinnyTailParams, SkinnyParams>>;
-template <int KIND, bool TR, int NG, bool ACT, int MODE>
-__global__ void __launch_bounds__(512) skinny_kernel(const __grid_constant__ ParamsOf<MODE> p) {
-  constexpr bool TAIL = MODE != kPlain, EXPERTS = MODE == kOfExperts;
+// TAIL: a linear layer's tail, too.
+template <bool TAIL>
+using ParamsOf = std::conditional_t<TAIL, SkinnyTailParams, SkinnyParams>;
+template <int KIND, bool TR, int NG, bool ACT, bool TAIL>
+__global__ void __launch_bounds__(512) skinny_kernel(const __grid_constant__ ParamsOf<TAIL> p) {
   constexpr int ES = Elem<KIND>::ES, NB = 8 * NG;
   using T = typename AccType<KIND>::T;
   extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -197,24 +196,9 @@ __global__ void __launch_bounds__(512) skinny_kernel(const __grid_constant__ Par
   constexpr int PITCH = NB + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int g = lane >> 2, t = lane & 3;
-  const int row = blockIdx.x;
+  const int row = blockIdx.x, n0 = blockIdx.y * NB;
   if (!p.a_stable) grid_dependency_wait();
-  int n0 = blockIdx.y * NB, n_end = p.N, packed_row = row;
-  const float* row_bias = p.row_bias;
-  if constexpr (EXPERTS) {
-    if (p.zero_rest) {   // zeros for the tokens in no expert's run: this tile row's columns, the tokens dealt out over the slots
-      const int before = p.bounds[0], behind = p.bounds[p.n_experts], rest = before + p.N - behind;
-      for (int i = (int)blockIdx.y + (int)gridDim.y * warp; i < rest; i += (int)gridDim.y * warps)
-        if (row * 32 + lane < p.M) store_value(p.out, p.out_dtype, (long long)(i < before ? i : i - before + behind) * p.ldc + row * 32 + lane, 0.0f);
-    }
-    if ((int)blockIdx.y >= p.head[0]) return;
-    const int4 c = p.chunks[blockIdx.y];
-    n0 = c.y;
-    n_end = c.z;
-    packed_row += c.x * (int)gridDim.x;
-    if (row_bias != nullptr) row_bias = bias_of_expert(row_bias, p.tail.bias_dtype, c.x, p.M);
-  }
-  const int t0 = p.row_ptr[packed_row], t1 = p.row_ptr[packed_row + 1];
+  const int t0 = p.row_ptr[row], t1 = p.row_ptr[row + 1];
   T d[2][NG][4];
 #pragma unroll
   for (int h = 0; h < 2; ++h)
@@ -241,7 +225,7 @@ __global__ void __launch_bounds__(512) skinny_kernel(const __grid_constant__ Par
 #pragma unroll
       for (int i = 0; i < NG; ++i) {
         const int n = n0 + 8 * i + g;
-        load_b_tr<ES>(b + (long long)n * p.ldb, k0, p.K, t, n < n_end, bw[i]);
+        load_b_tr<ES>(b + (long long)n * p.ldb, k0, p.K, t, n < p.N, bw[i]);
       }
     } else {
       load_b<ES, NG>(b, p.ldb, k0, p.K, n0 + NG * g, p.N, t, bw);
@@ -268,16 +252,16 @@ __global__ void __launch_bounds__(512) skinny_kernel(const __grid_constant__ Par
     x.c = TR ? (o >> 5) : o % NB;
     x.n = n0 + x.c;
     x.r = row * 32 + x.m;
-    x.in = x.n < n_end && x.r < p.M;
+    x.in = x.n < p.N && x.r < p.M;
     x.cs = p.b_scale;
     x.bias = x.row_bias = x.residual = 0.0f;
     if (x.in) {
       if (p.col_scale != nullptr) x.cs *= p.col_scale[x.n];
       if (p.bias != nullptr) x.bias = p.bias[x.n];
       if constexpr (TAIL) {
-        if (row_bias != nullptr) x.row_bias = load_value(row_bias, p.tail.bias_dtype, x.r);
-      } else if (ACT && row_bias != nullptr) {
-        x.row_bias = row_bias[x.r];
+        if (p.row_bias != nullptr) x.row_bias = load_value(p.row_bias, p.tail.bias_dtype, x.r);
+      } else if (ACT && p.row_bias != nullptr) {
+        x.row_bias = p.row_bias[x.r];
       }
       if constexpr (TAIL)
         if (p.tail.residual != nullptr) x.residual = load_value(p.tail.residual, p.tail.residual_dtype, (long long)x.n * p.tail.ldr + x.r);
@@ -302,7 +286,7 @@ __global__ void __launch_bounds__(512) skinny_kernel(const __grid_constant__ Par
         mine[m * PITCH + (TR ? 8 * i + j : NG * j + i)] = d[h][i][e];
       }
   __syncthreads();
-  const float rs = p.row_scale != nullptr && t1 > t0 ? p.row_scale[packed_row] : 1.0f;
+  const float rs = p.row_scale != nullptr && t1 > t0 ? p.row_scale[row] : 1.0f;
   for (int o = threadIdx.x; o < 32 * NB; o += blockDim.x) {
     if (!ACT || o >= (int)blockDim.x) x = output(o);
     if (!x.in) continue;
@@ -322,20 +306,130 @@ __global__ void __launch_bounds__(512) skinny_kernel(const __grid_constant__ Par
   }
 }
 
-template <int KIND, bool TR, int NG, bool ACT, int MODE>
-cudaError_t launch(const ParamsOf<MODE>& p, int nbr, int slots, int warps, cudaStream_t st) {
-  auto kernel = skinny_kernel<KIND, TR, NG, ACT, MODE>;
+// A layer of experts with a few tokens for each: items (chunk of at most eight tokens, tile row), taken by resident CTAs, whose tiles and
+// tokens come through a ring in shared memory (producer_loop of pipeline.cuh, panels without a swizzle): a stage is four tiles, one per
+// warp, which keeps its sums in registers to the end of the row.  The weights are read once and that bounds it, so the ring keeps 120 KB
+// of an SM in flight; a CTA per item instead, every warp with loads of its own, is a chain of five latencies of which one carries the
+// weights.  8 experts of 2048 -> 8192, 80 % (54 MB): 8 tokens 18.0 -> 15.7 us, 32 tokens 23.0 -> 19.9.  What a CTA pays per item on top
+// of its bytes - stages that the row does not fill, the sums' exchange - is hidden behind the other CTAs: two of twice the warps 19.0
+// and 22.5, four of them 15.8 and 20.1 but 49 against 45 us with rows four times as long, of which each then takes three or four.
+struct Stream {
+  static constexpr int PW = 2, WARPS = 4, TOKENS = 8, CTAS_PER_SM = 3, THREADS = 32 * (PW + WARPS);
+};
+template <int KIND>
+__global__ void __launch_bounds__(Stream::THREADS, Stream::CTAS_PER_SM) expert_stream_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ ExpertParams x,
+                                                                          const __grid_constant__ SpmmParams p) {
+  constexpr int ES = Elem<KIND>::ES, NB = Stream::TOKENS, PITCH = NB + 1, W = Stream::WARPS;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ PipeBars bars;
+  __shared__ int ctl_s[2];   // abort flag, wait limit in ms
+  volatile int* ctl = ctl_s;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t stage_bytes = (uint32_t)p.group * (panel_bytes<ES>(x) + (uint32_t)(kTileBytes * ES));
+  warm_index(p, x);
+  if (threadIdx.x == 0) {
+    ctl_s[0] = 0;
+    ctl_s[1] = p.wait_limit_ms;
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(smem_u32(&bars.full[s]), 1);
+      mbar_init(smem_u32(&bars.empty[s]), W);
+    }
+    fence_mbar_init();
+    if (p.tiles != nullptr) prefetch_tmap(&tmap);
+  }
+  __syncthreads();
+  if (warp < Stream::PW) {
+    producer_loop<Stream, ES, 1, false, false, ExpertParams>(p, &tmap, &bars, ring, stage_bytes, ctl, lane, warp, x);
+  } else {
+    const int w = warp - Stream::PW, tid = (int)threadIdx.x - 32 * Stream::PW, g = lane >> 2, t = lane & 3;
+    const uint8_t* base = smem_raw + (ring - smem_u32(smem_raw));
+    float* red = reinterpret_cast<float*>(smem_raw + (ring - smem_u32(smem_raw)) + p.part_off);   // [2][W][32][PITCH]
+    grid_dependency_wait();
+    const OutDesc od = out_desc(p);
+    if (x.zero_rest) zero_rest_rows(od, x, tid, 32 * W);
+    int begin, end, step, stage = 0, turn = 0;
+    uint32_t phase = 0;
+    bool alive = true;   // (after a wait that gave up the others do, too, at once: every warp still comes to every barrier)
+    seg_range<false>(p, begin, end, step, x);
+    ExpertItems items;
+    for (int i = begin; i < end; i += step, turn ^= 1) {
+      const Seg item = items.next(p, x, i, step, end);
+      const int row = item.row, t0 = item.t0, t1 = item.t1, n0 = item.n0, n1 = item.n1;
+      // (asked for here: behind the products it would cost an item a trip to memory)
+      float of_row = 0.0f;
+      if (p.row_bias != nullptr && row * kTile + lane < p.M)
+        of_row = load_value(bias_of_expert(p.row_bias, x.tail.bias_dtype, item.expert, p.M), x.tail.bias_dtype, row * kTile + lane);
+      float d[2][4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) d[0][e] = d[1][e] = 0.0f;
+      for (int at = t0; at < t1; at += W) {
+        alive = mbar_wait_warp(smem_u32(&bars.full[stage]), phase, ctl) && alive;
+        if (alive && at + w < t1) {
+          const uint8_t* here = base + (uint32_t)stage * stage_bytes;
+          const uint8_t *panel = here + panel_off<ES>(p, w, 0, x), *tile = here + tile_off<ES>(p, W, w, x);
+          uint32_t aw[4][2 * ES], bw[2 * ES];
+#pragma unroll
+          for (int h = 0; h < ES / 2; ++h) {
+            const uint4 v = *reinterpret_cast<const uint4*>(panel + g * (32 * ES) + (h * 4 + t) * 16);
+            bw[4 * h] = v.x; bw[4 * h + 1] = v.y; bw[4 * h + 2] = v.z; bw[4 * h + 3] = v.w;
+          }
+          order_words<ES>(bw);
+#pragma unroll
+          for (int rg = 0; rg < 4; ++rg) load_a<ES>(tile, rg, g, t, aw[rg]);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int k = 0; k < ES; ++k)
+              mma32<KIND>(d[h], aw[2 * h][2 * k], aw[2 * h + 1][2 * k], aw[2 * h][2 * k + 1], aw[2 * h + 1][2 * k + 1], bw[2 * k], bw[2 * k + 1]);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bars.empty[stage]));
+        if (++stage == p.stages) { stage = 0; phase ^= 1u; }
+      }
+      float* mine = red + (turn * W + w) * (32 * PITCH);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mine[(16 * h + g + 8 * (e >> 1)) * PITCH + 2 * t + (e & 1)] = d[h][e];
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * W) : "memory");   // (one per item: the other half of `red` is written before the next)
+      if (!alive) continue;
+#pragma unroll
+      for (int o = tid; o < 32 * NB; o += 32 * W) {
+        const int m = o & 31, n = n0 + (o >> 5), r = row * kTile + m;
+        if (n >= n1 || r >= p.M) continue;
+        float v = of_row;
+#pragma unroll
+        for (int k = 0; k < W; ++k) v += red[((turn * W + k) * 32 + m) * PITCH + (o >> 5)];
+        if (x.tail.pre != nullptr) store_value(x.tail.pre, p.out_dtype, (long long)n * x.tail.ldp + r, v);
+        store_value(p.out, p.out_dtype, (long long)n * p.ldc + r, activate(v, p.act));
+      }
+    }
+  }
+  grid_launch_dependents();
+  __syncthreads();
+  if (ctl_s[0]) {
+    const uint64_t since = globaltimer_ns();   // let copies still in flight land before shared memory is given back
+    while (globaltimer_ns() - since < 200000ull) {
+    }
+    if (threadIdx.x == 0 && p.status != nullptr) atomicCAS(p.status, 0, kStatusTimeout);
+    __syncthreads();
+  }
+}
+
+template <int KIND, bool TR, int NG, bool ACT, bool TAIL>
+cudaError_t launch(const ParamsOf<TAIL>& p, int nbr, int warps, cudaStream_t st) {
+  auto kernel = skinny_kernel<KIND, TR, NG, ACT, TAIL>;
   const int smem = warps * 32 * (8 * NG + 1) * 4;
   if (smem > 48 * 1024 && ensure_smem((const void*)kernel, smem)) return cudaErrorInvalidValue;
-  return launch_pdl(kernel, dim3((unsigned)nbr, (unsigned)slots), 32 * warps, smem, st, p);
+  return launch_pdl(kernel, dim3((unsigned)nbr, (unsigned)((p.N + 8 * NG - 1) / (8 * NG))), 32 * warps, smem, st, p);
 }
 template <int KIND, bool TR, int NG>
 cudaError_t launch(const SkinnyTailParams& p, bool tail, int nbr, int warps, cudaStream_t st) {
-  const int slots = (p.N + 8 * NG - 1) / (8 * NG);
   if constexpr (TR)
-    if (tail) return launch<KIND, TR, NG, true, kWithTail>(p, nbr, slots, warps, st);
-  return p.act != VOID_ACT_NONE || p.row_bias != nullptr ? launch<KIND, TR, NG, true, kPlain>(p, nbr, slots, warps, st)
-                                                         : launch<KIND, TR, NG, false, kPlain>(p, nbr, slots, warps, st);
+    if (tail) return launch<KIND, TR, NG, true, true>(p, nbr, warps, st);
+  return p.act != VOID_ACT_NONE || p.row_bias != nullptr ? launch<KIND, TR, NG, true, false>(p, nbr, warps, st)
+                                                         : launch<KIND, TR, NG, false, false>(p, nbr, warps, st);
 }
 template <int KIND, bool TR>
 cudaError_t launch_columns(const SkinnyTailParams& p, bool tail, int nbr, int warps, cudaStream_t st) {
@@ -349,22 +443,31 @@ cudaError_t launch_columns(const SkinnyTailParams& p, bool tail, int nbr, int wa
 int row_warps(long long tiles) { return tiles >= 24 ? 16 : (tiles >= 6 ? 8 : 4); }
 
 template <int KIND>
-cudaError_t launch_experts(const SkinnyExpertParams& p, int nbr, int slots, int chunk, int warps, cudaStream_t st) {
-  if (chunk == 8) return launch<KIND, true, 1, true, kOfExperts>(p, nbr, slots, warps, st);
-  if (chunk == 16) return launch<KIND, true, 2, true, kOfExperts>(p, nbr, slots, warps, st);
-  return chunk == 32 ? launch<KIND, true, 4, true, kOfExperts>(p, nbr, slots, warps, st) : cudaErrorInvalidValue;
+int launch_stream(SpmmParams p, const ExpertParams& x, const CUtensorMap& map, int grid, int smem_per_sm, cudaStream_t st) {
+  auto kernel = expert_stream_kernel<KIND>;
+  const int sums = 2 * Stream::WARPS * 32 * (Stream::TOKENS + 1) * 4, stage = p.group * (x.panel_bytes + kTileBytes * Elem<KIND>::ES);
+  p.stages = (smem_per_sm / Stream::CTAS_PER_SM - 1024 - 640 - 1024 - sums) / stage;
+  if (p.stages > 8) p.stages = 8;
+  if (p.stages < Stream::PW) return VOID_ERR_SHAPE;
+  p.last_group = p.group;
+  p.part_off = p.stages * stage;
+  const int smem = p.part_off + sums + 1024;
+  if (ensure_smem((const void*)kernel, smem)) return VOID_ERR_CUDA;
+  return status_of(launch_pdl(kernel, grid, Stream::THREADS, smem, st, map, x, p));
 }
 
 }  // namespace
 
-// nnz_row: stored tiles of a tile row, on average; slots: chunks there can be at most.
-cudaError_t skinny_experts_launch(const SkinnyExpertParams& p, int kind, int nbr, long long nnz_row, int chunk, int slots, cudaStream_t st) {
-  const int warps = row_warps(nnz_row);
+// items: work items there can be at most.
+int expert_stream_launch(SpmmParams p, const ExpertParams& x, int kind, const CUtensorMap& map, long long items, const DeviceInfo& dev, cudaStream_t st) {
+  p.np = p.terms = 1;
+  p.group = Stream::WARPS;
+  const int ctas = Stream::CTAS_PER_SM * dev.sms, grid = items < ctas ? (int)items : ctas;
   switch (kind) {
-    case VOID_KIND_F16: return launch_experts<VOID_KIND_F16>(p, nbr, slots, chunk, warps, st);
-    case VOID_KIND_BF16: return launch_experts<VOID_KIND_BF16>(p, nbr, slots, chunk, warps, st);
-    case VOID_KIND_TF32: return launch_experts<VOID_KIND_TF32>(p, nbr, slots, chunk, warps, st);
-    default: return cudaErrorInvalidValue;
+    case VOID_KIND_F16: return launch_stream<VOID_KIND_F16>(p, x, map, grid, dev.smem_per_sm, st);
+    case VOID_KIND_BF16: return launch_stream<VOID_KIND_BF16>(p, x, map, grid, dev.smem_per_sm, st);
+    case VOID_KIND_TF32: return launch_stream<VOID_KIND_TF32>(p, x, map, grid, dev.smem_per_sm, st);
+    default: return VOID_ERR_BAD_ARG;
   }
 }
 

@@ -27,15 +27,6 @@ struct SkinnyTailParams : SkinnyParams {
   Tail tail;                // read by the kernels with one
 };
 
-// Experts: every CTA takes a tile row of the weight of one chunk of tokens (experts.cu), at most 32 of them.
-struct SkinnyExpertParams : SkinnyTailParams {
-  const int32_t* head;
-  const int32_t* bounds;
-  const int4* chunks;
-  int n_experts, zero_rest;
-};
-cudaError_t skinny_experts_launch(const SkinnyExpertParams& p, int kind, int nbr, long long nnz_row, int chunk, int slots, cudaStream_t st);
-
 cudaError_t skinny_launch(const SkinnyTailParams& p, int kind, bool transposed, bool tail, int nbr, long long nnz, cudaStream_t st);
 
 }  // namespace vb
