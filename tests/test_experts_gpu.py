@@ -367,7 +367,7 @@ def test_refusals():
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n, k, m, density, counts, before, behind", [
     (4, 1024, 2000, 0.3, [700, 0, 1500, 331], 0, 0), (4, 1024, 2000, 0.3, [700, 0, 1500, 331], 5, 300), (3, 2048, 4096, 0.45, [900, 1, 400], 0, 77),
-    (8, 515, 1100, 0.5, [600, 601, 0, 0, 1, 700, 129, 1000], 3, 1),
+    (8, 515, 1104, 0.5, [600, 601, 0, 0, 1, 700, 129, 1000], 3, 1),
 ])
 def test_groups_of_tile_rows(n, k, m, density, counts, before, behind, dtype):
     # (the first calls take the row kernel; from the fourth on a store for groups of each expert's tile rows is there)

@@ -227,6 +227,14 @@ __device__ __forceinline__ void finish_fragments(const OutDesc& o, int r0, const
   }
 }
 
+__device__ __forceinline__ uint32_t pack16(float lo, float hi, int dtype) {
+  if (dtype == VOID_OUT_F16) {
+    const __half2 t = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&t);
+  }
+  const __nv_bfloat162 t = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&t);
+}
 // Sixteen consecutive elements of a row-major matrix from `first` on, `cols` of them inside, in whole 32-byte sectors or 16-byte pieces
 // where they lie so.  (A sector in two stores goes to L2 twice: bf16 4096^2, 90 %, 4096 tokens, plain 44.2 us and 39.4 in whole sectors,
 // with a residual 58.0 and 48.0, keeping the value before the activation too 83 and 66.)
@@ -252,15 +260,7 @@ __device__ __forceinline__ void store16_row(void* out, int dtype, size_t first, 
   } else {
     uint32_t h[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      if (dtype == VOID_OUT_F16) {
-        const __half2 t = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
-        h[k] = *reinterpret_cast<const uint32_t*>(&t);
-      } else {
-        const __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
-        h[k] = *reinterpret_cast<const uint32_t*>(&t);
-      }
-    }
+    for (int k = 0; k < 8; ++k) h[k] = pack16(v[2 * k], v[2 * k + 1], dtype);
     uint16_t* dst = reinterpret_cast<uint16_t*>(out) + first;
     if (cols >= 16 && (reinterpret_cast<uintptr_t>(dst) & 31u) == 0) {
       st_global_v8(dst, h);
@@ -275,19 +275,110 @@ __device__ __forceinline__ void store16_row(void* out, int dtype, size_t first, 
   }
 }
 
+// Rows that do not lie in whole 16-byte pieces (a pitch of an odd number of elements): written by the lane that owns it, every element
+// of 32 rows would be a store of 32 sectors.  Instead eight lanes exchange words first - w[i] of lane j becomes w[j] of lane i - and then
+// write eight words of a row together, four rows at a time.  The kernels that can (kLoose) are others, for the code and the registers
+// of it: bf16 4096^2, 90 %, 4096 tokens with a residual takes 46 us, with the code for both 70.
+__device__ __forceinline__ void turn8(uint32_t (&w)[8]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int s = 4; s > 0; s >>= 1)
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if ((i & s) == 0) {
+        const bool high = (lane & s) != 0;
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, high ? w[i] : w[i + s], s);
+        if (high) w[i] = got;
+        else w[i + s] = got;
+      }
+}
+__host__ __device__ __forceinline__ bool in_pieces(const void* base, int dtype, long long ld, int bytes = 16) {
+  return ((reinterpret_cast<uintptr_t>(base) | (uintptr_t)(ld * (dtype == VOID_OUT_F32 ? 4 : 2))) & (uintptr_t)(bytes - 1)) == 0;
+}
+// Eight words of each of the warp's rows (lane n's row is n) of an [N, M] matrix, from column c0 on: eight fp32 or sixteen 16-bit values.
+// For whole warps.
+struct Words8 { uint32_t w[8]; };
+__device__ __forceinline__ void store_loose(void* out, int dtype, long long ld, int n, int N, int c0, int M, Words8 x) {
+  const int j = threadIdx.x & 7, first = n - j;
+  turn8(x.w);
+  if (dtype == VOID_OUT_F32) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (first + i < N && c0 + j < M) reinterpret_cast<uint32_t*>(out)[(size_t)(first + i) * (size_t)ld + c0 + j] = x.w[i];
+    return;
+  }
+  const int c = c0 + 2 * j;
+  const bool words = in_pieces(out, dtype, ld, 4);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    uint16_t* dst = reinterpret_cast<uint16_t*>(out) + (size_t)(first + i) * (size_t)ld + c;
+    if (first + i >= N) continue;
+    if (words && c + 1 < M) {
+      *reinterpret_cast<uint32_t*>(dst) = x.w[i];
+    } else {
+      if (c < M) dst[0] = (uint16_t)x.w[i];
+      if (c + 1 < M) dst[1] = (uint16_t)(x.w[i] >> 16);
+    }
+  }
+}
+// (to be turned: the loads can be on their way while something else is done)
+__device__ __forceinline__ Words8 load_loose(const void* from, int dtype, long long ld, int n, int N, int c0, int M) {
+  const int j = threadIdx.x & 7, first = n - j;
+  Words8 x;
+  if (dtype == VOID_OUT_F32) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      x.w[i] = first + i < N && c0 + j < M ? reinterpret_cast<const uint32_t*>(from)[(size_t)(first + i) * (size_t)ld + c0 + j] : 0u;
+  } else {
+    const int c = c0 + 2 * j;
+    const bool words = in_pieces(from, dtype, ld, 4);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint16_t* src = reinterpret_cast<const uint16_t*>(from) + (size_t)(first + i) * (size_t)ld + c;
+      x.w[i] = 0u;
+      if (first + i >= N) continue;
+      if (words && c + 1 < M) {
+        x.w[i] = *reinterpret_cast<const uint32_t*>(src);
+      } else {
+        if (c < M) x.w[i] = src[0];
+        if (c + 1 < M) x.w[i] |= (uint32_t)src[1] << 16;
+      }
+    }
+  }
+  return x;
+}
+// Sixteen columns from c0 on of the lane's row n of an [N, M] matrix; LOOSE: of the warp's rows, which may lie anyhow.
+template <bool LOOSE>
+__device__ __forceinline__ void store16_rows(void* out, int dtype, long long ld, int n, int N, int c0, int M, const float (&v)[16]) {
+  if constexpr (!LOOSE) {
+    if (n < N) store16_row(out, dtype, (size_t)n * (size_t)ld + c0, M - c0, v);
+  } else if (dtype == VOID_OUT_F32) {
+#pragma unroll
+    for (int half = 0; half < 16; half += 8) {
+      Words8 x;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x.w[i] = __float_as_uint(v[half + i]);
+      store_loose(out, dtype, ld, n, N, c0 + half, M, x);
+    }
+  } else {
+    Words8 x;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x.w[i] = pack16(v[2 * i], v[2 * i + 1], dtype);
+    store_loose(out, dtype, ld, n, N, c0, M, x);
+  }
+}
+
 // Transposed output (C stored as [N, M], m contiguous): the thread owns output row n and sixteen consecutive
-// columns m0 .. m0 + 15 of it, so the values leave in 16-byte stores.  bias_n is the bias of this n, the
+// columns m0 .. m0 + 15 of it, so the values leave in 16-byte stores (LOOSE: for whole warps, C may lie anyhow).  bias_n is the bias of this n, the
 // per-m bias (o.row_bias) is the same for every thread of the warp.
-template <int KIND, bool ACT = true>
+template <int KIND, bool ACT = true, bool LOOSE = false>
 __device__ __forceinline__ void finish16_tr(const OutDesc& o, int row, int n, int m0, const uint32_t* r,
                                             float row_scale, float cs, float bias_n) {
-  if (n >= o.N) return;
   const int c0 = row * kTile + m0;   // first output column (a row index of A)
-  const int cols = o.M - c0;         // columns left
-  if (cols <= 0) return;
+  if (c0 >= o.M || (!LOOSE && n >= o.N)) return;
   float v[16];
   finished<KIND, 8, ACT>(o, c0, r, row_scale, cs, bias_n, v);
-  store16_row(o.out, o.dtype, (size_t)n * o.ldc + c0, cols, v);
+  store16_rows<LOOSE>(o.out, o.dtype, o.ldc, n, o.N, c0, o.M, v);
 }
 
 // What a linear layer's epilogue may do besides: keep the value before the activation, add a residual behind it.
@@ -369,13 +460,48 @@ __device__ __forceinline__ void add16(const void* from, int dtype, size_t first,
     }
   }
 }
+// The same of the lane's row n of an [N, M] matrix; LOOSE: of the warp's rows, which may lie anyhow.
+template <bool LOOSE>
+__device__ __forceinline__ void add16_rows(const void* from, int dtype, long long ld, int n, int N, int c0, int M, float (&v)[16]) {
+  if constexpr (!LOOSE) {
+    if (n < N) add16(from, dtype, (size_t)n * (size_t)ld + c0, M - c0, v);
+  } else if (dtype == VOID_OUT_F32) {
+#pragma unroll
+    for (int half = 0; half < 16; half += 8) {
+      Words8 x = load_loose(from, dtype, ld, n, N, c0 + half, M);
+      turn8(x.w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[half + i] += __uint_as_float(x.w[i]);
+    }
+  } else {
+    const bool f16 = dtype == VOID_OUT_F16;
+    Words8 x = load_loose(from, dtype, ld, n, N, c0, M);
+    turn8(x.w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[2 * i] += f16_value(x.w[i] & 0xffffu, f16);
+      v[2 * i + 1] += f16_value(x.w[i] >> 16, f16);
+    }
+  }
+}
 // The residual of COLS columns of a tile row from m0 on, asked for before the accumulators are there: 16-bit ones that lie in whole
-// sectors.
-template <int COLS>
+// sectors, or (LOOSE) anyhow.
+template <int COLS, bool LOOSE = false>
 struct Ahead {
   uint32_t w[COLS / 2];
   bool valid;
   __device__ __forceinline__ void load(const OutDesc& o, const Tail& t, int row, int n, int m0 = 0) {
+    if constexpr (LOOSE) {
+      valid = t.residual != nullptr && t.residual_dtype != VOID_OUT_F32;
+      if (!valid) return;
+#pragma unroll
+      for (int k = 0; k < COLS / 2; k += 8) {
+        const Words8 x = load_loose(t.residual, t.residual_dtype, t.ldr, n, o.N, row * kTile + m0 + 2 * k, o.M);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[k + i] = x.w[i];
+      }
+      return;
+    }
     const uint16_t* src = reinterpret_cast<const uint16_t*>(t.residual) + (size_t)n * t.ldr + row * kTile + m0;
     valid = t.residual != nullptr && t.residual_dtype != VOID_OUT_F32 && n < o.N && row * kTile + kTile <= o.M && (reinterpret_cast<uintptr_t>(src) & 31u) == 0;
     if (valid)
@@ -393,18 +519,18 @@ __device__ __forceinline__ float bias_of_lane(const float* bias, int dtype, int 
 }
 // finish16_tr with the rest of a linear layer: z = dequantised accumulator + bias, kept where asked; act(z) + residual.  For whole
 // warps: of_lane is bias_of_lane.  ahead: the residual where it is there already.
-template <int KIND>
+template <int KIND, bool LOOSE = false>
 __device__ __forceinline__ void finish16_tail(const OutDesc& o, const Tail& t, int row, int n, int m0, const uint32_t* r, float row_scale,
                                               float cs, float bias_n, float of_lane, const uint32_t* ahead = nullptr) {
-  const int c0 = row * kTile + m0, cols = o.M - c0;
-  if (cols <= 0) return;
+  const int c0 = row * kTile + m0;
+  if (c0 >= o.M) return;
   float v[16];
   finished<KIND, 8, false>(o, c0, r, row_scale, cs, bias_n, v);
   if (o.row_bias != nullptr)
 #pragma unroll
     for (int k = 0; k < 16; ++k) v[k] += __shfl_sync(0xffffffffu, of_lane, m0 + k);
-  if (n >= o.N) return;
-  if (t.pre != nullptr) store16_row(t.pre, o.dtype, (size_t)n * t.ldp + c0, cols, v);
+  if (!LOOSE && n >= o.N) return;
+  if (t.pre != nullptr) store16_rows<false>(t.pre, o.dtype, t.ldp, n, o.N, c0, o.M, v);
   if (o.act != VOID_ACT_NONE) {
     f32x2 x[8];
 #pragma unroll
@@ -415,15 +541,19 @@ __device__ __forceinline__ void finish16_tail(const OutDesc& o, const Tail& t, i
   }
   if (ahead != nullptr) {
     const bool f16 = t.residual_dtype == VOID_OUT_F16;
+    Words8 x;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x.w[k] = ahead[k];
+    if constexpr (LOOSE) turn8(x.w);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      v[2 * k] += f16_value(ahead[k] & 0xffffu, f16);
-      v[2 * k + 1] += f16_value(ahead[k] >> 16, f16);
+      v[2 * k] += f16_value(x.w[k] & 0xffffu, f16);
+      v[2 * k + 1] += f16_value(x.w[k] >> 16, f16);
     }
   } else if (t.residual != nullptr) {
-    add16(t.residual, t.residual_dtype, (size_t)n * t.ldr + c0, cols, v);
+    add16_rows<LOOSE>(t.residual, t.residual_dtype, t.ldr, n, o.N, c0, o.M, v);
   }
-  store16_row(o.out, o.dtype, (size_t)n * o.ldc + c0, cols, v);
+  store16_rows<LOOSE>(o.out, o.dtype, o.ldc, n, o.N, c0, o.M, v);
 }
 
 }  // namespace vb

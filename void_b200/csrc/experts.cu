@@ -169,7 +169,7 @@ int experts_launch(const void_spmm_args* a, const void_epilogue* e, const void_e
   p.idesc = instr_desc(1, format, format, 0, 0, 128, 32);
   int grid = dev.sms * Mid::CTAS_PER_SM;
   if (items < grid) grid = (int)items;
-  const ExpertLaunch l = {grid, p.stages * p.group * unit + slack + 1024, st, tmap, experts, p};
+  const ExpertLaunch l = {grid, p.stages * p.group * unit + slack + 1024, !in_pieces(a->out, a->out_dtype, a->ldc), st, tmap, experts, p};
   return kind == VOID_KIND_TF32 ? launch_experts<VOID_KIND_TF32>(l) : launch_experts<VOID_KIND_F16>(l);
 }
 

@@ -593,10 +593,15 @@ void set_residual(Tail& t, const at::Tensor& given, const at::Tensor& out) {
   t.e.ldr = rows > 1 ? r.stride(0) : cols;
   t.e.residual_dtype = out_code(r.scalar_type());
 }
+// Whether rows of results or of a residual lie in whole 16-byte pieces.  Where they do not, the row kernel writes and reads them eight
+// lanes together (kLoose), which the kernel for groups of tile rows does not: bf16 4095 x 4096, 90 %, 4096 tokens, 64 and 156 us.
+bool in_pieces(const void* at, int64_t ld, int64_t es) { return ((reinterpret_cast<uintptr_t>(at) | (uintptr_t)(ld * es)) & 15u) == 0; }
+bool in_pieces(const at::Tensor& t) { return in_pieces(t.const_data_ptr(), t.dim() == 2 ? t.stride(0) : 0, t.element_size()); }
 // A plain product with everything filled in; tokens: the group store of a linear layer that reads them as they lie (transposed = 1).
 void launch_product(Packed* p, const void_spmm_args& s, void_stream_t st, const void_epilogue* tail = nullptr, GroupStore* tokens = nullptr) {
   if (s.scale_mode == VOID_SCALE_ROW_MEAN) {
-    GroupStore* g = s.transposed == 1 ? tokens : group_store(p, s.N, st);
+    GroupStore* g = s.transposed == 1 ? tokens
+                    : s.transposed == 2 && !in_pieces(s.out, s.ldc, s.out_dtype == VOID_OUT_F32 ? 4 : 2) ? nullptr : group_store(p, s.N, st);
     if (g != nullptr) {
       g->readers.add(c10::cuda::getCurrentCUDAStream(p->device), {&g->index, &g->blob});
       if (p->captured && capturing(st)) g->captured = true;
@@ -656,7 +661,8 @@ PyObject* spmm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (out.device() != dev) fail("out and B are on different devices");
   }
   const void_stream_t st = launch_stream(pk);
-  GroupStore* tokens = tr && none(a[11]) ? group_store(pk, N, st, true) : nullptr;
+  const bool whole = in_pieces(out) && (n < 13 || none(a[12]) || in_pieces(cuda_tensor(a[12], "residual")));
+  GroupStore* tokens = tr && none(a[11]) && whole ? group_store(pk, N, st, true) : nullptr;
   const bool copied = tr && none(a[11]) && tokens == nullptr && copy_pays(pk->kind, pk->args.nnz, N, pk->K);
   const at::Tensor b = copied ? transposed_copy(b_in, es) : kernel_operand(b_in, es, tr ? 0 : pk->args.nnz * ((N + 127) / 128));
 
@@ -766,7 +772,8 @@ at::Tensor two_layers(Packed* first, Packed* second, const at::Tensor& x, PyObje
   const int64_t N = x.size(0);
   const void_stream_t st = launch_stream(pk[0]);
   launch_stream(pk[1]);
-  GroupStore* tokens[2] = {group_store(pk[0], N, st, true), group_store(pk[1], N, st, true)};
+  const bool whole = pk[1]->M * es % 16 == 0 && (none(residual) || in_pieces(cuda_tensor(residual, "residual")));   // (of the second result)
+  GroupStore* tokens[2] = {group_store(pk[0], N, st, true), whole ? group_store(pk[1], N, st, true) : nullptr};
   const bool columns = (tokens[0] == nullptr || tokens[1] == nullptr) && N > 128 &&
                        copy_saves_ns(kind, pk[0]->args.nnz + pk[1]->args.nnz, N) > copy_costs_ns(N, pk[0]->K, es);
   at::Tensor in = columns ? transposed_copy(x, es) : kernel_operand(x, es), bias[2], out;
@@ -1531,7 +1538,7 @@ PyObject* expert_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
   plan.x.zero_rest = none(a[7]) ? 1 : 0;
   const void_stream_t st = launch_stream(pk);
-  GroupStore* g = plan.x.chunk == 128 ? group_store(pk, N, st, true, (int32_t)experts, plan.x.row_order) : nullptr;
+  GroupStore* g = plan.x.chunk == 128 && in_pieces(out) ? group_store(pk, N, st, true, (int32_t)experts, plan.x.row_order) : nullptr;
   if (g != nullptr) {
     g->readers.add(c10::cuda::getCurrentCUDAStream(pk->device), {&g->index, &g->blob});
     if (pk->captured && capturing(st)) g->captured = true;

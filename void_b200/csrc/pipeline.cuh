@@ -541,7 +541,8 @@ __device__ __forceinline__ void pipeline_teardown(const SpmmParams& p, int* ctl_
 //   kTraced  time stamps (slim INT8 only, with kActive)
 //   kTail    what a linear layer adds (Tail in epilogue.cuh; transposed results only, with kActive)
 //   kExperts the weight of one of several experts for each run of tokens (ExpertParams; B and C transposed, with kActive and kTail)
-constexpr int kStaged = 1, kSplit = 2, kActive = 4, kTraced = 8, kTail = 16, kExperts = 32;
+//   kLoose   results or a residual in rows that do not lie in 16-byte pieces (transposed results only, with kActive)
+constexpr int kStaged = 1, kSplit = 2, kActive = 4, kTraced = 8, kTail = 16, kExperts = 32, kLoose = 64;
 struct RowaccLaunch {
   int shape;   // 1 wide, 2 slim, 6 mid
   int transposed;
@@ -559,6 +560,7 @@ int launch_rowacc(const RowaccLaunch& l);
 // The same for experts (mid shape).
 struct ExpertLaunch {
   int grid, smem_bytes;
+  bool loose;
   cudaStream_t stream;
   const CUtensorMap& b;
   const ExpertParams& x;

@@ -44,11 +44,12 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) spmm_rowacc_kernel
                                                                                  const __grid_constant__ ExtraOf<EPI> x,
                                                                                  const __grid_constant__ SpmmParams p) {
   constexpr bool STAGED = (EPI & kStaged) != 0, SPLIT = (EPI & kSplit) != 0, ACT = (EPI & kActive) != 0, TRACE = (EPI & kTraced) != 0;
-  constexpr bool TAIL = (EPI & kTail) != 0, EXPERTS = (EPI & kExperts) != 0;
+  constexpr bool TAIL = (EPI & kTail) != 0, EXPERTS = (EPI & kExperts) != 0, LOOSE = (EPI & kLoose) != 0;
   // (what the roles are told about experts; the others read nothing of it)
   using Runs = std::conditional_t<EXPERTS, ExpertParams, Nothing>;
   static_assert(!TR || (!STAGED && !SPLIT), "transposed results are stored directly, of whole rows");
   static_assert(!TAIL || (TR && ACT), "linear layers only");
+  static_assert(!LOOSE || (TR && ACT), "results as they lie");
   static_assert(!EXPERTS || (TR == 1 && TAIL), "tokens as they lie");
   static_assert(!STAGED || C::COLS == kTile, "an epilogue warp stages whole columns of a tile row");
   extern __shared__ uint8_t smem_raw[];
@@ -215,7 +216,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) spmm_rowacc_kernel
         of_lane = bias_of_lane(p.row_bias, x.bias_dtype, row, p.M);
       }
       // (of the first panel, where a warp has registers for it: a slim CTA's spill, 48 -> 58 us at bf16 4096^2, 90 %, 4096 tokens)
-      Ahead<C::COLS> ahead;
+      Ahead<C::COLS, LOOSE> ahead;
       ahead.valid = false;
       if constexpr (TAIL && !EXPERTS && C::COLS < kTile) ahead.load(od, x, row, n_base, m_first);
       // one warp waits, the named barrier hands its verdict to all epilogue warps, so that they
@@ -426,10 +427,10 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) spmm_rowacc_kernel
           }
 #pragma unroll
           for (int c = 0; c < C::COLS; c += 16) {
-            if constexpr (EXPERTS) finish16_tail<KIND>(to, x.tail, row, n, m_first + c, &r[c], rs, csq, biasq, of_lane);
+            if constexpr (EXPERTS) finish16_tail<KIND, LOOSE>(to, x.tail, row, n, m_first + c, &r[c], rs, csq, biasq, of_lane);
             else if constexpr (TAIL)
-              finish16_tail<KIND>(to, x, row, n, m_first + c, &r[c], rs, csq, biasq, of_lane, q == 0 && ahead.valid ? ahead.w + c / 2 : nullptr);
-            else if (TR) finish16_tr<KIND, ACT>(to, row, n, m_first + c, &r[c], rs, csq, biasq);
+              finish16_tail<KIND, LOOSE>(to, x, row, n, m_first + c, &r[c], rs, csq, biasq, of_lane, q == 0 && ahead.valid ? ahead.w + c / 2 : nullptr);
+            else if (TR) finish16_tr<KIND, ACT, LOOSE>(to, row, n, m_first + c, &r[c], rs, csq, biasq);
             else finish16<KIND, ACT>(to, row, n, m_first + c, &r[c], rs, csq, biasq);
           }
         }
@@ -456,8 +457,12 @@ int launch_rowacc(const RowaccLaunch& l) {
 template <int KIND, class C>
 int launch_rowacc(const RowaccLaunch& l) {
   if constexpr (KIND != VOID_KIND_F8E4M3 && (KIND != VOID_KIND_I8 || C::COLS == kTile)) {
+    if (l.transposed && (l.epilogue & kTail) && (l.epilogue & kLoose))
+      return l.transposed == 1 ? launch_rowacc<KIND, C, 1, kActive | kTail | kLoose>(l) : launch_rowacc<KIND, C, 2, kActive | kTail | kLoose>(l);
     if (l.transposed && (l.epilogue & kTail))
       return l.transposed == 1 ? launch_rowacc<KIND, C, 1, kActive | kTail>(l) : launch_rowacc<KIND, C, 2, kActive | kTail>(l);
+    if (l.transposed && (l.epilogue & kLoose))
+      return l.transposed == 1 ? launch_rowacc<KIND, C, 1, kActive | kLoose>(l) : launch_rowacc<KIND, C, 2, kActive | kLoose>(l);
     if (l.transposed)
       return l.transposed == 1
                  ? (l.epilogue & kActive ? launch_rowacc<KIND, C, 1, kActive>(l) : launch_rowacc<KIND, C, 1, 0>(l))
@@ -497,7 +502,8 @@ int launch_rowacc(const RowaccLaunch& l) {
 
 template <int KIND>
 int launch_experts(const ExpertLaunch& l) {
-  auto kernel = spmm_rowacc_kernel<KIND, Mid, 1, kActive | kTail | kExperts>;
+  constexpr int kEpilogue = kActive | kTail | kExperts;
+  auto kernel = l.loose ? spmm_rowacc_kernel<KIND, Mid, 1, kEpilogue | kLoose> : spmm_rowacc_kernel<KIND, Mid, 1, kEpilogue>;
   if (ensure_smem((const void*)kernel, l.smem_bytes)) return VOID_ERR_CUDA;
   return status_of(launch_pdl(kernel, l.grid, Mid::THREADS, l.smem_bytes, l.stream, l.b, l.x, l.p));
 }

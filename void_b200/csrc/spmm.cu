@@ -354,6 +354,8 @@ static int spmm_launch(const void_spmm_args* a, int kind, cudaStream_t stream, c
   // eight warps with 16 columns each, which also have the registers to ask for the residual ahead.  bf16, us, slim or mid / wide, with a
   // residual and with all of training (z kept, GELU): 4096^2, 90 %, 4096 tokens 47.3 / 45.6 and 65.5 / 60.5; 75 % 86.5 / 82.8 and 100.5 /
   // 95.7; 2048 -> 8192, 80 %, 2048 tokens 45.5 / 44.4 and 63.7 / 59.3; 5008 -> 3008, 85 %, 333 tokens 10.0 / 9.2 and 14.7 / 13.6.
+  const bool loose = tr && (!in_pieces(a->out, a->out_dtype, a->ldc) ||
+                            (tail != nullptr && tail->residual != nullptr && !in_pieces(tail->residual, tail->residual_dtype, tail->ldr)));
   if (a->cta_shape == 0 && es == 2 && tr_b && tail != nullptr && (tail->residual != nullptr || tail->pre != nullptr)) shape = 1;
   if (shape == 0) shape = (!drain && np <= 2) ? ((floating && np == 1 && a->segs == nullptr && !short_rows) ? 1 : 2) : ((drain && np == 1) ? kDefaultDrainShape : 1);
   if (shape == 2 && (np > 2 || (drain && np > 1))) return VOID_ERR_BAD_ARG;
@@ -568,9 +570,9 @@ static int spmm_launch(const void_spmm_args* a, int kind, cudaStream_t stream, c
   const bool traced = a->trace != nullptr;
   if (!drain) {
     const bool split = a->segs != nullptr || a->acc_out != nullptr || a->worker_partials != nullptr;
-    const bool active = split || traced || tail != nullptr || a->act != VOID_ACT_NONE || a->row_bias != nullptr;
+    const bool active = split || traced || loose || tail != nullptr || a->act != VOID_ACT_NONE || a->row_bias != nullptr;
     const int epilogue = (staged ? kStaged : 0) | (split ? kSplit : 0) | (active ? kActive : 0) | (traced ? kTraced : 0) |
-                         (tail != nullptr ? kTail : 0);
+                         (tail != nullptr ? kTail : 0) | (loose ? kLoose : 0);
     const Tail none = {};
     const RowaccLaunch l = {shape, a->transposed, epilogue, grid, smem_bytes, stream, tmap, tmap_c, peers, tail != nullptr ? *tail : none, p};
     return kind == VOID_KIND_I8       ? launch_rowacc<VOID_KIND_I8>(l)
