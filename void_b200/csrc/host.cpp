@@ -13,6 +13,7 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
@@ -1332,6 +1333,21 @@ at::Tensor gradient_of_values(const Structure& st, const at::Tensor& g_in, const
 void no_second_derivative(const char* what) {
   TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled(), what, " has no second derivative: its backward pass cannot be recorded (create_graph=True)");
 }
+// A backward pass that is captured into a graph, towards a leaf that an eager graph which still lives belongs to: the leaf's gradient
+// would be handed over on the legacy default stream, where its node was made, and a wait of that stream on a captured one ends the
+// process.  Refused here, where it is still an error like others.
+void no_eager_leaf(const torch::autograd::Node& node) {
+  const c10::cuda::CUDAStream here = c10::cuda::getCurrentCUDAStream();
+  if (!capturing(here.stream())) return;
+  for (size_t i = 0; i < node.num_outputs(); ++i) {
+    const auto leaf = std::dynamic_pointer_cast<torch::autograd::AccumulateGrad>(node.next_edge(i).function);
+    if (leaf == nullptr || !node.task_should_compute_output(i)) continue;
+    const auto stream = leaf->stream();
+    TORCH_CHECK(!stream.has_value() || c10::cuda::CUDAStream(*stream).stream() != nullptr,
+                "a backward pass cannot be captured while a graph of the same leaves that was recorded on the default stream lives: delete its "
+                "outputs first, or record it on a side stream");
+  }
+}
 at::Tensor column_sums(const at::Tensor& m) {
   at::Tensor out = new_cuda({m.size(1)}, m.scalar_type(), m.device());
   check(void_column_sum(m.const_data_ptr(), out_code(m.scalar_type()), std::max<int64_t>(m.stride(0), m.size(1)), (int32_t)m.size(0),
@@ -1387,6 +1403,7 @@ struct ProductBackward : torch::autograd::Node {
     at::Tensor g = grads[0].contiguous();
     if (task_should_compute_output(3)) out[3] = grads[0];
     c10::cuda::OptionalCUDAGuard guard(b.device());
+    no_eager_leaf(*this);
     // (a backward pass that is recorded itself gets the bias gradient from an operator that can be differentiated)
     if (task_should_compute_output(2) && at::GradMode::is_enabled()) out[2] = g.sum(0);
     at::AutoDispatchBelowADInplaceOrView below;
@@ -1627,6 +1644,7 @@ struct ExpertBackward : torch::autograd::Node {
     no_second_derivative("a layer of experts");
     const at::Tensor v = values.unpack(), x = dense.unpack();
     c10::cuda::OptionalCUDAGuard guard(x.device());
+    no_eager_leaf(*this);
     at::AutoDispatchBelowADInplaceOrView below;
     try {
       const c10::Device dev = x.device();
@@ -1745,6 +1763,7 @@ struct NormBackward : torch::autograd::Node {
     no_second_derivative("the layer norm");
     const at::Tensor xs = x.unpack(), given = weight.unpack();   // (raises where the graph has been freed)
     c10::cuda::OptionalCUDAGuard guard(xs.device());
+    no_eager_leaf(*this);
     at::AutoDispatchBelowADInplaceOrView below;
     const at::Tensor w = given.defined() ? given.contiguous() : given;
     const at::Tensor rows = token_rows(xs), g = token_rows(as_type(grads[0], xs.scalar_type()));
