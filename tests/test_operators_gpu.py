@@ -86,6 +86,27 @@ def test_experts_into_a_result_that_lies_anyhow(each, dtype):
     void.check_device_status()
 
 
+@pytest.mark.parametrize("each", [3, 7, 60, 200])
+def test_infinities_of_other_tokens_stay_with_them(each):
+    counts = [each, 2, 2 * each - 1, 0, 1]
+    weights, e = experts_of(5, 72, 96, 0.5, torch.float16)
+    tokens, offsets = sum(counts) + 5, offsets_of(counts, 2)
+    x, bias = rand(tokens, 96, dtype=torch.float16), rand(5, 72, seed=1)
+    clean = void.void_expert_linear(e, x, offsets, bias, 3)
+    bad, rows = x.clone(), torch.ones(tokens, dtype=torch.bool, device="cuda")
+    for at, value in ((0, "nan"), (1, "inf"), (2 + each, "nan"), (tokens - 4, "-inf"), (tokens - 1, "nan"), (4 + each, "inf")):
+        bad[at], rows[at] = float(value), False
+    y = void.void_expert_linear(e, bad, offsets, bias, 3)
+    assert torch.equal(y[rows], clean[rows])
+    assert not y[[0, 1, tokens - 1]].any() and not y[2 + each].isfinite().any()
+
+
+def test_a_result_of_experts_that_is_its_input_is_refused():
+    e, x = experts_of(2, 64, 64, 0.5, torch.float16)[1], rand(10, 64, dtype=torch.float16)
+    with pytest.raises(_lib.VoidB200Error, match="must not be x"):
+        void.void_expert_linear(e, x, offsets_of([4, 6]), out=x)
+
+
 DROP_FIRST_GROUP = 1 << 16
 
 

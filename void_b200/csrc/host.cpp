@@ -1527,6 +1527,7 @@ PyObject* expert_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (out.dim() != 2 || out.size(0) != N || out.size(1) != M || (M > 1 && out.stride(1) != 1) || (N > 1 && out.stride(0) < M))
       fail("out must be a row-major [" + std::to_string(N) + ", " + std::to_string(M) + "] tensor");
     if (out.device() != dev) fail("out and x are on different devices");
+    if (N > 0 && out.const_data_ptr() == x_in.const_data_ptr()) fail("out must not be x: every tile row of the experts reads all of a token");
   }
   ExpertPlan plan = expert_plan(offsets, N, experts, dev, pk->args.status);
   const at::Tensor x = kernel_operand(x_in, es);

@@ -96,7 +96,7 @@ def void_expert_linear(experts: VOIDExperts, x: torch.Tensor, offsets: torch.Ten
     """y[t] = act(x[t] @ A_e^T + bias[e]) for the tokens offsets[e] <= t < offsets[e + 1] of every expert e; x [tokens, in] in
     float32 (multiplied as TF32), float16 or bfloat16, sorted by expert, y [tokens, out] in x's type.  ``offsets`` is int32 or int64
     [n_experts + 1] on x's device and is not read by the host: a captured call may be replayed with others.  ``bias`` is
-    [n_experts, out].  Rows in no run (before the first offset, behind the last) are zeros; with ``out`` they are left as they are.
+    [n_experts, out].  Rows in no run (before the first offset, behind the last) are zeros; with ``out`` (which must not be x) they are left as they are.
     Offsets that fall or lie outside the batch are taken as empty runs and reported by check_device_status.  Inference form of
     SparseExperts: nothing is differentiated."""
     if not isinstance(experts, VOIDExperts):
