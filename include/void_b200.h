@@ -463,11 +463,12 @@ VOID_API int void_activation_grad(const void* g, int64_t ldg, const void* z, int
  * taken).  Experts without tokens get zeros.  ws: void_expert_activation_grad_ws_bytes bytes, needed with dbias.
  * ------------------------------------------------------------------------------------- */
 typedef struct void_experts {
-  const int32_t* plan;       /* of void_expert_plan */
+  const int32_t* plan;       /* of void_expert_plan; for void_expert_linear with up to 32 experts also the offsets themselves */
   int32_t n_experts, chunk;
   const int32_t* row_order;  /* [n_experts * nbr]: tile row (within its expert) of the k-th row taken, or NULL for k; entries are
                                 clamped, see void_spmm_args.row_order */
-  int32_t zero_rest, reserved;
+  int32_t zero_rest;
+  int32_t offset_bytes;      /* 0: plan is a plan; 4 or 8: it is the offsets, of that many bytes each */
 } void_experts;
 VOID_API int64_t void_expert_plan_words(int32_t n_experts, int32_t rows, int32_t chunk);
 VOID_API int void_expert_plan(const void* offsets, int32_t offset_bytes, int32_t n_experts, int32_t rows, int32_t chunk, int32_t* plan,

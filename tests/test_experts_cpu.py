@@ -70,6 +70,8 @@ def _linear(args=(), experts=(), tail=None, kind=_lib.KIND_F16):
     (dict(args=dict(ldb=62)), ALIGN), (dict(args=dict(ldb=48)), ALIGN), (dict(args=dict(tiles=1040)), ALIGN), (dict(args=dict(b=1032)), ALIGN),
     (dict(experts=dict(n_experts=0)), BAD_ARG), (dict(experts=dict(chunk=48)), BAD_ARG), (dict(experts=dict(chunk=0)), BAD_ARG),
     (dict(experts=dict(plan=None)), BAD_ARG), (dict(experts=dict(plan=1032)), ALIGN),
+    (dict(experts=dict(offset_bytes=3)), BAD_ARG), (dict(experts=dict(offset_bytes=4, n_experts=33)), BAD_ARG),
+    (dict(experts=dict(offset_bytes=8, plan=1028)), ALIGN), (dict(experts=dict(offset_bytes=4, plan=1026)), ALIGN),
     (dict(tail=dict(residual=1024, ldr=32)), BAD_ARG), (dict(tail=dict(pre=1024, ldp=31)), BAD_ARG),
     (dict(args=dict(N=2 ** 30, nbr=2 ** 20, M=2 ** 25, ldc=2 ** 25)), TOO_LARGE),
 ])
@@ -94,7 +96,7 @@ def test_grouped_form_refuses():
         return st
     assert lib.void_expert_grouped(None, None, ctypes.byref(x), ctypes.byref(g), _lib.KIND_F16, None) == BAD_ARG
     assert call() == BAD_ARG                                     # an empty store
-    for bad in (dict(kind=_lib.KIND_I8), dict(chunk=32), dict(n_experts=0), dict(plan=None), dict(transposed=2), dict(col_scale=1024), dict(row_scale=1024)):
+    for bad in (dict(kind=_lib.KIND_I8), dict(chunk=32), dict(n_experts=0), dict(plan=None), dict(offset_bytes=4), dict(transposed=2), dict(col_scale=1024), dict(row_scale=1024)):
         assert call(**bad) == BAD_ARG, bad
     g.blob = g.records = g.stage_ptr = g.group_rows = 1024
     g.max_entries = g.max_tiles = 1
@@ -133,6 +135,13 @@ def test_activation_gradient_refuses(bad, status):
     x = _lib.Experts(plan=v["plan"], n_experts=v["n_experts"], chunk=v["chunk"])
     assert _lib.load().void_expert_activation_grad(ptr(v["g"]), v["ldg"], ptr(v["z"]), v["ldz"], v["elem"], ctypes.byref(x), v["rows"], v["cols"], v["act"],
                                                    ptr(v["dz"]), v["lddz"], ptr(v["db"]), v["be"], ptr(v["ws"]), v["ws_bytes"], None) == status
+
+
+def test_offsets_stand_for_a_plan_in_the_product_alone():
+    lib, p = _lib.load(), ctypes.c_void_p(1024)
+    x = _lib.Experts(plan=1024, n_experts=2, chunk=8, offset_bytes=4)
+    assert lib.void_expert_tile_grad(p, 64, p, 64, 32, 32, 4, _lib.KIND_F16, ctypes.byref(x), p, 1, p, p, p, 1, None, None) == BAD_ARG
+    assert lib.void_expert_activation_grad(p, 8, p, 8, 1, ctypes.byref(x), 4, 8, 2, p, 8, p, 1, p, 1 << 40, None) == BAD_ARG
 
 
 def test_stacking_and_its_refusals():

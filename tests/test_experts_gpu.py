@@ -44,7 +44,8 @@ CASES = [
     (2, 515, 333, [31, 33], 0, 0), (8, 1024, 640, [0, 700, 1, 129, 128, 127, 0, 3], 0, 0), (5, 128, 64, [128, 256, 0, 1, 130], 7, 60),
     (3, 96, 64, [0, 0, 0], 0, 10), (40, 64, 64, [3, 0, 9, 1] * 10, 0, 0), (70, 64, 33, [100 * (e % 7 == 3) + e % 3 for e in range(70)], 1, 5),
     (1500, 32, 32, [e % 4 for e in range(1500)], 0, 2), (2, 2048, 1000, [1000, 1300], 0, 17),
-    (6, 130, 96, [40, 0, 1, 0, 3, 0], 0, 1), (2, 640, 300, [190, 1], 0, 0), (3, 1500, 90, [20, 2, 0], 1, 0), (2, 1500, 70, [4, 2], 0, 0),
+    (6, 130, 96, [40, 0, 1, 0, 3, 0], 0, 1), (2, 640, 300, [190, 1], 0, 0), (3, 1500, 90, [20, 2, 0], 1, 0),
+    (32, 64, 64, [e % 5 for e in range(31)] + [40], 3, 2), (33, 64, 64, [9] + [e % 3 for e in range(32)], 0, 1), (32, 64, 40, [0] * 31 + [300], 0, 0), (2, 1500, 70, [4, 2], 0, 0),
 ]
 
 

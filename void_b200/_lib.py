@@ -56,7 +56,7 @@ class Epilogue(ctypes.Structure):
 
 class Experts(ctypes.Structure):
     """Mirror of ``struct void_experts``."""
-    _fields_ = [("plan", c_vp), ("n_experts", c_i32), ("chunk", c_i32), ("row_order", c_vp), ("zero_rest", c_i32), ("reserved", c_i32)]
+    _fields_ = [("plan", c_vp), ("n_experts", c_i32), ("chunk", c_i32), ("row_order", c_vp), ("zero_rest", c_i32), ("offset_bytes", c_i32)]
 
 
 class GroupStore(ctypes.Structure):

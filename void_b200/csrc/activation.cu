@@ -291,7 +291,7 @@ int void_expert_activation_grad(const void* g, int64_t ldg, const void* z, int64
                                 int32_t cols, int32_t act, void* dz, int64_t lddz, void* dbias, int32_t bias_elem, void* ws, size_t ws_bytes,
                                 void_stream_t stream) {
   using namespace vb;
-  if (x == nullptr || x->plan == nullptr || x->n_experts < 1 || x->chunk < 1) return VOID_ERR_BAD_ARG;
+  if (x == nullptr || x->plan == nullptr || x->offset_bytes != 0 || x->n_experts < 1 || x->chunk < 1) return VOID_ERR_BAD_ARG;
   if (elem < VOID_ELEM_F32 || elem > VOID_ELEM_BF16 || rows < 0 || cols < 0 || act < VOID_ACT_NONE || act > VOID_ACT_SILU) return VOID_ERR_BAD_ARG;
   if (ldg < cols || (z != nullptr && ldz < cols) || (dz != nullptr && lddz < cols)) return VOID_ERR_BAD_ARG;
   if (dbias != nullptr && bias_elem != elem && bias_elem != VOID_ELEM_F32) return VOID_ERR_BAD_ARG;

@@ -399,6 +399,8 @@ struct ExpertParams {
   const int32_t* head;        // number of chunks
   const int32_t* bounds;      // [experts + 1]: where the experts' runs of tokens begin, and the end of the last
   const int4* chunks;         // expert, first token, token behind the last
+  const void* offsets;        // or, for these three: the runs' offsets themselves, of up to 32 experts (RunTable)
+  int offset_bytes, chunk;    // of one of them; tokens of a chunk
   const int32_t* row_order;   // [experts][tile rows]: tile row of the k-th row taken, or null for k
   int n_experts, zero_rest;   // zero_rest: tokens outside all runs get zeros
   int panel_bytes;            // of a panel in shared memory (row kernel): as many tokens as a chunk has
@@ -407,9 +409,63 @@ struct Nothing {};
 template <class X>
 constexpr bool kExpertsOf = std::is_same<X, ExpertParams>::value;
 
-// Zeros for the tokens in no expert's run, dealt out over the CTAs.
+// The plan of up to 32 experts as a warp makes it for itself, expert e's run and first chunk in lane e, as expert_plan_kernel would: a few
+// steps of shuffles for a launch of two or three microseconds.  For whole warps, behind the wait on the kernel before.
+struct RunTable {
+  int begin, end, first, total;   // tokens; chunks before the run's, chunks in all
+  bool bad;                       // the offsets are not as given
+  __device__ __forceinline__ RunTable(const ExpertParams& x, int rows) {
+    const int lane = threadIdx.x & 31, e = lane < x.n_experts ? lane : x.n_experts - 1;
+    auto offset = [&](int i) {
+      return x.offset_bytes == 8 ? reinterpret_cast<const long long*>(x.offsets)[i] : (long long)reinterpret_cast<const int32_t*>(x.offsets)[i];
+    };
+    auto inside = [&](long long o) { return o < 0 ? 0 : (o > rows ? rows : (int)o); };
+    const long long from = offset(0), to = offset(e + 1);
+    const int low = inside(from);
+    end = inside(to);
+    if (end < low) end = low;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, end, o);
+      if (lane >= o && u > end) end = u;
+    }
+    begin = __shfl_up_sync(0xffffffffu, end, 1);
+    if (lane == 0) begin = low;
+    const int shift = __ffs(x.chunk) - 1, mine = (end - begin + x.chunk - 1) >> shift;
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += u;
+    }
+    first = upto - mine;
+    total = __shfl_sync(0xffffffffu, upto, 31);
+    bad = from != low || to != end;
+  }
+  // chunk c < total of each lane, as x.chunks has it: the last expert whose first chunk is not behind it
+  __device__ __forceinline__ int4 chunk(const ExpertParams& x, int c) const {
+    int e = 0;
+#pragma unroll 4
+    for (int k = 1; k < 32; ++k) {
+      const int f = __shfl_sync(0xffffffffu, first, k);
+      if (k < x.n_experts && f <= c) e = k;
+    }
+    const int n0 = __shfl_sync(0xffffffffu, begin, e) + (c - __shfl_sync(0xffffffffu, first, e)) * x.chunk, stop = __shfl_sync(0xffffffffu, end, e);
+    return make_int4(e, n0, n0 + x.chunk < stop ? n0 + x.chunk : stop, 0);
+  }
+};
+// Zeros for the tokens in no expert's run, dealt out over the CTAs.  For whole warps.
 __device__ __forceinline__ void zero_rest_rows(const OutDesc& o, const ExpertParams& x, int tid, int threads) {
-  const int before = x.bounds[0], behind = x.bounds[x.n_experts], rest = before + o.N - behind;
+  int before, behind;
+  if (x.offsets != nullptr) {
+    const RunTable runs(x, o.N);
+    before = __shfl_sync(0xffffffffu, runs.begin, 0);
+    behind = __shfl_sync(0xffffffffu, runs.end, 31);
+  } else {
+    before = x.bounds[0];
+    behind = x.bounds[x.n_experts];
+  }
+  const int rest = before + o.N - behind;
   for (int i = blockIdx.x; i < rest; i += gridDim.x) {
     const size_t first = (size_t)(i < before ? i : i - before + behind) * (size_t)o.ldc;
     if (o.dtype == VOID_OUT_F32)

@@ -3,7 +3,7 @@
 //     out_t = act(x_t A_e^T + bias_e)          offsets[e] <= t < offsets[e + 1]
 //
 // The weights are one packed store, expert behind expert; the runs are cut into chunks of tokens on the device (the host does not
-// know the offsets), and a work item is (chunk, tile row).  The products themselves are those of rowacc.cuh (chunks of 32, 64 or 128
+// know the offsets; by a kernel of one block, or for up to 32 experts by each warp for itself, RunTable), and a work item is (chunk, tile row).  The products themselves are those of rowacc.cuh (chunks of 32, 64 or 128
 // tokens, B and C as they lie) and, for a handful of tokens per expert, of skinny.cu (chunks of 8).  A chunk never spans two experts: what
 // a tile load brings beyond its end belongs to rows of the result that are not stored.
 #include "experts.cuh"
@@ -13,7 +13,7 @@ namespace vb {
 
 namespace {
 
-constexpr int kPlanThreads = 1024, kStatusBadOffsets = 3;
+constexpr int kPlanThreads = 1024;
 
 struct Max { __device__ __forceinline__ int operator()(int a, int b) const { return a > b ? a : b; } };
 struct Sum { __device__ __forceinline__ int operator()(int a, int b) const { return a + b; } };
@@ -100,6 +100,8 @@ int experts_launch(const void_spmm_args* a, const void_epilogue* e, const void_e
   if (x->chunk != 8 && x->chunk != 32 && x->chunk != 64 && x->chunk != kPanelN) return VOID_ERR_BAD_ARG;
   if (a->M == 0 || a->N == 0) return VOID_OK;
   if (a->out == nullptr || a->row_ptr == nullptr || x->plan == nullptr) return VOID_ERR_BAD_ARG;
+  const bool given = x->offset_bytes != 0;   // offsets in the place of a plan: the kernels make it, warp by warp
+  if (given && ((x->offset_bytes != 4 && x->offset_bytes != 8) || x->n_experts > 32)) return VOID_ERR_BAD_ARG;
   if (a->nnz > 0 && (a->tiles == nullptr || a->tile_cols == nullptr || a->b == nullptr)) return VOID_ERR_BAD_ARG;
   if (a->out_dtype < VOID_OUT_F32 || a->out_dtype > VOID_OUT_BF16 || a->act < VOID_ACT_NONE || a->act > VOID_ACT_SILU) return VOID_ERR_BAD_ARG;
   if (a->transposed != 1 || a->scale_mode != VOID_SCALE_ROW_MEAN || a->row_scale != nullptr || a->col_scale != nullptr || a->bias != nullptr ||
@@ -111,7 +113,7 @@ int experts_launch(const void_spmm_args* a, const void_epilogue* e, const void_e
   if ((long long)a->nbr * kTile < a->M || a->ldc < a->M) return VOID_ERR_SHAPE;
   const int es = kind == VOID_KIND_TF32 ? 4 : 2;
   if ((reinterpret_cast<uintptr_t>(a->tiles) & 1023u) != 0 || (reinterpret_cast<uintptr_t>(a->b) & 15u) != 0 || (a->ldb & 15) != 0 ||
-      a->ldb < (long long)a->K * es || (reinterpret_cast<uintptr_t>(x->plan) & 15u) != 0)
+      a->ldb < (long long)a->K * es || (reinterpret_cast<uintptr_t>(x->plan) & (given ? x->offset_bytes - 1u : 15u)) != 0)
     return VOID_ERR_ALIGN;
   const PlanView v = plan_of(*x, a->N);
   if ((long long)v.capacity * a->nbr > 0x7fffffffll) return VOID_ERR_TOO_LARGE;
@@ -149,7 +151,7 @@ int experts_launch(const void_spmm_args* a, const void_epilogue* e, const void_e
   memset(&tmap, 0, sizeof(tmap));
   if (a->nnz > 0 && !panel_map_transposed(&tmap, a->b, a->ldb, a->K, a->N, es, x->chunk, !few)) return VOID_ERR_TENSOR_MAP;
   const int panel = x->chunk * kTile * es;
-  const ExpertParams experts = {tail, v.head, v.bounds, v.chunks, x->row_order, x->n_experts, x->zero_rest, panel};
+  const ExpertParams experts = {tail, v.head, v.bounds, v.chunks, given ? x->plan : nullptr, x->offset_bytes, x->chunk, x->row_order, x->n_experts, x->zero_rest, panel};
   if (few) return expert_stream_launch(p, experts, kind, tmap, items, dev, st);
   p.np = 1;
   p.terms = 1;

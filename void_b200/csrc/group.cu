@@ -758,7 +758,7 @@ int void_expert_grouped(const void_spmm_args* a, const void_epilogue* e, const v
                         void_stream_t stream) {
   using namespace vb;
   if (a == nullptr || x == nullptr || s == nullptr) return VOID_ERR_BAD_ARG;
-  if (x->plan == nullptr || x->n_experts < 1 || x->chunk != kPanelN || a->transposed != 1 || kind == VOID_KIND_I8) return VOID_ERR_BAD_ARG;
+  if (x->plan == nullptr || x->offset_bytes != 0 || x->n_experts < 1 || x->chunk != kPanelN || a->transposed != 1 || kind == VOID_KIND_I8) return VOID_ERR_BAD_ARG;
   if (a->row_scale != nullptr || a->col_scale != nullptr || a->bias != nullptr) return VOID_ERR_BAD_ARG;
   Tail tail = {};
   if (e != nullptr) {
@@ -768,7 +768,7 @@ int void_expert_grouped(const void_spmm_args* a, const void_epilogue* e, const v
   }
   if (a->M == 0 || a->N == 0) return VOID_OK;
   const PlanView v = plan_of(*x, a->N);
-  const ExpertParams experts = {tail, v.head, v.bounds, v.chunks, nullptr, x->n_experts, x->zero_rest, 0};
+  const ExpertParams experts = {tail, v.head, v.bounds, v.chunks, nullptr, 0, x->chunk, nullptr, x->n_experts, x->zero_rest, 0};
   return spmm_grouped(a, s, kind, nullptr, stream, &experts, v.capacity);
 }
 int void_spmm_grouped_linear(const void_spmm_args* a, const void_epilogue* e, const void_group_store* s, int32_t kind, void_stream_t stream) {

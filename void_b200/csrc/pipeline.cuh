@@ -95,6 +95,7 @@ constexpr int kDefaultDrainShape = 2;   // cta_shape the one-panel per-tile kern
 // device status codes (written to the status word)
 constexpr int kStatusTimeout = 1;
 constexpr int kStatusBadPlan = 2;   // a split row of the plan points outside the scratch the caller provided
+constexpr int kStatusBadOffsets = 3;   // offsets of experts' runs that fall or lie outside the batch
 
 // The order in which the work items (tile row, chunk of columns) of a launch without a plan are taken: pass by pass over all
 // tile rows, a pass with the chunks whose part of B stays in L2 while every tile fetches its panels from it.  A is read once
@@ -213,10 +214,12 @@ struct ExpertItems {
     const int lane = threadIdx.x & 31;
     if (ready == 0) {
       ready = 32;
-      const long long mine = (long long)i + (long long)lane * step;
-      if (mine < end) {
-        const int c = (int)mine / p.nbr, k = (int)mine - c * p.nbr;
-        const int4 chunk = x.chunks[c];
+      const long long at = (long long)i + (long long)lane * step;
+      const int mine = at < end ? (int)at : i, c = mine / p.nbr, k = mine - c * p.nbr;
+      int4 chunk = make_int4(0, 0, 0, 0);
+      if (x.offsets != nullptr) chunk = RunTable(x, p.N).chunk(x, c);
+      if (at < end) {
+        if (x.offsets == nullptr) chunk = x.chunks[c];
         expert = chunk.x;
         n0 = chunk.y;
         n1 = chunk.z;
@@ -225,9 +228,9 @@ struct ExpertItems {
           const int r = x.row_order[(size_t)expert * p.nbr + k];
           row = r < 0 ? 0 : (r >= p.nbr ? p.nbr - 1 : r);
         }
-        const int32_t* at = p.row_ptr + (size_t)expert * p.nbr + row;
-        t0 = at[0];
-        t1 = at[1];
+        const int32_t* tiles = p.row_ptr + (size_t)expert * p.nbr + row;
+        t0 = tiles[0];
+        t1 = tiles[1];
       }
     }
     const int from = 32 - ready--;
@@ -242,6 +245,10 @@ struct ExpertItems {
     return s;
   }
 };
+// Whether the offsets were as given, told by one warp of the launch.
+__device__ __forceinline__ void report_offsets(const SpmmParams& p, const ExpertParams& x) {
+  if (blockIdx.x == 0 && x.offsets != nullptr && RunTable(x, p.N).bad && p.status != nullptr) atomicCAS(p.status, 0, kStatusBadOffsets);
+}
 struct NoItems {};
 template <class X>
 using ItemsOf = std::conditional_t<kExpertsOf<X>, ExpertItems, NoItems>;
@@ -291,7 +298,7 @@ template <bool PLAN, class X = Nothing>
 __device__ __forceinline__ void seg_range(const SpmmParams& p, int& begin, int& end, int& step, const X& x = X{}) {
   if constexpr (kExpertsOf<X>) {
     begin = blockIdx.x;
-    end = x.head[0] * p.nbr;
+    end = (x.offsets != nullptr ? RunTable(x, p.N).total : x.head[0]) * p.nbr;
     step = gridDim.x;
   } else if (PLAN && p.segs != nullptr) {
     begin = p.cta_seg_ptr[blockIdx.x];

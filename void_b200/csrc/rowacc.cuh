@@ -187,8 +187,10 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM) spmm_rowacc_kernel
     ItemsOf<Runs> items;
     if (!EXPERTS && begin < end) seg_next = load_seg_word<SPLIT>(p, begin, lane);
     if (p.a_stable) grid_dependency_wait();
-    if constexpr (EXPERTS)
+    if constexpr (EXPERTS) {
+      if (epi_tid < 32) report_offsets(p, x);
       if (x.zero_rest) zero_rest_rows(od, x, epi_tid, C::EPI_THREADS);
+    }
     if (epi_tid == 0) stamp<TRACE>(p, 0);
     for (int i = begin; i < end; i += step, ++it) {
       const int seg = seg_next;

@@ -318,7 +318,8 @@ __global__ void __launch_bounds__(512) skinny_kernel(const __grid_constant__ Par
 // tokens come through a ring in shared memory (producer_loop of pipeline.cuh, panels without a swizzle): a stage is four tiles, one per
 // warp, which keeps its sums in registers to the end of the row.  The weights are read once and that bounds it, so the ring keeps 120 KB
 // of an SM in flight; a CTA per item instead, every warp with loads of its own, is a chain of five latencies of which one carries the
-// weights.  8 experts of 2048 -> 8192, 80 % (54 MB): 8 tokens 18.0 -> 15.7 us, 32 tokens 23.0 -> 19.9.  What a CTA pays per item on top
+// weights.  8 experts of 2048 -> 8192, 80 % (54 MB): 8 tokens 18.0 -> 15.7 us, 32 tokens 23.0 -> 19.9 (and
+// 14.6 and 18.8 without a launch for the plan).  What a CTA pays per item on top
 // of its bytes - stages that the row does not fill, the sums' exchange - is hidden behind the other CTAs: two of twice the warps 19.0
 // and 22.5, four of them 15.8 and 20.1 but 49 against 45 us with rows four times as long, of which each then takes three or four.
 struct Stream {
@@ -355,6 +356,7 @@ __global__ void __launch_bounds__(Stream::THREADS, Stream::CTAS_PER_SM) expert_s
     float* red = reinterpret_cast<float*>(smem_raw + (ring - smem_u32(smem_raw)) + p.part_off);   // [2][W][32][PITCH]
     grid_dependency_wait();
     const OutDesc od = out_desc(p);
+    if (tid < 32) report_offsets(p, x);
     if (x.zero_rest) zero_rest_rows(od, x, tid, 32 * W);
     int begin, end, step, stage = 0, turn = 0;
     uint32_t phase = 0;

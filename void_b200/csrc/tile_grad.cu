@@ -371,7 +371,7 @@ int void_linear_tile_grad(const void* grad_out, int64_t ldg, const void* x, int6
 int void_expert_tile_grad(const void* grad_out, int64_t ldg, const void* x, int64_t ldx, int32_t M, int32_t K, int32_t N, int32_t kind,
                           const void_experts* experts, const int32_t* items, int32_t n_items, const int32_t* tile_cols,
                           const int32_t* block_indices, void* grad_tiles, int32_t out_dtype, int32_t* status, void_stream_t stream) {
-  if (experts == nullptr || experts->plan == nullptr || experts->n_experts < 1 || M < 1 || N < 1) return VOID_ERR_BAD_ARG;
+  if (experts == nullptr || experts->plan == nullptr || experts->offset_bytes != 0 || experts->n_experts < 1 || M < 1 || N < 1) return VOID_ERR_BAD_ARG;
   const vbg::RunParams runs = {vb::plan_of(*experts, N).bounds, (M + 31) / 32};
   return vbg::tile_grad(grad_out, ldg, x, ldx, M, K, N, kind, items, n_items, tile_cols, block_indices, grad_tiles, out_dtype, status,
                         reinterpret_cast<cudaStream_t>(stream), true, &runs);
