@@ -9,6 +9,7 @@ import void_b200 as void
 from test_experts_gpu import check_forward, experts_of, offsets_of
 from test_linear_cpu import layer64, rounded, within
 from test_linear_gpu import rand, weight
+from test_norm_gpu import check, make
 from void_b200 import _lib
 
 pytestmark = pytest.mark.gpu
@@ -105,6 +106,16 @@ def test_a_result_of_experts_that_is_its_input_is_refused():
     e, x = experts_of(2, 64, 64, 0.5, torch.float16)[1], rand(10, 64, dtype=torch.float16)
     with pytest.raises(_lib.VoidB200Error, match="must not be x"):
         void.void_expert_linear(e, x, offsets_of([4, 6]), out=x)
+
+
+# (rows enough for the blocks that stay, whose threads take sixteen elements one by one up to 6144, and 32 beyond)
+@pytest.mark.parametrize("dtype, params", [(torch.float32, torch.float32), (torch.bfloat16, torch.float32), (torch.float16, torch.float16)])
+@pytest.mark.parametrize("rows, cols", [(1800, 4097), (1900, 5003), (1777, 6143), (1800, 6145), (2300, 4095), (2000, 8191)])
+def test_norm_of_many_rows_that_lie_in_no_pieces(rows, cols, dtype, params):
+    x, w, b, g = make(rows, cols, dtype, params)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    y = void.void_layer_norm(x, w, b)
+    check(x, w, b, g, y, torch.autograd.grad(y, leaves, g))
 
 
 DROP_FIRST_GROUP = 1 << 16

@@ -268,7 +268,7 @@ struct Params {
 // takes many elements and computes in pairs.  16384 x 4096 bf16, eight elements per thread and single operations: 0.70 instructions per
 // clock and scheduler, 72 us; parameters read for every row again: 72 us with fp32 ones, 60 with bf16.
 template <typename T, typename P, int E, int C, int S, int MOST>
-__global__ void __launch_bounds__(MOST, MOST <= 256 ? (C > 16 ? 2 : 3) : 1) layer_norm_rows_kernel(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(MOST, MOST <= 256 ? (C > 16 ? 2 : 3) : (MOST <= 384 ? 2 : 1)) layer_norm_rows_kernel(const __grid_constant__ NormParams p) {
   constexpr int PIECE = (int)sizeof(T) * E, NV = C / E;
   constexpr bool WHOLE = PIECE == 16;
   extern __shared__ __align__(16) uint8_t ring[];
@@ -783,9 +783,8 @@ bool through_ring(long long rows, int cols, int sms) { return rows > 2ll * sms &
 // (forward a block has to walk a few rows before it gains on blocks of one row each: 4096 bf16, 2048 rows 9.8 and 9.2 us, 16384 rows 52 and
 // 68; 5003 fp32, 3001 rows 33 and 46)
 int forward_blocks_per_sm(int cols) { return cols <= 256 * kColumns ? 768 * kColumns / cols : (cols <= 512 * kColumns ? 2 : 1); }
-// Blocks of a launch that fills the SMs: what registers and shared memory leave room for.
-int resident_blocks(const DeviceInfo& dev, long long rows, int threads, int smem, int per_sm_threads) {
-  int per_sm = threads <= 256 ? per_sm_threads / threads : 1;
+// Blocks of a launch that fills the SMs: what registers (per_sm of them) and shared memory leave room for.
+int resident_blocks(const DeviceInfo& dev, long long rows, int smem, int per_sm) {
   const int fit = (dev.smem_per_sm - 4096) / (smem + 2048);
   if (per_sm > fit) per_sm = fit;
   if (per_sm < 1) per_sm = 1;
@@ -804,12 +803,16 @@ cudaError_t forward_rows(NormParams p, const DeviceInfo& dev, cudaStream_t st) {
   p.slot_bytes = ring_slot<T, E, C>(p.cols, threads);
   const int smem = S * (int)p.slot_bytes;
   if (ensure_smem((const void*)kernel, smem)) return cudaErrorInvalidValue;
-  return launch_pdl(kernel, dim3((unsigned)resident_blocks(dev, p.rows, threads, smem, C > kColumns ? 512 : 768)), threads, smem, st, p);
+  const int per_sm = threads <= 256 ? (C > kColumns ? 512 : 768) / threads : (MOST <= 384 ? 2 : 1);
+  return launch_pdl(kernel, dim3((unsigned)resident_blocks(dev, p.rows, smem, per_sm)), threads, smem, st, p);
 }
 // Rows of up to 4096 elements in threads of 16, longer ones in threads of 32 (bf16, GB/s: 4096 5190 and 5060, 8192 4390 and 4770, 16384
-// 3890 and 5290).
+// 3890 and 5290).  Element by element it is a little better to keep 16 as long as two blocks fit an SM (fp32, 5003 elements, 3001 rows 28.4 and
+// 26.4 us, 8000 rows 68.3 and 63.9).
 template <typename T, typename P, int E>
 cudaError_t forward_rows(const NormParams& p, const DeviceInfo& dev, cudaStream_t st) {
+  if constexpr (E == 1)
+    if (p.cols > 256 * kColumns && p.cols <= 384 * kColumns) return forward_rows<T, P, E, kColumns, 384>(p, dev, st);
   if (p.cols <= 256 * kColumns) return forward_rows<T, P, E, kColumns, 256>(p, dev, st);
   return p.cols <= 512 * kColumns ? forward_rows<T, P, E, 2 * kColumns, 256>(p, dev, st) : forward_rows<T, P, E, 2 * kColumns, 512>(p, dev, st);
 }
@@ -854,7 +857,7 @@ cudaError_t backward_rows(NormGradParams p, const DeviceInfo& dev, int* blocks, 
   p.slot_bytes = ring_slot<T, E, C>(p.cols, threads);
   const int smem = 2 * S * (int)p.slot_bytes;
   if (ensure_smem((const void*)kernel, smem)) return cudaErrorInvalidValue;
-  *blocks = resident_blocks(dev, p.rows, threads, smem, 512);
+  *blocks = resident_blocks(dev, p.rows, smem, threads <= 256 ? 512 / threads : 1);
   return launch_pdl(kernel, dim3((unsigned)*blocks), threads, smem, st, p);
 }
 template <typename T, typename P, int E>
