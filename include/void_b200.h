@@ -487,6 +487,13 @@ VOID_API int void_expert_tile_grad(const void* grad_out, int64_t ldg, const void
                                    int32_t kind, const void_experts* experts, const int32_t* items, int32_t n_items,
                                    const int32_t* tile_cols, const int32_t* block_indices, void* grad_tiles, int32_t out_dtype,
                                    int32_t* status, void_stream_t stream);
+/* z [N, M] of such a layer with fp16 or bf16 tiles, where it lies so near to zero that the sums' errors reach its sign, computed again in
+ * 64 bits (ReLU's slope for a backward pass).  x [N, K] and values [nnz, 32, 32] of the kind's type, block_indices the place of each of
+ * row_ptr's tiles in values, bias as in void_epilogue; z on 16 bytes, ldz a multiple of 8.  experts: NULL, or as for void_expert_linear with a
+ * plan (row_ptr and the bias of all experts). */
+VOID_API int void_relu_border(const void* x, int64_t ldx, const void* values, const int32_t* row_ptr, const int32_t* block_indices,
+                              const int32_t* tile_cols, int32_t M, int32_t K, int32_t N, int32_t kind, const void* bias, int32_t bias_dtype,
+                              void* z, int64_t ldz, const void_experts* experts, void_stream_t stream);
 VOID_API size_t void_expert_activation_grad_ws_bytes(const void_experts* experts, int32_t rows, int32_t cols);
 VOID_API int void_expert_activation_grad(const void* g, int64_t ldg, const void* z, int64_t ldz, int32_t elem, const void_experts* experts,
                                          int32_t rows, int32_t cols, int32_t act, void* dz, int64_t lddz, void* dbias, int32_t bias_elem,

@@ -180,3 +180,20 @@ def test_python_operators_refuse_what_they_cannot_do():
         void.SparseLinear(96, 64, a, activation="tanh")
     with pytest.raises(AssertionError, match="w2 must have shape"):
         void.SparseFeedForward(a, a)
+
+
+@pytest.mark.parametrize("bad, status", [
+    (dict(kind=_lib.KIND_TF32), BAD_ARG), (dict(kind=_lib.KIND_I8), BAD_ARG), (dict(M=-1), BAD_ARG), (dict(K=-1), BAD_ARG), (dict(N=-1), BAD_ARG),
+    (dict(ldx=63), BAD_ARG), (dict(ldz=31), BAD_ARG), (dict(bd=5), BAD_ARG), (dict(x=None), BAD_ARG), (dict(values=None), BAD_ARG), (dict(rows=None), BAD_ARG),
+    (dict(at=None), BAD_ARG), (dict(cols=None), BAD_ARG), (dict(z=None), BAD_ARG), (dict(z=8), ALIGN), (dict(ldz=36), ALIGN),
+    (dict(plan=None), BAD_ARG), (dict(plan=1024, offset_bytes=4), BAD_ARG), (dict(plan=1024, n_experts=0), BAD_ARG), (dict(M=0), 0), (dict(N=0), 0),
+])
+def test_relu_border_refuses(bad, status):
+    v = dict(x=16, ldx=64, values=16, rows=16, at=16, cols=16, M=32, K=64, N=4, kind=_lib.KIND_F16, bias=None, bd=0, z=16, ldz=32, offset_bytes=0, n_experts=2)
+    v.update(bad)
+    ptr = lambda p: None if p is None else ctypes.c_void_p(p)   # noqa: E731
+    x = None
+    if "plan" in v:
+        x = ctypes.byref(_lib.Experts(plan=v["plan"], n_experts=v["n_experts"], chunk=8, offset_bytes=v["offset_bytes"]))
+    assert _lib.load().void_relu_border(ptr(v["x"]), v["ldx"], ptr(v["values"]), ptr(v["rows"]), ptr(v["at"]), ptr(v["cols"]), v["M"], v["K"], v["N"], v["kind"],
+                                        ptr(v["bias"]), v["bd"], ptr(v["z"]), v["ldz"], x, None) == status

@@ -118,6 +118,32 @@ def test_norm_of_many_rows_that_lie_in_no_pieces(rows, cols, dtype, params):
     check(x, w, b, g, y, torch.autograd.grad(y, leaves, g))
 
 
+# The slope of ReLU is one where z is positive, however near to zero: with gradients of ones the bias's is the number of such tokens.
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n, k, m, density", [(700, 8192, 2048, 0.3), (300, 5003, 3001, 0.5), (2000, 1024, 1000, 1.0)])
+def test_slopes_next_to_the_border_of_relu(n, k, m, density, dtype):
+    a, x = weight(m, k, density, dtype), rand(n, k, dtype=dtype).requires_grad_(True)
+    layer = void.SparseLinear(k, m, a, dtype=torch.float32, activation="relu")
+    with torch.no_grad():
+        layer.bias.copy_(rand(m, seed=1, scale=0.1))
+    y = layer(x)
+    counts, = torch.autograd.grad(y, (layer.bias,), torch.ones_like(y))
+    z = x.detach().double() @ a.to_dense().double().t() + layer.bias.detach().double()
+    assert torch.equal(counts, (z > 0).sum(0).float())
+    weights, e = experts_of(3, m, k, density, dtype)
+    runs, bias = [n // 2, 0, n // 3], rand(3, m, seed=2, scale=0.1)
+    experts = void.SparseExperts(e, activation="relu", dtype=torch.float32)
+    with torch.no_grad():
+        experts.bias.copy_(bias)
+    y = experts(x, offsets_of(runs, 5))
+    counts, = torch.autograd.grad(y, (experts.bias,), torch.ones_like(y))
+    at = 5
+    for i, c in enumerate(runs):
+        z = x.detach()[at:at + c].double() @ weights[i].to_dense().double().t() + bias[i].double()
+        assert torch.equal(counts[i], (z > 0).sum(0).float())
+        at += c
+
+
 DROP_FIRST_GROUP = 1 << 16
 
 

@@ -114,6 +114,7 @@ _PROTOTYPES = {
     "void_spmm_i8_static_scratch": (ctypes.c_int, [ctypes.POINTER(SpmmArgs), c_i32, c_vp]),
     "void_spmm_linear": (ctypes.c_int, [ctypes.POINTER(SpmmArgs), ctypes.POINTER(Epilogue), c_i32, c_vp]),
     "void_spmm_grouped_linear": (ctypes.c_int, [ctypes.POINTER(SpmmArgs), ctypes.POINTER(Epilogue), ctypes.POINTER(GroupStore), c_i32, c_vp]),
+    "void_relu_border": (ctypes.c_int, [c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_i32, c_i32, c_i32, c_i32, c_vp, c_i32, c_vp, c_i64, c_vp, c_vp]),
     "void_activation_grad_ws_bytes": (c_sz, [c_i32, c_i32]),
     "void_activation_grad": (ctypes.c_int, [c_vp, c_i64, c_vp, c_i64, c_i32, c_i32, c_i32, c_i32, c_vp, c_i64, c_vp, c_i32, c_vp, c_sz,
                                             c_vp]),

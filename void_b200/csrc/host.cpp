@@ -1305,6 +1305,12 @@ at::Tensor product_of_values(const Structure& st, bool a_transposed, const at::T
   }
   if (tail.get() != nullptr && linear && N > 0 && M > 0) check(void_spmm_linear(&s, tail.get(), kind, stream), "void_spmm_linear");
   else check(void_spmm_fp(&s, kind, stream), "void_spmm_fp");
+  if (pre != nullptr && act == VOID_ACT_RELU && es == 2 && st.nnz > 0) {   // (no tiles: z is the bias)
+    const at::Tensor x = K > 1 && (b_typed.stride(1) != 1 || (N > 1 && b_typed.stride(0) < K)) ? b_typed.contiguous() : b_typed;
+    check(void_relu_border(x.const_data_ptr(), N > 1 ? x.stride(0) : K, values.const_data_ptr(), s.row_ptr, st.block_indices[way].const_data_ptr<int32_t>(),
+                           s.tile_cols, (int32_t)M, (int32_t)K, (int32_t)N, kind, s.row_bias, tail.e.bias_dtype, tail.e.pre, tail.e.ldp, nullptr, stream),
+          "void_relu_border");
+  }
   return out;
 }
 
@@ -1629,6 +1635,11 @@ at::Tensor expert_product(const Structure& st, bool a_transposed, const at::Tens
     tail.ldp = pre->stride(0);
   }
   check(void_expert_linear(&s, &tail, &e, kind, stream), "void_expert_linear");
+  if (pre != nullptr && act == VOID_ACT_RELU && es == 2 && st.nnz > 0) {
+    check(void_relu_border(x.const_data_ptr(), N > 1 ? x.stride(0) : K, values.const_data_ptr(), s.row_ptr, st.block_indices[way].const_data_ptr<int32_t>(),
+                           s.tile_cols, (int32_t)M, (int32_t)K, (int32_t)N, kind, s.row_bias, tail.bias_dtype, tail.pre, tail.ldp, &plan.x, stream),
+          "void_relu_border");
+  }
   return out;
 }
 struct ExpertBackward : torch::autograd::Node {
