@@ -219,10 +219,11 @@ __global__ void __launch_bounds__(256) partial_sums_kernel(const float* partials
 
 // Values of z that lie next to ReLU's border, computed again.  The slope there is a question of z's sign, and the tensor cores cut what they hold
 // after every product that they add, by half of 2^-23 of it: z of a row of 108 tiles is off by 1.4e-5 of its size, and 3 of 300 000 slopes came out
-// wrong.  What lies within 2^-21 of its strip's largest value for every tile, ten times as much, is summed in 64 bits, by a block together: of normal values
-// one in ten thousand for such rows.  A strip is 256 columns of a token; a sum of nothing but zeros is right as it is.  us, forward pass with SiLU and
-// with ReLU and this behind it: 4096^2, 90 %, 4096 tokens 51.7 and 71.3; 2048^2, 50 %, 512 tokens 14.0 and 21.2; 14336 -> 14240, 76 %, 44 tokens 75.5
-// and 106.  A warp for each value instead, and 16 tiles on their way at once: 83, 22 and 110.
+// wrong.  What lies within 2^-21 of its strip's largest value for every tile, ten times as much, and for sixteen more, since the errors of a few tiles do
+// not average out, is summed in 64 bits, by a block together: of normal values one in ten thousand for such rows.  A strip is 256 columns of a token; a
+// sum of nothing but zeros is right as it is (what fp16 would round to zero has kept its sign, keep_sign).  us, forward pass with SiLU and with ReLU and
+// this behind it: 4096^2, 90 %, 4096 tokens 52 and 75; 2048^2, 50 %, 512 tokens 14 and 22; 14336 -> 14240, 76 %, 44 tokens 75 and 111.  A warp
+// for each value instead, and 16 tiles on their way at once: 83, 22 and 110.
 constexpr int kStrip = 256, kBorderWarps = 8, kBorderTokens = 4;   // columns of a block, its warps, tokens of a warp at a time
 struct BorderParams {
   const void *x, *values, *bias;
@@ -279,7 +280,7 @@ __global__ void __launch_bounds__(32 * kBorderWarps) relu_border_kernel(const __
         const int e = n < p.N ? expert_of((int)n) : -1;
         tiles = e < 0 ? 0 : tiles_of(e);
       }
-      const float border = most < 1e38f ? (float)tiles * (1.0f / 2097152.0f) * most : 0.0f;
+      const float border = most < 1e38f ? (float)(tiles > 0 ? tiles + 16 : 0) * (1.0f / 2097152.0f) * most : 0.0f;
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         if (v[i] > 0.0f && v[i] < border) list[atomicAdd(&found, 1)] = (uint16_t)((warp * kBorderTokens + k) << 8 | (lane * 8 + i));

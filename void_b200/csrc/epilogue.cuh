@@ -573,6 +573,14 @@ __device__ __forceinline__ float bias_of_lane(const float* bias, int dtype, int 
   if (dtype == VOID_OUT_F32) return bias[m];
   return f16_value(reinterpret_cast<const uint16_t*>(bias)[m], dtype == VOID_OUT_F16);
 }
+// Of a z that is kept, ReLU's slope asks the sign: what fp16 would round to zero keeps it (fp16's smallest step), and a sum that its bias takes to
+// nothing stays next to zero, to be computed again (relu_border_kernel).
+constexpr float kLeast = 5.9604645e-8f;
+__device__ __forceinline__ float keep_sign(float z) { return z != 0.0f && fabsf(z) < kLeast ? copysignf(kLeast, z) : z; }
+__device__ __forceinline__ float with_bias(float sum, float bias, bool signs) {
+  const float z = sum + bias;
+  return signs && z == 0.0f && sum != 0.0f ? kLeast : z;
+}
 // finish16_tr with the rest of a linear layer: z = dequantised accumulator + bias, kept where asked; act(z) + residual.  For whole
 // warps: of_lane is bias_of_lane.  ahead: the residual where it is there already.
 template <int KIND, bool LOOSE = false>
@@ -582,11 +590,23 @@ __device__ __forceinline__ void finish16_tail(const OutDesc& o, const Tail& t, i
   if (c0 >= o.M) return;
   float v[16];
   finished<KIND, 8, false>(o, c0, r, row_scale, cs, bias_n, v);
-  if (o.row_bias != nullptr)
+  if (o.row_bias != nullptr) {
+    if (t.pre != nullptr && o.act == VOID_ACT_RELU) {
 #pragma unroll
-    for (int k = 0; k < 16; ++k) v[k] += __shfl_sync(0xffffffffu, of_lane, m0 + k);
+      for (int k = 0; k < 16; ++k) v[k] = with_bias(v[k], __shfl_sync(0xffffffffu, of_lane, m0 + k), true);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 16; ++k) v[k] += __shfl_sync(0xffffffffu, of_lane, m0 + k);
+    }
+  }
   if (!LOOSE && n >= o.N) return;
-  if (t.pre != nullptr) store16_rows<false>(t.pre, o.dtype, t.ldp, n, o.N, c0, o.M, v);
+  if (t.pre != nullptr) {
+    // (in place: the result is then off by fp16's smallest step, and the kernel needs no more registers)
+    if (o.act == VOID_ACT_RELU && o.dtype == VOID_OUT_F16)
+#pragma unroll
+      for (int k = 0; k < 16; ++k) v[k] = keep_sign(v[k]);
+    store16_rows<false>(t.pre, o.dtype, t.ldp, n, o.N, c0, o.M, v);
+  }
   if (o.act != VOID_ACT_NONE) {
     f32x2 x[8];
 #pragma unroll

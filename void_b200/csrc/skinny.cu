@@ -303,8 +303,9 @@ __global__ void __launch_bounds__(512) skinny_kernel(const __grid_constant__ Par
     float v = KIND == VOID_KIND_I8 ? __int2float_rn((int)s) : (float)s;
     v = (v * rs) * x.cs + x.bias;
     if constexpr (TAIL) {
-      v += x.row_bias;
-      if (p.tail.pre != nullptr) store_value(p.tail.pre, p.out_dtype, (long long)x.n * p.tail.ldp + x.r, v);
+      v = with_bias(v, x.row_bias, p.tail.pre != nullptr && p.act == VOID_ACT_RELU);
+      if (p.tail.pre != nullptr)
+        store_value(p.tail.pre, p.out_dtype, (long long)x.n * p.tail.ldp + x.r, p.act == VOID_ACT_RELU && p.out_dtype == VOID_OUT_F16 ? keep_sign(v) : v);
       v = activate(v, p.act) + x.residual;
     } else if constexpr (ACT) {
       v = activate(v + x.row_bias, p.act);
@@ -408,10 +409,12 @@ __global__ void __launch_bounds__(Stream::THREADS, Stream::CTAS_PER_SM) expert_s
       for (int o = tid; o < 32 * NB; o += 32 * W) {
         const int m = o & 31, n = n0 + (o >> 5), r = row * kTile + m;
         if (n >= n1 || r >= p.M) continue;
-        float v = of_row;
+        float v = 0.0f;
 #pragma unroll
         for (int k = 0; k < W; ++k) v += red[((turn * W + k) * 32 + m) * PITCH + (o >> 5)];
-        if (x.tail.pre != nullptr) store_value(x.tail.pre, p.out_dtype, (long long)n * x.tail.ldp + r, v);
+        v = with_bias(v, of_row, x.tail.pre != nullptr && p.act == VOID_ACT_RELU);
+        if (x.tail.pre != nullptr)
+          store_value(x.tail.pre, p.out_dtype, (long long)n * x.tail.ldp + r, p.act == VOID_ACT_RELU && p.out_dtype == VOID_OUT_F16 ? keep_sign(v) : v);
         store_value(p.out, p.out_dtype, (long long)n * p.ldc + r, activate(v, p.act));
       }
     }
