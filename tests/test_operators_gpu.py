@@ -144,6 +144,34 @@ def test_slopes_next_to_the_border_of_relu(n, k, m, density, dtype):
         at += c
 
 
+# z = a + 2^-25 - a: what fp16 rounds to nothing, or the sum loses beside a; and its negative.
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n", [3, 40, 300])
+def test_slopes_of_sums_that_their_bias_takes_to_nothing(n, dtype):
+    a = weight(64, 32, 1.0, dtype)
+    a.values.zero_()
+    sizes = [0.25, 0.25, 1.0, 1.0, 64.0, 64.0]
+    for i, size in enumerate(sizes):                      # rows of the first tile
+        a.values[0, i, 0], a.values[0, i, 1] = size, 2.0 ** -13 * (1 if i % 2 == 0 else -1)
+    a.values[0, 31, 0] = 4.0
+    x = torch.zeros(n, 32, dtype=dtype, device="cuda")
+    x[:, 0], x[:, 1] = 1.0, 2.0 ** -12
+    bias = torch.zeros(64, device="cuda")
+    bias[:len(sizes)] = -torch.tensor(sizes, device="cuda")
+    want = torch.zeros(64, device="cuda")
+    want[[0, 2, 4, 31]] = float(n)
+    layer = void.SparseLinear(32, 64, a, dtype=torch.float32, activation="relu")
+    experts = void.SparseExperts(void.stack_experts([a, a]), activation="relu", dtype=torch.float32)
+    with torch.no_grad():
+        layer.bias.copy_(bias)
+        experts.bias.copy_(bias)
+    y = layer(x.requires_grad_(True))
+    assert torch.equal(torch.autograd.grad(y, (layer.bias,), torch.ones_like(y))[0], want)
+    y = experts(x, offsets_of([n, 0]))
+    counts, = torch.autograd.grad(y, (experts.bias,), torch.ones_like(y))
+    assert torch.equal(counts[0], want) and not counts[1].any()
+
+
 DROP_FIRST_GROUP = 1 << 16
 
 
