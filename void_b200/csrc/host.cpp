@@ -788,7 +788,11 @@ at::Tensor two_layers(Packed* first, Packed* second, const at::Tensor& x, PyObje
     s.N = (int32_t)N;
     s.b_scale = 1.0f;
     Tail tail;
-    if (!none(given[layer])) s.row_bias = bias_as_it_is(tensor(given[layer], "bias"), dev, p->M, &tail.e.bias_dtype, bias[layer], "bias");
+    if (!none(given[layer])) {
+      const at::Tensor& b = tensor(given[layer], "bias");
+      // (results that leave as rows of features are a plain product's, whose row biases are fp32)
+      s.row_bias = bias_as_it_is(columns && layer == 0 ? b.to(dev, at::kFloat) : b, dev, p->M, &tail.e.bias_dtype, bias[layer], "bias");
+    }
     if (layer == 1) out = new_cuda({N, p->M}, x.scalar_type(), dev);
     else out = columns ? pitched(p->M, N, x.scalar_type(), es, dev) : pitched(N, p->M, x.scalar_type(), es, dev);
     s.out = out.data_ptr();
