@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import void_b200 as void
+from test_experts_gpu import offsets_of
 from test_linear_cpu import within
 from test_linear_gpu import feed_forward64, rand, weight
 
@@ -24,3 +25,34 @@ def test_mlp_with_biases_of_16_bits_on_a_transposed_copy(groups, dtype):
         torch.cuda.synchronize()
     odd = rand(2048, 1032, dtype=dtype)[:, 1:1025]       # a residual that lies in no 16-byte pieces
     within(void.fused_sparse_mlp(x, w1, w2, "gelu", b1, b2, residual=odd), ref - x.double() + odd.double(), e + e)
+
+
+TYPES = [torch.float16, torch.bfloat16, torch.float32]
+
+
+def relu_layers(dense, bias, dtype):
+    """A linear layer and a layer of two experts with these weights, in training with ReLU; and how they are called on n tokens."""
+    a = void.dense_to_void(dense.to(dtype), threshold=-1.0)
+    layer = void.SparseLinear(dense.shape[1], dense.shape[0], a, dtype=torch.float32, activation="relu")
+    experts = void.SparseExperts(void.stack_experts([a, a]), activation="relu", dtype=torch.float32)
+    with torch.no_grad():
+        layer.bias.copy_(bias)
+        experts.bias.copy_(bias)
+    return [(layer, layer.sparse_weight.values, lambda x: layer(x)),
+            (experts, experts.values, lambda x: experts(x, offsets_of([x.shape[0] - x.shape[0] // 3, x.shape[0] // 3])))]
+
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m", [64, 45])
+def test_infinite_gradients_stop_where_relu_has_no_slope(m, dtype):
+    dense, bias = weight(m, 96, 1.0, torch.float32).to_dense(), rand(m, seed=1)
+    x, g = rand(40, 96, dtype=dtype), rand(40, m, dtype=dtype, seed=3)
+    bias[7] = -1e4 if dtype != torch.float16 else -1e3
+    bad = g.clone()
+    g[:, 7] = 0.0
+    bad[:, 7] = float("inf")
+    bad[3, 7] = float("nan")
+    for layer, values, call in relu_layers(dense, bias, dtype):
+        got = [torch.autograd.grad(call(x.requires_grad_(True)), (x, values, layer.bias), t) for t in (g, bad)]
+        assert all(torch.equal(p, q) for p, q in zip(*got))

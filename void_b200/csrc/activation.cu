@@ -20,11 +20,10 @@ namespace vb {
 
 namespace {
 
-// act'(z) of two values.  With s = sigmoid(w(z)): (z s)' = s + z s (1 - s) w'(z).
+// act'(z) of two values, of GELU and SiLU.  With s = sigmoid(w(z)): (z s)' = s + z s (1 - s) w'(z).
 __device__ __forceinline__ f32x2 slopes(f32x2 z, int act) {
   float a, b;
   unpair(z, a, b);
-  if (act == VOID_ACT_RELU) return pair(a > 0.0f ? 1.0f : 0.0f, b > 0.0f ? 1.0f : 0.0f);
   // (kGelu1, kGelu3 and kSilu carry -log2(e), for a sigmoid of powers of two)
   const bool gelu = act == VOID_ACT_GELU;
   const f32x2 square = mul2(z, z), one = pair(1.0f, 1.0f);
@@ -39,6 +38,14 @@ __device__ __forceinline__ f32x2 slopes(f32x2 z, int act) {
   unpair(rest, r0, r1);
   // (far out s is 0 or 1 to the last bit while z grows: nothing is left of the second term)
   return pair(r0 > 0.0f ? a : s0, r1 > 0.0f ? b : s1);
+}
+// d act'(z).  Where ReLU has no slope nothing comes through, an infinite gradient no more than others.
+__device__ __forceinline__ f32x2 through(f32x2 d, f32x2 z, int act) {
+  if (act != VOID_ACT_RELU) return mul2(d, slopes(z, act));
+  float a, b, da, db;
+  unpair(z, a, b);
+  unpair(d, da, db);
+  return pair(a > 0.0f ? da : 0.0f, b > 0.0f ? db : 0.0f);
 }
 
 template <typename T> __device__ __forceinline__ float value(T v);
@@ -131,7 +138,7 @@ __global__ void __launch_bounds__(kGradThreads, 4) activation_grad_kernel(const 
 #pragma unroll
         for (int e = 0; e < PAIRS; ++e) {
           d[e] = pair(value<T>(gv.e[2 * e]), value<T>(gv.e[2 * e + 1]));
-          if (active) d[e] = mul2(d[e], slopes(pair(value<T>(zv.e[2 * e]), value<T>(zv.e[2 * e + 1])), p.act));
+          if (active) d[e] = through(d[e], pair(value<T>(zv.e[2 * e]), value<T>(zv.e[2 * e + 1])), p.act);
           s[e] = add2(s[e], d[e]);
         }
         if (p.dz == nullptr) continue;
@@ -154,7 +161,7 @@ __global__ void __launch_bounds__(kGradThreads, 4) activation_grad_kernel(const 
       for (; left > 0; left -= 2, g += 2 * g_step, z += 2 * z_step, dz += 2 * dz_step) {
         const bool two = left > 1;
         f32x2 d = pair(value<T>(g[0]), two ? value<T>(g[g_step]) : 0.0f);
-        if (active) d = mul2(d, slopes(pair(value<T>(z[0]), two ? value<T>(z[z_step]) : 0.0f), p.act));
+        if (active) d = through(d, pair(value<T>(z[0]), two ? value<T>(z[z_step]) : 0.0f), p.act);
         s[0] = add2(s[0], d);
         float a, b;
         unpair(d, a, b);
