@@ -433,7 +433,9 @@ typedef struct void_epilogue {
   int64_t ldr;
   int32_t residual_dtype;  /* VOID_OUT_F32, or args->out_dtype                                                       */
   int32_t bias_dtype;      /* what args->row_bias points to: VOID_OUT_F32 (0), VOID_OUT_F16 or VOID_OUT_BF16         */
-  void* pre;               /* [N, M] of type args->out_dtype, ldp elements between rows: z, for a backward pass; or NULL */
+  void* pre;               /* [N, M] of type args->out_dtype, ldp elements between rows: z, for a backward pass; or NULL.
+                              With VOID_ACT_RELU its sign is that of the sum: fp16's smallest number for what fp16 would round to zero, -0 where
+                              a sum that is not zero and its bias make zero                                                             */
   int64_t ldp;
 } void_epilogue;
 VOID_API int void_spmm_linear(const void_spmm_args* args, const void_epilogue* epilogue, int32_t kind, void_stream_t stream);
@@ -487,8 +489,9 @@ VOID_API int void_expert_tile_grad(const void* grad_out, int64_t ldg, const void
                                    int32_t kind, const void_experts* experts, const int32_t* items, int32_t n_items,
                                    const int32_t* tile_cols, const int32_t* block_indices, void* grad_tiles, int32_t out_dtype,
                                    int32_t* status, void_stream_t stream);
-/* z [N, M] of such a layer with fp16 or bf16 tiles, where it lies so near to zero that the sums' errors reach its sign, computed again in
- * 64 bits (ReLU's slope for a backward pass).  x [N, K] and values [nnz, 32, 32] of the kind's type, block_indices the place of each of
+/* z [N, M] of such a layer with fp16 or bf16 tiles, where it lies so near to zero that the sums' errors reach its sign (measured by what is typical of the
+ * token and by the bias) or is -0, computed again in 64 bits (ReLU's slope for a backward pass); of 32 tokens and 256 columns at most 256 values, the others
+ * keep the sign they have.  x [N, K] and values [nnz, 32, 32] of the kind's type, block_indices the place of each of
  * row_ptr's tiles in values, bias as in void_epilogue; z on 16 bytes, ldz a multiple of 8.  experts: NULL, or as for void_expert_linear with a
  * plan (row_ptr and the bias of all experts). */
 VOID_API int void_relu_border(const void* x, int64_t ldx, const void* values, const int32_t* row_ptr, const int32_t* block_indices,

@@ -56,3 +56,78 @@ def test_infinite_gradients_stop_where_relu_has_no_slope(m, dtype):
     for layer, values, call in relu_layers(dense, bias, dtype):
         got = [torch.autograd.grad(call(x.requires_grad_(True)), (x, values, layer.bias), t) for t in (g, bad)]
         assert all(torch.equal(p, q) for p, q in zip(*got))
+
+
+def tile_rows(layer):
+    return layer.block_rows if isinstance(layer, void.SparseExperts) else layer.sparse_weight.block_rows
+
+
+# z = size - size = 0, in one output of many or in all of them: zero, without a slope.
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", [1.0, 2.0 ** -10, 2.0 ** -30])
+@pytest.mark.parametrize("n", [1, 8, 40, 300])
+@pytest.mark.parametrize("alone", [True, False])
+def test_a_sum_that_its_bias_cancels_is_zero_and_has_no_slope(alone, n, size, dtype):
+    m, k = 64, 96
+    size = max(size, 2.0 ** -24) if dtype == torch.float16 else size
+    dense, bias = weight(m, k, 1.0, torch.float32).to_dense(), rand(m, seed=1)
+    rows = torch.tensor([5] if alone else list(range(m)), device="cuda")
+    dense[rows] = 0.0
+    dense[rows, 0] = size
+    bias[rows] = -size
+    x, g = rand(n, k, dtype=dtype), rand(n, m, dtype=dtype, seed=3)
+    x[:, 0] = 1.0
+    for layer, values, call in relu_layers(dense, bias, dtype):
+        y = call(x.requires_grad_(True))
+        dx, dv, db = torch.autograd.grad(y, (x, values, layer.bias), g)
+        assert not y[:, rows].any() and not db[..., rows].any()
+        assert not (dv[tile_rows(layer) % 2 == 0][:, 5].any() if alone else dv.any() or dx.any())
+
+
+# Sums around half of fp16's smallest number: the result is the sum rounded, the slope asks for its sign.
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [1, 8, 40, 300])
+def test_results_in_training_are_those_of_the_sums(n, dtype):
+    dense, bias = torch.zeros(32, 64, device="cuda"), torch.zeros(32, device="cuda")
+    dense[:8, 0] = 2.0 ** -13 * torch.tensor([0.5, -0.5, 1.0, -1.0, 1.5, -1.5, 0.25, -0.25], device="cuda")
+    dense[8, 0], bias[9] = 1.0, 2.0 ** -26
+    x = torch.zeros(n, 64, dtype=dtype, device="cuda")
+    x[:, 0] = 2.0 ** -12
+    z = dense[:, 0].double() * 2.0 ** -12 + bias.double()
+    for layer, _, call in relu_layers(dense, bias, dtype):
+        y = call(x.requires_grad_(True))
+        db, = torch.autograd.grad(y, (layer.bias,), torch.ones_like(y))
+        assert torch.equal(y, z.clamp_min(0).to(dtype).expand(n, 32))
+        assert torch.equal(db.reshape(-1, 32).sum(0), n * (z > 0).float())
+
+
+# Every sum of a token is all but cancelled by its bias: what is left, some 2^-24 of the sum, has to give the slope.
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n, scale", [(1, 1.0), (40, 1.0), (300, 1.0), (40, 100.0)])
+def test_slopes_of_a_token_whose_sums_are_all_cancelled(n, scale, dtype):
+    m, k = 256, 3200
+    dense, x = weight(m, k, 1.0, torch.float32).to_dense().to(dtype).float(), rand(n, k, dtype=dtype)
+    x[0] *= scale
+    sums = x[0].double() @ dense.double().t()
+    nudge = (torch.arange(m, device="cuda") % 7 - 3).double() * 2.0 ** -23
+    bias = -(sums * (1.0 + nudge)).float()
+    g = torch.zeros(n, m, dtype=dtype, device="cuda")
+    g[0] = 1.0
+    for layer, _, call in relu_layers(dense, bias, dtype):
+        y = call(x.requires_grad_(True))
+        db, = torch.autograd.grad(y, (layer.bias,), g)
+        assert torch.equal(db.reshape(-1, m).sum(0), (sums + bias.double() > 0).float())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_slopes_are_the_same_every_time_where_most_sums_are_cancelled(dtype):
+    m, k, n = 300, 1600, 333
+    dense, x = weight(m, k, 1.0, torch.float32).to_dense().to(dtype).float(), rand(1, k, dtype=dtype).expand(n, k).contiguous()
+    bias = -(x[0].double() @ dense.double().t()).float()
+    for layer, values, call in relu_layers(dense, bias, dtype):
+        grads = []
+        for _ in range(3):
+            y = call(x.requires_grad_(True))
+            grads.append(torch.autograd.grad(y, (x, values, layer.bias), torch.ones_like(y)))
+        assert all(torch.equal(p, q) for other in grads[1:] for p, q in zip(grads[0], other))
+        assert bool((grads[0][2] >= 0).all()) and bool((y >= 0).all()) and float(y.detach().max()) < 1e-3

@@ -225,13 +225,21 @@ __global__ void __launch_bounds__(256) partial_sums_kernel(const float* partials
 }
 
 // Values of z that lie next to ReLU's border, computed again.  The slope there is a question of z's sign, and the tensor cores cut what they hold
-// after every product that they add, by half of 2^-23 of it: z of a row of 108 tiles is off by 1.4e-5 of its size, and 3 of 300 000 slopes came out
-// wrong.  What lies within 2^-21 of its strip's largest value for every tile, ten times as much, and for sixteen more, since the errors of a few tiles do
-// not average out, is summed in 64 bits, by a block together: of normal values one in ten thousand for such rows.  A strip is 256 columns of a token; a
-// sum of nothing but zeros is right as it is (what fp16 would round to zero has kept its sign, keep_sign).  us, forward pass with SiLU and with ReLU and
-// this behind it: 4096^2, 90 %, 4096 tokens 52 and 75; 2048^2, 50 %, 512 tokens 14 and 22; 14336 -> 14240, 76 %, 44 tokens 75 and 111.  A warp
-// for each value instead, and 16 tiles on their way at once: 83, 22 and 110.
-constexpr int kStrip = 256, kBorderWarps = 8, kBorderTokens = 4;   // columns of a block, its warps, tokens of a warp at a time
+// after every product that they add, by half of 2^-23 of it: of 35 million sums of rows of 3 to 107 tiles none was off by more than 3.2 times
+// (tiles + 16) 2^-23 of what is typical of its token, the square of the mean root of |sum| over a strip of up to 256 columns (which one large value hardly
+// moves).  The border is eight times that, and as many times four for the bias, which a sum that it cancels has grown to.  What lies inside, or is -0 (with_bias),
+// is summed in 64 bits: of normal values one in thirty thousand for rows of 13 tiles, at most kMostDoubtful of a block's 8192 whatever the values are; those
+// beyond, the last of the block, keep the sign they were summed to.  The order is that of tokens and columns: the same result every time.
+// (What fp16 would round to zero has kept its sign, keep_sign.)  One value is summed by the block, eight of them by a warp each.
+// us, forward pass with SiLU and with ReLU and this behind it, fp16, bias and residual: 4096^2, 90 %, 4096 tokens 63 and 87; 2048^2, 50 %, 512 tokens 14
+// and 23; 14336 -> 14240, 76 %, 44 tokens 76 and 96 (mostly the way to the tiles of one or two values per block); 16 experts of 2048 -> 4096, 90 %, 8192 tokens bf16 82 and
+// 121.  One output in 32 a thousand times the others, or one bias of each strip 3e4: 4 to 9 us more (a border relative to the strip's largest value: 25 ms).
+__device__ __forceinline__ float sqrt_approx(float v) {
+  float r;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+constexpr int kStrip = 256, kBorderWarps = 8, kBorderTokens = 4, kMostDoubtful = 256;   // columns of a block, its warps, tokens of a warp at a time
 struct BorderParams {
   const void *x, *values, *bias;
   const int32_t *row_ptr, *block_indices, *tile_cols, *bounds;
@@ -242,73 +250,129 @@ struct BorderParams {
 template <typename T>
 __global__ void __launch_bounds__(32 * kBorderWarps) relu_border_kernel(const __grid_constant__ BorderParams p) {
   constexpr int BATCH = kBorderWarps * kBorderTokens;
-  __shared__ uint16_t list[BATCH * kStrip];   // (token of the batch) << 8 | column of the strip
-  __shared__ int found;
+  __shared__ uint16_t list[kMostDoubtful];   // (token of the batch) << 8 | column of the strip
+  __shared__ int counts[kBorderWarps];
   __shared__ double sums[kBorderWarps];
   grid_dependency_wait();
-  // (the last strip begins early enough to be whole: its largest value is the measure)
-  const int last = p.M > kStrip ? (p.M - kStrip + 7) & ~7 : 0, strip = (int)blockIdx.x * kStrip < last ? (int)blockIdx.x * kStrip : last;
+  // strips of whole pieces of eight columns, none much narrower than the others: it would say little about what is typical
+  const long long pieces = (p.M + 7) >> 3;
+  const int strip = (int)(pieces * blockIdx.x / gridDim.x) * 8, strip_end = (int)(pieces * (blockIdx.x + 1) / gridDim.x) * 8;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, m0 = strip + lane * 8;
-  auto expert_of = [&](int n) {   // the last whose run does not begin behind the token; -1: in no run
-    if (p.bounds == nullptr) return 0;
-    if (n < p.bounds[0] || n >= p.bounds[p.n_experts]) return -1;
-    int e = 0, hi = p.n_experts;
+  const int cols = m0 >= strip_end ? 0 : (p.M - m0 < 8 ? p.M - m0 : 8);
+  int run_begin = 0, run_end = p.N, run = 0;   // of the token asked for last: tokens of its run, expert (-1: in no run)
+  if (p.bounds != nullptr) run_end = 0;
+  auto expert_of = [&](int n) {
+    if (n >= run_begin && n < run_end) return run;
+    const int before = p.bounds[0], behind = p.bounds[p.n_experts];
+    if (n < before || n >= behind) {
+      run = -1;
+      run_begin = n < before ? 0 : behind;
+      run_end = n < before ? before : p.N;
+      return run;
+    }
+    int e = 0, hi = p.n_experts;   // the last whose run does not begin behind the token
     while (hi - e > 1) {
       const int mid = (e + hi) >> 1;
       if (p.bounds[mid] <= n) e = mid;
       else hi = mid;
     }
-    return e;
+    run = e;
+    run_begin = p.bounds[e];
+    run_end = p.bounds[e + 1];
+    return run;
   };
-  auto tiles_of = [&](int e) { return m0 < p.M ? p.row_ptr[(size_t)e * p.nbr + (m0 >> 5) + 1] - p.row_ptr[(size_t)e * p.nbr + (m0 >> 5)] : 0; };
-  int tiles = p.bounds == nullptr ? tiles_of(0) : 0;
-  if (threadIdx.x == 0) found = 0;
-  __syncthreads();
+  auto bias_at = [&](size_t at) {
+    return p.bias_dtype == VOID_OUT_F32 ? reinterpret_cast<const float*>(p.bias)[at]
+                                        : f16_value(reinterpret_cast<const uint16_t*>(p.bias)[at], p.bias_dtype == VOID_OUT_F16);
+  };
+  // of the lane's columns, for the expert that the token belongs to: 2^-21 (tiles + 16); the biases, NaN (no comparison holds) where there are no tiles
+  int held = -1;
+  float unit = 0.0f, each = 0.0f, bias[8];
+  auto take = [&](int e) {
+    if (e < 0 || e == held) return;
+    held = e;
+    const int32_t* row = p.row_ptr + (size_t)e * p.nbr + (m0 >> 5);
+    const int tiles = cols > 0 ? row[1] - row[0] : 0;
+    unit = (float)(tiles + 16) * (1.0f / 2097152.0f);
+    const int all = __reduce_add_sync(0xffffffffu, tiles > 0 ? cols : 0);
+    each = all > 0 ? 1.0f / (float)all : 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      bias[i] = tiles > 0 && i < cols ? (p.bias != nullptr ? bias_at((size_t)e * p.M + m0 + i) : 0.0f) : __int_as_float(0x7fffffff);
+  };
   for (long long first = (long long)blockIdx.y * BATCH; first < p.N; first += (long long)gridDim.y * BATCH) {
-    union { uint4 v; T t[8]; } u[kBorderTokens];
+    union { uint4 v; T t[8]; uint16_t bits[8]; } u[kBorderTokens];
 #pragma unroll
     for (int k = 0; k < kBorderTokens; ++k) {
       const long long n = first + warp * kBorderTokens + k;
       u[k].v = make_uint4(0u, 0u, 0u, 0u);
-      if (m0 < p.M && n < p.N) u[k].v = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.z) + n * p.ldz + m0);
+      if (cols > 0 && n < p.N) u[k].v = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.z) + n * p.ldz + m0);
     }
+    uint32_t doubtful = 0u;   // bit 8 k + i: column i of token k
 #pragma unroll
     for (int k = 0; k < kBorderTokens; ++k) {
       const long long n = first + warp * kBorderTokens + k;
-      float v[8], most = 0.0f;
+      const int e = n < p.N ? expert_of((int)n) : -1;
+      take(e);
+      if (e < 0) continue;
+      float root = 0.0f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        v[i] = m0 + i < p.M ? fabsf(value<T>(u[k].t[i])) : 0.0f;
-        most = fmaxf(most, v[i]);
+        const float s = fabsf(value<T>(u[k].t[i]) - bias[i]);
+        if (s < 1e30f) root += sqrt_approx(s);
       }
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-      if (p.bounds != nullptr) {
-        const int e = n < p.N ? expert_of((int)n) : -1;
-        tiles = e < 0 ? 0 : tiles_of(e);
-      }
-      const float border = most < 1e38f ? (float)(tiles > 0 ? tiles + 16 : 0) * (1.0f / 2097152.0f) * most : 0.0f;
+      for (int o = 16; o > 0; o >>= 1) root += __shfl_xor_sync(0xffffffffu, root, o);
+      root *= each;
+      const float typical = unit * 2.0f * root * root;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (v[i] > 0.0f && v[i] < border) list[atomicAdd(&found, 1)] = (uint16_t)((warp * kBorderTokens + k) << 8 | (lane * 8 + i));
+      for (int i = 0; i < 8; ++i)   // (of the zeros only -0)
+        if (fabsf(value<T>(u[k].t[i])) < fmaf(unit, fabsf(bias[i]), typical) && u[k].bits[i] != 0) doubtful |= 1u << (8 * k + i);
     }
+    if (!__syncthreads_or(doubtful != 0u)) continue;
+    int place[kBorderTokens], found = 0;   // in the warp's part of the list: token by token
+#pragma unroll
+    for (int k = 0; k < kBorderTokens; ++k) {
+      const int mine = __popc((doubtful >> (8 * k)) & 255u);
+      int upto = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int before = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += before;
+      }
+      place[k] = found + upto - mine;
+      found += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    if (lane == 0) counts[warp] = found;
     __syncthreads();
-    // the block together, a warp every eighth tile
-    const int count = found;
-    __syncthreads();   // (all have read it before a warp finds the next)
-    for (int c = 0; c < count; ++c) {
-      const int n = (int)(first + (list[c] >> 8)), m = strip + (list[c] & 255), e = expert_of(n);
+    int base = 0, count = 0;
+#pragma unroll
+    for (int w = 0; w < kBorderWarps; ++w) {
+      if (w < warp) base += counts[w];
+      count += counts[w];
+    }
+    if (count > kMostDoubtful) count = kMostDoubtful;
+#pragma unroll
+    for (int k = 0; k < kBorderTokens; ++k)
+      for (uint32_t bits = (doubtful >> (8 * k)) & 255u, at = (uint32_t)(base + place[k]); bits != 0u; bits &= bits - 1u, ++at)
+        if (at < (uint32_t)kMostDoubtful) list[at] = (uint16_t)((warp * kBorderTokens + k) << 8 | (lane * 8 + __ffs(bits) - 1));
+    __syncthreads();
+    for (int c = 0, share; c < count; c += kBorderWarps / share) {
+      const int left = count - c;
+      share = left >= 8 ? 1 : (left >= 4 ? 2 : (left >= 2 ? 4 : 8));   // warps of a value, which take its tiles in turn
+      const int v = list[c + warp / share], part = warp % share;
+      const int n = (int)(first + (v >> 8)), m = strip + (v & 255), e = expert_of(n);
       const int32_t* row = p.row_ptr + (size_t)e * p.nbr + (m >> 5);
       const T *x = reinterpret_cast<const T*>(p.x) + (long long)n * p.ldx, *values = reinterpret_cast<const T*>(p.values) + (m & 31) * 32 + lane;
       double s = 0.0;
       const int end = row[1];
-      for (int t = row[0] + warp; t < end; t += 4 * kBorderWarps) {
+      for (int t = row[0] + part; t < end; t += 4 * share) {
         float a[4], b[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const bool in = t + i * kBorderWarps < end;
-          const int k = in ? p.tile_cols[t + i * kBorderWarps] * 32 + lane : p.K;
-          a[i] = in ? value<T>(values[(size_t)p.block_indices[t + i * kBorderWarps] * 1024]) : 0.0f;
+          const bool in = t + i * share < end;
+          const int k = in ? p.tile_cols[t + i * share] * 32 + lane : p.K;
+          a[i] = in ? value<T>(values[(size_t)p.block_indices[t + i * share] * 1024]) : 0.0f;
           b[i] = k < p.K ? value<T>(x[k]) : 0.0f;
           if (k >= p.K) a[i] = 0.0f;
         }
@@ -317,27 +381,21 @@ __global__ void __launch_bounds__(32 * kBorderWarps) relu_border_kernel(const __
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      if (lane == 0) sums[warp] = s;
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        s = 0.0;
-#pragma unroll
-        for (int w = 0; w < kBorderWarps; ++w) s += sums[w];
-        const size_t at = (size_t)e * p.M + m;
-        if (p.bias != nullptr)
-          s += p.bias_dtype == VOID_OUT_F32 ? (double)reinterpret_cast<const float*>(p.bias)[at]
-                                            : (double)f16_value(reinterpret_cast<const uint16_t*>(p.bias)[at], p.bias_dtype == VOID_OUT_F16);
+      if (share > 1) {
+        if (lane == 0) sums[warp] = s;
+        __syncthreads();
+      }
+      if (part == 0 && lane == 0) {
+        for (int w = 1; w < share; ++w) s += sums[warp + w];
+        if (p.bias != nullptr) s += (double)bias_at((size_t)e * p.M + m);
         union { uint16_t bits; T t; } r;
         r.t = rounded<T>((float)s);
         if (s != 0.0 && (r.bits & 0x7fffu) == 0) r.bits = s > 0.0 ? 0x0001u : 0x8001u;   // (the sign is what is asked for)
         reinterpret_cast<T*>(p.z)[(long long)n * p.ldz + m] = r.t;
       }
-      __syncthreads();
+      if (share > 1) __syncthreads();
     }
-    if (count > 0) {
-      if (threadIdx.x == 0) found = 0;
-      __syncthreads();
-    }
+    __syncthreads();   // (the list is read to its end before a warp writes the next)
   }
   grid_launch_dependents();
 }

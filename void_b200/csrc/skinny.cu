@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(512) skinny_kernel(const __grid_constant__ Par
     if constexpr (TAIL) {
       v = with_bias(v, x.row_bias, p.tail.pre != nullptr && p.act == VOID_ACT_RELU);
       if (p.tail.pre != nullptr)
-        store_value(p.tail.pre, p.out_dtype, (long long)x.n * p.tail.ldp + x.r, p.act == VOID_ACT_RELU && p.out_dtype == VOID_OUT_F16 ? keep_sign(v) : v);
+        store_value(p.tail.pre, p.out_dtype, (long long)x.n * p.tail.ldp + x.r, keep_sign(v, p.act, p.out_dtype));
       v = activate(v, p.act) + x.residual;
     } else if constexpr (ACT) {
       v = activate(v + x.row_bias, p.act);
@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(Stream::THREADS, Stream::CTAS_PER_SM) expert_s
         for (int k = 0; k < W; ++k) v += red[((turn * W + k) * 32 + m) * PITCH + (o >> 5)];
         v = with_bias(v, of_row, x.tail.pre != nullptr && p.act == VOID_ACT_RELU);
         if (x.tail.pre != nullptr)
-          store_value(x.tail.pre, p.out_dtype, (long long)n * x.tail.ldp + r, p.act == VOID_ACT_RELU && p.out_dtype == VOID_OUT_F16 ? keep_sign(v) : v);
+          store_value(x.tail.pre, p.out_dtype, (long long)n * x.tail.ldp + r, keep_sign(v, p.act, p.out_dtype));
         store_value(p.out, p.out_dtype, (long long)n * p.ldc + r, activate(v, p.act));
       }
     }
