@@ -608,10 +608,10 @@ VOID_API int void_reduce_slots(const void* slots, const uint8_t* contrib, int32_
  *     y = (x - mean) / sqrt(var + eps) * weight + bias           mean and (biased) variance of the token's `cols` features
  * x [rows, cols] and y row-major of type elem (VOID_ELEM_*), ldx / ldy elements between rows; weight and bias [cols], of type
  * param_elem (elem, or VOID_ELEM_F32), each may be NULL.  stats [2][rows] (mean, 1 / sqrt(var + eps)) is written where not NULL:
- * the backward pass reads it.  Statistics are fp32.  y may be x.
+ * the backward pass reads it.  Statistics are fp32.  y may be x (the same place and pitch).
  * void_layer_norm_grad: dx (NULL: not wanted), dweight and dbias (likewise; type param_elem) from the gradient g of y.  The sums
  * over tokens are taken in a fixed order, in fp32.  ws: void_layer_norm_grad_ws_bytes(rows, cols) bytes, needed with dweight or
- * dbias.  dx may be g or x.
+ * dbias.  dx may be g or x (the same place and pitch).
  * ------------------------------------------------------------------------------------- */
 VOID_API int void_layer_norm(const void* x, int32_t elem, int64_t ldx, int64_t rows, int32_t cols, const void* weight,
                              const void* bias, int32_t param_elem, float eps, void* y, int64_t ldy, float* stats,

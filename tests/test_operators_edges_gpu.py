@@ -7,6 +7,9 @@ import void_b200 as void
 from test_experts_gpu import offsets_of
 from test_linear_cpu import within
 from test_linear_gpu import feed_forward64, rand, weight
+from test_norm_cpu import norm64, norm_grad64
+from test_norm_gpu import backward_bounds, make
+from void_b200 import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -131,3 +134,26 @@ def test_slopes_are_the_same_every_time_where_most_sums_are_cancelled(dtype):
             grads.append(torch.autograd.grad(y, (x, values, layer.bias), torch.ones_like(y)))
         assert all(torch.equal(p, q) for other in grads[1:] for p, q in zip(grads[0], other))
         assert bool((grads[0][2] >= 0).all()) and bool((y >= 0).all()) and float(y.detach().max()) < 1e-3
+
+
+# dx may take the place of g or of x, through the C ABI, in rows of every length.
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("place", ["g", "x"])
+@pytest.mark.parametrize("rows, cols", [(5, 100), (700, 1024), (9, 8200), (40, 8201), (33, 20000), (700, 16392)])
+def test_norm_gradient_in_the_place_of_an_operand(rows, cols, place, dtype):
+    x, w, b, g = make(rows, cols, dtype, torch.float32)
+    lib, elem, stream = _lib.load(), _lib.ELEM_CODE[dtype], torch.cuda.current_stream().cuda_stream
+    y, stats = torch.empty_like(x), torch.empty(2, rows, device="cuda")
+    assert lib.void_layer_norm(x.data_ptr(), elem, cols, rows, cols, w.data_ptr(), b.data_ptr(), _lib.ELEM_CODE[torch.float32], 1e-5, y.data_ptr(), cols,
+                               stats.data_ptr(), stream) == 0
+    xd, wd, gd = x.double(), w.double(), g.double()
+    _, unit, rstd = norm64(xd, wd, b.double(), 1e-5)
+    refs = norm_grad64(gd, unit, rstd, wd)
+    bounds = backward_bounds(xd, wd, gd, unit, rstd, *refs, dtype, torch.float32)
+    dx = g if place == "g" else x
+    dw, db = torch.empty_like(w), torch.empty_like(w)
+    ws = torch.empty(lib.void_layer_norm_grad_ws_bytes(rows, cols), dtype=torch.uint8, device="cuda")
+    assert lib.void_layer_norm_grad(g.data_ptr(), cols, x.data_ptr(), cols, elem, rows, cols, w.data_ptr(), _lib.ELEM_CODE[torch.float32], stats.data_ptr(),
+                                    dx.data_ptr(), cols, dw.data_ptr(), db.data_ptr(), ws.data_ptr(), ws.numel(), stream) == 0
+    for got, ref, bound in zip((dx, dw, db), refs, bounds):
+        within(got, ref, bound)

@@ -886,9 +886,10 @@ cudaError_t backward(const NormGradParams& p, const DeviceInfo& dev, P* dweight,
     }
   } else {
     blocks = (int)((p.rows + 7) / 8 < kColumnBlocks ? (p.rows + 7) / 8 : kColumnBlocks);
-    if (p.rows > 0 && p.dx != nullptr) rc = launch_pdl(layer_norm_grad_long_kernel<T, P, VEC>, dim3((unsigned)p.rows), 1024, 0, st, p);
-    if (rc == cudaSuccess && p.rows > 0 && p.partials != nullptr)
+    // (the sums first: dx may take the place of g or x)
+    if (p.rows > 0 && p.partials != nullptr)
       rc = launch_pdl(layer_norm_columns_kernel<T>, dim3((unsigned)((p.cols + 31) / 32), (unsigned)blocks), 256, 0, st, p);
+    if (rc == cudaSuccess && p.rows > 0 && p.dx != nullptr) rc = launch_pdl(layer_norm_grad_long_kernel<T, P, VEC>, dim3((unsigned)p.rows), 1024, 0, st, p);
   }
   if (rc == cudaSuccess && p.partials != nullptr)
     rc = launch_pdl(layer_norm_sums_kernel<P>, dim3((unsigned)((p.cols + 31) / 32), 2), 256, 0, st, p.partials, blocks, p.cols, dweight, dbias);
