@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import void_b200 as void
-from test_experts_gpu import offsets_of
+from test_experts_gpu import experts_of, offsets_of
 from test_linear_cpu import within
 from test_linear_gpu import feed_forward64, rand, weight
 from test_norm_cpu import norm64, norm_grad64
@@ -157,3 +157,52 @@ def test_norm_gradient_in_the_place_of_an_operand(rows, cols, place, dtype):
                                     dx.data_ptr(), cols, dw.data_ptr(), db.data_ptr(), ws.data_ptr(), ws.numel(), stream) == 0
     for got, ref, bound in zip((dx, dw, db), refs, bounds):
         within(got, ref, bound)
+
+
+def test_norm_into_memory_that_an_operand_shares():
+    x, w, b, _ = make(300, 1000, torch.bfloat16, torch.bfloat16)
+    want = void.void_layer_norm(x, w, b)
+    buf = torch.empty(303, 1000, dtype=torch.bfloat16, device="cuda")
+    for first, to in ((0, 3), (3, 0), (0, 0), (1, 2)):        # rows further on, further back, the very same
+        buf[first:first + 300] = x
+        out = buf[to:to + 300]
+        assert void.void_layer_norm(buf[first:first + 300], w, b, out=out) is out and torch.equal(out, want)
+    wide = torch.empty(300, 1008, dtype=torch.bfloat16, device="cuda")
+    wide[:, :1000] = x                                       # the same beginning, another pitch
+    out = wide.flatten()[:300000].view(300, 1000)
+    assert torch.equal(void.void_layer_norm(wide[:, :1000], w, b, out=out), want)
+    buf[0], buf[1] = w, b                                    # parameters where the first rows of the result will be
+    assert torch.equal(void.void_layer_norm(x, buf[0], buf[1], out=buf[:300]), want)
+
+
+def test_experts_into_memory_that_an_operand_shares_is_refused():
+    weights, e = experts_of(2, 64, 64, 0.5, torch.float16)
+    offsets, x = offsets_of([4, 6]), rand(10, 64, dtype=torch.float16)
+    want = void.void_expert_linear(e, x, offsets)
+    buf = torch.empty(22, 64, dtype=torch.float16, device="cuda")
+    for first, to in ((0, 1), (9, 0), (5, 5)):
+        with pytest.raises(_lib.VoidB200Error, match="must not be x, nor"):
+            void.void_expert_linear(e, buf[first:first + 10], offsets, out=buf[to:to + 10])
+    pair = torch.empty(10, 128, dtype=torch.float16, device="cuda")
+    with pytest.raises(_lib.VoidB200Error, match="must not be x, nor"):
+        void.void_expert_linear(e, pair[:, :64], offsets, out=pair[:, 56:120])
+    pair[:, 64:] = x                                         # side by side, behind one another: nothing in common
+    assert torch.equal(void.void_expert_linear(e, pair[:, 64:], offsets, out=pair[:, :64]), want) and torch.equal(pair[:, 64:], x)
+    buf[12:] = x
+    assert torch.equal(void.void_expert_linear(e, buf[12:], offsets, out=buf[:10]), want)
+    with pytest.raises(_lib.VoidB200Error, match="bias or the offsets"):
+        void.void_expert_linear(e, x, offsets, buf[:2], out=buf[:10])
+    with pytest.raises(_lib.VoidB200Error, match="row-major"):
+        void.void_expert_linear(e, x.float(), offsets, out=torch.empty(2, 10, 64, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [3, 40, 300])
+def test_a_layer_into_its_own_tokens(n, dtype):
+    a, x = weight(200, 200, 0.5, dtype), rand(n, 200, dtype=dtype)
+    want = void.void_linear(a, x, residual=x)
+    stream = x.clone()
+    assert torch.equal(void.void_linear(a, stream, out=stream, residual=stream), want)
+    buf = torch.empty(n + 1, 200, dtype=dtype, device="cuda")
+    buf[1:] = x
+    assert torch.equal(void.void_linear(a, buf[1:], out=buf[:n], residual=x), want)

@@ -576,6 +576,24 @@ const float* bias_as_it_is(const at::Tensor& bias, c10::Device dev, int64_t coun
   *dtype = out_code(keep.scalar_type());
   return static_cast<const float*>(keep.const_data_ptr());
 }
+// Whether two tensors may have memory in common.  Matrices of one pitch may lie side by side in it.
+bool meet(const at::Tensor& a, const at::Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  auto begin = [](const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()); };
+  auto bytes = [](const at::Tensor& t) {
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+    return (last + 1) * t.element_size();
+  };
+  const uintptr_t from = begin(a), to = begin(b);
+  if (from + (uintptr_t)bytes(a) <= to || to + (uintptr_t)bytes(b) <= from) return false;
+  auto rows_of = [](const at::Tensor& t) { return t.dim() == 2 && t.size(0) > 1 && (t.size(1) == 1 || t.stride(1) == 1); };
+  if (!rows_of(a) || !rows_of(b)) return true;
+  const int64_t pitch = a.stride(0) * a.element_size(), wide_a = a.size(1) * a.element_size(), wide_b = b.size(1) * b.element_size();
+  if (pitch <= 0 || b.stride(0) * b.element_size() != pitch || wide_a > pitch || wide_b > pitch) return true;
+  const int64_t apart = (((int64_t)(to - from)) % pitch + pitch) % pitch;   // of their rows' beginnings
+  return apart < wide_a || apart + wide_b > pitch;
+}
 // A residual [rows, cols] for a result `out`: of its type or fp32, rows with unit stride; other ones are copied, and so is one that
 // shares memory with `out` and is not the very same matrix.
 void set_residual(Tail& t, const at::Tensor& given, const at::Tensor& out) {
@@ -586,8 +604,7 @@ void set_residual(Tail& t, const at::Tensor& given, const at::Tensor& out) {
   const int64_t rows = given.size(0), cols = given.size(1);
   at::Tensor r = given.scalar_type() == out.scalar_type() || given.scalar_type() == at::kFloat ? given : given.to(at::kFloat);
   if ((cols > 1 && r.stride(1) != 1) || (rows > 1 && r.stride(0) < cols)) r = r.contiguous();
-  if (r.storage().unsafeGetStorageImpl() == out.storage().unsafeGetStorageImpl() &&
-      !(r.const_data_ptr() == out.const_data_ptr() && r.scalar_type() == out.scalar_type() && (rows <= 1 || r.stride(0) == out.stride(0))))
+  if (meet(r, out) && !(r.const_data_ptr() == out.const_data_ptr() && r.scalar_type() == out.scalar_type() && (rows <= 1 || r.stride(0) == out.stride(0))))
     r = r.clone(at::MemoryFormat::Contiguous);
   t.residual = r;
   t.e.residual = rows > 0 && cols > 0 ? r.const_data_ptr() : nullptr;
@@ -665,7 +682,9 @@ PyObject* spmm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const bool whole = in_pieces(out) && (n < 13 || none(a[12]) || in_pieces(cuda_tensor(a[12], "residual")));
   GroupStore* tokens = tr && none(a[11]) && whole ? group_store(pk, N, st, true) : nullptr;
   const bool copied = tr && none(a[11]) && tokens == nullptr && copy_pays(pk->kind, pk->args.nnz, N, pk->K);
-  const at::Tensor b = copied ? transposed_copy(b_in, es) : kernel_operand(b_in, es, tr ? 0 : pk->args.nnz * ((N + 127) / 128));
+  at::Tensor b = copied ? transposed_copy(b_in, es) : kernel_operand(b_in, es, tr ? 0 : pk->args.nnz * ((N + 127) / 128));
+  // (a layer that updates its own tokens, x + x A^T: every tile row reads all of a token)
+  if (tr && !none(a[2]) && meet(b, out)) b = kernel_operand(b.clone(at::MemoryFormat::Contiguous), es);
 
   void_spmm_args s = pk->args;
   const bool per_tile = PyObject_IsTrue(a[4]) == 1;
@@ -1545,7 +1564,8 @@ PyObject* expert_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (out.dim() != 2 || out.size(0) != N || out.size(1) != M || (M > 1 && out.stride(1) != 1) || (N > 1 && out.stride(0) < M))
       fail("out must be a row-major [" + std::to_string(N) + ", " + std::to_string(M) + "] tensor");
     if (out.device() != dev) fail("out and x are on different devices");
-    if (N > 0 && out.const_data_ptr() == x_in.const_data_ptr()) fail("out must not be x: every tile row of the experts reads all of a token");
+    if (meet(out, x_in)) fail("out must not be x, nor have memory in common with it: every tile row of the experts reads all of a token");
+    if (meet(out, offsets) || (!none(a[5]) && meet(out, tensor(a[5], "bias")))) fail("out must have no memory in common with the bias or the offsets");
   }
   const at::Tensor x = kernel_operand(x_in, es);
   void_spmm_args s = pk->args;
@@ -1847,7 +1867,7 @@ PyObject* layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   at::Tensor y, stats;
   {
     at::AutoDispatchBelowADInplaceOrView below;
-    const at::Tensor rows = token_rows(x);
+    at::Tensor rows = token_rows(x), w = weight.defined() ? weight.contiguous() : weight, b = bias.defined() ? bias.contiguous() : bias;
     const int64_t count = rows.size(0);
     if (none(a[4])) {
       y = new_cuda(x.sizes(), type, dev);
@@ -1857,9 +1877,12 @@ PyObject* layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
       if (y.sizes() != x.sizes() || y.scalar_type() != type || y.device() != dev || !y.is_contiguous())
         fail("out must be a contiguous tensor of x's shape and type on its device");
       if (!y.is_inference()) y.unsafeGetTensorImpl()->bump_version();
+      // what shares memory with the result is read from a copy, unless it is the very same rows
+      if (meet(rows, y) && !(rows.const_data_ptr() == y.const_data_ptr() && row_step(rows) == cols)) rows = rows.clone(at::MemoryFormat::Contiguous);
+      if (w.defined() && meet(w, y)) w = w.clone();
+      if (b.defined() && meet(b, y)) b = b.clone();
     }
     if (recorded) stats = new_cuda({2, count}, at::kFloat, dev);
-    const at::Tensor w = weight.defined() ? weight.contiguous() : weight, b = bias.defined() ? bias.contiguous() : bias;
     check(void_layer_norm(rows.const_data_ptr(), out_code(type), row_step(rows), count, (int32_t)cols, w.defined() ? w.const_data_ptr() : nullptr,
                           b.defined() ? b.const_data_ptr() : nullptr, out_code(params), (float)eps, y.data_ptr(), cols,
                           stats.defined() ? stats.data_ptr<float>() : nullptr, stream_of(dev.index())),

@@ -96,7 +96,8 @@ def void_expert_linear(experts: VOIDExperts, x: torch.Tensor, offsets: torch.Ten
     """y[t] = act(x[t] @ A_e^T + bias[e]) for the tokens offsets[e] <= t < offsets[e + 1] of every expert e; x [tokens, in] in
     float32 (multiplied as TF32), float16 or bfloat16, sorted by expert, y [tokens, out] in x's type.  ``offsets`` is int32 or int64
     [n_experts + 1] on x's device and is not read by the host: a captured call may be replayed with others.  ``bias`` is
-    [n_experts, out].  Rows in no run (before the first offset, behind the last) are zeros; with ``out`` (which must not be x) they are left as they are.
+    [n_experts, out].  Rows in no run (before the first offset, behind the last) are zeros; with ``out`` (which must have no memory in common with an operand)
+    they are left as they are.
     Offsets that fall or lie outside the batch are taken as empty runs and reported by check_device_status.  Inference form of
     SparseExperts: nothing is differentiated."""
     if not isinstance(experts, VOIDExperts):
@@ -112,6 +113,8 @@ def void_expert_linear(experts: VOIDExperts, x: torch.Tensor, offsets: torch.Ten
         raise _lib.VoidB200Error("void_expert_linear: x must be float32, float16 or bfloat16, got %s" % dtype)
     if out is not None and out.dtype != dtype:
         raise _lib.VoidB200Error("void_expert_linear: out must be of x's type, got %s" % out.dtype)
+    if out is not None and tuple(out.shape) != (x.shape[0], M):
+        raise _lib.VoidB200Error("void_expert_linear: out must be a row-major [%d, %d] tensor, got %s" % (x.shape[0], M, tuple(out.shape)))
     kind = product_kind(tensor, x)
     packed = packed_fp(tensor, kind)
     order = _row_order(packed, n_experts)

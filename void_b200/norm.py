@@ -14,7 +14,8 @@ def void_layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias
                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y = (x - mean) / sqrt(var + eps) * weight + bias over the last dimension of x [..., D] (float32, float16 or bfloat16), y in
     x's type.  weight and bias [D] are of x's type or float32, both of one; each may be left out.  Differentiable once in x, weight
-    and bias.  ``out`` (contiguous; may be x itself) takes the result where nothing is differentiated."""
+    and bias.  ``out`` (contiguous; may be x itself, or share memory with an operand in another way) takes the result where nothing is
+    differentiated."""
     if torch._C._are_functorch_transforms_active():
         raise RuntimeError("the layer norm cannot be used inside torch.func transforms (vmap, grad, jvp, ...)")
     _lib.require_cuda(x, weight, bias, out)

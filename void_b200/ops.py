@@ -102,7 +102,8 @@ def void_linear(a, x: torch.Tensor, bias: Optional[torch.Tensor] = None, activat
     they lie in memory.  ``a`` is a floating VOIDTensor (y in x's dtype) or an Int8VOIDTensor (x int8 with
     per-row scales ``x_scale`` [batch], or a float scalar; y fp32 unless ``out_dtype`` / ``out`` say otherwise).
     ``bias`` has one value per output feature; ``residual`` [batch, out] (float32, float16 or bfloat16) is added in fp32 behind the
-    activation, in the same kernel.  It may be ``out`` itself: the residual stream is then updated in place."""
+    activation, in the same kernel.  It may be ``out`` itself: the residual stream is then updated in place (an ``out`` that shares memory with x
+    costs a copy of x)."""
     size = x.shape                                      # (attributes of tensors cost 0.1 us each, half of what this function does)
     M, K = a.shape
     assert len(size) == 2 and size[1] == K, f"Dimension mismatch: A is {a.shape}, x is {tuple(size)}"
