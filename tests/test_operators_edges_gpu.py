@@ -206,3 +206,20 @@ def test_a_layer_into_its_own_tokens(n, dtype):
     buf = torch.empty(n + 1, 200, dtype=dtype, device="cuda")
     buf[1:] = x
     assert torch.equal(void.void_linear(a, buf[1:], out=buf[:n], residual=x), want)
+
+
+def test_a_result_that_was_given_counts_as_written():
+    dtype = torch.bfloat16
+    a, e = weight(64, 64, 0.5, dtype), experts_of(2, 64, 64, 0.5, dtype)[1]
+    x, r = rand(10, 64, dtype=dtype), rand(10, 64, dtype=dtype, seed=1)
+    for write in (lambda out: void.void_expert_linear(e, x, offsets_of([4, 6]), out=out), lambda out: void.void_linear(a, x, out=out, residual=out),
+                  lambda out: void.void_layer_norm(x, out=out)):
+        factor, out = torch.ones(10, 64, dtype=dtype, device="cuda", requires_grad=True), r.clone()
+        y = factor * out
+        write(out)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+    with torch.inference_mode():
+        out = torch.empty_like(r)
+        void.void_expert_linear(e, x, offsets_of([4, 6]), out=out)
+        void.void_linear(a, x, out=out, residual=r)

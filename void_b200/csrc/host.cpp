@@ -594,6 +594,10 @@ bool meet(const at::Tensor& a, const at::Tensor& b) {
   const int64_t apart = (((int64_t)(to - from)) % pitch + pitch) % pitch;   // of their rows' beginnings
   return apart < wide_a || apart + wide_b > pitch;
 }
+// A result that was given: autograd sees that it was written.
+void mark_written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 // A residual [rows, cols] for a result `out`: of its type or fp32, rows with unit stride; other ones are copied, and so is one that
 // shares memory with `out` and is not the very same matrix.
 void set_residual(Tail& t, const at::Tensor& given, const at::Tensor& out) {
@@ -769,6 +773,7 @@ PyObject* spmm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   else if (es > 1) check(void_spmm_fp(&s, pk->kind, st), "void_spmm_fp");
   else check(pk->kind == VOID_KIND_I8 ? void_spmm_i8(&s, st) : void_spmm_f8(&s, st), "void_spmm");
   if (!none(a[2])) {
+    mark_written(out);
     Py_INCREF(a[2]);
     return a[2];
   }
@@ -1604,6 +1609,7 @@ PyObject* expert_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     check(void_expert_linear(&s, &tail, &plan.x, pk->kind, st), "void_expert_linear");
   }
   if (!none(a[7])) {
+    mark_written(out);
     Py_INCREF(a[7]);
     return a[7];
   }
@@ -1876,7 +1882,7 @@ PyObject* layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
       if (recorded || (at::GradMode::is_enabled() && y.requires_grad())) fail("out= cannot be differentiated through");
       if (y.sizes() != x.sizes() || y.scalar_type() != type || y.device() != dev || !y.is_contiguous())
         fail("out must be a contiguous tensor of x's shape and type on its device");
-      if (!y.is_inference()) y.unsafeGetTensorImpl()->bump_version();
+      mark_written(y);
       // what shares memory with the result is read from a copy, unless it is the very same rows
       if (meet(rows, y) && !(rows.const_data_ptr() == y.const_data_ptr() && row_step(rows) == cols)) rows = rows.clone(at::MemoryFormat::Contiguous);
       if (w.defined() && meet(w, y)) w = w.clone();
