@@ -223,3 +223,15 @@ def test_a_result_that_was_given_counts_as_written():
         out = torch.empty_like(r)
         void.void_expert_linear(e, x, offsets_of([4, 6]), out=out)
         void.void_linear(a, x, out=out, residual=r)
+
+
+# A layer's product counts once towards the third one, behind which a store for groups of tile rows is built.
+def test_a_linear_layer_is_counted_once_before_a_group_store_is_built():
+    a, x = weight(4096, 4096, 0.45, torch.bfloat16), rand(2048, 4096, dtype=torch.bfloat16)
+    void.void_linear(a, x)
+    torch.cuda.synchronize()
+    held = torch.cuda.memory_allocated()
+    void.void_linear(a, x)
+    assert torch.cuda.memory_allocated() - held < a.values.numel()
+    void.void_linear(a, x)
+    assert torch.cuda.memory_allocated() - held > 2 * a.values.numel()

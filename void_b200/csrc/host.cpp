@@ -535,8 +535,9 @@ std::unique_ptr<GroupStore> build_group_store(const Packed* p, int64_t G, int32_
 // The group store that serves this product, or null.  Its build is queued behind the third product it would have served - a
 // tensor that is multiplied once or twice does not pay for it - once for each of up to two widths.  Nothing waits for it:
 // products go to the other kernel until it is complete, and then read it on any stream and ahead of their stream's order.
-// tokens: for a linear layer that reads them as they lie; experts: for that of so many experts, their rows in the order `order`.
-GroupStore* group_store(Packed* p, int64_t N, void_stream_t st, bool tokens = false, int32_t experts = 0, const int32_t* order = nullptr) {
+// tokens: for a linear layer that reads them as they lie; experts: for that of so many experts, their rows in the order `order`.  counted: of
+// a layer that may ask for both kinds, whether this product counts already.
+GroupStore* group_store(Packed* p, int64_t N, void_stream_t st, bool tokens, bool* counted, int32_t experts = 0, const int32_t* order = nullptr) {
   if (!p->grouped || N <= 64 || p->args.nnz < (tokens ? 512 : 4096) || p->kind == VOID_KIND_F8E4M3) return nullptr;   // (FP8 of two terms: within 5 % either way)
   const int slots = 2 * void_device_sm_count();
   const GroupLoad w = group_load(p, N, experts);
@@ -555,10 +556,13 @@ GroupStore* group_store(Packed* p, int64_t N, void_stream_t st, bool tokens = fa
     if (saves > hit_saves && complete(p->groups[n].get(), st)) { hit = p->groups[n].get(); hit_saves = saves; }
   }
   if (best < 0.93 * shape.saves && n < kMaxGroupStores && p->stable && group_blob_bytes(p) <= (4ll << 30) && p->group_calls >= 0 && !capturing(st) &&
-      ++p->group_calls >= 3) {
-    p->group_calls = -1;   // for good, if there is no room for it
-    p->groups[n] = build_group_store(p, (int64_t)shape.groups * weights, experts, order, st);
-    if (p->groups[n] != nullptr) p->group_calls = 0;
+      !*counted) {
+    *counted = true;
+    if (++p->group_calls >= 3) {
+      p->group_calls = -1;   // for good, if there is no room for it
+      p->groups[n] = build_group_store(p, (int64_t)shape.groups * weights, experts, order, st);
+      if (p->groups[n] != nullptr) p->group_calls = 0;
+    }
   }
   return pays(hit_saves) ? hit : nullptr;
 }
@@ -619,11 +623,12 @@ void set_residual(Tail& t, const at::Tensor& given, const at::Tensor& out) {
 // lanes together (kLoose), which the kernel for groups of tile rows does not: bf16 4095 x 4096, 90 %, 4096 tokens, 64 and 156 us.
 bool in_pieces(const void* at, int64_t ld, int64_t es) { return ((reinterpret_cast<uintptr_t>(at) | (uintptr_t)(ld * es)) & 15u) == 0; }
 bool in_pieces(const at::Tensor& t) { return in_pieces(t.const_data_ptr(), t.dim() == 2 ? t.stride(0) : 0, t.element_size()); }
-// A plain product with everything filled in; tokens: the group store of a linear layer that reads them as they lie (transposed = 1).
-void launch_product(Packed* p, const void_spmm_args& s, void_stream_t st, const void_epilogue* tail = nullptr, GroupStore* tokens = nullptr) {
+// A plain product with everything filled in; tokens: the group store of a linear layer that reads them as they lie (transposed = 1); counted: as in
+// group_store.
+void launch_product(Packed* p, const void_spmm_args& s, void_stream_t st, const void_epilogue* tail, GroupStore* tokens, bool counted) {
   if (s.scale_mode == VOID_SCALE_ROW_MEAN) {
     GroupStore* g = s.transposed == 1 ? tokens
-                    : s.transposed == 2 && !in_pieces(s.out, s.ldc, s.out_dtype == VOID_OUT_F32 ? 4 : 2) ? nullptr : group_store(p, s.N, st);
+                    : s.transposed == 2 && !in_pieces(s.out, s.ldc, s.out_dtype == VOID_OUT_F32 ? 4 : 2) ? nullptr : group_store(p, s.N, st, false, &counted);
     if (g != nullptr) {
       g->readers.add(c10::cuda::getCurrentCUDAStream(p->device), {&g->index, &g->blob});
       if (p->captured && capturing(st)) g->captured = true;
@@ -684,7 +689,8 @@ PyObject* spmm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
   const void_stream_t st = launch_stream(pk);
   const bool whole = in_pieces(out) && (n < 13 || none(a[12]) || in_pieces(cuda_tensor(a[12], "residual")));
-  GroupStore* tokens = tr && none(a[11]) && whole ? group_store(pk, N, st, true) : nullptr;
+  bool counted = false;
+  GroupStore* tokens = tr && none(a[11]) && whole ? group_store(pk, N, st, true, &counted) : nullptr;
   const bool copied = tr && none(a[11]) && tokens == nullptr && copy_pays(pk->kind, pk->args.nnz, N, pk->K);
   at::Tensor b = copied ? transposed_copy(b_in, es) : kernel_operand(b_in, es, tr ? 0 : pk->args.nnz * ((N + 127) / 128));
   // (a layer that updates its own tokens, x + x A^T: every tile row reads all of a token)
@@ -769,7 +775,7 @@ PyObject* spmm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   // bit 2: the packed store (and the plan, whose builder synchronises) is complete, so the kernel may read it
   // before it waits for the previous kernel; bit 30 (measurements) keeps it from doing so
   s.flags = (int32_t)(flags & 0xffff) | ((pk->stable && !(flags & (1ll << 30))) ? 4 : 0);
-  if (none(a[11])) launch_product(pk, s, st, tail.get(), tokens);
+  if (none(a[11])) launch_product(pk, s, st, tail.get(), tokens, counted);
   else if (es > 1) check(void_spmm_fp(&s, pk->kind, st), "void_spmm_fp");
   else check(pk->kind == VOID_KIND_I8 ? void_spmm_i8(&s, st) : void_spmm_f8(&s, st), "void_spmm");
   if (!none(a[2])) {
@@ -798,7 +804,8 @@ at::Tensor two_layers(Packed* first, Packed* second, const at::Tensor& x, PyObje
   const void_stream_t st = launch_stream(pk[0]);
   launch_stream(pk[1]);
   const bool whole = pk[1]->M * es % 16 == 0 && (none(residual) || in_pieces(cuda_tensor(residual, "residual")));   // (of the second result)
-  GroupStore* tokens[2] = {group_store(pk[0], N, st, true), whole ? group_store(pk[1], N, st, true) : nullptr};
+  bool counted[2] = {false, false};
+  GroupStore* tokens[2] = {group_store(pk[0], N, st, true, &counted[0]), whole ? group_store(pk[1], N, st, true, &counted[1]) : nullptr};
   const bool columns = (tokens[0] == nullptr || tokens[1] == nullptr) && N > 128 &&
                        copy_saves_ns(kind, pk[0]->args.nnz + pk[1]->args.nnz, N) > copy_costs_ns(N, pk[0]->K, es);
   at::Tensor in = columns ? transposed_copy(x, es) : kernel_operand(x, es), bias[2], out;
@@ -826,7 +833,7 @@ at::Tensor two_layers(Packed* first, Packed* second, const at::Tensor& x, PyObje
     s.transposed = columns ? (layer == 0 ? 0 : 2) : 1;
     s.flags = p->stable ? 4 : 0;
     if (layer == 1 && !none(residual)) set_residual(tail, cuda_tensor(residual, "residual"), out);
-    launch_product(p, s, st, tail.get(), tokens[layer]);
+    launch_product(p, s, st, tail.get(), tokens[layer], counted[layer]);
     in = out;
   }
   return out;
@@ -1597,7 +1604,8 @@ PyObject* expert_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
   const void_stream_t st = launch_stream(pk);
   const int32_t* rows = order.defined() ? order.const_data_ptr<int32_t>() : nullptr;
-  GroupStore* g = expert_chunk(N, experts) == 128 && in_pieces(out) ? group_store(pk, N, st, true, (int32_t)experts, rows) : nullptr;
+  bool counted = false;
+  GroupStore* g = expert_chunk(N, experts) == 128 && in_pieces(out) ? group_store(pk, N, st, true, &counted, (int32_t)experts, rows) : nullptr;
   ExpertPlan plan = expert_plan(offsets, N, experts, dev, pk->args.status, g == nullptr);
   plan.x.row_order = rows;
   plan.x.zero_rest = none(a[7]) ? 1 : 0;
