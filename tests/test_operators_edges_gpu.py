@@ -235,3 +235,20 @@ def test_a_linear_layer_is_counted_once_before_a_group_store_is_built():
     assert torch.cuda.memory_allocated() - held < a.values.numel()
     void.void_linear(a, x)
     assert torch.cuda.memory_allocated() - held > 2 * a.values.numel()
+
+
+# The bias's gradient is a sum of its own type, whatever the tokens' is.
+@pytest.mark.parametrize("act", ["relu", "silu", "none"])
+def test_bias_gradients_in_their_own_type(act):
+    a, x = weight(64, 96, 0.5, torch.bfloat16), rand(257, 96, dtype=torch.bfloat16)
+    experts = void.SparseExperts(void.stack_experts([a, a]), activation=act, dtype=torch.float16)
+    layers = [(experts, lambda: experts(x, offsets_of([257, 0])))]
+    if act != "none":
+        layer = void.SparseLinear(96, 64, a, dtype=torch.float16, activation=act)
+        layers.append((layer, lambda: layer(x)))
+    for layer, call in layers:
+        with torch.no_grad():
+            layer.bias.fill_(50.0)       # (slopes of one)
+        y = call()
+        db, = torch.autograd.grad(y, (layer.bias,), torch.ones_like(y))
+        assert db.dtype == torch.float16 and torch.equal(db.reshape(-1, 64)[0].float(), torch.full((64,), 257.0, device="cuda"))

@@ -1397,7 +1397,9 @@ at::Tensor column_sums(const at::Tensor& m) {
   return out;
 }
 
-// dz = g act'(z) [N, M] and its column sums, the gradient of the bias (of type bias_type; left out where `bias` is null).
+// The type that the gradient of a bias is summed to: the bias's own where the kernels write it, else fp32 (autograd then rounds once).
+at::ScalarType bias_sum_type(at::ScalarType bias, at::ScalarType tokens) { return bias == tokens ? tokens : at::kFloat; }
+// dz = g act'(z) [N, M] and its column sums, the gradient of the bias (for one of type bias_type; left out where `bias` is null).
 at::Tensor activation_gradient(const at::Tensor& g_in, const at::Tensor& z, int32_t act, at::Tensor* bias, at::ScalarType bias_type) {
   const c10::Device dev = z.device();
   const at::Tensor g = as_type(g_in, z.scalar_type()).contiguous();
@@ -1406,7 +1408,7 @@ at::Tensor activation_gradient(const at::Tensor& g_in, const at::Tensor& z, int3
   const at::Tensor dz = pitched(rows, cols, z.scalar_type(), (int)z.element_size(), dev);
   at::Tensor ws;
   if (bias != nullptr) {
-    *bias = new_cuda({cols}, bias_type == at::kFloat ? at::kFloat : z.scalar_type(), dev);
+    *bias = new_cuda({cols}, bias_sum_type(bias_type, z.scalar_type()), dev);
     ws = new_cuda({(int64_t)void_activation_grad_ws_bytes((int32_t)rows, (int32_t)cols)}, at::kByte, dev);
   }
   check(void_activation_grad(g.const_data_ptr(), cols, z.const_data_ptr(), z.stride(0), elem, (int32_t)rows, (int32_t)cols, act,
@@ -1715,7 +1717,7 @@ struct ExpertBackward : torch::autograd::Node {
         at::Tensor ws;
         if (act != VOID_ACT_NONE) dz = pitched(N, M, g.scalar_type(), (int)g.element_size(), dev);
         if (sums) {
-          out[2] = new_cuda({E, M}, bias_type == at::kFloat ? at::kFloat : g.scalar_type(), dev);
+          out[2] = new_cuda({E, M}, bias_sum_type(bias_type, g.scalar_type()), dev);
           ws = new_cuda({(int64_t)void_expert_activation_grad_ws_bytes(&plan.x, (int32_t)N, (int32_t)M)}, at::kByte, dev);
         }
         check(void_expert_activation_grad(g.const_data_ptr(), M, pre.defined() ? pre.const_data_ptr() : nullptr, pre.defined() ? pre.stride(0) : M, elem,
