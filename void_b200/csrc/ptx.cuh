@@ -127,6 +127,10 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, vo
 __device__ __forceinline__ void prefetch_l2(const void* at) {
   asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
 }
+// Of `bytes` bytes at once, by one thread (address and number multiples of 16).
+__device__ __forceinline__ void bulk_prefetch_l2(const void* at, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(at), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void prefetch_tmap(const CUtensorMap* m) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
 }

@@ -212,11 +212,12 @@ __global__ void __launch_bounds__(512) skinny_kernel(const __grid_constant__ Par
   if (t0 + warp + lane * warps < t1) cols = p.tile_cols[t0 + warp + lane * warps];
   if (p.a_stable) {
     // The row's tiles come into the second cache while the kernel before this one ends; a warp then has more of them on their way than
-    // its registers hold.  bf16 with bias, GELU and residual, weights from memory, us: 4096^2, 80 %, 1 token 5.5 -> 4.9, 16 tokens 6.4 -> 5.6,
-    // 50 %, 8 tokens 8.7 -> 8.0; 2048 -> 8192, 90 %, 8 tokens 4.7 -> 3.9 (all in the second cache before: 4.6 -> 4.8, 5.8 -> 5.6, 7.0 -> 7.3, 3.5).
-    const int lines = ES * 8 * (KIND == VOID_KIND_F8E4M3 ? p.terms : 1);
-    const long long mine = (long long)(t1 - t0) * lines;
-    for (long long i = threadIdx.x; i < mine; i += blockDim.x) prefetch_l2(p.tiles + ((size_t)t0 * lines + (size_t)i) * 128);
+    // its registers hold.  One thread asks for all of them (a prefetch per line by every thread takes registers and time: 16 tokens with everything in L2
+    // 5.3).  bf16, linear layer with bias and GELU and plain product, without and with, us, weights from memory: 4096^2, 80 %, 1 token 5.2 -> 4.5 and 7.5
+    // -> 7.0, 16 tokens 5.2 -> 4.5 and 6.7 -> 6.3, 50 %, 8 tokens 8.4 -> 7.6 and 9.6 -> 9.0; 2048 -> 8192, 90 %, 8 tokens 4.4 -> 3.5 and 4.8 -> 4.0; all in the
+    // second cache before: 3.95 -> 4.0 and 6.4 -> 6.4, 4.3 -> 4.3 and 6.0 -> 5.95, 6.6 -> 6.75 and 8.4 -> 8.5, 3.1 -> 3.2 and 3.7 -> 3.7.
+    const long long tile = ES * 1024 * (KIND == VOID_KIND_F8E4M3 ? p.terms : 1), bytes = (t1 - t0) * tile;
+    if (threadIdx.x == 0 && blockIdx.y == 0 && bytes > 0) bulk_prefetch_l2(p.tiles + t0 * tile, (uint32_t)(bytes < (1 << 30) ? bytes : (1 << 30)));
     grid_dependency_wait();
   }
   int seen = 0;
