@@ -5,7 +5,7 @@ import torch
 
 import void_b200 as void
 from test_experts_gpu import experts_of, offsets_of
-from test_linear_cpu import within
+from test_linear_cpu import U, rounded, within
 from test_linear_gpu import feed_forward64, rand, weight
 from test_norm_cpu import norm64, norm_grad64
 from test_norm_gpu import backward_bounds, make
@@ -252,3 +252,26 @@ def test_bias_gradients_in_their_own_type(act):
         y = call()
         db, = torch.autograd.grad(y, (layer.bias,), torch.ones_like(y))
         assert db.dtype == torch.float16 and torch.equal(db.reshape(-1, 64)[0].float(), torch.full((64,), 257.0, device="cuda"))
+
+
+@pytest.mark.parametrize("density", [0.1, 0.5])
+def test_int8_layers_with_a_residual_by_every_kernel(density):
+    # (rows, rows on a transposed copy, groups of tile rows on that copy; a residual that lies anyhow leaves the groups)
+    n, k, m = 1100, 4096, 4096
+    q = void.quantize_void_tensor(weight(m, k, density, torch.float32))
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    x = torch.randint(-128, 128, (n, k), generator=gen, device="cuda", dtype=torch.int8)
+    scale, bias, around = rand(n).abs() + 0.1, rand(m, seed=1), rand(n, m + 3, dtype=torch.bfloat16, seed=2)
+    row = q.block_rows.long().cpu()
+    mean = torch.zeros(128, dtype=torch.float64).scatter_reduce(0, row, q.scales.double().cpu(), "mean", include_self=False).cuda()
+    dense = torch.zeros(128, 128, 32, 32, device="cuda", dtype=torch.float64)
+    dense[q.block_rows.long(), q.block_cols.long()] = q.values.double()
+    part = (x.double() @ dense.permute(0, 2, 1, 3).reshape(m, k).t()) * mean.repeat_interleave(32) * scale.double()[:, None]
+    z = part + bias.double()
+    for r in (around[:, :m].contiguous(), around[:, 1:m + 1]):
+        ref = z.clamp_min(0) + r.double()
+        # exact sums, one rounding to fp32; the mean scale (a sum of up to K / 32 terms), two products and two sums in fp32
+        e = (k / 32 + 8) * U * part.abs() + 4 * U * (bias.double().abs() + ref.abs() + r.double().abs())
+        for _ in range(5):
+            within(void.void_linear(q, x, bias, 1, x_scale=scale, out_dtype=torch.bfloat16, residual=r), ref, rounded(e, ref, torch.bfloat16))
+            torch.cuda.synchronize()
