@@ -51,11 +51,11 @@ inline DeviceInfo device_info() {
 
 // cudaFuncSetAttribute per (kernel, device), repeated only when a larger ring is asked for.
 // All kernels share one C++ function-pointer type, so the record is keyed by the pointer value.  The table
-// holds every instantiation of the library on up to 16 devices; beyond that the attribute is simply set again
+// holds every instantiation of the library (about 500) on up to 8 devices; beyond that the attribute is simply set again
 // on every launch of the pairs that found no room (correct, a little slower).
 inline int ensure_smem(const void* kernel, int bytes) {
   struct Rec { const void* fn; int dev; int bytes; };
-  constexpr int kRecs = 192 * 16;
+  constexpr int kRecs = 512 * 8;
   static Rec recs[kRecs];
   static int n_recs = 0;
   static std::mutex mu;

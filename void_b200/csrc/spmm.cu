@@ -351,9 +351,10 @@ static int spmm_launch(const void_spmm_args* a, int kind, cudaStream_t stream, c
   if (large16 && total_panels > 1) shape = slim_rows ? 2 : 6;
   if (plain && np == 1 && es == 4 && n_items > 6ll * dev.sms && !(tr_b && short_rows)) shape = 6;
   // What a linear layer reads and writes besides keeps the epilogue of 16-bit rows busy for as long as the products take, so its rows go to
-  // eight warps with 16 columns each, which also have the registers to ask for the residual ahead.  bf16, us, slim or mid / wide, with a
-  // residual and with all of training (z kept, GELU): 4096^2, 90 %, 4096 tokens 47.3 / 45.6 and 65.5 / 60.5; 75 % 86.5 / 82.8 and 100.5 /
-  // 95.7; 2048 -> 8192, 80 %, 2048 tokens 45.5 / 44.4 and 63.7 / 59.3; 5008 -> 3008, 85 %, 333 tokens 10.0 / 9.2 and 14.7 / 13.6.
+  // eight warps with 16 columns each, which also have the registers to ask for the residual ahead.  bf16, us, slim / mid / wide, with a residual and with
+  // all of training (z kept, GELU): 4096^2, 4096 tokens, 75 % 91 / 88 / 88 and 97 / 94 / 93; 90 % 48.3 / 44.0 / 44.8 and 56.8 / 51.0 / 50.6; 95 % 39.3 / 33.2 / 33.2
+  // and 50.8 / 44.8 / 41.6; 99 % (a tile or two per row) 37.3 / 31.4 / 31.0 and 48.0 / 42.6 / 40.2; 2048 -> 8192, 2048 tokens, 75 % 54 / 52 / 52 and 61 / 58 / 57.5,
+  // 95 % 33.5 / 29.4 / 29.5 and 46.8 / 41.4 / 39.4; 5024 -> 3008, 333 tokens, 75 % 11.8 / 11.3 / 10.9 and 12.5 / 12.2 / 11.4, 95 % 6.5 / 5.9 / 5.5 and 7.1 / 6.7 / 5.9.
   const bool loose = tr && (!in_pieces(a->out, a->out_dtype, a->ldc) ||
                             (tail != nullptr && tail->residual != nullptr && !in_pieces(tail->residual, tail->residual_dtype, tail->ldr)));
   if (a->cta_shape == 0 && es == 2 && tr_b && tail != nullptr && (tail->residual != nullptr || tail->pre != nullptr)) shape = 1;
