@@ -82,11 +82,14 @@ def stack_experts(weights: Sequence[VOIDTensor]) -> VOIDExperts:
             raise ValueError("stack_experts takes weights of one shape, type and device, got %s %s on %s and %s %s on %s" % (
                 tuple(first.shape), first.values.dtype, first.values.device, tuple(w.shape), w.values.dtype, w.values.device))
     rows, cols = (first.shape[0] + 31) // 32, first.shape[1]
-    block_rows = torch.cat([w.block_rows.to(torch.int32) for w in weights])
-    if block_rows.numel() and not 0 <= int(block_rows.min()) <= int(block_rows.max()) < rows:     # (they would be another expert's)
-        raise ValueError("invalid VOID tile list: block rows outside the block grid of %s" % (tuple(first.shape),))
-    block_rows += torch.repeat_interleave(torch.arange(len(weights), dtype=torch.int32) * rows,
-                                          torch.tensor([w.block_rows.numel() for w in weights])).to(block_rows.device)
+    block_rows = torch.cat([w.block_rows for w in weights]).to(torch.int32)
+    if block_rows.numel():
+        low, high = torch.stack(block_rows.aminmax()).tolist()
+        if low < 0 or high >= rows:                        # (they would be another expert's)
+            raise ValueError("invalid VOID tile list: block rows outside the block grid of %s" % (tuple(first.shape),))
+    counts = torch.tensor([w.block_rows.numel() for w in weights], device=block_rows.device)
+    block_rows += torch.repeat_interleave(torch.arange(len(weights), dtype=torch.int32, device=block_rows.device) * rows, counts,
+                                          output_size=block_rows.numel())
     tensor = VOIDTensor(values=torch.cat([w.values for w in weights]), block_rows=block_rows,
                         block_cols=torch.cat([w.block_cols.to(torch.int32) for w in weights]),
                         morton_codes=torch.empty(0, dtype=torch.int64, device=first.values.device), shape=(len(weights) * rows * 32, cols),
