@@ -20,7 +20,8 @@ from .norm import VOIDLayerNorm
 
 # Index arrays per sparsity structure: tile index and column list of A and of A^T, work items of the tile gradient.  The
 # autograd functions only see bare tensors, and a layer's structure stays fixed while its values train, so the derived
-# arrays are kept here, keyed by the identity of the index tensors (a handful of layers; oldest dropped).
+# arrays are kept here, keyed by the identity of the index tensors (a handful of layers; oldest dropped, a layer that is gone no sooner).  The
+# first pass with a tile list builds them: 0.45 ms for up to 6000 tiles, with a wait for the GPU.
 _STRUCTURE = {}
 _STRUCTURE_MAX = 64
 
@@ -125,7 +126,9 @@ class VOIDLinearFunction(Function):
         dL/dA_values = (dL/dz)^T @ x      - for the stored tiles only (void_linear_tile_grad reads both as they lie)
         dL/dbias     = column sums of dL/dz
         dL/dresidual = dL/dy
-    With an activation z is kept for the backward pass, in y's type, and the layer can be differentiated once.
+    With an activation z is kept for the backward pass, in y's type, and the layer can be differentiated once.  ReLU's slope is one where z > 0.
+    In fp16 and bf16 z is computed again in 64 bits where the sum's errors reach its sign, for at most 256 of the values of 32 tokens and 256
+    outputs (beyond, and in fp32, which is multiplied as TF32, the sign is that of the sum as it came); an infinite gradient does not pass a slope of zero.
     The reference's SparseLinear computes (A @ x^T)^T through VOIDSpMMFunction and adds the bias as a
     separate op (void/autograd.py:320-344)."""
 

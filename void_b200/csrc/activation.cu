@@ -225,10 +225,10 @@ __global__ void __launch_bounds__(256) partial_sums_kernel(const float* partials
 }
 
 // Values of z that lie next to ReLU's border, computed again.  The slope there is a question of z's sign, and the tensor cores cut what they hold
-// after every product that they add, by half of 2^-23 of it: of 35 million sums of rows of 3 to 107 tiles none was off by more than 3.2 times
+// after every product that they add, by half of 2^-23 of it: of 45 million sums of rows of 3 to 107 tiles none was off by more than 3.2 times
 // (tiles + 16) 2^-23 of what is typical of its token, the square of the mean root of |sum| over a strip of up to 256 columns (which one large value hardly
 // moves).  The border is eight times that, and as many times four for the bias, which a sum that it cancels has grown to.  What lies inside, or is -0 (with_bias),
-// is summed in 64 bits: of normal values one in thirty thousand for rows of 13 tiles, at most kMostDoubtful of a block's 8192 whatever the values are; those
+// is summed in 64 bits: of normal values one in sixty thousand for rows of 13 tiles, at most kMostDoubtful of a block's 8192 whatever the values are; those
 // beyond, the last of the block, keep the sign they were summed to.  The order is that of tokens and columns: the same result every time.
 // (What fp16 would round to zero has kept its sign, keep_sign.)  One value is summed by the block, eight of them by a warp each.
 // us, forward pass with SiLU and with ReLU and this behind it, fp16, bias and residual: 4096^2, 90 %, 4096 tokens 63 and 87; 2048^2, 50 %, 512 tokens 14

@@ -3,8 +3,9 @@
 //     xh = (x - mean) / sqrt(var + eps)          y = xh w + b                       per token, D features
 //     gw = g w       dx = rstd (gw - mean(gw) - xh mean(gw xh))       dw = sum over tokens of g xh       db = sum over tokens of g
 //
-// Memory bounds both: 2 D elements per token forward (x, y), 3 D backward (g, x, dx).  On B200, of 6.5 TB/s of copies: 16384 x 4096 bf16 5.2
-// TB/s forward (52 us) and 4.8 backward (84 us), 8192 x 8192 5.9 and 4.7, 3001 x 5003 fp32 4.2 and 3.5.  A token's row stays in registers between its
+// Memory bounds both: 2 D elements per token forward (x, y), 3 D backward (g, x, dx).  On B200, of 6.5 TB/s of copies: 16384 x 4096 bf16 5.3
+// TB/s forward (51 us) and 4.9 backward (82 us with the sums over tokens), 8192 x 8192 6.0 and 4.7, 3001 x 5003 fp32 4.5 and 4.1; a row per block,
+// 2048 x 4096 bf16 2.9 and 1.8.  A token's row stays in registers between its
 // reductions, so it comes in once; the variance is the mean square of the centred values (two passes over registers: no
 // cancellation for rows with a large mean).  All sums are fp32.  Backward, the block walks many rows and a thread keeps the same
 // columns throughout, so the sums over tokens stay in its registers; they leave as one row of partial sums per block, which a second
@@ -265,8 +266,8 @@ struct Params {
 
 // C: elements of a thread, in pieces of E; S: rows in shared memory; MOST: threads at most.  What bounds such a kernel beside memory is
 // the number of its instructions (the two sums over a block take a hundred per warp and row whatever a thread has of the row), so a thread
-// takes many elements and computes in pairs.  16384 x 4096 bf16, eight elements per thread and single operations: 0.70 instructions per
-// clock and scheduler, 72 us; parameters read for every row again: 72 us with fp32 ones, 60 with bf16.
+// takes many elements and computes in pairs.  16384 x 4096 bf16, eight elements per thread and single operations: 72 us;
+// parameters read for every row again: 72 us with fp32 ones, 60 with bf16; this way 51, at 0.67 instructions per clock and scheduler.
 template <typename T, typename P, int E, int C, int S, int MOST>
 __global__ void __launch_bounds__(MOST, MOST <= 256 ? (C > 16 ? 2 : 3) : (MOST <= 384 ? 2 : 1)) layer_norm_rows_kernel(const __grid_constant__ NormParams p) {
   constexpr int PIECE = (int)sizeof(T) * E, NV = C / E;
