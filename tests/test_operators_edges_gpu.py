@@ -275,3 +275,17 @@ def test_int8_layers_with_a_residual_by_every_kernel(density):
         for _ in range(5):
             within(void.void_linear(q, x, bias, 1, x_scale=scale, out_dtype=torch.bfloat16, residual=r), ref, rounded(e, ref, torch.bfloat16))
             torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_weights_taken_from_a_layer_follow_its_training(dtype):
+    a, x = weight(64, 96, 0.5, dtype), rand(40, 96, dtype=dtype)
+    experts, layer = void.SparseExperts(void.stack_experts([a, a]), bias=False), void.SparseLinear(96, 64, a, bias=False)
+    kept, matrix, offsets = experts.get_experts(), layer.sparse_weight.get_void_tensor(), offsets_of([25, 15])
+    for _ in range(3):
+        want, want2 = void.void_expert_linear(kept, x, offsets), void.void_linear(matrix, x)
+        assert not kept.values.requires_grad and not matrix.values.requires_grad
+        with torch.no_grad():                                # a step of an optimiser
+            experts.values.mul_(2.0)
+            layer.sparse_weight.values.mul_(2.0)
+        assert torch.equal(void.void_expert_linear(kept, x, offsets), 2 * want) and torch.equal(void.void_linear(matrix, x), 2 * want2)

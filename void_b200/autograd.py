@@ -163,7 +163,7 @@ class VOIDSpMM(torch.nn.Module):
         return y.squeeze(1) if squeeze else y
 
     def get_void_tensor(self) -> VOIDTensor:
-        return _bare_void(self.values.data, self.block_rows, self.block_cols, self.shape, self.tile_size, self.n_blocks)
+        return _bare_void(self.values.detach(), self.block_rows, self.block_cols, self.shape, self.tile_size, self.n_blocks)
 
 
 class SparseLinear(torch.nn.Module):

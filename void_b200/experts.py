@@ -198,9 +198,9 @@ class SparseExperts(torch.nn.Module):
         return _lib.native().expert_values_product(st, self.values, x, offsets, self.bias, self._activation)
 
     def get_experts(self) -> VOIDExperts:
-        """The weights as they are now, for void_expert_linear (they share memory with the parameter)."""
+        """The weights for void_expert_linear: they share memory with the parameter and follow its changes."""
         rows = (self.out_features + 31) // 32
-        tensor = VOIDTensor(values=self.values.data, block_rows=self.block_rows, block_cols=self.block_cols,
+        tensor = VOIDTensor(values=self.values.detach(), block_rows=self.block_rows, block_cols=self.block_cols,
                             morton_codes=torch.empty(0, dtype=torch.int64, device=self.values.device),
                             shape=(self.n_experts * rows * 32, self.in_features), tile_size=(32, 32), nnz_original=0, n_blocks=self.n_blocks,
                             density=0.0, dtype=self.values.dtype)
