@@ -289,3 +289,30 @@ def test_weights_taken_from_a_layer_follow_its_training(dtype):
             experts.values.mul_(2.0)
             layer.sparse_weight.values.mul_(2.0)
         assert torch.equal(void.void_expert_linear(kept, x, offsets), 2 * want) and torch.equal(void.void_linear(matrix, x), 2 * want2)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_relu_in_training_captured_and_replayed_with_other_tokens(dtype):
+    dense, bias = weight(200, 96, 1.0, torch.float32).to_dense(), rand(200, seed=1)
+    bias[::3] = 0.0
+    x, g = rand(150, 96, dtype=dtype), rand(150, 200, dtype=dtype, seed=3)
+    x.requires_grad_(True)
+    for layer, values, call in relu_layers(dense, bias, dtype):
+        def step():
+            y = call(x)
+            return [y.detach(), *torch.autograd.grad(y, (x, values, layer.bias), g)]
+        if isinstance(layer, void.SparseExperts):            # (the offsets are made outside: a capture copies nothing from the host)
+            offsets = offsets_of([100, 50])
+            call = lambda t, f=layer, o=offsets: f(t, o)     # noqa: E731
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step()
+        for seed in (50, 51):
+            with torch.no_grad():
+                x.copy_(rand(150, 96, dtype=dtype, seed=seed))
+                x[7] = 0.0
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(outs, step()))
