@@ -213,7 +213,7 @@ def test_a_result_that_was_given_counts_as_written():
     a, e = weight(64, 64, 0.5, dtype), experts_of(2, 64, 64, 0.5, dtype)[1]
     x, r = rand(10, 64, dtype=dtype), rand(10, 64, dtype=dtype, seed=1)
     for write in (lambda out: void.void_expert_linear(e, x, offsets_of([4, 6]), out=out), lambda out: void.void_linear(a, x, out=out, residual=out),
-                  lambda out: void.void_layer_norm(x, out=out)):
+                  lambda out: void.void_layer_norm(x, out=out), lambda out: void.void_spmv(a, x[0], out=out[0])):
         factor, out = torch.ones(10, 64, dtype=dtype, device="cuda", requires_grad=True), r.clone()
         y = factor * out
         write(out)

@@ -895,6 +895,7 @@ PyObject* spmv(PyObject*, PyObject* const* a, Py_ssize_t n) {
   s.flags = pk->stable ? 4 : 0;
   check(void_spmm_fp(&s, pk->kind, launch_stream(pk)), "void_spmm_fp");
   if (!none(a[2])) {
+    mark_written(out);
     Py_INCREF(a[2]);
     return a[2];
   }
