@@ -621,6 +621,75 @@ VOID_API int void_layer_norm_grad(const void* g, int64_t ldg, const void* x, int
                                   int32_t cols, const void* weight, int32_t param_elem, const float* stats, void* dx,
                                   int64_t lddx, void* dweight, void* dbias, void* ws, size_t ws_bytes, void_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Tokens on their way to experts and back (no counterpart in the reference).
+ * void_route: the top_k (at most 32) largest of each token's n_experts (at most 1024) scores [rows, n_experts] of type elem, lds elements
+ * between rows, in falling order, ties to the lowest index, NaN above all; experts [rows, top_k] and weights [rows, top_k], the softmax of the
+ * scores at those places, over the chosen ones (normalize) or over all.  A score of -infinity is never chosen: such a slot gets expert -1
+ * and weight 0.  void_route_grad: the gradient of the scores [rows, n_experts] from that of the weights, g [rows, top_k].
+ * void_sort_by_expert: position [count] of every choice (ids of index_bytes 4 or 8) when all are sorted by expert in the order given, -1 where an id
+ * lies outside [0, n_experts); offsets [n_experts + 1].  ws: void_sort_by_expert_ws_bytes bytes.
+ * void_dispatch: the same for experts [tokens, top_k], and the rows of out [tokens * top_k, cols] filled: row position[t, j] with token t,
+ * those behind the last run with zeros if zero_rest, else left alone.
+ * void_combine: out[t] = residual[t] + sum_j weights[t, j] rows[position[t, j]], fp32 sums in the order of j; weights [tokens, top_k] of
+ * weight_elem, or NULL for ones; residual of elem or fp32, or NULL; choices without a row are left out.  out may be the residual.
+ * void_combine_grad: drows (NULL: not wanted; rows from *used_rows on are zeroed) and dweights (likewise; of weight_elem) from the gradient
+ * g [tokens, cols] of void_combine's result.  void_dispatch's gradient is void_combine without weights.
+ * ------------------------------------------------------------------------------------- */
+VOID_API int void_route(const void* scores, int32_t elem, int64_t lds, int64_t rows, int32_t n_experts, int32_t top_k, int32_t normalize,
+                        int32_t* experts, float* weights, void_stream_t stream);
+VOID_API int void_route_grad(const void* scores, int32_t elem, int64_t lds, int64_t rows, int32_t n_experts, int32_t top_k, int32_t normalize,
+                             const float* g, int64_t ldg, void* dscores, int64_t ldd, void_stream_t stream);
+VOID_API size_t void_sort_by_expert_ws_bytes(int64_t count, int32_t n_experts);
+VOID_API int void_sort_by_expert(const void* experts, int32_t index_bytes, int64_t count, int32_t n_experts, int32_t* offsets, int32_t* position,
+                                 void* ws, size_t ws_bytes, void_stream_t stream);
+VOID_API int void_dispatch(const void* x, int32_t elem, int64_t ldx, int64_t tokens, int32_t cols, const void* experts, int32_t index_bytes,
+                           int32_t top_k, int32_t n_experts, int32_t* offsets, int32_t* position, void* out, int64_t ldo, int32_t zero_rest,
+                           void* ws, size_t ws_bytes, void_stream_t stream);
+VOID_API int void_combine(const void* rows, int32_t elem, int64_t ldx, int64_t tokens, int32_t cols, int32_t top_k, const int32_t* position,
+                          const void* weights, int32_t weight_elem, const void* residual, int64_t ldr, int32_t residual_elem, void* out, int64_t ldo,
+                          void_stream_t stream);
+VOID_API int void_combine_grad(const void* g, int64_t ldg, const void* rows, int64_t ldx, int32_t elem, int64_t tokens, int32_t cols, int32_t top_k,
+                               const int32_t* position, const int32_t* used_rows, const void* weights, int32_t weight_elem, void* drows,
+                               int64_t ldd, void* dweights, void_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Linear layers with dense e4m3 weights that carry a scale for each block of 128 x 128, on tokens in e4m3 with a scale for each token's 128
+ * features (no counterpart in the reference, whose FP8 tiles are 32 x 32, void/fp8.py:438-570):
+ *     out[t, m] = act(sum_b x_scale[t, b] a_scale[m / 128, b] sum_{k in b} x[t, k] a[m, k] + bias[m]) + residual[t, m]
+ * a [M, K] (experts: n_experts of them, expert_stride bytes apart), lda bytes between rows; x [N, K], ldx bytes between rows: addresses, pitches
+ * and expert_stride are multiples of 16.  Scales are fp32 with element strides of their own.  bias [M] (experts: [n_experts, M]) of bias_elem or
+ * NULL; residual [N, M] or NULL (one matrix or experts; may be out, the same place and pitch).
+ * experts: NULL, or the plan of void_expert_plan (offset_bytes 0) with chunks of 32, 64, 128 or 256 tokens; row_order is not used.  Rows in no
+ * run are zeroed if zero_rest, else left alone.
+ * void_quant_fp8_blocks: q [rows, cols] e4m3, ldq bytes between rows, and scales [ceil(rows / block_rows), ceil(cols / 128)] (element strides
+ * scale_row, scale_col) of a matrix of type elem, for block_rows 1 or 128.  A scale is the smallest power of two (2^-100 at the least) that
+ * keeps the block within 448, so that nothing is rounded but the quotient to e4m3; a block that holds an infinity or NaN gets a scale of NaN.
+ * ------------------------------------------------------------------------------------- */
+typedef struct void_fp8_args {
+  const void* a;
+  int64_t lda, expert_stride;                       /* bytes */
+  const float* a_scale;
+  int64_t a_scale_row, a_scale_col, a_scale_expert; /* elements */
+  const void* x;
+  int64_t ldx;                                      /* bytes */
+  const float* x_scale;
+  int64_t x_scale_row, x_scale_col;
+  const void* bias;
+  const void* residual;
+  int64_t ldr;
+  void* out;
+  int64_t ldc;
+  int32_t M, K, N;
+  int32_t bias_elem, residual_elem, out_elem;       /* VOID_ELEM_* */
+  int32_t act;
+  int32_t test_hooks;                               /* 0 outside tests */
+  int32_t* status;                                  /* as in void_spmm_args, or NULL */
+} void_fp8_args;
+VOID_API int void_quant_fp8_blocks(const void* x, int32_t elem, int64_t ldx, int64_t rows, int32_t cols, int32_t block_rows, void* q, int64_t ldq,
+                                   float* scales, int64_t scale_row, int64_t scale_col, void_stream_t stream);
+VOID_API int void_fp8_linear(const void_fp8_args* args, const void_experts* experts, void_stream_t stream);
+
 /* number of SMs of the current device (grid sizing on the host side) */
 VOID_API int void_device_sm_count(void);
 

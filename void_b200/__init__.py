@@ -22,6 +22,8 @@ from .autograd import (VOIDSpMMFunction, VOIDLinearFunction, VOIDSpMM, SparseLin
                        void_spmm_autograd)
 from .norm import void_layer_norm, VOIDLayerNorm
 from .experts import VOIDExperts, stack_experts, void_expert_linear, SparseExperts
+from .fp8_blocks import FP8BlockTensor, quantize_fp8_blocks
+from .routing import ExpertRoutes, void_route, sort_by_expert, void_dispatch, void_combine
 from .stream_k import (StreamKWorkload, compute_stream_k_workload, void_spmm_stream_k, analyze_workload_balance)
 from .scheduler import WorkloadProfile, analyze_workload
 from .distributed import (ShardingStrategy, DistributedVOIDTensor, shard_void_tensor, distributed_void_spmm,

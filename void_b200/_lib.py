@@ -65,6 +65,14 @@ class GroupStore(ctypes.Structure):
                 ("max_entries", c_i32), ("max_tiles", c_i32), ("reserved", c_i32)]
 
 
+class Fp8Args(ctypes.Structure):
+    """Mirror of ``struct void_fp8_args``."""
+    _fields_ = [("a", c_vp), ("lda", c_i64), ("expert_stride", c_i64), ("a_scale", c_vp), ("a_scale_row", c_i64), ("a_scale_col", c_i64),
+                ("a_scale_expert", c_i64), ("x", c_vp), ("ldx", c_i64), ("x_scale", c_vp), ("x_scale_row", c_i64), ("x_scale_col", c_i64),
+                ("bias", c_vp), ("residual", c_vp), ("ldr", c_i64), ("out", c_vp), ("ldc", c_i64), ("M", c_i32), ("K", c_i32), ("N", c_i32),
+                ("bias_elem", c_i32), ("residual_elem", c_i32), ("out_elem", c_i32), ("act", c_i32), ("test_hooks", c_i32), ("status", c_vp)]
+
+
 _PROTOTYPES = {
     "void_strerror": (ctypes.c_char_p, [ctypes.c_int]),
     "void_b200_abi_version": (ctypes.c_int, []),
@@ -130,6 +138,15 @@ _PROTOTYPES = {
     "void_expert_activation_grad_ws_bytes": (c_sz, [ctypes.POINTER(Experts), c_i32, c_i32]),
     "void_expert_activation_grad": (ctypes.c_int, [c_vp, c_i64, c_vp, c_i64, c_i32, ctypes.POINTER(Experts), c_i32, c_i32, c_i32, c_vp, c_i64,
                                                    c_vp, c_i32, c_vp, c_sz, c_vp]),
+    "void_route": (ctypes.c_int, [c_vp, c_i32, c_i64, c_i64, c_i32, c_i32, c_i32, c_vp, c_vp, c_vp]),
+    "void_route_grad": (ctypes.c_int, [c_vp, c_i32, c_i64, c_i64, c_i32, c_i32, c_i32, c_vp, c_i64, c_vp, c_i64, c_vp]),
+    "void_sort_by_expert_ws_bytes": (c_sz, [c_i64, c_i32]),
+    "void_sort_by_expert": (ctypes.c_int, [c_vp, c_i32, c_i64, c_i32, c_vp, c_vp, c_vp, c_sz, c_vp]),
+    "void_dispatch": (ctypes.c_int, [c_vp, c_i32, c_i64, c_i64, c_i32, c_vp, c_i32, c_i32, c_i32, c_vp, c_vp, c_vp, c_i64, c_i32, c_vp, c_sz, c_vp]),
+    "void_combine": (ctypes.c_int, [c_vp, c_i32, c_i64, c_i64, c_i32, c_i32, c_vp, c_vp, c_i32, c_vp, c_i64, c_i32, c_vp, c_i64, c_vp]),
+    "void_combine_grad": (ctypes.c_int, [c_vp, c_i64, c_vp, c_i64, c_i32, c_i64, c_i32, c_i32, c_vp, c_vp, c_vp, c_i32, c_vp, c_i64, c_vp, c_vp]),
+    "void_quant_fp8_blocks": (ctypes.c_int, [c_vp, c_i32, c_i64, c_i64, c_i32, c_i32, c_vp, c_i64, c_vp, c_i64, c_i64, c_vp]),
+    "void_fp8_linear": (ctypes.c_int, [ctypes.POINTER(Fp8Args), ctypes.POINTER(Experts), c_vp]),
     "void_layer_norm": (ctypes.c_int, [c_vp, c_i32, c_i64, c_i64, c_i32, c_vp, c_vp, c_i32, c_f32, c_vp, c_i64, c_vp, c_vp]),
     "void_layer_norm_grad_ws_bytes": (c_sz, [c_i64, c_i32]),
     "void_layer_norm_grad": (ctypes.c_int, [c_vp, c_i64, c_vp, c_i64, c_i32, c_i64, c_i32, c_vp, c_i32, c_vp, c_vp, c_i64, c_vp, c_vp,

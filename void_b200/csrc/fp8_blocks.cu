@@ -1,0 +1,652 @@
+// Linear layers whose weights are dense e4m3 matrices with a scale for each block of 128 x 128, on tokens in e4m3 with a scale for each
+// token's 128 features:
+//
+//     out[t, m] = act( sum_b sx[t, b] sa[m / 128, b] sum_{k in block b} x[t, k] a[m, k]  + bias[m] ) + residual[t, m]
+//
+// of one matrix, or of the matrices of experts for tokens sorted by expert.  The product is computed transposed: features are the 128 lanes
+// of tensor memory, tokens the columns (16 to 256 of them, whatever a run of tokens leaves), so a short run costs what its tokens cost.
+// The scales differ from block to block of k, so every block's product is an accumulator of its own, which eight warps read back, multiply by
+// sx sa (one number per token: sa is the same for all lanes) and add in registers, while the tensor cores fill the other of two.
+//
+// With fewer work items than SMs, the blocks of k are dealt to a cluster of CTAs, whose partial sums meet through shared memory, added in the
+// order of the CTAs.
+#include <cuda_runtime.h>
+#include <cudaTypedefs.h>
+#include <stdint.h>
+#include <string.h>
+
+#include "../../include/void_b200.h"
+#include "epilogue.cuh"
+#include "experts.cuh"
+#include "kinds.cuh"
+#include "launch.cuh"
+#include "pipeline.cuh"
+#include "ptx.cuh"
+#include "values.cuh"
+
+namespace vb {
+
+namespace {
+
+constexpr int kBlock = 128;          // features of a block, and of a work item
+constexpr int kTokenBox = 32;        // tokens that one copy brings
+constexpr unsigned kEvery = 0xffffffffu;
+
+// ------------------------------------------------------------------------------------------ quantisers
+struct QuantParams {
+  const void* x;
+  long long ldx, ldq, scale_row, scale_col;
+  long long rows;
+  int cols;
+  uint8_t* q;
+  float* scales;
+};
+// The smallest power of two that keeps numbers up to `amax` within e4m3's 448 = 1.75 * 2^8, and its reciprocal: no rounding but that to
+// e4m3 itself.  bits: of amax, so that NaN is larger than all; a block that holds one, or an infinity, gets a scale of NaN.
+__device__ __forceinline__ float block_scale(uint32_t bits, float& inverse) {
+  int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  e = e < -100 ? -100 : e;
+  inverse = __int_as_float((127 - e) << 23);
+  if (bits >= 0x7f800000u) {
+    inverse = 0.0f;
+    return __int_as_float(0x7fc00000);
+  }
+  return __int_as_float((127 + e) << 23);
+}
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+constexpr int kQuantThreads = 256;
+
+// A scale per row and 128 columns.  Rows in 16-byte pieces: 128 columns lie in 16 lanes (fp32: 32), a warp takes `HELD` groups of 512 bytes of a
+// row at a time; others element by element.
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(kQuantThreads) quant_rows_kernel(const __grid_constant__ QuantParams p) {
+  constexpr int VEC = WIDE ? 16 / (int)sizeof(T) : 4, HELD = WIDE ? 4 : 2;
+  constexpr int LANES = kBlock / VEC;   // of a block of 128 columns: 16 or 32
+  constexpr int STEP = 32 * VEC;
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  const int pieces = (p.cols + STEP * HELD - 1) / (STEP * HELD);
+  const long long items = p.rows * pieces;
+  for (long long i = (long long)blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5); i < items; i += (long long)gridDim.x * (kQuantThreads / 32)) {
+    const long long row = i / pieces;
+    const int c0 = (int)(i - row * pieces) * (STEP * HELD);
+    const T* x = reinterpret_cast<const T*>(p.x) + row * p.ldx;
+    uint8_t* q = p.q + row * p.ldq;
+    float v[HELD][VEC];
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+      if constexpr (WIDE) {
+        const int c = c0 + h * STEP + lane * VEC;
+        Piece<T, VEC> piece;
+        if (c < p.cols) piece.load(x + c);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[h][e] = c < p.cols ? piece.get(e) : 0.0f;
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const int c = c0 + h * STEP + e * 32 + lane;
+          v[h][e] = c < p.cols ? to_float<T>(x[c]) : 0.0f;
+        }
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+      uint32_t most = 0;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) most = max(most, magnitude(v[h][e]));
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(kEvery, most, o));
+      float inverse;
+      const float scale = block_scale(most, inverse);
+      const int first = c0 + h * STEP + (WIDE ? lane / LANES * kBlock : 0);
+      if (first < p.cols && lane % LANES == 0) p.scales[row * p.scale_row + (long long)(first / kBlock) * p.scale_col] = scale;
+      if constexpr (WIDE) {
+        const int c = c0 + h * STEP + lane * VEC;
+        if (c < p.cols) {
+          uint32_t w[VEC / 4];
+#pragma unroll
+          for (int k = 0; k < VEC / 4; ++k)
+            w[k] = e4m3x2(v[h][4 * k] * inverse, v[h][4 * k + 1] * inverse) | e4m3x2(v[h][4 * k + 2] * inverse, v[h][4 * k + 3] * inverse) << 16;
+          if constexpr (VEC == 8) *reinterpret_cast<uint2*>(q + c) = make_uint2(w[0], w[1]);
+          else *reinterpret_cast<uint32_t*>(q + c) = w[0];
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const int c = c0 + h * STEP + e * 32 + lane;
+          if (c < p.cols) q[c] = (uint8_t)e4m3x2(v[h][e] * inverse, 0.0f);
+        }
+      }
+    }
+  }
+}
+
+// A scale per 128 x 128, a block each (weights, once).
+template <typename T>
+__global__ void __launch_bounds__(kQuantThreads) quant_blocks_kernel(const __grid_constant__ QuantParams p) {
+  __shared__ uint32_t most_of[kQuantThreads / 32];
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const long long r0 = (long long)blockIdx.y * kBlock;
+  const int c = blockIdx.x * kBlock + (threadIdx.x & 127);
+  uint32_t most = 0;
+  for (int r = threadIdx.x >> 7; r < kBlock; r += 2)
+    if (r0 + r < p.rows && c < p.cols) most = max(most, magnitude(to_float<T>(reinterpret_cast<const T*>(p.x)[(r0 + r) * p.ldx + c])));
+  most = __reduce_max_sync(kEvery, most);
+  if ((threadIdx.x & 31) == 0) most_of[threadIdx.x >> 5] = most;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kQuantThreads / 32; ++w) most = max(most, most_of[w]);
+  float inverse;
+  const float scale = block_scale(most, inverse);
+  if (threadIdx.x == 0) p.scales[(long long)blockIdx.y * p.scale_row + (long long)blockIdx.x * p.scale_col] = scale;
+  for (int r = threadIdx.x >> 7; r < kBlock; r += 2)
+    if (r0 + r < p.rows && c < p.cols)
+      p.q[(r0 + r) * p.ldq + c] = (uint8_t)e4m3x2(to_float<T>(reinterpret_cast<const T*>(p.x)[(r0 + r) * p.ldx + c]) * inverse, 0.0f);
+}
+
+template <typename T>
+int quant_of_type(const QuantParams& p, int block_rows, int sms, cudaStream_t st) {
+  if (block_rows == kBlock) {
+    const long long down = (p.rows + kBlock - 1) / kBlock;
+    if (down > 65535) return VOID_ERR_TOO_LARGE;
+    return status_of(launch_pdl(quant_blocks_kernel<T>, dim3((unsigned)((p.cols + kBlock - 1) / kBlock), (unsigned)down), kQuantThreads, 0, st, p));
+  }
+  constexpr int VEC = 16 / (int)sizeof(T);
+  const bool wide = p.cols % VEC == 0 && ((reinterpret_cast<uintptr_t>(p.x) | (uintptr_t)(p.ldx * sizeof(T))) & 15u) == 0 &&
+                    ((reinterpret_cast<uintptr_t>(p.q) | (uintptr_t)p.ldq) & 7u) == 0;
+  const int step = wide ? 32 * VEC * 4 : 32 * 4 * 2;
+  const long long items = p.rows * ((p.cols + step - 1) / step), blocks = (items + kQuantThreads / 32 - 1) / (kQuantThreads / 32);
+  const int grid = (int)(blocks < 32ll * sms ? blocks : 32ll * sms);
+  return status_of(wide ? launch_pdl(quant_rows_kernel<T, true>, grid, kQuantThreads, 0, st, p) : launch_pdl(quant_rows_kernel<T, false>, grid, kQuantThreads, 0, st, p));
+}
+
+// ------------------------------------------------------------------------------------------ products
+constexpr int kThreads = 384;         // copies, products, scales (2), then eight warps that add up
+constexpr int kAdders = 8, kFirstAdder = 4;
+constexpr int kMaxRing = 12, kScaleSlots = 8;
+
+struct Fp8Params {
+  int M, K, N, k_blocks, m_tiles;
+  int chunk, n_chunks, group;     // one matrix: tokens of an item, items along the tokens, and of them those taken together
+  const int32_t *head, *bounds;   // experts: the plan of experts.cu
+  const int4* chunks;
+  int n_experts, zero_rest;
+  const float* a_scale;
+  long long as_row, as_col, as_expert;
+  const float* x_scale;
+  long long xs_row, xs_col;
+  const void* bias;
+  int bias_elem;
+  const void* residual;
+  long long ldr;
+  int residual_elem;
+  void* out;
+  long long ldc;
+  int out_elem, act;
+  int splits;                     // CTAs of a cluster, which share an item's blocks of k
+  int stages;
+  int32_t* status;
+  int wait_limit_ms, drop_first;  // drop_first: test hook, the first stage is never filled
+};
+struct __align__(8) Fp8Bars {
+  uint64_t full[kMaxRing], empty[kMaxRing];
+  uint64_t acc_full[2], acc_empty[2];
+  uint64_t scale_full[kScaleSlots], scale_empty[kScaleSlots];
+};
+struct Item {
+  int m, n0, n1, expert;
+};
+__device__ __forceinline__ int items_of(const Fp8Params& p) { return (p.head != nullptr ? p.head[0] : p.n_chunks) * p.m_tiles; }
+// Items that follow one another share tokens or weights: of one matrix, `group` chunks of tokens meet every 128 features.
+__device__ __forceinline__ Item item_at(const Fp8Params& p, int i) {
+  Item t;
+  if (p.head != nullptr) {
+    const int c = i / p.m_tiles;
+    const int4 chunk = p.chunks[c];
+    t.m = i - c * p.m_tiles;
+    t.expert = chunk.x;
+    t.n0 = chunk.y;
+    t.n1 = chunk.z;
+    return t;
+  }
+  const int per = p.group * p.m_tiles, g = i / per, first = g * p.group, wide = p.n_chunks - first < p.group ? p.n_chunks - first : p.group;
+  const int rest = i - g * per;
+  t.m = rest / wide;
+  t.expert = 0;
+  t.n0 = (first + rest - t.m * wide) * p.chunk;
+  t.n1 = t.n0 + p.chunk < p.N ? t.n0 + p.chunk : p.N;
+  return t;
+}
+__device__ __forceinline__ void tma_load_a(uint32_t dst, const CUtensorMap* m, int x, int y, int z, uint32_t bar) { tma_load_3d(dst, m, x, y, z, bar); }
+
+__device__ __forceinline__ uint32_t cluster_address(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_meet() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// What is between a sum and the result, for one lane's feature.
+struct Finish {
+  float bias;
+  __device__ __forceinline__ Finish(const Fp8Params& p, const Item& t, int m) {
+    bias = p.bias != nullptr && m < p.M ? element(p.bias, p.bias_elem, (long long)t.expert * p.M + m) : 0.0f;
+  }
+};
+__device__ __forceinline__ void store_result(const Fp8Params& p, long long token, int m, float v) { set_element(p.out, p.out_elem, token * p.ldc + m, v); }
+
+// NT: tokens of an item at most.
+template <int NT, int CTAS>
+__global__ void __launch_bounds__(kThreads, CTAS) fp8_block_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUtensorMap map_a,
+                                                                   const __grid_constant__ CUtensorMap map_x) {
+  constexpr int CG = NT == 256 || NT == 32 ? 16 : 32;   // columns read back at a time
+  constexpr int GROUPS = NT / 2 / CG;              // of them for one warp: every other one
+  constexpr uint32_t kStageA = kBlock * kBlock, kStage = kStageA + NT * kBlock;
+  constexpr uint32_t kTmem = NT * 2 < 32 ? 32 : NT * 2;
+  extern __shared__ uint8_t raw[];
+  __shared__ Fp8Bars bars;
+  __shared__ __align__(16) float scale_ring[kScaleSlots][NT];
+  __shared__ uint32_t tmem_s;
+  __shared__ int ctl_s[2];
+  volatile int* ctl = ctl_s;
+  const uint32_t ring = (smem_u32(raw) + 1023u) & ~1023u;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    ctl_s[0] = 0;
+    ctl_s[1] = p.wait_limit_ms;
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(smem_u32(&bars.full[s]), 1);
+      mbar_init(smem_u32(&bars.empty[s]), 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(smem_u32(&bars.acc_full[s]), 1);
+      mbar_init(smem_u32(&bars.acc_empty[s]), kAdders);
+    }
+    for (int s = 0; s < kScaleSlots; ++s) {
+      mbar_init(smem_u32(&bars.scale_full[s]), 1);
+      mbar_init(smem_u32(&bars.scale_empty[s]), kAdders);
+    }
+    fence_mbar_init();
+    prefetch_tmap(&map_a);
+    prefetch_tmap(&map_x);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(&tmem_s), kTmem);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_s;
+  grid_dependency_wait();
+
+  const int rank = p.splits > 1 ? (int)cluster_rank() : 0;
+  const int b0 = (int)((long long)p.k_blocks * rank / p.splits), b1 = (int)((long long)p.k_blocks * (rank + 1) / p.splits);
+  const int step = (int)gridDim.x / p.splits, begin = (int)blockIdx.x / p.splits, end = items_of(p);
+  // With several CTAs per item a launch has a cluster for every item, so that the ring is free when the sums meet in its place.
+  if (warp == 0) {
+    int stage = 0;
+    uint32_t phase = 0;
+    bool first = true;
+    for (int i = begin; i < end && !ctl[0]; i += step) {
+      const Item t = item_at(p, i);
+      const int boxes = (t.n1 - t.n0 + kTokenBox - 1) / kTokenBox;
+      for (int b = b0; b < b1; ++b) {
+        if (!mbar_wait_warp(smem_u32(&bars.empty[stage]), phase ^ 1u, ctl)) break;
+        const uint32_t full = smem_u32(&bars.full[stage]), at = ring + (uint32_t)stage * kStage;
+        const bool drop = first && p.drop_first != 0;
+        first = false;
+        if (lane == 0 && !drop) mbar_expect_tx(full, kStageA + (uint32_t)boxes * (kTokenBox * kBlock));
+        __syncwarp();
+        if (!drop) {
+          if (lane == 0) tma_load_a(at, &map_a, b * kBlock, t.m * kBlock, t.expert, full);
+          if (lane >= 1 && lane <= boxes)
+            tma_load_2d(at + kStageA + (uint32_t)(lane - 1) * (kTokenBox * kBlock), &map_x, b * kBlock, t.n0 + (lane - 1) * kTokenBox, full);
+        }
+        if (++stage == p.stages) { stage = 0; phase ^= 1u; }
+      }
+    }
+  } else if (warp == 1) {
+    constexpr uint64_t kDescHi = smem_desc_hi(16, 1024, kLayoutSw128);
+    const bool leader = elect_one();
+    int stage = 0;
+    uint32_t phase = 0, it = 0;
+    bool ok = true;
+    for (int i = begin; i < end && ok; i += step) {
+      const Item t = item_at(p, i);
+      const uint32_t idesc = instr_desc(1, 0, 0, 0, 0, 128, (uint32_t)(t.n1 - t.n0 + 15) & ~15u);
+      for (int b = b0; b < b1; ++b, ++it) {
+        const uint32_t slot = it & 1u;
+        ok = mbar_wait_warp(smem_u32(&bars.acc_empty[slot]), ((it >> 1) & 1u) ^ 1u, ctl) && mbar_wait_warp(smem_u32(&bars.full[stage]), phase, ctl);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t at = ring + (uint32_t)stage * kStage;
+        const uint64_t da = smem_desc(kDescHi, at), db = smem_desc(kDescHi, at + kStageA);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)   // 32 features each: 32 bytes further in rows of 128
+          issue_mma<VOID_KIND_F8E4M3>(leader, tmem + slot * NT, da + 2 * k, db + 2 * k, idesc, k > 0);
+        tc_commit_if(leader, smem_u32(&bars.empty[stage]));
+        tc_commit_if(leader, smem_u32(&bars.acc_full[slot]));
+        if (++stage == p.stages) { stage = 0; phase ^= 1u; }
+      }
+    }
+  } else if (warp < kFirstAdder) {
+    // The products of both scales, every other block of k for either warp; those of the next block are on their way meanwhile.
+    constexpr int PER = (NT + 31) / 32;
+    uint32_t it0 = 0;
+    bool ok = true;
+    for (int i = begin; i < end && ok; i += step) {
+      const Item t = item_at(p, i);
+      const float* sa = p.a_scale + t.expert * p.as_expert + t.m * p.as_row;
+      const float* sx = p.x_scale + (long long)t.n0 * p.xs_row;
+      float next[PER], next_a = 0.0f;
+      auto fetch = [&](int b) {
+        next_a = sa[b * p.as_col];
+#pragma unroll
+        for (int k = 0; k < PER; ++k) next[k] = t.n0 + lane + 32 * k < t.n1 ? sx[(lane + 32 * k) * p.xs_row + b * p.xs_col] : 0.0f;
+      };
+      // (block b is iteration it0 + b - b0 of the CTA)
+      int b = b0 + (int)(((it0 & 1u) ^ (uint32_t)(warp - 2)) & 1u);
+      if (b < b1) fetch(b);
+      for (; b < b1; b += 2) {
+        const uint32_t it = it0 + (uint32_t)(b - b0), slot = it % kScaleSlots;
+        float now[PER];
+#pragma unroll
+        for (int k = 0; k < PER; ++k) now[k] = next[k] * next_a;
+        if (b + 2 < b1) fetch(b + 2);
+        ok = mbar_wait_warp(smem_u32(&bars.scale_empty[slot]), ((it / kScaleSlots) & 1u) ^ 1u, ctl);
+        if (!ok) break;
+#pragma unroll
+        for (int k = 0; k < PER; ++k)
+          if (lane + 32 * k < NT) scale_ring[slot][lane + 32 * k] = now[k];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bars.scale_full[slot]));
+      }
+      it0 += (uint32_t)(b1 - b0);
+    }
+  } else {
+    const int quad = warp & 3, side = (warp - kFirstAdder) >> 2;
+    uint32_t it = 0;
+    bool ok = true;
+    for (int i = begin; i < end && ok; i += step) {
+      const Item t = item_at(p, i);
+      const int n = t.n1 - t.n0, m = t.m * kBlock + quad * 32 + lane;
+      f32x2 sum[GROUPS][CG / 2];
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+        for (int c = 0; c < CG / 2; ++c) sum[g][c] = pair(0.0f, 0.0f);
+      for (int b = b0; b < b1; ++b, ++it) {
+        const uint32_t slot = it & 1u, ring_slot = it % kScaleSlots;
+        ok = mbar_wait_warp(smem_u32(&bars.scale_full[ring_slot]), (it / kScaleSlots) & 1u, ctl) &&
+             mbar_wait_warp(smem_u32(&bars.acc_full[slot]), (it >> 1) & 1u, ctl);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t from = tmem + slot * NT + ((uint32_t)(quad * 32) << 16);
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+          const int c0 = (2 * g + side) * CG;
+          if (c0 < n) {
+            uint32_t r[CG];
+            if constexpr (CG == 32) tmem_ld_32x32(from + (uint32_t)c0, r);
+            else tmem_ld_32x16p(from + (uint32_t)c0, r);
+            tmem_ld_wait();
+            const float4* s4 = reinterpret_cast<const float4*>(&scale_ring[ring_slot][c0]);
+#pragma unroll
+            for (int c = 0; c < CG / 4; ++c) {
+              const float4 s = s4[c];
+              sum[g][2 * c] = fma2(pair(__uint_as_float(r[4 * c]), __uint_as_float(r[4 * c + 1])), pair(s.x, s.y), sum[g][2 * c]);
+              sum[g][2 * c + 1] = fma2(pair(__uint_as_float(r[4 * c + 2]), __uint_as_float(r[4 * c + 3])), pair(s.z, s.w), sum[g][2 * c + 1]);
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(smem_u32(&bars.acc_empty[slot]));
+          mbar_arrive(smem_u32(&bars.scale_empty[ring_slot]));
+        }
+      }
+      if (!ok) break;
+      if (p.splits > 1) {
+        float* part = reinterpret_cast<float*>(raw + (ring - smem_u32(raw)));   // [tokens][128]
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+          const int c0 = (2 * g + side) * CG;
+#pragma unroll
+          for (int c = 0; c < CG / 2; ++c) {
+            float a, d;
+            unpair(sum[g][c], a, d);
+            if (c0 + 2 * c < n) part[(c0 + 2 * c) * kBlock + quad * 32 + lane] = a;
+            if (c0 + 2 * c + 1 < n) part[(c0 + 2 * c + 1) * kBlock + quad * 32 + lane] = d;
+          }
+        }
+        break;   // (one item per cluster)
+      }
+      if (m < p.M) {
+        const Finish f(p, t, m);
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+          const int c0 = (2 * g + side) * CG;
+          if (c0 < n) {
+            f32x2 y[CG / 2];
+#pragma unroll
+            for (int c = 0; c < CG / 2; ++c) y[c] = add2(sum[g][c], pair(f.bias, f.bias));
+            activate<CG / 2>(y, p.act);
+            const long long token = t.n0 + c0;
+#pragma unroll
+            for (int h = 0; h < CG; h += 8) {   // eight residuals on their way together
+              float r[8];
+#pragma unroll
+              for (int c = 0; c < 8; ++c)
+                r[c] = p.residual != nullptr && c0 + h + c < n ? element(p.residual, p.residual_elem, (token + h + c) * p.ldr + m) : 0.0f;
+#pragma unroll
+              for (int c = 0; c < 8; c += 2) {
+                float a, d;
+                unpair(y[(h + c) / 2], a, d);
+                if (p.residual != nullptr) { a += r[c]; d += r[c + 1]; }
+                if (c0 + h + c < n) store_result(p, token + h + c, m, a);
+                if (c0 + h + c + 1 < n) store_result(p, token + h + c + 1, m, d);
+              }
+            }
+          }
+        }
+      }
+      __syncwarp();
+    }
+  }
+  if (p.splits > 1) {
+    __syncwarp();
+    cluster_meet();
+    if (begin < end && warp >= kFirstAdder) {
+      const Item t = item_at(p, begin);
+      const int n = t.n1 - t.n0, quad = warp & 3, side = (warp - kFirstAdder) >> 2, m = t.m * kBlock + quad * 32 + lane;
+      const Finish f(p, t, m);
+      const int share = (n + p.splits - 1) / p.splits, c1 = min(n, (rank + 1) * share);
+      for (int c = rank * share + side; c < c1; c += 2) {
+        float v = 0.0f;
+        for (int q = 0; q < p.splits; ++q) v += ld_cluster(cluster_address(ring + (uint32_t)(c * kBlock + quad * 32 + lane) * 4u, (uint32_t)q));
+        if (m < p.M) {
+          v = activate(v + f.bias, p.act);
+          if (p.residual != nullptr) v += element(p.residual, p.residual_elem, (long long)(t.n0 + c) * p.ldr + m);
+          store_result(p, t.n0 + c, m, v);
+        }
+      }
+    }
+    __syncwarp();
+    cluster_meet();   // (nobody leaves while others read its sums)
+  }
+  if (p.head != nullptr && p.zero_rest) {   // tokens in no run
+    const int low = p.bounds[0], high = p.bounds[p.n_experts];
+    for (int r = (int)blockIdx.x; r < low + p.N - high; r += (int)gridDim.x) {
+      const long long token = r < low ? r : high + r - low;
+      for (int m = tid; m < p.M; m += kThreads) store_result(p, token, m, 0.0f);
+    }
+  }
+  grid_launch_dependents();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (ctl_s[0]) {   // let copies that may still be in flight land before shared memory is given back
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 200000ull) {
+    }
+    if (tid == 0 && p.status != nullptr) atomicCAS(p.status, 0, kStatusTimeout);
+    __syncthreads();
+  }
+  if (warp == 1) tmem_dealloc(tmem, kTmem);
+}
+
+bool rows_map(CUtensorMap* m, const void* at, long long ld, long long expert, int K, int rows, int experts, int box_rows) {
+  PFN_cuTensorMapEncodeTiled_v12000 enc = get_encode();
+  if (enc == nullptr) return false;
+  const cuuint64_t gdim[3] = {(cuuint64_t)K, (cuuint64_t)rows, (cuuint64_t)experts};
+  const cuuint64_t gstride[2] = {(cuuint64_t)ld, (cuuint64_t)expert};
+  const cuuint32_t box[3] = {(cuuint32_t)kBlock, (cuuint32_t)box_rows, 1};
+  const cuuint32_t estride[3] = {1, 1, 1};
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, experts > 0 ? 3 : 2, const_cast<void*>(at), gdim, gstride, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int NT, int CTAS>
+int launch_fp8(Fp8Params p, const CUtensorMap& a, const CUtensorMap& x, long long items, const DeviceInfo& dev, cudaStream_t st) {
+  constexpr int kStage = kBlock * kBlock + NT * kBlock;
+  const int fixed = (int)sizeof(Fp8Bars) + kScaleSlots * NT * 4 + 64 + 1024 + 1024;   // (and what the system keeps of a CTA's)
+  p.stages = (dev.smem_per_sm / CTAS - fixed) / kStage;
+  if (p.stages > kMaxRing) p.stages = kMaxRing;
+  const int most = (dev.max_smem - fixed) / kStage;
+  if (p.stages > most) p.stages = most;
+  const int smem = p.stages * kStage + 1024;
+  if (p.stages < 2) return VOID_ERR_SHAPE;
+  const void* kernel = reinterpret_cast<const void*>(fp8_block_kernel<NT, CTAS>);
+  if (ensure_smem(kernel, smem) != 0) return VOID_ERR_CUDA;
+  const long long slots = (long long)dev.sms * CTAS;
+  // Fewer items than half the places for CTAs: the blocks of k are shared, as long as every CTA has two of them and the sums fit the ring.
+  int splits = 1;
+  while (splits < 8 && items * splits * 2 <= slots && p.k_blocks >= splits * 4 && NT * kBlock * 4 <= p.stages * kStage) splits *= 2;
+  p.splits = splits;
+  const long long grid = splits > 1 ? items * splits : (items < slots ? items : slots);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)splits;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = splits > 1 ? 2 : 1;
+  return status_of(cudaLaunchKernelEx(&cfg, fp8_block_kernel<NT, CTAS>, p, a, x));
+}
+
+int fp8_linear(const void_fp8_args* a, const void_experts* x, cudaStream_t st) {
+  if (a == nullptr || a->M < 0 || a->K < 0 || a->N < 0) return VOID_ERR_BAD_ARG;
+  if (a->out_elem < VOID_ELEM_F32 || a->out_elem > VOID_ELEM_BF16 || a->bias_elem < VOID_ELEM_F32 || a->bias_elem > VOID_ELEM_BF16 ||
+      a->residual_elem < VOID_ELEM_F32 || a->residual_elem > VOID_ELEM_BF16 || a->act < VOID_ACT_NONE || a->act > VOID_ACT_SILU)
+    return VOID_ERR_BAD_ARG;
+  if (a->M == 0 || a->N == 0) return VOID_OK;
+  if (a->out == nullptr || a->K == 0 || a->a == nullptr || a->x == nullptr || a->a_scale == nullptr || a->x_scale == nullptr) return VOID_ERR_BAD_ARG;
+  if (x != nullptr && (x->n_experts < 1 || x->plan == nullptr || x->offset_bytes != 0 || (x->chunk != 32 && x->chunk != 64 && x->chunk != 128 && x->chunk != 256)))
+    return VOID_ERR_BAD_ARG;
+  if (a->ldc < a->M || (a->residual != nullptr && a->ldr < a->M)) return VOID_ERR_SHAPE;
+  if ((reinterpret_cast<uintptr_t>(a->a) & 15u) != 0 || (reinterpret_cast<uintptr_t>(a->x) & 15u) != 0 || (a->lda & 15) != 0 || (a->ldx & 15) != 0 ||
+      a->lda < a->K || a->ldx < a->K || (x != nullptr && ((a->expert_stride & 15) != 0 || a->expert_stride < 0 || (reinterpret_cast<uintptr_t>(x->plan) & 15u) != 0)))
+    return VOID_ERR_ALIGN;
+  const DeviceInfo dev = device_info();
+  if (!dev.ok) return VOID_ERR_CUDA;
+  if (dev.cc_major != 10) return VOID_ERR_ARCH;
+  Fp8Params p = {};
+  p.M = a->M; p.K = a->K; p.N = a->N;
+  p.k_blocks = (a->K + kBlock - 1) / kBlock;
+  p.m_tiles = (a->M + kBlock - 1) / kBlock;
+  p.a_scale = a->a_scale; p.as_row = a->a_scale_row; p.as_col = a->a_scale_col; p.as_expert = a->a_scale_expert;
+  p.x_scale = a->x_scale; p.xs_row = a->x_scale_row; p.xs_col = a->x_scale_col;
+  p.bias = a->bias; p.bias_elem = a->bias_elem;
+  p.residual = a->residual; p.ldr = a->ldr; p.residual_elem = a->residual_elem;
+  p.out = a->out; p.ldc = a->ldc; p.out_elem = a->out_elem; p.act = a->act;
+  p.status = a->status;
+  p.wait_limit_ms = (a->test_hooks & 0xffff) ? (a->test_hooks & 0xffff) : kDefaultWaitLimitMs;
+  p.drop_first = (a->test_hooks >> 16) & 1;
+  long long chunks;
+  int most;   // tokens of an item
+  if (x != nullptr) {
+    const PlanView v = plan_of(*x, a->N);
+    p.head = v.head; p.bounds = v.bounds; p.chunks = v.chunks;
+    p.n_experts = x->n_experts;
+    p.zero_rest = x->zero_rest;
+    chunks = v.capacity;
+    most = x->chunk;
+  } else {
+    chunks = ((long long)a->N + 255) / 256;
+    p.chunk = (int)((a->N + chunks - 1) / chunks + 15) / 16 * 16;
+    p.n_chunks = (int)((a->N + p.chunk - 1) / p.chunk);
+    p.group = 8;
+    chunks = p.n_chunks;
+    most = p.chunk;
+  }
+  const long long items = chunks * p.m_tiles;
+  if (items > 0x3fffffff) return VOID_ERR_TOO_LARGE;
+  CUtensorMap map_a, map_x;
+  const int experts = x != nullptr ? x->n_experts : 1;
+  if (!rows_map(&map_a, a->a, a->lda, x != nullptr ? a->expert_stride : (a->lda * a->M + 15) / 16 * 16, a->K, a->M, experts, kBlock) ||
+      !rows_map(&map_x, a->x, a->ldx, 0, a->K, a->N, 0, kTokenBox))
+    return VOID_ERR_TENSOR_MAP;
+  if (most <= 32) return launch_fp8<32, 2>(p, map_a, map_x, items, dev, st);
+  if (most <= 64) return launch_fp8<64, 2>(p, map_a, map_x, items, dev, st);
+  if (most <= 128) return launch_fp8<128, 1>(p, map_a, map_x, items, dev, st);
+  return launch_fp8<256, 1>(p, map_a, map_x, items, dev, st);
+}
+
+}  // namespace
+
+}  // namespace vb
+
+extern "C" {
+
+int void_quant_fp8_blocks(const void* x, int32_t elem, int64_t ldx, int64_t rows, int32_t cols, int32_t block_rows, void* q, int64_t ldq, float* scales,
+                          int64_t scale_row, int64_t scale_col, void_stream_t stream) {
+  using namespace vb;
+  if (rows < 0 || cols < 0 || elem < VOID_ELEM_F32 || elem > VOID_ELEM_BF16 || (block_rows != 1 && block_rows != kBlock)) return VOID_ERR_BAD_ARG;
+  if (rows > 1 && (ldx < cols || ldq < cols)) return VOID_ERR_SHAPE;
+  if (rows == 0 || cols == 0) return VOID_OK;
+  if (x == nullptr || q == nullptr || scales == nullptr) return VOID_ERR_BAD_ARG;
+  const DeviceInfo dev = device_info();
+  if (!dev.ok) return VOID_ERR_CUDA;
+  if (dev.cc_major != 10) return VOID_ERR_ARCH;
+  QuantParams p = {};
+  p.x = x; p.ldx = ldx; p.ldq = ldq; p.scale_row = scale_row; p.scale_col = scale_col; p.rows = rows; p.cols = cols;
+  p.q = reinterpret_cast<uint8_t*>(q); p.scales = scales;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (elem == VOID_ELEM_F32) return quant_of_type<float>(p, block_rows, dev.sms, st);
+  return elem == VOID_ELEM_F16 ? quant_of_type<__half>(p, block_rows, dev.sms, st) : quant_of_type<__nv_bfloat16>(p, block_rows, dev.sms, st);
+}
+
+int void_fp8_linear(const void_fp8_args* args, const void_experts* experts, void_stream_t stream) {
+  return vb::fp8_linear(args, experts, reinterpret_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -1528,7 +1528,7 @@ int32_t expert_chunk(int64_t rows, int64_t experts) {
 }
 // own: whether the product makes the plan itself where it can (up to 32 experts): nothing else reads it.  A launch less: 8 experts of
 // 2048 -> 8192, fp16, 80 %, 1 token 7.6 -> 6.5 us, 8 tokens 15.7 -> 14.6, 32 tokens 19.9 -> 18.8, 512 tokens 27.7 -> 24.6.
-ExpertPlan expert_plan(const at::Tensor& offsets_in, int64_t rows, int64_t experts, c10::Device dev, int32_t* status, bool own = false) {
+ExpertPlan expert_plan(const at::Tensor& offsets_in, int64_t rows, int64_t experts, c10::Device dev, int32_t* status, bool own = false, int32_t chunk = 0) {
   if (offsets_in.dim() != 1 || offsets_in.size(0) != experts + 1)
     fail("offsets must be a vector of " + std::to_string(experts + 1) + " integers, one more than there are experts");
   if (offsets_in.device() != dev) fail("tokens and offsets are on different devices");
@@ -1537,7 +1537,7 @@ ExpertPlan expert_plan(const at::Tensor& offsets_in, int64_t rows, int64_t exper
   const at::Tensor offsets = offsets_in.contiguous();
   ExpertPlan plan;
   plan.x.n_experts = (int32_t)experts;
-  plan.x.chunk = expert_chunk(rows, experts);
+  plan.x.chunk = chunk > 0 ? chunk : expert_chunk(rows, experts);
   if (own && experts <= 32 && rows > 0) {
     plan.words = offsets;
     plan.x.plan = static_cast<const int32_t*>(offsets.const_data_ptr());
@@ -1922,6 +1922,478 @@ PyObject* layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   NATIVE_END
 }
 
+// ------------------------------------------------------------------------------------------ tokens to experts and back
+bool floating(at::ScalarType t) { return t == at::kFloat || t == at::kHalf || t == at::kBFloat16; }
+void no_tangents(std::initializer_list<const at::Tensor*> operands, const char* what) {
+  for (const at::Tensor* t : operands)
+    TORCH_CHECK_NOT_IMPLEMENTED(!torch::autograd::isFwGradDefined(*t), what, " has no forward-mode derivative: an operand carries a tangent");
+}
+// A result [rows, cols] that was given, row-major.
+at::Tensor given_rows(PyObject* o, int64_t rows, int64_t cols, at::ScalarType type, c10::Device dev, bool recorded) {
+  const at::Tensor& out = cuda_tensor(o, "out");
+  if (recorded || (at::GradMode::is_enabled() && out.requires_grad())) fail("out= cannot be differentiated through");
+  if (out.dim() != 2 || out.size(0) != rows || out.size(1) != cols || out.scalar_type() != type || (cols > 1 && out.stride(1) != 1) ||
+      (rows > 1 && out.stride(0) < cols))
+    fail("out must be a row-major [" + std::to_string(rows) + ", " + std::to_string(cols) + "] tensor of type " + c10::toString(type));
+  if (out.device() != dev) fail("out and its operands are on different devices");
+  return out;
+}
+struct RouteBackward : torch::autograd::Node {
+  torch::autograd::SavedVariable scores;
+  int32_t top = 0, normalize = 0;
+
+  std::string name() const override { return "VOIDRouteBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    scores.reset_data();
+  }
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    torch::autograd::variable_list out(1);
+    if (!grads[0].defined()) return out;
+    no_second_derivative("the router");
+    const at::Tensor s = scores.unpack();
+    c10::cuda::OptionalCUDAGuard guard(s.device());
+    no_eager_leaf(*this);
+    at::AutoDispatchBelowADInplaceOrView below;
+    const at::Tensor rows = token_rows(s), g = token_rows(as_type(grads[0], at::kFloat));
+    const at::Tensor ds = new_cuda(s.sizes(), s.scalar_type(), s.device());
+    const int status = void_route_grad(rows.const_data_ptr(), out_code(s.scalar_type()), row_step(rows), rows.size(0), (int32_t)rows.size(1), top, normalize,
+                                       g.const_data_ptr<float>(), row_step(g), ds.data_ptr(), s.size(1), stream_of(s.device().index()));
+    TORCH_CHECK(status == VOID_OK, "void_b200 void_route_grad failed: ", void_strerror(status), " (status ", status, ")");
+    out[0] = ds;
+    return out;
+  }
+};
+// route(scores [N, E], top_k, normalize) -> (experts int32 [N, top_k], weights fp32 [N, top_k]); differentiable in the scores
+PyObject* route(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NATIVE_BEGIN
+  if (n != 3) throw torch::TypeError("route takes 3 arguments");
+  const at::Tensor& scores = cuda_tensor(a[0], "scores");
+  const int64_t top = integer(a[1]);
+  const int32_t normalize = PyObject_IsTrue(a[2]) == 1 ? 1 : 0;
+  if (!floating(scores.scalar_type())) fail(std::string("scores must be float32, float16 or bfloat16, got ") + c10::toString(scores.scalar_type()));
+  if (scores.dim() != 2) fail("scores must be a [tokens, experts] matrix");
+  const int64_t N = scores.size(0), E = scores.size(1);
+  if (E < 1 || E > 1024) fail("the router takes 1 to 1024 experts, got " + std::to_string(E));
+  if (top < 1 || top > E || top > 32) fail("top_k must lie in 1 .. " + std::to_string(std::min<int64_t>(E, 32)) + ", got " + std::to_string(top));
+  no_tangents({&scores}, "the router");
+  const bool recorded = torch::autograd::compute_requires_grad(scores);
+  const c10::Device dev = scores.device();
+  c10::cuda::OptionalCUDAGuard guard;
+  if (c10::cuda::current_device() != dev.index()) guard.set_device(dev);
+  at::Tensor chosen, weights;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const at::Tensor rows = token_rows(scores);
+    chosen = new_cuda({N, top}, at::kInt, dev);
+    weights = new_cuda({N, top}, at::kFloat, dev);
+    check(void_route(rows.const_data_ptr(), out_code(rows.scalar_type()), row_step(rows), N, (int32_t)E, (int32_t)top, normalize, chosen.data_ptr<int32_t>(),
+                     weights.data_ptr<float>(), stream_of(dev.index())),
+          "void_route");
+  }
+  if (recorded) {
+    auto node = std::shared_ptr<RouteBackward>(new RouteBackward(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(scores));
+    node->scores = torch::autograd::SavedVariable(scores, false);
+    node->top = (int32_t)top;
+    node->normalize = normalize;
+    torch::autograd::set_history(weights, node);
+  }
+  return Py_BuildValue("NN", THPVariable_Wrap(chosen), THPVariable_Wrap(weights));
+  NATIVE_END
+}
+
+// What a sort by expert works on.
+struct Choices {
+  at::Tensor experts, offsets, position, ws;
+  int64_t tokens = 0, top = 0, n_experts = 0;
+  int32_t index_bytes() const { return (int32_t)experts.element_size(); }
+};
+Choices choices(PyObject* experts, PyObject* n_experts) {
+  Choices c;
+  const at::Tensor& e = cuda_tensor(experts, "experts");
+  c.n_experts = integer(n_experts);
+  if (e.scalar_type() != at::kInt && e.scalar_type() != at::kLong) fail(std::string("experts must be int32 or int64, got ") + c10::toString(e.scalar_type()));
+  if (e.dim() != 2 || e.size(1) < 1) fail("experts must be a [tokens, top_k] matrix");
+  if (c.n_experts < 1 || c.n_experts > 1024) fail("tokens are sorted by 1 to 1024 experts, got " + std::to_string(c.n_experts));
+  c.tokens = e.size(0);
+  c.top = e.size(1);
+  if (c.tokens > 0x7fffffff / c.top) fail("tokens are sorted for at most 2^31 - 1 choices");
+  c.experts = e.contiguous();
+  return c;
+}
+void room_for(Choices& c) {
+  const c10::Device dev = c.experts.device();
+  c.offsets = new_cuda({c.n_experts + 1}, at::kInt, dev);
+  c.position = new_cuda({c.tokens, c.top}, at::kInt, dev);
+  const size_t bytes = void_sort_by_expert_ws_bytes(c.tokens * c.top, (int32_t)c.n_experts);
+  if (bytes > 0) c.ws = new_cuda({(int64_t)bytes}, at::kByte, dev);
+}
+// sort_by_expert(experts [N, top_k], n_experts) -> (offsets int32 [n_experts + 1], position int32 [N, top_k])
+PyObject* sort_by_expert(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NATIVE_BEGIN
+  if (n != 2) throw torch::TypeError("sort_by_expert takes 2 arguments");
+  c10::cuda::OptionalCUDAGuard guard(cuda_tensor(a[0], "experts").device());
+  Choices c = choices(a[0], a[1]);
+  room_for(c);
+  check(void_sort_by_expert(c.experts.const_data_ptr(), c.index_bytes(), c.tokens * c.top, (int32_t)c.n_experts, c.offsets.data_ptr<int32_t>(),
+                            c.position.data_ptr<int32_t>(), c.ws.defined() ? c.ws.data_ptr() : nullptr, c.ws.defined() ? (size_t)c.ws.numel() : 0,
+                            stream_of(c.experts.device().index())),
+        "void_sort_by_expert");
+  return Py_BuildValue("NN", THPVariable_Wrap(c.offsets), THPVariable_Wrap(c.position));
+  NATIVE_END
+}
+
+struct DispatchBackward : torch::autograd::Node {
+  torch::autograd::SavedVariable position;
+  int64_t cols = 0;
+  at::ScalarType type = at::kFloat;
+
+  std::string name() const override { return "VOIDDispatchBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    position.reset_data();
+  }
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    torch::autograd::variable_list out(1);
+    if (!grads[0].defined()) return out;
+    no_second_derivative("the dispatch of tokens");
+    const at::Tensor at = position.unpack();
+    c10::cuda::OptionalCUDAGuard guard(at.device());
+    no_eager_leaf(*this);
+    at::AutoDispatchBelowADInplaceOrView below;
+    const at::Tensor g = token_rows(as_type(grads[0], type));
+    const at::Tensor dx = new_cuda({at.size(0), cols}, type, at.device());
+    const int status = void_combine(g.const_data_ptr(), out_code(type), row_step(g), at.size(0), (int32_t)cols, (int32_t)at.size(1),
+                                    at.const_data_ptr<int32_t>(), nullptr, VOID_ELEM_F32, nullptr, 0, out_code(type), dx.data_ptr(), cols,
+                                    stream_of(at.device().index()));
+    TORCH_CHECK(status == VOID_OK, "void_b200 void_combine failed: ", void_strerror(status), " (status ", status, ")");
+    out[0] = dx;
+    return out;
+  }
+};
+// dispatch(x [N, D], experts [N, top_k], n_experts, out | None) -> (rows [N * top_k, D], offsets, position); differentiable in x
+PyObject* dispatch(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NATIVE_BEGIN
+  if (n != 4) throw torch::TypeError("dispatch takes 4 arguments");
+  const at::Tensor& x = cuda_tensor(a[0], "x");
+  const c10::Device dev = x.device();
+  if (!floating(x.scalar_type())) fail(std::string("x must be float32, float16 or bfloat16, got ") + c10::toString(x.scalar_type()));
+  if (x.dim() != 2) fail("x must be a [tokens, features] matrix");
+  if (x.size(1) > 0x7fffffff) fail("tokens have at most 2^31 - 1 features");
+  no_tangents({&x}, "the dispatch of tokens");
+  const bool recorded = torch::autograd::compute_requires_grad(x);
+  c10::cuda::OptionalCUDAGuard guard;
+  if (c10::cuda::current_device() != dev.index()) guard.set_device(dev);
+  Choices c = choices(a[1], a[2]);
+  if (c.experts.device() != dev) fail("x and experts are on different devices");
+  if (c.tokens != x.size(0)) fail("experts must have a row for each of the " + std::to_string(x.size(0)) + " tokens, got " + std::to_string(c.tokens));
+  const int64_t cols = x.size(1), count = c.tokens * c.top;
+  at::Tensor rows;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    at::Tensor tokens = token_rows(x);
+    if (none(a[3])) {
+      rows = new_cuda({count, cols}, x.scalar_type(), dev);
+    } else {
+      rows = given_rows(a[3], count, cols, x.scalar_type(), dev, recorded);
+      if (meet(tokens, rows)) tokens = tokens.clone(at::MemoryFormat::Contiguous);
+      if (meet(c.experts, rows)) c.experts = c.experts.clone();
+      mark_written(rows);
+    }
+    room_for(c);
+    check(void_dispatch(tokens.const_data_ptr(), out_code(x.scalar_type()), row_step(tokens), c.tokens, (int32_t)cols, c.experts.const_data_ptr(), c.index_bytes(),
+                        (int32_t)c.top, (int32_t)c.n_experts, c.offsets.data_ptr<int32_t>(), c.position.data_ptr<int32_t>(), rows.data_ptr(), row_step(rows),
+                        none(a[3]) ? 1 : 0, c.ws.defined() ? c.ws.data_ptr() : nullptr, c.ws.defined() ? (size_t)c.ws.numel() : 0, stream_of(dev.index())),
+          "void_dispatch");
+  }
+  if (recorded) {
+    auto node = std::shared_ptr<DispatchBackward>(new DispatchBackward(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(x));
+    node->position = torch::autograd::SavedVariable(c.position, false);
+    node->cols = cols;
+    node->type = x.scalar_type();
+    torch::autograd::set_history(rows, node);
+  }
+  PyObject* result = a[3];
+  if (none(result)) result = THPVariable_Wrap(rows);
+  else Py_INCREF(result);
+  return Py_BuildValue("NNN", result, THPVariable_Wrap(c.offsets), THPVariable_Wrap(c.position));
+  NATIVE_END
+}
+
+struct CombineBackward : torch::autograd::Node {
+  torch::autograd::SavedVariable rows, weights, position, offsets;
+  int64_t cols = 0;
+  at::ScalarType type = at::kFloat;
+  bool weighted = false;
+
+  std::string name() const override { return "VOIDCombineBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    rows.reset_data();
+    weights.reset_data();
+    position.reset_data();
+    offsets.reset_data();
+  }
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    torch::autograd::variable_list out(3);
+    if (!grads[0].defined()) return out;
+    no_second_derivative("the combination of experts' rows");
+    const at::Tensor ys = rows.unpack(), given = weights.unpack(), at = position.unpack(), ends = offsets.unpack();
+    c10::cuda::OptionalCUDAGuard guard(at.device());
+    no_eager_leaf(*this);
+    at::AutoDispatchBelowADInplaceOrView below;
+    const int64_t tokens = at.size(0), top = at.size(1);
+    const at::Tensor g = token_rows(as_type(grads[0], type)), w = weighted ? given.contiguous() : given;
+    at::Tensor y;
+    if (task_should_compute_output(0)) out[0] = new_cuda({tokens * top, cols}, type, at.device());
+    if (weighted && task_should_compute_output(1)) {
+      out[1] = new_cuda({tokens, top}, w.scalar_type(), at.device());
+      y = token_rows(ys);
+    }
+    if (task_should_compute_output(2)) out[2] = grads[0];
+    const int status = void_combine_grad(
+        g.const_data_ptr(), row_step(g), y.defined() ? y.const_data_ptr() : nullptr, y.defined() ? row_step(y) : cols, out_code(type), tokens, (int32_t)cols,
+        (int32_t)top, at.const_data_ptr<int32_t>(), ends.const_data_ptr<int32_t>() + ends.size(0) - 1, weighted ? w.const_data_ptr() : nullptr,
+        weighted ? out_code(w.scalar_type()) : VOID_ELEM_F32, out[0].defined() ? out[0].data_ptr() : nullptr, cols,
+        out[1].defined() ? out[1].data_ptr() : nullptr, stream_of(at.device().index()));
+    TORCH_CHECK(status == VOID_OK, "void_b200 void_combine_grad failed: ", void_strerror(status), " (status ", status, ")");
+    return out;
+  }
+};
+// combine(rows [N * top_k, D], position [N, top_k], offsets, weights [N, top_k] | None, residual [N, D] | None, out | None) -> [N, D];
+// differentiable in rows, weights and residual
+PyObject* combine(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NATIVE_BEGIN
+  if (n != 6) throw torch::TypeError("combine takes 6 arguments");
+  const at::Tensor& ys = cuda_tensor(a[0], "rows");
+  const at::Tensor &position = cuda_tensor(a[1], "position"), &offsets = cuda_tensor(a[2], "offsets");
+  const at::Tensor absent;
+  const at::Tensor &weights = none(a[3]) ? absent : cuda_tensor(a[3], "weights"), &residual = none(a[4]) ? absent : cuda_tensor(a[4], "residual");
+  const c10::Device dev = ys.device();
+  const at::ScalarType type = ys.scalar_type();
+  if (!floating(type)) fail(std::string("the experts' rows must be float32, float16 or bfloat16, got ") + c10::toString(type));
+  if (position.dim() != 2 || position.scalar_type() != at::kInt || !position.is_contiguous() || offsets.dim() != 1 || offsets.scalar_type() != at::kInt ||
+      !offsets.is_contiguous() || offsets.size(0) < 1)
+    fail("routes must be those of sort_by_expert or void_dispatch");
+  const int64_t tokens = position.size(0), top = position.size(1);
+  if (ys.dim() != 2 || ys.size(0) != tokens * top)
+    fail("the experts' rows must be a matrix with a row for each of the " + std::to_string(tokens) + " x " + std::to_string(top) + " choices");
+  const int64_t cols = ys.size(1);
+  if (cols > 0x7fffffff) fail("tokens have at most 2^31 - 1 features");
+  if (weights.defined()) {
+    if (weights.dim() != 2 || weights.size(0) != tokens || weights.size(1) != top)
+      fail("weights must be a [" + std::to_string(tokens) + ", " + std::to_string(top) + "] tensor");
+    if (!floating(weights.scalar_type())) fail(std::string("weights must be float32, float16 or bfloat16, got ") + c10::toString(weights.scalar_type()));
+  }
+  if (residual.defined()) {
+    if (residual.dim() != 2 || residual.size(0) != tokens || residual.size(1) != cols)
+      fail("residual must be a [" + std::to_string(tokens) + ", " + std::to_string(cols) + "] tensor");
+    if (!floating(residual.scalar_type())) fail(std::string("residual must be float32, float16 or bfloat16, got ") + c10::toString(residual.scalar_type()));
+  }
+  for (const at::Tensor* t : {&position, &offsets, &weights, &residual})
+    if (t->defined() && t->device() != dev) fail("the experts' rows and what goes with them are on different devices");
+  no_tangents({&ys, &weights, &residual}, "the combination of experts' rows");
+  const bool recorded = torch::autograd::compute_requires_grad(ys, weights, residual);
+  c10::cuda::OptionalCUDAGuard guard;
+  if (c10::cuda::current_device() != dev.index()) guard.set_device(dev);
+  at::Tensor y;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    at::Tensor rows = token_rows(ys), w = weights.defined() ? weights.contiguous() : weights, r = residual, at = position;
+    if (r.defined()) r = token_rows(r.scalar_type() == type || r.scalar_type() == at::kFloat ? r : r.to(at::kFloat));
+    if (none(a[5])) {
+      y = new_cuda({tokens, cols}, type, dev);
+    } else {
+      y = given_rows(a[5], tokens, cols, type, dev, recorded);
+      // what shares memory with the result is read from a copy, unless it is a residual in the very same place
+      if (meet(rows, y)) rows = rows.clone(at::MemoryFormat::Contiguous);
+      if (w.defined() && meet(w, y)) w = w.clone();
+      if (meet(at, y)) at = at.clone();
+      if (r.defined() && meet(r, y) && !(r.const_data_ptr() == y.const_data_ptr() && r.scalar_type() == type && row_step(r) == row_step(y)))
+        r = r.clone(at::MemoryFormat::Contiguous);
+      mark_written(y);
+    }
+    check(void_combine(rows.const_data_ptr(), out_code(type), row_step(rows), tokens, (int32_t)cols, (int32_t)top, at.const_data_ptr<int32_t>(),
+                       w.defined() ? w.const_data_ptr() : nullptr, w.defined() ? out_code(w.scalar_type()) : VOID_ELEM_F32,
+                       r.defined() ? r.const_data_ptr() : nullptr, r.defined() ? row_step(r) : cols, r.defined() ? out_code(r.scalar_type()) : VOID_ELEM_F32,
+                       y.data_ptr(), row_step(y), stream_of(dev.index())),
+          "void_combine");
+  }
+  if (!none(a[5])) {
+    Py_INCREF(a[5]);
+    return a[5];
+  }
+  if (recorded) {
+    auto node = std::shared_ptr<CombineBackward>(new CombineBackward(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(ys, weights, residual));
+    if (weights.defined() && weights.requires_grad()) node->rows = torch::autograd::SavedVariable(ys, false);   // (read for the weights' gradient only)
+    if (weights.defined()) node->weights = torch::autograd::SavedVariable(weights, false);
+    node->position = torch::autograd::SavedVariable(position, false);
+    node->offsets = torch::autograd::SavedVariable(offsets, false);
+    node->cols = cols;
+    node->type = type;
+    node->weighted = weights.defined();
+    torch::autograd::set_history(y, node);
+  }
+  return THPVariable_Wrap(y);
+  NATIVE_END
+}
+
+// ------------------------------------------------------------------------------------------ 8-bit weights with scales of blocks
+// x [N, K] in e4m3 with a scale per row and 128 columns (block_rows 1), or per 128 x 128 (128): rows on 16 bytes; the scales of rows lie
+// token behind token, as the products read them.
+struct Quantised {
+  at::Tensor values, scales;
+};
+Quantised quantised(const at::Tensor& x_in, int64_t block_rows) {
+  const at::Tensor x = token_rows(x_in);
+  const c10::Device dev = x.device();
+  const int64_t rows = x.size(0), cols = x.size(1), across = (cols + 127) / 128, pitch = (cols + 15) / 16 * 16;
+  Quantised q;
+  q.values = new_cuda({rows, pitch}, at::kFloat8_e4m3fn, dev);
+  if (pitch != cols) q.values = q.values.narrow(1, 0, cols);
+  if (block_rows == 1) {
+    const int64_t padded = (rows + 3) / 4 * 4;
+    q.scales = new_cuda({across, padded}, at::kFloat, dev).t();
+    if (padded != rows) q.scales = q.scales.narrow(0, 0, rows);
+  } else {
+    q.scales = new_cuda({(rows + 127) / 128, across}, at::kFloat, dev);
+  }
+  check(void_quant_fp8_blocks(x.const_data_ptr(), out_code(x.scalar_type()), row_step(x), rows, (int32_t)cols, (int32_t)block_rows, q.values.data_ptr(),
+                              pitch, q.scales.data_ptr<float>(), q.scales.stride(0), q.scales.stride(1), stream_of(dev.index())),
+        "void_quant_fp8_blocks");
+  return q;
+}
+// quant_fp8_blocks(x [N, K], block_rows) -> (values, scales)
+PyObject* quant_fp8_blocks(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NATIVE_BEGIN
+  if (n != 2) throw torch::TypeError("quant_fp8_blocks takes 2 arguments");
+  const at::Tensor& x = cuda_tensor(a[0], "x");
+  if (x.dim() != 2) fail("a matrix is quantised in blocks, got " + std::to_string(x.dim()) + " dimensions");
+  if (!floating(x.scalar_type())) fail(std::string("blocks are quantised from float32, float16 or bfloat16, got ") + c10::toString(x.scalar_type()));
+  if (x.size(1) > 0x7ffffff0) fail("a matrix that is quantised has at most 2^31 - 16 columns");
+  c10::cuda::OptionalCUDAGuard guard(x.device());
+  at::AutoDispatchBelowADInplaceOrView below;
+  const Quantised q = quantised(x, integer(a[1]));
+  return Py_BuildValue("NN", THPVariable_Wrap(q.values), THPVariable_Wrap(q.scales));
+  NATIVE_END
+}
+
+// Tokens of a work item, by those an expert has on average.
+int32_t fp8_chunk(int64_t rows, int64_t experts) {
+  const int64_t each = (rows + experts - 1) / experts;
+  return each <= 24 ? 32 : (each <= 48 ? 64 : (each <= 96 ? 128 : 256));
+}
+// fp8_linear(values, scales, x, x_scales | None, offsets | None, bias | None, act, out | None, out_dtype, residual | None, status) -> out
+// values [M, K] or (with offsets) [experts, M, K] in e4m3; x [N, K] in e4m3 with x_scales, or floating: quantised first
+PyObject* fp8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NATIVE_BEGIN
+  if (n != 11) throw torch::TypeError("fp8_linear takes 11 arguments");
+  const at::Tensor &values_in = cuda_tensor(a[0], "values"), &scales = cuda_tensor(a[1], "scales"), &x_in = cuda_tensor(a[2], "x");
+  const c10::Device dev = x_in.device();
+  const bool runs = !none(a[4]);
+  const int64_t dims = runs ? 3 : 2;
+  if (values_in.dim() != dims || scales.dim() != dims) fail("weights and scales must have " + std::to_string(dims) + " dimensions here");
+  const int64_t E = runs ? values_in.size(0) : 1, M = values_in.size(dims - 2), K = values_in.size(dims - 1), N = x_in.size(0);
+  if (x_in.dim() != 2 || x_in.size(1) != K) fail("x must be a matrix of tokens with " + std::to_string(K) + " features");
+  if (values_in.device() != dev || scales.device() != dev) fail("the weights and x are on different devices");
+  if (M > 0x7fffff00 || K > 0x7fffff00 || N > 0x40000000) fail("the product is too large");
+  c10::cuda::OptionalCUDAGuard guard;
+  if (c10::cuda::current_device() != dev.index()) guard.set_device(dev);
+  at::AutoDispatchBelowADInplaceOrView below;
+  const at::ScalarType type = reinterpret_cast<THPDtype*>(a[8])->scalar_type;
+  out_code(type);
+  at::Tensor out;
+  if (none(a[7])) {
+    out = new_cuda({N, M}, type, dev);
+  } else {
+    out = given_rows(a[7], N, M, type, dev, false);
+    for (const at::Tensor* t : {&values_in, &scales})
+      if (meet(out, *t)) fail("out must have no memory in common with the weights");
+    if (runs && meet(out, tensor(a[4], "offsets"))) fail("out must have no memory in common with the offsets");
+    if (!none(a[5]) && meet(out, tensor(a[5], "bias"))) fail("out must have no memory in common with the bias");
+  }
+  at::Tensor values = values_in, x, x_scales;
+  auto lies = [](const at::Tensor& t) {   // rows on 16 bytes
+    const int64_t d = t.dim();
+    if ((reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15u) != 0 || (t.size(d - 1) > 1 && t.stride(d - 1) != 1)) return false;
+    for (int64_t i = 0; i + 1 < d; ++i)
+      if (t.size(i) > 1 && (t.stride(i) % 16 != 0 || t.stride(i) < t.size(d - 1))) return false;
+    return true;
+  };
+  auto laid_out = [&](const at::Tensor& t) {
+    if (lies(t)) return t;
+    c10::SmallVector<int64_t, 3> size(t.sizes().begin(), t.sizes().end());
+    size.back() = (size.back() + 15) / 16 * 16;
+    const at::Tensor copy = new_cuda(size, t.scalar_type(), dev).narrow(t.dim() - 1, 0, t.size(t.dim() - 1));
+    copy.copy_(t);
+    return copy;
+  };
+  values = laid_out(values);
+  if (none(a[3])) {
+    const Quantised q = quantised(x_in, 1);
+    x = q.values;
+    x_scales = q.scales;
+  } else {
+    x = laid_out(x_in);
+    x_scales = cuda_tensor(a[3], "x's scales");
+    if (x_scales.device() != dev) fail("x and its scales are on different devices");
+    if (meet(out, x)) x = laid_out(x.clone());
+    if (meet(out, x_scales)) x_scales = x_scales.clone();
+  }
+  void_fp8_args s = {};
+  auto pitch = [](const at::Tensor& t) {
+    const int64_t d = t.dim(), wide = (t.size(d - 1) + 15) / 16 * 16;
+    return t.size(d - 2) > 1 ? t.stride(d - 2) : wide;
+  };
+  s.a = values.const_data_ptr();
+  s.lda = pitch(values);
+  s.expert_stride = E > 1 ? values.stride(0) : (s.lda * M + 15) / 16 * 16;
+  s.a_scale = scales.const_data_ptr<float>();
+  s.a_scale_row = scales.stride(dims - 2);
+  s.a_scale_col = scales.stride(dims - 1);
+  s.a_scale_expert = runs ? scales.stride(0) : 0;
+  s.x = x.const_data_ptr();
+  s.ldx = pitch(x);
+  s.x_scale = x_scales.const_data_ptr<float>();
+  s.x_scale_row = x_scales.stride(0);
+  s.x_scale_col = x_scales.stride(1);
+  at::Tensor bias;
+  if (!none(a[5])) s.bias = bias_as_it_is(tensor(a[5], "bias"), dev, E * M, &s.bias_elem, bias, runs ? "the experts' bias" : "bias");
+  Tail tail;
+  if (!none(a[9])) {
+    set_residual(tail, cuda_tensor(a[9], "residual"), out);
+    s.residual = tail.e.residual;
+    s.ldr = tail.e.ldr;
+    s.residual_elem = tail.e.residual_dtype;
+  }
+  s.out = out.data_ptr();
+  s.ldc = N > 1 ? out.stride(0) : M;
+  s.M = (int32_t)M;
+  s.K = (int32_t)K;
+  s.N = (int32_t)N;
+  s.out_elem = out_code(type);
+  s.act = (int32_t)integer(a[6]);
+  if (s.act < VOID_ACT_NONE || s.act > VOID_ACT_SILU) fail("unknown activation code " + std::to_string(s.act));
+  s.status = cuda_tensor(a[10], "status").data_ptr<int32_t>();
+  ExpertPlan plan;
+  if (runs) {
+    plan = expert_plan(cuda_tensor(a[4], "offsets"), N, E, dev, s.status, false, fp8_chunk(N, E));
+    plan.x.zero_rest = none(a[7]) ? 1 : 0;
+  }
+  check(void_fp8_linear(&s, runs ? &plan.x : nullptr, stream_of(dev.index())), "void_fp8_linear");
+  if (none(a[7])) return THPVariable_Wrap(out);
+  mark_written(out);
+  Py_INCREF(a[7]);
+  return a[7];
+  NATIVE_END
+}
+
 PyObject* set_error(PyObject*, PyObject* cls) {
   Py_INCREF(cls);
   g_error = cls;
@@ -1957,6 +2429,12 @@ PyMethodDef kMethods[] = {
     FAST(layer_norm),
     FAST(expert_linear),
     FAST(expert_values_product),
+    FAST(route),
+    FAST(sort_by_expert),
+    FAST(dispatch),
+    FAST(combine),
+    FAST(quant_fp8_blocks),
+    FAST(fp8_linear),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

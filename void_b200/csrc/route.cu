@@ -1,0 +1,691 @@
+// Tokens on their way to the experts and back:
+//
+//   router     the k largest of a token's scores, and w = softmax of them (over the chosen ones, or over all)
+//              ds_i = p_i (g_i - sum_j g_j p_j)
+//   sort       row of every choice (token t, slot j) when all are sorted by expert, in the order of the tokens
+//   dispatch   xs[row(t, j)] = x[t]
+//   combine    y[t] = r[t] + sum_j w[t, j] ys[row(t, j)]
+//              dys[row(t, j)] = w[t, j] dy[t],  dw[t, j] = <dy[t], ys[row(t, j)]>; dispatch's gradient is combine without weights
+//
+// A choice of no expert (an id outside [0, experts)) is dropped: it has row -1, brings nothing into the sum, and leaves a row behind the last
+// run, which dispatch and combine's gradient fill with zeros.  All sums are fp32 and taken in the order of the slots; nothing depends on the
+// order in which blocks ran.
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/void_b200.h"
+#include "launch.cuh"
+#include "ptx.cuh"
+#include "values.cuh"
+
+namespace vb {
+
+namespace {
+
+constexpr unsigned kAll = 0xffffffffu;
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+  return v;
+}
+
+// ------------------------------------------------------------------------------------------ router
+// Numbers as unsigned ones of the same order: NaN above all, -0 the same as 0, 0 for what is taken or not there.
+__device__ __forceinline__ uint32_t order_key(float x) {
+  if (x != x) return 0xffffffffu;
+  const uint32_t b = __float_as_uint(x + 0.0f);
+  return (b >> 31) ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k); }
+constexpr uint32_t kKeyOfMinusInfinity = 0x007fffffu;
+
+struct RouteParams {
+  const void* scores;
+  long long lds, rows;
+  int experts, top, normalize;
+  int32_t* chosen;    // forward
+  float* weights;
+  const float* g;     // backward
+  long long ldg;
+  void* ds;
+  long long ldd;
+};
+constexpr int kRouteWarps = 4;
+
+// A warp per token, expert e in lane e % 32.  A slot takes two warp-wide reductions in hardware: the largest key, then the lowest index
+// that has it.  The backward pass chooses again, from the scores: what it keeps of the forward pass is nothing that a caller could change.
+// A few tokens are a launch and one trip to memory; 16384 tokens of 128 fp32 scores move 8 MB.
+template <typename T, int PER_LANE, bool GRAD>
+__global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const __grid_constant__ RouteParams p) {
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  for (long long t = (long long)blockIdx.x * kRouteWarps + (threadIdx.x >> 5); t < p.rows; t += (long long)gridDim.x * kRouteWarps) {
+    const T* row = reinterpret_cast<const T*>(p.scores) + t * p.lds;
+    float s[PER_LANE];
+    uint32_t key[PER_LANE];
+#pragma unroll
+    for (int v = 0; v < PER_LANE; ++v) {
+      const int e = lane + 32 * v;
+      s[v] = e < p.experts ? to_float<T>(row[e]) : -INFINITY;
+    }
+    float slot_grad = 0.0f;
+    if constexpr (GRAD) slot_grad = lane < p.top ? p.g[t * p.ldg + lane] : 0.0f;
+#pragma unroll
+    for (int v = 0; v < PER_LANE; ++v) key[v] = lane + 32 * v < p.experts ? order_key(s[v]) : 0u;
+    int taken = 0, id = -1;   // id, score: of the slot that is this lane's
+    float score = 0.0f, largest = 0.0f;
+    for (int j = 0; j < p.top; ++j) {
+      uint32_t best = 0;
+#pragma unroll
+      for (int v = 0; v < PER_LANE; ++v) best = key[v] > best ? key[v] : best;
+      best = __reduce_max_sync(kAll, best);
+      if (best <= kKeyOfMinusInfinity) break;   // (an expert whose score is -infinity is never chosen)
+      uint32_t at = kAll;
+#pragma unroll
+      for (int v = PER_LANE - 1; v >= 0; --v) at = key[v] == best ? (uint32_t)(lane + 32 * v) : at;
+      at = __reduce_min_sync(kAll, at);
+#pragma unroll
+      for (int v = 0; v < PER_LANE; ++v) key[v] = at == (uint32_t)(lane + 32 * v) ? 0u : key[v];
+      if (j == 0) largest = of_key(best);
+      if (lane == j) {
+        id = (int)at;
+        score = of_key(best);
+      }
+      ++taken;
+    }
+    const float mine = lane < taken ? expf(score - largest) : 0.0f;
+    float total;
+    if (p.normalize) {
+      total = warp_sum(mine);
+    } else {
+      float part = 0.0f;
+#pragma unroll
+      for (int v = 0; v < PER_LANE; ++v) {
+        s[v] = taken > 0 ? expf(s[v] - largest) : 0.0f;
+        part += s[v];
+      }
+      total = warp_sum(part);
+    }
+    const float w = lane < taken ? mine / total : 0.0f;
+    if constexpr (!GRAD) {
+      if (lane < p.top) {
+        p.chosen[t * p.top + lane] = id;
+        p.weights[t * p.top + lane] = w;
+      }
+    } else {
+      const float mean = warp_sum(lane < taken ? slot_grad * w : 0.0f);
+      float d[PER_LANE];
+#pragma unroll
+      for (int v = 0; v < PER_LANE; ++v) d[v] = p.normalize || taken == 0 ? 0.0f : s[v] / total * -mean;
+      for (int j = 0; j < taken; ++j) {
+        const int at = __shfl_sync(kAll, id, j);
+        const float value = __shfl_sync(kAll, w * (slot_grad - mean), j);
+#pragma unroll
+        for (int v = 0; v < PER_LANE; ++v) d[v] = at == lane + 32 * v ? value : d[v];
+      }
+      T* out = reinterpret_cast<T*>(p.ds) + t * p.ldd;
+#pragma unroll
+      for (int v = 0; v < PER_LANE; ++v)
+        if (lane + 32 * v < p.experts) out[lane + 32 * v] = from_float<T>(d[v]);
+    }
+  }
+}
+
+template <typename T, bool GRAD>
+int route_of_type(const RouteParams& p, int sms, cudaStream_t st) {
+  const long long blocks = (p.rows + kRouteWarps - 1) / kRouteWarps;
+  const int grid = (int)(blocks < 16ll * sms ? blocks : 16ll * sms), threads = 32 * kRouteWarps;
+  const int per_lane = (p.experts + 31) / 32;
+  if (per_lane <= 1) return status_of(launch_pdl(route_kernel<T, 1, GRAD>, grid, threads, 0, st, p));
+  if (per_lane <= 2) return status_of(launch_pdl(route_kernel<T, 2, GRAD>, grid, threads, 0, st, p));
+  if (per_lane <= 4) return status_of(launch_pdl(route_kernel<T, 4, GRAD>, grid, threads, 0, st, p));
+  if (per_lane <= 8) return status_of(launch_pdl(route_kernel<T, 8, GRAD>, grid, threads, 0, st, p));
+  if (per_lane <= 16) return status_of(launch_pdl(route_kernel<T, 16, GRAD>, grid, threads, 0, st, p));
+  return status_of(launch_pdl(route_kernel<T, 32, GRAD>, grid, threads, 0, st, p));
+}
+template <bool GRAD>
+int route_launch(const RouteParams& p, int elem, cudaStream_t st) {
+  if (p.rows < 0 || p.experts < 1 || p.top < 1 || elem < VOID_ELEM_F32 || elem > VOID_ELEM_BF16) return VOID_ERR_BAD_ARG;
+  if (p.top > p.experts || p.lds < 0 || (p.rows > 1 && GRAD && (p.ldd < p.experts || p.ldg < 0))) return VOID_ERR_SHAPE;
+  if (p.experts > 1024 || p.top > 32 || p.rows > 0x7fffffffll) return VOID_ERR_TOO_LARGE;
+  if (p.rows == 0) return VOID_OK;
+  if (p.scores == nullptr || (GRAD ? p.g == nullptr || p.ds == nullptr : p.chosen == nullptr || p.weights == nullptr)) return VOID_ERR_BAD_ARG;
+  const DeviceInfo dev = device_info();
+  if (!dev.ok) return VOID_ERR_CUDA;
+  if (dev.cc_major != 10) return VOID_ERR_ARCH;
+  if (elem == VOID_ELEM_F32) return route_of_type<float, GRAD>(p, dev.sms, st);
+  return elem == VOID_ELEM_F16 ? route_of_type<__half, GRAD>(p, dev.sms, st) : route_of_type<__nv_bfloat16, GRAD>(p, dev.sms, st);
+}
+
+// ------------------------------------------------------------------------------------------ sort
+// A counting sort that keeps the order of the choices within an expert.  The choices are dealt to blocks in order; a first launch counts
+// every block's choices per expert (one block alone counts for itself), the second adds up what lies before a block and ranks its own: a warp
+// ranks 32 choices at once by asking which lanes have the same expert, and 32 warps meet in a table of their counts.
+constexpr int kSortThreads = 1024, kSortSteps = 4, kSortTile = kSortThreads * kSortSteps;
+constexpr int kMaxSortExperts = 1024;
+
+struct SortParams {
+  const void* experts;
+  long long count, share;   // choices, and of one block (a multiple of a tile)
+  int n_experts, pitch;     // pitch: entries between the warps' counts in shared memory
+  int32_t* table;           // [blocks][experts] counts, or null: one block
+  int32_t* offsets;
+  int32_t* position;
+};
+template <typename I>
+__device__ __forceinline__ int expert_of(const void* experts, long long i, int n_experts) {
+  const long long e = (long long)reinterpret_cast<const I*>(experts)[i];
+  return e < 0 || e >= n_experts ? -1 : (int)e;
+}
+template <typename I>
+__device__ __forceinline__ void count_choices(const SortParams& p, long long begin, long long end, int32_t* counts) {
+  for (int e = threadIdx.x; e < p.n_experts; e += blockDim.x) counts[e] = 0;
+  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  for (long long i = begin + threadIdx.x; i - lane < end; i += blockDim.x) {
+    const int e = i < end ? expert_of<I>(p.experts, i, p.n_experts) : -1;
+    const unsigned same = __match_any_sync(kAll, e);
+    if (e >= 0 && lane == __ffs(same) - 1) atomicAdd(&counts[e], __popc(same));   // (whole numbers: any order gives the same)
+  }
+  __syncthreads();
+}
+
+template <typename I>
+__global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const __grid_constant__ SortParams p) {
+  __shared__ int32_t counts[kMaxSortExperts];
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const long long begin = (long long)blockIdx.x * p.share, end = begin + p.share < p.count ? begin + p.share : p.count;
+  count_choices<I>(p, begin, end, counts);
+  for (int e = threadIdx.x; e < p.n_experts; e += blockDim.x) p.table[(long long)blockIdx.x * p.n_experts + e] = counts[e];
+}
+
+template <typename I>
+__global__ void __launch_bounds__(kSortThreads) sort_place_kernel(const __grid_constant__ SortParams p) {
+  extern __shared__ uint16_t warp_counts[];   // [32][pitch]
+  __shared__ int32_t base[kMaxSortExperts];   // rows of the experts before, and of this expert's choices in blocks and tiles before
+  __shared__ int32_t warp_total[32];
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const long long begin = (long long)blockIdx.x * p.share, end = begin + p.share < p.count ? begin + p.share : p.count;
+  int total = 0, before = 0;
+  if (p.table == nullptr) {
+    count_choices<I>(p, begin, end, base);
+    total = tid < p.n_experts ? base[tid] : 0;
+  } else if (tid < p.n_experts) {
+#pragma unroll 8
+    for (int b = 0; b < (int)gridDim.x; ++b) {
+      const int c = p.table[(long long)b * p.n_experts + tid];
+      total += c;
+      before += b < (int)blockIdx.x ? c : 0;
+    }
+  }
+  // rows before every expert's: an exclusive sum over the block
+  int upto = total;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(kAll, upto, o);
+    if (lane >= o) upto += u;
+  }
+  if (lane == 31) warp_total[warp] = upto;
+  __syncthreads();
+  int first = upto - total;
+  for (int w = 0; w < warp; ++w) first += warp_total[w];
+  if (tid < p.n_experts) base[tid] = first + before;
+  if (blockIdx.x == 0) {
+    if (tid < p.n_experts) p.offsets[tid] = first;
+    if (tid == p.n_experts - 1) p.offsets[p.n_experts] = first + total;
+  }
+  uint16_t* counts = warp_counts + warp * p.pitch;
+  for (long long tile = begin; tile < end; tile += kSortTile) {
+    for (int i = tid; i < 16 * p.pitch; i += kSortThreads) reinterpret_cast<uint32_t*>(warp_counts)[i] = 0u;
+    __syncthreads();
+    int expert[kSortSteps], rank[kSortSteps];
+    const long long from = tile + (long long)warp * (32 * kSortSteps) + lane;
+#pragma unroll
+    for (int k = 0; k < kSortSteps; ++k) expert[k] = from + 32 * k < end ? expert_of<I>(p.experts, from + 32 * k, p.n_experts) : -1;
+#pragma unroll
+    for (int k = 0; k < kSortSteps; ++k) {
+      const unsigned same = __match_any_sync(kAll, expert[k]);
+      const int ahead = expert[k] >= 0 ? counts[expert[k]] : 0;
+      __syncwarp();
+      if (expert[k] >= 0 && lane == __ffs(same) - 1) counts[expert[k]] = (uint16_t)(ahead + __popc(same));
+      __syncwarp();
+      rank[k] = ahead + __popc(same & ((1u << lane) - 1u));
+    }
+    __syncthreads();
+    // counts of the warps before, in the place of every warp's own: a warp adds up an expert's
+    for (int e = warp; e < p.n_experts; e += 32) {
+      const int c = warp_counts[lane * p.pitch + e];
+      int sum = c;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(kAll, sum, o);
+        if (lane >= o) sum += u;
+      }
+      warp_counts[lane * p.pitch + e] = (uint16_t)(sum - c);
+      if (lane == 31) reinterpret_cast<int32_t*>(warp_counts + 32 * p.pitch)[e] = sum;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kSortSteps; ++k) {
+      const long long i = from + 32 * k;
+      if (i < end) p.position[i] = expert[k] >= 0 ? base[expert[k]] + counts[expert[k]] + rank[k] : -1;
+    }
+    __syncthreads();
+    for (int e = tid; e < p.n_experts; e += kSortThreads) base[e] += reinterpret_cast<int32_t*>(warp_counts + 32 * p.pitch)[e];
+    __syncthreads();
+  }
+}
+
+// Blocks of a sort, and the choices of one: a tile each, until every SM has a block.
+inline int sort_blocks(long long count, int sms) {
+  const long long tiles = (count + kSortTile - 1) / kSortTile;
+  return (int)(tiles < 1 ? 1 : (tiles < sms ? tiles : sms));
+}
+inline long long sort_share(long long count, int blocks) {
+  const long long tiles = (count + kSortTile - 1) / kSortTile;
+  return (tiles + blocks - 1) / blocks * kSortTile;
+}
+constexpr int kMaxSortBlocks = 256;
+
+// ------------------------------------------------------------------------------------------ rows of tokens
+constexpr int kRowThreads = 256;
+// Pieces of a row that one thread holds at a time: 16-byte pieces two, single elements eight.
+template <int VEC> constexpr int kHeld = VEC > 1 ? 2 : 8;
+// Choices that the sort's own block is not worth a launch for: every warp ranks its token's choices by counting.
+constexpr int kFewChoices = 1024;
+
+struct RowParams {
+  const void* x;            // tokens (dispatch), rows (combine, its gradient)
+  long long ldx;
+  const void* g;            // combine's gradient: dy
+  long long ldg;
+  const void* residual;
+  long long ldr;
+  int residual_elem;
+  const void* weights;      // [tokens][top], or null: ones
+  int weight_elem;
+  const int32_t* position;  // [tokens][top]
+  const int32_t* used;      // rows in runs
+  long long tokens, rows;   // rows: tokens * top
+  int cols, top;
+  void* out;                // rows (dispatch, gradient; may be null), tokens (combine)
+  long long ldo;
+  void* dw;                 // gradient of the weights, of their type, or null
+  int zero_rest;
+  // dispatch that sorts by itself
+  const void* experts;
+  int32_t *offsets, *positions;
+  int n_experts;
+};
+// Whether a choice has a row; positions are not trusted.
+__device__ __forceinline__ bool has_row(const RowParams& p, int row) { return row >= 0 && row < p.rows; }
+
+// Zeros in the rows behind the last run, dealt to the launch's blocks.
+template <typename T, int VEC>
+__device__ __forceinline__ void zero_rest(const RowParams& p, long long used, int c0, int c1) {
+  Piece<T, VEC> zero;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) zero.set(e, 0.0f);
+  for (long long r = (used < 0 ? 0 : used) + blockIdx.x; r < p.rows; r += gridDim.x)
+    for (int c = c0 + threadIdx.x * VEC; c < c1; c += kRowThreads * VEC) zero.store(reinterpret_cast<T*>(p.out) + r * p.ldo + c);
+}
+
+// Token by token, so that x is read once; a token's copies go where its choices were sorted to.  blockIdx.y: part of the columns.
+// SORT (few choices): the rows are not known yet, each is the number of choices that come before it.
+template <typename T, int VEC, typename I, bool SORT>
+__global__ void __launch_bounds__(kRowThreads) dispatch_kernel(const __grid_constant__ RowParams p) {
+  constexpr int U = kHeld<VEC>;
+  __shared__ int32_t ids[SORT ? kFewChoices : 1];
+  __shared__ int32_t place[SORT ? kFewChoices : 1];   // of this token's choices
+  __shared__ int32_t rows_used;
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int c0 = blockIdx.y * (kRowThreads * VEC * U);
+  const int c1 = c0 + kRowThreads * VEC * U < p.cols ? c0 + kRowThreads * VEC * U : p.cols;
+  const T* x = reinterpret_cast<const T*>(p.x);
+  T* out = reinterpret_cast<T*>(p.out);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if constexpr (SORT) {
+    for (int i = threadIdx.x; i < (int)p.rows; i += kRowThreads) ids[i] = expert_of<I>(p.experts, i, p.n_experts);
+    if (threadIdx.x == 0) rows_used = 0;
+    __syncthreads();
+    if (warp == 0) {
+      int n = 0;
+      for (int i = lane; i < (int)p.rows; i += 32) n += ids[i] >= 0;
+      n = __reduce_add_sync(kAll, n);
+      if (lane == 0) rows_used = n;
+    }
+    if (blockIdx.x == 0 && blockIdx.y == 0) {
+      for (int e = warp; e <= p.n_experts; e += kRowThreads / 32) {
+        int n = 0;
+        for (int i = lane; i < (int)p.rows; i += 32) n += ids[i] >= 0 && ids[i] < e;
+        n = __reduce_add_sync(kAll, n);
+        if (lane == 0) p.offsets[e] = n;
+      }
+    }
+  }
+  for (long long t = blockIdx.x; t < p.tokens; t += gridDim.x) {
+    Piece<T, VEC> piece[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int c = c0 + (u * kRowThreads + threadIdx.x) * VEC;
+      if (c < c1) piece[u].load(x + t * p.ldx + c);
+    }
+    if constexpr (SORT) {
+      __syncthreads();
+      for (int j = warp; j < p.top; j += kRowThreads / 32) {
+        const int me = (int)t * p.top + j, e = ids[me];
+        int n = 0;
+        for (int i = lane; i < (int)p.rows; i += 32) n += ids[i] >= 0 && (ids[i] < e || (ids[i] == e && i < me));
+        n = __reduce_add_sync(kAll, n);
+        if (lane == 0) {
+          place[j] = e >= 0 ? n : -1;
+          if (blockIdx.y == 0) p.positions[me] = place[j];
+        }
+      }
+      __syncthreads();
+    }
+    for (int j = 0; j < p.top; ++j) {
+      const int row = SORT ? place[j] : p.position[t * p.top + j];
+      if (!has_row(p, row)) continue;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int c = c0 + (u * kRowThreads + threadIdx.x) * VEC;
+        if (c < c1) piece[u].store(out + (long long)row * p.ldo + c);
+      }
+    }
+  }
+  if (p.zero_rest) {
+    if constexpr (SORT) __syncthreads();
+    zero_rest<T, VEC>(p, SORT ? rows_used : *p.used, c0, c1);
+  }
+}
+
+constexpr int kTogether = 4;   // rows of a token whose loads are in flight together
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kRowThreads) combine_kernel(const __grid_constant__ RowParams p) {
+  constexpr int U = kHeld<VEC>;
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int c0 = blockIdx.y * (kRowThreads * VEC * U);
+  const T* ys = reinterpret_cast<const T*>(p.x);
+  T* out = reinterpret_cast<T*>(p.out);
+  for (long long t = blockIdx.x; t < p.tokens; t += gridDim.x) {
+    float sum[U][VEC];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) sum[u][e] = 0.0f;
+    for (int j0 = 0; j0 < p.top; j0 += kTogether) {
+      int row[kTogether];
+      float w[kTogether];
+#pragma unroll
+      for (int k = 0; k < kTogether; ++k) {
+        const bool in = j0 + k < p.top;
+        row[k] = in ? p.position[t * p.top + j0 + k] : -1;
+        if (!has_row(p, row[k])) row[k] = -1;
+        w[k] = in && p.weights != nullptr ? element(p.weights, p.weight_elem, t * p.top + j0 + k) : 1.0f;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int c = c0 + (u * kRowThreads + threadIdx.x) * VEC;
+        if (c >= p.cols) continue;
+        Piece<T, VEC> piece[kTogether];
+#pragma unroll
+        for (int k = 0; k < kTogether; ++k)
+          if (row[k] >= 0) piece[k].load(ys + (long long)row[k] * p.ldx + c);
+#pragma unroll
+        for (int k = 0; k < kTogether; ++k)
+          if (row[k] >= 0) {   // (a dropped choice's weight may be anything)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) sum[u][e] = fmaf(w[k], piece[k].get(e), sum[u][e]);
+          }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int c = c0 + (u * kRowThreads + threadIdx.x) * VEC;
+      if (c >= p.cols) continue;
+      if (p.residual != nullptr) {
+        if (p.residual_elem == VOID_ELEM_F32 && sizeof(T) != 4) {
+          const float* r = reinterpret_cast<const float*>(p.residual) + t * p.ldr + c;
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) sum[u][e] += r[e];
+        } else {
+          Piece<T, VEC> r;
+          r.load(reinterpret_cast<const T*>(p.residual) + t * p.ldr + c);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) sum[u][e] += r.get(e);
+        }
+      }
+      Piece<T, VEC> y;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) y.set(e, sum[u][e]);
+      y.store(out + t * p.ldo + c);
+    }
+  }
+}
+
+// A block per token: dy is read once (and again from the first cache for more than four choices), the rows of its choices meet it.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kRowThreads) combine_grad_kernel(const __grid_constant__ RowParams p) {
+  __shared__ float part[kTogether][kRowThreads / 32];
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const T *ys = reinterpret_cast<const T*>(p.x), *g = reinterpret_cast<const T*>(p.g);
+  T* out = reinterpret_cast<T*>(p.out);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (long long t = blockIdx.x; t < p.tokens; t += gridDim.x) {
+    for (int j0 = 0; j0 < p.top; j0 += kTogether) {
+      int row[kTogether];
+      float w[kTogether], dot[kTogether];
+#pragma unroll
+      for (int k = 0; k < kTogether; ++k) {
+        const bool in = j0 + k < p.top;
+        row[k] = in ? p.position[t * p.top + j0 + k] : -1;
+        if (!has_row(p, row[k])) row[k] = -1;
+        w[k] = in && p.weights != nullptr ? element(p.weights, p.weight_elem, t * p.top + j0 + k) : 1.0f;
+        dot[k] = 0.0f;
+      }
+#pragma unroll 2
+      for (int c = threadIdx.x * VEC; c < p.cols; c += kRowThreads * VEC) {
+        Piece<T, VEC> d, y[kTogether];
+        d.load(g + t * p.ldg + c);
+        if (p.dw != nullptr) {
+#pragma unroll
+          for (int k = 0; k < kTogether; ++k)
+            if (row[k] >= 0) y[k].load(ys + (long long)row[k] * p.ldx + c);
+        }
+#pragma unroll
+        for (int k = 0; k < kTogether; ++k) {
+          if (row[k] < 0) continue;
+          if (p.dw != nullptr) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) dot[k] = fmaf(d.get(e), y[k].get(e), dot[k]);
+          }
+          if (out != nullptr) {
+            Piece<T, VEC> q;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) q.set(e, w[k] * d.get(e));
+            q.store(out + (long long)row[k] * p.ldo + c);
+          }
+        }
+      }
+      if (p.dw != nullptr) {
+#pragma unroll
+        for (int k = 0; k < kTogether; ++k) {
+          const float s = warp_sum(dot[k]);
+          if (lane == 0) part[k][warp] = s;
+        }
+        __syncthreads();
+        if (threadIdx.x < kTogether && j0 + (int)threadIdx.x < p.top) {
+          float s = 0.0f;
+#pragma unroll
+          for (int i = 0; i < kRowThreads / 32; ++i) s += part[threadIdx.x][i];
+          set_element(p.dw, p.weight_elem, t * p.top + j0 + threadIdx.x, s);
+        }
+        __syncthreads();
+      }
+    }
+  }
+  if (out != nullptr && p.zero_rest) zero_rest<T, VEC>(p, *p.used, 0, p.cols);
+}
+
+// Whether rows of `elem_bytes` elements lie in whole 16-byte pieces.
+inline bool in_pieces(const void* at, long long ld, int elem_bytes) { return ((reinterpret_cast<uintptr_t>(at) | (uintptr_t)(ld * elem_bytes)) & 15u) == 0; }
+inline int elem_size(int elem) { return elem == VOID_ELEM_F32 ? 4 : 2; }
+
+enum class RowOp { Dispatch, DispatchSort32, DispatchSort64, Combine, CombineGrad };
+template <typename T, int VEC>
+cudaError_t launch_rows(RowOp op, const RowParams& p, int sms, cudaStream_t st) {
+  const long long width = (long long)kRowThreads * VEC * kHeld<VEC>;
+  const unsigned parts = op == RowOp::CombineGrad ? 1u : (unsigned)((p.cols + width - 1) / width);
+  const long long most = 64ll * sms;
+  const dim3 grid((unsigned)(p.tokens < most ? p.tokens : most), parts);
+  switch (op) {
+    case RowOp::Dispatch: return launch_pdl(dispatch_kernel<T, VEC, int32_t, false>, grid, kRowThreads, 0, st, p);
+    case RowOp::DispatchSort32: return launch_pdl(dispatch_kernel<T, VEC, int32_t, true>, grid, kRowThreads, 0, st, p);
+    case RowOp::DispatchSort64: return launch_pdl(dispatch_kernel<T, VEC, int64_t, true>, grid, kRowThreads, 0, st, p);
+    case RowOp::Combine: return launch_pdl(combine_kernel<T, VEC>, grid, kRowThreads, 0, st, p);
+    default: return launch_pdl(combine_grad_kernel<T, VEC>, grid, kRowThreads, 0, st, p);
+  }
+}
+template <typename T>
+int rows_of_type(RowOp op, const RowParams& p, bool wide, int sms, cudaStream_t st) {
+  return status_of(wide ? launch_rows<T, 16 / (int)sizeof(T)>(op, p, sms, st) : launch_rows<T, 1>(op, p, sms, st));
+}
+int rows_launch(RowOp op, RowParams& p, int elem, cudaStream_t st) {
+  if (elem < VOID_ELEM_F32 || elem > VOID_ELEM_BF16 || p.tokens < 0 || p.top < 1 || p.cols < 0) return VOID_ERR_BAD_ARG;
+  if (p.tokens > 0x7fffffffll / p.top) return VOID_ERR_TOO_LARGE;
+  p.rows = p.tokens * p.top;
+  const bool combine = op == RowOp::Combine, grad = op == RowOp::CombineGrad;
+  if (p.tokens > 1 && ((p.ldx < p.cols && (combine || p.x != nullptr)) || (p.out != nullptr && p.ldo < p.cols) || (grad && p.ldg < p.cols) || (p.residual != nullptr && p.ldr < p.cols)))
+    return VOID_ERR_SHAPE;
+  if (p.tokens == 0 || (p.cols == 0 && p.dw == nullptr)) return VOID_OK;
+  const DeviceInfo dev = device_info();
+  if (!dev.ok) return VOID_ERR_CUDA;
+  if (dev.cc_major != 10) return VOID_ERR_ARCH;
+  const int es = elem_size(elem);
+  bool wide = p.cols % (16 / es) == 0 && (p.x == nullptr || in_pieces(p.x, p.ldx, es)) && (p.out == nullptr || in_pieces(p.out, p.ldo, es));
+  if (grad) wide = wide && in_pieces(p.g, p.ldg, es);
+  if (p.residual != nullptr) wide = wide && in_pieces(p.residual, p.ldr, elem_size(p.residual_elem));
+  if (elem == VOID_ELEM_F32) return rows_of_type<float>(op, p, wide, dev.sms, st);
+  return elem == VOID_ELEM_F16 ? rows_of_type<__half>(op, p, wide, dev.sms, st) : rows_of_type<__nv_bfloat16>(op, p, wide, dev.sms, st);
+}
+
+int sort_launch(SortParams p, int index_bytes, void* ws, size_t ws_bytes, cudaStream_t st) {
+  const DeviceInfo dev = device_info();
+  if (!dev.ok) return VOID_ERR_CUDA;
+  if (dev.cc_major != 10) return VOID_ERR_ARCH;
+  const int sms = dev.sms < kMaxSortBlocks ? dev.sms : kMaxSortBlocks, blocks = sort_blocks(p.count, sms);
+  p.share = sort_share(p.count, blocks);
+  p.pitch = 2 * ((p.n_experts + 1) / 2 | 1);   // an odd number of words: a warp adds up a column without conflicts
+  const int smem = 32 * p.pitch * 2 + 4 * p.n_experts;
+  if (blocks > 1) {
+    if (ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 3u) != 0 || ws_bytes < (size_t)blocks * p.n_experts * 4) return VOID_ERR_WORKSPACE;
+    p.table = reinterpret_cast<int32_t*>(ws);
+    const cudaError_t rc = index_bytes == 4 ? launch_pdl(sort_count_kernel<int32_t>, blocks, kSortThreads, 0, st, p)
+                                            : launch_pdl(sort_count_kernel<int64_t>, blocks, kSortThreads, 0, st, p);
+    if (rc != cudaSuccess) return VOID_ERR_CUDA;
+  }
+  if (index_bytes == 4) {
+    if (ensure_smem(reinterpret_cast<const void*>(sort_place_kernel<int32_t>), smem) != 0) return VOID_ERR_CUDA;
+    return status_of(launch_pdl(sort_place_kernel<int32_t>, blocks, kSortThreads, smem, st, p));
+  }
+  if (ensure_smem(reinterpret_cast<const void*>(sort_place_kernel<int64_t>), smem) != 0) return VOID_ERR_CUDA;
+  return status_of(launch_pdl(sort_place_kernel<int64_t>, blocks, kSortThreads, smem, st, p));
+}
+// The arguments of a sort, or why not.
+int check_sort(const void* experts, int32_t index_bytes, int64_t count, int32_t n_experts, const int32_t* offsets, const int32_t* position) {
+  if (n_experts < 1 || count < 0 || (index_bytes != 4 && index_bytes != 8) || offsets == nullptr) return VOID_ERR_BAD_ARG;
+  if (count > 0 && (experts == nullptr || position == nullptr)) return VOID_ERR_BAD_ARG;
+  if (n_experts > kMaxSortExperts || count > 0x7fffffffll) return VOID_ERR_TOO_LARGE;
+  if ((reinterpret_cast<uintptr_t>(experts) & (uintptr_t)(index_bytes - 1)) != 0) return VOID_ERR_ALIGN;
+  return VOID_OK;
+}
+
+}  // namespace
+
+}  // namespace vb
+
+extern "C" {
+
+int void_route(const void* scores, int32_t elem, int64_t lds, int64_t rows, int32_t n_experts, int32_t top_k, int32_t normalize, int32_t* experts,
+               float* weights, void_stream_t stream) {
+  vb::RouteParams p = {};
+  p.scores = scores; p.lds = lds; p.rows = rows; p.experts = n_experts; p.top = top_k; p.normalize = normalize; p.chosen = experts; p.weights = weights;
+  return vb::route_launch<false>(p, elem, reinterpret_cast<cudaStream_t>(stream));
+}
+int void_route_grad(const void* scores, int32_t elem, int64_t lds, int64_t rows, int32_t n_experts, int32_t top_k, int32_t normalize,
+                    const float* g, int64_t ldg, void* dscores, int64_t ldd, void_stream_t stream) {
+  vb::RouteParams p = {};
+  p.scores = scores; p.lds = lds; p.rows = rows; p.experts = n_experts; p.top = top_k; p.normalize = normalize; p.g = g; p.ldg = ldg; p.ds = dscores; p.ldd = ldd;
+  return vb::route_launch<true>(p, elem, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t void_sort_by_expert_ws_bytes(int64_t count, int32_t n_experts) {
+  if (count < 0 || n_experts < 1) return 0;
+  const int blocks = vb::sort_blocks(count, vb::kMaxSortBlocks);
+  return blocks > 1 ? (size_t)blocks * n_experts * 4 : 0;
+}
+int void_sort_by_expert(const void* experts, int32_t index_bytes, int64_t count, int32_t n_experts, int32_t* offsets, int32_t* position, void* ws,
+                        size_t ws_bytes, void_stream_t stream) {
+  const int bad = vb::check_sort(experts, index_bytes, count, n_experts, offsets, position);
+  if (bad != VOID_OK) return bad;
+  vb::SortParams p = {};
+  p.experts = experts; p.count = count; p.n_experts = n_experts; p.offsets = offsets; p.position = position;
+  return vb::sort_launch(p, index_bytes, ws, ws_bytes, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int void_dispatch(const void* x, int32_t elem, int64_t ldx, int64_t tokens, int32_t cols, const void* experts, int32_t index_bytes, int32_t top_k,
+                  int32_t n_experts, int32_t* offsets, int32_t* position, void* out, int64_t ldo, int32_t zero_rest, void* ws, size_t ws_bytes,
+                  void_stream_t stream) {
+  if (tokens < 0 || top_k < 1 || cols < 0) return VOID_ERR_BAD_ARG;
+  if (tokens > 0x7fffffffll / top_k) return VOID_ERR_TOO_LARGE;
+  const int bad = vb::check_sort(experts, index_bytes, tokens * top_k, n_experts, offsets, position);
+  if (bad != VOID_OK) return bad;
+  if (tokens > 0 && cols > 0 && (x == nullptr || out == nullptr)) return VOID_ERR_BAD_ARG;
+  const long long count = tokens * top_k;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  vb::RowParams p = {};
+  p.x = x; p.ldx = ldx; p.tokens = tokens; p.cols = cols; p.top = top_k; p.out = out; p.ldo = ldo; p.zero_rest = zero_rest;
+  p.position = position; p.used = offsets + n_experts;
+  if (tokens > 0 && cols > 0 && count <= vb::kFewChoices) {
+    p.experts = experts; p.offsets = offsets; p.positions = position; p.n_experts = n_experts;
+    return vb::rows_launch(index_bytes == 4 ? vb::RowOp::DispatchSort32 : vb::RowOp::DispatchSort64, p, elem, st);
+  }
+  const int sorted = void_sort_by_expert(experts, index_bytes, count, n_experts, offsets, position, ws, ws_bytes, stream);
+  return sorted != VOID_OK ? sorted : vb::rows_launch(vb::RowOp::Dispatch, p, elem, st);
+}
+
+int void_combine(const void* rows, int32_t elem, int64_t ldx, int64_t tokens, int32_t cols, int32_t top_k, const int32_t* position, const void* weights,
+                 int32_t weight_elem, const void* residual, int64_t ldr, int32_t residual_elem, void* out, int64_t ldo, void_stream_t stream) {
+  if (tokens > 0 && cols > 0 && (rows == nullptr || position == nullptr || out == nullptr)) return VOID_ERR_BAD_ARG;
+  if (weight_elem < VOID_ELEM_F32 || weight_elem > VOID_ELEM_BF16) return VOID_ERR_BAD_ARG;
+  if (residual != nullptr && residual_elem != elem && residual_elem != VOID_ELEM_F32) return VOID_ERR_BAD_ARG;
+  vb::RowParams p = {};
+  p.x = rows; p.ldx = ldx; p.tokens = tokens; p.cols = cols; p.top = top_k; p.position = position; p.weights = weights; p.weight_elem = weight_elem;
+  p.residual = residual; p.ldr = ldr; p.residual_elem = residual_elem; p.out = out; p.ldo = ldo;
+  return vb::rows_launch(vb::RowOp::Combine, p, elem, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int void_combine_grad(const void* g, int64_t ldg, const void* rows, int64_t ldx, int32_t elem, int64_t tokens, int32_t cols, int32_t top_k,
+                      const int32_t* position, const int32_t* used_rows, const void* weights, int32_t weight_elem, void* drows, int64_t ldd,
+                      void* dweights, void_stream_t stream) {
+  if (weight_elem < VOID_ELEM_F32 || weight_elem > VOID_ELEM_BF16) return VOID_ERR_BAD_ARG;
+  if (tokens > 0 && (position == nullptr || used_rows == nullptr || (cols > 0 && (g == nullptr || (dweights != nullptr && rows == nullptr)))))
+    return VOID_ERR_BAD_ARG;
+  if (drows == nullptr && dweights == nullptr) return VOID_OK;
+  vb::RowParams p = {};
+  p.x = rows; p.ldx = ldx; p.g = g; p.ldg = ldg; p.tokens = tokens; p.cols = cols; p.top = top_k; p.position = position; p.used = used_rows;
+  p.weights = weights; p.weight_elem = weight_elem; p.out = drows; p.ldo = ldd; p.dw = dweights; p.zero_rest = 1;
+  return vb::rows_launch(vb::RowOp::CombineGrad, p, elem, reinterpret_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

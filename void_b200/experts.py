@@ -5,13 +5,14 @@ weights of all experts are one list of tiles and one packed store; a run may hav
 offsets stay on the device (csrc/experts.cu).
 """
 from dataclasses import dataclass
-from typing import Optional, Sequence, Tuple
+from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
 from . import _lib
 from .autograd import _require_operands, tile_grad_items
 from .format import Derived, VOIDTensor, build_tile_index
+from .fp8_blocks import FP8BlockTensor
 from .fusion import layer_activation
 from .ops import _KIND_DTYPE, packed_fp, product_kind
 
@@ -98,7 +99,7 @@ def stack_experts(weights: Sequence[VOIDTensor]) -> VOIDExperts:
     return VOIDExperts(tensor, len(weights), tuple(first.shape))
 
 
-def void_expert_linear(experts: VOIDExperts, x: torch.Tensor, offsets: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: int = 0,
+def void_expert_linear(experts: Union[VOIDExperts, FP8BlockTensor], x: torch.Tensor, offsets: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: int = 0,
                        out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y[t] = act(x[t] @ A_e^T + bias[e]) for the tokens offsets[e] <= t < offsets[e + 1] of every expert e; x [tokens, in] in
     float32 (multiplied as TF32), float16 or bfloat16, sorted by expert, y [tokens, out] in x's type.  ``offsets`` is int32 or int64
@@ -106,7 +107,17 @@ def void_expert_linear(experts: VOIDExperts, x: torch.Tensor, offsets: torch.Ten
     [n_experts, out].  Rows in no run (before the first offset, behind the last) are zeros; with ``out`` (which must have no memory in common with an operand)
     they are left as they are.
     Offsets that fall or lie outside the batch are taken as empty runs and reported by check_device_status.  Inference form of
-    SparseExperts: nothing is differentiated."""
+    SparseExperts: nothing is differentiated.
+    ``experts`` may also be an FP8BlockTensor [n_experts, out, in], dense weights in e4m3 with a scale per 128 x 128; x is then quantised with a
+    scale for each token's 128 features, or given as such an FP8BlockTensor (y float32, or of ``out``'s type)."""
+    if type(experts) is FP8BlockTensor:
+        if experts.n_experts is None:
+            raise _lib.VoidB200Error("void_expert_linear takes weights [n_experts, out, in], got %s" % (experts.shape,))
+        E, M, K = experts.shape
+        assert len(x.shape) == 2 and x.shape[1] == K, f"Dimension mismatch: the experts are {(M, K)}, x is {tuple(x.shape)}"
+        if bias is not None:
+            assert bias.shape == (E, M), f"bias must have shape {(E, M)}, got {tuple(bias.shape)}"
+        return experts._product(x, offsets, bias, activation, out, None, None)
     if not isinstance(experts, VOIDExperts):
         raise TypeError("void_expert_linear takes a VOIDExperts (stack_experts), got %s" % type(experts).__name__)
     assert x.dim() == 2 and x.shape[1] == experts.shape[1], f"Dimension mismatch: the experts are {experts.shape}, x is {tuple(x.shape)}"

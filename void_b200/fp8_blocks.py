@@ -1,0 +1,132 @@
+"""Dense e4m3 matrices with a scale for each block of 128 columns: weights of linear layers and of experts on B200.
+
+The reference's FP8 tensors are 32x32 tiles with a scale each (void/fp8.py:438-570); this is an extension for dense weights, whose blocks are
+128 x 128, and for tokens, whose blocks are one token's 128 features.  ops.void_linear and experts.void_expert_linear take them
+(csrc/fp8_blocks.cu): products on the FP8 tensor cores, both scales applied to each block's fp32 sum.  Inference only, like the other
+quantised products.
+"""
+from typing import Optional
+
+import torch
+
+from . import _lib
+
+BLOCK = 128
+
+
+def _rows_on_16_bytes(values: torch.Tensor) -> torch.Tensor:
+    """The values themselves where their rows start on 16-byte boundaries, else a copy whose rows do."""
+    cols = values.shape[-1]
+    if values.data_ptr() % 16 == 0 and (cols <= 1 or values.stride(-1) == 1) and all(
+            s % 16 == 0 and s >= cols for n, s in zip(values.shape[:-1], values.stride()[:-1]) if n > 1):
+        return values
+    copy = torch.empty(*values.shape[:-1], (cols + 15) // 16 * 16, dtype=values.dtype, device=values.device)[..., :cols]
+    copy.view(torch.uint8).copy_(values.view(torch.uint8))
+    return copy
+
+
+class FP8BlockTensor:
+    """A matrix [rows, cols], or the matrices of experts [experts, rows, cols], in float8_e4m3fn (``values``) with float32 ``scales``
+    [..., ceil(rows / 128), ceil(cols / 128)] (weights) or [rows, ceil(cols / 128)] (tokens): the matrix stands for values * scale of their
+    block.  ``values`` and ``scales`` are the tensors given (values with rows that do not start on 16-byte boundaries: a copy), and products
+    read them as they are at the time of the call."""
+    __slots__ = ("values", "scales", "block_rows", "_status")
+
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor):
+        if values.dtype is not torch.float8_e4m3fn:
+            raise _lib.VoidB200Error("an FP8BlockTensor holds float8_e4m3fn values, got %s" % values.dtype)
+        if scales.dtype is not torch.float32:
+            raise _lib.VoidB200Error("an FP8BlockTensor's scales are float32, got %s" % scales.dtype)
+        if values.dim() not in (2, 3) or scales.dim() != values.dim() or 0 in values.shape:
+            raise ValueError("an FP8BlockTensor is a matrix or a stack of matrices with scales of as many dimensions, none of them empty, got %s and %s"
+                             % (tuple(values.shape), tuple(scales.shape)))
+        if values.device != scales.device:
+            raise _lib.VoidB200Error("values and scales are on different devices")
+        rows, cols = values.shape[-2:]
+        across, down = (cols + BLOCK - 1) // BLOCK, (rows + BLOCK - 1) // BLOCK
+        if tuple(scales.shape) == (*values.shape[:-2], down, across):
+            self.block_rows = BLOCK
+        elif values.dim() == 2 and tuple(scales.shape) == (rows, across):
+            self.block_rows = 1
+        else:
+            raise ValueError("scales of a %s matrix must be %s (or, of tokens, %s), got %s" % (
+                tuple(values.shape), (*values.shape[:-2], down, across), (rows, across), tuple(scales.shape)))
+        self.values, self.scales, self._status = _rows_on_16_bytes(values), scales, None
+
+    @property
+    def shape(self):
+        return tuple(self.values.shape)
+
+    @property
+    def device(self) -> torch.device:
+        return self.values.device
+
+    @property
+    def n_experts(self) -> Optional[int]:
+        return self.values.shape[0] if self.values.dim() == 3 else None
+
+    @property
+    def memory_bytes(self) -> int:
+        return self.values.numel() + 4 * self.scales.numel()
+
+    def to(self, device) -> "FP8BlockTensor":
+        return FP8BlockTensor(self.values.to(device), self.scales.to(device))
+
+    def cuda(self) -> "FP8BlockTensor":
+        return self.to("cuda")
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The matrix it stands for, values * scale in float32 rounded to ``dtype``."""
+        rows, cols = self.values.shape[-2:]
+        scales = self.scales.repeat_interleave(BLOCK, -1)[..., :cols]
+        if self.block_rows != 1:
+            scales = scales.repeat_interleave(self.block_rows, -2)[..., :rows, :]
+        return (self.values.float() * scales).to(dtype)
+
+    def _product(self, x, offsets, bias, activation, out, out_dtype, residual) -> torch.Tensor:
+        values, scales = self.values, self.scales
+        if self.block_rows != BLOCK and values.shape[-2] > 1:
+            raise _lib.VoidB200Error("weights carry a scale for each block of 128 x 128, got scales %s" % (tuple(scales.shape),))
+        x_scales = None
+        if isinstance(x, FP8BlockTensor):
+            if x.block_rows != 1 and x.values.shape[0] > 1:
+                raise _lib.VoidB200Error("tokens carry a scale for each token's 128 features, got scales %s" % (tuple(x.scales.shape),))
+            x, x_scales = x.values, x.scales
+            dtype = out_dtype or (torch.float32 if out is None else out.dtype)
+        else:
+            if x.dtype not in _lib.OUT_DTYPE_CODE:
+                raise _lib.VoidB200Error("x must be float32, float16 or bfloat16, or an FP8BlockTensor, got %s" % x.dtype)
+            dtype = out_dtype or (x.dtype if out is None else out.dtype)
+        _lib.require_cuda(values, scales, x, x_scales, offsets, bias, out, residual)
+        if out is not None and out.dtype is not dtype:
+            raise _lib.VoidB200Error("out must be of type %s, got %s" % (dtype, out.dtype))
+        status = self._status
+        if status is None or status.device != values.device:
+            status = self._status = _lib.status_word(values.device)
+        return _lib.native().fp8_linear(values, scales, x, x_scales, offsets, bias, activation, out, dtype, residual, status)
+
+    def __repr__(self) -> str:
+        return f"FP8BlockTensor(shape={self.shape}, block={(self.block_rows, BLOCK)}, device={self.values.device})"
+
+
+def quantize_fp8_blocks(x: torch.Tensor, block_rows: int = BLOCK) -> FP8BlockTensor:
+    """x [rows, cols] (float32, float16 or bfloat16) in e4m3 with a scale for each 128 x 128 block (weights; also of x [experts, rows, cols]), or with
+    ``block_rows=1`` for each row's 128 columns (tokens, as void_linear and void_expert_linear take them).  A scale is the smallest
+    power of two that keeps its block within 448, so that only the quotients are rounded, once; a block that holds an infinity or NaN gets a
+    scale of NaN."""
+    if block_rows not in (1, BLOCK):
+        raise ValueError("blocks have 1 or %d rows, got %s" % (BLOCK, block_rows))
+    if x.dim() not in (2, 3) or (x.dim() == 3 and block_rows == 1) or 0 in x.shape:
+        raise ValueError("quantize_fp8_blocks takes a matrix (or, of weights, a stack of them) that is not empty, got %s" % (tuple(x.shape),))
+    _lib.require_cuda(x)
+    if x.dim() == 2:
+        return FP8BlockTensor(*_lib.native().quant_fp8_blocks(x, block_rows))
+    parts = [_lib.native().quant_fp8_blocks(m, block_rows) for m in x]
+    pitch = (x.shape[2] + 15) // 16 * 16
+    values = torch.empty(*x.shape[:2], pitch, dtype=torch.float8_e4m3fn, device=x.device)[..., :x.shape[2]]
+    for to, (given, _) in zip(values, parts):
+        to.view(torch.uint8).copy_(given.view(torch.uint8))
+    return FP8BlockTensor(values, torch.stack([s for _, s in parts]))
+
+
+__all__ = ["FP8BlockTensor", "quantize_fp8_blocks"]

@@ -13,6 +13,7 @@ import torch
 
 from . import _lib, _spmm
 from .format import VOIDTensor, index_is_current, note_index
+from .fp8_blocks import FP8BlockTensor
 from .int_quant import Int8VOIDTensor
 
 _KIND_DTYPE = {_lib.KIND_F16: torch.float16, _lib.KIND_BF16: torch.bfloat16, _lib.KIND_TF32: torch.float32}
@@ -99,11 +100,15 @@ def void_linear(a, x: torch.Tensor, bias: Optional[torch.Tensor] = None, activat
     """y = act(x @ A^T + bias) (+ residual) for activations x [batch, in] and a VOID weight A [out, in]: the linear layer
     without transposed copies.  The reference computes (A @ x^T)^T and so copies x^T and returns a strided
     view (void/fusion.py:586-598, :817-829; void/autograd.py:336); here the kernel reads x and writes y as
-    they lie in memory.  ``a`` is a floating VOIDTensor (y in x's dtype) or an Int8VOIDTensor (x int8 with
-    per-row scales ``x_scale`` [batch], or a float scalar; y fp32 unless ``out_dtype`` / ``out`` say otherwise).
+    they lie in memory.  ``a`` is a floating VOIDTensor (y in x's dtype), an Int8VOIDTensor (x int8 with
+    per-row scales ``x_scale`` [batch], or a float scalar; y fp32 unless ``out_dtype`` / ``out`` say otherwise) or an FP8BlockTensor, a dense
+    matrix in e4m3 with a scale per 128 x 128 (x floating, quantised with a scale for each token's 128 features, y in x's dtype; or x as such an
+    FP8BlockTensor, y fp32; unless ``out_dtype`` / ``out`` say otherwise).
     ``bias`` has one value per output feature; ``residual`` [batch, out] (float32, float16 or bfloat16) is added in fp32 behind the
     activation, in the same kernel.  It may be ``out`` itself: the residual stream is then updated in place (an ``out`` that shares memory with x
     costs a copy of x)."""
+    if type(a) is FP8BlockTensor:
+        return _fp8_linear(a, x, bias, activation, out, x_scale, out_dtype, residual)
     size = x.shape                                      # (attributes of tensors cost 0.1 us each, half of what this function does)
     M, K = a.shape
     assert len(size) == 2 and size[1] == K, f"Dimension mismatch: A is {a.shape}, x is {tuple(size)}"
@@ -127,6 +132,21 @@ def void_linear(a, x: torch.Tensor, bias: Optional[torch.Tensor] = None, activat
     if dtype is not _KIND_DTYPE[kind]:
         x = x.to(_KIND_DTYPE[kind])
     return _lib.native().spmm(packed.native, x, out, dtype, False, None, 1.0, None, bias, activation, True, None, residual)
+
+
+def _fp8_linear(a: FP8BlockTensor, x, bias, activation, out, x_scale, out_dtype, residual) -> torch.Tensor:
+    """void_linear with dense 8-bit weights."""
+    if x_scale is not None:
+        raise _lib.VoidB200Error("void_linear with an FP8BlockTensor takes quantised activations as an FP8BlockTensor, not with x_scale")
+    if a.n_experts is not None:
+        raise _lib.VoidB200Error("the weights of experts go with void_expert_linear")
+    size, (M, K) = x.shape, a.shape
+    assert len(size) == 2 and size[1] == K, f"Dimension mismatch: A is {a.shape}, x is {tuple(size)}"
+    if residual is not None:
+        assert residual.shape == (size[0], M), f"residual must have shape {(size[0], M)}, got {tuple(residual.shape)}"
+    if bias is not None:
+        assert bias.shape == (M,), f"bias must have shape ({M},), got {tuple(bias.shape)}"
+    return a._product(x, None, bias, activation, out, out_dtype, residual)
 
 
 def void_spmv(a: VOIDTensor, x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
