@@ -237,6 +237,11 @@ __device__ __forceinline__ float ld_cluster(uint32_t addr) {
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
   return v;
 }
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -255,11 +260,21 @@ struct Finish {
 };
 __device__ __forceinline__ void store_result(const Fp8Params& p, long long token, int m, float v) { set_element(p.out, p.out_elem, token * p.ldc + m, v); }
 
+// Zeros for tokens in no run.
+__device__ __forceinline__ void zero_tokens_in_no_run(const Fp8Params& p) {
+  if (p.head == nullptr || !p.zero_rest) return;
+  const int low = p.bounds[0], high = p.bounds[p.n_experts];
+  for (int r = (int)blockIdx.x; r < low + p.N - high; r += (int)gridDim.x) {
+    const long long token = r < low ? r : high + r - low;
+    for (int m = threadIdx.x; m < p.M; m += kThreads) store_result(p, token, m, 0.0f);
+  }
+}
+
 // NT: tokens of an item at most.
 template <int NT, int CTAS>
 __global__ void __launch_bounds__(kThreads, CTAS) fp8_block_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUtensorMap map_a,
                                                                    const __grid_constant__ CUtensorMap map_x) {
-  constexpr int CG = NT == 256 || NT == 32 ? 16 : 32;   // columns read back at a time
+  constexpr int CG = NT / 2 < 32 ? NT / 2 : 32;   // columns read back at a time
   constexpr int GROUPS = NT / 2 / CG;              // of them for one warp: every other one
   constexpr uint32_t kStageA = kBlock * kBlock, kStage = kStageA + NT * kBlock;
   constexpr uint32_t kTmem = NT * 2 < 32 ? 32 : NT * 2;
@@ -484,8 +499,11 @@ __global__ void __launch_bounds__(kThreads, CTAS) fp8_block_kernel(const __grid_
       const Finish f(p, t, m);
       const int share = (n + p.splits - 1) / p.splits, c1 = min(n, (rank + 1) * share);
       for (int c = rank * share + side; c < c1; c += 2) {
-        float v = 0.0f;
-        for (int q = 0; q < p.splits; ++q) v += ld_cluster(cluster_address(ring + (uint32_t)(c * kBlock + quad * 32 + lane) * 4u, (uint32_t)q));
+        float part[8], v = 0.0f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) part[q] = q < p.splits ? ld_cluster(cluster_address(ring + (uint32_t)(c * kBlock + quad * 32 + lane) * 4u, (uint32_t)q)) : 0.0f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v += part[q];
         if (m < p.M) {
           v = activate(v + f.bias, p.act);
           if (p.residual != nullptr) v += element(p.residual, p.residual_elem, (long long)(t.n0 + c) * p.ldr + m);
@@ -496,13 +514,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) fp8_block_kernel(const __grid_
     __syncwarp();
     cluster_meet();   // (nobody leaves while others read its sums)
   }
-  if (p.head != nullptr && p.zero_rest) {   // tokens in no run
-    const int low = p.bounds[0], high = p.bounds[p.n_experts];
-    for (int r = (int)blockIdx.x; r < low + p.N - high; r += (int)gridDim.x) {
-      const long long token = r < low ? r : high + r - low;
-      for (int m = tid; m < p.M; m += kThreads) store_result(p, token, m, 0.0f);
-    }
-  }
+  zero_tokens_in_no_run(p);
   grid_launch_dependents();
   tc_fence_before();
   __syncthreads();
@@ -517,6 +529,340 @@ __global__ void __launch_bounds__(kThreads, CTAS) fp8_block_kernel(const __grid_
   if (warp == 1) tmem_dealloc(tmem, kTmem);
 }
 
+// ------------------------------------------------------------------------------------------ many tokens
+// Tokens are the lanes here (128 of them, what a chunk lacks is multiplied for nothing), 256 features the columns: a thread that adds up has
+// one token and one block of 128 features, so that both scales are one number of its own, and its results are 128 neighbours in memory.
+// Every block of k costs an SM 512 clocks of products; reading back 256 columns and adding them takes eight warps less than that.
+constexpr int kWideTokens = 128, kWideFeatures = 256;
+constexpr uint32_t kWideStage = (kWideTokens + kWideFeatures) * kBlock;
+constexpr int kWideAhead = 4;                 // scales that are on their way, blocks of k
+constexpr int kWidePitch = kWideFeatures + 4; // of partial sums in shared memory: 16-byte pieces of eight rows meet all banks
+constexpr int kCopier = 8, kIssuer = 9, kBiasWarp = 10;
+struct __align__(8) WideBars {
+  uint64_t full[kMaxRing], empty[kMaxRing];
+  uint64_t acc_full[2], acc_empty[2], bias_full[2], bias_empty[2];
+};
+// 32 bytes of results or residuals: 16 numbers of 16 bits, or 8 of 32.
+__device__ __forceinline__ void unpack16(const uint32_t (&u)[8], int elem, float (&v)[16]) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    if (elem == VOID_ELEM_F16) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[k]));
+      v[2 * k] = f.x; v[2 * k + 1] = f.y;
+    } else {
+      v[2 * k] = __uint_as_float(u[k] << 16);
+      v[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
+    }
+  }
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, int elem) {
+  uint32_t r;
+  if (elem == VOID_ELEM_F16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+// 16 neighbouring results of a token whose rows lie on 32 bytes.
+__device__ __forceinline__ void finish16(const Fp8Params& p, long long token, int m, float (&y)[16]) {
+  if (p.residual != nullptr) {
+    const long long at = token * p.ldr + m;
+    if (p.residual_elem == VOID_ELEM_F32) {
+      const float* r = reinterpret_cast<const float*>(p.residual) + at;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t u[8];
+        ld_global_v8(r + 8 * h, u);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) y[8 * h + k] += __uint_as_float(u[k]);
+      }
+    } else {
+      uint32_t u[8];
+      float r[16];
+      ld_global_v8(reinterpret_cast<const uint16_t*>(p.residual) + at, u);
+      unpack16(u, p.residual_elem, r);
+#pragma unroll
+      for (int k = 0; k < 16; ++k) y[k] += r[k];
+    }
+  }
+  const long long at = token * p.ldc + m;
+  uint32_t u[8];
+  if (p.out_elem == VOID_ELEM_F32) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) u[k] = __float_as_uint(y[8 * h + k]);
+      st_global_v8(reinterpret_cast<float*>(p.out) + at + 8 * h, u);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) u[k] = pack2(y[2 * k], y[2 * k + 1], p.out_elem);
+    st_global_v8(reinterpret_cast<uint16_t*>(p.out) + at, u);
+  }
+}
+
+// LOOSE: rows of results or residuals that do not lie on 32 bytes.
+template <bool LOOSE>
+__global__ void __launch_bounds__(kThreads, 1) fp8_wide_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUtensorMap map_a,
+                                                               const __grid_constant__ CUtensorMap map_x) {
+  constexpr int COLS = kBlock;    // of an adding warp
+  extern __shared__ uint8_t raw[];
+  __shared__ WideBars bars;
+  __shared__ __align__(16) float bias_s[2][kWideFeatures];
+  __shared__ uint32_t tmem_s;
+  __shared__ int ctl_s[2];
+  volatile int* ctl = ctl_s;
+  const uint32_t ring = (smem_u32(raw) + 1023u) & ~1023u;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    ctl_s[0] = 0;
+    ctl_s[1] = p.wait_limit_ms;
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(smem_u32(&bars.full[s]), 1);
+      mbar_init(smem_u32(&bars.empty[s]), 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(smem_u32(&bars.acc_full[s]), 1);
+      mbar_init(smem_u32(&bars.acc_empty[s]), kAdders);
+      mbar_init(smem_u32(&bars.bias_full[s]), 1);
+      mbar_init(smem_u32(&bars.bias_empty[s]), kAdders);
+    }
+    fence_mbar_init();
+    prefetch_tmap(&map_a);
+    prefetch_tmap(&map_x);
+  }
+  if (warp == kIssuer) {
+    tmem_alloc(smem_u32(&tmem_s), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_s;
+  grid_dependency_wait();
+
+  const int rank = p.splits > 1 ? (int)cluster_rank() : 0;
+  const int b0 = (int)((long long)p.k_blocks * rank / p.splits), b1 = (int)((long long)p.k_blocks * (rank + 1) / p.splits);
+  const int step = (int)gridDim.x / p.splits, begin = (int)blockIdx.x / p.splits, end = items_of(p);
+  // (4 * 56 + 8 * 224 = 12 * 168, what the block was launched with)
+  if (warp >= kAdders) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+  if (warp == kCopier) {
+    int stage = 0;
+    uint32_t phase = 0;
+    bool first = true;
+    for (int i = begin; i < end && !ctl[0]; i += step) {
+      const Item t = item_at(p, i);
+      const int boxes = (t.n1 - t.n0 + kTokenBox - 1) / kTokenBox;
+      const int halves = p.M - t.m * kWideFeatures > kBlock ? 2 : 1;
+      for (int b = b0; b < b1; ++b) {
+        if (!mbar_wait_warp(smem_u32(&bars.empty[stage]), phase ^ 1u, ctl)) break;
+        const uint32_t full = smem_u32(&bars.full[stage]), at = ring + (uint32_t)stage * kWideStage;
+        const bool drop = first && p.drop_first != 0;
+        first = false;
+        if (lane == 0 && !drop) mbar_expect_tx(full, (uint32_t)(halves * kBlock + boxes * kTokenBox) * kBlock);
+        __syncwarp();
+        if (!drop) {
+          if (lane < halves) tma_load_a(at + kWideTokens * kBlock + (uint32_t)lane * (kBlock * kBlock), &map_a, b * kBlock, t.m * kWideFeatures + lane * kBlock, t.expert, full);
+          else if (lane >= 4 && lane < 4 + boxes)
+            tma_load_2d(at + (uint32_t)(lane - 4) * (kTokenBox * kBlock), &map_x, b * kBlock, t.n0 + (lane - 4) * kTokenBox, full);
+        }
+        if (++stage == p.stages) { stage = 0; phase ^= 1u; }
+      }
+    }
+  } else if (warp == kIssuer) {
+    constexpr uint64_t kDescHi = smem_desc_hi(16, 1024, kLayoutSw128);
+    const bool leader = elect_one();
+    int stage = 0;
+    uint32_t phase = 0, it = 0;
+    bool ok = true;
+    for (int i = begin; i < end && ok; i += step) {
+      const Item t = item_at(p, i);
+      const int left = p.M - t.m * kWideFeatures;
+      const uint32_t idesc = instr_desc(1, 0, 0, 0, 0, kWideTokens, left > kBlock ? kWideFeatures : kBlock);
+      for (int b = b0; b < b1; ++b, ++it) {
+        const uint32_t slot = it & 1u;
+        ok = mbar_wait_warp(smem_u32(&bars.acc_empty[slot]), ((it >> 1) & 1u) ^ 1u, ctl) && mbar_wait_warp(smem_u32(&bars.full[stage]), phase, ctl);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t at = ring + (uint32_t)stage * kWideStage;
+        const uint64_t dx = smem_desc(kDescHi, at), da = smem_desc(kDescHi, at + kWideTokens * kBlock);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)   // 32 features each: 32 bytes further in rows of 128
+          issue_mma<VOID_KIND_F8E4M3>(leader, tmem + slot * kWideFeatures, dx + 2 * k, da + 2 * k, idesc, k > 0);
+        tc_commit_if(leader, smem_u32(&bars.empty[stage]));
+        tc_commit_if(leader, smem_u32(&bars.acc_full[slot]));
+        if (++stage == p.stages) { stage = 0; phase ^= 1u; }
+      }
+    }
+  } else if (warp == kBiasWarp) {   // biases of an item, asked for while the one before is multiplied
+    uint32_t it = 0;
+    for (int i = begin; i < end; i += step, ++it) {
+      const Item t = item_at(p, i);
+      float v[kWideFeatures / 32];
+#pragma unroll
+      for (int k = 0; k < kWideFeatures / 32; ++k) {
+        const int m = t.m * kWideFeatures + lane + 32 * k;
+        v[k] = p.bias != nullptr && m < p.M ? element(p.bias, p.bias_elem, (long long)t.expert * p.M + m) : 0.0f;
+      }
+      if (!mbar_wait_warp(smem_u32(&bars.bias_empty[it & 1u]), ((it >> 1) & 1u) ^ 1u, ctl)) break;
+#pragma unroll
+      for (int k = 0; k < kWideFeatures / 32; ++k) bias_s[it & 1u][lane + 32 * k] = v[k];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&bars.bias_full[it & 1u]));
+    }
+  } else if (warp < kAdders) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    const int quad = warp & 3, side = warp >> 2;
+    uint32_t it = 0, item = 0;
+    bool ok = true;
+    for (int i = begin; i < end && ok; i += step, ++item) {
+      const Item t = item_at(p, i);
+      const int n = t.n1 - t.n0, token = quad * 32 + lane, m0 = t.m * kWideFeatures + side * kBlock;
+      const bool mine = token < n, any = m0 < p.M;   // (any: this half of the features is there)
+      const float* sx = p.x_scale + (long long)(t.n0 + token) * p.xs_row;
+      const float* sa = p.a_scale + t.expert * p.as_expert + (long long)(2 * t.m + side) * p.as_row;
+      float ahead_x[kWideAhead], ahead_a[kWideAhead], scale[kWideAhead];
+      auto fetch = [&](int b) {
+#pragma unroll
+        for (int k = 0; k < kWideAhead; ++k) {
+          const bool in = mine && any && b + k < b1;
+          ahead_x[k] = in ? sx[(long long)(b + k) * p.xs_col] : 0.0f;
+          ahead_a[k] = in ? sa[(long long)(b + k) * p.as_col] : 0.0f;
+        }
+      };
+      fetch(b0);
+      f32x2 sum[COLS / 2];
+#pragma unroll
+      for (int c = 0; c < COLS / 2; ++c) sum[c] = pair(0.0f, 0.0f);
+      for (int b = b0; b < b1 && ok; b += kWideAhead) {
+#pragma unroll
+        for (int k = 0; k < kWideAhead; ++k) scale[k] = ahead_x[k] * ahead_a[k];
+        if (b + kWideAhead < b1) fetch(b + kWideAhead);
+#pragma unroll 1
+        for (int k = 0; k < kWideAhead && b + k < b1; ++k, ++it) {
+          const uint32_t slot = it & 1u;
+          const float s = scale[0];
+#pragma unroll
+          for (int j = 0; j + 1 < kWideAhead; ++j) scale[j] = scale[j + 1];
+          ok = mbar_wait_warp(smem_u32(&bars.acc_full[slot]), (it >> 1) & 1u, ctl);
+          if (!ok) break;
+          tc_fence_after();
+          if (any) {
+            const uint32_t from = tmem + slot * kWideFeatures + (uint32_t)(side * COLS) + ((uint32_t)(quad * 32) << 16);
+            const f32x2 s2 = pair(s, s);
+            uint32_t r[2][32];
+            tmem_ld_32x32(from, r[0]);
+#pragma unroll
+            for (int g = 0; g < COLS / 32; ++g) {
+              tmem_ld_wait();
+              if (g + 1 < COLS / 32) tmem_ld_32x32(from + 32u * (g + 1), r[(g + 1) & 1]);
+#pragma unroll
+              for (int c = 0; c < 16; ++c)
+                sum[16 * g + c] = fma2(pair(__uint_as_float(r[g & 1][2 * c]), __uint_as_float(r[g & 1][2 * c + 1])), s2, sum[16 * g + c]);
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&bars.acc_empty[slot]));
+        }
+      }
+      if (!ok) break;
+      if (p.splits > 1) {
+        float* part = reinterpret_cast<float*>(raw + (ring - smem_u32(raw))) + token * kWidePitch + side * COLS;   // [tokens][features]
+        if (mine && any) {
+#pragma unroll
+          for (int c = 0; c < COLS / 2; c += 2) {
+            float4 v;
+            unpair(sum[c], v.x, v.y);
+            unpair(sum[c + 1], v.z, v.w);
+            *reinterpret_cast<float4*>(part + 2 * c) = v;
+          }
+        }
+        break;   // (one item per cluster)
+      }
+      ok = mbar_wait_warp(smem_u32(&bars.bias_full[item & 1u]), (item >> 1) & 1u, ctl);
+      if (!ok) break;
+      if (mine && any) {
+        const float4* bias = reinterpret_cast<const float4*>(&bias_s[item & 1u][side * COLS]);
+        const long long row = t.n0 + token;
+#pragma unroll
+        for (int c0 = 0; c0 < COLS; c0 += 16) {
+          f32x2 y2[8];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const float4 q = bias[c0 / 4 + c];
+            y2[2 * c] = add2(sum[c0 / 2 + 2 * c], pair(q.x, q.y));
+            y2[2 * c + 1] = add2(sum[c0 / 2 + 2 * c + 1], pair(q.z, q.w));
+          }
+          activate<8>(y2, p.act);
+          float y[16];
+#pragma unroll
+          for (int c = 0; c < 8; ++c) unpair(y2[c], y[2 * c], y[2 * c + 1]);
+          const int m = m0 + c0;
+          if (!LOOSE && m + 16 <= p.M) {
+            finish16(p, row, m, y);
+          } else {
+#pragma unroll
+            for (int c = 0; c < 16; ++c)
+              if (m + c < p.M) {
+                if (p.residual != nullptr) y[c] += element(p.residual, p.residual_elem, row * p.ldr + m + c);
+                store_result(p, row, m + c, y[c]);
+              }
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&bars.bias_empty[item & 1u]));
+    }
+  }
+  if (p.splits > 1) {
+    __syncwarp();
+    cluster_meet();
+    if (begin < end && warp < kAdders) {   // rows of tokens dealt to the CTAs and their warps, features to lanes
+      const Item t = item_at(p, begin);
+      const int n = t.n1 - t.n0, share = (n + p.splits - 1) / p.splits, r1 = min(n, (rank + 1) * share), m0 = t.m * kWideFeatures;
+      for (int r = rank * share + warp; r < r1; r += kAdders) {
+        for (int h = 0; h < 2; ++h) {
+          const int m = m0 + 128 * h + 4 * lane;
+          if (m >= p.M) continue;
+          const uint32_t at = ring + (uint32_t)(r * kWidePitch + 128 * h + 4 * lane) * 4u;
+          float4 part[8];
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            if (q < p.splits) part[q] = ld_cluster4(cluster_address(at, (uint32_t)q));
+          float y[4] = {part[0].x, part[0].y, part[0].z, part[0].w};
+#pragma unroll
+          for (int q = 1; q < 8; ++q)
+            if (q < p.splits) {
+              y[0] += part[q].x; y[1] += part[q].y; y[2] += part[q].z; y[3] += part[q].w;
+            }
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (m + k < p.M) {
+              if (p.bias != nullptr) y[k] += element(p.bias, p.bias_elem, (long long)t.expert * p.M + m + k);
+              y[k] = activate(y[k], p.act);
+              if (p.residual != nullptr) y[k] += element(p.residual, p.residual_elem, (long long)(t.n0 + r) * p.ldr + m + k);
+              store_result(p, t.n0 + r, m + k, y[k]);
+            }
+        }
+      }
+    }
+    __syncwarp();
+    cluster_meet();   // (nobody leaves while others read its sums)
+  }
+  zero_tokens_in_no_run(p);
+  grid_launch_dependents();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (ctl_s[0]) {   // let copies that may still be in flight land before shared memory is given back
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 200000ull) {
+    }
+    if (tid == 0 && p.status != nullptr) atomicCAS(p.status, 0, kStatusTimeout);
+    __syncthreads();
+  }
+  if (warp == kIssuer) tmem_dealloc(tmem, 512);
+}
+
 bool rows_map(CUtensorMap* m, const void* at, long long ld, long long expert, int K, int rows, int experts, int box_rows) {
   PFN_cuTensorMapEncodeTiled_v12000 enc = get_encode();
   if (enc == nullptr) return false;
@@ -528,26 +874,15 @@ bool rows_map(CUtensorMap* m, const void* at, long long ld, long long expert, in
              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int NT, int CTAS>
-int launch_fp8(Fp8Params p, const CUtensorMap& a, const CUtensorMap& x, long long items, const DeviceInfo& dev, cudaStream_t st) {
-  constexpr int kStage = kBlock * kBlock + NT * kBlock;
-  const int fixed = (int)sizeof(Fp8Bars) + kScaleSlots * NT * 4 + 64 + 1024 + 1024;   // (and what the system keeps of a CTA's)
-  p.stages = (dev.smem_per_sm / CTAS - fixed) / kStage;
-  if (p.stages > kMaxRing) p.stages = kMaxRing;
-  const int most = (dev.max_smem - fixed) / kStage;
-  if (p.stages > most) p.stages = most;
-  const int smem = p.stages * kStage + 1024;
-  if (p.stages < 2) return VOID_ERR_SHAPE;
-  const void* kernel = reinterpret_cast<const void*>(fp8_block_kernel<NT, CTAS>);
-  if (ensure_smem(kernel, smem) != 0) return VOID_ERR_CUDA;
-  const long long slots = (long long)dev.sms * CTAS;
-  // Fewer items than half the places for CTAs: the blocks of k are shared, as long as every CTA has two of them and the sums fit the ring.
+// Launch with `splits` CTAs per item, in clusters.  Fewer items than half the places for CTAs: the blocks of k are shared, as long as every CTA has two of
+// them.
+cudaError_t launch_split(void (*kernel)(Fp8Params, CUtensorMap, CUtensorMap), Fp8Params& p, const CUtensorMap& a, const CUtensorMap& x, long long items,
+                         long long places, int smem, cudaStream_t st) {
   int splits = 1;
-  while (splits < 8 && items * splits * 2 <= slots && p.k_blocks >= splits * 4 && NT * kBlock * 4 <= p.stages * kStage) splits *= 2;
+  while (splits < 8 && items * splits * 2 <= places && p.k_blocks >= splits * 4) splits *= 2;
   p.splits = splits;
-  const long long grid = splits > 1 ? items * splits : (items < slots ? items : slots);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid);
+  cfg.gridDim = dim3((unsigned)(splits > 1 ? items * splits : (items < places ? items : places)));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = st;
@@ -560,8 +895,36 @@ int launch_fp8(Fp8Params p, const CUtensorMap& a, const CUtensorMap& x, long lon
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = splits > 1 ? 2 : 1;
-  return status_of(cudaLaunchKernelEx(&cfg, fp8_block_kernel<NT, CTAS>, p, a, x));
+  return cudaLaunchKernelEx(&cfg, kernel, p, a, x);
 }
+// Stages of a ring in the shared memory that `ctas` CTAs leave each other.
+int ring_stages(const DeviceInfo& dev, int ctas, int stage_bytes, int fixed) {
+  fixed += 64 + 1024 + 1024;   // (alignment, and what the system keeps of a CTA's)
+  int stages = (dev.smem_per_sm / ctas - fixed) / stage_bytes;
+  const int most = (dev.max_smem - fixed) / stage_bytes;
+  if (stages > most) stages = most;
+  return stages > kMaxRing ? kMaxRing : stages;
+}
+template <int NT, int CTAS>
+int launch_few(Fp8Params p, const CUtensorMap& a, const CUtensorMap& x, long long items, const DeviceInfo& dev, cudaStream_t st) {
+  constexpr int kStage = kBlock * kBlock + NT * kBlock;
+  static_assert(NT * kBlock * 4 <= 2 * kStage, "the partial sums lie in the ring");
+  p.stages = ring_stages(dev, CTAS, kStage, (int)sizeof(Fp8Bars) + kScaleSlots * NT * 4);
+  const int smem = p.stages * kStage + 1024;
+  if (p.stages < 2) return VOID_ERR_SHAPE;
+  if (ensure_smem(reinterpret_cast<const void*>(fp8_block_kernel<NT, CTAS>), smem) != 0) return VOID_ERR_CUDA;
+  return status_of(launch_split(fp8_block_kernel<NT, CTAS>, p, a, x, items, (long long)dev.sms * CTAS, smem, st));
+}
+template <bool LOOSE>
+int launch_wide(Fp8Params p, const CUtensorMap& a, const CUtensorMap& x, long long items, const DeviceInfo& dev, cudaStream_t st) {
+  p.stages = ring_stages(dev, 1, (int)kWideStage, (int)sizeof(WideBars) + 2 * kWideFeatures * 4);
+  const int smem = p.stages * (int)kWideStage + 1024;
+  if (p.stages * (int)kWideStage < kWideTokens * kWidePitch * 4) return VOID_ERR_SHAPE;
+  if (ensure_smem(reinterpret_cast<const void*>(fp8_wide_kernel<LOOSE>), smem) != 0) return VOID_ERR_CUDA;
+  return status_of(launch_split(fp8_wide_kernel<LOOSE>, p, a, x, items, dev.sms, smem, st));
+}
+// Rows of results and residuals in pieces of 32 bytes.
+bool on_32_bytes(const void* at, long long ld, int elem) { return ((reinterpret_cast<uintptr_t>(at) | (uintptr_t)(ld * (elem == VOID_ELEM_F32 ? 4 : 2))) & 31u) == 0; }
 
 int fp8_linear(const void_fp8_args* a, const void_experts* x, cudaStream_t st) {
   if (a == nullptr || a->M < 0 || a->K < 0 || a->N < 0) return VOID_ERR_BAD_ARG;
@@ -570,7 +933,7 @@ int fp8_linear(const void_fp8_args* a, const void_experts* x, cudaStream_t st) {
     return VOID_ERR_BAD_ARG;
   if (a->M == 0 || a->N == 0) return VOID_OK;
   if (a->out == nullptr || a->K == 0 || a->a == nullptr || a->x == nullptr || a->a_scale == nullptr || a->x_scale == nullptr) return VOID_ERR_BAD_ARG;
-  if (x != nullptr && (x->n_experts < 1 || x->plan == nullptr || x->offset_bytes != 0 || (x->chunk != 32 && x->chunk != 64 && x->chunk != 128 && x->chunk != 256)))
+  if (x != nullptr && (x->n_experts < 1 || x->plan == nullptr || x->offset_bytes != 0 || (x->chunk != 32 && x->chunk != 64 && x->chunk != 128)))
     return VOID_ERR_BAD_ARG;
   if (a->ldc < a->M || (a->residual != nullptr && a->ldr < a->M)) return VOID_ERR_SHAPE;
   if ((reinterpret_cast<uintptr_t>(a->a) & 15u) != 0 || (reinterpret_cast<uintptr_t>(a->x) & 15u) != 0 || (a->lda & 15) != 0 || (a->ldx & 15) != 0 ||
@@ -582,7 +945,6 @@ int fp8_linear(const void_fp8_args* a, const void_experts* x, cudaStream_t st) {
   Fp8Params p = {};
   p.M = a->M; p.K = a->K; p.N = a->N;
   p.k_blocks = (a->K + kBlock - 1) / kBlock;
-  p.m_tiles = (a->M + kBlock - 1) / kBlock;
   p.a_scale = a->a_scale; p.as_row = a->a_scale_row; p.as_col = a->a_scale_col; p.as_expert = a->a_scale_expert;
   p.x_scale = a->x_scale; p.xs_row = a->x_scale_row; p.xs_col = a->x_scale_col;
   p.bias = a->bias; p.bias_elem = a->bias_elem;
@@ -591,22 +953,21 @@ int fp8_linear(const void_fp8_args* a, const void_experts* x, cudaStream_t st) {
   p.status = a->status;
   p.wait_limit_ms = (a->test_hooks & 0xffff) ? (a->test_hooks & 0xffff) : kDefaultWaitLimitMs;
   p.drop_first = (a->test_hooks >> 16) & 1;
+  // Up to 64 tokens lie in the columns of the tensor memory, more of them in its lanes.
+  const int chunk = x != nullptr ? x->chunk : (a->N <= 32 ? 32 : (a->N <= 64 ? 64 : kWideTokens));
+  const bool wide = chunk == kWideTokens;
+  p.m_tiles = wide ? (a->M + kWideFeatures - 1) / kWideFeatures : (a->M + kBlock - 1) / kBlock;
   long long chunks;
-  int most;   // tokens of an item
   if (x != nullptr) {
     const PlanView v = plan_of(*x, a->N);
     p.head = v.head; p.bounds = v.bounds; p.chunks = v.chunks;
     p.n_experts = x->n_experts;
     p.zero_rest = x->zero_rest;
     chunks = v.capacity;
-    most = x->chunk;
   } else {
-    chunks = ((long long)a->N + 255) / 256;
-    p.chunk = (int)((a->N + chunks - 1) / chunks + 15) / 16 * 16;
-    p.n_chunks = (int)((a->N + p.chunk - 1) / p.chunk);
-    p.group = 8;
-    chunks = p.n_chunks;
-    most = p.chunk;
+    p.chunk = chunk;
+    chunks = p.n_chunks = (int)(((long long)a->N + chunk - 1) / chunk);
+    p.group = 16;
   }
   const long long items = chunks * p.m_tiles;
   if (items > 0x3fffffff) return VOID_ERR_TOO_LARGE;
@@ -615,10 +976,12 @@ int fp8_linear(const void_fp8_args* a, const void_experts* x, cudaStream_t st) {
   if (!rows_map(&map_a, a->a, a->lda, x != nullptr ? a->expert_stride : (a->lda * a->M + 15) / 16 * 16, a->K, a->M, experts, kBlock) ||
       !rows_map(&map_x, a->x, a->ldx, 0, a->K, a->N, 0, kTokenBox))
     return VOID_ERR_TENSOR_MAP;
-  if (most <= 32) return launch_fp8<32, 2>(p, map_a, map_x, items, dev, st);
-  if (most <= 64) return launch_fp8<64, 2>(p, map_a, map_x, items, dev, st);
-  if (most <= 128) return launch_fp8<128, 1>(p, map_a, map_x, items, dev, st);
-  return launch_fp8<256, 1>(p, map_a, map_x, items, dev, st);
+  if (wide) {
+    const bool loose = !on_32_bytes(a->out, a->ldc, a->out_elem) || (a->residual != nullptr && !on_32_bytes(a->residual, a->ldr, a->residual_elem));
+    return loose ? launch_wide<true>(p, map_a, map_x, items, dev, st) : launch_wide<false>(p, map_a, map_x, items, dev, st);
+  }
+  if (chunk == 32) return launch_few<32, 2>(p, map_a, map_x, items, dev, st);
+  return launch_few<64, 2>(p, map_a, map_x, items, dev, st);
 }
 
 }  // namespace

@@ -2287,7 +2287,7 @@ PyObject* quant_fp8_blocks(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // Tokens of a work item, by those an expert has on average.
 int32_t fp8_chunk(int64_t rows, int64_t experts) {
   const int64_t each = (rows + experts - 1) / experts;
-  return each <= 24 ? 32 : (each <= 48 ? 64 : (each <= 96 ? 128 : 256));
+  return each <= 24 ? 32 : (each <= 64 ? 64 : 128);
 }
 // fp8_linear(values, scales, x, x_scales | None, offsets | None, bias | None, act, out | None, out_dtype, residual | None, status) -> out
 // values [M, K] or (with offsets) [experts, M, K] in e4m3; x [N, K] in e4m3 with x_scales, or floating: quantised first
