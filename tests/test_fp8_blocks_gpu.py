@@ -111,7 +111,7 @@ def _weights(m, k, seed):
 
 SIZES = [(1, 1, 1), (1, 128, 128), (2, 130, 17), (15, 128, 300), (16, 256, 256), (17, 100, 500), (31, 513, 129), (32, 1000, 640), (33, 128, 2048), (64, 300, 1030),
          (65, 260, 128), (100, 129, 777), (128, 128, 1024), (129, 384, 4096), (200, 255, 256), (256, 256, 128), (257, 140, 300), (300, 2500, 3000),
-         (512, 130, 200), (513, 1, 129), (700, 4100, 257), (1111, 640, 640), (3, 20000, 400), (4, 128, 30000)]
+         (512, 130, 200), (513, 1, 129), (700, 4100, 257), (1500, 2001, 300), (2100, 2064, 300), (1111, 640, 640), (3, 20000, 400), (4, 128, 30000)]
 
 
 @pytest.mark.parametrize("n, m, k", SIZES)
@@ -195,7 +195,7 @@ def test_results_that_are_given():
 
 EXPERTS = [  # runs, rows behind them, M, K
     ([1], 0, 128, 128), ([0, 0, 3], 0, 130, 200), ([5, 0, 40, 1], 7, 300, 257), ([100, 30, 0, 200], 0, 256, 512), ([300, 260, 1, 0, 15], 13, 140, 300),
-    ([0, 0], 20, 128, 256), ([700, 2, 600], 1, 260, 640), ([17] * 40, 3, 64, 128), ([1] * 70, 0, 200, 384), ([0] * 5 + [513], 0, 129, 129)]
+    ([0, 0], 20, 128, 256), ([700, 2, 600], 1, 260, 640), ([900, 0, 333], 40, 2001, 200), ([17] * 40, 3, 64, 128), ([1] * 70, 0, 200, 384), ([0] * 5 + [513], 0, 129, 129)]
 
 
 @pytest.mark.parametrize("runs, spare, m, k", EXPERTS)

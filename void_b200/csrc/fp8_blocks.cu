@@ -225,7 +225,6 @@ __device__ __forceinline__ Item item_at(const Fp8Params& p, int i) {
   t.n1 = t.n0 + p.chunk < p.N ? t.n0 + p.chunk : p.N;
   return t;
 }
-__device__ __forceinline__ void tma_load_a(uint32_t dst, const CUtensorMap* m, int x, int y, int z, uint32_t bar) { tma_load_3d(dst, m, x, y, z, bar); }
 
 __device__ __forceinline__ uint32_t cluster_address(uint32_t addr, uint32_t rank) {
   uint32_t r;
@@ -251,14 +250,15 @@ __device__ __forceinline__ void cluster_meet() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// What is between a sum and the result, for one lane's feature.
-struct Finish {
-  float bias;
-  __device__ __forceinline__ Finish(const Fp8Params& p, const Item& t, int m) {
-    bias = p.bias != nullptr && m < p.M ? element(p.bias, p.bias_elem, (long long)t.expert * p.M + m) : 0.0f;
+__device__ __forceinline__ void store_result(const Fp8Params& p, long long token, int m, float v) {
+  const long long at = token * p.ldc + m;
+  if (p.out_elem == VOID_ELEM_F32) {
+    reinterpret_cast<float*>(p.out)[at] = v;
+  } else {
+    const unsigned short h = p.out_elem == VOID_ELEM_F16 ? __half_as_ushort(__float2half_rn(v)) : __bfloat16_as_ushort(__float2bfloat16_rn(v));
+    reinterpret_cast<unsigned short*>(p.out)[at] = h;
   }
-};
-__device__ __forceinline__ void store_result(const Fp8Params& p, long long token, int m, float v) { set_element(p.out, p.out_elem, token * p.ldc + m, v); }
+}
 
 // Zeros for tokens in no run.
 __device__ __forceinline__ void zero_tokens_in_no_run(const Fp8Params& p) {
@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) fp8_block_kernel(const __grid_
         if (lane == 0 && !drop) mbar_expect_tx(full, kStageA + (uint32_t)boxes * (kTokenBox * kBlock));
         __syncwarp();
         if (!drop) {
-          if (lane == 0) tma_load_a(at, &map_a, b * kBlock, t.m * kBlock, t.expert, full);
+          if (lane == 0) tma_load_3d(at, &map_a, b * kBlock, t.m * kBlock, t.expert, full);
           if (lane >= 1 && lane <= boxes)
             tma_load_2d(at + kStageA + (uint32_t)(lane - 1) * (kTokenBox * kBlock), &map_x, b * kBlock, t.n0 + (lane - 1) * kTokenBox, full);
         }
@@ -406,6 +406,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) fp8_block_kernel(const __grid_
     for (int i = begin; i < end && ok; i += step) {
       const Item t = item_at(p, i);
       const int n = t.n1 - t.n0, m = t.m * kBlock + quad * 32 + lane;
+      const uint32_t bias_raw = p.bias != nullptr && m < p.M ? raw_element(p.bias, p.bias_elem, (long long)t.expert * p.M + m) : 0u;
       f32x2 sum[GROUPS][CG / 2];
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g)
@@ -459,29 +460,29 @@ __global__ void __launch_bounds__(kThreads, CTAS) fp8_block_kernel(const __grid_
         break;   // (one item per cluster)
       }
       if (m < p.M) {
-        const Finish f(p, t, m);
+        const float bias = of_raw(bias_raw, p.bias_elem);
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g) {
           const int c0 = (2 * g + side) * CG;
           if (c0 < n) {
             f32x2 y[CG / 2];
 #pragma unroll
-            for (int c = 0; c < CG / 2; ++c) y[c] = add2(sum[g][c], pair(f.bias, f.bias));
+            for (int c = 0; c < CG / 2; ++c) y[c] = add2(sum[g][c], pair(bias, bias));
             activate<CG / 2>(y, p.act);
             const long long token = t.n0 + c0;
 #pragma unroll
             for (int h = 0; h < CG; h += 8) {   // eight residuals on their way together
-              float r[8];
+              uint32_t res[8];
 #pragma unroll
               for (int c = 0; c < 8; ++c)
-                r[c] = p.residual != nullptr && c0 + h + c < n ? element(p.residual, p.residual_elem, (token + h + c) * p.ldr + m) : 0.0f;
+                res[c] = p.residual != nullptr && c0 + h + c < n ? raw_element(p.residual, p.residual_elem, (token + h + c) * p.ldr + m) : 0u;
 #pragma unroll
-              for (int c = 0; c < 8; c += 2) {
+              for (int c = 0; c < 8; ++c) {
                 float a, d;
                 unpair(y[(h + c) / 2], a, d);
-                if (p.residual != nullptr) { a += r[c]; d += r[c + 1]; }
-                if (c0 + h + c < n) store_result(p, token + h + c, m, a);
-                if (c0 + h + c + 1 < n) store_result(p, token + h + c + 1, m, d);
+                float v = c % 2 ? d : a;
+                if (p.residual != nullptr) v += of_raw(res[c], p.residual_elem);
+                if (c0 + h + c < n) store_result(p, token + h + c, m, v);
               }
             }
           }
@@ -494,21 +495,35 @@ __global__ void __launch_bounds__(kThreads, CTAS) fp8_block_kernel(const __grid_
     __syncwarp();
     cluster_meet();
     if (begin < end && warp >= kFirstAdder) {
+      constexpr int HELD = 4;   // tokens whose sums and residuals are on their way together
       const Item t = item_at(p, begin);
       const int n = t.n1 - t.n0, quad = warp & 3, side = (warp - kFirstAdder) >> 2, m = t.m * kBlock + quad * 32 + lane;
-      const Finish f(p, t, m);
       const int share = (n + p.splits - 1) / p.splits, c1 = min(n, (rank + 1) * share);
-      for (int c = rank * share + side; c < c1; c += 2) {
-        float part[8], v = 0.0f;
+      const uint32_t bias_raw = p.bias != nullptr && m < p.M ? raw_element(p.bias, p.bias_elem, (long long)t.expert * p.M + m) : 0u;
+      for (int c0 = rank * share + side; c0 < c1; c0 += 2 * HELD) {
+        uint32_t res[HELD];
+        float v[HELD];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) part[q] = q < p.splits ? ld_cluster(cluster_address(ring + (uint32_t)(c * kBlock + quad * 32 + lane) * 4u, (uint32_t)q)) : 0.0f;
-#pragma unroll
-        for (int q = 0; q < 8; ++q) v += part[q];
-        if (m < p.M) {
-          v = activate(v + f.bias, p.act);
-          if (p.residual != nullptr) v += element(p.residual, p.residual_elem, (long long)(t.n0 + c) * p.ldr + m);
-          store_result(p, t.n0 + c, m, v);
+        for (int k = 0; k < HELD; ++k) {
+          v[k] = 0.0f;
+          res[k] = p.residual != nullptr && m < p.M && c0 + 2 * k < c1 ? raw_element(p.residual, p.residual_elem, (long long)(t.n0 + c0 + 2 * k) * p.ldr + m) : 0u;
         }
+#pragma unroll 2
+        for (int q = 0; q < p.splits; ++q) {
+          float part[HELD];
+#pragma unroll
+          for (int k = 0; k < HELD; ++k)
+            part[k] = ld_cluster(cluster_address(ring + (uint32_t)(min(c0 + 2 * k, c1 - 1) * kBlock + quad * 32 + lane) * 4u, (uint32_t)q));
+#pragma unroll
+          for (int k = 0; k < HELD; ++k) v[k] += part[k];
+        }
+#pragma unroll
+        for (int k = 0; k < HELD; ++k)
+          if (m < p.M && c0 + 2 * k < c1) {
+            float y = activate(v[k] + of_raw(bias_raw, p.bias_elem), p.act);
+            if (p.residual != nullptr) y += of_raw(res[k], p.residual_elem);
+            store_result(p, t.n0 + c0 + 2 * k, m, y);
+          }
       }
     }
     __syncwarp();
@@ -530,59 +545,43 @@ __global__ void __launch_bounds__(kThreads, CTAS) fp8_block_kernel(const __grid_
 }
 
 // ------------------------------------------------------------------------------------------ many tokens
-// Tokens are the lanes here (128 of them, what a chunk lacks is multiplied for nothing), 256 features the columns: a thread that adds up has
-// one token and one block of 128 features, so that both scales are one number of its own, and its results are 128 neighbours in memory.
-// Every block of k costs an SM 512 clocks of products; reading back 256 columns and adding them takes eight warps less than that.
+// Tokens are the lanes here, 256 features the columns: a thread that adds up has one token and one block of 128 features, so that both
+// scales are one number of its own, and its results are 128 neighbours in memory.  Eight warps read an accumulator back and add it while the
+// tensor cores fill the other one; they hold 128 sums a thread, which takes registers from the other warps (setmaxnreg).
 constexpr int kWideTokens = 128, kWideFeatures = 256;
-constexpr uint32_t kWideStage = (kWideTokens + kWideFeatures) * kBlock;
 constexpr int kWideAhead = 4;                 // scales that are on their way, blocks of k
 constexpr int kWidePitch = kWideFeatures + 4; // of partial sums in shared memory: 16-byte pieces of eight rows meet all banks
 constexpr int kCopier = 8, kIssuer = 9, kBiasWarp = 10;
+constexpr uint32_t kWideStage = (kWideTokens + kWideFeatures) * kBlock;
 struct __align__(8) WideBars {
   uint64_t full[kMaxRing], empty[kMaxRing];
   uint64_t acc_full[2], acc_empty[2], bias_full[2], bias_empty[2];
 };
-// 32 bytes of results or residuals: 16 numbers of 16 bits, or 8 of 32.
-__device__ __forceinline__ void unpack16(const uint32_t (&u)[8], int elem, float (&v)[16]) {
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    if (elem == VOID_ELEM_F16) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[k]));
-      v[2 * k] = f.x; v[2 * k + 1] = f.y;
-    } else {
-      v[2 * k] = __uint_as_float(u[k] << 16);
-      v[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
-    }
-  }
-}
 __device__ __forceinline__ uint32_t pack2(float a, float b, int elem) {
   uint32_t r;
   if (elem == VOID_ELEM_F16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
   else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
   return r;
 }
-// 16 neighbouring results of a token whose rows lie on 32 bytes.
-__device__ __forceinline__ void finish16(const Fp8Params& p, long long token, int m, float (&y)[16]) {
-  if (p.residual != nullptr) {
-    const long long at = token * p.ldr + m;
-    if (p.residual_elem == VOID_ELEM_F32) {
-      const float* r = reinterpret_cast<const float*>(p.residual) + at;
+// Adds 16 residuals, a piece of 32 bytes or (fp32) two, to 16 results.
+__device__ __forceinline__ void add_residual(float (&y)[16], const uint32_t (&u)[8], const uint32_t (&v)[8], int elem) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t u[8];
-        ld_global_v8(r + 8 * h, u);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) y[8 * h + k] += __uint_as_float(u[k]);
-      }
+  for (int k = 0; k < 8; ++k) {
+    if (elem == VOID_ELEM_F32) {
+      y[k] += __uint_as_float(u[k]);
+      y[8 + k] += __uint_as_float(v[k]);
+    } else if (elem == VOID_ELEM_F16) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[k]));
+      y[2 * k] += f.x;
+      y[2 * k + 1] += f.y;
     } else {
-      uint32_t u[8];
-      float r[16];
-      ld_global_v8(reinterpret_cast<const uint16_t*>(p.residual) + at, u);
-      unpack16(u, p.residual_elem, r);
-#pragma unroll
-      for (int k = 0; k < 16; ++k) y[k] += r[k];
+      y[2 * k] += __uint_as_float(u[k] << 16);
+      y[2 * k + 1] += __uint_as_float(u[k] & 0xffff0000u);
     }
   }
+}
+// 16 neighbouring results of a row that lies on 32 bytes.
+__device__ __forceinline__ void store16(const Fp8Params& p, long long token, int m, const float (&y)[16]) {
   const long long at = token * p.ldc + m;
   uint32_t u[8];
   if (p.out_elem == VOID_ELEM_F32) {
@@ -599,6 +598,96 @@ __device__ __forceinline__ void finish16(const Fp8Params& p, long long token, in
   }
 }
 
+// A cluster's sums meet: its tokens are dealt to the CTAs, halves of their rows to the adding warps, features to lanes.  The pieces of four halves, of one CTA
+// after the other, are on their way together.  Four features of a lane lie side by side, or (LOOSE) 32 apart, so that neighbours in memory are
+// neighbouring lanes' either way.
+template <bool LOOSE>
+__device__ __forceinline__ void add_parts(const Fp8Params& p, const Item& t, uint32_t ring, int rank, int warp, int lane) {
+  constexpr int HELD = 4, APART = LOOSE ? 32 : 1;
+  const int n = t.n1 - t.n0, share = (n + p.splits - 1) / p.splits, r0 = rank * share, r1 = min(n, r0 + share), units = (r1 - r0) * 2;
+  const int half = warp & 1, f0 = half * kBlock + (LOOSE ? lane : 4 * lane), m = t.m * kWideFeatures + f0;
+  bool in[4];
+  uint32_t bias[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    in[c] = m + c * APART < p.M;
+    bias[c] = in[c] && p.bias != nullptr ? raw_element(p.bias, p.bias_elem, (long long)t.expert * p.M + m + c * APART) : 0u;
+  }
+  const bool whole = !LOOSE && m + 4 <= p.M;   // (then rows lie on 32 bytes: four results are one store)
+  for (int u0 = warp; u0 < units; u0 += kAdders * HELD) {   // (units of one warp are all first halves, or all second ones)
+    float y[HELD][4];
+    uint32_t res[HELD][4];
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) {
+      const int u = u0 + k * kAdders;
+      const long long at = (long long)(t.n0 + r0 + u / 2) * p.ldr + m;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        y[k][c] = 0.0f;
+        res[k][c] = 0u;
+      }
+      if (p.residual == nullptr || u >= units) continue;
+      if (whole && p.residual_elem != VOID_ELEM_F32) {
+        const uint2 v = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p.residual) + at);
+        res[k][0] = v.x & 0xffffu; res[k][1] = v.x >> 16; res[k][2] = v.y & 0xffffu; res[k][3] = v.y >> 16;
+      } else if (whole) {
+        const uint4 v = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(p.residual) + at);
+        res[k][0] = v.x; res[k][1] = v.y; res[k][2] = v.z; res[k][3] = v.w;
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (in[c]) res[k][c] = raw_element(p.residual, p.residual_elem, at + c * APART);
+      }
+    }
+#pragma unroll 2
+    for (int q = 0; q < p.splits; ++q) {
+      float part[HELD][4];
+#pragma unroll
+      for (int k = 0; k < HELD; ++k) {
+        const int row = r0 + min(u0 + k * kAdders, units - 1) / 2;
+        const uint32_t from = cluster_address(ring + (uint32_t)(row * kWidePitch + f0) * 4u, (uint32_t)q);
+        if constexpr (LOOSE) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) part[k][c] = ld_cluster(from + 128u * c);
+        } else {
+          const float4 v = ld_cluster4(from);
+          part[k][0] = v.x; part[k][1] = v.y; part[k][2] = v.z; part[k][3] = v.w;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < HELD; ++k)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) y[k][c] += part[k][c];
+    }
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) {
+      const int u = u0 + k * kAdders;
+      if (u >= units) continue;
+      f32x2 z[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        z[c] = add2(pair(y[k][2 * c], y[k][2 * c + 1]), pair(of_raw(bias[2 * c], p.bias_elem), of_raw(bias[2 * c + 1], p.bias_elem)));
+      activate<2>(z, p.act);
+      float v[4];
+      unpair(z[0], v[0], v[1]);
+      unpair(z[1], v[2], v[3]);
+      if (p.residual != nullptr) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[c] += of_raw(res[k][c], p.residual_elem);
+      }
+      const long long token = t.n0 + r0 + u / 2, at = token * p.ldc + m;
+      if (whole && p.out_elem == VOID_ELEM_F32)
+        *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + at) = make_float4(v[0], v[1], v[2], v[3]);
+      else if (whole)
+        *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.out) + at) = make_uint2(pack2(v[0], v[1], p.out_elem), pack2(v[2], v[3], p.out_elem));
+      else
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (in[c]) store_result(p, token, m + c * APART, v[c]);
+    }
+  }
+}
+
 // LOOSE: rows of results or residuals that do not lie on 32 bytes.
 template <bool LOOSE>
 __global__ void __launch_bounds__(kThreads, 1) fp8_wide_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUtensorMap map_a,
@@ -607,6 +696,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_wide_kernel(const __grid_cons
   extern __shared__ uint8_t raw[];
   __shared__ WideBars bars;
   __shared__ __align__(16) float bias_s[2][kWideFeatures];
+  __shared__ float strips[kAdders][32 * 17];   // results of a warp on their way from lanes that are tokens to lanes that are features
   __shared__ uint32_t tmem_s;
   __shared__ int ctl_s[2];
   volatile int* ctl = ctl_s;
@@ -650,8 +740,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_wide_kernel(const __grid_cons
     bool first = true;
     for (int i = begin; i < end && !ctl[0]; i += step) {
       const Item t = item_at(p, i);
-      const int boxes = (t.n1 - t.n0 + kTokenBox - 1) / kTokenBox;
-      const int halves = p.M - t.m * kWideFeatures > kBlock ? 2 : 1;
+      const int boxes = (t.n1 - t.n0 + kTokenBox - 1) / kTokenBox, m0 = t.m * kWideFeatures, halves = p.M - m0 > kBlock ? 2 : 1;
       for (int b = b0; b < b1; ++b) {
         if (!mbar_wait_warp(smem_u32(&bars.empty[stage]), phase ^ 1u, ctl)) break;
         const uint32_t full = smem_u32(&bars.full[stage]), at = ring + (uint32_t)stage * kWideStage;
@@ -660,7 +749,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_wide_kernel(const __grid_cons
         if (lane == 0 && !drop) mbar_expect_tx(full, (uint32_t)(halves * kBlock + boxes * kTokenBox) * kBlock);
         __syncwarp();
         if (!drop) {
-          if (lane < halves) tma_load_a(at + kWideTokens * kBlock + (uint32_t)lane * (kBlock * kBlock), &map_a, b * kBlock, t.m * kWideFeatures + lane * kBlock, t.expert, full);
+          if (lane < halves) tma_load_3d(at + kWideTokens * kBlock + (uint32_t)lane * (kBlock * kBlock), &map_a, b * kBlock, m0 + lane * kBlock, t.expert, full);
           else if (lane >= 4 && lane < 4 + boxes)
             tma_load_2d(at + (uint32_t)(lane - 4) * (kTokenBox * kBlock), &map_x, b * kBlock, t.n0 + (lane - 4) * kTokenBox, full);
         }
@@ -675,11 +764,10 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_wide_kernel(const __grid_cons
     bool ok = true;
     for (int i = begin; i < end && ok; i += step) {
       const Item t = item_at(p, i);
-      const int left = p.M - t.m * kWideFeatures;
-      const uint32_t idesc = instr_desc(1, 0, 0, 0, 0, kWideTokens, left > kBlock ? kWideFeatures : kBlock);
+      const uint32_t idesc = instr_desc(1, 0, 0, 0, 0, kWideTokens, p.M - t.m * kWideFeatures > kBlock ? kWideFeatures : kBlock);
       for (int b = b0; b < b1; ++b, ++it) {
         const uint32_t slot = it & 1u;
-        ok = mbar_wait_warp(smem_u32(&bars.acc_empty[slot]), ((it >> 1) & 1u) ^ 1u, ctl) && mbar_wait_warp(smem_u32(&bars.full[stage]), phase, ctl);
+        ok = mbar_wait_warp(smem_u32(&bars.full[stage]), phase, ctl) && mbar_wait_warp(smem_u32(&bars.acc_empty[slot]), ((it >> 1) & 1u) ^ 1u, ctl);
         if (!ok) break;
         tc_fence_after();
         const uint32_t at = ring + (uint32_t)stage * kWideStage;
@@ -694,7 +782,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_wide_kernel(const __grid_cons
     }
   } else if (warp == kBiasWarp) {   // biases of an item, asked for while the one before is multiplied
     uint32_t it = 0;
-    for (int i = begin; i < end; i += step, ++it) {
+    for (int i = begin; i < end && p.splits == 1; i += step, ++it) {
       const Item t = item_at(p, i);
       float v[kWideFeatures / 32];
 #pragma unroll
@@ -715,9 +803,10 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_wide_kernel(const __grid_cons
     bool ok = true;
     for (int i = begin; i < end && ok; i += step, ++item) {
       const Item t = item_at(p, i);
-      const int n = t.n1 - t.n0, token = quad * 32 + lane, m0 = t.m * kWideFeatures + side * kBlock;
-      const bool mine = token < n, any = m0 < p.M;   // (any: this half of the features is there)
-      const float* sx = p.x_scale + (long long)(t.n0 + token) * p.xs_row;
+      const int n = t.n1 - t.n0, token = quad * 32 + lane, m0 = t.m * kWideFeatures + side * COLS;
+      const bool mine = token < n, any = m0 < p.M && quad * 32 < n;   // (any: of what this warp reads back)
+      const long long row = t.n0 + token;
+      const float* sx = p.x_scale + row * p.xs_row;
       const float* sa = p.a_scale + t.expert * p.as_expert + (long long)(2 * t.m + side) * p.as_row;
       float ahead_x[kWideAhead], ahead_a[kWideAhead], scale[kWideAhead];
       auto fetch = [&](int b) {
@@ -729,9 +818,14 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_wide_kernel(const __grid_cons
         }
       };
       fetch(b0);
-      f32x2 sum[COLS / 2];
+      if (mine && any && p.residual != nullptr) {   // on its way into the second cache while the products are made
+        const int es = p.residual_elem == VOID_ELEM_F32 ? 4 : 2, bytes = (p.M - m0 < COLS ? p.M - m0 : COLS) * es;
+        const uint8_t* from = reinterpret_cast<const uint8_t*>(p.residual) + (row * p.ldr + m0) * es;
+        for (int at = 0; at < bytes; at += 128) prefetch_l2(from + at);
+      }
+      float sum[COLS];   // (pairs of numbers in one instruction read three pairs of registers: half as fast as this)
 #pragma unroll
-      for (int c = 0; c < COLS / 2; ++c) sum[c] = pair(0.0f, 0.0f);
+      for (int c = 0; c < COLS; ++c) sum[c] = 0.0f;
       for (int b = b0; b < b1 && ok; b += kWideAhead) {
 #pragma unroll
         for (int k = 0; k < kWideAhead; ++k) scale[k] = ahead_x[k] * ahead_a[k];
@@ -741,27 +835,30 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_wide_kernel(const __grid_cons
           const uint32_t slot = it & 1u;
           const float s = scale[0];
 #pragma unroll
-          for (int j = 0; j + 1 < kWideAhead; ++j) scale[j] = scale[j + 1];
+          for (int q = 0; q + 1 < kWideAhead; ++q) scale[q] = scale[q + 1];
           ok = mbar_wait_warp(smem_u32(&bars.acc_full[slot]), (it >> 1) & 1u, ctl);
           if (!ok) break;
           tc_fence_after();
+          auto hand_back = [&] {   // all is read back: the next product may begin
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&bars.acc_empty[slot]));
+          };
           if (any) {
             const uint32_t from = tmem + slot * kWideFeatures + (uint32_t)(side * COLS) + ((uint32_t)(quad * 32) << 16);
-            const f32x2 s2 = pair(s, s);
             uint32_t r[2][32];
             tmem_ld_32x32(from, r[0]);
 #pragma unroll
             for (int g = 0; g < COLS / 32; ++g) {
               tmem_ld_wait();
               if (g + 1 < COLS / 32) tmem_ld_32x32(from + 32u * (g + 1), r[(g + 1) & 1]);
+              else hand_back();
 #pragma unroll
-              for (int c = 0; c < 16; ++c)
-                sum[16 * g + c] = fma2(pair(__uint_as_float(r[g & 1][2 * c]), __uint_as_float(r[g & 1][2 * c + 1])), s2, sum[16 * g + c]);
+              for (int c = 0; c < 32; ++c) sum[32 * g + c] = fmaf(__uint_as_float(r[g & 1][c]), s, sum[32 * g + c]);
             }
+          } else {
+            hand_back();
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&bars.acc_empty[slot]));
         }
       }
       if (!ok) break;
@@ -769,83 +866,82 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_wide_kernel(const __grid_cons
         float* part = reinterpret_cast<float*>(raw + (ring - smem_u32(raw))) + token * kWidePitch + side * COLS;   // [tokens][features]
         if (mine && any) {
 #pragma unroll
-          for (int c = 0; c < COLS / 2; c += 2) {
-            float4 v;
-            unpair(sum[c], v.x, v.y);
-            unpair(sum[c + 1], v.z, v.w);
-            *reinterpret_cast<float4*>(part + 2 * c) = v;
-          }
+          for (int c = 0; c < COLS; c += 4) *reinterpret_cast<float4*>(part + c) = make_float4(sum[c], sum[c + 1], sum[c + 2], sum[c + 3]);
         }
         break;   // (one item per cluster)
       }
       ok = mbar_wait_warp(smem_u32(&bars.bias_full[item & 1u]), (item >> 1) & 1u, ctl);
       if (!ok) break;
-      if (mine && any) {
+      if (any) {
         const float4* bias = reinterpret_cast<const float4*>(&bias_s[item & 1u][side * COLS]);
-        const long long row = t.n0 + token;
+        const int pieces = p.residual_elem == VOID_ELEM_F32 ? 2 : 1;   // of 32 bytes, of 16 residuals
+        const uint8_t* from = reinterpret_cast<const uint8_t*>(p.residual) + (row * p.ldr + m0) * (pieces == 2 ? 4 : 2);
+        uint32_t res[4][8];   // four pieces of residuals on their way together: of 64 results, or (fp32) of 32
+        auto fetch_residuals = [&](int c0, int width) {
 #pragma unroll
-        for (int c0 = 0; c0 < COLS; c0 += 16) {
-          f32x2 y2[8];
+          for (int q = 0; q < 4; ++q)
+            if (mine && m0 + (c0 + q * width) / 16 * 16 + 16 <= p.M) ld_global_v8(from + (c0 + q * width) / width * 32, res[q]);
+        };
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const float4 q = bias[c0 / 4 + c];
-            y2[2 * c] = add2(sum[c0 / 2 + 2 * c], pair(q.x, q.y));
-            y2[2 * c + 1] = add2(sum[c0 / 2 + 2 * c + 1], pair(q.z, q.w));
-          }
-          activate<8>(y2, p.act);
-          float y[16];
+        for (int h = 0; h < COLS; h += 64) {
+          if (!LOOSE && p.residual != nullptr && pieces == 1) fetch_residuals(h, 16);
 #pragma unroll
-          for (int c = 0; c < 8; ++c) unpair(y2[c], y[2 * c], y[2 * c + 1]);
-          const int m = m0 + c0;
-          if (!LOOSE && m + 16 <= p.M) {
-            finish16(p, row, m, y);
-          } else {
+          for (int q = 0; q < 4; ++q) {
+            if (!LOOSE && p.residual != nullptr && pieces == 2 && q % 2 == 0) fetch_residuals(h + 16 * q, 8);
+            const int c0 = h + 16 * q, m = m0 + c0;
+            f32x2 y2[8];
 #pragma unroll
-            for (int c = 0; c < 16; ++c)
-              if (m + c < p.M) {
-                if (p.residual != nullptr) y[c] += element(p.residual, p.residual_elem, row * p.ldr + m + c);
-                store_result(p, row, m + c, y[c]);
+            for (int c = 0; c < 4; ++c) {
+              const float4 v = bias[c0 / 4 + c];
+              y2[2 * c] = add2(pair(sum[c0 + 4 * c], sum[c0 + 4 * c + 1]), pair(v.x, v.y));
+              y2[2 * c + 1] = add2(pair(sum[c0 + 4 * c + 2], sum[c0 + 4 * c + 3]), pair(v.z, v.w));
+            }
+            activate<8>(y2, p.act);
+            float y[16];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) unpair(y2[c], y[2 * c], y[2 * c + 1]);
+            if (!LOOSE && m + 16 <= p.M) {
+              if (p.residual != nullptr) add_residual(y, pieces == 2 ? res[q % 2 * 2] : res[q], res[q % 2 * 2 + 1], p.residual_elem);
+              if (mine) store16(p, row, m, y);
+            } else if (m < p.M) {   // two rows at a time, 16 lanes each
+              float* strip = strips[warp];
+              __syncwarp();
+#pragma unroll
+              for (int c = 0; c < 16; ++c) strip[lane * 17 + c] = y[c];
+              __syncwarp();
+              const int col = lane & 15;
+              // (loops that stay loops: unrolled for every group of columns, this code is read from memory for each item)
+              const int first = lane >> 4, rows_left = m + col < p.M ? n - quad * 32 : 0;
+              const long long at = row - lane + first;
+#pragma unroll 1
+              for (int k0 = 0; k0 < 32; k0 += 16) {
+                uint32_t raw_res[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                  raw_res[k] = p.residual != nullptr && k0 + 2 * k + first < rows_left ? raw_element(p.residual, p.residual_elem, (at + k0 + 2 * k) * p.ldr + m + col) : 0u;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                  float v = strip[(k0 + 2 * k + first) * 17 + col];
+                  if (p.residual != nullptr) v += of_raw(raw_res[k], p.residual_elem);
+                  if (k0 + 2 * k + first < rows_left) store_result(p, at + k0 + 2 * k, m + col, v);
+                }
               }
+            }
           }
         }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&bars.bias_empty[item & 1u]));
     }
-  }
-  if (p.splits > 1) {
-    __syncwarp();
-    cluster_meet();
-    if (begin < end && warp < kAdders) {   // rows of tokens dealt to the CTAs and their warps, features to lanes
-      const Item t = item_at(p, begin);
-      const int n = t.n1 - t.n0, share = (n + p.splits - 1) / p.splits, r1 = min(n, (rank + 1) * share), m0 = t.m * kWideFeatures;
-      for (int r = rank * share + warp; r < r1; r += kAdders) {
-        for (int h = 0; h < 2; ++h) {
-          const int m = m0 + 128 * h + 4 * lane;
-          if (m >= p.M) continue;
-          const uint32_t at = ring + (uint32_t)(r * kWidePitch + 128 * h + 4 * lane) * 4u;
-          float4 part[8];
-#pragma unroll
-          for (int q = 0; q < 8; ++q)
-            if (q < p.splits) part[q] = ld_cluster4(cluster_address(at, (uint32_t)q));
-          float y[4] = {part[0].x, part[0].y, part[0].z, part[0].w};
-#pragma unroll
-          for (int q = 1; q < 8; ++q)
-            if (q < p.splits) {
-              y[0] += part[q].x; y[1] += part[q].y; y[2] += part[q].z; y[3] += part[q].w;
-            }
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (m + k < p.M) {
-              if (p.bias != nullptr) y[k] += element(p.bias, p.bias_elem, (long long)t.expert * p.M + m + k);
-              y[k] = activate(y[k], p.act);
-              if (p.residual != nullptr) y[k] += element(p.residual, p.residual_elem, (long long)(t.n0 + r) * p.ldr + m + k);
-              store_result(p, t.n0 + r, m + k, y[k]);
-            }
-        }
-      }
+    if (p.splits > 1) {
+      __syncwarp();
+      cluster_meet();
+      if (begin < end) add_parts<LOOSE>(p, item_at(p, begin), ring, rank, warp, lane);
     }
+  }
+  if (p.splits > 1) {   // (the adding warps have met the others already)
     __syncwarp();
+    if (warp >= kAdders) cluster_meet();
     cluster_meet();   // (nobody leaves while others read its sums)
   }
   zero_tokens_in_no_run(p);
@@ -876,14 +972,44 @@ bool rows_map(CUtensorMap* m, const void* at, long long ld, long long expert, in
 
 // Launch with `splits` CTAs per item, in clusters.  Fewer items than half the places for CTAs: the blocks of k are shared, as long as every CTA has two of
 // them.
+// How many clusters of `splits` such CTAs a device holds at a time: a cluster lies within one of its groups of SMs, so some SMs are left over (36
+// clusters of four CTAs, one per SM, took two turns where 32 fit).
+int clusters_at_once(const void* kernel, int splits, int threads, int smem) {
+  struct Rec { const void* fn; int dev, splits, smem, clusters; };
+  static Rec recs[256];
+  static int n_recs = 0;
+  static std::mutex mu;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  const std::lock_guard<std::mutex> lock(mu);
+  for (int i = 0; i < n_recs; ++i)
+    if (recs[i].fn == kernel && recs[i].dev == dev && recs[i].splits == splits && recs[i].smem == smem) return recs[i].clusters;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)splits);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)splits;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int clusters = 0;
+  if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) return 0;
+  if (n_recs < 256) recs[n_recs++] = {kernel, dev, splits, smem, clusters};
+  return clusters;
+}
 cudaError_t launch_split(void (*kernel)(Fp8Params, CUtensorMap, CUtensorMap), Fp8Params& p, const CUtensorMap& a, const CUtensorMap& x, long long items,
-                         long long places, int smem, cudaStream_t st) {
+                         long long places, int threads, int smem, cudaStream_t st) {
   int splits = 1;
-  while (splits < 8 && items * splits * 2 <= places && p.k_blocks >= splits * 4) splits *= 2;
+  while (splits < 8 && p.k_blocks >= splits * 4 && items * splits * 2 <= places &&
+         items <= clusters_at_once(reinterpret_cast<const void*>(kernel), splits * 2, threads, smem))
+    splits *= 2;
   p.splits = splits;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(splits > 1 ? items * splits : (items < places ? items : places)));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
@@ -913,15 +1039,16 @@ int launch_few(Fp8Params p, const CUtensorMap& a, const CUtensorMap& x, long lon
   const int smem = p.stages * kStage + 1024;
   if (p.stages < 2) return VOID_ERR_SHAPE;
   if (ensure_smem(reinterpret_cast<const void*>(fp8_block_kernel<NT, CTAS>), smem) != 0) return VOID_ERR_CUDA;
-  return status_of(launch_split(fp8_block_kernel<NT, CTAS>, p, a, x, items, (long long)dev.sms * CTAS, smem, st));
+  return status_of(launch_split(fp8_block_kernel<NT, CTAS>, p, a, x, items, (long long)dev.sms * CTAS, kThreads, smem, st));
 }
 template <bool LOOSE>
 int launch_wide(Fp8Params p, const CUtensorMap& a, const CUtensorMap& x, long long items, const DeviceInfo& dev, cudaStream_t st) {
-  p.stages = ring_stages(dev, 1, (int)kWideStage, (int)sizeof(WideBars) + 2 * kWideFeatures * 4);
-  const int smem = p.stages * (int)kWideStage + 1024;
-  if (p.stages * (int)kWideStage < kWideTokens * kWidePitch * 4) return VOID_ERR_SHAPE;
+  constexpr int kStage = (int)kWideStage;
+  p.stages = ring_stages(dev, 1, kStage, (int)sizeof(WideBars) + 2 * kWideFeatures * 4 + kAdders * 32 * 17 * 4);
+  const int smem = p.stages * kStage + 1024;
+  if (p.stages * kStage < kWideTokens * kWidePitch * 4) return VOID_ERR_SHAPE;
   if (ensure_smem(reinterpret_cast<const void*>(fp8_wide_kernel<LOOSE>), smem) != 0) return VOID_ERR_CUDA;
-  return status_of(launch_split(fp8_wide_kernel<LOOSE>, p, a, x, items, dev.sms, smem, st));
+  return status_of(launch_split(fp8_wide_kernel<LOOSE>, p, a, x, items, dev.sms, kThreads, smem, st));
 }
 // Rows of results and residuals in pieces of 32 bytes.
 bool on_32_bytes(const void* at, long long ld, int elem) { return ((reinterpret_cast<uintptr_t>(at) | (uintptr_t)(ld * (elem == VOID_ELEM_F32 ? 4 : 2))) & 31u) == 0; }

@@ -2372,8 +2372,33 @@ PyObject* fp8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     s.ldr = tail.e.ldr;
     s.residual_elem = tail.e.residual_dtype;
   }
-  s.out = out.data_ptr();
-  s.ldc = N > 1 ? out.stride(0) : M;
+  // Many results in rows that do not lie on 32 bytes are written to a matrix whose rows do, and copied (its residual is copied before): 4000 x 4001,
+  // K = 4096, bf16 91 us and 10 for the copy against 152.  Few items share the blocks of k, and their sums' way to memory is another.
+  at::Tensor target = out;
+  auto on_32_bytes = [](const at::Tensor& t) {
+    return ((reinterpret_cast<uintptr_t>(t.const_data_ptr()) | (uintptr_t)(t.size(0) > 1 ? t.stride(0) * t.element_size() : 0)) & 31u) == 0;
+  };
+  auto on_whole_lines = [&](const at::Tensor& like, at::ScalarType of) {
+    const int64_t es = (int64_t)c10::elementSize(of), ld = (like.size(1) * es + 31) / 32 * 32 / es;
+    return new_cuda({like.size(0), ld}, of, dev).narrow(1, 0, like.size(1));
+  };
+  auto copy_rows = [&](const at::Tensor& from, const at::Tensor& to) {
+    const int64_t es = (int64_t)from.element_size();
+    check(void_copy_rows(from.const_data_ptr(), (from.size(0) > 1 ? from.stride(0) : M) * es, to.data_ptr(), (to.size(0) > 1 ? to.stride(0) : M) * es, (int32_t)es, N,
+                         (int32_t)M, stream_of(dev.index())),
+          "void_copy_rows");
+  };
+  const bool many = N > 64 && N * M >= (1 << 19) && (N + 127) / 128 * ((M + 255) / 256) > 74;
+  if (many && s.residual != nullptr && !on_32_bytes(tail.residual)) {
+    const at::Tensor lines = on_whole_lines(tail.residual, tail.residual.scalar_type());
+    copy_rows(tail.residual, lines);
+    tail.residual = lines;
+    s.residual = lines.const_data_ptr();
+    s.ldr = lines.stride(0);
+  }
+  if (many && !on_32_bytes(out) && !(runs && !none(a[7]))) target = on_whole_lines(out, type);
+  s.out = target.data_ptr();
+  s.ldc = N > 1 ? target.stride(0) : M;
   s.M = (int32_t)M;
   s.K = (int32_t)K;
   s.N = (int32_t)N;
@@ -2387,6 +2412,7 @@ PyObject* fp8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     plan.x.zero_rest = none(a[7]) ? 1 : 0;
   }
   check(void_fp8_linear(&s, runs ? &plan.x : nullptr, stream_of(dev.index())), "void_fp8_linear");
+  if (!target.is_same(out)) out.copy_(target);
   if (none(a[7])) return THPVariable_Wrap(out);
   mark_written(out);
   Py_INCREF(a[7]);

@@ -54,4 +54,12 @@ __device__ __forceinline__ void set_element(void* at, int elem, long long i, flo
   else reinterpret_cast<__nv_bfloat16*>(at)[i] = __float2bfloat16_rn(v);
 }
 
+// The same in two steps: the loads of several elements are on their way together, which a conversion behind each would prevent.
+__device__ __forceinline__ uint32_t raw_element(const void* at, int elem, long long i) {
+  return elem == 0 ? reinterpret_cast<const uint32_t*>(at)[i] : (uint32_t)reinterpret_cast<const uint16_t*>(at)[i];
+}
+__device__ __forceinline__ float of_raw(uint32_t u, int elem) {
+  return elem == 0 ? __uint_as_float(u) : (elem == 1 ? __half2float(__ushort_as_half((unsigned short)u)) : __uint_as_float(u << 16));
+}
+
 }  // namespace vb
