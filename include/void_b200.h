@@ -660,7 +660,8 @@ VOID_API int void_combine_grad(const void* g, int64_t ldg, const void* rows, int
  * a [M, K] (experts: n_experts of them, expert_stride bytes apart), lda bytes between rows; x [N, K], ldx bytes between rows: addresses, pitches
  * and expert_stride are multiples of 16.  Scales are fp32 with element strides of their own.  bias [M] (experts: [n_experts, M]) of bias_elem or
  * NULL; residual [N, M] or NULL (one matrix or experts; may be out, the same place and pitch).
- * experts: NULL, or the plan of void_expert_plan (offset_bytes 0) with chunks of 32, 64 or 128 tokens; row_order is not used.  Rows in no
+ * experts: NULL, or as for void_expert_linear (a plan, or for up to 32 experts the offsets themselves) with chunks of 32, 64 or 128 tokens; row_order
+ * is not used.  Rows in no
  * run are zeroed if zero_rest, else left alone.
  * void_quant_fp8_blocks: q [rows, cols] e4m3, ldq bytes between rows, and scales [ceil(rows / block_rows), ceil(cols / 128)] (element strides
  * scale_row, scale_col) of a matrix of type elem, for block_rows 1 or 128.  A scale is the smallest power of two (2^-100 at the least) that

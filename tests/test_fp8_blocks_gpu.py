@@ -193,6 +193,21 @@ def test_results_that_are_given():
     assert void.void_linear(w, x[:0]).shape == (0, 300)
 
 
+def test_refusals():
+    w = _weights(256, 256, 1)
+    e = void.FP8BlockTensor(w.values.view(2, 128, 256), w.scales.view(2, 1, 2))
+    x, tokens = torch.randn(256, 256, device="cuda"), void.quantize_fp8_blocks(torch.randn(256, 256, device="cuda"), 1)
+    offsets = torch.tensor([0, 100, 256], device="cuda")
+    for call, text in [
+            (lambda: void.void_linear(tokens, x), "128 x 128"), (lambda: void.void_linear(w, w), "each token"), (lambda: void.void_linear(w, x.double()), "float32"),
+            (lambda: void.void_linear(w, x, out_dtype=torch.float64), "output dtype"), (lambda: void.void_linear(w, x, activation=7), "activation code"),
+            (lambda: void.void_expert_linear(e, w, offsets), "each token"), (lambda: void.void_expert_linear(e, x.int(), offsets), "float32"),
+            (lambda: void.void_linear(void.FP8BlockTensor(w.values.cpu(), w.scales.cpu()), x), "no CPU path"),
+            (lambda: void.void_linear(w, x.cpu()), "no CPU path"), (lambda: void.void_linear(w, x, residual=x.cpu()), "GPU only")]:
+        with pytest.raises(_lib.VoidB200Error, match=text):
+            call()
+
+
 EXPERTS = [  # runs, rows behind them, M, K
     ([1], 0, 128, 128), ([0, 0, 3], 0, 130, 200), ([5, 0, 40, 1], 7, 300, 257), ([100, 30, 0, 200], 0, 256, 512), ([300, 260, 1, 0, 15], 13, 140, 300),
     ([0, 0], 20, 128, 256), ([700, 2, 600], 1, 260, 640), ([900, 0, 333], 40, 2001, 200), ([17] * 40, 3, 64, 128), ([1] * 70, 0, 200, 384), ([0] * 5 + [513], 0, 129, 129)]

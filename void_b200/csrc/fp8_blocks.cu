@@ -62,8 +62,22 @@ __device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(
 
 constexpr int kQuantThreads = 256;
 
-// A scale per row and 128 columns.  Rows in 16-byte pieces: 128 columns lie in 16 lanes (fp32: 32), a warp takes `HELD` groups of 512 bytes of a
-// row at a time; others element by element.
+// The largest magnitude of 16-bit numbers as their bits, two at a time (NaN above infinity above all others).
+__device__ __forceinline__ uint32_t magnitudes(uint32_t pair16) { return pair16 & 0x7fff7fffu; }
+__device__ __forceinline__ uint32_t max_halves(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t bits_of_half(uint32_t h);   // of the fp32 number that a 16-bit magnitude stands for
+template <>
+__device__ __forceinline__ uint32_t bits_of_half<__nv_bfloat16>(uint32_t h) { return h << 16; }
+template <>
+__device__ __forceinline__ uint32_t bits_of_half<__half>(uint32_t h) { return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h))) & 0x7fffffffu; }
+
+// A scale per row and 128 columns.  Rows in 16-byte pieces: 128 columns lie in 16 lanes (fp32: 32), a warp has `HELD` groups of 512 bytes of a
+// row at a time on their way; others element by element.  blockIdx.y: part of the columns.
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kQuantThreads) quant_rows_kernel(const __grid_constant__ QuantParams p) {
   constexpr int VEC = WIDE ? 16 / (int)sizeof(T) : 4, HELD = WIDE ? 4 : 2;
@@ -71,56 +85,67 @@ __global__ void __launch_bounds__(kQuantThreads) quant_rows_kernel(const __grid_
   constexpr int STEP = 32 * VEC;
   grid_dependency_wait();
   grid_launch_dependents();
-  const int lane = threadIdx.x & 31;
-  const int pieces = (p.cols + STEP * HELD - 1) / (STEP * HELD);
-  const long long items = p.rows * pieces;
-  for (long long i = (long long)blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5); i < items; i += (long long)gridDim.x * (kQuantThreads / 32)) {
-    const long long row = i / pieces;
-    const int c0 = (int)(i - row * pieces) * (STEP * HELD);
+  const int lane = threadIdx.x & 31, c0 = (int)blockIdx.y * (STEP * HELD);
+  for (long long row = (long long)blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5); row < p.rows; row += (long long)gridDim.x * (kQuantThreads / 32)) {
     const T* x = reinterpret_cast<const T*>(p.x) + row * p.ldx;
     uint8_t* q = p.q + row * p.ldq;
-    float v[HELD][VEC];
+    float* scales = p.scales + row * p.scale_row;
+    if constexpr (WIDE) {
+      uint4 raw[HELD];
 #pragma unroll
-    for (int h = 0; h < HELD; ++h) {
-      if constexpr (WIDE) {
+      for (int h = 0; h < HELD; ++h) {
         const int c = c0 + h * STEP + lane * VEC;
-        Piece<T, VEC> piece;
-        if (c < p.cols) piece.load(x + c);
+        raw[h] = c < p.cols ? *reinterpret_cast<const uint4*>(x + c) : make_uint4(0, 0, 0, 0);
+      }
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[h][e] = c < p.cols ? piece.get(e) : 0.0f;
-      } else {
+      for (int h = 0; h < HELD; ++h) {
+        uint32_t most;
+        if constexpr (VEC == 8) {
+          most = max_halves(max_halves(magnitudes(raw[h].x), magnitudes(raw[h].y)), max_halves(magnitudes(raw[h].z), magnitudes(raw[h].w)));
+#pragma unroll
+          for (int o = LANES / 2; o > 0; o >>= 1) most = max_halves(most, __shfl_xor_sync(kEvery, most, o));
+          most = bits_of_half<T>(max(most & 0xffffu, most >> 16));
+        } else {
+          most = max(max(raw[h].x & 0x7fffffffu, raw[h].y & 0x7fffffffu), max(raw[h].z & 0x7fffffffu, raw[h].w & 0x7fffffffu));
+          most = __reduce_max_sync(kEvery, most);
+        }
+        float inverse;
+        const float scale = block_scale(most, inverse);
+        const int c = c0 + h * STEP + lane * VEC;
+        if (c < p.cols) {
+          if (lane % LANES == 0) scales[(long long)(c / kBlock) * p.scale_col] = scale;
+          Piece<T, VEC> piece;
+          memcpy(piece.v, &raw[h], 16);
+          uint32_t w[VEC / 4];
+#pragma unroll
+          for (int k = 0; k < VEC / 4; ++k)
+            w[k] = e4m3x2(piece.get(4 * k) * inverse, piece.get(4 * k + 1) * inverse) | e4m3x2(piece.get(4 * k + 2) * inverse, piece.get(4 * k + 3) * inverse) << 16;
+          if constexpr (VEC == 8) *reinterpret_cast<uint2*>(q + c) = make_uint2(w[0], w[1]);
+          else *reinterpret_cast<uint32_t*>(q + c) = w[0];
+        }
+      }
+    } else {
+      float v[HELD][VEC];
+#pragma unroll
+      for (int h = 0; h < HELD; ++h)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           const int c = c0 + h * STEP + e * 32 + lane;
           v[h][e] = c < p.cols ? to_float<T>(x[c]) : 0.0f;
         }
-      }
-    }
 #pragma unroll
-    for (int h = 0; h < HELD; ++h) {
-      uint32_t most = 0;
+      for (int h = 0; h < HELD; ++h) {
+        uint32_t most = 0;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) most = max(most, magnitude(v[h][e]));
-#pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(kEvery, most, o));
-      float inverse;
-      const float scale = block_scale(most, inverse);
-      const int first = c0 + h * STEP + (WIDE ? lane / LANES * kBlock : 0);
-      if (first < p.cols && lane % LANES == 0) p.scales[row * p.scale_row + (long long)(first / kBlock) * p.scale_col] = scale;
-      if constexpr (WIDE) {
-        const int c = c0 + h * STEP + lane * VEC;
-        if (c < p.cols) {
-          uint32_t w[VEC / 4];
-#pragma unroll
-          for (int k = 0; k < VEC / 4; ++k)
-            w[k] = e4m3x2(v[h][4 * k] * inverse, v[h][4 * k + 1] * inverse) | e4m3x2(v[h][4 * k + 2] * inverse, v[h][4 * k + 3] * inverse) << 16;
-          if constexpr (VEC == 8) *reinterpret_cast<uint2*>(q + c) = make_uint2(w[0], w[1]);
-          else *reinterpret_cast<uint32_t*>(q + c) = w[0];
-        }
-      } else {
+        for (int e = 0; e < VEC; ++e) most = max(most, magnitude(v[h][e]));
+        most = __reduce_max_sync(kEvery, most);
+        float inverse;
+        const float scale = block_scale(most, inverse);
+        const int first = c0 + h * STEP;
+        if (first < p.cols && lane == 0) scales[(long long)(first / kBlock) * p.scale_col] = scale;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-          const int c = c0 + h * STEP + e * 32 + lane;
+          const int c = first + e * 32 + lane;
           if (c < p.cols) q[c] = (uint8_t)e4m3x2(v[h][e] * inverse, 0.0f);
         }
       }
@@ -163,8 +188,9 @@ int quant_of_type(const QuantParams& p, int block_rows, int sms, cudaStream_t st
   const bool wide = p.cols % VEC == 0 && ((reinterpret_cast<uintptr_t>(p.x) | (uintptr_t)(p.ldx * sizeof(T))) & 15u) == 0 &&
                     ((reinterpret_cast<uintptr_t>(p.q) | (uintptr_t)p.ldq) & 7u) == 0;
   const int step = wide ? 32 * VEC * 4 : 32 * 4 * 2;
-  const long long items = p.rows * ((p.cols + step - 1) / step), blocks = (items + kQuantThreads / 32 - 1) / (kQuantThreads / 32);
-  const int grid = (int)(blocks < 32ll * sms ? blocks : 32ll * sms);
+  const long long parts = (p.cols + (long long)step - 1) / step, blocks = (p.rows + kQuantThreads / 32 - 1) / (kQuantThreads / 32);
+  if (parts > 65535) return VOID_ERR_TOO_LARGE;
+  const dim3 grid((unsigned)(blocks < 0x7fffffffll ? blocks : 0x7fffffffll), (unsigned)parts);
   return status_of(wide ? launch_pdl(quant_rows_kernel<T, true>, grid, kQuantThreads, 0, st, p) : launch_pdl(quant_rows_kernel<T, false>, grid, kQuantThreads, 0, st, p));
 }
 
@@ -178,7 +204,8 @@ struct Fp8Params {
   int chunk, n_chunks, group;     // one matrix: tokens of an item, items along the tokens, and of them those taken together
   const int32_t *head, *bounds;   // experts: the plan of experts.cu
   const int4* chunks;
-  int n_experts, zero_rest;
+  const void* offsets;            // or, of up to 32 experts, the runs' offsets themselves
+  int offset_bytes, n_experts, zero_rest;
   const float* a_scale;
   long long as_row, as_col, as_expert;
   const float* x_scale;
@@ -204,10 +231,47 @@ struct __align__(8) Fp8Bars {
 struct Item {
   int m, n0, n1, expert;
 };
-__device__ __forceinline__ int items_of(const Fp8Params& p) { return (p.head != nullptr ? p.head[0] : p.n_chunks) * p.m_tiles; }
-// Items that follow one another share tokens or weights: of one matrix, `group` chunks of tokens meet every 128 features.
-__device__ __forceinline__ Item item_at(const Fp8Params& p, int i) {
+// The plan of up to 32 experts, which a warp makes for its CTA from the offsets (RunTable): a launch less.
+struct Runs {
+  int begin[32], end[32], first[32];   // tokens; chunks before the run's
+  int total;                           // chunks in all
+};
+// Behind the wait on the kernel before; for all threads.
+__device__ __forceinline__ void find_runs(const Fp8Params& p, Runs& runs) {
+  if (p.offsets == nullptr) return;
+  if (threadIdx.x < 32) {
+    ExpertParams x = {};
+    x.offsets = p.offsets;
+    x.offset_bytes = p.offset_bytes;
+    x.chunk = p.chunk;
+    x.n_experts = p.n_experts;
+    const RunTable table(x, p.N);
+    runs.begin[threadIdx.x] = table.begin;
+    runs.end[threadIdx.x] = table.end;
+    runs.first[threadIdx.x] = table.first;
+    if (threadIdx.x == 0) runs.total = table.total;
+    if (blockIdx.x == 0 && table.bad && p.status != nullptr) atomicCAS(p.status, 0, kStatusBadOffsets);
+  }
+  __syncthreads();
+}
+__device__ __forceinline__ int items_of(const Fp8Params& p, const Runs& runs) {
+  return (p.offsets != nullptr ? runs.total : (p.head != nullptr ? p.head[0] : p.n_chunks)) * p.m_tiles;
+}
+// Items that follow one another share tokens or weights: of one matrix, `group` chunks of tokens meet every piece of features.
+__device__ __forceinline__ Item item_at(const Fp8Params& p, const Runs& runs, int i) {
   Item t;
+  if (p.offsets != nullptr) {
+    const int c = i / p.m_tiles;
+    int e = 0;   // the last expert whose first chunk is not behind it
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+      if (e + o < p.n_experts && runs.first[e + o] <= c) e += o;
+    t.m = i - c * p.m_tiles;
+    t.expert = e;
+    t.n0 = runs.begin[e] + (c - runs.first[e]) * p.chunk;
+    t.n1 = min(t.n0 + p.chunk, runs.end[e]);
+    return t;
+  }
   if (p.head != nullptr) {
     const int c = i / p.m_tiles;
     const int4 chunk = p.chunks[c];
@@ -225,7 +289,6 @@ __device__ __forceinline__ Item item_at(const Fp8Params& p, int i) {
   t.n1 = t.n0 + p.chunk < p.N ? t.n0 + p.chunk : p.N;
   return t;
 }
-
 __device__ __forceinline__ uint32_t cluster_address(uint32_t addr, uint32_t rank) {
   uint32_t r;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
@@ -261,9 +324,9 @@ __device__ __forceinline__ void store_result(const Fp8Params& p, long long token
 }
 
 // Zeros for tokens in no run.
-__device__ __forceinline__ void zero_tokens_in_no_run(const Fp8Params& p) {
-  if (p.head == nullptr || !p.zero_rest) return;
-  const int low = p.bounds[0], high = p.bounds[p.n_experts];
+__device__ __forceinline__ void zero_tokens_in_no_run(const Fp8Params& p, const Runs& runs) {
+  if ((p.head == nullptr && p.offsets == nullptr) || !p.zero_rest) return;
+  const int low = p.offsets != nullptr ? runs.begin[0] : p.bounds[0], high = p.offsets != nullptr ? runs.end[p.n_experts - 1] : p.bounds[p.n_experts];
   for (int r = (int)blockIdx.x; r < low + p.N - high; r += (int)gridDim.x) {
     const long long token = r < low ? r : high + r - low;
     for (int m = threadIdx.x; m < p.M; m += kThreads) store_result(p, token, m, 0.0f);
@@ -283,6 +346,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) fp8_block_kernel(const __grid_
   __shared__ __align__(16) float scale_ring[kScaleSlots][NT];
   __shared__ uint32_t tmem_s;
   __shared__ int ctl_s[2];
+  __shared__ Runs runs;
   volatile int* ctl = ctl_s;
   const uint32_t ring = (smem_u32(raw) + 1023u) & ~1023u;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -313,18 +377,18 @@ __global__ void __launch_bounds__(kThreads, CTAS) fp8_block_kernel(const __grid_
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_s;
-  grid_dependency_wait();
-
   const int rank = p.splits > 1 ? (int)cluster_rank() : 0;
   const int b0 = (int)((long long)p.k_blocks * rank / p.splits), b1 = (int)((long long)p.k_blocks * (rank + 1) / p.splits);
-  const int step = (int)gridDim.x / p.splits, begin = (int)blockIdx.x / p.splits, end = items_of(p);
+  grid_dependency_wait();
+  find_runs(p, runs);
+  const int step = (int)gridDim.x / p.splits, begin = (int)blockIdx.x / p.splits, end = items_of(p, runs);
   // With several CTAs per item a launch has a cluster for every item, so that the ring is free when the sums meet in its place.
   if (warp == 0) {
     int stage = 0;
     uint32_t phase = 0;
     bool first = true;
     for (int i = begin; i < end && !ctl[0]; i += step) {
-      const Item t = item_at(p, i);
+      const Item t = item_at(p, runs, i);
       const int boxes = (t.n1 - t.n0 + kTokenBox - 1) / kTokenBox;
       for (int b = b0; b < b1; ++b) {
         if (!mbar_wait_warp(smem_u32(&bars.empty[stage]), phase ^ 1u, ctl)) break;
@@ -348,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) fp8_block_kernel(const __grid_
     uint32_t phase = 0, it = 0;
     bool ok = true;
     for (int i = begin; i < end && ok; i += step) {
-      const Item t = item_at(p, i);
+      const Item t = item_at(p, runs, i);
       const uint32_t idesc = instr_desc(1, 0, 0, 0, 0, 128, (uint32_t)(t.n1 - t.n0 + 15) & ~15u);
       for (int b = b0; b < b1; ++b, ++it) {
         const uint32_t slot = it & 1u;
@@ -371,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) fp8_block_kernel(const __grid_
     uint32_t it0 = 0;
     bool ok = true;
     for (int i = begin; i < end && ok; i += step) {
-      const Item t = item_at(p, i);
+      const Item t = item_at(p, runs, i);
       const float* sa = p.a_scale + t.expert * p.as_expert + t.m * p.as_row;
       const float* sx = p.x_scale + (long long)t.n0 * p.xs_row;
       float next[PER], next_a = 0.0f;
@@ -404,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) fp8_block_kernel(const __grid_
     uint32_t it = 0;
     bool ok = true;
     for (int i = begin; i < end && ok; i += step) {
-      const Item t = item_at(p, i);
+      const Item t = item_at(p, runs, i);
       const int n = t.n1 - t.n0, m = t.m * kBlock + quad * 32 + lane;
       const uint32_t bias_raw = p.bias != nullptr && m < p.M ? raw_element(p.bias, p.bias_elem, (long long)t.expert * p.M + m) : 0u;
       f32x2 sum[GROUPS][CG / 2];
@@ -496,7 +560,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) fp8_block_kernel(const __grid_
     cluster_meet();
     if (begin < end && warp >= kFirstAdder) {
       constexpr int HELD = 4;   // tokens whose sums and residuals are on their way together
-      const Item t = item_at(p, begin);
+      const Item t = item_at(p, runs, begin);
       const int n = t.n1 - t.n0, quad = warp & 3, side = (warp - kFirstAdder) >> 2, m = t.m * kBlock + quad * 32 + lane;
       const int share = (n + p.splits - 1) / p.splits, c1 = min(n, (rank + 1) * share);
       const uint32_t bias_raw = p.bias != nullptr && m < p.M ? raw_element(p.bias, p.bias_elem, (long long)t.expert * p.M + m) : 0u;
@@ -529,7 +593,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) fp8_block_kernel(const __grid_
     __syncwarp();
     cluster_meet();   // (nobody leaves while others read its sums)
   }
-  zero_tokens_in_no_run(p);
+  zero_tokens_in_no_run(p, runs);
   grid_launch_dependents();
   tc_fence_before();
   __syncthreads();
@@ -699,6 +763,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_wide_kernel(const __grid_cons
   __shared__ float strips[kAdders][32 * 17];   // results of a warp on their way from lanes that are tokens to lanes that are features
   __shared__ uint32_t tmem_s;
   __shared__ int ctl_s[2];
+  __shared__ Runs runs;
   volatile int* ctl = ctl_s;
   const uint32_t ring = (smem_u32(raw) + 1023u) & ~1023u;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -728,10 +793,11 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_wide_kernel(const __grid_cons
   tc_fence_after();
   const uint32_t tmem = tmem_s;
   grid_dependency_wait();
+  find_runs(p, runs);
 
   const int rank = p.splits > 1 ? (int)cluster_rank() : 0;
   const int b0 = (int)((long long)p.k_blocks * rank / p.splits), b1 = (int)((long long)p.k_blocks * (rank + 1) / p.splits);
-  const int step = (int)gridDim.x / p.splits, begin = (int)blockIdx.x / p.splits, end = items_of(p);
+  const int step = (int)gridDim.x / p.splits, begin = (int)blockIdx.x / p.splits, end = items_of(p, runs);
   // (4 * 56 + 8 * 224 = 12 * 168, what the block was launched with)
   if (warp >= kAdders) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
   if (warp == kCopier) {
@@ -739,7 +805,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_wide_kernel(const __grid_cons
     uint32_t phase = 0;
     bool first = true;
     for (int i = begin; i < end && !ctl[0]; i += step) {
-      const Item t = item_at(p, i);
+      const Item t = item_at(p, runs, i);
       const int boxes = (t.n1 - t.n0 + kTokenBox - 1) / kTokenBox, m0 = t.m * kWideFeatures, halves = p.M - m0 > kBlock ? 2 : 1;
       for (int b = b0; b < b1; ++b) {
         if (!mbar_wait_warp(smem_u32(&bars.empty[stage]), phase ^ 1u, ctl)) break;
@@ -763,7 +829,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_wide_kernel(const __grid_cons
     uint32_t phase = 0, it = 0;
     bool ok = true;
     for (int i = begin; i < end && ok; i += step) {
-      const Item t = item_at(p, i);
+      const Item t = item_at(p, runs, i);
       const uint32_t idesc = instr_desc(1, 0, 0, 0, 0, kWideTokens, p.M - t.m * kWideFeatures > kBlock ? kWideFeatures : kBlock);
       for (int b = b0; b < b1; ++b, ++it) {
         const uint32_t slot = it & 1u;
@@ -783,7 +849,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_wide_kernel(const __grid_cons
   } else if (warp == kBiasWarp) {   // biases of an item, asked for while the one before is multiplied
     uint32_t it = 0;
     for (int i = begin; i < end && p.splits == 1; i += step, ++it) {
-      const Item t = item_at(p, i);
+      const Item t = item_at(p, runs, i);
       float v[kWideFeatures / 32];
 #pragma unroll
       for (int k = 0; k < kWideFeatures / 32; ++k) {
@@ -802,7 +868,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_wide_kernel(const __grid_cons
     uint32_t it = 0, item = 0;
     bool ok = true;
     for (int i = begin; i < end && ok; i += step, ++item) {
-      const Item t = item_at(p, i);
+      const Item t = item_at(p, runs, i);
       const int n = t.n1 - t.n0, token = quad * 32 + lane, m0 = t.m * kWideFeatures + side * COLS;
       const bool mine = token < n, any = m0 < p.M && quad * 32 < n;   // (any: of what this warp reads back)
       const long long row = t.n0 + token;
@@ -936,7 +1002,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_wide_kernel(const __grid_cons
     if (p.splits > 1) {
       __syncwarp();
       cluster_meet();
-      if (begin < end) add_parts<LOOSE>(p, item_at(p, begin), ring, rank, warp, lane);
+      if (begin < end) add_parts<LOOSE>(p, item_at(p, runs, begin), ring, rank, warp, lane);
     }
   }
   if (p.splits > 1) {   // (the adding warps have met the others already)
@@ -944,7 +1010,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_wide_kernel(const __grid_cons
     if (warp >= kAdders) cluster_meet();
     cluster_meet();   // (nobody leaves while others read its sums)
   }
-  zero_tokens_in_no_run(p);
+  zero_tokens_in_no_run(p, runs);
   grid_launch_dependents();
   tc_fence_before();
   __syncthreads();
@@ -1035,7 +1101,7 @@ template <int NT, int CTAS>
 int launch_few(Fp8Params p, const CUtensorMap& a, const CUtensorMap& x, long long items, const DeviceInfo& dev, cudaStream_t st) {
   constexpr int kStage = kBlock * kBlock + NT * kBlock;
   static_assert(NT * kBlock * 4 <= 2 * kStage, "the partial sums lie in the ring");
-  p.stages = ring_stages(dev, CTAS, kStage, (int)sizeof(Fp8Bars) + kScaleSlots * NT * 4);
+  p.stages = ring_stages(dev, CTAS, kStage, (int)(sizeof(Fp8Bars) + sizeof(Runs)) + kScaleSlots * NT * 4);
   const int smem = p.stages * kStage + 1024;
   if (p.stages < 2) return VOID_ERR_SHAPE;
   if (ensure_smem(reinterpret_cast<const void*>(fp8_block_kernel<NT, CTAS>), smem) != 0) return VOID_ERR_CUDA;
@@ -1044,7 +1110,7 @@ int launch_few(Fp8Params p, const CUtensorMap& a, const CUtensorMap& x, long lon
 template <bool LOOSE>
 int launch_wide(Fp8Params p, const CUtensorMap& a, const CUtensorMap& x, long long items, const DeviceInfo& dev, cudaStream_t st) {
   constexpr int kStage = (int)kWideStage;
-  p.stages = ring_stages(dev, 1, kStage, (int)sizeof(WideBars) + 2 * kWideFeatures * 4 + kAdders * 32 * 17 * 4);
+  p.stages = ring_stages(dev, 1, kStage, (int)(sizeof(WideBars) + sizeof(Runs)) + 2 * kWideFeatures * 4 + kAdders * 32 * 17 * 4);
   const int smem = p.stages * kStage + 1024;
   if (p.stages * kStage < kWideTokens * kWidePitch * 4) return VOID_ERR_SHAPE;
   if (ensure_smem(reinterpret_cast<const void*>(fp8_wide_kernel<LOOSE>), smem) != 0) return VOID_ERR_CUDA;
@@ -1060,11 +1126,11 @@ int fp8_linear(const void_fp8_args* a, const void_experts* x, cudaStream_t st) {
     return VOID_ERR_BAD_ARG;
   if (a->M == 0 || a->N == 0) return VOID_OK;
   if (a->out == nullptr || a->K == 0 || a->a == nullptr || a->x == nullptr || a->a_scale == nullptr || a->x_scale == nullptr) return VOID_ERR_BAD_ARG;
-  if (x != nullptr && (x->n_experts < 1 || x->plan == nullptr || x->offset_bytes != 0 || (x->chunk != 32 && x->chunk != 64 && x->chunk != 128)))
+  if (x != nullptr && (x->n_experts < 1 || x->plan == nullptr || (x->offset_bytes != 0 && ((x->offset_bytes != 4 && x->offset_bytes != 8) || x->n_experts > 32)) || (x->chunk != 32 && x->chunk != 64 && x->chunk != 128)))
     return VOID_ERR_BAD_ARG;
   if (a->ldc < a->M || (a->residual != nullptr && a->ldr < a->M)) return VOID_ERR_SHAPE;
   if ((reinterpret_cast<uintptr_t>(a->a) & 15u) != 0 || (reinterpret_cast<uintptr_t>(a->x) & 15u) != 0 || (a->lda & 15) != 0 || (a->ldx & 15) != 0 ||
-      a->lda < a->K || a->ldx < a->K || (x != nullptr && ((a->expert_stride & 15) != 0 || a->expert_stride < 0 || (reinterpret_cast<uintptr_t>(x->plan) & 15u) != 0)))
+      a->lda < a->K || a->ldx < a->K || (x != nullptr && ((a->expert_stride & 15) != 0 || a->expert_stride < 0 || (reinterpret_cast<uintptr_t>(x->plan) & (x->offset_bytes != 0 ? x->offset_bytes - 1u : 15u)) != 0)))
     return VOID_ERR_ALIGN;
   const DeviceInfo dev = device_info();
   if (!dev.ok) return VOID_ERR_CUDA;
@@ -1087,7 +1153,13 @@ int fp8_linear(const void_fp8_args* a, const void_experts* x, cudaStream_t st) {
   long long chunks;
   if (x != nullptr) {
     const PlanView v = plan_of(*x, a->N);
-    p.head = v.head; p.bounds = v.bounds; p.chunks = v.chunks;
+    if (x->offset_bytes != 0) {
+      p.offsets = x->plan;
+      p.offset_bytes = x->offset_bytes;
+    } else {
+      p.head = v.head; p.bounds = v.bounds; p.chunks = v.chunks;
+    }
+    p.chunk = chunk;
     p.n_experts = x->n_experts;
     p.zero_rest = x->zero_rest;
     chunks = v.capacity;

@@ -2289,7 +2289,7 @@ int32_t fp8_chunk(int64_t rows, int64_t experts) {
   const int64_t each = (rows + experts - 1) / experts;
   return each <= 24 ? 32 : (each <= 64 ? 64 : 128);
 }
-// fp8_linear(values, scales, x, x_scales | None, offsets | None, bias | None, act, out | None, out_dtype, residual | None, status) -> out
+// fp8_linear(values, scales, x, x_scales | None, offsets | None, bias | None, act, out | None, out_dtype | None, residual | None, status) -> out
 // values [M, K] or (with offsets) [experts, M, K] in e4m3; x [N, K] in e4m3 with x_scales, or floating: quantised first
 PyObject* fp8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   NATIVE_BEGIN
@@ -2301,12 +2301,19 @@ PyObject* fp8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (values_in.dim() != dims || scales.dim() != dims) fail("weights and scales must have " + std::to_string(dims) + " dimensions here");
   const int64_t E = runs ? values_in.size(0) : 1, M = values_in.size(dims - 2), K = values_in.size(dims - 1), N = x_in.size(0);
   if (x_in.dim() != 2 || x_in.size(1) != K) fail("x must be a matrix of tokens with " + std::to_string(K) + " features");
+  if (none(a[3]) && !floating(x_in.scalar_type()))
+    fail(std::string("x must be float32, float16 or bfloat16, or an FP8BlockTensor, got ") + c10::toString(x_in.scalar_type()));
   if (values_in.device() != dev || scales.device() != dev) fail("the weights and x are on different devices");
+  if (values_in.scalar_type() != at::kFloat8_e4m3fn || scales.scalar_type() != at::kFloat) fail("weights are float8_e4m3fn with float32 scales");
+  if (scales.size(dims - 2) != (M + 127) / 128 || scales.size(dims - 1) != (K + 127) / 128 || (runs && scales.size(0) != E))
+    fail("weights carry a scale for each block of 128 x 128");
   if (M > 0x7fffff00 || K > 0x7fffff00 || N > 0x40000000) fail("the product is too large");
   c10::cuda::OptionalCUDAGuard guard;
   if (c10::cuda::current_device() != dev.index()) guard.set_device(dev);
   at::AutoDispatchBelowADInplaceOrView below;
-  const at::ScalarType type = reinterpret_cast<THPDtype*>(a[8])->scalar_type;
+  if (!none(a[8]) && !THPDtype_Check(a[8])) throw torch::TypeError("out_dtype must be a torch.dtype");
+  const at::ScalarType type = !none(a[8]) ? reinterpret_cast<THPDtype*>(a[8])->scalar_type
+                              : !none(a[7]) ? cuda_tensor(a[7], "out").scalar_type() : (none(a[3]) ? x_in.scalar_type() : at::kFloat);
   out_code(type);
   at::Tensor out;
   if (none(a[7])) {
@@ -2318,7 +2325,7 @@ PyObject* fp8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (runs && meet(out, tensor(a[4], "offsets"))) fail("out must have no memory in common with the offsets");
     if (!none(a[5]) && meet(out, tensor(a[5], "bias"))) fail("out must have no memory in common with the bias");
   }
-  at::Tensor values = values_in, x, x_scales;
+  at::Tensor values = values_in, x, x_scales, workspace;
   auto lies = [](const at::Tensor& t) {   // rows on 16 bytes
     const int64_t d = t.dim();
     if ((reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15u) != 0 || (t.size(d - 1) > 1 && t.stride(d - 1) != 1)) return false;
@@ -2335,22 +2342,40 @@ PyObject* fp8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return copy;
   };
   values = laid_out(values);
-  if (none(a[3])) {
-    const Quantised q = quantised(x_in, 1);
-    x = q.values;
-    x_scales = q.scales;
-  } else {
-    x = laid_out(x_in);
-    x_scales = cuda_tensor(a[3], "x's scales");
-    if (x_scales.device() != dev) fail("x and its scales are on different devices");
-    if (meet(out, x)) x = laid_out(x.clone());
-    if (meet(out, x_scales)) x_scales = x_scales.clone();
-  }
   void_fp8_args s = {};
   auto pitch = [](const at::Tensor& t) {
     const int64_t d = t.dim(), wide = (t.size(d - 1) + 15) / 16 * 16;
     return t.size(d - 2) > 1 ? t.stride(d - 2) : wide;
   };
+  if (none(a[3])) {   // x is quantised first: values and scales in one workspace
+    const at::Tensor rows = token_rows(x_in);
+    const int64_t padded = (N + 3) / 4 * 4;
+    s.ldx = (K + 15) / 16 * 16;
+    const int64_t values_bytes = (N * s.ldx + 255) / 256 * 256;
+    workspace = new_cuda({values_bytes + (K + 127) / 128 * padded * 4}, at::kByte, dev);
+    uint8_t* at = static_cast<uint8_t*>(workspace.data_ptr());
+    float* sx = reinterpret_cast<float*>(at + values_bytes);
+    check(void_quant_fp8_blocks(rows.const_data_ptr(), out_code(rows.scalar_type()), row_step(rows), N, (int32_t)K, 1, at, s.ldx, sx, 1, padded, stream_of(dev.index())),
+          "void_quant_fp8_blocks");
+    s.x = at;
+    s.x_scale = sx;
+    s.x_scale_row = 1;
+    s.x_scale_col = padded;
+  } else {
+    if (x_in.scalar_type() != at::kFloat8_e4m3fn) fail("quantised tokens are float8_e4m3fn");
+    x = laid_out(x_in);
+    x_scales = cuda_tensor(a[3], "x's scales");
+    if (x_scales.device() != dev) fail("x and its scales are on different devices");
+    if (x_scales.scalar_type() != at::kFloat || x_scales.dim() != 2 || x_scales.size(0) != N || x_scales.size(1) != (K + 127) / 128)
+      fail("tokens carry a scale for each token's 128 features");
+    if (meet(out, x)) x = laid_out(x.clone());
+    if (meet(out, x_scales)) x_scales = x_scales.clone();
+    s.x = x.const_data_ptr();
+    s.ldx = pitch(x);
+    s.x_scale = x_scales.const_data_ptr<float>();
+    s.x_scale_row = x_scales.stride(0);
+    s.x_scale_col = x_scales.stride(1);
+  }
   s.a = values.const_data_ptr();
   s.lda = pitch(values);
   s.expert_stride = E > 1 ? values.stride(0) : (s.lda * M + 15) / 16 * 16;
@@ -2358,11 +2383,6 @@ PyObject* fp8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   s.a_scale_row = scales.stride(dims - 2);
   s.a_scale_col = scales.stride(dims - 1);
   s.a_scale_expert = runs ? scales.stride(0) : 0;
-  s.x = x.const_data_ptr();
-  s.ldx = pitch(x);
-  s.x_scale = x_scales.const_data_ptr<float>();
-  s.x_scale_row = x_scales.stride(0);
-  s.x_scale_col = x_scales.stride(1);
   at::Tensor bias;
   if (!none(a[5])) s.bias = bias_as_it_is(tensor(a[5], "bias"), dev, E * M, &s.bias_elem, bias, runs ? "the experts' bias" : "bias");
   Tail tail;
@@ -2408,7 +2428,7 @@ PyObject* fp8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   s.status = cuda_tensor(a[10], "status").data_ptr<int32_t>();
   ExpertPlan plan;
   if (runs) {
-    plan = expert_plan(cuda_tensor(a[4], "offsets"), N, E, dev, s.status, false, fp8_chunk(N, E));
+    plan = expert_plan(cuda_tensor(a[4], "offsets"), N, E, dev, s.status, true, fp8_chunk(N, E));
     plan.x.zero_rest = none(a[7]) ? 1 : 0;
   }
   check(void_fp8_linear(&s, runs ? &plan.x : nullptr, stream_of(dev.index())), "void_fp8_linear");

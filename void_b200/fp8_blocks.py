@@ -84,26 +84,15 @@ class FP8BlockTensor:
         return (self.values.float() * scales).to(dtype)
 
     def _product(self, x, offsets, bias, activation, out, out_dtype, residual) -> torch.Tensor:
-        values, scales = self.values, self.scales
-        if self.block_rows != BLOCK and values.shape[-2] > 1:
-            raise _lib.VoidB200Error("weights carry a scale for each block of 128 x 128, got scales %s" % (tuple(scales.shape),))
-        x_scales = None
-        if isinstance(x, FP8BlockTensor):
-            if x.block_rows != 1 and x.values.shape[0] > 1:
-                raise _lib.VoidB200Error("tokens carry a scale for each token's 128 features, got scales %s" % (tuple(x.scales.shape),))
+        values, x_scales = self.values, None
+        if type(x) is FP8BlockTensor:
             x, x_scales = x.values, x.scales
-            dtype = out_dtype or (torch.float32 if out is None else out.dtype)
-        else:
-            if x.dtype not in _lib.OUT_DTYPE_CODE:
-                raise _lib.VoidB200Error("x must be float32, float16 or bfloat16, or an FP8BlockTensor, got %s" % x.dtype)
-            dtype = out_dtype or (x.dtype if out is None else out.dtype)
-        _lib.require_cuda(values, scales, x, x_scales, offsets, bias, out, residual)
-        if out is not None and out.dtype is not dtype:
-            raise _lib.VoidB200Error("out must be of type %s, got %s" % (dtype, out.dtype))
+        if not (values.is_cuda and x.is_cuda):
+            _lib.require_cuda(values, x)
         status = self._status
-        if status is None or status.device != values.device:
+        if status is None:
             status = self._status = _lib.status_word(values.device)
-        return _lib.native().fp8_linear(values, scales, x, x_scales, offsets, bias, activation, out, dtype, residual, status)
+        return _lib.native().fp8_linear(values, self.scales, x, x_scales, offsets, bias, activation, out, out_dtype, residual, status)
 
     def __repr__(self) -> str:
         return f"FP8BlockTensor(shape={self.shape}, block={(self.block_rows, BLOCK)}, device={self.values.device})"
