@@ -55,8 +55,8 @@ def test_sort_refuses(bad, status):
 
 def test_sort_workspace():
     words = _lib.load().void_sort_by_expert_ws_bytes
-    assert words(0, 8) == 0 and words(4096, 8) == 0 and words(-1, 8) == 0 and words(100000, 0) == 0
-    assert words(4097, 8) == 2 * 8 * 4
+    assert words(0, 8) == 0 and words(32768, 8) == 0 and words(-1, 8) == 0 and words(1000000, 0) == 0
+    assert words(32769, 8) == 9 * 8 * 4
     assert words(2 ** 31 - 1, 1024) == 256 * 1024 * 4
 
 

@@ -159,7 +159,7 @@ def _ids(n, top, experts, kind, seed, dtype=torch.int32):
     return ids.to(dtype)
 
 
-SORTS = [(0, 2, 4), (1, 1, 1), (1, 3, 1024), (33, 1, 7), (17, 4, 64), (512, 2, 9), (513, 2, 9), (1365, 3, 33), (4096, 1, 5), (4097, 1, 1000), (5000, 8, 256)]
+SORTS = [(0, 2, 4), (1, 1, 1), (1, 3, 1024), (33, 1, 7), (17, 4, 64), (512, 2, 9), (513, 2, 9), (1365, 3, 33), (4096, 1, 5), (4097, 1, 1000), (5000, 5, 256), (8192, 1, 3), (8193, 1, 12), (16384, 2, 64), (16385, 2, 65), (5000, 8, 256)]
 
 
 @pytest.mark.parametrize("kind", ["any", "dropped", "one", "none"])

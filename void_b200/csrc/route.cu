@@ -10,6 +10,7 @@
 // A choice of no expert (an id outside [0, experts)) is dropped: it has row -1, brings nothing into the sum, and leaves a row behind the last
 // run, which dispatch and combine's gradient fill with zeros.  All sums are fp32 and taken in the order of the slots; nothing depends on the
 // order in which blocks ran.
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -160,17 +161,18 @@ int route_launch(const RouteParams& p, int elem, cudaStream_t st) {
 }
 
 // ------------------------------------------------------------------------------------------ sort
-// A counting sort that keeps the order of the choices within an expert.  The choices are dealt to blocks in order; a first launch counts
-// every block's choices per expert (one block alone counts for itself), the second adds up what lies before a block and ranks its own: a warp
-// ranks 32 choices at once by asking which lanes have the same expert, and 32 warps meet in a table of their counts.
+// A counting sort that keeps the order of the choices within an expert: a warp ranks 32 choices at once by asking which lanes have the same
+// expert, 32 warps meet in a table of their counts, and the CTAs of a cluster add up each other's.  More choices than one cluster holds in registers
+// (32768) are dealt to blocks in order, which a launch of its own counts first.
 constexpr int kSortThreads = 1024, kSortSteps = 4, kSortTile = kSortThreads * kSortSteps;
 constexpr int kMaxSortExperts = 1024;
+constexpr int kSortCluster = 8, kMostInCluster = kSortCluster * kSortTile;
 
 struct SortParams {
   const void* experts;
   long long count, share;   // choices, and of one block (a multiple of a tile)
   int n_experts, pitch;     // pitch: entries between the warps' counts in shared memory
-  int32_t* table;           // [blocks][experts] counts, or null: one block
+  int32_t* table;           // [blocks][experts] counts
   int32_t* offsets;
   int32_t* position;
 };
@@ -179,6 +181,31 @@ __device__ __forceinline__ int expert_of(const void* experts, long long i, int n
   const long long e = (long long)reinterpret_cast<const I*>(experts)[i];
   return e < 0 || e >= n_experts ? -1 : (int)e;
 }
+// Sum of the values of the threads before, for the whole block; `s` has a word per warp.
+__device__ __forceinline__ int sum_before(int v, int32_t* s) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int upto = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(kAll, upto, o);
+    if (lane >= o) upto += u;
+  }
+  if (lane == 31) s[warp] = upto;
+  __syncthreads();
+  int first = upto - v;
+  for (int w = 0; w < warp; ++w) first += s[w];
+  return first;
+}
+// Lanes with the same expert as this one (a dropped choice: any): a vote for each bit of the number.  __match_any_sync takes a step for every expert that
+// there is: 32768 choices of 64 experts 7.4 us that way.
+__device__ __forceinline__ unsigned same_expert(int expert, int bits) {
+  unsigned same = __ballot_sync(kAll, expert >= 0);
+  for (int b = 0; b < bits; ++b) {
+    const unsigned set = __ballot_sync(kAll, expert >> b & 1);
+    same &= (expert >> b & 1) ? set : ~set;
+  }
+  return same;
+}
 template <typename I>
 __device__ __forceinline__ void count_choices(const SortParams& p, long long begin, long long end, int32_t* counts) {
   for (int e = threadIdx.x; e < p.n_experts; e += blockDim.x) counts[e] = 0;
@@ -186,10 +213,89 @@ __device__ __forceinline__ void count_choices(const SortParams& p, long long beg
   const int lane = threadIdx.x & 31;
   for (long long i = begin + threadIdx.x; i - lane < end; i += blockDim.x) {
     const int e = i < end ? expert_of<I>(p.experts, i, p.n_experts) : -1;
-    const unsigned same = __match_any_sync(kAll, e);
+    const unsigned same = same_expert(e, 32 - __clz(p.n_experts - 1));
     if (e >= 0 && lane == __ffs(same) - 1) atomicAdd(&counts[e], __popc(same));   // (whole numbers: any order gives the same)
   }
   __syncthreads();
+}
+
+// Ranks of a warp's choices among its own, and their counts in the warp's row of the table.
+template <int STEPS>
+__device__ __forceinline__ void rank_choices(const int (&expert)[STEPS], int (&rank)[STEPS], uint16_t* counts, int n_experts) {
+  const int lane = threadIdx.x & 31, bits = 32 - __clz(n_experts - 1);
+  unsigned mates[STEPS];
+#pragma unroll
+  for (int k = 0; k < STEPS; ++k) mates[k] = same_expert(expert[k], bits);
+#pragma unroll
+  for (int k = 0; k < STEPS; ++k) {
+    const unsigned same = mates[k];
+    const int ahead = expert[k] >= 0 ? counts[expert[k]] : 0;
+    __syncwarp();
+    if (expert[k] >= 0 && lane == __ffs(same) - 1) counts[expert[k]] = (uint16_t)(ahead + __popc(same));
+    __syncwarp();
+    rank[k] = ahead + __popc(same & ((1u << lane) - 1u));
+  }
+}
+// Counts of the warps before, in the place of every warp's own (a warp adds up an expert's), and of all.
+__device__ __forceinline__ void add_up_warps(uint16_t* warp_counts, int pitch, int n_experts, int32_t* totals) {
+  const int lane = threadIdx.x & 31;
+  for (int e = threadIdx.x >> 5; e < n_experts; e += kSortThreads / 32) {
+    const int c = warp_counts[lane * pitch + e];
+    int sum = c;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(kAll, sum, o);
+      if (lane >= o) sum += u;
+    }
+    warp_counts[lane * pitch + e] = (uint16_t)(sum - c);
+    if (lane == 31) totals[e] = sum;
+  }
+}
+
+// All choices by one cluster, STEPS of them in a thread's registers.
+template <typename I, int STEPS>
+__global__ void __launch_bounds__(kSortThreads) sort_cluster_kernel(const __grid_constant__ SortParams p) {
+  extern __shared__ uint16_t warp_counts[];   // [32][pitch]
+  __shared__ int32_t totals[kMaxSortExperts], base[kMaxSortExperts], warp_total[32];
+  const cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, blocks = (int)gridDim.x;
+  for (int i = tid; i < 16 * p.pitch; i += kSortThreads) reinterpret_cast<uint32_t*>(warp_counts)[i] = 0u;
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const long long begin = (long long)blockIdx.x * p.share, end = begin + p.share < p.count ? begin + p.share : p.count;
+  const long long from = begin + warp * (32 * STEPS) + lane;
+  int expert[STEPS], rank[STEPS];
+#pragma unroll
+  for (int k = 0; k < STEPS; ++k) expert[k] = from + 32 * k < end ? expert_of<I>(p.experts, from + 32 * k, p.n_experts) : -1;
+  __syncthreads();
+  rank_choices<STEPS>(expert, rank, warp_counts + warp * p.pitch, p.n_experts);
+  __syncthreads();
+  add_up_warps(warp_counts, p.pitch, p.n_experts, totals);
+  cluster.sync();
+  int total = 0, before = 0;
+  if (tid < p.n_experts) {
+#pragma unroll
+    for (int b = 0; b < kSortCluster; ++b)
+      if (b < blocks) {
+        const int c = *cluster.map_shared_rank(totals + tid, b);
+        total += c;
+        before += b < (int)blockIdx.x ? c : 0;
+      }
+  }
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  const int first = sum_before(total, warp_total);
+  if (tid < p.n_experts) base[tid] = first + before;
+  if (blockIdx.x == 0) {
+    if (tid < p.n_experts) p.offsets[tid] = first;
+    if (tid == p.n_experts - 1) p.offsets[p.n_experts] = first + total;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < STEPS; ++k) {
+    const long long i = from + 32 * k;
+    if (i < end) p.position[i] = expert[k] >= 0 ? base[expert[k]] + warp_counts[warp * p.pitch + expert[k]] + rank[k] : -1;
+  }
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");   // (no CTA leaves while others read its counts)
 }
 
 template <typename I>
@@ -212,10 +318,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(const __grid_c
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const long long begin = (long long)blockIdx.x * p.share, end = begin + p.share < p.count ? begin + p.share : p.count;
   int total = 0, before = 0;
-  if (p.table == nullptr) {
-    count_choices<I>(p, begin, end, base);
-    total = tid < p.n_experts ? base[tid] : 0;
-  } else if (tid < p.n_experts) {
+  if (tid < p.n_experts) {
 #pragma unroll 8
     for (int b = 0; b < (int)gridDim.x; ++b) {
       const int c = p.table[(long long)b * p.n_experts + tid];
@@ -223,17 +326,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(const __grid_c
       before += b < (int)blockIdx.x ? c : 0;
     }
   }
-  // rows before every expert's: an exclusive sum over the block
-  int upto = total;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(kAll, upto, o);
-    if (lane >= o) upto += u;
-  }
-  if (lane == 31) warp_total[warp] = upto;
-  __syncthreads();
-  int first = upto - total;
-  for (int w = 0; w < warp; ++w) first += warp_total[w];
+  const int first = sum_before(total, warp_total);
   if (tid < p.n_experts) base[tid] = first + before;
   if (blockIdx.x == 0) {
     if (tid < p.n_experts) p.offsets[tid] = first;
@@ -247,28 +340,9 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(const __grid_c
     const long long from = tile + (long long)warp * (32 * kSortSteps) + lane;
 #pragma unroll
     for (int k = 0; k < kSortSteps; ++k) expert[k] = from + 32 * k < end ? expert_of<I>(p.experts, from + 32 * k, p.n_experts) : -1;
-#pragma unroll
-    for (int k = 0; k < kSortSteps; ++k) {
-      const unsigned same = __match_any_sync(kAll, expert[k]);
-      const int ahead = expert[k] >= 0 ? counts[expert[k]] : 0;
-      __syncwarp();
-      if (expert[k] >= 0 && lane == __ffs(same) - 1) counts[expert[k]] = (uint16_t)(ahead + __popc(same));
-      __syncwarp();
-      rank[k] = ahead + __popc(same & ((1u << lane) - 1u));
-    }
+    rank_choices<kSortSteps>(expert, rank, counts, p.n_experts);
     __syncthreads();
-    // counts of the warps before, in the place of every warp's own: a warp adds up an expert's
-    for (int e = warp; e < p.n_experts; e += 32) {
-      const int c = warp_counts[lane * p.pitch + e];
-      int sum = c;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(kAll, sum, o);
-        if (lane >= o) sum += u;
-      }
-      warp_counts[lane * p.pitch + e] = (uint16_t)(sum - c);
-      if (lane == 31) reinterpret_cast<int32_t*>(warp_counts + 32 * p.pitch)[e] = sum;
-    }
+    add_up_warps(warp_counts, p.pitch, p.n_experts, reinterpret_cast<int32_t*>(warp_counts + 32 * p.pitch));
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kSortSteps; ++k) {
@@ -281,7 +355,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(const __grid_c
   }
 }
 
-// Blocks of a sort, and the choices of one: a tile each, until every SM has a block.
+// Blocks of a sort that one cluster does not hold, and the choices of one.
 inline int sort_blocks(long long count, int sms) {
   const long long tiles = (count + kSortTile - 1) / kSortTile;
   return (int)(tiles < 1 ? 1 : (tiles < sms ? tiles : sms));
@@ -294,8 +368,8 @@ constexpr int kMaxSortBlocks = 256;
 
 // ------------------------------------------------------------------------------------------ rows of tokens
 constexpr int kRowThreads = 256;
-// Pieces of a row that one thread holds at a time: 16-byte pieces two, single elements eight.
-template <int VEC> constexpr int kHeld = VEC > 1 ? 2 : 8;
+// 16-byte pieces of a row that one thread holds at a time.
+constexpr int kHeld = 2;
 // Choices that the sort's own block is not worth a launch for: every warp ranks its token's choices by counting.
 constexpr int kFewChoices = 1024;
 
@@ -325,28 +399,83 @@ struct RowParams {
 // Whether a choice has a row; positions are not trusted.
 __device__ __forceinline__ bool has_row(const RowParams& p, int row) { return row >= 0 && row < p.rows; }
 
-// Zeros in the rows behind the last run, dealt to the launch's blocks.
-template <typename T, int VEC>
-__device__ __forceinline__ void zero_rest(const RowParams& p, long long used, int c0, int c1) {
+// 16 bytes of a row from column `c` on, whatever address that is: WIDE, rows that lie in 16-byte pieces, one load; others from the one or two aligned
+// pieces that hold them, shifted (all threads of a row by the same).  No piece is read that has no byte of the row in it; what is not the row's is
+// anything.
+template <typename T, bool WIDE>
+__device__ __forceinline__ void load_piece(Piece<T, 16 / sizeof(T)>& piece, const T* row, int c, int cols) {
+  if constexpr (WIDE) {
+    piece.load(row + c);
+  } else {
+    const long long at = reinterpret_cast<long long>(row) + (long long)c * (int)sizeof(T);
+    const long long lo = reinterpret_cast<long long>(row), hi = lo + (long long)cols * (int)sizeof(T), base = at & ~15ll;
+    const int shift = (int)(at & 15);
+    uint4 u = make_uint4(0, 0, 0, 0), v = u;
+    if (base + 16 > lo && base < hi) u = *reinterpret_cast<const uint4*>(base);
+    if (shift != 0) {
+      if (base + 32 > lo && base + 16 < hi) v = *reinterpret_cast<const uint4*>(base + 16);
+      uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+      if (shift & 8) {
+#pragma unroll
+        for (int k = 0; k < 6; ++k) w[k] = w[k + 2];
+      }
+      if (shift & 4) {
+#pragma unroll
+        for (int k = 0; k < 5; ++k) w[k] = w[k + 1];
+      }
+      if (sizeof(T) == 2 && (shift & 2)) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(w[k], w[k + 1], 16);
+      }
+      u = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    memcpy(piece.v, &u, 16);
+  }
+}
+// The pieces of a row that is written begin at its aligned addresses, so the first may lie partly ahead of the row (c < 0), and the last behind it.
+template <typename T, bool WIDE>
+__device__ __forceinline__ int first_piece(const T* row) {
+  return WIDE ? 0 : -(int)((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T));
+}
+template <typename T, bool WIDE>
+__device__ __forceinline__ void store_piece(const Piece<T, 16 / sizeof(T)>& piece, T* row, int c, int cols) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  if (WIDE || (c >= 0 && c + VEC <= cols)) {
+    piece.store(row + c);
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e)
+      if (c + e >= 0 && c + e < cols) row[c + e] = piece.v[e];
+  }
+}
+
+// Zeros in the rows behind the last run, dealt to the launch's blocks; pieces [first, end) of each.
+template <typename T, bool WIDE>
+__device__ __forceinline__ void zero_rest(const RowParams& p, long long used, int first, int end) {
+  constexpr int VEC = 16 / (int)sizeof(T);
   Piece<T, VEC> zero;
 #pragma unroll
   for (int e = 0; e < VEC; ++e) zero.set(e, 0.0f);
-  for (long long r = (used < 0 ? 0 : used) + blockIdx.x; r < p.rows; r += gridDim.x)
-    for (int c = c0 + threadIdx.x * VEC; c < c1; c += kRowThreads * VEC) zero.store(reinterpret_cast<T*>(p.out) + r * p.ldo + c);
+  for (long long r = (used < 0 ? 0 : used) + blockIdx.x; r < p.rows; r += gridDim.x) {
+    T* row = reinterpret_cast<T*>(p.out) + r * p.ldo;
+    for (int i = first + threadIdx.x; i < end; i += kRowThreads) {
+      const int c = first_piece<T, WIDE>(row) + i * VEC;
+      if (c < p.cols) store_piece<T, WIDE>(zero, row, c, p.cols);
+    }
+  }
 }
 
 // Token by token, so that x is read once; a token's copies go where its choices were sorted to.  blockIdx.y: part of the columns.
 // SORT (few choices): the rows are not known yet, each is the number of choices that come before it.
-template <typename T, int VEC, typename I, bool SORT>
+template <typename T, bool WIDE, typename I, bool SORT>
 __global__ void __launch_bounds__(kRowThreads) dispatch_kernel(const __grid_constant__ RowParams p) {
-  constexpr int U = kHeld<VEC>;
+  constexpr int VEC = 16 / (int)sizeof(T), U = kHeld;
   __shared__ int32_t ids[SORT ? kFewChoices : 1];
   __shared__ int32_t place[SORT ? kFewChoices : 1];   // of this token's choices
   __shared__ int32_t rows_used;
   grid_dependency_wait();
   grid_launch_dependents();
-  const int c0 = blockIdx.y * (kRowThreads * VEC * U);
-  const int c1 = c0 + kRowThreads * VEC * U < p.cols ? c0 + kRowThreads * VEC * U : p.cols;
+  const int i0 = blockIdx.y * (kRowThreads * U);   // the block's pieces
   const T* x = reinterpret_cast<const T*>(p.x);
   T* out = reinterpret_cast<T*>(p.out);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -371,10 +500,12 @@ __global__ void __launch_bounds__(kRowThreads) dispatch_kernel(const __grid_cons
   }
   for (long long t = blockIdx.x; t < p.tokens; t += gridDim.x) {
     Piece<T, VEC> piece[U];
+    if constexpr (WIDE) {   // (else every copy's pieces are others)
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int c = c0 + (u * kRowThreads + threadIdx.x) * VEC;
-      if (c < c1) piece[u].load(x + t * p.ldx + c);
+      for (int u = 0; u < U; ++u) {
+        const int c = (i0 + u * kRowThreads + threadIdx.x) * VEC;
+        if (c < p.cols) load_piece<T, WIDE>(piece[u], x + t * p.ldx, c, p.cols);
+      }
     }
     if constexpr (SORT) {
       __syncthreads();
@@ -393,30 +524,41 @@ __global__ void __launch_bounds__(kRowThreads) dispatch_kernel(const __grid_cons
     for (int j = 0; j < p.top; ++j) {
       const int row = SORT ? place[j] : p.position[t * p.top + j];
       if (!has_row(p, row)) continue;
+      T* to = out + (long long)row * p.ldo;
+      const int first = first_piece<T, WIDE>(to);
+      if constexpr (!WIDE) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int c = first + (i0 + u * kRowThreads + threadIdx.x) * VEC;
+          if (c < p.cols) load_piece<T, WIDE>(piece[u], x + t * p.ldx, c, p.cols);
+        }
+      }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int c = c0 + (u * kRowThreads + threadIdx.x) * VEC;
-        if (c < c1) piece[u].store(out + (long long)row * p.ldo + c);
+        const int c = first + (i0 + u * kRowThreads + threadIdx.x) * VEC;
+        if (c < p.cols) store_piece<T, WIDE>(piece[u], to, c, p.cols);
       }
     }
   }
   if (p.zero_rest) {
     if constexpr (SORT) __syncthreads();
-    zero_rest<T, VEC>(p, SORT ? rows_used : *p.used, c0, c1);
+    zero_rest<T, WIDE>(p, SORT ? rows_used : *p.used, i0, i0 + kRowThreads * U);
   }
 }
 
 constexpr int kTogether = 4;   // rows of a token whose loads are in flight together
 
-template <typename T, int VEC>
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kRowThreads) combine_kernel(const __grid_constant__ RowParams p) {
-  constexpr int U = kHeld<VEC>;
+  constexpr int VEC = 16 / (int)sizeof(T), U = kHeld;
   grid_dependency_wait();
   grid_launch_dependents();
-  const int c0 = blockIdx.y * (kRowThreads * VEC * U);
+  const int i0 = blockIdx.y * (kRowThreads * U);
   const T* ys = reinterpret_cast<const T*>(p.x);
   T* out = reinterpret_cast<T*>(p.out);
   for (long long t = blockIdx.x; t < p.tokens; t += gridDim.x) {
+    T* to = out + t * p.ldo;
+    const int c0 = first_piece<T, WIDE>(to) + i0 * VEC;
     float sum[U][VEC];
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -439,7 +581,7 @@ __global__ void __launch_bounds__(kRowThreads) combine_kernel(const __grid_const
         Piece<T, VEC> piece[kTogether];
 #pragma unroll
         for (int k = 0; k < kTogether; ++k)
-          if (row[k] >= 0) piece[k].load(ys + (long long)row[k] * p.ldx + c);
+          if (row[k] >= 0) load_piece<T, WIDE>(piece[k], ys + (long long)row[k] * p.ldx, c, p.cols);
 #pragma unroll
         for (int k = 0; k < kTogether; ++k)
           if (row[k] >= 0) {   // (a dropped choice's weight may be anything)
@@ -455,11 +597,20 @@ __global__ void __launch_bounds__(kRowThreads) combine_kernel(const __grid_const
       if (p.residual != nullptr) {
         if (p.residual_elem == VOID_ELEM_F32 && sizeof(T) != 4) {
           const float* r = reinterpret_cast<const float*>(p.residual) + t * p.ldr + c;
+          if constexpr (WIDE) {
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) sum[u][e] += r[e];
+            for (int e = 0; e < VEC; e += 4) {
+              const float4 v = *reinterpret_cast<const float4*>(r + e);
+              sum[u][e] += v.x; sum[u][e + 1] += v.y; sum[u][e + 2] += v.z; sum[u][e + 3] += v.w;
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+              if (c + e >= 0 && c + e < p.cols) sum[u][e] += r[e];
+          }
         } else {
           Piece<T, VEC> r;
-          r.load(reinterpret_cast<const T*>(p.residual) + t * p.ldr + c);
+          load_piece<T, WIDE>(r, reinterpret_cast<const T*>(p.residual) + t * p.ldr, c, p.cols);
 #pragma unroll
           for (int e = 0; e < VEC; ++e) sum[u][e] += r.get(e);
         }
@@ -467,64 +618,69 @@ __global__ void __launch_bounds__(kRowThreads) combine_kernel(const __grid_const
       Piece<T, VEC> y;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) y.set(e, sum[u][e]);
-      y.store(out + t * p.ldo + c);
+      store_piece<T, WIDE>(y, to, c, p.cols);
     }
   }
 }
 
-// A block per token: dy is read once (and again from the first cache for more than four choices), the rows of its choices meet it.
-template <typename T, int VEC>
+// A block per token: dy is read once (and again from the first cache for more than four choices), the rows of its choices meet it.  Rows that lie
+// anyhow (not WIDE) are taken one by one, each with its own pieces.
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kRowThreads) combine_grad_kernel(const __grid_constant__ RowParams p) {
-  __shared__ float part[kTogether][kRowThreads / 32];
+  constexpr int VEC = 16 / (int)sizeof(T), TOGETHER = WIDE ? kTogether : 1;
+  __shared__ float part[TOGETHER][kRowThreads / 32];
   grid_dependency_wait();
   grid_launch_dependents();
   const T *ys = reinterpret_cast<const T*>(p.x), *g = reinterpret_cast<const T*>(p.g);
   T* out = reinterpret_cast<T*>(p.out);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (long long t = blockIdx.x; t < p.tokens; t += gridDim.x) {
-    for (int j0 = 0; j0 < p.top; j0 += kTogether) {
-      int row[kTogether];
-      float w[kTogether], dot[kTogether];
+    for (int j0 = 0; j0 < p.top; j0 += TOGETHER) {
+      int row[TOGETHER];
+      float w[TOGETHER], dot[TOGETHER];
 #pragma unroll
-      for (int k = 0; k < kTogether; ++k) {
+      for (int k = 0; k < TOGETHER; ++k) {
         const bool in = j0 + k < p.top;
         row[k] = in ? p.position[t * p.top + j0 + k] : -1;
         if (!has_row(p, row[k])) row[k] = -1;
         w[k] = in && p.weights != nullptr ? element(p.weights, p.weight_elem, t * p.top + j0 + k) : 1.0f;
         dot[k] = 0.0f;
       }
+      const T* lies = WIDE || row[0] < 0 ? g : (out != nullptr ? out + (long long)row[0] * p.ldo : ys + (long long)row[0] * p.ldx);
+      const int first = WIDE ? 0 : first_piece<T, WIDE>(lies), end = !WIDE && row[0] < 0 ? first : p.cols;
 #pragma unroll 2
-      for (int c = threadIdx.x * VEC; c < p.cols; c += kRowThreads * VEC) {
-        Piece<T, VEC> d, y[kTogether];
-        d.load(g + t * p.ldg + c);
+      for (int c = first + (int)threadIdx.x * VEC; c < end; c += kRowThreads * VEC) {
+        Piece<T, VEC> d, y[TOGETHER];
+        load_piece<T, WIDE>(d, g + t * p.ldg, c, p.cols);
         if (p.dw != nullptr) {
 #pragma unroll
-          for (int k = 0; k < kTogether; ++k)
-            if (row[k] >= 0) y[k].load(ys + (long long)row[k] * p.ldx + c);
+          for (int k = 0; k < TOGETHER; ++k)
+            if (row[k] >= 0) load_piece<T, WIDE>(y[k], ys + (long long)row[k] * p.ldx, c, p.cols);
         }
 #pragma unroll
-        for (int k = 0; k < kTogether; ++k) {
+        for (int k = 0; k < TOGETHER; ++k) {
           if (row[k] < 0) continue;
           if (p.dw != nullptr) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) dot[k] = fmaf(d.get(e), y[k].get(e), dot[k]);
+            for (int e = 0; e < VEC; ++e)
+              if (WIDE || (c + e >= 0 && c + e < p.cols)) dot[k] = fmaf(d.get(e), y[k].get(e), dot[k]);
           }
           if (out != nullptr) {
             Piece<T, VEC> q;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) q.set(e, w[k] * d.get(e));
-            q.store(out + (long long)row[k] * p.ldo + c);
+            store_piece<T, WIDE>(q, out + (long long)row[k] * p.ldo, c, p.cols);
           }
         }
       }
       if (p.dw != nullptr) {
 #pragma unroll
-        for (int k = 0; k < kTogether; ++k) {
+        for (int k = 0; k < TOGETHER; ++k) {
           const float s = warp_sum(dot[k]);
           if (lane == 0) part[k][warp] = s;
         }
         __syncthreads();
-        if (threadIdx.x < kTogether && j0 + (int)threadIdx.x < p.top) {
+        if (threadIdx.x < TOGETHER && j0 + (int)threadIdx.x < p.top) {
           float s = 0.0f;
 #pragma unroll
           for (int i = 0; i < kRowThreads / 32; ++i) s += part[threadIdx.x][i];
@@ -534,7 +690,7 @@ __global__ void __launch_bounds__(kRowThreads) combine_grad_kernel(const __grid_
       }
     }
   }
-  if (out != nullptr && p.zero_rest) zero_rest<T, VEC>(p, *p.used, 0, p.cols);
+  if (out != nullptr && p.zero_rest) zero_rest<T, WIDE>(p, *p.used, 0, (p.cols + VEC - 1) / VEC + 1);
 }
 
 // Whether rows of `elem_bytes` elements lie in whole 16-byte pieces.
@@ -542,27 +698,28 @@ inline bool in_pieces(const void* at, long long ld, int elem_bytes) { return ((r
 inline int elem_size(int elem) { return elem == VOID_ELEM_F32 ? 4 : 2; }
 
 enum class RowOp { Dispatch, DispatchSort32, DispatchSort64, Combine, CombineGrad };
-template <typename T, int VEC>
+template <typename T, bool WIDE>
 cudaError_t launch_rows(RowOp op, const RowParams& p, int sms, cudaStream_t st) {
-  const long long width = (long long)kRowThreads * VEC * kHeld<VEC>;
-  const unsigned parts = op == RowOp::CombineGrad ? 1u : (unsigned)((p.cols + width - 1) / width);
+  constexpr int VEC = 16 / (int)sizeof(T);
+  const long long pieces = ((long long)p.cols + VEC - 1) / VEC + (WIDE ? 0 : 1), width = kRowThreads * kHeld;
+  const unsigned parts = op == RowOp::CombineGrad ? 1u : (unsigned)((pieces + width - 1) / width);
   const long long most = 64ll * sms;
   const dim3 grid((unsigned)(p.tokens < most ? p.tokens : most), parts);
   switch (op) {
-    case RowOp::Dispatch: return launch_pdl(dispatch_kernel<T, VEC, int32_t, false>, grid, kRowThreads, 0, st, p);
-    case RowOp::DispatchSort32: return launch_pdl(dispatch_kernel<T, VEC, int32_t, true>, grid, kRowThreads, 0, st, p);
-    case RowOp::DispatchSort64: return launch_pdl(dispatch_kernel<T, VEC, int64_t, true>, grid, kRowThreads, 0, st, p);
-    case RowOp::Combine: return launch_pdl(combine_kernel<T, VEC>, grid, kRowThreads, 0, st, p);
-    default: return launch_pdl(combine_grad_kernel<T, VEC>, grid, kRowThreads, 0, st, p);
+    case RowOp::Dispatch: return launch_pdl(dispatch_kernel<T, WIDE, int32_t, false>, grid, kRowThreads, 0, st, p);
+    case RowOp::DispatchSort32: return launch_pdl(dispatch_kernel<T, WIDE, int32_t, true>, grid, kRowThreads, 0, st, p);
+    case RowOp::DispatchSort64: return launch_pdl(dispatch_kernel<T, WIDE, int64_t, true>, grid, kRowThreads, 0, st, p);
+    case RowOp::Combine: return launch_pdl(combine_kernel<T, WIDE>, grid, kRowThreads, 0, st, p);
+    default: return launch_pdl(combine_grad_kernel<T, WIDE>, grid, kRowThreads, 0, st, p);
   }
 }
 template <typename T>
 int rows_of_type(RowOp op, const RowParams& p, bool wide, int sms, cudaStream_t st) {
-  return status_of(wide ? launch_rows<T, 16 / (int)sizeof(T)>(op, p, sms, st) : launch_rows<T, 1>(op, p, sms, st));
+  return status_of(wide ? launch_rows<T, true>(op, p, sms, st) : launch_rows<T, false>(op, p, sms, st));
 }
 int rows_launch(RowOp op, RowParams& p, int elem, cudaStream_t st) {
   if (elem < VOID_ELEM_F32 || elem > VOID_ELEM_BF16 || p.tokens < 0 || p.top < 1 || p.cols < 0) return VOID_ERR_BAD_ARG;
-  if (p.tokens > 0x7fffffffll / p.top) return VOID_ERR_TOO_LARGE;
+  if (p.tokens > 0x7fffffffll / p.top || p.cols > 100000000) return VOID_ERR_TOO_LARGE;   // (blocks along a row)
   p.rows = p.tokens * p.top;
   const bool combine = op == RowOp::Combine, grad = op == RowOp::CombineGrad;
   if (p.tokens > 1 && ((p.ldx < p.cols && (combine || p.x != nullptr)) || (p.out != nullptr && p.ldo < p.cols) || (grad && p.ldg < p.cols) || (p.residual != nullptr && p.ldr < p.cols)))
@@ -579,27 +736,48 @@ int rows_launch(RowOp op, RowParams& p, int elem, cudaStream_t st) {
   return elem == VOID_ELEM_F16 ? rows_of_type<__half>(op, p, wide, dev.sms, st) : rows_of_type<__nv_bfloat16>(op, p, wide, dev.sms, st);
 }
 
-int sort_launch(SortParams p, int index_bytes, void* ws, size_t ws_bytes, cudaStream_t st) {
+template <typename I, int STEPS>
+int launch_sort_cluster(SortParams p, cudaStream_t st) {
+  int blocks = 1;
+  while ((long long)blocks * kSortThreads * STEPS < p.count) blocks *= 2;
+  p.share = (long long)kSortThreads * STEPS;
+  const int smem = 32 * p.pitch * 2;
+  if (ensure_smem(reinterpret_cast<const void*>(sort_cluster_kernel<I, STEPS>), smem) != 0) return VOID_ERR_CUDA;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(kSortThreads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)blocks;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return status_of(cudaLaunchKernelEx(&cfg, sort_cluster_kernel<I, STEPS>, p));
+}
+template <typename I>
+int sort_of_index(SortParams p, void* ws, size_t ws_bytes, int sms, cudaStream_t st) {
+  p.pitch = 2 * ((p.n_experts + 1) / 2 | 1);   // an odd number of words: a warp adds up a column without conflicts
+  if (p.count <= kSortCluster * kSortThreads) return launch_sort_cluster<I, 1>(p, st);
+  if (p.count <= kMostInCluster) return launch_sort_cluster<I, kSortSteps>(p, st);
+  const int blocks = sort_blocks(p.count, sms < kMaxSortBlocks ? sms : kMaxSortBlocks), smem = 32 * p.pitch * 2 + 4 * p.n_experts;
+  p.share = sort_share(p.count, blocks);
+  if (ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 3u) != 0 || ws_bytes < (size_t)blocks * p.n_experts * 4) return VOID_ERR_WORKSPACE;
+  p.table = reinterpret_cast<int32_t*>(ws);
+  const cudaError_t rc = launch_pdl(sort_count_kernel<I>, blocks, kSortThreads, 0, st, p);
+  if (rc != cudaSuccess) return VOID_ERR_CUDA;
+  if (ensure_smem(reinterpret_cast<const void*>(sort_place_kernel<I>), smem) != 0) return VOID_ERR_CUDA;
+  return status_of(launch_pdl(sort_place_kernel<I>, blocks, kSortThreads, smem, st, p));
+}
+int sort_launch(const SortParams& p, int index_bytes, void* ws, size_t ws_bytes, cudaStream_t st) {
   const DeviceInfo dev = device_info();
   if (!dev.ok) return VOID_ERR_CUDA;
   if (dev.cc_major != 10) return VOID_ERR_ARCH;
-  const int sms = dev.sms < kMaxSortBlocks ? dev.sms : kMaxSortBlocks, blocks = sort_blocks(p.count, sms);
-  p.share = sort_share(p.count, blocks);
-  p.pitch = 2 * ((p.n_experts + 1) / 2 | 1);   // an odd number of words: a warp adds up a column without conflicts
-  const int smem = 32 * p.pitch * 2 + 4 * p.n_experts;
-  if (blocks > 1) {
-    if (ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 3u) != 0 || ws_bytes < (size_t)blocks * p.n_experts * 4) return VOID_ERR_WORKSPACE;
-    p.table = reinterpret_cast<int32_t*>(ws);
-    const cudaError_t rc = index_bytes == 4 ? launch_pdl(sort_count_kernel<int32_t>, blocks, kSortThreads, 0, st, p)
-                                            : launch_pdl(sort_count_kernel<int64_t>, blocks, kSortThreads, 0, st, p);
-    if (rc != cudaSuccess) return VOID_ERR_CUDA;
-  }
-  if (index_bytes == 4) {
-    if (ensure_smem(reinterpret_cast<const void*>(sort_place_kernel<int32_t>), smem) != 0) return VOID_ERR_CUDA;
-    return status_of(launch_pdl(sort_place_kernel<int32_t>, blocks, kSortThreads, smem, st, p));
-  }
-  if (ensure_smem(reinterpret_cast<const void*>(sort_place_kernel<int64_t>), smem) != 0) return VOID_ERR_CUDA;
-  return status_of(launch_pdl(sort_place_kernel<int64_t>, blocks, kSortThreads, smem, st, p));
+  return index_bytes == 4 ? sort_of_index<int32_t>(p, ws, ws_bytes, dev.sms, st) : sort_of_index<int64_t>(p, ws, ws_bytes, dev.sms, st);
 }
 // The arguments of a sort, or why not.
 int check_sort(const void* experts, int32_t index_bytes, int64_t count, int32_t n_experts, const int32_t* offsets, const int32_t* position) {
@@ -631,8 +809,7 @@ int void_route_grad(const void* scores, int32_t elem, int64_t lds, int64_t rows,
 
 size_t void_sort_by_expert_ws_bytes(int64_t count, int32_t n_experts) {
   if (count < 0 || n_experts < 1) return 0;
-  const int blocks = vb::sort_blocks(count, vb::kMaxSortBlocks);
-  return blocks > 1 ? (size_t)blocks * n_experts * 4 : 0;
+  return count > vb::kMostInCluster ? (size_t)vb::sort_blocks(count, vb::kMaxSortBlocks) * n_experts * 4 : 0;
 }
 int void_sort_by_expert(const void* experts, int32_t index_bytes, int64_t count, int32_t n_experts, int32_t* offsets, int32_t* position, void* ws,
                         size_t ws_bytes, void_stream_t stream) {
