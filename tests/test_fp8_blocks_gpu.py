@@ -165,6 +165,38 @@ def test_weights_are_read_at_the_call():
     assert (void.void_linear(w, x) == 0).all()
 
 
+def test_weights_scales_and_biases_written_just_before():
+    """The product reads its weights ahead of the end of the kernel that quantises x: nothing else may still be under way then."""
+    n, m, k = 24, 4096, 4096
+    given = [_weights(m, k, s) for s in (1, 2)]
+    biases = [torch.randn(m, generator=_gen(s), device="cuda") for s in (3, 4)]
+    x = torch.randn(n, k, generator=_gen(5), device="cuda")
+    want = [void.void_linear(w, x, b) for w, b in zip(given, biases)]
+    w, bias = void.FP8BlockTensor(given[0].values.clone(), given[0].scales.clone()), biases[0].clone()
+    got = []
+    for i in range(40):
+        bias.copy_(biases[i % 2])
+        w.scales.copy_(given[i % 2].scales)
+        w.values.view(torch.uint8).copy_(given[i % 2].values.view(torch.uint8))
+        got.append(void.void_linear(w, x, bias))
+    for i, y in enumerate(got):
+        assert torch.equal(y, want[i % 2]), i
+    # and what the operator itself brings into place: a residual that is copied, biases of another type, a plan of many experts
+    E = 40
+    experts = void.quantize_fp8_blocks(torch.randn(E, 128, 256, generator=_gen(6), device="cuda"))
+    tokens = torch.randn(400, 256, generator=_gen(7), device="cuda")
+    offsets = torch.arange(E + 1, device="cuda") * 10
+    want = void.void_expert_linear(experts, tokens, offsets)
+    for _ in range(20):
+        offsets.zero_()
+        offsets.add_(torch.arange(E + 1, device="cuda") * 10)
+        assert torch.equal(void.void_expert_linear(experts, tokens, offsets), want)
+    r = torch.randn(m, n, generator=_gen(8), device="cuda").double()
+    want = void.void_linear(w, x, bias.float(), residual=r.t().float().contiguous())
+    for _ in range(20):
+        assert torch.equal(void.void_linear(w, x, bias.double(), residual=r.float().t()), want)
+
+
 def test_results_that_are_given():
     w = _weights(300, 256, 7)
     x = torch.randn(40, 256, generator=_gen(8), device="cuda").half()

@@ -120,4 +120,4 @@ def test_routes_that_were_written_to_are_refused():
 
 
 def test_mirror_is_the_header():
-    assert ctypes.sizeof(_lib.Fp8Args) == 176
+    assert ctypes.sizeof(_lib.Fp8Args) == 184

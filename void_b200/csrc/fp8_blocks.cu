@@ -220,6 +220,7 @@ struct Fp8Params {
   int out_elem, act;
   int splits;                     // CTAs of a cluster, which share an item's blocks of k
   int stages;
+  int early;                      // what is read but the tokens and their scales was complete before the kernel in flight started
   int32_t* status;
   int wait_limit_ms, drop_first;  // drop_first: test hook, the first stage is never filled
 };
@@ -379,29 +380,42 @@ __global__ void __launch_bounds__(kThreads, CTAS) fp8_block_kernel(const __grid_
   const uint32_t tmem = tmem_s;
   const int rank = p.splits > 1 ? (int)cluster_rank() : 0;
   const int b0 = (int)((long long)p.k_blocks * rank / p.splits), b1 = (int)((long long)p.k_blocks * (rank + 1) / p.splits);
-  grid_dependency_wait();
+  if (!p.early) grid_dependency_wait();
   find_runs(p, runs);
   const int step = (int)gridDim.x / p.splits, begin = (int)blockIdx.x / p.splits, end = items_of(p, runs);
   // With several CTAs per item a launch has a cluster for every item, so that the ring is free when the sums meet in its place.
   if (warp == 0) {
-    int stage = 0;
+    int stage = 0, ahead = 0;   // ahead: stages whose weights have been asked for already
     uint32_t phase = 0;
     bool first = true;
+    auto weights = [&](const Item& t, int b, int s, int boxes) {
+      const uint32_t full = smem_u32(&bars.full[s]);
+      mbar_expect_tx(full, kStageA + (uint32_t)boxes * (kTokenBox * kBlock));
+      tma_load_3d(ring + (uint32_t)s * kStage, &map_a, b * kBlock, t.m * kBlock, t.expert, full);
+    };
+    if (p.early) {   // the ring's first weights, while the tokens are still being quantised
+      if (begin < end && !p.drop_first) {
+        const Item t = item_at(p, runs, begin);
+        ahead = min(p.stages, b1 - b0);
+        if (lane == 0)
+          for (int s = 0; s < ahead; ++s) weights(t, b0 + s, s, (t.n1 - t.n0 + kTokenBox - 1) / kTokenBox);
+        __syncwarp();
+      }
+      grid_dependency_wait();
+    }
     for (int i = begin; i < end && !ctl[0]; i += step) {
       const Item t = item_at(p, runs, i);
       const int boxes = (t.n1 - t.n0 + kTokenBox - 1) / kTokenBox;
       for (int b = b0; b < b1; ++b) {
         if (!mbar_wait_warp(smem_u32(&bars.empty[stage]), phase ^ 1u, ctl)) break;
-        const uint32_t full = smem_u32(&bars.full[stage]), at = ring + (uint32_t)stage * kStage;
         const bool drop = first && p.drop_first != 0;
         first = false;
-        if (lane == 0 && !drop) mbar_expect_tx(full, kStageA + (uint32_t)boxes * (kTokenBox * kBlock));
+        if (ahead > 0) --ahead;
+        else if (lane == 0 && !drop) weights(t, b, stage, boxes);
         __syncwarp();
-        if (!drop) {
-          if (lane == 0) tma_load_3d(at, &map_a, b * kBlock, t.m * kBlock, t.expert, full);
-          if (lane >= 1 && lane <= boxes)
-            tma_load_2d(at + kStageA + (uint32_t)(lane - 1) * (kTokenBox * kBlock), &map_x, b * kBlock, t.n0 + (lane - 1) * kTokenBox, full);
-        }
+        if (lane >= 1 && lane <= boxes && !drop)
+          tma_load_2d(ring + (uint32_t)stage * kStage + kStageA + (uint32_t)(lane - 1) * (kTokenBox * kBlock), &map_x, b * kBlock, t.n0 + (lane - 1) * kTokenBox,
+                      smem_u32(&bars.full[stage]));
         if (++stage == p.stages) { stage = 0; phase ^= 1u; }
       }
     }
@@ -432,6 +446,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) fp8_block_kernel(const __grid_
   } else if (warp < kFirstAdder) {
     // The products of both scales, every other block of k for either warp; those of the next block are on their way meanwhile.
     constexpr int PER = (NT + 31) / 32;
+    if (p.early) grid_dependency_wait();
     uint32_t it0 = 0;
     bool ok = true;
     for (int i = begin; i < end && ok; i += step) {
@@ -593,6 +608,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) fp8_block_kernel(const __grid_
     __syncwarp();
     cluster_meet();   // (nobody leaves while others read its sums)
   }
+  if (p.early) grid_dependency_wait();
   zero_tokens_in_no_run(p, runs);
   grid_launch_dependents();
   tc_fence_before();
@@ -792,7 +808,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_wide_kernel(const __grid_cons
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_s;
-  grid_dependency_wait();
+  if (!p.early) grid_dependency_wait();
   find_runs(p, runs);
 
   const int rank = p.splits > 1 ? (int)cluster_rank() : 0;
@@ -801,24 +817,38 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_wide_kernel(const __grid_cons
   // (4 * 56 + 8 * 224 = 12 * 168, what the block was launched with)
   if (warp >= kAdders) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
   if (warp == kCopier) {
-    int stage = 0;
+    int stage = 0, ahead = 0;   // ahead: stages whose weights have been asked for already
     uint32_t phase = 0;
     bool first = true;
+    auto weights = [&](const Item& t, int b, int s) {
+      const int m0 = t.m * kWideFeatures, halves = p.M - m0 > kBlock ? 2 : 1, boxes = (t.n1 - t.n0 + kTokenBox - 1) / kTokenBox;
+      const uint32_t full = smem_u32(&bars.full[s]), at = ring + (uint32_t)s * kWideStage + kWideTokens * kBlock;
+      mbar_expect_tx(full, (uint32_t)(halves * kBlock + boxes * kTokenBox) * kBlock);
+      for (int h = 0; h < halves; ++h) tma_load_3d(at + (uint32_t)h * (kBlock * kBlock), &map_a, b * kBlock, m0 + h * kBlock, t.expert, full);
+    };
+    if (p.early) {   // the ring's first weights, while the tokens are still being quantised
+      if (begin < end && !p.drop_first) {
+        const Item t = item_at(p, runs, begin);
+        ahead = min(p.stages, b1 - b0);
+        if (lane == 0)
+          for (int s = 0; s < ahead; ++s) weights(t, b0 + s, s);
+        __syncwarp();
+      }
+      grid_dependency_wait();
+    }
     for (int i = begin; i < end && !ctl[0]; i += step) {
       const Item t = item_at(p, runs, i);
-      const int boxes = (t.n1 - t.n0 + kTokenBox - 1) / kTokenBox, m0 = t.m * kWideFeatures, halves = p.M - m0 > kBlock ? 2 : 1;
+      const int boxes = (t.n1 - t.n0 + kTokenBox - 1) / kTokenBox;
       for (int b = b0; b < b1; ++b) {
         if (!mbar_wait_warp(smem_u32(&bars.empty[stage]), phase ^ 1u, ctl)) break;
-        const uint32_t full = smem_u32(&bars.full[stage]), at = ring + (uint32_t)stage * kWideStage;
         const bool drop = first && p.drop_first != 0;
         first = false;
-        if (lane == 0 && !drop) mbar_expect_tx(full, (uint32_t)(halves * kBlock + boxes * kTokenBox) * kBlock);
+        if (ahead > 0) --ahead;
+        else if (lane == 0 && !drop) weights(t, b, stage);
         __syncwarp();
-        if (!drop) {
-          if (lane < halves) tma_load_3d(at + kWideTokens * kBlock + (uint32_t)lane * (kBlock * kBlock), &map_a, b * kBlock, m0 + lane * kBlock, t.expert, full);
-          else if (lane >= 4 && lane < 4 + boxes)
-            tma_load_2d(at + (uint32_t)(lane - 4) * (kTokenBox * kBlock), &map_x, b * kBlock, t.n0 + (lane - 4) * kTokenBox, full);
-        }
+        if (lane >= 1 && lane <= boxes && !drop)
+          tma_load_2d(ring + (uint32_t)stage * kWideStage + (uint32_t)(lane - 1) * (kTokenBox * kBlock), &map_x, b * kBlock, t.n0 + (lane - 1) * kTokenBox,
+                      smem_u32(&bars.full[stage]));
         if (++stage == p.stages) { stage = 0; phase ^= 1u; }
       }
     }
@@ -864,6 +894,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_wide_kernel(const __grid_cons
     }
   } else if (warp < kAdders) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    if (p.early) grid_dependency_wait();
     const int quad = warp & 3, side = warp >> 2;
     uint32_t it = 0, item = 0;
     bool ok = true;
@@ -1010,6 +1041,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_wide_kernel(const __grid_cons
     if (warp >= kAdders) cluster_meet();
     cluster_meet();   // (nobody leaves while others read its sums)
   }
+  if (p.early) grid_dependency_wait();
   zero_tokens_in_no_run(p, runs);
   grid_launch_dependents();
   tc_fence_before();
@@ -1036,8 +1068,7 @@ bool rows_map(CUtensorMap* m, const void* at, long long ld, long long expert, in
              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Launch with `splits` CTAs per item, in clusters.  Fewer items than half the places for CTAs: the blocks of k are shared, as long as every CTA has two of
-// them.
+// Launch with `splits` CTAs per item, in clusters: as many as there are places for, as long as every CTA has four blocks of k.
 // How many clusters of `splits` such CTAs a device holds at a time: a cluster lies within one of its groups of SMs, so some SMs are left over (36
 // clusters of four CTAs, one per SM, took two turns where 32 fit).
 int clusters_at_once(const void* kernel, int splits, int threads, int smem) {
@@ -1069,9 +1100,8 @@ int clusters_at_once(const void* kernel, int splits, int threads, int smem) {
 cudaError_t launch_split(void (*kernel)(Fp8Params, CUtensorMap, CUtensorMap), Fp8Params& p, const CUtensorMap& a, const CUtensorMap& x, long long items,
                          long long places, int threads, int smem, cudaStream_t st) {
   int splits = 1;
-  while (splits < 8 && p.k_blocks >= splits * 4 && items * splits * 2 <= places &&
-         items <= clusters_at_once(reinterpret_cast<const void*>(kernel), splits * 2, threads, smem))
-    splits *= 2;
+  for (int s = 8; s > 1 && splits == 1; --s)
+    if (items * s <= places && p.k_blocks >= 4 * s && items <= clusters_at_once(reinterpret_cast<const void*>(kernel), s, threads, smem)) splits = s;
   p.splits = splits;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(splits > 1 ? items * splits : (items < places ? items : places)));
@@ -1144,6 +1174,7 @@ int fp8_linear(const void_fp8_args* a, const void_experts* x, cudaStream_t st) {
   p.residual = a->residual; p.ldr = a->ldr; p.residual_elem = a->residual_elem;
   p.out = a->out; p.ldc = a->ldc; p.out_elem = a->out_elem; p.act = a->act;
   p.status = a->status;
+  p.early = a->x_in_flight;
   p.wait_limit_ms = (a->test_hooks & 0xffff) ? (a->test_hooks & 0xffff) : kDefaultWaitLimitMs;
   p.drop_first = (a->test_hooks >> 16) & 1;
   // Up to 64 tokens lie in the columns of the tensor memory, more of them in its lanes.

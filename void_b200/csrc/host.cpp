@@ -2347,21 +2347,7 @@ PyObject* fp8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t d = t.dim(), wide = (t.size(d - 1) + 15) / 16 * 16;
     return t.size(d - 2) > 1 ? t.stride(d - 2) : wide;
   };
-  if (none(a[3])) {   // x is quantised first: values and scales in one workspace
-    const at::Tensor rows = token_rows(x_in);
-    const int64_t padded = (N + 3) / 4 * 4;
-    s.ldx = (K + 15) / 16 * 16;
-    const int64_t values_bytes = (N * s.ldx + 255) / 256 * 256;
-    workspace = new_cuda({values_bytes + (K + 127) / 128 * padded * 4}, at::kByte, dev);
-    uint8_t* at = static_cast<uint8_t*>(workspace.data_ptr());
-    float* sx = reinterpret_cast<float*>(at + values_bytes);
-    check(void_quant_fp8_blocks(rows.const_data_ptr(), out_code(rows.scalar_type()), row_step(rows), N, (int32_t)K, 1, at, s.ldx, sx, 1, padded, stream_of(dev.index())),
-          "void_quant_fp8_blocks");
-    s.x = at;
-    s.x_scale = sx;
-    s.x_scale_row = 1;
-    s.x_scale_col = padded;
-  } else {
+  if (!none(a[3])) {
     if (x_in.scalar_type() != at::kFloat8_e4m3fn) fail("quantised tokens are float8_e4m3fn");
     x = laid_out(x_in);
     x_scales = cuda_tensor(a[3], "x's scales");
@@ -2430,6 +2416,22 @@ PyObject* fp8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (runs) {
     plan = expert_plan(cuda_tensor(a[4], "offsets"), N, E, dev, s.status, true, fp8_chunk(N, E));
     plan.x.zero_rest = none(a[7]) ? 1 : 0;
+  }
+  if (none(a[3])) {   // x is quantised first, values and scales in one workspace: the last launch before the product, which counts on that (x_in_flight)
+    const at::Tensor rows = token_rows(x_in);
+    const int64_t padded = (N + 3) / 4 * 4;
+    s.ldx = (K + 15) / 16 * 16;
+    const int64_t values_bytes = (N * s.ldx + 255) / 256 * 256;
+    workspace = new_cuda({values_bytes + (K + 127) / 128 * padded * 4}, at::kByte, dev);
+    uint8_t* at = static_cast<uint8_t*>(workspace.data_ptr());
+    float* sx = reinterpret_cast<float*>(at + values_bytes);
+    check(void_quant_fp8_blocks(rows.const_data_ptr(), out_code(rows.scalar_type()), row_step(rows), N, (int32_t)K, 1, at, s.ldx, sx, 1, padded, stream_of(dev.index())),
+          "void_quant_fp8_blocks");
+    s.x = at;
+    s.x_in_flight = N > 0 ? 1 : 0;
+    s.x_scale = sx;
+    s.x_scale_row = 1;
+    s.x_scale_col = padded;
   }
   check(void_fp8_linear(&s, runs ? &plan.x : nullptr, stream_of(dev.index())), "void_fp8_linear");
   if (!target.is_same(out)) out.copy_(target);
