@@ -341,6 +341,15 @@ def test_captured_products_of_two_graphs():
         assert torch.equal(results[0], want) and torch.equal(results[1], want)
 
 
+def test_a_capture_without_a_call_before():
+    w, x = _weights(1536, 1300, 1), torch.randn(11, 1300, generator=_gen(2), device="cuda")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = void.void_linear(w, x)
+    g.replay()
+    assert torch.equal(y, void.void_linear(w, x))
+
+
 def test_streams():
     w = _weights(1000, 2000, 1)
     x = torch.randn(40, 2000, generator=_gen(2), device="cuda")

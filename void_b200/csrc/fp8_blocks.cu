@@ -1068,10 +1068,10 @@ bool rows_map(CUtensorMap* m, const void* at, long long ld, long long expert, in
              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Launch with `splits` CTAs per item, in clusters: as many as there are places for, as long as every CTA has four blocks of k.
 // How many clusters of `splits` such CTAs a device holds at a time: a cluster lies within one of its groups of SMs, so some SMs are left over (36
-// clusters of four CTAs, one per SM, took two turns where 32 fit).
-int clusters_at_once(const void* kernel, int splits, int threads, int smem) {
+// clusters of four CTAs, one per SM, took two turns where 33 fit).  For kernels that hold tensor memory
+// the runtime answers for one CTA per SM.
+int clusters_at_once(const void* kernel, int splits, int smem) {
   struct Rec { const void* fn; int dev, splits, smem, clusters; };
   static Rec recs[256];
   static int n_recs = 0;
@@ -1083,7 +1083,7 @@ int clusters_at_once(const void* kernel, int splits, int threads, int smem) {
     if (recs[i].fn == kernel && recs[i].dev == dev && recs[i].splits == splits && recs[i].smem == smem) return recs[i].clusters;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)splits);
-  cfg.blockDim = dim3((unsigned)threads);
+  cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = (size_t)smem;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1097,15 +1097,21 @@ int clusters_at_once(const void* kernel, int splits, int threads, int smem) {
   if (n_recs < 256) recs[n_recs++] = {kernel, dev, splits, smem, clusters};
   return clusters;
 }
+// Launch with `splits` CTAs per item, in clusters: as many as there are SMs for, as long as every CTA has four blocks of k, or places (`ctas` per SM) if
+// it still has `least`.  8 tokens, 16384^2 51.5 us with one CTA per SM, 48.2 with two of 64 blocks each; 8192^2 16.7 and 17.2 (16 blocks); 40 tokens, 8192^2 23.6
+// and 20.7; 60 tokens, 4096^2 11.7 and 13.2 (4 blocks).
 cudaError_t launch_split(void (*kernel)(Fp8Params, CUtensorMap, CUtensorMap), Fp8Params& p, const CUtensorMap& a, const CUtensorMap& x, long long items,
-                         long long places, int threads, int smem, cudaStream_t st) {
+                         const DeviceInfo& dev, int ctas, int least, int smem, cudaStream_t st) {
+  const long long places = (long long)dev.sms * ctas;
   int splits = 1;
   for (int s = 8; s > 1 && splits == 1; --s)
-    if (items * s <= places && p.k_blocks >= 4 * s && items <= clusters_at_once(reinterpret_cast<const void*>(kernel), s, threads, smem)) splits = s;
+    if (p.k_blocks >= 4 * s && (items * s <= dev.sms || (items * s <= places && p.k_blocks >= least * s)) &&
+        items <= ctas * clusters_at_once(reinterpret_cast<const void*>(kernel), s, smem))
+      splits = s;
   p.splits = splits;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(splits > 1 ? items * splits : (items < places ? items : places)));
-  cfg.blockDim = dim3((unsigned)threads);
+  cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
@@ -1135,7 +1141,7 @@ int launch_few(Fp8Params p, const CUtensorMap& a, const CUtensorMap& x, long lon
   const int smem = p.stages * kStage + 1024;
   if (p.stages < 2) return VOID_ERR_SHAPE;
   if (ensure_smem(reinterpret_cast<const void*>(fp8_block_kernel<NT, CTAS>), smem) != 0) return VOID_ERR_CUDA;
-  return status_of(launch_split(fp8_block_kernel<NT, CTAS>, p, a, x, items, (long long)dev.sms * CTAS, kThreads, smem, st));
+  return status_of(launch_split(fp8_block_kernel<NT, CTAS>, p, a, x, items, dev, CTAS, NT == 32 ? 32 : 16, smem, st));
 }
 template <bool LOOSE>
 int launch_wide(Fp8Params p, const CUtensorMap& a, const CUtensorMap& x, long long items, const DeviceInfo& dev, cudaStream_t st) {
@@ -1144,7 +1150,7 @@ int launch_wide(Fp8Params p, const CUtensorMap& a, const CUtensorMap& x, long lo
   const int smem = p.stages * kStage + 1024;
   if (p.stages * kStage < kWideTokens * kWidePitch * 4) return VOID_ERR_SHAPE;
   if (ensure_smem(reinterpret_cast<const void*>(fp8_wide_kernel<LOOSE>), smem) != 0) return VOID_ERR_CUDA;
-  return status_of(launch_split(fp8_wide_kernel<LOOSE>, p, a, x, items, dev.sms, kThreads, smem, st));
+  return status_of(launch_split(fp8_wide_kernel<LOOSE>, p, a, x, items, dev, 1, 4, smem, st));
 }
 // Rows of results and residuals in pieces of 32 bytes.
 bool on_32_bytes(const void* at, long long ld, int elem) { return ((reinterpret_cast<uintptr_t>(at) | (uintptr_t)(ld * (elem == VOID_ELEM_F32 ? 4 : 2))) & 31u) == 0; }
