@@ -369,7 +369,8 @@ constexpr int kMaxSortBlocks = 256;
 // ------------------------------------------------------------------------------------------ rows of tokens
 constexpr int kRowThreads = 256;
 // 16-byte pieces of a row that one thread holds at a time.
-constexpr int kHeld = 2;
+template <bool WIDE>
+constexpr int kHeld = WIDE ? 2 : 1;
 // Choices that the sort's own block is not worth a launch for: every warp ranks its token's choices by counting.
 constexpr int kFewChoices = 1024;
 
@@ -399,39 +400,60 @@ struct RowParams {
 // Whether a choice has a row; positions are not trusted.
 __device__ __forceinline__ bool has_row(const RowParams& p, int row) { return row >= 0 && row < p.rows; }
 
-// 16 bytes of a row from column `c` on, whatever address that is: WIDE, rows that lie in 16-byte pieces, one load; others from the one or two aligned
-// pieces that hold them, shifted (all threads of a row by the same).  No piece is read that has no byte of the row in it; what is not the row's is
-// anything.
+// The 16-byte pieces of a row, from column `first` (at most 0) on, whatever address that is: WIDE, rows that lie in 16-byte pieces (first is 0), one
+// load each; others from the one or two aligned pieces that hold them, shifted (all threads of a row by the same).  No piece is read that has no byte
+// of the row in it; what is not the row's is anything.  In two steps, so that several loads are on their way together: the shift waits for its own.
 template <typename T, bool WIDE>
-__device__ __forceinline__ void load_piece(Piece<T, 16 / sizeof(T)>& piece, const T* row, int c, int cols) {
-  if constexpr (WIDE) {
-    piece.load(row + c);
-  } else {
-    const long long at = reinterpret_cast<long long>(row) + (long long)c * (int)sizeof(T);
-    const long long lo = reinterpret_cast<long long>(row), hi = lo + (long long)cols * (int)sizeof(T), base = at & ~15ll;
-    const int shift = (int)(at & 15);
-    uint4 u = make_uint4(0, 0, 0, 0), v = u;
-    if (base + 16 > lo && base < hi) u = *reinterpret_cast<const uint4*>(base);
-    if (shift != 0) {
-      if (base + 32 > lo && base + 16 < hi) v = *reinterpret_cast<const uint4*>(base + 16);
-      uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-      if (shift & 8) {
-#pragma unroll
-        for (int k = 0; k < 6; ++k) w[k] = w[k + 2];
-      }
-      if (shift & 4) {
-#pragma unroll
-        for (int k = 0; k < 5; ++k) w[k] = w[k + 1];
-      }
-      if (sizeof(T) == 2 && (shift & 2)) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(w[k], w[k + 1], 16);
-      }
-      u = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-    memcpy(piece.v, &u, 16);
+struct Row {
+  using Wanted = Piece<T, 16 / sizeof(T)>;
+  struct Raw {
+    Wanted piece;
+  };
+  const T* row;
+  __device__ __forceinline__ Row(const T* at, int, int) : row(at) {}
+  __device__ __forceinline__ void load(Raw& raw, int i) const { raw.piece.load(row + i * (16 / (int)sizeof(T))); }
+  __device__ __forceinline__ Wanted get(const Raw& raw) const { return raw.piece; }
+};
+template <typename T>
+struct Row<T, false> {
+  using Wanted = Piece<T, 16 / sizeof(T)>;
+  struct Raw {
+    uint4 u, v;
+  };
+  const uint4* base;
+  int shift, low, high;   // bytes; aligned pieces [low, high) hold the row
+  __device__ __forceinline__ Row(const T* row, int first, int cols) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(row) + (intptr_t)first * (intptr_t)sizeof(T), start = at & ~(uintptr_t)15;
+    base = reinterpret_cast<const uint4*>(start);
+    shift = (int)(at & 15u);
+    const long long lead = (long long)(reinterpret_cast<uintptr_t>(row) - start);
+    low = (int)(lead >> 4);
+    high = (int)((lead + (long long)cols * (int)sizeof(T) + 15) >> 4);
   }
-}
+  __device__ __forceinline__ void load(Raw& raw, int i) const {
+    raw.u = raw.v = make_uint4(0, 0, 0, 0);
+    if (i >= low && i < high) raw.u = base[i];
+    if (shift != 0 && i + 1 >= low && i + 1 < high) raw.v = base[i + 1];
+  }
+  __device__ __forceinline__ Wanted get(const Raw& raw) const {
+    uint32_t w[8] = {raw.u.x, raw.u.y, raw.u.z, raw.u.w, raw.v.x, raw.v.y, raw.v.z, raw.v.w};
+    if (shift & 8) {   // (branches: all threads take the same)
+#pragma unroll
+      for (int k = 0; k < 6; ++k) w[k] = w[k + 2];
+    }
+    if (shift & 4) {
+#pragma unroll
+      for (int k = 0; k < 5; ++k) w[k] = w[k + 1];
+    }
+    if (sizeof(T) == 2 && (shift & 2)) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(w[k], w[k + 1], 16);
+    }
+    Wanted piece;
+    memcpy(piece.v, w, 16);
+    return piece;
+  }
+};
 // The pieces of a row that is written begin at its aligned addresses, so the first may lie partly ahead of the row (c < 0), and the last behind it.
 template <typename T, bool WIDE>
 __device__ __forceinline__ int first_piece(const T* row) {
@@ -469,7 +491,7 @@ __device__ __forceinline__ void zero_rest(const RowParams& p, long long used, in
 // SORT (few choices): the rows are not known yet, each is the number of choices that come before it.
 template <typename T, bool WIDE, typename I, bool SORT>
 __global__ void __launch_bounds__(kRowThreads) dispatch_kernel(const __grid_constant__ RowParams p) {
-  constexpr int VEC = 16 / (int)sizeof(T), U = kHeld;
+  constexpr int VEC = 16 / (int)sizeof(T), U = kHeld<WIDE>;
   __shared__ int32_t ids[SORT ? kFewChoices : 1];
   __shared__ int32_t place[SORT ? kFewChoices : 1];   // of this token's choices
   __shared__ int32_t rows_used;
@@ -499,12 +521,13 @@ __global__ void __launch_bounds__(kRowThreads) dispatch_kernel(const __grid_cons
     }
   }
   for (long long t = blockIdx.x; t < p.tokens; t += gridDim.x) {
-    Piece<T, VEC> piece[U];
+    typename Row<T, WIDE>::Raw raw[U];
     if constexpr (WIDE) {   // (else every copy's pieces are others)
+      const Row<T, WIDE> token(x + t * p.ldx, 0, p.cols);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int c = (i0 + u * kRowThreads + threadIdx.x) * VEC;
-        if (c < p.cols) load_piece<T, WIDE>(piece[u], x + t * p.ldx, c, p.cols);
+        const int i = i0 + u * kRowThreads + threadIdx.x;
+        if (i * VEC < p.cols) token.load(raw[u], i);
       }
     }
     if constexpr (SORT) {
@@ -526,17 +549,18 @@ __global__ void __launch_bounds__(kRowThreads) dispatch_kernel(const __grid_cons
       if (!has_row(p, row)) continue;
       T* to = out + (long long)row * p.ldo;
       const int first = first_piece<T, WIDE>(to);
+      const Row<T, WIDE> token(x + t * p.ldx, first, p.cols);
       if constexpr (!WIDE) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int c = first + (i0 + u * kRowThreads + threadIdx.x) * VEC;
-          if (c < p.cols) load_piece<T, WIDE>(piece[u], x + t * p.ldx, c, p.cols);
+          const int i = i0 + u * kRowThreads + threadIdx.x;
+          if (first + i * VEC < p.cols) token.load(raw[u], i);
         }
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int c = first + (i0 + u * kRowThreads + threadIdx.x) * VEC;
-        if (c < p.cols) store_piece<T, WIDE>(piece[u], to, c, p.cols);
+        if (c < p.cols) store_piece<T, WIDE>(token.get(raw[u]), to, c, p.cols);
       }
     }
   }
@@ -550,7 +574,7 @@ constexpr int kTogether = 4;   // rows of a token whose loads are in flight toge
 
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kRowThreads) combine_kernel(const __grid_constant__ RowParams p) {
-  constexpr int VEC = 16 / (int)sizeof(T), U = kHeld;
+  constexpr int VEC = 16 / (int)sizeof(T), U = kHeld<WIDE>, TOGETHER = WIDE || sizeof(T) == 4 ? kTogether : 2;
   grid_dependency_wait();
   grid_launch_dependents();
   const int i0 = blockIdx.y * (kRowThreads * U);
@@ -558,17 +582,17 @@ __global__ void __launch_bounds__(kRowThreads) combine_kernel(const __grid_const
   T* out = reinterpret_cast<T*>(p.out);
   for (long long t = blockIdx.x; t < p.tokens; t += gridDim.x) {
     T* to = out + t * p.ldo;
-    const int c0 = first_piece<T, WIDE>(to) + i0 * VEC;
+    const int first = first_piece<T, WIDE>(to);
     float sum[U][VEC];
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) sum[u][e] = 0.0f;
-    for (int j0 = 0; j0 < p.top; j0 += kTogether) {
-      int row[kTogether];
-      float w[kTogether];
+    for (int j0 = 0; j0 < p.top; j0 += TOGETHER) {
+      int row[TOGETHER];
+      float w[TOGETHER];
 #pragma unroll
-      for (int k = 0; k < kTogether; ++k) {
+      for (int k = 0; k < TOGETHER; ++k) {
         const bool in = j0 + k < p.top;
         row[k] = in ? p.position[t * p.top + j0 + k] : -1;
         if (!has_row(p, row[k])) row[k] = -1;
@@ -576,23 +600,24 @@ __global__ void __launch_bounds__(kRowThreads) combine_kernel(const __grid_const
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int c = c0 + (u * kRowThreads + threadIdx.x) * VEC;
-        if (c >= p.cols) continue;
-        Piece<T, VEC> piece[kTogether];
+        const int i = i0 + u * kRowThreads + threadIdx.x;
+        if (first + i * VEC >= p.cols) continue;
+        typename Row<T, WIDE>::Raw raw[TOGETHER];
 #pragma unroll
-        for (int k = 0; k < kTogether; ++k)
-          if (row[k] >= 0) load_piece<T, WIDE>(piece[k], ys + (long long)row[k] * p.ldx, c, p.cols);
+        for (int k = 0; k < TOGETHER; ++k)
+          if (row[k] >= 0) Row<T, WIDE>(ys + (long long)row[k] * p.ldx, first, p.cols).load(raw[k], i);
 #pragma unroll
-        for (int k = 0; k < kTogether; ++k)
+        for (int k = 0; k < TOGETHER; ++k)
           if (row[k] >= 0) {   // (a dropped choice's weight may be anything)
+            const Piece<T, VEC> piece = Row<T, WIDE>(ys + (long long)row[k] * p.ldx, first, p.cols).get(raw[k]);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) sum[u][e] = fmaf(w[k], piece[k].get(e), sum[u][e]);
+            for (int e = 0; e < VEC; ++e) sum[u][e] = fmaf(w[k], piece.get(e), sum[u][e]);
           }
       }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int c = c0 + (u * kRowThreads + threadIdx.x) * VEC;
+      const int i = i0 + u * kRowThreads + threadIdx.x, c = first + i * VEC;
       if (c >= p.cols) continue;
       if (p.residual != nullptr) {
         if (p.residual_elem == VOID_ELEM_F32 && sizeof(T) != 4) {
@@ -609,8 +634,10 @@ __global__ void __launch_bounds__(kRowThreads) combine_kernel(const __grid_const
               if (c + e >= 0 && c + e < p.cols) sum[u][e] += r[e];
           }
         } else {
-          Piece<T, VEC> r;
-          load_piece<T, WIDE>(r, reinterpret_cast<const T*>(p.residual) + t * p.ldr, c, p.cols);
+          const Row<T, WIDE> residual(reinterpret_cast<const T*>(p.residual) + t * p.ldr, first, p.cols);
+          typename Row<T, WIDE>::Raw raw;
+          residual.load(raw, i);
+          const Piece<T, VEC> r = residual.get(raw);
 #pragma unroll
           for (int e = 0; e < VEC; ++e) sum[u][e] += r.get(e);
         }
@@ -626,8 +653,8 @@ __global__ void __launch_bounds__(kRowThreads) combine_kernel(const __grid_const
 // A block per token: dy is read once (and again from the first cache for more than four choices), the rows of its choices meet it.  Rows that lie
 // anyhow (not WIDE) are taken one by one, each with its own pieces.
 template <typename T, bool WIDE>
-__global__ void __launch_bounds__(kRowThreads) combine_grad_kernel(const __grid_constant__ RowParams p) {
-  constexpr int VEC = 16 / (int)sizeof(T), TOGETHER = WIDE ? kTogether : 1;
+__global__ void __launch_bounds__(kRowThreads, WIDE ? 4 : 5) combine_grad_kernel(const __grid_constant__ RowParams p) {
+  constexpr int VEC = 16 / (int)sizeof(T), TOGETHER = kTogether;
   __shared__ float part[TOGETHER][kRowThreads / 32];
   grid_dependency_wait();
   grid_launch_dependents();
@@ -646,31 +673,61 @@ __global__ void __launch_bounds__(kRowThreads) combine_grad_kernel(const __grid_
         w[k] = in && p.weights != nullptr ? element(p.weights, p.weight_elem, t * p.top + j0 + k) : 1.0f;
         dot[k] = 0.0f;
       }
-      const T* lies = WIDE || row[0] < 0 ? g : (out != nullptr ? out + (long long)row[0] * p.ldo : ys + (long long)row[0] * p.ldx);
-      const int first = WIDE ? 0 : first_piece<T, WIDE>(lies), end = !WIDE && row[0] < 0 ? first : p.cols;
-#pragma unroll 2
-      for (int c = first + (int)threadIdx.x * VEC; c < end; c += kRowThreads * VEC) {
-        Piece<T, VEC> d, y[TOGETHER];
-        load_piece<T, WIDE>(d, g + t * p.ldg, c, p.cols);
-        if (p.dw != nullptr) {
+      auto store_grad = [&](const Piece<T, VEC>& d, int k, int c) {
+        Piece<T, VEC> q;
 #pragma unroll
-          for (int k = 0; k < TOGETHER; ++k)
-            if (row[k] >= 0) load_piece<T, WIDE>(y[k], ys + (long long)row[k] * p.ldx, c, p.cols);
+        for (int e = 0; e < VEC; ++e) q.set(e, w[k] * d.get(e));
+        store_piece<T, WIDE>(q, out + (long long)row[k] * p.ldo, c, p.cols);
+      };
+      if constexpr (WIDE) {
+#pragma unroll 2
+        for (int c = (int)threadIdx.x * VEC; c < p.cols; c += kRowThreads * VEC) {
+          Piece<T, VEC> d, y[TOGETHER];
+          d.load(g + t * p.ldg + c);
+          if (p.dw != nullptr) {
+#pragma unroll
+            for (int k = 0; k < TOGETHER; ++k)
+              if (row[k] >= 0) y[k].load(ys + (long long)row[k] * p.ldx + c);
+          }
+#pragma unroll
+          for (int k = 0; k < TOGETHER; ++k) {
+            if (row[k] < 0) continue;
+            if (p.dw != nullptr) {
+#pragma unroll
+              for (int e = 0; e < VEC; ++e) dot[k] = fmaf(d.get(e), y[k].get(e), dot[k]);
+            }
+            if (out != nullptr) store_grad(d, k, c);
+          }
         }
+      } else {
 #pragma unroll
         for (int k = 0; k < TOGETHER; ++k) {
           if (row[k] < 0) continue;
-          if (p.dw != nullptr) {
+          const T* from = ys + (long long)row[k] * p.ldx;
+          const int first = first_piece<T, WIDE>(out != nullptr ? out + (long long)row[k] * p.ldo : from);
+          float sum = 0.0f;
+          const Row<T, WIDE> dy(g + t * p.ldg, first, p.cols), y_row(from, first, p.cols);
+#pragma unroll 1
+          for (int i = threadIdx.x; first + i * VEC < p.cols; i += kRowThreads) {
+            typename Row<T, WIDE>::Raw raw_d, raw_y;
+            dy.load(raw_d, i);
+            if (p.dw != nullptr) y_row.load(raw_y, i);
+            const Piece<T, VEC> d = dy.get(raw_d);
+            const int c = first + i * VEC;
+            if (out != nullptr) store_grad(d, k, c);
+            if (p.dw != nullptr) {
+              const Piece<T, VEC> y = y_row.get(raw_y);
+              if (c >= 0 && c + VEC <= p.cols) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e)
-              if (WIDE || (c + e >= 0 && c + e < p.cols)) dot[k] = fmaf(d.get(e), y[k].get(e), dot[k]);
-          }
-          if (out != nullptr) {
-            Piece<T, VEC> q;
+                for (int e = 0; e < VEC; ++e) sum = fmaf(d.get(e), y.get(e), sum);
+              } else {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) q.set(e, w[k] * d.get(e));
-            store_piece<T, WIDE>(q, out + (long long)row[k] * p.ldo, c, p.cols);
+                for (int e = 0; e < VEC; ++e)
+                  if (c + e >= 0 && c + e < p.cols) sum = fmaf(d.get(e), y.get(e), sum);
+              }
+            }
           }
+          dot[k] = sum;
         }
       }
       if (p.dw != nullptr) {
@@ -701,7 +758,7 @@ enum class RowOp { Dispatch, DispatchSort32, DispatchSort64, Combine, CombineGra
 template <typename T, bool WIDE>
 cudaError_t launch_rows(RowOp op, const RowParams& p, int sms, cudaStream_t st) {
   constexpr int VEC = 16 / (int)sizeof(T);
-  const long long pieces = ((long long)p.cols + VEC - 1) / VEC + (WIDE ? 0 : 1), width = kRowThreads * kHeld;
+  const long long pieces = ((long long)p.cols + VEC - 1) / VEC + (WIDE ? 0 : 1), width = kRowThreads * kHeld<WIDE>;
   const unsigned parts = op == RowOp::CombineGrad ? 1u : (unsigned)((pieces + width - 1) / width);
   const long long most = 64ll * sms;
   const dim3 grid((unsigned)(p.tokens < most ? p.tokens : most), parts);
