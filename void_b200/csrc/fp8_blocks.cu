@@ -77,7 +77,8 @@ template <>
 __device__ __forceinline__ uint32_t bits_of_half<__half>(uint32_t h) { return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h))) & 0x7fffffffu; }
 
 // A scale per row and 128 columns.  Rows in 16-byte pieces: 128 columns lie in 16 lanes (fp32: 32), a warp has `HELD` groups of 512 bytes of a
-// row at a time on their way; others element by element.  blockIdx.y: part of the columns.
+// row at a time on their way; others element by element.  blockIdx.y: part of the columns.  8192 x 8192 bf16: 35 us, 5.7 TB/s (fp32 maxima and a division for
+// every piece's place: 57).
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kQuantThreads) quant_rows_kernel(const __grid_constant__ QuantParams p) {
   constexpr int VEC = WIDE ? 16 / (int)sizeof(T) : 4, HELD = WIDE ? 4 : 2;
@@ -334,6 +335,9 @@ __device__ __forceinline__ void zero_tokens_in_no_run(const Fp8Params& p, const 
   }
 }
 
+// Few tokens: the weights are read once and that is all.  8 tokens, 8192 x 8192: 16.5 us (4.1 TB/s): 0.8 until the first copies are asked for, 2 to the first
+// block, 12.5 of streaming, 2.5 for the sums of a cluster; 16384 x 16384: 48 (5.6 TB/s).  Weights asked for by prefetches ahead of the wait on the kernel
+// before: 18.2 to 20.8 with the quantiser in front, against 18.5 without.
 // NT: tokens of an item at most.
 template <int NT, int CTAS>
 __global__ void __launch_bounds__(kThreads, CTAS) fp8_block_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUtensorMap map_a,
@@ -628,6 +632,13 @@ __global__ void __launch_bounds__(kThreads, CTAS) fp8_block_kernel(const __grid_
 // Tokens are the lanes here, 256 features the columns: a thread that adds up has one token and one block of 128 features, so that both
 // scales are one number of its own, and its results are 128 neighbours in memory.  Eight warps read an accumulator back and add it while the
 // tensor cores fill the other one; they hold 128 sums a thread, which takes registers from the other warps (setmaxnreg).
+//
+// 8192 tokens, 8192 x 8192, bf16 with residual: 605 us at 1.97 GHz (1.82 PFLOP/s), 747 under the power cap (1.61 GHz, 989 W).  Its parts by themselves, in
+// copies of the kernel: products 319, copies 371 (48 KB for every 128 x 256 x 128), both 478 (they share the bandwidth of shared memory), adding 390 to
+// 490, all without the way out 561.  With features in the lanes and tokens in the columns, the scales read from shared memory: 1680.
+// Taken back: two SMs for one item (cta_group::2; 32 KB a block, but accumulators handed back across SMs, of which there are only two: 1088); sixteen
+// adding warps of 64 columns (641); two accumulators of 128 columns each for every block (695: products of 128 columns are bound by shared memory);
+// the next block's first columns asked for ahead of the last of this one (823: registers are moved); pairs of numbers in one instruction (635).
 constexpr int kWideTokens = 128, kWideFeatures = 256;
 constexpr int kWideAhead = 4;                 // scales that are on their way, blocks of k
 constexpr int kWidePitch = kWideFeatures + 4; // of partial sums in shared memory: 16-byte pieces of eight rows meet all banks
