@@ -43,7 +43,7 @@ def _linear(experts=None, **bad):
     (dict(a=None), BAD_ARG), (dict(x=None), BAD_ARG), (dict(a_scale=None), BAD_ARG), (dict(x_scale=None), BAD_ARG), (dict(out=None), BAD_ARG),
     (dict(M=-1), BAD_ARG), (dict(K=0), BAD_ARG), (dict(act=4), BAD_ARG), (dict(out_elem=3), BAD_ARG), (dict(bias_elem=-1), BAD_ARG),
     (dict(residual_elem=3), BAD_ARG), (dict(ldc=63), SHAPE), (dict(residual=4096, ldr=63), SHAPE), (dict(a=4104), ALIGN), (dict(x=4104), ALIGN),
-    (dict(lda=264), ALIGN), (dict(ldx=264), ALIGN), (dict(lda=240), ALIGN), (dict(ldx=240), ALIGN), (dict(N=0), 0), (dict(M=0), 0),
+    (dict(lda=264), ALIGN), (dict(ldx=264), ALIGN), (dict(lda=240), ALIGN), (dict(ldx=240), ALIGN), (dict(N=0), 0), (dict(M=0), 0), (dict(K=2 ** 28 + 1), TOO_LARGE),
     (dict(experts=dict(chunk=48)), BAD_ARG), (dict(experts=dict(chunk=256)), BAD_ARG), (dict(experts=dict(plan=None)), BAD_ARG), (dict(experts=dict(n_experts=0)), BAD_ARG),
     (dict(experts=dict(offset_bytes=3)), BAD_ARG), (dict(experts=dict(offset_bytes=4, n_experts=33)), BAD_ARG),
     (dict(experts=dict(offset_bytes=8, plan=4100)), ALIGN), (dict(experts=dict(plan=4104)), ALIGN), (dict(experts={}, expert_stride=264), ALIGN),

@@ -301,6 +301,53 @@ def test_combine_against_differences():
             assert abs(dw[t, j].item() - float(value(y64, w64 + step) - value(y64, w64 - step))) < 1e-6
 
 
+def test_single_columns_and_gradients_that_are_repeated():
+    ids = torch.tensor([[0, 2], [1, -1], [2, 2], [0, 1]], device="cuda")
+    for d in (1, 5):
+        x = torch.randn(4, d, generator=_gen(1), device="cuda").requires_grad_(True)
+        w = torch.rand(4, 2, generator=_gen(2), device="cuda").requires_grad_(True)
+        rows, routes = void.void_dispatch(x, ids, 3)
+        dx, = torch.autograd.grad(rows.sum(), x, retain_graph=True)           # (the gradient of a sum has no strides)
+        assert torch.equal(dx, (ids >= 0).sum(1, keepdim=True).float().expand(4, d))
+        ys = rows.detach().requires_grad_(True)
+        dys, dw = torch.autograd.grad(void.void_combine(ys, routes, w).sum(), (ys, w))
+        place = routes.position.long()
+        chosen = torch.where((place >= 0)[:, :, None], ys.detach()[place.clamp_min(0)].double(), 0.0)
+        _close(dw, chosen.sum(2), chosen.abs().sum(2) * U * d)               # (a sum of d numbers, in whatever order: at most d roundings)
+        assert torch.equal(dys[place[0, 1]], w.detach()[0, 1].expand(d))
+    column = torch.randn(1, 1, device="cuda").expand(4, 1)
+    assert torch.equal(void.void_dispatch(column, ids, 3)[0], void.void_dispatch(column.contiguous(), ids, 3)[0])
+    scores = torch.randn(4, 1, device="cuda").requires_grad_(True)
+    ds, = torch.autograd.grad(void.void_route(scores, 1)[1].sum(), scores)
+    assert (ds == 0).all()
+    assert torch.equal(void.void_combine(column[:1].expand(8, 1), void.sort_by_expert(ids, 3), residual=column), (1 + (ids >= 0).sum(1, keepdim=True)) * column)
+
+
+def test_no_tokens_and_no_features():
+    for n, d in ((0, 8), (3, 0), (0, 0)):
+        x = torch.randn(n, d, device="cuda", requires_grad=True)
+        w = torch.rand(n, 2, device="cuda", requires_grad=True)
+        rows, routes = void.void_dispatch(x, torch.zeros(n, 2, dtype=torch.int64, device="cuda"), 4)
+        assert rows.shape == (2 * n, d) and routes.offsets.tolist() == [0] + [2 * n] * 4
+        y = void.void_combine(rows, routes, w, x)
+        dx, dw = torch.autograd.grad(y.sum(), (x, w))
+        assert dx.shape == (n, d) and (dw == 0).all()
+    ids, w = void.void_route(torch.randn(0, 5, device="cuda", requires_grad=True), 2)
+    assert ids.shape == w.shape == (0, 2)
+
+
+def test_many_choices_of_few_tokens():
+    for n, top, experts in ((1, 1024, 1000), (1, 1500, 7), (3, 700, 64)):
+        ids = torch.randint(-1, experts, (n, top), generator=_gen(n), device="cuda")
+        x = torch.randn(n, 40, generator=_gen(2), device="cuda")
+        rows, routes = void.void_dispatch(x, ids, experts)
+        offsets, position = _sorted(torch.where(ids < 0, -1, ids), experts)
+        assert torch.equal(routes.offsets, offsets) and torch.equal(routes.position, position)
+        y = void.void_combine(rows, routes)
+        exact = x.double() * (ids >= 0).sum(1, keepdim=True)
+        _close(y, exact, exact.abs() * U * (top + 1))
+
+
 def test_given_results():
     ids = _ids(40, 3, 6, "dropped", 2)
     x = torch.randn(40, 48, generator=_gen(1), device="cuda")

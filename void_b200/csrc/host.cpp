@@ -1923,6 +1923,10 @@ PyObject* layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // ------------------------------------------------------------------------------------------ tokens to experts and back
+// A matrix whose rows lie one behind the other, for what reads rows by their pitch (a column that is repeated has none).
+at::Tensor matrix_rows(const at::Tensor& m) {
+  return (m.size(1) > 1 && m.stride(1) != 1) || (m.size(0) > 1 && m.stride(0) < m.size(1)) ? m.contiguous() : m;
+}
 bool floating(at::ScalarType t) { return t == at::kFloat || t == at::kHalf || t == at::kBFloat16; }
 void no_tangents(std::initializer_list<const at::Tensor*> operands, const char* what) {
   for (const at::Tensor* t : operands)
@@ -1956,7 +1960,7 @@ struct RouteBackward : torch::autograd::Node {
     c10::cuda::OptionalCUDAGuard guard(s.device());
     no_eager_leaf(*this);
     at::AutoDispatchBelowADInplaceOrView below;
-    const at::Tensor rows = token_rows(s), g = token_rows(as_type(grads[0], at::kFloat));
+    const at::Tensor rows = matrix_rows(s), g = matrix_rows(as_type(grads[0], at::kFloat));
     const at::Tensor ds = new_cuda(s.sizes(), s.scalar_type(), s.device());
     const int status = void_route_grad(rows.const_data_ptr(), out_code(s.scalar_type()), row_step(rows), rows.size(0), (int32_t)rows.size(1), top, normalize,
                                        g.const_data_ptr<float>(), row_step(g), ds.data_ptr(), s.size(1), stream_of(s.device().index()));
@@ -1985,7 +1989,7 @@ PyObject* route(PyObject*, PyObject* const* a, Py_ssize_t n) {
   at::Tensor chosen, weights;
   {
     at::AutoDispatchBelowADInplaceOrView below;
-    const at::Tensor rows = token_rows(scores);
+    const at::Tensor rows = matrix_rows(scores);
     chosen = new_cuda({N, top}, at::kInt, dev);
     weights = new_cuda({N, top}, at::kFloat, dev);
     check(void_route(rows.const_data_ptr(), out_code(rows.scalar_type()), row_step(rows), N, (int32_t)E, (int32_t)top, normalize, chosen.data_ptr<int32_t>(),
@@ -2064,7 +2068,7 @@ struct DispatchBackward : torch::autograd::Node {
     c10::cuda::OptionalCUDAGuard guard(at.device());
     no_eager_leaf(*this);
     at::AutoDispatchBelowADInplaceOrView below;
-    const at::Tensor g = token_rows(as_type(grads[0], type));
+    const at::Tensor g = matrix_rows(as_type(grads[0], type));
     const at::Tensor dx = new_cuda({at.size(0), cols}, type, at.device());
     const int status = void_combine(g.const_data_ptr(), out_code(type), row_step(g), at.size(0), (int32_t)cols, (int32_t)at.size(1),
                                     at.const_data_ptr<int32_t>(), nullptr, VOID_ELEM_F32, nullptr, 0, out_code(type), dx.data_ptr(), cols,
@@ -2094,7 +2098,7 @@ PyObject* dispatch(PyObject*, PyObject* const* a, Py_ssize_t n) {
   at::Tensor rows;
   {
     at::AutoDispatchBelowADInplaceOrView below;
-    at::Tensor tokens = token_rows(x);
+    at::Tensor tokens = matrix_rows(x);
     if (none(a[3])) {
       rows = new_cuda({count, cols}, x.scalar_type(), dev);
     } else {
@@ -2148,12 +2152,12 @@ struct CombineBackward : torch::autograd::Node {
     no_eager_leaf(*this);
     at::AutoDispatchBelowADInplaceOrView below;
     const int64_t tokens = at.size(0), top = at.size(1);
-    const at::Tensor g = token_rows(as_type(grads[0], type)), w = weighted ? given.contiguous() : given;
+    const at::Tensor g = matrix_rows(as_type(grads[0], type)), w = weighted ? given.contiguous() : given;
     at::Tensor y;
     if (task_should_compute_output(0)) out[0] = new_cuda({tokens * top, cols}, type, at.device());
     if (weighted && task_should_compute_output(1)) {
       out[1] = new_cuda({tokens, top}, w.scalar_type(), at.device());
-      y = token_rows(ys);
+      y = matrix_rows(ys);
     }
     if (task_should_compute_output(2)) out[2] = grads[0];
     const int status = void_combine_grad(
@@ -2204,8 +2208,8 @@ PyObject* combine(PyObject*, PyObject* const* a, Py_ssize_t n) {
   at::Tensor y;
   {
     at::AutoDispatchBelowADInplaceOrView below;
-    at::Tensor rows = token_rows(ys), w = weights.defined() ? weights.contiguous() : weights, r = residual, at = position;
-    if (r.defined()) r = token_rows(r.scalar_type() == type || r.scalar_type() == at::kFloat ? r : r.to(at::kFloat));
+    at::Tensor rows = matrix_rows(ys), w = weights.defined() ? weights.contiguous() : weights, r = residual, at = position;
+    if (r.defined()) r = matrix_rows(r.scalar_type() == type || r.scalar_type() == at::kFloat ? r : r.to(at::kFloat));
     if (none(a[5])) {
       y = new_cuda({tokens, cols}, type, dev);
     } else {
@@ -2251,7 +2255,7 @@ struct Quantised {
   at::Tensor values, scales;
 };
 Quantised quantised(const at::Tensor& x_in, int64_t block_rows) {
-  const at::Tensor x = token_rows(x_in);
+  const at::Tensor x = matrix_rows(x_in);
   const c10::Device dev = x.device();
   const int64_t rows = x.size(0), cols = x.size(1), across = (cols + 127) / 128, pitch = (cols + 15) / 16 * 16;
   Quantised q;
@@ -2418,7 +2422,7 @@ PyObject* fp8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     plan.x.zero_rest = none(a[7]) ? 1 : 0;
   }
   if (none(a[3])) {   // x is quantised first, values and scales in one workspace: the last launch before the product, which counts on that (x_in_flight)
-    const at::Tensor rows = token_rows(x_in);
+    const at::Tensor rows = matrix_rows(x_in);
     const int64_t padded = (N + 3) / 4 * 4;
     s.ldx = (K + 15) / 16 * 16;
     const int64_t values_bytes = (N * s.ldx + 255) / 256 * 256;
