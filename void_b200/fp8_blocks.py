@@ -30,7 +30,7 @@ class FP8BlockTensor:
     [..., ceil(rows / 128), ceil(cols / 128)] (weights) or [rows, ceil(cols / 128)] (tokens): the matrix stands for values * scale of their
     block.  ``values`` and ``scales`` are the tensors given (values with rows that do not start on 16-byte boundaries: a copy), and products
     read them as they are at the time of the call."""
-    __slots__ = ("values", "scales", "block_rows", "_status")
+    __slots__ = ("values", "scales", "block_rows", "shape", "n_experts", "_status")
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor):
         if values.dtype is not torch.float8_e4m3fn:
@@ -52,18 +52,12 @@ class FP8BlockTensor:
             raise ValueError("scales of a %s matrix must be %s (or, of tokens, %s), got %s" % (
                 tuple(values.shape), (*values.shape[:-2], down, across), (rows, across), tuple(scales.shape)))
         self.values, self.scales, self._status = _rows_on_16_bytes(values), scales, None
-
-    @property
-    def shape(self):
-        return tuple(self.values.shape)
+        self.shape = tuple(values.shape)                                       # (experts, rows, columns), or without the first
+        self.n_experts: Optional[int] = self.shape[0] if len(self.shape) == 3 else None
 
     @property
     def device(self) -> torch.device:
         return self.values.device
-
-    @property
-    def n_experts(self) -> Optional[int]:
-        return self.values.shape[0] if self.values.dim() == 3 else None
 
     @property
     def memory_bytes(self) -> int:

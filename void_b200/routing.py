@@ -19,14 +19,11 @@ class ExpertRoutes:
 
     def __init__(self, offsets: torch.Tensor, position: torch.Tensor, n_experts: int):
         self.offsets, self.position, self.n_experts = offsets, position, n_experts
-        self._versions = self._now()
-
-    def _now(self):
-        return None if self.position.is_inference() else (self.offsets._version, self.position._version)
+        self._versions = None if position.is_inference() else offsets._version + position._version
 
     def check(self):
         """Raises where the routes were written to since they were made: rows would be left that no choice has."""
-        if self._versions is not None and self._versions != self._now():
+        if self._versions is not None and self._versions != self.offsets._version + self.position._version:   # (they only grow)
             raise _lib.VoidB200Error("the routes have been written to since the tokens were sorted: drop choices (-1) before they are sorted")
 
     @property
@@ -41,9 +38,11 @@ class ExpertRoutes:
         return f"ExpertRoutes(n_tokens={self.n_tokens}, top_k={self.top_k}, n_experts={self.n_experts})"
 
 
+_transforms = torch._C._are_functorch_transforms_active
+
+
 def _no_transforms(what: str) -> None:
-    if torch._C._are_functorch_transforms_active():
-        raise RuntimeError("%s cannot be used inside torch.func transforms (vmap, grad, jvp, ...)" % what)
+    raise RuntimeError("%s cannot be used inside torch.func transforms (vmap, grad, jvp, ...)" % what)
 
 
 def void_route(scores: torch.Tensor, top_k: int, normalize: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -52,8 +51,10 @@ def void_route(scores: torch.Tensor, top_k: int, normalize: bool = True) -> Tupl
     scores over the chosen experts, or with ``normalize=False`` over all.  A score of -inf is never chosen: where fewer than ``top_k``
     others are left, the expert is -1 (which void_dispatch drops) and the weight 0.  NaN counts as the largest and makes a token's weights NaN.
     Differentiable once in the scores."""
-    _no_transforms("the router")
-    _lib.require_cuda(scores)
+    if _transforms():
+        _no_transforms("the router")
+    if not scores.is_cuda:
+        _lib.require_cuda(scores)
     return _lib.native().route(scores, top_k, normalize)
 
 
@@ -69,8 +70,10 @@ def void_dispatch(x: torch.Tensor, experts: torch.Tensor, n_experts: int, out: O
     """Tokens x [tokens, features] (float32, float16 or bfloat16) copied into the run of each of their experts: rows [tokens * top_k, features]
     sorted by expert, as void_expert_linear and SparseExperts take them, and the routes (sort_by_expert).  Rows behind the last run, one for
     every dropped choice, are zeros; with ``out`` (row-major) they are left as they are.  Differentiable once in x."""
-    _no_transforms("the dispatch of tokens")
-    _lib.require_cuda(x, experts, out)
+    if _transforms():
+        _no_transforms("the dispatch of tokens")
+    if not (x.is_cuda and experts.is_cuda):
+        _lib.require_cuda(x, experts)
     rows, offsets, position = _lib.native().dispatch(x, experts, n_experts, out)
     return rows, ExpertRoutes(offsets, position, n_experts)
 
@@ -81,10 +84,12 @@ def void_combine(rows: torch.Tensor, routes: ExpertRoutes, weights: Optional[tor
     in rows' type.  ``weights`` [tokens, top_k] and ``residual`` [tokens, features] are float32, float16 or bfloat16; without weights the rows
     are added.  A dropped choice adds nothing, whatever its weight.  Differentiable once in rows, weights and residual.  ``out`` (row-major;
     may be the residual, or share memory with an operand in another way) takes the result where nothing is differentiated."""
-    _no_transforms("the combination of experts' rows")
+    if _transforms():
+        _no_transforms("the combination of experts' rows")
     if not isinstance(routes, ExpertRoutes):
         raise TypeError("void_combine takes ExpertRoutes (sort_by_expert, void_dispatch), got %s" % type(routes).__name__)
-    _lib.require_cuda(rows, weights, residual, out)
+    if not rows.is_cuda:
+        _lib.require_cuda(rows)
     routes.check()
     return _lib.native().combine(rows, routes.position, routes.offsets, weights, residual, out)
 
