@@ -689,6 +689,56 @@ __device__ __forceinline__ void store16(const Fp8Params& p, long long token, int
   }
 }
 
+// 64 results of a row that lies on 32 bytes, and their residuals: four pieces of 32 bytes, or (fp32) twice four, fetched here.
+template <class FETCH>
+__device__ __forceinline__ void add_residuals(f32x2 (&y)[32], uint32_t (&u)[4][8], int elem, FETCH fetch) {
+  if (elem == VOID_ELEM_F32) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      fetch(32 * h);
+#pragma unroll
+      for (int k = 0; k < 16; ++k) y[16 * h + k] = add2(y[16 * h + k], pair(__uint_as_float(u[k / 4][2 * (k % 4)]), __uint_as_float(u[k / 4][2 * (k % 4) + 1])));
+    }
+  } else if (elem == VOID_ELEM_F16) {
+#pragma unroll
+    for (int k = 0; k < 32; ++k) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[k / 8][k % 8]));
+      y[k] = add2(y[k], pair(f.x, f.y));
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 32; ++k) y[k] = add2(y[k], pair(__uint_as_float(u[k / 8][k % 8] << 16), __uint_as_float(u[k / 8][k % 8] & 0xffff0000u)));
+  }
+}
+__device__ __forceinline__ void store64(const Fp8Params& p, long long token, int m, const f32x2 (&y)[32]) {
+  const long long at = token * p.ldc + m;
+  uint32_t u[8];
+  float a, b;
+  if (p.out_elem == VOID_ELEM_F32) {
+#pragma unroll
+    for (int k = 0; k < 32; ++k) {
+      unpair(y[k], a, b);
+      u[2 * (k % 4)] = __float_as_uint(a);
+      u[2 * (k % 4) + 1] = __float_as_uint(b);
+      if (k % 4 == 3) st_global_v8(reinterpret_cast<float*>(p.out) + at + 8 * (k / 4), u);
+    }
+  } else if (p.out_elem == VOID_ELEM_F16) {
+#pragma unroll
+    for (int k = 0; k < 32; ++k) {
+      unpair(y[k], a, b);
+      u[k % 8] = pack2(a, b, VOID_ELEM_F16);
+      if (k % 8 == 7) st_global_v8(reinterpret_cast<uint16_t*>(p.out) + at + 16 * (k / 8), u);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 32; ++k) {
+      unpair(y[k], a, b);
+      u[k % 8] = pack2(a, b, VOID_ELEM_BF16);
+      if (k % 8 == 7) st_global_v8(reinterpret_cast<uint16_t*>(p.out) + at + 16 * (k / 8), u);
+    }
+  }
+}
+
 // A cluster's sums meet: its tokens are dealt to the CTAs, halves of their rows to the adding warps, features to lanes.  The pieces of four halves, of one CTA
 // after the other, are on their way together.  Four features of a lane lie side by side, or (LOOSE) 32 apart, so that neighbours in memory are
 // neighbouring lanes' either way.
@@ -993,6 +1043,19 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_wide_kernel(const __grid_cons
 #pragma unroll
         for (int h = 0; h < COLS; h += 64) {
           if (!LOOSE && p.residual != nullptr && pieces == 1) fetch_residuals(h, 16);
+          if (!LOOSE && m0 + h + 64 <= p.M) {   // 64 results step by step: two warps of a scheduler wait for each other's instructions, and each for its own
+            f32x2 y[32];
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+              const float4 v = bias[h / 4 + c];
+              y[2 * c] = add2(pair(sum[h + 4 * c], sum[h + 4 * c + 1]), pair(v.x, v.y));
+              y[2 * c + 1] = add2(pair(sum[h + 4 * c + 2], sum[h + 4 * c + 3]), pair(v.z, v.w));
+            }
+            activate<32>(y, p.act);
+            if (p.residual != nullptr) add_residuals(y, res, p.residual_elem, [&](int c) { fetch_residuals(h + c, 8); });
+            if (mine) store64(p, row, m0 + h, y);
+            continue;
+          }
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             if (!LOOSE && p.residual != nullptr && pieces == 2 && q % 2 == 0) fetch_residuals(h + 16 * q, 8);
