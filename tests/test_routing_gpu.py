@@ -411,6 +411,20 @@ def test_refusals():
 
 
 # ------------------------------------------------------------------------------------------ as they are used
+def test_tokens_written_just_before():
+    """Tokens are asked for while their choices are still being sorted: what writes them must be through by then."""
+    given = [torch.randn(3000, 512, generator=_gen(s), device="cuda") for s in (1, 2)]
+    ids = torch.randint(0, 32, (3000, 2), generator=_gen(3), device="cuda")
+    want = [void.void_dispatch(x, ids, 32)[0] for x in given]
+    x = given[0].clone()
+    got = []
+    for i in range(60):
+        x.copy_(given[i % 2])
+        got.append(void.void_dispatch(x, ids, 32)[0] if i % 3 else void.void_dispatch(x.mul_(1), ids.add_(0), 32)[0])
+    for i, rows in enumerate(got):
+        assert torch.equal(rows, want[i % 2]), i
+
+
 def test_captured_and_replayed_with_other_tokens():
     x, scores = torch.randn(24, 64, generator=_gen(1), device="cuda"), torch.randn(24, 8, generator=_gen(2), device="cuda")
 
