@@ -68,6 +68,7 @@ DISPATCH_BASE = dict(x=AT, elem=0, ldx=16, tokens=4, cols=16, experts=AT, index_
 @pytest.mark.parametrize("bad, status", [
     (dict(x=None), BAD_ARG), (dict(out=None), BAD_ARG), (dict(experts=None), BAD_ARG), (dict(elem=3), BAD_ARG), (dict(tokens=-1), BAD_ARG), (dict(top=0), BAD_ARG),
     (dict(cols=-1), BAD_ARG), (dict(ldx=15), SHAPE), (dict(ldo=15), SHAPE), (dict(tokens=2 ** 30, top=2), TOO_LARGE), (dict(n_experts=1025), TOO_LARGE),
+    (dict(cols=68000000, ldx=68000000, ldo=68000000), TOO_LARGE),
 ])
 def test_dispatch_refuses(bad, status):
     assert _call("void_dispatch", DISPATCH, DISPATCH_BASE, **bad) == status
@@ -82,6 +83,7 @@ COMBINE_BASE = dict(rows=AT, elem=1, ldx=16, tokens=4, cols=16, top=2, position=
     (dict(rows=None), BAD_ARG), (dict(out=None), BAD_ARG), (dict(position=None), BAD_ARG), (dict(elem=3), BAD_ARG), (dict(weight_elem=3), BAD_ARG),
     (dict(residual_elem=2), BAD_ARG), (dict(ldx=15), SHAPE), (dict(ldo=15), SHAPE), (dict(ldr=15), SHAPE), (dict(top=0), BAD_ARG),
     (dict(tokens=2 ** 30), TOO_LARGE), (dict(tokens=0), 0), (dict(cols=0), 0),
+    (dict(cols=68000000, ldx=68000000, ldr=68000000, ldo=68000000), TOO_LARGE),
 ])
 def test_combine_refuses(bad, status):
     assert _call("void_combine", COMBINE, COMBINE_BASE, **bad) == status

@@ -793,7 +793,7 @@ int rows_of_type(RowOp op, const RowParams& p, bool wide, int sms, cudaStream_t 
 }
 int rows_launch(RowOp op, RowParams& p, int elem, cudaStream_t st) {
   if (elem < VOID_ELEM_F32 || elem > VOID_ELEM_BF16 || p.tokens < 0 || p.top < 1 || p.cols < 0) return VOID_ERR_BAD_ARG;
-  if (p.tokens > 0x7fffffffll / p.top || p.cols > 100000000) return VOID_ERR_TOO_LARGE;   // (blocks along a row)
+  if (p.tokens > 0x7fffffffll / p.top || p.cols > 65535 * kRowThreads * 4 - 8) return VOID_ERR_TOO_LARGE;   // (blocks along a row of fp32 that lies anyhow)
   p.rows = p.tokens * p.top;
   const bool combine = op == RowOp::Combine, grad = op == RowOp::CombineGrad;
   if (p.tokens > 1 && ((p.ldx < p.cols && (combine || p.x != nullptr)) || (p.out != nullptr && p.ldo < p.cols) || (grad && p.ldg < p.cols) || (p.residual != nullptr && p.ldr < p.cols)))
