@@ -1,0 +1,33 @@
+"""Tokens to experts and back on a B200: operands that change from call to call, and calls that are refused."""
+import pytest
+import torch
+
+import void_b200 as void
+from void_b200 import _lib
+from test_routing_gpu import _gen, _sorted
+
+pytestmark = pytest.mark.gpu
+
+
+def test_tokens_and_choices_written_just_before_by_a_few_blocks():
+    """Every call has other tokens and other choices, written by kernels of a few blocks right before it: nothing that a multiprocessor read in the call
+    before may be used again."""
+    n, top, d, experts = 700, 2, 8, 24
+    for dtype, index in ((torch.float32, torch.int64), (torch.bfloat16, torch.int32)):
+        x, ids = torch.empty(n, d, dtype=dtype, device="cuda"), torch.empty(n, top, dtype=index, device="cuda")
+        given = [(torch.randn(n, d, generator=_gen(s), device="cuda").to(dtype), torch.randint(-1, experts, (n, top), generator=_gen(10 + s), device="cuda").to(index))
+                 for s in range(5)]
+        sorted_ids = [_sorted(ids_, experts) for _, ids_ in given]
+        got = []
+        for i in range(60):
+            x.copy_(given[i % 5][0])
+            ids.copy_(given[i % 5][1])
+            got.append(void.void_dispatch(x, ids, experts))
+        for i, (rows, routes) in enumerate(got):
+            tokens = given[i % 5][0]
+            offsets, position = sorted_ids[i % 5]
+            assert torch.equal(routes.offsets, offsets) and torch.equal(routes.position, position), i
+            at = position.flatten()
+            want = torch.zeros(n * top, d, dtype=dtype, device="cuda")
+            want[at[at >= 0].long()] = tokens.repeat_interleave(top, 0)[at >= 0]
+            assert torch.equal(rows, want), i

@@ -394,7 +394,6 @@ struct RowParams {
   long long ldo;
   void* dw;                 // gradient of the weights, of their type, or null
   int zero_rest;
-  int early;                // dispatch behind its own sort: x was complete before that started, and is asked for ahead of its end
   // dispatch that sorts by itself
   const void* experts;
   int32_t *offsets, *positions;
@@ -493,18 +492,14 @@ __device__ __forceinline__ void zero_rest(const RowParams& p, long long used, in
 // Memory bounds it: 8192 x 4096 bf16 to four experts each 54 us behind the sort, 336 MB at 6.2 TB/s; rows that lie anyhow (4095) 78.
 // Token by token, so that x is read once; a token's copies go where its choices were sorted to.  blockIdx.y: part of the columns.
 // SORT (few choices): the rows are not known yet, each is the number of choices that come before it.
-// Behind its own sort a block asks for its first token ahead of the sort's end: 59 us in all, 61 without.
 template <typename T, bool WIDE, typename I, bool SORT>
 __global__ void __launch_bounds__(kRowThreads) dispatch_kernel(const __grid_constant__ RowParams p) {
   constexpr int VEC = 16 / (int)sizeof(T), U = kHeld<WIDE>;
   __shared__ int32_t ids[SORT ? kFewChoices : 1];
   __shared__ int32_t place[SORT ? kFewChoices : 1];   // of this token's choices
   __shared__ int32_t rows_used;
-  bool waited = SORT || !WIDE || !p.early;
-  if (waited) {
-    grid_dependency_wait();
-    grid_launch_dependents();
-  }
+  grid_dependency_wait();
+  grid_launch_dependents();
   const int i0 = blockIdx.y * (kRowThreads * U);   // the block's pieces
   const T* x = reinterpret_cast<const T*>(p.x);
   T* out = reinterpret_cast<T*>(p.out);
@@ -537,11 +532,6 @@ __global__ void __launch_bounds__(kRowThreads) dispatch_kernel(const __grid_cons
         const int i = i0 + u * kRowThreads + threadIdx.x;
         if (i * VEC < p.cols) token.load(raw[u], i);
       }
-    }
-    if (!waited) {
-      grid_dependency_wait();
-      grid_launch_dependents();
-      waited = true;
     }
     if constexpr (SORT) {
       __syncthreads();
@@ -912,7 +902,6 @@ int void_dispatch(const void* x, int32_t elem, int64_t ldx, int64_t tokens, int3
     return vb::rows_launch(index_bytes == 4 ? vb::RowOp::DispatchSort32 : vb::RowOp::DispatchSort64, p, elem, st);
   }
   const int sorted = void_sort_by_expert(experts, index_bytes, count, n_experts, offsets, position, ws, ws_bytes, stream);
-  p.early = 1;
   return sorted != VOID_OK ? sorted : vb::rows_launch(vb::RowOp::Dispatch, p, elem, st);
 }
 
