@@ -686,9 +686,7 @@ typedef struct void_fp8_args {
   int32_t act;
   int32_t test_hooks;                               /* 0 outside tests */
   int32_t* status;                                  /* as in void_spmm_args, or NULL */
-  int32_t x_in_flight;                              /* 1: the launch before this one on the stream is the void_quant_fp8_blocks that writes x and
-                                                       x_scale, so that all else was complete when it started and is read ahead of its end */
-  int32_t reserved;
+  int32_t reserved[2];                              /* 0 */
 } void_fp8_args;
 VOID_API int void_quant_fp8_blocks(const void* x, int32_t elem, int64_t ldx, int64_t rows, int32_t cols, int32_t block_rows, void* q, int64_t ldq,
                                    float* scales, int64_t scale_row, int64_t scale_col, void_stream_t stream);

@@ -1,4 +1,4 @@
-"""Routing: a kernel that starts beside the end of the kernel before it waits for that one as a whole, every thread
+"""Routing and 8-bit layers: a kernel that starts beside the end of the kernel before it waits for that one as a whole, every thread
 of it and before anything else, and reads nothing of an operand ahead of the wait."""
 import re
 
@@ -6,7 +6,7 @@ import pytest
 
 from test_kernel_rules_cpu import KERNELS, WAIT
 
-FILES = ("route.cu",)
+FILES = ("route.cu", "fp8_blocks.cu")
 # members of the parameters that are sizes and rules of the launch, not addresses
 SIZES = {"pitch", "stages", "wait_limit_ms", "splits", "k_blocks"}
 MINE = [k for k in KERNELS if k[0] in FILES]
@@ -17,7 +17,8 @@ def _depth(text):
 
 
 def test_the_kernels_are_found():
-    assert {"route_kernel", "sort_cluster_kernel", "sort_count_kernel", "sort_place_kernel", "dispatch_kernel", "combine_kernel", "combine_grad_kernel"} <= {k[1] for k in MINE}
+    assert {"route_kernel", "sort_cluster_kernel", "sort_count_kernel", "sort_place_kernel", "dispatch_kernel", "combine_kernel", "combine_grad_kernel",
+            "quant_rows_kernel", "quant_blocks_kernel", "fp8_block_kernel", "fp8_wide_kernel"} <= {k[1] for k in MINE}
 
 
 @pytest.mark.parametrize("kernel", MINE, ids=lambda k: k[1])

@@ -70,7 +70,7 @@ class Fp8Args(ctypes.Structure):
     _fields_ = [("a", c_vp), ("lda", c_i64), ("expert_stride", c_i64), ("a_scale", c_vp), ("a_scale_row", c_i64), ("a_scale_col", c_i64),
                 ("a_scale_expert", c_i64), ("x", c_vp), ("ldx", c_i64), ("x_scale", c_vp), ("x_scale_row", c_i64), ("x_scale_col", c_i64),
                 ("bias", c_vp), ("residual", c_vp), ("ldr", c_i64), ("out", c_vp), ("ldc", c_i64), ("M", c_i32), ("K", c_i32), ("N", c_i32),
-                ("bias_elem", c_i32), ("residual_elem", c_i32), ("out_elem", c_i32), ("act", c_i32), ("test_hooks", c_i32), ("status", c_vp), ("x_in_flight", c_i32), ("reserved", c_i32)]
+                ("bias_elem", c_i32), ("residual_elem", c_i32), ("out_elem", c_i32), ("act", c_i32), ("test_hooks", c_i32), ("status", c_vp), ("reserved", c_i32 * 2)]
 
 
 _PROTOTYPES = {

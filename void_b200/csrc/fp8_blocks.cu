@@ -221,7 +221,6 @@ struct Fp8Params {
   int out_elem, act;
   int splits;                     // CTAs of a cluster, which share an item's blocks of k
   int stages;
-  int early;                      // what is read but the tokens and their scales was complete before the kernel in flight started
   int32_t* status;
   int wait_limit_ms, drop_first;  // drop_first: test hook, the first stage is never filled
 };
@@ -384,29 +383,14 @@ __global__ void __launch_bounds__(kThreads, CTAS) fp8_block_kernel(const __grid_
   const uint32_t tmem = tmem_s;
   const int rank = p.splits > 1 ? (int)cluster_rank() : 0;
   const int b0 = (int)((long long)p.k_blocks * rank / p.splits), b1 = (int)((long long)p.k_blocks * (rank + 1) / p.splits);
-  if (!p.early) grid_dependency_wait();
+  grid_dependency_wait();
   find_runs(p, runs);
   const int step = (int)gridDim.x / p.splits, begin = (int)blockIdx.x / p.splits, end = items_of(p, runs);
   // With several CTAs per item a launch has a cluster for every item, so that the ring is free when the sums meet in its place.
   if (warp == 0) {
-    int stage = 0, ahead = 0;   // ahead: stages whose weights have been asked for already
+    int stage = 0;
     uint32_t phase = 0;
     bool first = true;
-    auto weights = [&](const Item& t, int b, int s, int boxes) {
-      const uint32_t full = smem_u32(&bars.full[s]);
-      mbar_expect_tx(full, kStageA + (uint32_t)boxes * (kTokenBox * kBlock));
-      tma_load_3d(ring + (uint32_t)s * kStage, &map_a, b * kBlock, t.m * kBlock, t.expert, full);
-    };
-    if (p.early) {   // the ring's first weights, while the tokens are still being quantised
-      if (begin < end && !p.drop_first) {
-        const Item t = item_at(p, runs, begin);
-        ahead = min(p.stages, b1 - b0);
-        if (lane == 0)
-          for (int s = 0; s < ahead; ++s) weights(t, b0 + s, s, (t.n1 - t.n0 + kTokenBox - 1) / kTokenBox);
-        __syncwarp();
-      }
-      grid_dependency_wait();
-    }
     for (int i = begin; i < end && !ctl[0]; i += step) {
       const Item t = item_at(p, runs, i);
       const int boxes = (t.n1 - t.n0 + kTokenBox - 1) / kTokenBox;
@@ -414,8 +398,11 @@ __global__ void __launch_bounds__(kThreads, CTAS) fp8_block_kernel(const __grid_
         if (!mbar_wait_warp(smem_u32(&bars.empty[stage]), phase ^ 1u, ctl)) break;
         const bool drop = first && p.drop_first != 0;
         first = false;
-        if (ahead > 0) --ahead;
-        else if (lane == 0 && !drop) weights(t, b, stage, boxes);
+        if (lane == 0 && !drop) {
+          const uint32_t full = smem_u32(&bars.full[stage]);
+          mbar_expect_tx(full, kStageA + (uint32_t)boxes * (kTokenBox * kBlock));
+          tma_load_3d(ring + (uint32_t)stage * kStage, &map_a, b * kBlock, t.m * kBlock, t.expert, full);
+        }
         __syncwarp();
         if (lane >= 1 && lane <= boxes && !drop)
           tma_load_2d(ring + (uint32_t)stage * kStage + kStageA + (uint32_t)(lane - 1) * (kTokenBox * kBlock), &map_x, b * kBlock, t.n0 + (lane - 1) * kTokenBox,
@@ -450,7 +437,6 @@ __global__ void __launch_bounds__(kThreads, CTAS) fp8_block_kernel(const __grid_
   } else if (warp < kFirstAdder) {
     // The products of both scales, every other block of k for either warp; those of the next block are on their way meanwhile.
     constexpr int PER = (NT + 31) / 32;
-    if (p.early) grid_dependency_wait();
     uint32_t it0 = 0;
     bool ok = true;
     for (int i = begin; i < end && ok; i += step) {
@@ -612,7 +598,6 @@ __global__ void __launch_bounds__(kThreads, CTAS) fp8_block_kernel(const __grid_
     __syncwarp();
     cluster_meet();   // (nobody leaves while others read its sums)
   }
-  if (p.early) grid_dependency_wait();
   zero_tokens_in_no_run(p, runs);
   grid_launch_dependents();
   tc_fence_before();
@@ -869,7 +854,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_wide_kernel(const __grid_cons
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_s;
-  if (!p.early) grid_dependency_wait();
+  grid_dependency_wait();
   find_runs(p, runs);
 
   const int rank = p.splits > 1 ? (int)cluster_rank() : 0;
@@ -878,34 +863,21 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_wide_kernel(const __grid_cons
   // (4 * 56 + 8 * 224 = 12 * 168, what the block was launched with)
   if (warp >= kAdders) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
   if (warp == kCopier) {
-    int stage = 0, ahead = 0;   // ahead: stages whose weights have been asked for already
+    int stage = 0;
     uint32_t phase = 0;
     bool first = true;
-    auto weights = [&](const Item& t, int b, int s) {
-      const int m0 = t.m * kWideFeatures, halves = p.M - m0 > kBlock ? 2 : 1, boxes = (t.n1 - t.n0 + kTokenBox - 1) / kTokenBox;
-      const uint32_t full = smem_u32(&bars.full[s]), at = ring + (uint32_t)s * kWideStage + kWideTokens * kBlock;
-      mbar_expect_tx(full, (uint32_t)(halves * kBlock + boxes * kTokenBox) * kBlock);
-      for (int h = 0; h < halves; ++h) tma_load_3d(at + (uint32_t)h * (kBlock * kBlock), &map_a, b * kBlock, m0 + h * kBlock, t.expert, full);
-    };
-    if (p.early) {   // the ring's first weights, while the tokens are still being quantised
-      if (begin < end && !p.drop_first) {
-        const Item t = item_at(p, runs, begin);
-        ahead = min(p.stages, b1 - b0);
-        if (lane == 0)
-          for (int s = 0; s < ahead; ++s) weights(t, b0 + s, s);
-        __syncwarp();
-      }
-      grid_dependency_wait();
-    }
     for (int i = begin; i < end && !ctl[0]; i += step) {
       const Item t = item_at(p, runs, i);
-      const int boxes = (t.n1 - t.n0 + kTokenBox - 1) / kTokenBox;
+      const int m0 = t.m * kWideFeatures, halves = p.M - m0 > kBlock ? 2 : 1, boxes = (t.n1 - t.n0 + kTokenBox - 1) / kTokenBox;
       for (int b = b0; b < b1; ++b) {
         if (!mbar_wait_warp(smem_u32(&bars.empty[stage]), phase ^ 1u, ctl)) break;
         const bool drop = first && p.drop_first != 0;
         first = false;
-        if (ahead > 0) --ahead;
-        else if (lane == 0 && !drop) weights(t, b, stage);
+        if (lane == 0 && !drop) {
+          const uint32_t full = smem_u32(&bars.full[stage]), at = ring + (uint32_t)stage * kWideStage + kWideTokens * kBlock;
+          mbar_expect_tx(full, (uint32_t)(halves * kBlock + boxes * kTokenBox) * kBlock);
+          for (int h = 0; h < halves; ++h) tma_load_3d(at + (uint32_t)h * (kBlock * kBlock), &map_a, b * kBlock, m0 + h * kBlock, t.expert, full);
+        }
         __syncwarp();
         if (lane >= 1 && lane <= boxes && !drop)
           tma_load_2d(ring + (uint32_t)stage * kWideStage + (uint32_t)(lane - 1) * (kTokenBox * kBlock), &map_x, b * kBlock, t.n0 + (lane - 1) * kTokenBox,
@@ -955,7 +927,6 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_wide_kernel(const __grid_cons
     }
   } else if (warp < kAdders) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-    if (p.early) grid_dependency_wait();
     const int quad = warp & 3, side = warp >> 2;
     uint32_t it = 0, item = 0;
     bool ok = true;
@@ -1115,7 +1086,6 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_wide_kernel(const __grid_cons
     if (warp >= kAdders) cluster_meet();
     cluster_meet();   // (nobody leaves while others read its sums)
   }
-  if (p.early) grid_dependency_wait();
   zero_tokens_in_no_run(p, runs);
   grid_launch_dependents();
   tc_fence_before();
@@ -1255,7 +1225,6 @@ int fp8_linear(const void_fp8_args* a, const void_experts* x, cudaStream_t st) {
   p.residual = a->residual; p.ldr = a->ldr; p.residual_elem = a->residual_elem;
   p.out = a->out; p.ldc = a->ldc; p.out_elem = a->out_elem; p.act = a->act;
   p.status = a->status;
-  p.early = a->x_in_flight;
   p.wait_limit_ms = (a->test_hooks & 0xffff) ? (a->test_hooks & 0xffff) : kDefaultWaitLimitMs;
   p.drop_first = (a->test_hooks >> 16) & 1;
   // Up to 64 tokens lie in the columns of the tensor memory, more of them in its lanes.

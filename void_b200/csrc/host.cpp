@@ -2421,7 +2421,7 @@ PyObject* fp8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     plan = expert_plan(cuda_tensor(a[4], "offsets"), N, E, dev, s.status, true, fp8_chunk(N, E));
     plan.x.zero_rest = none(a[7]) ? 1 : 0;
   }
-  if (none(a[3])) {   // x is quantised first, values and scales in one workspace: the last launch before the product, which counts on that (x_in_flight)
+  if (none(a[3])) {   // x is quantised first, values and scales in one workspace
     const at::Tensor rows = matrix_rows(x_in);
     const int64_t padded = (N + 3) / 4 * 4;
     s.ldx = (K + 15) / 16 * 16;
@@ -2432,7 +2432,6 @@ PyObject* fp8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     check(void_quant_fp8_blocks(rows.const_data_ptr(), out_code(rows.scalar_type()), row_step(rows), N, (int32_t)K, 1, at, s.ldx, sx, 1, padded, stream_of(dev.index())),
           "void_quant_fp8_blocks");
     s.x = at;
-    s.x_in_flight = N > 0 ? 1 : 0;
     s.x_scale = sx;
     s.x_scale_row = 1;
     s.x_scale_col = padded;
