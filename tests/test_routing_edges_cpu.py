@@ -1,0 +1,29 @@
+"""Routing, what needs no GPU: refusals of the entry points and operators at their smallest and largest sizes."""
+import pytest
+import torch
+
+from test_routing_cpu import CGRAD, CGRAD_BASE, COMBINE, COMBINE_BASE, DISPATCH, DISPATCH_BASE, SHAPE, _call
+
+
+def test_dispatch_of_one_token_refuses_rows_that_overlap():
+    for bad in (dict(ldo=15), dict(ldo=0), dict(ldo=-16), dict(ldo=15, top=3, index_bytes=8)):
+        assert _call("void_dispatch", DISPATCH, DISPATCH_BASE, **dict(bad, tokens=1)) == SHAPE
+
+
+def test_combine_of_one_token_refuses_rows_that_overlap():
+    for bad in (dict(ldx=15), dict(ldx=0), dict(ldx=15, residual=None, top=4)):
+        assert _call("void_combine", COMBINE, COMBINE_BASE, **dict(bad, tokens=1)) == SHAPE
+
+
+def test_gradient_of_one_token_refuses_rows_that_overlap():
+    for bad in (dict(ldd=15), dict(ldx=15), dict(ldd=0, dweights=None), dict(ldx=0, drows=None)):
+        assert _call("void_combine_grad", CGRAD, CGRAD_BASE, **dict(bad, tokens=1)) == SHAPE
+
+
+def test_one_row_has_no_pitch():
+    """A single token with a single choice: no pitch is ever used, and none refused (without a GPU the calls end later, for that)."""
+    for name, order, base, pitches in (("void_dispatch", DISPATCH, DISPATCH_BASE, dict(ldx=0, ldo=0)), ("void_combine", COMBINE, COMBINE_BASE, dict(ldx=0, ldr=0, ldo=0)),
+                                       ("void_combine_grad", CGRAD, CGRAD_BASE, dict(ldg=0, ldx=0, ldd=0))):
+        if torch.cuda.is_available():
+            pytest.skip("the call would read addresses that are none")
+        assert _call(name, order, base, **dict(pitches, tokens=1, top=1)) != SHAPE

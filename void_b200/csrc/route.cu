@@ -786,7 +786,10 @@ int rows_launch(RowOp op, RowParams& p, int elem, cudaStream_t st) {
   if (p.tokens > 0x7fffffffll / p.top || p.cols > 65535 * kRowThreads * 4 - 8) return VOID_ERR_TOO_LARGE;   // (blocks along a row of fp32 that lies anyhow)
   p.rows = p.tokens * p.top;
   const bool combine = op == RowOp::Combine, grad = op == RowOp::CombineGrad;
-  if (p.tokens > 1 && ((p.ldx < p.cols && (combine || p.x != nullptr)) || (p.out != nullptr && p.ldo < p.cols) || (grad && p.ldg < p.cols) || (p.residual != nullptr && p.ldr < p.cols)))
+  // A matrix has a row per token, or (what lies in runs) one per choice.
+  const long long rows_x = combine || grad ? p.rows : p.tokens, rows_out = combine ? p.tokens : p.rows;
+  if ((rows_x > 1 && p.x != nullptr && p.ldx < p.cols) || (rows_out > 1 && p.out != nullptr && p.ldo < p.cols) ||
+      (p.tokens > 1 && ((grad && p.ldg < p.cols) || (p.residual != nullptr && p.ldr < p.cols))))
     return VOID_ERR_SHAPE;
   if (p.tokens == 0 || (p.cols == 0 && p.dw == nullptr)) return VOID_OK;
   const DeviceInfo dev = device_info();
