@@ -49,3 +49,21 @@ def test_residuals_and_biases_written_just_before_by_a_few_blocks(n):
         got.append(void.void_linear(w, x, bias, residual=residual))
     for i, y in enumerate(got):
         assert torch.equal(y, want[i % 5]), i
+
+
+def test_tangents_are_refused():
+    import torch.autograd.forward_ad as fwd
+    w, experts = _weights(256, 256, 1), void.quantize_fp8_blocks(torch.randn(2, 256, 256, generator=_gen(1), device="cuda"))
+    x, bias, offsets = torch.randn(4, 256, device="cuda"), torch.randn(256, device="cuda"), torch.tensor([0, 1, 4], device="cuda")
+    quantised = void.quantize_fp8_blocks(x, 1)
+    with fwd.dual_level():
+        x_dual, bias_dual, biases = fwd.make_dual(x, x), fwd.make_dual(bias, bias), fwd.make_dual(bias.expand(2, 256).contiguous(), bias.expand(2, 256).contiguous())
+        scales = [fwd.make_dual(t.scales, torch.ones_like(t.scales)) for t in (w, quantised)]
+        for call in (lambda: void.void_linear(w, x_dual), lambda: void.void_linear(w, x, bias_dual), lambda: void.void_linear(w, quantised, residual=x_dual),
+                     lambda: void.void_linear(void.FP8BlockTensor(w.values, scales[0]), x), lambda: void.void_linear(w, void.FP8BlockTensor(quantised.values, scales[1])),
+                     lambda: void.void_expert_linear(experts, x_dual, offsets), lambda: void.void_expert_linear(experts, x, offsets, biases),
+                     lambda: void.quantize_fp8_blocks(x_dual), lambda: void.quantize_fp8_blocks(x_dual, 1),
+                     lambda: void.quantize_fp8_blocks(x_dual.expand(2, 4, 256))):
+            with pytest.raises(NotImplementedError, match="tangent"):
+                call()
+    assert void.void_linear(w, x, bias).shape == (4, 256)

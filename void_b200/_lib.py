@@ -239,6 +239,14 @@ def require_cuda(*tensors):
 _STATUS = {}
 
 
+transforms_active = torch._C._are_functorch_transforms_active
+
+
+def no_transforms(what):
+    """What operators that torch.func does not know raise inside its transforms (transforms_active)."""
+    raise RuntimeError("%s cannot be used inside torch.func transforms (vmap, grad, jvp, ...)" % what)
+
+
 def status_word(device):
     """Per-device int32 status word the kernels write when a bounded wait gives up."""
     key = torch.device(device).index if torch.device(device).index is not None else torch.cuda.current_device()

@@ -2280,6 +2280,7 @@ PyObject* quant_fp8_blocks(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const at::Tensor& x = cuda_tensor(a[0], "x");
   if (x.dim() != 2) fail("a matrix is quantised in blocks, got " + std::to_string(x.dim()) + " dimensions");
   if (!floating(x.scalar_type())) fail(std::string("blocks are quantised from float32, float16 or bfloat16, got ") + c10::toString(x.scalar_type()));
+  no_tangents({&x}, "the quantiser of blocks");
   if (x.size(1) > 0x7ffffff0) fail("a matrix that is quantised has at most 2^31 - 16 columns");
   c10::cuda::OptionalCUDAGuard guard(x.device());
   at::AutoDispatchBelowADInplaceOrView below;
@@ -2312,6 +2313,10 @@ PyObject* fp8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (scales.size(dims - 2) != (M + 127) / 128 || scales.size(dims - 1) != (K + 127) / 128 || (runs && scales.size(0) != E))
     fail("weights carry a scale for each block of 128 x 128");
   if (M > 0x7fffff00 || K > 0x7fffff00 || N > 0x40000000) fail("the product is too large");
+  const at::Tensor absent;
+  no_tangents({&scales, &x_in, none(a[3]) ? &absent : &tensor(a[3], "x's scales"), none(a[5]) ? &absent : &tensor(a[5], "bias"),
+               none(a[9]) ? &absent : &tensor(a[9], "residual")},
+              "a layer with 8-bit weights");
   c10::cuda::OptionalCUDAGuard guard;
   if (c10::cuda::current_device() != dev.index()) guard.set_device(dev);
   at::AutoDispatchBelowADInplaceOrView below;

@@ -78,6 +78,8 @@ class FP8BlockTensor:
         return (self.values.float() * scales).to(dtype)
 
     def _product(self, x, offsets, bias, activation, out, out_dtype, residual) -> torch.Tensor:
+        if _lib.transforms_active():
+            _lib.no_transforms("a layer with 8-bit weights")
         values, x_scales = self.values, None
         if type(x) is FP8BlockTensor:
             x, x_scales = x.values, x.scales
@@ -97,6 +99,8 @@ def quantize_fp8_blocks(x: torch.Tensor, block_rows: int = BLOCK) -> FP8BlockTen
     ``block_rows=1`` for each row's 128 columns (tokens, as void_linear and void_expert_linear take them).  A scale is the smallest
     power of two that keeps its block within 448, so that only the quotients are rounded, once; a block that holds an infinity or NaN gets a
     scale of NaN."""
+    if _lib.transforms_active():
+        _lib.no_transforms("the quantiser of blocks")
     if block_rows not in (1, BLOCK):
         raise ValueError("blocks have 1 or %d rows, got %s" % (BLOCK, block_rows))
     if x.dim() not in (2, 3) or (x.dim() == 3 and block_rows == 1) or 0 in x.shape:

@@ -38,21 +38,14 @@ class ExpertRoutes:
         return f"ExpertRoutes(n_tokens={self.n_tokens}, top_k={self.top_k}, n_experts={self.n_experts})"
 
 
-_transforms = torch._C._are_functorch_transforms_active
-
-
-def _no_transforms(what: str) -> None:
-    raise RuntimeError("%s cannot be used inside torch.func transforms (vmap, grad, jvp, ...)" % what)
-
-
 def void_route(scores: torch.Tensor, top_k: int, normalize: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
     """The ``top_k`` (at most 32) experts of each token with the largest scores [tokens, experts] (float32, float16 or bfloat16, up to 1024
     experts) as int32 [tokens, top_k], largest first, ties to the lowest index, and their weights, float32 [tokens, top_k]: the softmax of the
     scores over the chosen experts, or with ``normalize=False`` over all.  A score of -inf is never chosen: where fewer than ``top_k``
     others are left, the expert is -1 (which void_dispatch drops) and the weight 0.  NaN counts as the largest and makes a token's weights NaN.
     Differentiable once in the scores."""
-    if _transforms():
-        _no_transforms("the router")
+    if _lib.transforms_active():
+        _lib.no_transforms("the router")
     if not scores.is_cuda:
         _lib.require_cuda(scores)
     return _lib.native().route(scores, top_k, normalize)
@@ -62,6 +55,8 @@ def sort_by_expert(experts: torch.Tensor, n_experts: int) -> ExpertRoutes:
     """Sorts the choices ``experts`` (int32 or int64 [tokens, top_k]) by expert, in the order of the tokens within an expert.  A choice
     outside [0, n_experts) is dropped: it belongs to no run.  At most 1024 experts; nothing is read by the host, so a captured call may be
     replayed with other choices."""
+    if _lib.transforms_active():
+        _lib.no_transforms("the sort by expert")
     _lib.require_cuda(experts)
     return ExpertRoutes(*_lib.native().sort_by_expert(experts, n_experts), n_experts)
 
@@ -70,8 +65,8 @@ def void_dispatch(x: torch.Tensor, experts: torch.Tensor, n_experts: int, out: O
     """Tokens x [tokens, features] (float32, float16 or bfloat16) copied into the run of each of their experts: rows [tokens * top_k, features]
     sorted by expert, as void_expert_linear and SparseExperts take them, and the routes (sort_by_expert).  Rows behind the last run, one for
     every dropped choice, are zeros; with ``out`` (row-major) they are left as they are.  Differentiable once in x."""
-    if _transforms():
-        _no_transforms("the dispatch of tokens")
+    if _lib.transforms_active():
+        _lib.no_transforms("the dispatch of tokens")
     if not (x.is_cuda and experts.is_cuda):
         _lib.require_cuda(x, experts)
     rows, offsets, position = _lib.native().dispatch(x, experts, n_experts, out)
@@ -84,8 +79,8 @@ def void_combine(rows: torch.Tensor, routes: ExpertRoutes, weights: Optional[tor
     in rows' type.  ``weights`` [tokens, top_k] and ``residual`` [tokens, features] are float32, float16 or bfloat16; without weights the rows
     are added.  A dropped choice adds nothing, whatever its weight.  Differentiable once in rows, weights and residual.  ``out`` (row-major;
     may be the residual, or share memory with an operand in another way) takes the result where nothing is differentiated."""
-    if _transforms():
-        _no_transforms("the combination of experts' rows")
+    if _lib.transforms_active():
+        _lib.no_transforms("the combination of experts' rows")
     if not isinstance(routes, ExpertRoutes):
         raise TypeError("void_combine takes ExpertRoutes (sort_by_expert, void_dispatch), got %s" % type(routes).__name__)
     if not rows.is_cuda:
