@@ -635,7 +635,9 @@ VOID_API int void_layer_norm_grad(const void* g, int64_t ldg, const void* x, int
  * weight_elem, or NULL for ones; residual of elem or fp32, or NULL; choices without a row are left out.  out may be the residual.
  * void_combine_grad: drows (NULL: not wanted; rows from *used_rows on are zeroed) and dweights (likewise; of weight_elem) from the gradient
  * g [tokens, cols] of void_combine's result.  void_dispatch's gradient is void_combine without weights.
+ * Rows of tokens have at most VOID_MOST_FEATURES columns.
  * ------------------------------------------------------------------------------------- */
+#define VOID_MOST_FEATURES 67107832
 VOID_API int void_route(const void* scores, int32_t elem, int64_t lds, int64_t rows, int32_t n_experts, int32_t top_k, int32_t normalize,
                         int32_t* experts, float* weights, void_stream_t stream);
 VOID_API int void_route_grad(const void* scores, int32_t elem, int64_t lds, int64_t rows, int32_t n_experts, int32_t top_k, int32_t normalize,
@@ -666,6 +668,7 @@ VOID_API int void_combine_grad(const void* g, int64_t ldg, const void* rows, int
  * void_quant_fp8_blocks: q [rows, cols] e4m3, ldq bytes between rows, and scales [ceil(rows / block_rows), ceil(cols / 128)] (element strides
  * scale_row, scale_col) of a matrix of type elem, for block_rows 1 or 128.  A scale is the smallest power of two (2^-100 at the least) that
  * keeps the block within 448, so that nothing is rounded but the quotient to e4m3; a block that holds an infinity or NaN gets a scale of NaN.
+ * At most 8388480 rows (block_rows 128), or 16776960 columns (block_rows 1; of rows in whole 16-byte pieces 33553920 fp32 or 67107840 16-bit ones).
  * ------------------------------------------------------------------------------------- */
 typedef struct void_fp8_args {
   const void* a;

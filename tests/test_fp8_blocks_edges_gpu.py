@@ -67,3 +67,12 @@ def test_tangents_are_refused():
             with pytest.raises(NotImplementedError, match="tangent"):
                 call()
     assert void.void_linear(w, x, bias).shape == (4, 256)
+
+
+def test_too_many_columns_are_refused():
+    for cols, dtype in ((16776961, torch.bfloat16), (33553924, torch.float32), (67107848, torch.float16)):   # (odd rows; rows in whole 16-byte pieces)
+        with pytest.raises(_lib.VoidB200Error, match="documented maximum"):
+            void.quantize_fp8_blocks(torch.empty(1, cols, dtype=dtype, device="cuda"), 1)
+    x = torch.ones(1, 16776959, dtype=torch.bfloat16, device="cuda")
+    q = void.quantize_fp8_blocks(x, 1)
+    assert (q.values.float() * 2.0 ** -8 == 1).all() and (q.scales == 2.0 ** -8).all()

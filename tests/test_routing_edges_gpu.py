@@ -31,3 +31,14 @@ def test_tokens_and_choices_written_just_before_by_a_few_blocks():
             want = torch.zeros(n * top, d, dtype=dtype, device="cuda")
             want[at[at >= 0].long()] = tokens.repeat_interleave(top, 0)[at >= 0]
             assert torch.equal(rows, want), i
+
+
+def test_too_many_features_are_refused_with_the_limit():
+    x, ids = torch.empty(1, 67107833, dtype=torch.bfloat16, device="cuda"), torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    with pytest.raises(_lib.VoidB200Error, match="at most 67107832 features, got 67107833"):
+        void.void_dispatch(x, ids, 1)
+    with pytest.raises(_lib.VoidB200Error, match="at most 67107832 features, got 67107833"):
+        void.void_combine(x, void.sort_by_expert(ids, 1))
+    most = torch.ones(1, 67107832, dtype=torch.bfloat16, device="cuda")
+    rows, routes = void.void_dispatch(most, ids, 1)
+    assert torch.equal(rows, most) and torch.equal(void.void_combine(rows, routes), most)

@@ -2086,7 +2086,7 @@ PyObject* dispatch(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const c10::Device dev = x.device();
   if (!floating(x.scalar_type())) fail(std::string("x must be float32, float16 or bfloat16, got ") + c10::toString(x.scalar_type()));
   if (x.dim() != 2) fail("x must be a [tokens, features] matrix");
-  if (x.size(1) > 0x7fffffff) fail("tokens have at most 2^31 - 1 features");
+  if (x.size(1) > VOID_MOST_FEATURES) fail("tokens have at most " + std::to_string(VOID_MOST_FEATURES) + " features, got " + std::to_string(x.size(1)));
   no_tangents({&x}, "the dispatch of tokens");
   const bool recorded = torch::autograd::compute_requires_grad(x);
   c10::cuda::OptionalCUDAGuard guard;
@@ -2188,7 +2188,7 @@ PyObject* combine(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (ys.dim() != 2 || ys.size(0) != tokens * top)
     fail("the experts' rows must be a matrix with a row for each of the " + std::to_string(tokens) + " x " + std::to_string(top) + " choices");
   const int64_t cols = ys.size(1);
-  if (cols > 0x7fffffff) fail("tokens have at most 2^31 - 1 features");
+  if (cols > VOID_MOST_FEATURES) fail("tokens have at most " + std::to_string(VOID_MOST_FEATURES) + " features, got " + std::to_string(cols));
   if (weights.defined()) {
     if (weights.dim() != 2 || weights.size(0) != tokens || weights.size(1) != top)
       fail("weights must be a [" + std::to_string(tokens) + ", " + std::to_string(top) + "] tensor");
@@ -2281,7 +2281,7 @@ PyObject* quant_fp8_blocks(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (x.dim() != 2) fail("a matrix is quantised in blocks, got " + std::to_string(x.dim()) + " dimensions");
   if (!floating(x.scalar_type())) fail(std::string("blocks are quantised from float32, float16 or bfloat16, got ") + c10::toString(x.scalar_type()));
   no_tangents({&x}, "the quantiser of blocks");
-  if (x.size(1) > 0x7ffffff0) fail("a matrix that is quantised has at most 2^31 - 16 columns");
+  if (x.size(1) > 0x7ffffff0) fail("a matrix that is quantised in blocks has too many columns: " + std::to_string(x.size(1)));
   c10::cuda::OptionalCUDAGuard guard(x.device());
   at::AutoDispatchBelowADInplaceOrView below;
   const Quantised q = quantised(x, integer(a[1]));

@@ -370,6 +370,7 @@ constexpr int kMaxSortBlocks = 256;
 
 // ------------------------------------------------------------------------------------------ rows of tokens
 constexpr int kRowThreads = 256;
+static_assert(VOID_MOST_FEATURES == 65535 * kRowThreads * 4 - 8, "blocks along a row of fp32 that lies anyhow");
 // 16-byte pieces of a row that one thread holds at a time.
 template <bool WIDE>
 constexpr int kHeld = WIDE ? 2 : 1;
@@ -783,7 +784,7 @@ int rows_of_type(RowOp op, const RowParams& p, bool wide, int sms, cudaStream_t 
 }
 int rows_launch(RowOp op, RowParams& p, int elem, cudaStream_t st) {
   if (elem < VOID_ELEM_F32 || elem > VOID_ELEM_BF16 || p.tokens < 0 || p.top < 1 || p.cols < 0) return VOID_ERR_BAD_ARG;
-  if (p.tokens > 0x7fffffffll / p.top || p.cols > 65535 * kRowThreads * 4 - 8) return VOID_ERR_TOO_LARGE;   // (blocks along a row of fp32 that lies anyhow)
+  if (p.tokens > 0x7fffffffll / p.top || p.cols > VOID_MOST_FEATURES) return VOID_ERR_TOO_LARGE;
   p.rows = p.tokens * p.top;
   const bool combine = op == RowOp::Combine, grad = op == RowOp::CombineGrad;
   // A matrix has a row per token, or (what lies in runs) one per choice.
