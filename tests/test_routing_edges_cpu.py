@@ -1,6 +1,12 @@
 """Routing, what needs no GPU: refusals of the entry points and operators at their smallest and largest sizes."""
+import copy
+import pickle
+
 import pytest
 import torch
+
+import void_b200 as void
+from void_b200 import _lib
 
 from test_routing_cpu import CGRAD, CGRAD_BASE, COMBINE, COMBINE_BASE, DISPATCH, DISPATCH_BASE, SHAPE, _call
 
@@ -27,3 +33,19 @@ def test_one_row_has_no_pitch():
         if torch.cuda.is_available():
             pytest.skip("the call would read addresses that are none")
         assert _call(name, order, base, **dict(pitches, tokens=1, top=1)) != SHAPE
+
+
+def test_copies_of_routes_are_routes():
+    routes = void.ExpertRoutes(torch.tensor([0, 2, 4]), torch.tensor([[0, 2], [1, 3]], dtype=torch.int32), 2)
+    for copied in (copy.copy(routes), copy.deepcopy(routes), pickle.loads(pickle.dumps(routes))):
+        copied.check()
+        assert torch.equal(copied.offsets, routes.offsets) and torch.equal(copied.position, routes.position) and copied.n_experts == 2
+    copied = copy.deepcopy(routes)
+    copied.position[0, 0] = -1
+    with pytest.raises(_lib.VoidB200Error, match="written to"):
+        copied.check()
+    routes.check()
+    routes.position[0, 0] = -1
+    for way in (copy.copy, copy.deepcopy, pickle.dumps):
+        with pytest.raises(_lib.VoidB200Error, match="written to"):
+            way(routes)

@@ -26,6 +26,11 @@ class ExpertRoutes:
         if self._versions is not None and self._versions != self.offsets._version + self.position._version:   # (they only grow)
             raise _lib.VoidB200Error("the routes have been written to since the tokens were sorted: drop choices (-1) before they are sorted")
 
+    def __reduce__(self):
+        """Copies and files hold the routes; their tensors count what is written to them anew."""
+        self.check()
+        return ExpertRoutes, (self.offsets, self.position, self.n_experts)
+
     @property
     def n_tokens(self) -> int:
         return self.position.shape[0]
