@@ -1,4 +1,7 @@
 """Dense 8-bit weights with scales of blocks, what needs no GPU: refusals of the operators and copies of the tensor."""
+import copy
+import io
+
 import pytest
 import torch
 
@@ -19,3 +22,17 @@ def test_transforms_are_refused(call):
     for transform in (lambda: torch.func.vmap(call)(x[None]), lambda: torch.func.jvp(call, (x,), (x,)), lambda: torch.func.grad(lambda t: call(t).float().sum())(x)):
         with pytest.raises(RuntimeError, match="torch.func"):
             transform()
+
+
+def test_copies_hold_the_fields_alone():
+    """What a product keeps with a tensor (the device's status word) stays behind: a copy of the word would be one that nobody looks at."""
+    w = void.FP8BlockTensor(torch.randn(200, 130).to(E4M3), torch.randn(2, 2))
+    w._status = torch.zeros(1, dtype=torch.int32)
+    file = io.BytesIO()   # (torch's own way: pickle by itself does not bring 8-bit tensors back)
+    torch.save(w, file)
+    file.seek(0)
+    for copied in (copy.copy(w), copy.deepcopy(w), torch.load(file, weights_only=False)):
+        assert copied._status is None and (copied.shape, copied.block_rows, copied.n_experts) == ((200, 130), 128, None)
+        assert torch.equal(copied.values.view(torch.uint8), w.values.view(torch.uint8)) and torch.equal(copied.scales, w.scales)
+        assert copied.values.stride() == (144, 1)
+    assert copy.copy(w).values is w.values

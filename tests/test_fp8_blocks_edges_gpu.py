@@ -76,3 +76,11 @@ def test_too_many_columns_are_refused():
     x = torch.ones(1, 16776959, dtype=torch.bfloat16, device="cuda")
     q = void.quantize_fp8_blocks(x, 1)
     assert (q.values.float() * 2.0 ** -8 == 1).all() and (q.scales == 2.0 ** -8).all()
+
+
+def test_the_status_word_is_that_of_the_device():
+    """Values that were replaced by some of another device (here: of the host first) take their status word with them."""
+    w, x = _weights(256, 256, 1), torch.randn(4, 256, generator=_gen(1), device="cuda")
+    want = void.void_linear(w, x)
+    w._status = torch.zeros(1, dtype=torch.int32)
+    assert torch.equal(void.void_linear(w, x), want) and w._status is _lib.status_word(x.device)

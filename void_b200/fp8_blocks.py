@@ -55,6 +55,10 @@ class FP8BlockTensor:
         self.shape = tuple(values.shape)                                       # (experts, rows, columns), or without the first
         self.n_experts: Optional[int] = self.shape[0] if len(self.shape) == 3 else None
 
+    def __reduce__(self):
+        """Copies and files hold the fields; the status word is the device's."""
+        return FP8BlockTensor, (self.values, self.scales)
+
     @property
     def device(self) -> torch.device:
         return self.values.device
@@ -86,8 +90,8 @@ class FP8BlockTensor:
         if not (values.is_cuda and x.is_cuda):
             _lib.require_cuda(values, x)
         status = self._status
-        if status is None:
-            status = self._status = _lib.status_word(values.device)
+        if status is None or status.get_device() != x.get_device():
+            status = self._status = _lib.status_word(x.device)
         return _lib.native().fp8_linear(values, self.scales, x, x_scales, offsets, bias, activation, out, out_dtype, residual, status)
 
     def __repr__(self) -> str:
