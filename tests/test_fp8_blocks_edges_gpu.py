@@ -4,7 +4,7 @@ import torch
 
 import void_b200 as void
 from void_b200 import _lib
-from test_fp8_blocks_gpu import _gen, _weights
+from test_fp8_blocks_gpu import TYPES, _check, _dense, _gen, _weights
 
 pytestmark = pytest.mark.gpu
 
@@ -84,3 +84,64 @@ def test_the_status_word_is_that_of_the_device():
     want = void.void_linear(w, x)
     w._status = torch.zeros(1, dtype=torch.int32)
     assert torch.equal(void.void_linear(w, x), want) and w._status is _lib.status_word(x.device)
+
+
+# runs, rows behind them, M, K: few work items with eight blocks of k or more, which clusters share; of 24, 64 and more tokens an expert on average, empty runs
+# (clusters with nothing to do), results in rows on 32 bytes and off them, plans by the product and (33 experts and more) by a launch of their own
+SHARED = [([3, 0, 5, 1], 2, 130, 1024), ([10, 0, 20, 0, 7], 5, 128, 4096), ([0, 1, 0], 0, 257, 1030), ([60, 0, 40], 0, 256, 2048), ([64, 1, 33, 0], 9, 131, 1500),
+          ([200, 0, 150, 0], 13, 304, 1500), ([130, 0, 257], 40, 255, 4096), ([0, 300], 1, 64, 3000), ([4] * 33, 3, 64, 1024), ([100] * 35, 0, 200, 1300),
+          ([70, 2] * 18, 5, 129, 1100), ([0, 0, 0], 30, 128, 1024), ([0] * 40, 20, 128, 1024)]
+
+
+@pytest.mark.parametrize("runs, spare, m, k", SHARED)
+def test_experts_whose_blocks_are_shared(runs, spare, m, k):
+    experts, n = len(runs), sum(runs) + spare
+    parts = [_weights(m, k, e) for e in range(experts)]
+    w = void.FP8BlockTensor(torch.stack([p.values.view(torch.uint8) for p in parts]).view(torch.float8_e4m3fn), torch.stack([p.scales for p in parts]))
+    a = _dense(w)
+    ends = torch.tensor([0] + runs).cumsum(0)
+    used = sum(runs)
+    for i, dtype in enumerate(TYPES):
+        x = torch.randn(n, k, generator=_gen(5), device="cuda").to(dtype)
+        x[used:] = float("nan")
+        xd = _dense(void.quantize_fp8_blocks(x, 1))
+        bias = torch.randn(experts, m, generator=_gen(6), device="cuda").to(dtype) if i != 2 else None
+        act = (experts + i) % 4
+        got = void.void_expert_linear(w, x, ends.to((torch.int32, torch.int64)[i % 2]).cuda(), bias, act)
+        for e in range(experts):
+            if runs[e]:
+                _check(got[ends[e]:ends[e + 1]], xd[ends[e]:ends[e + 1]], a[e], None if bias is None else bias[e], act, None, dtype)
+        assert (got[used:] == 0).all()
+        outer = torch.full((n, m + 7), 5.0, dtype=dtype, device="cuda")     # (rows that lie anyhow)
+        void.void_expert_linear(w, x, ends.cuda(), bias, act, out=outer[:, 3:m + 3])
+        assert torch.equal(outer[:used, 3:m + 3], got[:used]) and (outer[used:] == 5).all() and (outer[:, :3] == 5).all() and (outer[:, m + 3:] == 5).all()
+    void.check_device_status()
+
+
+@pytest.mark.parametrize("n, m, k", [(40, 300, 1100), (8, 300, 5000), (200, 300, 700), (200, 300, 1100), (200, 301, 1100), (300, 2500, 700)])
+def test_waits_that_run_out_are_reported(n, m, k):
+    """The first stage of every ring is never filled, of both kernels, alone and in clusters: they give up after a tenth of a second and say so, and the next
+    product is right."""
+    import ctypes
+    w, x = _weights(m, k, 1), void.quantize_fp8_blocks(torch.randn(n, k, generator=_gen(2), device="cuda"), 1)
+    want = void.void_linear(w, x)
+    out = torch.empty_like(want)
+    status = _lib.status_word(x.device)
+    a = _lib.Fp8Args(a=w.values.data_ptr(), lda=w.values.stride(0), a_scale=w.scales.data_ptr(), a_scale_row=w.scales.stride(0), a_scale_col=1,
+                     x=x.values.data_ptr(), ldx=x.values.stride(0), x_scale=x.scales.data_ptr(), x_scale_row=x.scales.stride(0),
+                     x_scale_col=x.scales.stride(1), out=out.data_ptr(), ldc=m, M=m, K=k, N=n, test_hooks=100 | 1 << 16, status=status.data_ptr())
+    assert _lib.load().void_fp8_linear(ctypes.byref(a), None, _lib.stream_ptr(x.device)) == 0
+    with pytest.raises(_lib.VoidB200Error, match="wait gave up"):
+        void.check_device_status()
+    assert torch.equal(void.void_linear(w, x), want)
+    void.check_device_status()
+
+
+def test_a_token_s_result_in_other_batches():
+    """A token's result is the same in every batch for which the blocks of k are cut alike: here twelve of them, in threes (by three CTAs of a cluster)."""
+    w = _weights(700, 1500, 1)
+    x = torch.randn(600, 1500, generator=_gen(2), device="cuda")
+    for most, cuts in ((600, ((0, 200), (100, 300), (129, 590))), (64, ((0, 40), (20, 60), (31, 64))), (32, ((0, 1), (5, 9), (17, 32)))):
+        want = void.void_linear(w, x[:most])
+        for lo, hi in cuts:
+            assert torch.equal(void.void_linear(w, x[lo:hi]), want[lo:hi]), (most, lo, hi)
