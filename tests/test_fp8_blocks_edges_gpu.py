@@ -145,3 +145,31 @@ def test_a_token_s_result_in_other_batches():
         want = void.void_linear(w, x[:most])
         for lo, hi in cuts:
             assert torch.equal(void.void_linear(w, x[lo:hi]), want[lo:hi]), (most, lo, hi)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_weights_of_experts_are_quantised_into_one_place(dtype):
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Calls(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.names = set()
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.names.add(func.overloadpacket._qualified_op_name)
+            return func(*args, **(kwargs or {}))
+
+    for experts, m, k in ((1, 1, 1), (3, 130, 200), (5, 128, 256), (2, 300, 1111)):
+        x = (torch.randn(experts, m, k, generator=_gen(m), device="cuda") * torch.logspace(-2, 2, experts, device="cuda")[:, None, None]).to(dtype)
+        for given in (x, x.transpose(1, 2).contiguous().transpose(1, 2), torch.empty(experts + 1, m, k + 3, dtype=dtype, device="cuda")[1:, :, 1:k + 1].copy_(x)):
+            with Calls() as calls:
+                got = void.quantize_fp8_blocks(given)
+            if given is x:
+                assert not calls.names & {"aten::copy_", "aten::stack", "aten::cat", "aten::clone"}, calls.names
+            assert got.shape == (experts, m, k) and got.n_experts == experts and got.block_rows == 128
+            for e in range(experts):
+                want = void.quantize_fp8_blocks(x[e])
+                assert torch.equal(got.scales[e], want.scales) and torch.equal(got.values[e].view(torch.uint8), want.values.view(torch.uint8))
+    with pytest.raises(ValueError):
+        void.quantize_fp8_blocks(x, 1)

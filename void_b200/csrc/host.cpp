@@ -2249,43 +2249,39 @@ PyObject* combine(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // ------------------------------------------------------------------------------------------ 8-bit weights with scales of blocks
-// x [N, K] in e4m3 with a scale per row and 128 columns (block_rows 1), or per 128 x 128 (128): rows on 16 bytes; the scales of rows lie
-// token behind token, as the products read them.
-struct Quantised {
-  at::Tensor values, scales;
-};
-Quantised quantised(const at::Tensor& x_in, int64_t block_rows) {
-  const at::Tensor x = matrix_rows(x_in);
-  const c10::Device dev = x.device();
-  const int64_t rows = x.size(0), cols = x.size(1), across = (cols + 127) / 128, pitch = (cols + 15) / 16 * 16;
-  Quantised q;
-  q.values = new_cuda({rows, pitch}, at::kFloat8_e4m3fn, dev);
-  if (pitch != cols) q.values = q.values.narrow(1, 0, cols);
-  if (block_rows == 1) {
-    const int64_t padded = (rows + 3) / 4 * 4;
-    q.scales = new_cuda({across, padded}, at::kFloat, dev).t();
-    if (padded != rows) q.scales = q.scales.narrow(0, 0, rows);
-  } else {
-    q.scales = new_cuda({(rows + 127) / 128, across}, at::kFloat, dev);
-  }
-  check(void_quant_fp8_blocks(x.const_data_ptr(), out_code(x.scalar_type()), row_step(x), rows, (int32_t)cols, (int32_t)block_rows, q.values.data_ptr(),
-                              pitch, q.scales.data_ptr<float>(), q.scales.stride(0), q.scales.stride(1), stream_of(dev.index())),
-        "void_quant_fp8_blocks");
-  return q;
-}
-// quant_fp8_blocks(x [N, K], block_rows) -> (values, scales)
+// quant_fp8_blocks(x [rows, cols] or [experts, rows, cols], block_rows) -> (values, scales): x in e4m3 with a scale per row and 128 columns (1), or per
+// 128 x 128 (128); rows on 16 bytes; the scales of rows lie token behind token, as the products read them.
 PyObject* quant_fp8_blocks(PyObject*, PyObject* const* a, Py_ssize_t n) {
   NATIVE_BEGIN
   if (n != 2) throw torch::TypeError("quant_fp8_blocks takes 2 arguments");
   const at::Tensor& x = cuda_tensor(a[0], "x");
-  if (x.dim() != 2) fail("a matrix is quantised in blocks, got " + std::to_string(x.dim()) + " dimensions");
+  const int64_t block_rows = integer(a[1]), dims = x.dim();
+  if (dims != 2 && (dims != 3 || block_rows == 1)) fail("a matrix (or, of weights, a stack of them) is quantised in blocks, got " + std::to_string(dims) + " dimensions");
   if (!floating(x.scalar_type())) fail(std::string("blocks are quantised from float32, float16 or bfloat16, got ") + c10::toString(x.scalar_type()));
   no_tangents({&x}, "the quantiser of blocks");
-  if (x.size(1) > 0x7ffffff0) fail("a matrix that is quantised in blocks has too many columns: " + std::to_string(x.size(1)));
-  c10::cuda::OptionalCUDAGuard guard(x.device());
+  const int64_t E = dims == 3 ? x.size(0) : 1, rows = x.size(dims - 2), cols = x.size(dims - 1);
+  if (cols > 0x7ffffff0) fail("a matrix that is quantised in blocks has too many columns: " + std::to_string(cols));
+  const c10::Device dev = x.device();
+  c10::cuda::OptionalCUDAGuard guard(dev);
   at::AutoDispatchBelowADInplaceOrView below;
-  const Quantised q = quantised(x, integer(a[1]));
-  return Py_BuildValue("NN", THPVariable_Wrap(q.values), THPVariable_Wrap(q.scales));
+  const int64_t across = (cols + 127) / 128, down = (rows + 127) / 128, pitch = (cols + 15) / 16 * 16;
+  at::Tensor values = dims == 3 ? new_cuda({E, rows, pitch}, at::kFloat8_e4m3fn, dev) : new_cuda({rows, pitch}, at::kFloat8_e4m3fn, dev), scales;
+  if (pitch != cols) values = values.narrow(dims - 1, 0, cols);
+  if (block_rows == 1) {
+    const int64_t padded = (rows + 3) / 4 * 4;
+    scales = new_cuda({across, padded}, at::kFloat, dev).t();
+    if (padded != rows) scales = scales.narrow(0, 0, rows);
+  } else {
+    scales = dims == 3 ? new_cuda({E, down, across}, at::kFloat, dev) : new_cuda({down, across}, at::kFloat, dev);
+  }
+  for (int64_t e = 0; e < E; ++e) {
+    const at::Tensor m = matrix_rows(dims == 3 ? x.select(0, e) : x);
+    check(void_quant_fp8_blocks(m.const_data_ptr(), out_code(m.scalar_type()), row_step(m), rows, (int32_t)cols, (int32_t)block_rows,
+                                static_cast<uint8_t*>(values.data_ptr()) + e * rows * pitch, pitch, scales.data_ptr<float>() + e * down * across,
+                                scales.stride(dims - 2), scales.stride(dims - 1), stream_of(dev.index())),
+          "void_quant_fp8_blocks");
+  }
+  return Py_BuildValue("NN", THPVariable_Wrap(values), THPVariable_Wrap(scales));
   NATIVE_END
 }
 

@@ -110,14 +110,7 @@ def quantize_fp8_blocks(x: torch.Tensor, block_rows: int = BLOCK) -> FP8BlockTen
     if x.dim() not in (2, 3) or (x.dim() == 3 and block_rows == 1) or 0 in x.shape:
         raise ValueError("quantize_fp8_blocks takes a matrix (or, of weights, a stack of them) that is not empty, got %s" % (tuple(x.shape),))
     _lib.require_cuda(x)
-    if x.dim() == 2:
-        return FP8BlockTensor(*_lib.native().quant_fp8_blocks(x, block_rows))
-    parts = [_lib.native().quant_fp8_blocks(m, block_rows) for m in x]
-    pitch = (x.shape[2] + 15) // 16 * 16
-    values = torch.empty(*x.shape[:2], pitch, dtype=torch.float8_e4m3fn, device=x.device)[..., :x.shape[2]]
-    for to, (given, _) in zip(values, parts):
-        to.view(torch.uint8).copy_(given.view(torch.uint8))
-    return FP8BlockTensor(values, torch.stack([s for _, s in parts]))
+    return FP8BlockTensor(*_lib.native().quant_fp8_blocks(x, block_rows))
 
 
 __all__ = ["FP8BlockTensor", "quantize_fp8_blocks"]
