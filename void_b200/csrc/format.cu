@@ -15,6 +15,7 @@
 #include "../../include/void_b200.h"
 #include "launch.cuh"
 #include "ptx.cuh"
+#include "values.cuh"
 
 namespace vbf {
 
@@ -77,14 +78,7 @@ static bool ws_layout(int nbr, int nbc, WsLayout* w) {
   return true;
 }
 
-template <typename T>
-__device__ __forceinline__ float to_float(T v);
-template <>
-__device__ __forceinline__ float to_float<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
-template <>
-__device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+using vb::to_float;
 
 // L1 norm and nonzero count per tile of the block grid (elements outside the matrix count as the zero padding of
 // void/format.py:374-378); a tile is kept when its norm exceeds the threshold (:391-394).  A warp takes the 32 rows of a

@@ -3,10 +3,12 @@
 //
 //     out[t, m] = act( sum_b sx[t, b] sa[m / 128, b] sum_{k in block b} x[t, k] a[m, k]  + bias[m] ) + residual[t, m]
 //
-// of one matrix, or of the matrices of experts for tokens sorted by expert.  The product is computed transposed: features are the 128 lanes
-// of tensor memory, tokens the columns (16 to 256 of them, whatever a run of tokens leaves), so a short run costs what its tokens cost.
-// The scales differ from block to block of k, so every block's product is an accumulator of its own, which eight warps read back, multiply by
-// sx sa (one number per token: sa is the same for all lanes) and add in registers, while the tensor cores fill the other of two.
+// of one matrix, or of the matrices of experts for tokens sorted by expert.  The scales differ from block to block of k, so every block's product is
+// an accumulator of its own, which eight warps read back, multiply by sx sa and add in registers, while the tensor cores fill the other of two.
+//
+// Up to 64 tokens (of an expert, on average) the product is computed transposed (fp8_block_kernel): 128 features are the lanes of tensor memory and
+// the tokens its columns, in sixteens, so a short run costs what its tokens cost and the weights stream once; sx sa is one number per column.  More
+// tokens (fp8_wide_kernel) are the lanes, 128 of them, and 256 features the columns, so that sx sa is one number of a thread's own.
 //
 // With fewer work items than SMs, the blocks of k are dealt to a cluster of CTAs, whose partial sums meet through shared memory, added in the
 // order of the CTAs.
@@ -338,13 +340,14 @@ __device__ __forceinline__ void zero_tokens_in_no_run(const Fp8Params& p, const 
 // block, 12.5 of streaming, 2.5 for the sums of a cluster; 16384 x 16384: 48 (5.6 TB/s).  Weights asked for by prefetches ahead of the wait on the kernel
 // before: 18.2 to 20.8 with the quantiser in front, against 18.5 without.
 // NT: tokens of an item at most.
-template <int NT, int CTAS>
-__global__ void __launch_bounds__(kThreads, CTAS) fp8_block_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUtensorMap map_a,
-                                                                   const __grid_constant__ CUtensorMap map_x) {
-  constexpr int CG = NT / 2 < 32 ? NT / 2 : 32;   // columns read back at a time
-  constexpr int GROUPS = NT / 2 / CG;              // of them for one warp: every other one
+constexpr int kFewCtas = 2;   // of an SM
+template <int NT>
+__global__ void __launch_bounds__(kThreads, kFewCtas) fp8_block_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUtensorMap map_a,
+                                                                       const __grid_constant__ CUtensorMap map_x) {
+  static_assert(NT == 32 || NT == 64, "a warp reads 16 or 32 columns back at once");
+  constexpr int CG = NT / 2;   // columns of an adding warp
   constexpr uint32_t kStageA = kBlock * kBlock, kStage = kStageA + NT * kBlock;
-  constexpr uint32_t kTmem = NT * 2 < 32 ? 32 : NT * 2;
+  constexpr uint32_t kTmem = NT * 2;
   extern __shared__ uint8_t raw[];
   __shared__ Fp8Bars bars;
   __shared__ __align__(16) float scale_ring[kScaleSlots][NT];
@@ -436,7 +439,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) fp8_block_kernel(const __grid_
     }
   } else if (warp < kFirstAdder) {
     // The products of both scales, every other block of k for either warp; those of the next block are on their way meanwhile.
-    constexpr int PER = (NT + 31) / 32;
+    constexpr int PER = NT / 32;
     uint32_t it0 = 0;
     bool ok = true;
     for (int i = begin; i < end && ok; i += step) {
@@ -461,48 +464,41 @@ __global__ void __launch_bounds__(kThreads, CTAS) fp8_block_kernel(const __grid_
         ok = mbar_wait_warp(smem_u32(&bars.scale_empty[slot]), ((it / kScaleSlots) & 1u) ^ 1u, ctl);
         if (!ok) break;
 #pragma unroll
-        for (int k = 0; k < PER; ++k)
-          if (lane + 32 * k < NT) scale_ring[slot][lane + 32 * k] = now[k];
+        for (int k = 0; k < PER; ++k) scale_ring[slot][lane + 32 * k] = now[k];
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&bars.scale_full[slot]));
       }
       it0 += (uint32_t)(b1 - b0);
     }
   } else {
-    const int quad = warp & 3, side = (warp - kFirstAdder) >> 2;
+    const int quad = warp & 3, c0 = ((warp - kFirstAdder) >> 2) * CG;
     uint32_t it = 0;
     bool ok = true;
     for (int i = begin; i < end && ok; i += step) {
       const Item t = item_at(p, runs, i);
       const int n = t.n1 - t.n0, m = t.m * kBlock + quad * 32 + lane;
       const uint32_t bias_raw = p.bias != nullptr && m < p.M ? raw_element(p.bias, p.bias_elem, (long long)t.expert * p.M + m) : 0u;
-      f32x2 sum[GROUPS][CG / 2];
+      f32x2 sum[CG / 2];
 #pragma unroll
-      for (int g = 0; g < GROUPS; ++g)
-#pragma unroll
-        for (int c = 0; c < CG / 2; ++c) sum[g][c] = pair(0.0f, 0.0f);
+      for (int c = 0; c < CG / 2; ++c) sum[c] = pair(0.0f, 0.0f);
       for (int b = b0; b < b1; ++b, ++it) {
         const uint32_t slot = it & 1u, ring_slot = it % kScaleSlots;
         ok = mbar_wait_warp(smem_u32(&bars.scale_full[ring_slot]), (it / kScaleSlots) & 1u, ctl) &&
              mbar_wait_warp(smem_u32(&bars.acc_full[slot]), (it >> 1) & 1u, ctl);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t from = tmem + slot * NT + ((uint32_t)(quad * 32) << 16);
+        if (c0 < n) {
+          const uint32_t from = tmem + slot * NT + (uint32_t)c0 + ((uint32_t)(quad * 32) << 16);
+          uint32_t r[CG];
+          if constexpr (CG == 32) tmem_ld_32x32(from, r);
+          else tmem_ld_32x16p(from, r);
+          tmem_ld_wait();
+          const float4* s4 = reinterpret_cast<const float4*>(&scale_ring[ring_slot][c0]);
 #pragma unroll
-        for (int g = 0; g < GROUPS; ++g) {
-          const int c0 = (2 * g + side) * CG;
-          if (c0 < n) {
-            uint32_t r[CG];
-            if constexpr (CG == 32) tmem_ld_32x32(from + (uint32_t)c0, r);
-            else tmem_ld_32x16p(from + (uint32_t)c0, r);
-            tmem_ld_wait();
-            const float4* s4 = reinterpret_cast<const float4*>(&scale_ring[ring_slot][c0]);
-#pragma unroll
-            for (int c = 0; c < CG / 4; ++c) {
-              const float4 s = s4[c];
-              sum[g][2 * c] = fma2(pair(__uint_as_float(r[4 * c]), __uint_as_float(r[4 * c + 1])), pair(s.x, s.y), sum[g][2 * c]);
-              sum[g][2 * c + 1] = fma2(pair(__uint_as_float(r[4 * c + 2]), __uint_as_float(r[4 * c + 3])), pair(s.z, s.w), sum[g][2 * c + 1]);
-            }
+          for (int c = 0; c < CG / 4; ++c) {
+            const float4 s = s4[c];
+            sum[2 * c] = fma2(pair(__uint_as_float(r[4 * c]), __uint_as_float(r[4 * c + 1])), pair(s.x, s.y), sum[2 * c]);
+            sum[2 * c + 1] = fma2(pair(__uint_as_float(r[4 * c + 2]), __uint_as_float(r[4 * c + 3])), pair(s.z, s.w), sum[2 * c + 1]);
           }
         }
         tc_fence_before();
@@ -516,44 +512,34 @@ __global__ void __launch_bounds__(kThreads, CTAS) fp8_block_kernel(const __grid_
       if (p.splits > 1) {
         float* part = reinterpret_cast<float*>(raw + (ring - smem_u32(raw)));   // [tokens][128]
 #pragma unroll
-        for (int g = 0; g < GROUPS; ++g) {
-          const int c0 = (2 * g + side) * CG;
-#pragma unroll
-          for (int c = 0; c < CG / 2; ++c) {
-            float a, d;
-            unpair(sum[g][c], a, d);
-            if (c0 + 2 * c < n) part[(c0 + 2 * c) * kBlock + quad * 32 + lane] = a;
-            if (c0 + 2 * c + 1 < n) part[(c0 + 2 * c + 1) * kBlock + quad * 32 + lane] = d;
-          }
+        for (int c = 0; c < CG / 2; ++c) {
+          float a, d;
+          unpair(sum[c], a, d);
+          if (c0 + 2 * c < n) part[(c0 + 2 * c) * kBlock + quad * 32 + lane] = a;
+          if (c0 + 2 * c + 1 < n) part[(c0 + 2 * c + 1) * kBlock + quad * 32 + lane] = d;
         }
         break;   // (one item per cluster)
       }
-      if (m < p.M) {
+      if (m < p.M && c0 < n) {
         const float bias = of_raw(bias_raw, p.bias_elem);
+        f32x2 y[CG / 2];
 #pragma unroll
-        for (int g = 0; g < GROUPS; ++g) {
-          const int c0 = (2 * g + side) * CG;
-          if (c0 < n) {
-            f32x2 y[CG / 2];
+        for (int c = 0; c < CG / 2; ++c) y[c] = add2(sum[c], pair(bias, bias));
+        activate<CG / 2>(y, p.act);
+        const long long token = t.n0 + c0;
 #pragma unroll
-            for (int c = 0; c < CG / 2; ++c) y[c] = add2(sum[g][c], pair(bias, bias));
-            activate<CG / 2>(y, p.act);
-            const long long token = t.n0 + c0;
+        for (int h = 0; h < CG; h += 8) {   // eight residuals on their way together
+          uint32_t res[8];
 #pragma unroll
-            for (int h = 0; h < CG; h += 8) {   // eight residuals on their way together
-              uint32_t res[8];
+          for (int c = 0; c < 8; ++c)
+            res[c] = p.residual != nullptr && c0 + h + c < n ? raw_element(p.residual, p.residual_elem, (token + h + c) * p.ldr + m) : 0u;
 #pragma unroll
-              for (int c = 0; c < 8; ++c)
-                res[c] = p.residual != nullptr && c0 + h + c < n ? raw_element(p.residual, p.residual_elem, (token + h + c) * p.ldr + m) : 0u;
-#pragma unroll
-              for (int c = 0; c < 8; ++c) {
-                float a, d;
-                unpair(y[(h + c) / 2], a, d);
-                float v = c % 2 ? d : a;
-                if (p.residual != nullptr) v += of_raw(res[c], p.residual_elem);
-                if (c0 + h + c < n) store_result(p, token + h + c, m, v);
-              }
-            }
+          for (int c = 0; c < 8; ++c) {
+            float a, d;
+            unpair(y[(h + c) / 2], a, d);
+            float v = c % 2 ? d : a;
+            if (p.residual != nullptr) v += of_raw(res[c], p.residual_elem);
+            if (c0 + h + c < n) store_result(p, token + h + c, m, v);
           }
         }
       }
@@ -1177,15 +1163,15 @@ int ring_stages(const DeviceInfo& dev, int ctas, int stage_bytes, int fixed) {
   if (stages > most) stages = most;
   return stages > kMaxRing ? kMaxRing : stages;
 }
-template <int NT, int CTAS>
+template <int NT>
 int launch_few(Fp8Params p, const CUtensorMap& a, const CUtensorMap& x, long long items, const DeviceInfo& dev, cudaStream_t st) {
   constexpr int kStage = kBlock * kBlock + NT * kBlock;
   static_assert(NT * kBlock * 4 <= 2 * kStage, "the partial sums lie in the ring");
-  p.stages = ring_stages(dev, CTAS, kStage, (int)(sizeof(Fp8Bars) + sizeof(Runs)) + kScaleSlots * NT * 4);
+  p.stages = ring_stages(dev, kFewCtas, kStage, (int)(sizeof(Fp8Bars) + sizeof(Runs)) + kScaleSlots * NT * 4);
   const int smem = p.stages * kStage + 1024;
   if (p.stages < 2) return VOID_ERR_SHAPE;
-  if (ensure_smem(reinterpret_cast<const void*>(fp8_block_kernel<NT, CTAS>), smem) != 0) return VOID_ERR_CUDA;
-  return status_of(launch_split(fp8_block_kernel<NT, CTAS>, p, a, x, items, dev, CTAS, NT == 32 ? 32 : 16, smem, st));
+  if (ensure_smem(reinterpret_cast<const void*>(fp8_block_kernel<NT>), smem) != 0) return VOID_ERR_CUDA;
+  return status_of(launch_split(fp8_block_kernel<NT>, p, a, x, items, dev, kFewCtas, NT == 32 ? 32 : 16, smem, st));
 }
 template <bool LOOSE>
 int launch_wide(Fp8Params p, const CUtensorMap& a, const CUtensorMap& x, long long items, const DeviceInfo& dev, cudaStream_t st) {
@@ -1260,8 +1246,8 @@ int fp8_linear(const void_fp8_args* a, const void_experts* x, cudaStream_t st) {
     const bool loose = !on_32_bytes(a->out, a->ldc, a->out_elem) || (a->residual != nullptr && !on_32_bytes(a->residual, a->ldr, a->residual_elem));
     return loose ? launch_wide<true>(p, map_a, map_x, items, dev, st) : launch_wide<false>(p, map_a, map_x, items, dev, st);
   }
-  if (chunk == 32) return launch_few<32, 2>(p, map_a, map_x, items, dev, st);
-  return launch_few<64, 2>(p, map_a, map_x, items, dev, st);
+  if (chunk == 32) return launch_few<32>(p, map_a, map_x, items, dev, st);
+  return launch_few<64>(p, map_a, map_x, items, dev, st);
 }
 
 }  // namespace

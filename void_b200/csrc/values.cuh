@@ -18,27 +18,19 @@ template <> __device__ __forceinline__ float from_float<float>(float v) { return
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// VEC consecutive elements as they lie: a whole 16-byte piece, or one element.
-template <typename T, int VEC>
+// The elements of a whole 16-byte piece as they lie.
+template <typename T, int VEC = 16 / (int)sizeof(T)>
 struct Piece {
-  static_assert(VEC == 1 || VEC * sizeof(T) == 16, "a piece is one element or 16 bytes");
+  static_assert(VEC * sizeof(T) == 16, "a piece is 16 bytes");
   T v[VEC];
   __device__ __forceinline__ void load(const T* at) {
-    if constexpr (VEC == 1) {
-      v[0] = *at;
-    } else {
-      const uint4 u = *reinterpret_cast<const uint4*>(at);
-      memcpy(v, &u, 16);
-    }
+    const uint4 u = *reinterpret_cast<const uint4*>(at);
+    memcpy(v, &u, 16);
   }
   __device__ __forceinline__ void store(T* at) const {
-    if constexpr (VEC == 1) {
-      *at = v[0];
-    } else {
-      uint4 u;
-      memcpy(&u, v, 16);
-      *reinterpret_cast<uint4*>(at) = u;
-    }
+    uint4 u;
+    memcpy(&u, v, 16);
+    *reinterpret_cast<uint4*>(at) = u;
   }
   __device__ __forceinline__ float get(int e) const { return to_float<T>(v[e]); }
   __device__ __forceinline__ void set(int e, float x) { v[e] = from_float<T>(x); }
