@@ -173,3 +173,31 @@ def test_weights_of_experts_are_quantised_into_one_place(dtype):
                 assert torch.equal(got.scales[e], want.scales) and torch.equal(got.values[e].view(torch.uint8), want.values.view(torch.uint8))
     with pytest.raises(ValueError):
         void.quantize_fp8_blocks(x, 1)
+
+
+@pytest.mark.parametrize("chunk", [32, 64, 128])
+@pytest.mark.parametrize("runs, spare, m, k", [([17, 0, 70, 1], 3, 130, 500), ([130, 33], 0, 256, 1100), ([0, 65, 64, 0, 2], 5, 300, 2048)])
+def test_experts_by_chunks_of_any_length(runs, spare, m, k, chunk):
+    """What the entry point takes: chunks of 32, 64 and 128 tokens, whatever the experts have on average."""
+    import ctypes
+    experts, n, used = len(runs), sum(runs) + spare, sum(runs)
+    parts = [_weights(m, k, e) for e in range(experts)]
+    w = void.FP8BlockTensor(torch.stack([p.values.view(torch.uint8) for p in parts]).view(torch.float8_e4m3fn), torch.stack([p.scales for p in parts]))
+    x = void.quantize_fp8_blocks(torch.randn(n, k, generator=_gen(2), device="cuda"), 1)
+    bias = torch.randn(experts, m, generator=_gen(3), device="cuda")
+    ends = torch.tensor([0] + runs).cumsum(0)
+    offsets = ends.cuda()
+    out = torch.full((n, m), 5.0, device="cuda")
+    status = _lib.status_word(x.device)
+    a = _lib.Fp8Args(a=w.values.data_ptr(), lda=w.values.stride(1), expert_stride=w.values.stride(0), a_scale=w.scales.data_ptr(), a_scale_row=w.scales.stride(1),
+                     a_scale_col=1, a_scale_expert=w.scales.stride(0), x=x.values.data_ptr(), ldx=x.values.stride(0), x_scale=x.scales.data_ptr(),
+                     x_scale_row=x.scales.stride(0), x_scale_col=x.scales.stride(1), bias=bias.data_ptr(), out=out.data_ptr(), ldc=m, M=m, K=k, N=n,
+                     status=status.data_ptr())
+    plan = _lib.Experts(plan=offsets.data_ptr(), n_experts=experts, chunk=chunk, offset_bytes=8)
+    assert _lib.load().void_fp8_linear(ctypes.byref(a), ctypes.byref(plan), _lib.stream_ptr(x.device)) == 0
+    void.check_device_status()
+    xd, wd = _dense(x), _dense(w)
+    for e in range(experts):
+        if runs[e]:
+            _check(out[ends[e]:ends[e + 1]], xd[ends[e]:ends[e + 1]], wd[e], bias[e], 0, None, torch.float32)
+    assert (out[used:] == 5).all()
