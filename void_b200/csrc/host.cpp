@@ -2383,8 +2383,10 @@ PyObject* fp8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     s.ldr = tail.e.ldr;
     s.residual_elem = tail.e.residual_dtype;
   }
-  // Many results in rows that do not lie on 32 bytes are written to a matrix whose rows do, and copied (its residual is copied before): 4000 x 4001,
-  // K = 4096, bf16 91 us and 10 for the copy against 152.  Few items share the blocks of k, and their sums' way to memory is another.
+  // Many results in rows that do not lie on 32 bytes are written to a matrix whose rows do, and copied (its residual is copied before; void_copy_rows
+  // writes rows on 16 bytes only, so the way back is torch's).  us in graphs with the copy and without, bf16 K = 4096: 4000 tokens, 4001 features 121 and 155, 1024
+  // 39 and 43, 700 35 and 41; 333 tokens, 8191 34 and 41.  Fewer than half as many items as SMs share the blocks of k, and their sums' way to memory is another:
+  // 512 tokens, 4001 28 and 22, 256 21 and 18.  Narrow results are soon written: 16000 tokens, 33 features 33 and 27, 40000 tokens, 53 78 and 78.
   at::Tensor target = out;
   auto on_32_bytes = [](const at::Tensor& t) {
     return ((reinterpret_cast<uintptr_t>(t.const_data_ptr()) | (uintptr_t)(t.size(0) > 1 ? t.stride(0) * t.element_size() : 0)) & 31u) == 0;
@@ -2399,7 +2401,7 @@ PyObject* fp8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
                          (int32_t)M, stream_of(dev.index())),
           "void_copy_rows");
   };
-  const bool many = N > 64 && N * M >= (1 << 19) && (N + 127) / 128 * ((M + 255) / 256) > 74;
+  const bool many = N > 64 && M >= 64 && 2 * ((N + 127) / 128 * ((M + 255) / 256)) > void_device_sm_count();
   if (many && s.residual != nullptr && !on_32_bytes(tail.residual)) {
     const at::Tensor lines = on_whole_lines(tail.residual, tail.residual.scalar_type());
     copy_rows(tail.residual, lines);
