@@ -6,7 +6,7 @@
 // of one matrix, or of the matrices of experts for tokens sorted by expert.  The scales differ from block to block of k, so every block's product is
 // an accumulator of its own, which eight warps read back, multiply by sx sa and add in registers, while the tensor cores fill the other of two.
 //
-// Up to 64 tokens (of an expert, on average) the product is computed transposed (fp8_block_kernel): 128 features are the lanes of tensor memory and
+// Up to 64 tokens (of experts: up to 16 on average) the product is computed transposed (fp8_block_kernel): 128 features are the lanes of tensor memory and
 // the tokens its columns, in sixteens, so a short run costs what its tokens cost and the weights stream once; sx sa is one number per column.  More
 // tokens (fp8_wide_kernel) are the lanes, 128 of them, and 256 features the columns, so that sx sa is one number of a thread's own.
 //
@@ -156,7 +156,8 @@ __global__ void __launch_bounds__(kQuantThreads) quant_rows_kernel(const __grid_
   }
 }
 
-// A scale per 128 x 128, a block each (weights, once).
+// A scale per 128 x 128, a block each (weights, once, so that it is simple: x twice, element by element).  8192 x 8192 bf16 125 us, where memory would take
+// 31: waits for loads (12 of 19 cycles per instruction), 66.8 million instructions of warps.
 template <typename T>
 __global__ void __launch_bounds__(kQuantThreads) quant_blocks_kernel(const __grid_constant__ QuantParams p) {
   __shared__ uint32_t most_of[kQuantThreads / 32];
@@ -938,7 +939,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_wide_kernel(const __grid_cons
         const uint8_t* from = reinterpret_cast<const uint8_t*>(p.residual) + (row * p.ldr + m0) * es;
         for (int at = 0; at < bytes; at += 128) prefetch_l2(from + at);
       }
-      float sum[COLS];   // (pairs of numbers in one instruction read three pairs of registers: half as fast as this)
+      float sum[COLS];   // (pairs of numbers in one instruction, which read three pairs of registers: 635 us for 8192^3 against 605)
 #pragma unroll
       for (int c = 0; c < COLS; ++c) sum[c] = 0.0f;
       for (int b = b0; b < b1 && ok; b += kWideAhead) {
@@ -1128,8 +1129,10 @@ int clusters_at_once(const void* kernel, int splits, int smem) {
   return clusters;
 }
 // Launch with `splits` CTAs per item, in clusters: as many as there are SMs for, as long as every CTA has four blocks of k, or places (`ctas` per SM) if
-// it still has `least`.  8 tokens, 16384^2 51.5 us with one CTA per SM, 48.2 with two of 64 blocks each; 8192^2 16.7 and 17.2 (16 blocks); 40 tokens, 8192^2 23.6
-// and 20.7; 60 tokens, 4096^2 11.7 and 13.2 (4 blocks).
+// it still has `least`.  us in graphs with one CTA per SM and with two, by the blocks that each then has.  Items of 32 tokens (least 32), 8 tokens: 16 blocks
+// 8192^2 17.2 17.5, 4096 -> 16384 15.6 17.2; 32 blocks 16384 -> 8192 29.4 26.8, 8192 -> 12288 23.8 22.0; 64 blocks 16384^2 49.5 47.9.  Items of 64 (16), 64 tokens: 4 blocks
+// 4096^2 12.2 14.1; 8 blocks 8192 -> 4096 15.8 17.6, 4096 -> 8192 16.6 15.2; 16 blocks 8192^2 23.5 20.7, 4096 -> 16384 21.6 21.9, 16384 -> 4096 22.6 24.1; 32 blocks 16384 -> 8192
+// 37.9 31.1; 64 blocks 16384^2 63.9 55.5.
 cudaError_t launch_split(void (*kernel)(Fp8Params, CUtensorMap, CUtensorMap), Fp8Params& p, const CUtensorMap& a, const CUtensorMap& x, long long items,
                          const DeviceInfo& dev, int ctas, int least, int smem, cudaStream_t st) {
   const long long places = (long long)dev.sms * ctas;
@@ -1233,7 +1236,7 @@ int fp8_linear(const void_fp8_args* a, const void_experts* x, cudaStream_t st) {
   } else {
     p.chunk = chunk;
     chunks = p.n_chunks = (int)(((long long)a->N + chunk - 1) / chunk);
-    p.group = 16;
+    p.group = 16;   // 8192^3, us by groups of 1, 4, 16, 32, 64: 610 588 581 575 604; 4096 tokens, 4096 -> 16384 330 314 310 309 310; fewer tokens or features: no matter
   }
   const long long items = chunks * p.m_tiles;
   if (items > 0x3fffffff) return VOID_ERR_TOO_LARGE;
