@@ -81,3 +81,8 @@ def test_few_choices_of_many_experts_cost_what_the_sort_costs():
             best = min(best, a.elapsed_time(b) * 1e3 / len(kept))
         return best
     assert us(lambda: void.void_dispatch(x, ids, 1024)) < 2 * us(lambda: void.sort_by_expert(ids, 1024))
+
+
+def test_an_argument_without_a_truth_is_refused():
+    with pytest.raises(RuntimeError, match="ambiguous"):
+        void.void_route(torch.randn(4, 8, device="cuda"), 2, torch.tensor([1, 0]))

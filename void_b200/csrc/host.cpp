@@ -1975,7 +1975,8 @@ PyObject* route(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 3) throw torch::TypeError("route takes 3 arguments");
   const at::Tensor& scores = cuda_tensor(a[0], "scores");
   const int64_t top = integer(a[1]);
-  const int32_t normalize = PyObject_IsTrue(a[2]) == 1 ? 1 : 0;
+  const int32_t normalize = PyObject_IsTrue(a[2]);
+  if (normalize < 0) throw python_error();
   if (!floating(scores.scalar_type())) fail(std::string("scores must be float32, float16 or bfloat16, got ") + c10::toString(scores.scalar_type()));
   if (scores.dim() != 2) fail("scores must be a [tokens, experts] matrix");
   const int64_t N = scores.size(0), E = scores.size(1);
