@@ -6,6 +6,8 @@ import pytest
 import torch
 
 import void_b200 as void
+from void_b200 import _lib
+from test_fp8_blocks_cpu import ALIGN, _linear
 
 E4M3 = torch.float8_e4m3fn
 WEIGHT = void.FP8BlockTensor(torch.ones(256, 256).to(E4M3), torch.ones(2, 2))
@@ -36,3 +38,12 @@ def test_copies_hold_the_fields_alone():
         assert torch.equal(copied.values.view(torch.uint8), w.values.view(torch.uint8)) and torch.equal(copied.scales, w.scales)
         assert copied.values.stride() == (144, 1)
     assert copy.copy(w).values is w.values
+
+
+def test_addresses_that_hold_no_element_are_refused():
+    for bad in (dict(a_scale=4098), dict(x_scale=4098), dict(status=4098), dict(bias=4098), dict(bias=4097, bias_elem=2), dict(out=4098), dict(out=4097, out_elem=1),
+                dict(residual=4098, ldr=64), dict(residual=4097, ldr=64, residual_elem=2)):
+        assert _linear(**bad) == ALIGN, bad
+    for bad in (dict(x=4098, elem=0), dict(x=4097, elem=1), dict(scales=4098, elem=2)):
+        v = dict(dict(x=4096, elem=0, scales=4096), **bad)
+        assert _lib.load().void_quant_fp8_blocks(v["x"], v["elem"], 100, 4, 100, 1, 4096, 112, v["scales"], 1, 4, None) == ALIGN, bad

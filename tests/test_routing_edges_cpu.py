@@ -8,7 +8,7 @@ import torch
 import void_b200 as void
 from void_b200 import _lib
 
-from test_routing_cpu import CGRAD, CGRAD_BASE, COMBINE, COMBINE_BASE, DISPATCH, DISPATCH_BASE, SHAPE, _call
+from test_routing_cpu import ALIGN, AT, CGRAD, CGRAD_BASE, COMBINE, COMBINE_BASE, DISPATCH, DISPATCH_BASE, GRAD, GRAD_BASE, ROUTE, ROUTE_BASE, SHAPE, SORT, SORT_BASE, _call
 
 
 def test_dispatch_of_one_token_refuses_rows_that_overlap():
@@ -49,3 +49,17 @@ def test_copies_of_routes_are_routes():
     for way in (copy.copy, copy.deepcopy, pickle.dumps):
         with pytest.raises(_lib.VoidB200Error, match="written to"):
             way(routes)
+
+
+@pytest.mark.parametrize("name, order, base, words, halves", [
+    ("void_route", ROUTE, dict(ROUTE_BASE, elem=2), ("experts", "weights"), ("scores",)), ("void_route_grad", GRAD, dict(GRAD_BASE, elem=1), ("g",), ("scores", "ds")),
+    ("void_sort_by_expert", SORT, SORT_BASE, ("experts", "offsets", "position"), ()),
+    ("void_dispatch", DISPATCH, dict(DISPATCH_BASE, elem=1), ("experts", "offsets", "position"), ("x", "out")),
+    ("void_combine", COMBINE, COMBINE_BASE, ("position", "weights"), ("rows", "residual", "out")),
+    ("void_combine_grad", CGRAD, CGRAD_BASE, ("position", "used", "weights", "dweights"), ("g", "rows", "drows"))])
+def test_addresses_that_hold_no_element_are_refused(name, order, base, words, halves):
+    for field in words:
+        assert _call(name, order, base, **{field: AT + 2}) == ALIGN, field
+    for field in halves:
+        assert _call(name, order, base, **{field: AT + 1}) == ALIGN, field
+        assert _call(name, order, dict(base, elem=0, residual_elem=0) if "residual" in base else dict(base, elem=0), **{field: AT + 2}) == ALIGN, field

@@ -1202,6 +1202,10 @@ int fp8_linear(const void_fp8_args* a, const void_experts* x, cudaStream_t st) {
   if ((reinterpret_cast<uintptr_t>(a->a) & 15u) != 0 || (reinterpret_cast<uintptr_t>(a->x) & 15u) != 0 || (a->lda & 15) != 0 || (a->ldx & 15) != 0 ||
       a->lda < a->K || a->ldx < a->K || (x != nullptr && ((a->expert_stride & 15) != 0 || a->expert_stride < 0 || (reinterpret_cast<uintptr_t>(x->plan) & (x->offset_bytes != 0 ? x->offset_bytes - 1u : 15u)) != 0)))
     return VOID_ERR_ALIGN;
+  auto bytes_of = [](int elem) { return elem == VOID_ELEM_F32 ? 4 : 2; };
+  if (!lies_on(a->a_scale, 4) || !lies_on(a->x_scale, 4) || !lies_on(a->status, 4) || !lies_on(a->bias, bytes_of(a->bias_elem)) ||
+      !lies_on(a->residual, bytes_of(a->residual_elem)) || !lies_on(a->out, bytes_of(a->out_elem)))
+    return VOID_ERR_ALIGN;
   const DeviceInfo dev = device_info();
   if (!dev.ok) return VOID_ERR_CUDA;
   if (dev.cc_major != 10) return VOID_ERR_ARCH;
@@ -1266,6 +1270,7 @@ int void_quant_fp8_blocks(const void* x, int32_t elem, int64_t ldx, int64_t rows
   if (rows > 1 && (ldx < cols || ldq < cols)) return VOID_ERR_SHAPE;
   if (rows == 0 || cols == 0) return VOID_OK;
   if (x == nullptr || q == nullptr || scales == nullptr) return VOID_ERR_BAD_ARG;
+  if (!lies_on(x, elem == VOID_ELEM_F32 ? 4 : 2) || !lies_on(scales, 4)) return VOID_ERR_ALIGN;
   const DeviceInfo dev = device_info();
   if (!dev.ok) return VOID_ERR_CUDA;
   if (dev.cc_major != 10) return VOID_ERR_ARCH;

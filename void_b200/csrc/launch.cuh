@@ -95,6 +95,8 @@ cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, int threads, int smem_by
 }
 // Every launch reports its own status.  (The runtime's last error is the last call's that failed, which may be an earlier entry's:
 // cudaGetLastError behind a launch would report that one.)
+// Whether an address may hold elements of `bytes` bytes (a power of two).
+inline bool lies_on(const void* at, int bytes) { return (reinterpret_cast<uintptr_t>(at) & (uintptr_t)(bytes - 1)) == 0; }
 inline int status_of(cudaError_t rc) { return rc == cudaSuccess ? VOID_OK : VOID_ERR_CUDA; }
 // Launches that follow one another on a stream; none after the first that failed.
 class Launches {

@@ -24,6 +24,7 @@ namespace vb {
 namespace {
 
 constexpr unsigned kAll = 0xffffffffu;
+inline int elem_size(int elem) { return elem == VOID_ELEM_F32 ? 4 : 2; }
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -155,6 +156,7 @@ int route_launch(const RouteParams& p, int elem, cudaStream_t st) {
   if (p.experts > 1024 || p.top > 32 || p.rows > 0x7fffffffll) return VOID_ERR_TOO_LARGE;
   if (p.rows == 0) return VOID_OK;
   if (p.scores == nullptr || (GRAD ? p.g == nullptr || p.ds == nullptr : p.chosen == nullptr || p.weights == nullptr)) return VOID_ERR_BAD_ARG;
+  if (!lies_on(p.scores, elem_size(elem)) || !lies_on(p.ds, elem_size(elem)) || !lies_on(p.g, 4) || !lies_on(p.chosen, 4) || !lies_on(p.weights, 4)) return VOID_ERR_ALIGN;
   const DeviceInfo dev = device_info();
   if (!dev.ok) return VOID_ERR_CUDA;
   if (dev.cc_major != 10) return VOID_ERR_ARCH;
@@ -764,7 +766,6 @@ __global__ void __launch_bounds__(kRowThreads, WIDE ? 4 : 5) combine_grad_kernel
 
 // Whether rows of `elem_bytes` elements lie in whole 16-byte pieces.
 inline bool in_pieces(const void* at, long long ld, int elem_bytes) { return ((reinterpret_cast<uintptr_t>(at) | (uintptr_t)(ld * elem_bytes)) & 15u) == 0; }
-inline int elem_size(int elem) { return elem == VOID_ELEM_F32 ? 4 : 2; }
 
 enum class RowOp { Dispatch, DispatchSort32, DispatchSort64, Combine, CombineGrad };
 template <typename T, bool WIDE>
@@ -797,10 +798,13 @@ int rows_launch(RowOp op, RowParams& p, int elem, cudaStream_t st) {
       (p.tokens > 1 && ((grad && p.ldg < p.cols) || (p.residual != nullptr && p.ldr < p.cols))))
     return VOID_ERR_SHAPE;
   if (p.tokens == 0 || (p.cols == 0 && p.dw == nullptr)) return VOID_OK;
+  const int es = elem_size(elem);
+  if (!lies_on(p.x, es) || !lies_on(p.g, es) || !lies_on(p.out, es) || !lies_on(p.residual, elem_size(p.residual_elem)) || !lies_on(p.weights, elem_size(p.weight_elem)) ||
+      !lies_on(p.dw, elem_size(p.weight_elem)) || !lies_on(p.position, 4) || !lies_on(p.used, 4))
+    return VOID_ERR_ALIGN;
   const DeviceInfo dev = device_info();
   if (!dev.ok) return VOID_ERR_CUDA;
   if (dev.cc_major != 10) return VOID_ERR_ARCH;
-  const int es = elem_size(elem);
   bool wide = p.cols % (16 / es) == 0 && (p.x == nullptr || in_pieces(p.x, p.ldx, es)) && (p.out == nullptr || in_pieces(p.out, p.ldo, es));
   if (grad) wide = wide && in_pieces(p.g, p.ldg, es);
   if (p.residual != nullptr) wide = wide && in_pieces(p.residual, p.ldr, elem_size(p.residual_elem));
@@ -856,7 +860,7 @@ int check_sort(const void* experts, int32_t index_bytes, int64_t count, int32_t 
   if (n_experts < 1 || count < 0 || (index_bytes != 4 && index_bytes != 8) || offsets == nullptr) return VOID_ERR_BAD_ARG;
   if (count > 0 && (experts == nullptr || position == nullptr)) return VOID_ERR_BAD_ARG;
   if (n_experts > kMaxSortExperts || count > 0x7fffffffll) return VOID_ERR_TOO_LARGE;
-  if ((reinterpret_cast<uintptr_t>(experts) & (uintptr_t)(index_bytes - 1)) != 0) return VOID_ERR_ALIGN;
+  if (!lies_on(experts, index_bytes) || !lies_on(offsets, 4) || !lies_on(position, 4)) return VOID_ERR_ALIGN;
   return VOID_OK;
 }
 
