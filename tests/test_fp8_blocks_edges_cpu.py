@@ -7,7 +7,7 @@ import torch
 
 import void_b200 as void
 from void_b200 import _lib
-from test_fp8_blocks_cpu import ALIGN, _linear
+from test_fp8_blocks_cpu import ALIGN, TOO_LARGE, _linear
 
 E4M3 = torch.float8_e4m3fn
 WEIGHT = void.FP8BlockTensor(torch.ones(256, 256).to(E4M3), torch.ones(2, 2))
@@ -47,3 +47,8 @@ def test_addresses_that_hold_no_element_are_refused():
     for bad in (dict(x=4098, elem=0), dict(x=4097, elem=1), dict(scales=4098, elem=2)):
         v = dict(dict(x=4096, elem=0, scales=4096), **bad)
         assert _lib.load().void_quant_fp8_blocks(v["x"], v["elem"], 100, 4, 100, 1, 4096, 112, v["scales"], 1, 4, None) == ALIGN, bad
+
+
+def test_sizes_whose_ends_are_no_numbers_are_refused():
+    for bad in (dict(M=2 ** 31 - 1, ldc=2 ** 31), dict(M=2 ** 31 - 255, ldc=2 ** 31), dict(N=2 ** 30 + 1), dict(N=2 ** 31 - 1)):
+        assert _linear(**bad) == TOO_LARGE, bad

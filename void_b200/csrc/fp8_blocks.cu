@@ -1194,7 +1194,8 @@ int fp8_linear(const void_fp8_args* a, const void_experts* x, cudaStream_t st) {
       a->residual_elem < VOID_ELEM_F32 || a->residual_elem > VOID_ELEM_BF16 || a->act < VOID_ACT_NONE || a->act > VOID_ACT_SILU)
     return VOID_ERR_BAD_ARG;
   if (a->M == 0 || a->N == 0) return VOID_OK;
-  if (a->K > 1 << 28) return VOID_ERR_TOO_LARGE;   // (an item's time has to stay within the limit of the kernels' waits)
+  // (K: an item's time has to stay within the limit of the kernels' waits; M, N: places behind the last item are numbers, too)
+  if (a->K > 1 << 28 || a->M > 0x7fffff00 || a->N > 0x40000000) return VOID_ERR_TOO_LARGE;
   if (a->out == nullptr || a->K == 0 || a->a == nullptr || a->x == nullptr || a->a_scale == nullptr || a->x_scale == nullptr) return VOID_ERR_BAD_ARG;
   if (x != nullptr && (x->n_experts < 1 || x->plan == nullptr || (x->offset_bytes != 0 && ((x->offset_bytes != 4 && x->offset_bytes != 8) || x->n_experts > 32)) || (x->chunk != 32 && x->chunk != 64 && x->chunk != 128)))
     return VOID_ERR_BAD_ARG;
