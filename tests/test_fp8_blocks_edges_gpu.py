@@ -201,3 +201,31 @@ def test_experts_by_chunks_of_any_length(runs, spare, m, k, chunk):
         if runs[e]:
             _check(out[ends[e]:ends[e + 1]], xd[ends[e]:ends[e + 1]], wd[e], bias[e], 0, None, torch.float32)
     assert (out[used:] == 5).all()
+
+
+def test_the_status_word_is_not_made_by_a_capture():
+    """A process whose first launch is a captured product: the word that kernels report in is there before, and no replay clears what is reported."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch, void_b200 as void
+from void_b200 import _lib
+w = void.FP8BlockTensor(torch.ones(256, 256, device="cuda").to(torch.float8_e4m3fn), torch.ones(2, 2, device="cuda"))
+x = torch.ones(4, 256, device="cuda")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = void.void_linear(w, x)
+void.check_device_status()
+graph.replay()
+assert (y == 256).all()
+_lib.status_word("cuda:0").fill_(1)
+graph.replay()
+try:
+    void.check_device_status()
+except _lib.VoidB200Error:
+    print("reported")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and run.stdout.strip() == "reported", (run.stdout, run.stderr[-2000:])

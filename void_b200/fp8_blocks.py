@@ -54,6 +54,8 @@ class FP8BlockTensor:
         self.values, self.scales, self._status = _rows_on_16_bytes(values), scales, None
         self.shape = tuple(values.shape)                                       # (experts, rows, columns), or without the first
         self.n_experts: Optional[int] = self.shape[0] if len(self.shape) == 3 else None
+        if values.is_cuda and not torch.cuda.is_current_stream_capturing():   # (made inside a capture, the device's status word would be cleared by its replays)
+            _lib.status_word(values.device)
 
     def __reduce__(self):
         """Copies and files hold the fields; the status word is the device's."""
