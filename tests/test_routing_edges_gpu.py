@@ -86,3 +86,15 @@ def test_few_choices_of_many_experts_cost_what_the_sort_costs():
 def test_an_argument_without_a_truth_is_refused():
     with pytest.raises(RuntimeError, match="ambiguous"):
         void.void_route(torch.randn(4, 8, device="cuda"), 2, torch.tensor([1, 0]))
+
+
+@pytest.mark.parametrize("count, experts", [(8192, 1024), (8193, 1024), (32768, 1023), (32769, 1024), (200001, 1024), (140000, 1)])
+def test_sorts_of_many_choices_of_many_experts(count, experts):
+    ids = torch.randint(-1, experts, (count, 1), generator=_gen(count), device="cuda", dtype=torch.int32)
+    flat = ids.flatten()
+    order = torch.where(flat < 0, experts, flat).sort(stable=True).indices[: int((flat >= 0).sum())]
+    position = torch.full((count,), -1, dtype=torch.int32, device="cuda")
+    position[order] = torch.arange(order.numel(), dtype=torch.int32, device="cuda")
+    ends = torch.bincount(flat[flat >= 0], minlength=experts).cumsum(0).int()
+    routes = void.sort_by_expert(ids, experts)
+    assert torch.equal(routes.position.flatten(), position) and routes.offsets[0] == 0 and torch.equal(routes.offsets[1:], ends)
