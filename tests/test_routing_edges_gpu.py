@@ -45,7 +45,7 @@ def test_too_many_features_are_refused_with_the_limit():
 
 
 @pytest.mark.parametrize("tokens, top", [(1, 1), (64, 8), (513, 1), (57, 9), (128, 8)])
-@pytest.mark.parametrize("experts", [1, 7, 64, 65, 300, 1024])
+@pytest.mark.parametrize("experts", [1, 7, 51, 52, 64, 65, 249, 300, 1024])
 def test_dispatch_on_either_side_of_few_choices_and_experts(tokens, top, experts):
     ids = torch.randint(-1, experts + 1, (tokens, top), generator=_gen(tokens + experts), device="cuda")
     x = torch.randn(tokens, 24, generator=_gen(3), device="cuda").bfloat16()

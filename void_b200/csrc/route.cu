@@ -377,11 +377,12 @@ static_assert(VOID_MOST_FEATURES == 65535 * kRowThreads * 4 - 8, "blocks along a
 // 16-byte pieces of a row that one thread holds at a time.
 template <bool WIDE>
 constexpr int kHeld = WIDE ? 2 : 1;
-// Choices, and experts, that the sort's own block is not worth a launch for: every warp ranks its token's choices by counting, and one block counts what
-// comes before every expert, eight experts at a time.  us in graphs, one launch and behind the sort (2048 bf16 features): 8 experts, 32 choices 2.3 and 4.4,
-// 256 2.9 and 4.7, 512 3.7 and 4.7, 1024 5.3 and 5.3; 64 experts 3.7 and 5.0, 4.2 and 5.2, 5.3 and 5.3, 8.0 and 5.6; 256 experts 8.4 and 6.0, 8.7 and 6.3, 11.3 and
-// 6.4, 16.9 and 6.8; 1024 experts, 1024 choices 52.9 and 10.7.
-constexpr int kFewChoices = 512, kFewExperts = 64;
+// Choices that the sort's own block is not worth a launch for: every warp ranks its token's choices by counting, and one block counts what comes before every
+// expert, eight experts at a time, so that the form's time grows with either number.  us of the one launch, in graphs (2048 bf16 features): 32 choices of 64
+// experts 3.5, 128 5.1, 256 8.2; 512 choices of 8 3.6, 64 5.4, 128 7.4, 192 9.4; 1024 of 8 5.3, 32 6.5, 64 8.0, 256 17.0, 1024 53.  Behind the sort all of them take 4.5 to 6.7
+// (1024 experts 10.7), but called one after another 8.3, for the host has two launches to make (one: 6.0).  The border is where the one launch takes as long as that.
+constexpr int kFewChoices = 1024;
+inline bool few_choices(long long count, int n_experts) { return count <= kFewChoices && 5ll * n_experts + count <= 1280; }
 
 struct RowParams {
   const void* x;            // tokens (dispatch), rows (combine, its gradient)
@@ -909,7 +910,7 @@ int void_dispatch(const void* x, int32_t elem, int64_t ldx, int64_t tokens, int3
   vb::RowParams p = {};
   p.x = x; p.ldx = ldx; p.tokens = tokens; p.cols = cols; p.top = top_k; p.out = out; p.ldo = ldo; p.zero_rest = zero_rest;
   p.position = position; p.used = offsets + n_experts;
-  if (tokens > 0 && cols > 0 && count <= vb::kFewChoices && n_experts <= vb::kFewExperts) {
+  if (tokens > 0 && cols > 0 && vb::few_choices(count, n_experts)) {
     p.experts = experts; p.offsets = offsets; p.positions = position; p.n_experts = n_experts;
     return vb::rows_launch(index_bytes == 4 ? vb::RowOp::DispatchSort32 : vb::RowOp::DispatchSort64, p, elem, st);
   }
