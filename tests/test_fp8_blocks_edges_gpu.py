@@ -229,3 +229,23 @@ except _lib.VoidB200Error:
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     run = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
     assert run.returncode == 0 and run.stdout.strip() == "reported", (run.stdout, run.stderr[-2000:])
+
+
+@pytest.mark.parametrize("experts, m", [(3, 128), (37, 512), (149, 100)])
+@pytest.mark.parametrize("each", [16, 24, 25, 48, 49, 65])
+def test_experts_on_either_side_of_the_rule(experts, m, each):
+    """Tokens an expert has on average, and matrices, around what decides between items of 32 and of 128 tokens; one expert has the tokens of three."""
+    k, n = 200, experts * each
+    counts = [each] * experts
+    counts[0] += 2 * each
+    counts[1] -= each
+    counts[2] -= each
+    w = void.quantize_fp8_blocks(torch.randn(experts, m, k, generator=_gen(1), device="cuda"))
+    x = torch.randn(n, k, generator=_gen(2), device="cuda")
+    ends = torch.tensor([0] + counts).cumsum(0)
+    got = void.void_expert_linear(w, x, ends.cuda(), None, 2)
+    xd, a = _dense(void.quantize_fp8_blocks(x, 1)), _dense(w)
+    for e in range(experts):
+        if counts[e]:
+            _check(got[ends[e]:ends[e + 1]], xd[ends[e]:ends[e + 1]], a[e], None, 2, None, torch.float32)
+    void.check_device_status()

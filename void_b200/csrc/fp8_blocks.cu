@@ -6,7 +6,7 @@
 // of one matrix, or of the matrices of experts for tokens sorted by expert.  The scales differ from block to block of k, so every block's product is
 // an accumulator of its own, which eight warps read back, multiply by sx sa and add in registers, while the tensor cores fill the other of two.
 //
-// Up to 64 tokens (of experts: up to 16 on average) the product is computed transposed (fp8_block_kernel): 128 features are the lanes of tensor memory and
+// Up to 64 tokens (of experts: up to 48 or 24 on average, by the size of their matrices) the product is computed transposed (fp8_block_kernel): 128 features are the lanes of tensor memory and
 // the tokens its columns, in sixteens, so a short run costs what its tokens cost and the weights stream once; sx sa is one number per column.  More
 // tokens (fp8_wide_kernel) are the lanes, 128 of them, and 256 features the columns, so that sx sa is one number of a thread's own.
 //

@@ -2286,11 +2286,19 @@ PyObject* quant_fp8_blocks(PyObject*, PyObject* const* a, Py_ssize_t n) {
   NATIVE_END
 }
 
-// Tokens of a work item, by those an expert has on average.  us in graphs by 32, 64 and 128 of them, 8 experts of 2048 -> 8192: 16 tokens each 27.5 33.4 28.9, 24 28.4
-// 34.0 29.3, 32 28.8 34.4 29.5, 40 36.1 36.9 30.1, 64 37.4 37.8 31.3, 128 66 58 35; with three eighths of the tokens one expert's 16 each 26.8 33.8 29.2, 24 31.2 33.0 29.6,
-// 48 41.9 43.2 29.9.  16 experts of 2048 -> 2048: 16 each 16.3 18.5 16.5, 24 17.0 18.7 16.6, 40 22.3 20.2 16.8; uneven 16 each 16.2 18.7 17.4, 20 21.5 19.3 17.7.
-// So up to 16, since a popular expert's second chunk reads its weights again; items of 64 are for one matrix.
-int32_t fp8_chunk(int64_t rows, int64_t experts) { return (rows + experts - 1) / experts <= 16 ? 32 : 128; }
+// Tokens of a work item, by those an expert has on average.  A popular expert's second item of 32 reads its weights again, while items of 128, which are
+// 256 features wide, are too few to share the blocks of k where matrices are small: so up to 48 tokens each if an item of 32 for every expert and 128 features
+// finds an SM, else up to 24.  us in graphs by items of 32, 64 and 128 tokens, experts alike in size; then sizes falling as 1, 1/2, 1/3 ...:
+//   8 experts of 2048 -> 8192: 16 each 27.5 33.4 28.9; 24 29 34 30; 31 34 31; 48 37 38 32; 36 41 31; 128 66 58 35.  16 of 2048 -> 2048: 32 each 16.7 18.9 16.8; 19 27 18.
+//   32 of 2048 -> 2048: 24 each 29.8 - 30.4; 31.6 - 30.9; 32 each 30 36 31; 32 40 31.
+//   8 of 8192 -> 2048: 24 each 29.5 - 29.0; 32 - 32; 32 each 29 34 38; 33 36 43; 64 33 37 41; 33 48 44.  16 of 8192 -> 1024: 32 each 29 34 38; 33 44 44; 64 33 37 40; 52 49 45.
+//   4 of 4096^2: 32 each 16 20 22; 19 22 23; 64 20 22 24; 20 29 25.  6 of 8192 -> 2048: 40 each 32 30 28; 32 28 32.
+// Routed tokens fall unevenly: 256 of them to 2 of 8 experts, 2048 -> 4096 -> 2048 (64 each), both products 50 by items of 128 and 60 where the second, whose
+// matrices are the smaller ones, took 32.  Items of 64 are for one matrix.
+int32_t fp8_chunk(int64_t rows, int64_t experts, int64_t M) {
+  const int64_t most = experts * ((M + 127) / 128) <= void_device_sm_count() ? 48 : 24;
+  return (rows + experts - 1) / experts <= most ? 32 : 128;
+}
 // fp8_linear(values, scales, x, x_scales | None, offsets | None, bias | None, act, out | None, out_dtype | None, residual | None, status) -> out
 // values [M, K] or (with offsets) [experts, M, K] in e4m3; x [N, K] in e4m3 with x_scales, or floating: quantised first
 PyObject* fp8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -2422,7 +2430,7 @@ PyObject* fp8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   s.status = cuda_tensor(a[10], "status").data_ptr<int32_t>();
   ExpertPlan plan;
   if (runs) {
-    plan = expert_plan(cuda_tensor(a[4], "offsets"), N, E, dev, s.status, true, fp8_chunk(N, E));
+    plan = expert_plan(cuda_tensor(a[4], "offsets"), N, E, dev, s.status, true, fp8_chunk(N, E, M));
     plan.x.zero_rest = none(a[7]) ? 1 : 0;
   }
   if (none(a[3])) {   // x is quantised first, values and scales in one workspace
